@@ -81,6 +81,20 @@ SIGNATURES = {
                                                     _P, _SZ, _P]),
     "clef_swiglu": (ctypes.c_int, [_P, _P, _I64, _P, _P]),
     "clef_moe_combine": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _I32, _P, _P]),
+    "clef_f8_prepared_bytes": (_I64, [_I64, _I32]),
+    "clef_f8_weight_bytes": (_I64, [_I64, _I64, _I32]),
+    "clef_f8_prepare": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _P]),
+    "clef_f8_pack_weight": (ctypes.c_int, [_P, _I64, _I32, _I32, _P, _P, _P]),
+    "clef_f8_retile": (ctypes.c_int, [_P, _I64, _I32, _I32, _P, _P]),
+    "clef_f8_gemm": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I32, _I32, _P, _P, _P]),
+    "clef_f8_gemm_gate_up": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _P, _P]),
+    "clef_f8_project_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
+    "clef_f8_project": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _P, _I32, _P, _P, _P, _SZ, _P]),
+    "clef_moe_group_slots_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
+    "clef_moe_group_slots": (ctypes.c_int, [_P, _I64, _I32, _I32, _P, _P, _P, _SZ, _P]),
+    "clef_moe_expert_f8": (ctypes.c_int, [_P, _P, _I64, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _I32, _P, _P]),
+    "clef_moe_expert_gate_up_f8": (ctypes.c_int, [_P, _P, _I64, _P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32,
+                                                  _I32, _P, _P]),
     "clef_pack_cache_path": (ctypes.c_int, [_P, _P, _P, _SZ]),
     "clef_pack_cache_read": (ctypes.c_int, [_P, _P, _P, _SZ, _P, _SZ, _P]),
     "clef_pack_cache_write": (ctypes.c_int, [_P, _P, _P, _SZ, _P, _SZ]),
@@ -838,3 +852,279 @@ class MoeLayer:
                   self.gate.codes, self.gate.scales, self.up.codes, self.up.scales, self.down.codes, self.down.scales,
                   routes_out, out, ws, ws.numel())
         return out
+
+
+# ---------------------------------------------------------------- block-scaled FP8
+#
+# e4m3 values with one scale for each block of 128 along k (include/clef_i4.h,
+# "block-scaled FP8"); no counterpart in the reference.
+
+_BAD_F8 = "unsupported FP8 block shape"
+
+
+def _on_current(*tensors) -> None:
+    """The calls go to the current device's current stream: every operand has
+    to be there."""
+    device = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ClefError(-1, "operands must be on the current device")
+
+
+def _f8_rows(x: torch.Tensor):
+    """Address, rows, width and row pitch of bf16 rows: contiguous, or a
+    column range of wider rows (pitch a multiple of 8 elements)."""
+    if x.dim() != 2 or x.dtype != torch.bfloat16:
+        raise ClefError(-1, "FP8 quantizer takes bf16 rows")
+    rows, width = x.shape
+    if x.is_contiguous():
+        return x, rows, width, width
+    if rows > 0 and (x.stride(1) != 1 or x.stride(0) < width):
+        raise ClefError(-1, _BAD_F8)
+    return x.data_ptr(), rows, width, x.stride(0)
+
+
+def _f8_out(like: torch.Tensor, rows: int, cols: int, out: torch.Tensor | None) -> torch.Tensor:
+    if out is None:
+        return _n.empty(like, torch.bfloat16, rows, cols)
+    if out.dtype != torch.bfloat16 or tuple(out.shape) != (rows, cols) or not out.is_contiguous():
+        raise ClefError(-1, "output shape/dtype mismatch")
+    _on_current(out)
+    return out
+
+
+@dataclass
+class PreparedF8:
+    """prepare_f8 output: one uint8 buffer, e4m3 codes [rows][pitch] (pitch =
+    width rounded up to 128), then f32 scales [pitch / 128][rows]."""
+    storage: torch.Tensor
+    rows: int
+    width: int
+
+    @property
+    def pitch(self) -> int:
+        return (self.width + 127) // 128 * 128
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """float8_e4m3fn [rows][width], a view."""
+        codes = self.storage[: self.rows * self.pitch].view(torch.float8_e4m3fn)
+        return codes.view(self.rows, self.pitch)[:, : self.width]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """f32 [rows][ceil(width / 128)], a view (k-block major in memory)."""
+        start = self.rows * self.pitch
+        scales = self.storage[start: start + self.rows * self.pitch // 32].view(torch.float32)
+        return scales.view(self.pitch // 128, self.rows).t()
+
+    def call_args(self):
+        """codes and scales as call arguments: addresses, without views."""
+        if self.storage.dtype != torch.uint8 or self.storage.numel() < self.rows * self.pitch * 33 // 32:
+            raise ClefError(-1, "FP8 activation buffer too small")
+        base = _n.pointer(self.storage)
+        return base, base + self.rows * self.pitch
+
+
+def prepare_f8(x: torch.Tensor, out: torch.Tensor | None = None) -> PreparedF8:
+    """Block-scaled FP8 quantizer (clef_f8_prepare): bf16 rows to e4m3 codes
+    and, per row and 128 columns, the least power of two at or above amax /
+    448. x may be a column range of wider rows. `out`: a uint8 buffer to reuse."""
+    address, rows, width, pitch = _f8_rows(x)
+    _on_current(x)
+    nbytes = _n.value(_n.clef_f8_prepared_bytes, rows, width)
+    if nbytes < 0:
+        raise ClefError(-1, _BAD_F8)
+    if out is None:
+        out = _n.empty(x, torch.uint8, nbytes)
+    elif out.dtype != torch.uint8 or out.numel() < nbytes:
+        raise ClefError(-1, "FP8 activation buffer too small")
+    else:
+        _on_current(out)
+    _n.launch(_n.clef_f8_prepare, address, rows, width, pitch, out)
+    return PreparedF8(out, rows, width)
+
+
+@dataclass
+class F8Weight:
+    """One or more (`matrices`) weights [rows][cols] as tiled e4m3 codes with
+    an f32 scale per 128 x 128 block."""
+    codes: torch.Tensor   # uint8, tiled
+    scales: torch.Tensor  # f32 [matrices][ceil(rows / 128)][ceil(cols / 128)]
+    rows: int
+    cols: int
+    matrices: int = 1
+
+
+def _f8_weight_storage(w: torch.Tensor):
+    if w.dim() not in (2, 3):
+        raise ClefError(-1, _BAD_F8)
+    matrices, rows, cols = (1, *w.shape) if w.dim() == 2 else w.shape
+    nbytes = _n.value(_n.clef_f8_weight_bytes, matrices, rows, cols)
+    if nbytes < 0:
+        raise ClefError(-1, _BAD_F8)
+    _on_current(w)
+    scales = torch.empty((matrices, (rows + 127) // 128, (cols + 127) // 128), dtype=torch.float32, device=w.device)
+    return F8Weight(torch.empty(nbytes, dtype=torch.uint8, device=w.device), scales, rows, cols, matrices)
+
+
+def load_f8_weight(w: torch.Tensor) -> F8Weight:
+    """bf16 weight [rows][cols] (or [matrices][rows][cols]: the experts of a
+    layer) quantized per 128 x 128 block by the rule of prepare_f8."""
+    if w.dtype != torch.bfloat16:
+        raise ClefError(-1, "FP8 weights are packed from bf16 (f8_weight takes e4m3)")
+    out = _f8_weight_storage(w)
+    _n.launch(_n.clef_f8_pack_weight, w.contiguous(), out.matrices, out.rows, out.cols, out.codes, out.scales)
+    return out
+
+
+def f8_weight(codes: torch.Tensor, scales: torch.Tensor) -> F8Weight:
+    """A checkpoint's e4m3 weight [rows][cols] (or [matrices][rows][cols]) with
+    its scale per 128 x 128 block, f32 or float8_e8m0fnu [..][ceil(rows /
+    128)][ceil(cols / 128)]: what a code stands for is code * scale. The codes
+    are rearranged, the scales kept."""
+    if codes.dtype != torch.float8_e4m3fn or scales.dtype not in (torch.float32, torch.float8_e8m0fnu):
+        raise ClefError(-1, "FP8 checkpoint weights are e4m3 codes with f32 or e8m0 scales")
+    out = _f8_weight_storage(codes)
+    if scales.numel() != out.scales.numel() or tuple(scales.shape[-2:]) != tuple(out.scales.shape[-2:]):
+        raise ClefError(-1, "FP8 weight scales: one per 128 x 128 block")
+    _on_current(scales)
+    _n.launch(_n.clef_f8_retile, codes.contiguous(), out.matrices, out.rows, out.cols, out.codes)
+    out.scales.copy_(scales.float().view(out.scales.shape))
+    return out
+
+
+def project_f8(a: PreparedF8, w: F8Weight, residual: torch.Tensor | None = None, out: torch.Tensor | None = None
+               ) -> torch.Tensor:
+    """Block-scaled FP8 projection (clef_f8_gemm): bf16 [rows][w.rows]."""
+    if a.width != w.cols or w.matrices != 1:
+        raise ClefError(-1, _BAD_F8)
+    _on_current(a.storage, w.codes, residual)
+    _check_residual(residual, a.rows, w.rows)
+    out = _f8_out(a.storage, a.rows, w.rows, out)
+    codes, scales = a.call_args()
+    _n.launch(_n.clef_f8_gemm, codes, scales, w.codes, w.scales, a.rows, w.rows, w.cols, residual, out)
+    return out
+
+
+def _check_residual(residual: torch.Tensor | None, rows: int, cols: int) -> None:
+    if residual is not None and (tuple(residual.shape) != (rows, cols) or residual.dtype != torch.bfloat16):
+        raise ClefError(-1, "residual shape/dtype mismatch")
+
+
+def project_quantized_f8(x: torch.Tensor, w: F8Weight, residual: torch.Tensor | None = None,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+    """prepare_f8 and project_f8 in one call (clef_f8_project)."""
+    address, m, k, pitch = _f8_rows(x)
+    if k != w.cols or w.matrices != 1:
+        raise ClefError(-1, _BAD_F8)
+    _on_current(x, w.codes, residual)
+    _check_residual(residual, m, w.rows)
+    out = _f8_out(x, m, w.rows, out)
+    nbytes = _n.value(_n.clef_f8_project_workspace_bytes, m, w.rows, k)
+    ws = _n.empty(x, torch.uint8, nbytes) if nbytes > 0 else None
+    _n.launch(_n.clef_f8_project, address, m, k, pitch, w.codes, w.scales, w.rows, residual, out, ws, nbytes)
+    return out
+
+
+def project_gate_up_f8(a: PreparedF8, gate: F8Weight, up: F8Weight, out: torch.Tensor | None = None) -> torch.Tensor:
+    """h = silu(gate projection) * up projection in one product
+    (clef_f8_gemm_gate_up): bf16 [rows][gate.rows], rounded once."""
+    if a.width != gate.cols or (gate.rows, gate.cols, gate.matrices) != (up.rows, up.cols, 1) or gate.matrices != 1:
+        raise ClefError(-1, _BAD_F8)
+    _on_current(a.storage, gate.codes, up.codes)
+    out = _f8_out(a.storage, a.rows, gate.rows, out)
+    codes, scales = a.call_args()
+    _n.launch(_n.clef_f8_gemm_gate_up, codes, scales, gate.codes, gate.scales, up.codes, up.scales, a.rows, gate.rows,
+              gate.cols, out)
+    return out
+
+
+def omni_group_slots(routes: torch.Tensor, experts: int = 128):
+    """Routes listed by expert (clef_moe_group_slots): offsets int32 [experts +
+    1] and slots int32 [tokens * topk], expert e's route ordinals t * topk + r
+    ascending at offsets[e] .. offsets[e + 1]; -1 behind the last list. For
+    expert_f8 and expert_gate_up_f8."""
+    if routes.dim() != 2 or routes.dtype != torch.float32 or routes.shape[1] % 2 or routes.shape[1] == 0:
+        raise ClefError(-1, "routes are f32 [tokens][2 * topk]")
+    tokens, topk = routes.shape[0], routes.shape[1] // 2
+    _on_current(routes)
+    offsets = _n.empty(routes, torch.int32, experts + 1)
+    slots = _n.empty(routes, torch.int32, tokens * topk)
+    nbytes = _n.value(_n.clef_moe_group_slots_workspace_bytes, tokens, topk, experts)
+    ws = _n.empty(routes, torch.uint8, nbytes) if nbytes > 0 else None
+    _n.launch(_n.clef_moe_group_slots, routes, tokens, topk, experts, offsets, slots, ws, nbytes)
+    return offsets, slots
+
+
+def _check_lists(a: PreparedF8, w: F8Weight, offsets: torch.Tensor, slots: torch.Tensor | None, topk: int,
+                 input_routed: bool) -> int:
+    """The number of slots; a.rows says it where the lists are the places."""
+    if a.width != w.cols:
+        raise ClefError(-1, _BAD_F8)
+    if offsets.dtype != torch.int32 or offsets.numel() != w.matrices + 1 or (slots is not None
+                                                                             and slots.dtype != torch.int32):
+        raise ClefError(-1, "invalid grouped expert lists")
+    _on_current(a.storage, w.codes, offsets, slots)
+    if slots is not None:
+        return slots.numel()
+    return a.rows if input_routed else a.rows * topk
+
+
+def expert_f8(a: PreparedF8, w: F8Weight, offsets: torch.Tensor, slots: torch.Tensor | None, topk: int,
+              input_routed: bool, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The experts' products over ragged lists (clef_moe_expert_f8): slot s of
+    expert e takes row s (input_routed) or s // topk of `a` against matrix e of
+    w and gives row s of the output, bf16 [slots][w.rows]. slots None: the
+    places themselves (rows sorted by expert). Rows that no list names are left
+    as they were in `out`, undefined in a new output."""
+    total = _check_lists(a, w, offsets, slots, topk, input_routed)
+    out = _f8_out(a.storage, total, w.rows, out)
+    codes, scales = a.call_args()
+    _n.launch(_n.clef_moe_expert_f8, codes, scales, a.rows, w.codes, w.scales, offsets, slots, w.matrices, total, topk,
+              int(input_routed), w.cols, w.rows, out)
+    return out
+
+
+def expert_gate_up_f8(a: PreparedF8, gate: F8Weight, up: F8Weight, offsets: torch.Tensor,
+                      slots: torch.Tensor | None, topk: int, input_routed: bool = False,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """h = silu(gate) * up over the experts' lists (clef_moe_expert_gate_up_f8),
+    rows as in expert_f8."""
+    if (gate.rows, gate.cols, gate.matrices) != (up.rows, up.cols, up.matrices):
+        raise ClefError(-1, _BAD_F8)
+    total = _check_lists(a, gate, offsets, slots, topk, input_routed)
+    _on_current(up.codes)
+    out = _f8_out(a.storage, total, gate.rows, out)
+    codes, scales = a.call_args()
+    _n.launch(_n.clef_moe_expert_gate_up_f8, codes, scales, a.rows, gate.codes, gate.scales, up.codes, up.scales,
+              offsets, slots, gate.matrices, total, topk, int(input_routed), gate.cols, gate.rows, out)
+    return out
+
+
+class MoeLayerF8:
+    """The Omni MoE block on block-scaled FP8 experts: router, routes listed by
+    expert, gate/up with SwiGLU, down, combine (the steps of MoeLayer). The
+    weights hold one matrix per expert: gate and up [inter][hidden], down
+    [hidden][inter]. Every call takes its intermediates from torch's allocator."""
+
+    def __init__(self, gate: F8Weight, up: F8Weight, down: F8Weight, topk: int = 8,
+                 router: torch.Tensor | None = None):
+        if (gate.rows, gate.cols, gate.matrices) != (up.rows, up.cols, up.matrices) or \
+                (down.rows, down.cols, down.matrices) != (gate.cols, gate.rows, gate.matrices):
+            raise ClefError(-1, _BAD_F8)
+        self.gate, self.up, self.down, self.topk = gate, up, down, topk
+        self.router = router  # bf16 [experts][hidden] router gate, used when no logits are given
+
+    def __call__(self, x: torch.Tensor, logits: torch.Tensor | None = None) -> torch.Tensor:
+        if logits is None:
+            if self.router is None:
+                raise ClefError(-1, "MoE layer needs router logits or a router gate weight")
+            logits = router_logits(x, self.router)
+        if tuple(logits.shape) != (x.shape[0], self.gate.matrices):
+            raise ClefError(-1, "router logits: one per token and expert")
+        routes = omni_route(logits, self.topk)
+        offsets, slots = omni_group_slots(routes, self.gate.matrices)
+        h = expert_gate_up_f8(prepare_f8(x), self.gate, self.up, offsets, slots, self.topk)
+        values = expert_f8(prepare_f8(h), self.down, offsets, slots, self.topk, input_routed=True)
+        return omni_combine(values, routes)

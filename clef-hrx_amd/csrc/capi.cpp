@@ -12,6 +12,7 @@
 
 #include "../../include/clef_i4.h"
 #include "build_id.inc"  // CLEF_BUILD_ID, generated by the Makefile
+#include "f8.hpp"
 #include "kernels.hpp"
 
 namespace {
@@ -818,6 +819,187 @@ int clef_moe_layer_static(const uint16_t* x, const void* logits, int32_t logits_
   if (int rc = static_scratch(&ws)) return rc;
   return moe_layer_run(x, logits, logits_dtype, tokens, hidden, inter, experts, topk, gate_w, gate_s, up_w, up_s,
                        down_w, down_s, routes_out, out, ws, l, hs(stream));
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- block-scaled FP8
+
+namespace {
+
+constexpr const char* kF8Shape = "unsupported FP8 block shape";
+constexpr int32_t kF8Widest = 32768, kF8MostRows = 1048576, kF8MostExperts = 1024;
+
+bool f8_width(int32_t v) { return v >= 8 && v <= kF8Widest && v % 8 == 0; }
+
+// Output columns of a product: as many as rows of a weight.
+bool f8_columns(int32_t v) { return v >= 8 && v <= kF8MostRows && v % 8 == 0; }
+
+int check_f8_gemm(int64_t m, int32_t n, int32_t k) {
+  if (!(m >= 0 && m <= kF8MostRows && f8_columns(n) && f8_width(k))) return fail(kF8Shape);
+  return CLEF_OK;
+}
+
+int check_f8_weight(int64_t matrices, int32_t n, int32_t k) {
+  if (!(matrices >= 1 && matrices <= kF8MostExperts && f8_columns(n) && f8_width(k) &&
+        matrices * clef::f8_blocks(n) * clef::f8_blocks(k) < ((int64_t)1 << 31)))
+    return fail(kF8Shape);
+  return CLEF_OK;
+}
+
+int check_f8_lists(int64_t a_rows, const int32_t* offsets, const int32_t* slots, int64_t experts, int64_t total,
+                   int32_t topk, int32_t input_routed, int32_t k, int32_t n) {
+  if (!(experts >= 1 && experts <= kF8MostExperts && total >= 0 && total <= 16777216 && topk >= 1 && topk <= 128))
+    return fail("invalid grouped expert lists");
+  if (!(f8_columns(n) && f8_width(k))) return fail(kF8Shape);
+  if (total == 0) return CLEF_OK;
+  if (a_rows < (input_routed ? total : (total + topk - 1) / topk))
+    return fail("expert lists name more rows than the activation has");
+  if (a_rows > kF8MostRows * (int64_t)128 || a_rows * clef::f8_pitch(k) > (int64_t)0xFFFFFFFF)
+    return fail("expert activation operand of 4 GiB or more (split the tokens into chunks)");
+  if (a_rows * clef::f8_blocks(k) * 4 > (int64_t)0x7FFFFFFF)
+    return fail("expert activation scales of 2 GiB or more (split the tokens into chunks)");
+  if (!aligned(offsets, 4) || (slots && !aligned(slots, 4))) return fail("expert list pointer is NULL or not aligned");
+  return CLEF_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t clef_f8_prepared_bytes(int64_t rows, int32_t width) {
+  if (rows < 0 || !f8_width(width)) return -1;
+  return clef::f8_prepared_bytes(rows, width);
+}
+
+int64_t clef_f8_weight_bytes(int64_t matrices, int64_t n, int32_t k) {
+  if (matrices < 1 || n < 8 || !f8_width(k)) return -1;
+  return clef::f8_weight_bytes(matrices, n, k);
+}
+
+int clef_f8_prepare(const uint16_t* x, int64_t rows, int32_t width, int64_t x_stride, uint8_t* out,
+                    clef_stream_t stream) {
+  if (!(rows >= 0 && rows <= (int64_t)kF8MostRows * 128 && f8_width(width) && x_stride >= width && x_stride % 8 == 0))
+    return fail(kF8Shape);
+  if (rows == 0) return CLEF_OK;
+  if (!aligned(x, 16) || !aligned(out, 16)) return fail(kAlign);
+  float* scales = reinterpret_cast<float*>(out + rows * clef::f8_pitch(width));
+  return hip_status(clef::launch_f8_prepare(x, rows, width, x_stride, out, scales, hs(stream)));
+}
+
+int clef_f8_pack_weight(const uint16_t* w, int64_t matrices, int32_t n, int32_t k, uint8_t* codes, float* scales,
+                        clef_stream_t stream) {
+  if (int rc = check_f8_weight(matrices, n, k)) return rc;
+  if (!aligned(w, 16) || !aligned(codes, 16) || !aligned(scales, 16)) return fail(kAlign);
+  return hip_status(clef::launch_f8_pack(w, matrices, n, k, codes, scales, hs(stream)));
+}
+
+int clef_f8_retile(const uint8_t* w, int64_t matrices, int32_t n, int32_t k, uint8_t* codes, clef_stream_t stream) {
+  if (int rc = check_f8_weight(matrices, n, k)) return rc;
+  if (!aligned(w, 16) || !aligned(codes, 16)) return fail(kAlign);
+  return hip_status(clef::launch_f8_retile(w, matrices, n, k, codes, hs(stream)));
+}
+
+int clef_f8_gemm(const uint8_t* a, const float* a_scales, const uint8_t* w, const float* w_scales, int64_t m,
+                 int32_t n, int32_t k, const uint16_t* residual, uint16_t* out, clef_stream_t stream) {
+  if (int rc = check_f8_gemm(m, n, k)) return rc;
+  if (m == 0) return CLEF_OK;
+  if (!aligned(a, 16) || !aligned(a_scales, 16) || !aligned(w, 16) || !aligned(w_scales, 16) || !aligned(out, 16) ||
+      (residual && !aligned(residual, 16)))
+    return fail(kAlign);
+  clef::F8Args x{};
+  x.a = a, x.as = a_scales, x.rows = m, x.w = w, x.ws = w_scales, x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
+  x.residual = residual, x.out = out;
+  return hip_status(clef::launch_f8_gemm(x, false, hs(stream)));
+}
+
+int clef_f8_gemm_gate_up(const uint8_t* a, const float* a_scales, const uint8_t* gate, const float* gate_scales,
+                         const uint8_t* up, const float* up_scales, int64_t m, int32_t n, int32_t k, uint16_t* h,
+                         clef_stream_t stream) {
+  if (int rc = check_f8_gemm(m, n, k)) return rc;
+  if (m == 0) return CLEF_OK;
+  if (!aligned(a, 16) || !aligned(a_scales, 16) || !aligned(gate, 16) || !aligned(gate_scales, 16) ||
+      !aligned(up, 16) || !aligned(up_scales, 16) || !aligned(h, 16))
+    return fail(kAlign);
+  clef::F8Args x{};
+  x.a = a, x.as = a_scales, x.rows = m, x.w = gate, x.ws = gate_scales, x.w2 = up, x.ws2 = up_scales;
+  x.n = n, x.kb = clef::f8_blocks(k), x.k = k, x.out = h;
+  return hip_status(clef::launch_f8_gemm(x, true, hs(stream)));
+}
+
+size_t clef_f8_project_workspace_bytes(int64_t m, int32_t n, int32_t k) {
+  if (m < 1 || m > kF8MostRows || !f8_columns(n) || !f8_width(k) || clef::f8_project_fusable(m, n, k)) return 0;
+  return (size_t)clef::f8_prepared_bytes(m, k);
+}
+
+int clef_f8_project(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint8_t* w, const float* w_scales,
+                    int32_t n, const uint16_t* residual, uint16_t* out, void* workspace, size_t workspace_bytes,
+                    clef_stream_t stream) {
+  if (int rc = check_f8_gemm(m, n, k)) return rc;
+  if (!(x_stride >= k && x_stride % 8 == 0)) return fail(kF8Shape);
+  if (m == 0) return CLEF_OK;
+  if (!aligned(x, 16) || !aligned(w, 16) || !aligned(w_scales, 16) || !aligned(out, 16) ||
+      (residual && !aligned(residual, 16)))
+    return fail(kAlign);
+  if (clef::f8_project_fusable(m, n, k)) {
+    clef::F8Args y{};
+    y.x = x, y.x_stride = x_stride, y.k = k, y.rows = m, y.w = w, y.ws = w_scales, y.n = n;
+    y.kb = clef::f8_blocks(k), y.residual = residual, y.out = out;
+    return hip_status(clef::launch_f8_gemm(y, false, hs(stream)));
+  }
+  if (!aligned(workspace, 16)) return fail(kAlign);
+  if (workspace_bytes < clef_f8_project_workspace_bytes(m, n, k)) return fail(kWorkspace);
+  uint8_t* a = static_cast<uint8_t*>(workspace);
+  if (int rc = clef_f8_prepare(x, m, k, x_stride, a, stream)) return rc;
+  return clef_f8_gemm(a, reinterpret_cast<const float*>(a + m * clef::f8_pitch(k)), w, w_scales, m, n, k, residual, out,
+                      stream);
+}
+
+size_t clef_moe_group_slots_workspace_bytes(int64_t tokens, int32_t topk, int32_t experts) {
+  if (tokens < 0 || !(tokens == 0 || routes_in_range(tokens, topk)) || experts < 1 || experts > kF8MostExperts) return 0;
+  return clef::group_slots_workspace_bytes(tokens * topk, experts);
+}
+
+int clef_moe_group_slots(const float* routes, int64_t tokens, int32_t topk, int32_t experts, int32_t* offsets,
+                         int32_t* slots, void* workspace, size_t workspace_bytes, clef_stream_t stream) {
+  if (tokens != 0 && !routes_in_range(tokens, topk)) return fail("unsupported Omni route grouping shape");
+  if (experts < 1 || experts > kF8MostExperts || topk < 1) return fail("invalid grouped expert lists");
+  if (!aligned(offsets, 4) || (tokens > 0 && (!aligned(routes, 4) || !aligned(slots, 4))))
+    return fail("expert list pointer is NULL or not aligned");
+  const size_t need = clef::group_slots_workspace_bytes(tokens * topk, experts);
+  if (need > 0 && !aligned(workspace, 16)) return fail(kAlign);
+  if (workspace_bytes < need) return fail(kWorkspace);
+  return hip_status(clef::launch_group_slots(routes, tokens, topk, experts, offsets, slots, workspace, hs(stream)));
+}
+
+int clef_moe_expert_f8(const uint8_t* a, const float* a_scales, int64_t a_rows, const uint8_t* w, const float* w_scales,
+                       const int32_t* offsets, const int32_t* slots, int32_t experts, int64_t total, int32_t topk,
+                       int32_t input_routed, int32_t k, int32_t n, uint16_t* out, clef_stream_t stream) {
+  if (int rc = check_f8_lists(a_rows, offsets, slots, experts, total, topk, input_routed, k, n)) return rc;
+  if (total == 0) return CLEF_OK;
+  if (!aligned(a, 16) || !aligned(a_scales, 16) || !aligned(w, 16) || !aligned(w_scales, 16) || !aligned(out, 16))
+    return fail(kAlign);
+  clef::F8Args x{};
+  x.a = a, x.as = a_scales, x.rows = a_rows, x.w = w, x.ws = w_scales, x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
+  x.out = out, x.lists = {offsets, slots, experts, (int)total, input_routed ? 1 : topk};
+  return hip_status(clef::launch_f8_experts(x, false, hs(stream)));
+}
+
+int clef_moe_expert_gate_up_f8(const uint8_t* a, const float* a_scales, int64_t a_rows, const uint8_t* gate,
+                               const float* gate_scales, const uint8_t* up, const float* up_scales,
+                               const int32_t* offsets, const int32_t* slots, int32_t experts, int64_t total,
+                               int32_t topk, int32_t input_routed, int32_t k, int32_t n, uint16_t* h,
+                               clef_stream_t stream) {
+  if (int rc = check_f8_lists(a_rows, offsets, slots, experts, total, topk, input_routed, k, n)) return rc;
+  if (total == 0) return CLEF_OK;
+  if (!aligned(a, 16) || !aligned(a_scales, 16) || !aligned(gate, 16) || !aligned(gate_scales, 16) ||
+      !aligned(up, 16) || !aligned(up_scales, 16) || !aligned(h, 16))
+    return fail(kAlign);
+  clef::F8Args x{};
+  x.a = a, x.as = a_scales, x.rows = a_rows, x.w = gate, x.ws = gate_scales, x.w2 = up, x.ws2 = up_scales;
+  x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
+  x.out = h, x.lists = {offsets, slots, experts, (int)total, input_routed ? 1 : topk};
+  return hip_status(clef::launch_f8_experts(x, true, hs(stream)));
 }
 
 }  // extern "C"

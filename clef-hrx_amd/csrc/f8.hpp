@@ -1,0 +1,181 @@
+// Block-scaled FP8 (e4m3): layouts, launchers and the device helpers that its
+// kernels share. Values are e4m3 codes with one scale for each block of 128
+// along k: y[m][n] = sum_b sa[m][b] sw[n / 128][b] sum_{k in block b} qa[m][k] qw[n][k].
+//
+// Activation ("prepared"): codes row-major [rows][pitch], pitch the width
+// rounded up to 128 (the rest zeros), then f32 scales [pitch / 128][rows]: the
+// scales that a tile needs in one k-step lie side by side.
+//
+// Weight: blocks of 128 rows x 128 k (16 KiB), block (r / 128, k / 128) of one
+// matrix at ((r / 128) * kb + k / 128) * 16384; rows and columns past the end
+// are zeros. Inside a block the order is that of the matrix operand
+// (v_mfma_*_16x16x128): fragment f of 16 rows at 2048 f, its halves h at 1024 h,
+// lane l's 16 bytes at 16 l, holding row 16 f + l % 16, k = 64 h + 16 (l / 16)
+// .. + 15. So a wave loads a half fragment as one contiguous KiB, into
+// registers or LDS alike, and LDS reads of it are conflict-free as they lie.
+// Scales f32 [matrices][ceil(rows / 128)][kb].
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "common.hpp"
+#include "gemm_dma.hpp"
+#include "launch.hpp"
+
+namespace clef {
+
+constexpr int f8_blocks(int64_t width) { return (int)((width + 127) / 128); }
+constexpr int64_t f8_pitch(int64_t width) { return (width + 127) / 128 * 128; }
+constexpr int64_t f8_prepared_bytes(int64_t rows, int64_t width) {
+  return rows * f8_pitch(width) + 4 * rows * f8_blocks(width);
+}
+constexpr int64_t f8_weight_bytes(int64_t matrices, int64_t rows, int64_t cols) {
+  return matrices * f8_blocks(rows) * f8_blocks(cols) * 16384;
+}
+
+// A ragged list of rows per expert: slots[offsets[e] .. offsets[e + 1]) are
+// expert e's (slots NULL: the places themselves). Slot s reads activation row
+// s / div and writes output row s.
+struct F8Lists {
+  const int32_t* offsets;
+  const int32_t* slots;
+  int experts;
+  int total;  // slots (and output rows)
+  int div;
+};
+
+// One product. Without lists: rows m of `a` against one matrix. gate/up: w the
+// gate, w2 the up matrices, n the width of h.
+struct F8Args {
+  const uint8_t* a;
+  const float* as;  // [kb][rows]
+  int64_t rows;     // rows of a
+  const uint8_t* w;
+  const float* ws;
+  const uint8_t* w2;
+  const float* ws2;
+  int n, kb;  // output columns, blocks of 128 along k
+  const uint16_t* residual;
+  uint16_t* out;
+  F8Lists lists;
+  // x in bf16 where the kernel quantizes its rows itself
+  const uint16_t* x;
+  int64_t x_stride;
+  int k;
+};
+
+hipError_t launch_f8_prepare(const uint16_t* x, int64_t rows, int width, int64_t x_stride, uint8_t* codes,
+                             float* scales, hipStream_t stream);
+hipError_t launch_f8_pack(const uint16_t* w, int64_t matrices, int n, int k, uint8_t* codes, float* scales,
+                          hipStream_t stream);
+hipError_t launch_f8_retile(const uint8_t* w, int64_t matrices, int n, int k, uint8_t* codes, hipStream_t stream);
+hipError_t launch_f8_gemm(const F8Args& x, bool gate_up, hipStream_t stream);
+// Whether x [m][k] and the product against n columns run as one launch that
+// quantizes the rows itself (F8Args::x).
+bool f8_project_fusable(int64_t m, int n, int k);
+hipError_t launch_f8_experts(const F8Args& x, bool gate_up, hipStream_t stream);
+size_t group_slots_workspace_bytes(int64_t slots, int experts);
+hipError_t launch_group_slots(const float* routes, int64_t tokens, int topk, int experts, int32_t* offsets,
+                              int32_t* slots, void* workspace, hipStream_t stream);
+
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef int v8i_t __attribute__((ext_vector_type(8)));
+
+// D = W A^T of a 16 x 16 tile over 128 k, added to c. Lane l holds weight row
+// l % 16 in w and activation row l % 16 in a, the 32 values of its k-group
+// l / 16 (any order of k that both share); D's lane l holds activation row
+// l % 16 and weight rows 4 (l / 16) .. + 3. cbsz = blgp = 0: e4m3 both, block
+// scales 127 (e8m0) = 1.
+__device__ __forceinline__ v4f mfma_f8(v8i_t w, v8i_t a, v4f c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 0, 127, 0, 127);
+}
+
+__device__ __forceinline__ v8i_t join_halves(v4i lo, v4i hi) {
+  return v8i_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+
+// silu(g) u of two f32 sums. The hardware's exp2 and reciprocal (each within
+// 1 ulp): both are far below the bf16 rounding that follows, and their limits
+// give silu's (exp2 of -inf is 0, 1 / inf is 0).
+__device__ __forceinline__ float f8_swiglu(float g, float u) {
+  const float e = __builtin_amdgcn_exp2f(g * -1.44269504088896341f);
+  return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+}
+
+// Exponent field of a block's scale: the least power of two at or above
+// amax / 448, from the bf16 bits of amax: amax = 1.m 2^E is at most 448 2^(E -
+// 8) = 1.75 2^E while m <= 0x60. At least 2^-126, so the scale and its
+// reciprocal (field 254 - s) are normal.
+__device__ __forceinline__ uint32_t f8_scale_field(uint32_t amax_bits) {
+  const int f = (int)(amax_bits >> 7) - 8 + ((amax_bits & 0x7Fu) > 0x60u ? 1 : 0);
+  return (uint32_t)(f > 1 ? f : 1);
+}
+
+// Four e4m3 codes of two bf16 pairs times `inv` (a power of two: exact), each
+// rounded to nearest even once. |value| <= 448 by the choice of the scale;
+// infinities are made NaN, which e4m3 has (0x7F) where it has no infinity.
+__device__ __forceinline__ uint32_t f8_codes(uint32_t p0, uint32_t p1, float inv) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(p0) * inv, bf16_hi(p0) * inv, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(p1) * inv, bf16_hi(p1) * inv, w, true);
+}
+
+// The largest finite magnitude of a bf16 pair against the halves of `m`, as
+// bf16 bits; non-finite values count as zero (they stay NaN in the codes).
+__device__ __forceinline__ uint32_t f8_amax2(uint32_t m, uint32_t pair) {
+  const uint32_t lo = pair & 0x7FFFu, hi = (pair >> 16) & 0x7FFFu;
+  const uint32_t a = lo < 0x7F80u ? lo : 0u, b = hi < 0x7F80u ? hi : 0u;
+  const uint32_t c = a > b ? a : b;
+  return m > c ? m : c;
+}
+
+// Tile `tile` of the experts' lists cut into tiles of BM slots, experts
+// ascending: its expert, first place and slots; false when there are fewer
+// tiles. Offsets outside 0 .. total or descending are clamped, so every place
+// is a slot. Each wave finds it by itself (a scan over 64 experts at a time).
+template <int BM>
+__device__ __forceinline__ bool f8_find_tile(const F8Lists& l, int tile, int& expert, int& first, int& count) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int c = 0; c < l.experts; c += 64) {
+    const int e = c + lane;
+    int lo = 0, hi = 0;
+    if (e < l.experts) {
+      lo = l.offsets[e];
+      hi = l.offsets[e + 1];
+    }
+    lo = lo < 0 ? 0 : lo > l.total ? l.total : lo;
+    hi = hi < lo ? lo : hi > l.total ? l.total : hi;
+    const int n = (hi - lo + BM - 1) / BM;
+    int incl = n;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(incl, off, 64);
+      if (lane >= off) incl += o;
+    }
+    const unsigned long long mask = __ballot(before + incl > tile);
+    if (mask != 0ull) {
+      const int at = __builtin_ctzll(mask);
+      expert = c + at;
+      const int begin = __builtin_amdgcn_readlane(lo, at), end = __builtin_amdgcn_readlane(hi, at);
+      const int tiles = __builtin_amdgcn_readlane(n, at), upto = __builtin_amdgcn_readlane(incl, at);
+      first = begin + (tile - before - (upto - tiles)) * BM;
+      count = end - first < BM ? end - first : BM;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return false;
+}
+
+// The most tiles of bm slots that lists over `total` slots can have.
+inline int64_t f8_most_tiles(int64_t total, int experts, int bm) {
+  return total / bm + (total < experts ? total : experts);
+}
+
+}  // namespace
+
+}  // namespace clef

@@ -1,0 +1,156 @@
+// Block-scaled FP8 operands: the quantizer of activation rows and the two
+// ways to a tiled weight (bf16 rows quantized, e4m3 rows of a checkpoint
+// rearranged). Layouts in f8.hpp.
+#include "f8.hpp"
+
+namespace clef {
+
+namespace {
+
+// x bf16 [rows][width] (row pitch x_stride) -> codes [rows][pitch], scales
+// [kb][rows]. 16 lanes hold a block of 128 columns, 8 values each: one 16-byte
+// load, the maximum over the 16 lanes by DPP, one 8-byte store of codes (a
+// whole line per block). A workgroup covers 2^RLOG rows x CPW * STEPS blocks, so
+// that the scales of neighbouring rows go out together, with STEPS loads in
+// flight per lane. Bound by HBM: 2 bytes read and 1 written per value.
+template <int RLOG, int STEPS>
+__global__ __launch_bounds__(256) void f8_prepare_kernel(const uint16_t* __restrict__ x, int64_t rows, int width,
+                                                         int64_t x_stride, int kb, uint8_t* __restrict__ codes,
+                                                         float* __restrict__ scales) {
+  constexpr int R = 1 << RLOG, CPW = 16 / R;
+  const int group = threadIdx.x >> 4, l = threadIdx.x & 15;
+  const int64_t row = (int64_t)blockIdx.x * R + (group & (R - 1));
+  const int b0 = blockIdx.y * (CPW * STEPS) + (group >> RLOG);
+  const bool row_here = row < rows;
+  const uint16_t* xr = x + row * x_stride;
+  uint4 v[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int col = (b0 + s * CPW) * 128 + 8 * l;  // width % 8 == 0: the 8 columns are all inside or all past the end
+    v[s] = uint4{0, 0, 0, 0};
+    if (row_here && col < width) v[s] = *reinterpret_cast<const uint4*>(xr + col);
+  }
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int b = b0 + s * CPW;
+    uint32_t m = f8_amax2(f8_amax2(f8_amax2(f8_amax2(0u, v[s].x), v[s].y), v[s].z), v[s].w);
+    m = group_max16(m);
+    if (!row_here || b >= kb) continue;
+    const uint32_t field = f8_scale_field(m);
+    const float inv = as_float((254u - field) << 23);
+    uint2 q;
+    q.x = f8_codes(v[s].x, v[s].y, inv);
+    q.y = f8_codes(v[s].z, v[s].w, inv);
+    *reinterpret_cast<uint2*>(codes + row * ((int64_t)kb * 128) + b * 128 + 8 * l) = q;
+    if (l == 0) scales[(int64_t)b * rows + row] = as_float(field << 23);
+  }
+}
+
+// Byte of (row, k) of a 128 x 128 block in the operand order (f8.hpp).
+__device__ __forceinline__ int f8_block_byte(int row, int k) {
+  const int chunk = k >> 4;
+  return (row >> 4) * 2048 + (chunk >> 2) * 1024 + ((chunk & 3) * 16 + (row & 15)) * 16 + (k & 15);
+}
+
+// One workgroup per 128 x 128 block of a bf16 weight: thread t takes 8 chunks
+// of 8 columns (rows t / 16 + 16 i, columns 8 (t % 16) ..), the block's maximum
+// meets in LDS, and the codes go out in the operand order. Weights are packed
+// once, at load.
+__global__ __launch_bounds__(256) void f8_pack_kernel(const uint16_t* __restrict__ w, int n, int k, int nb, int kb,
+                                                      uint8_t* __restrict__ codes, float* __restrict__ scales) {
+  __shared__ uint32_t wave_max[4];
+  const int64_t block = blockIdx.x;
+  const int kt = (int)(block % kb);
+  const int64_t panel = block / kb;
+  const int rb = (int)(panel % nb);
+  const int64_t e = panel / nb;
+  const int l = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+  const int col = kt * 128 + 8 * l;
+  uint4 v[8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = rb * 128 + r0 + 16 * i;
+    v[i] = uint4{0, 0, 0, 0};
+    if (row < n && col < k) v[i] = *reinterpret_cast<const uint4*>(w + (e * n + row) * (int64_t)k + col);
+    m = f8_amax2(f8_amax2(f8_amax2(f8_amax2(m, v[i].x), v[i].y), v[i].z), v[i].w);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)m, off);
+    m = m > o ? m : o;
+  }
+  if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = m > wave_max[i] ? m : wave_max[i];
+  const uint32_t field = f8_scale_field(m);
+  const float inv = as_float((254u - field) << 23);
+  uint8_t* out = codes + block * 16384;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint2 q;
+    q.x = f8_codes(v[i].x, v[i].y, inv);
+    q.y = f8_codes(v[i].z, v[i].w, inv);
+    *reinterpret_cast<uint2*>(out + f8_block_byte(r0 + 16 * i, 8 * l)) = q;
+  }
+  if (threadIdx.x == 0) scales[block] = as_float(field << 23);
+}
+
+// e4m3 rows [matrices][n][k] -> blocks in the operand order; one workgroup per
+// block, 8 bytes per thread and row (k % 8 == 0).
+__global__ __launch_bounds__(256) void f8_retile_kernel(const uint8_t* __restrict__ w, int n, int k, int nb, int kb,
+                                                        uint8_t* __restrict__ codes) {
+  const int64_t block = blockIdx.x;
+  const int kt = (int)(block % kb);
+  const int64_t panel = block / kb;
+  const int rb = (int)(panel % nb);
+  const int64_t e = panel / nb;
+  const int l = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+  const int col = kt * 128 + 8 * l;
+  uint8_t* out = codes + block * 16384;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = rb * 128 + r0 + 16 * i;
+    uint2 q{0, 0};
+    if (row < n && col < k) q = *reinterpret_cast<const uint2*>(w + (e * n + row) * (int64_t)k + col);
+    *reinterpret_cast<uint2*>(out + f8_block_byte(r0 + 16 * i, 8 * l)) = q;
+  }
+}
+
+}  // namespace
+
+hipError_t launch_f8_prepare(const uint16_t* x, int64_t rows, int width, int64_t x_stride, uint8_t* codes,
+                             float* scales, hipStream_t stream) {
+  const int kb = f8_blocks(width);
+  constexpr int STEPS = 4;
+  auto run = [&](auto rlog) {
+    constexpr int R = 1 << decltype(rlog)::value, per = 16 / R * STEPS;
+    const dim3 grid((unsigned)((rows + R - 1) / R), (unsigned)((kb + per - 1) / per));
+    f8_prepare_kernel<decltype(rlog)::value, STEPS>
+        <<<grid, 256, 0, stream>>>(x, rows, width, x_stride, kb, codes, scales);
+  };
+  // rows per workgroup: 8 where there are rows, else as many as there are
+  if (rows >= 8)
+    run(std::integral_constant<int, 3>{});
+  else if (rows >= 3)
+    run(std::integral_constant<int, 2>{});
+  else
+    run(std::integral_constant<int, 0>{});
+  return hipGetLastError();
+}
+
+hipError_t launch_f8_pack(const uint16_t* w, int64_t matrices, int n, int k, uint8_t* codes, float* scales,
+                          hipStream_t stream) {
+  const int nb = f8_blocks(n), kb = f8_blocks(k);
+  f8_pack_kernel<<<(unsigned)(matrices * nb * kb), 256, 0, stream>>>(w, n, k, nb, kb, codes, scales);
+  return hipGetLastError();
+}
+
+hipError_t launch_f8_retile(const uint8_t* w, int64_t matrices, int n, int k, uint8_t* codes, hipStream_t stream) {
+  const int nb = f8_blocks(n), kb = f8_blocks(k);
+  f8_retile_kernel<<<(unsigned)(matrices * nb * kb), 256, 0, stream>>>(w, n, k, nb, kb, codes);
+  return hipGetLastError();
+}
+
+}  // namespace clef

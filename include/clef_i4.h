@@ -485,6 +485,94 @@ int clef_moe_layer_static(const uint16_t* x, const void* logits, int32_t logits_
 int clef_moe_router_logits(const uint16_t* x, const uint16_t* gate_w, int64_t tokens, int32_t hidden,
                            int32_t experts, uint16_t* logits, clef_stream_t stream);
 
+/* ------------------------------------------------ block-scaled FP8 */
+
+/* e4m3 values with one scale for each block of 128 along k (no counterpart in
+ * the reference, whose narrow formats are integers):
+ *   y[m][n] = sum_b sa[m][b] * sw[n/128][b] * sum_{k in block b} qa[m][k] * qw[n][k]
+ * in f32, rounded to bf16 once (behind the residual or SwiGLU). Widths and
+ * column counts are multiples of 8; blocks may end inside.
+ *   activation      codes [rows][pitch], pitch = width rounded up to 128 (the
+ *                   rest zeros), then f32 scales [pitch/128][rows]
+ *   tiled weight    128-row x 128-k blocks of 16 KiB, block (r/128, k/128) of
+ *                   a matrix at ((r/128)*ceil(cols/128) + k/128)*16384, byte
+ *                   (r, k) of a block at (r/16)*2048 + (k/64)*1024 +
+ *                   ((k/16)%4*16 + r%16)*16 + k%16; zeros past the end; f32
+ *                   scales [matrices][ceil(rows/128)][ceil(cols/128)]
+ * Shape preconditions (all of them -> "unsupported FP8 block shape"): 8 <=
+ * width <= 32768, width % 8 == 0; 8 <= n <= 1048576, n % 8 == 0; 0 <= rows <=
+ * 1048576 (2^27 for the quantizer). With no rows a call does nothing. */
+
+/* Bytes of a prepared activation / of a weight's codes; -1 for widths the
+ * functions below reject. */
+int64_t clef_f8_prepared_bytes(int64_t rows, int32_t width);
+int64_t clef_f8_weight_bytes(int64_t matrices, int64_t n, int32_t k);
+
+/* Quantizer of bf16 rows (row pitch x_stride elements, a multiple of 8): per
+ * row and block the scale is the least power of two at or above amax / 448
+ * (2^-126 at least) and the code e4m3(x / scale), exact but for e4m3's
+ * rounding to nearest even. Non-finite values do not count in amax and become
+ * NaN codes. */
+int clef_f8_prepare(const uint16_t* x, int64_t rows, int32_t width, int64_t x_stride, uint8_t* out,
+                    clef_stream_t stream);
+
+/* bf16 weights [matrices][n][k] -> tiled codes and scales, the quantizer's
+ * rule on each 128 x 128 block. */
+int clef_f8_pack_weight(const uint16_t* w, int64_t matrices, int32_t n, int32_t k, uint8_t* codes, float* scales,
+                        clef_stream_t stream);
+
+/* e4m3 weights [matrices][n][k] as a checkpoint holds them -> tiled codes
+ * (their scales are used as they are). 1 <= matrices <= 1024. */
+int clef_f8_retile(const uint8_t* w, int64_t matrices, int32_t n, int32_t k, uint8_t* codes, clef_stream_t stream);
+
+/* Projection of a prepared activation; residual bf16 [m][n], nullable. */
+int clef_f8_gemm(const uint8_t* a, const float* a_scales, const uint8_t* w, const float* w_scales, int64_t m,
+                 int32_t n, int32_t k, const uint16_t* residual, uint16_t* out, clef_stream_t stream);
+
+/* h[m][n] = silu(g) * u of the two projections' f32 sums, bf16 once. */
+int clef_f8_gemm_gate_up(const uint8_t* a, const float* a_scales, const uint8_t* gate, const float* gate_scales,
+                         const uint8_t* up, const float* up_scales, int64_t m, int32_t n, int32_t k, uint16_t* h,
+                         clef_stream_t stream);
+
+/* clef_f8_prepare and clef_f8_gemm in one call; the workspace (bytes below, 0
+ * where a few rows are quantized by the product itself) takes the activation. */
+size_t clef_f8_project_workspace_bytes(int64_t m, int32_t n, int32_t k);
+int clef_f8_project(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint8_t* w, const float* w_scales,
+                    int32_t n, const uint16_t* residual, uint16_t* out, void* workspace, size_t workspace_bytes,
+                    clef_stream_t stream);
+
+/* Routes (as clef_moe_route writes them, any number of experts up to 1024)
+ * listed by expert: offsets [experts + 1], slots [tokens * topk]: the route
+ * ordinals t*topk+r of expert e, ascending, at offsets[e] .. offsets[e+1]. A
+ * slot naming no expert is left out; the places behind the last list become
+ * -1. Preconditions: tokens <= 1048576, topk <= 128, tokens * topk <= 16777216
+ * -> "unsupported Omni route grouping shape". */
+size_t clef_moe_group_slots_workspace_bytes(int64_t tokens, int32_t topk, int32_t experts);
+int clef_moe_group_slots(const float* routes, int64_t tokens, int32_t topk, int32_t experts, int32_t* offsets,
+                         int32_t* slots, void* workspace, size_t workspace_bytes, clef_stream_t stream);
+
+/* The experts' products over ragged lists: the slots at offsets[e] ..
+ * offsets[e+1] (slots NULL: the places themselves) belong to matrix e of w;
+ * slot s takes activation row input_routed ? s : s / topk and writes row s of
+ * out bf16 [total][n]. Rows that no list names are left as they were. Offsets
+ * are clamped to 0 .. total and slots outside it are passed over. An expert's
+ * list may be empty, and a slot may be listed by one expert only (two would
+ * write one row). Preconditions: 1 <= experts <= 1024, total <= 16777216, 1 <=
+ * topk <= 128 -> "invalid grouped expert lists"; the shapes above; a_rows >=
+ * the rows that total slots need -> "expert lists name more rows than the
+ * activation has"; codes of the activation below 4 GiB and its scales below
+ * 2 GiB. */
+int clef_moe_expert_f8(const uint8_t* a, const float* a_scales, int64_t a_rows, const uint8_t* w, const float* w_scales,
+                       const int32_t* offsets, const int32_t* slots, int32_t experts, int64_t total, int32_t topk,
+                       int32_t input_routed, int32_t k, int32_t n, uint16_t* out, clef_stream_t stream);
+
+/* h = silu(gate) * up over the same lists, as clef_f8_gemm_gate_up. */
+int clef_moe_expert_gate_up_f8(const uint8_t* a, const float* a_scales, int64_t a_rows, const uint8_t* gate,
+                               const float* gate_scales, const uint8_t* up, const float* up_scales,
+                               const int32_t* offsets, const int32_t* slots, int32_t experts, int64_t total,
+                               int32_t topk, int32_t input_routed, int32_t k, int32_t n, uint16_t* h,
+                               clef_stream_t stream);
+
 /* ------------------------------------------------------- packed cache */
 
 /* Key of a packed-weight cache entry (src/packed_cache.rs:24-33): the weight

@@ -1,0 +1,129 @@
+"""Block-scaled FP8 entry points without a GPU: sizes, refusals."""
+import numpy as np
+import pytest
+
+import clef_i4
+
+FAKE = 1 << 20  # never dereferenced: every call below fails its checks first
+SHAPE = "unsupported FP8 block shape"
+
+
+def call(name, *args):
+    rc = getattr(clef_i4.lib(), name)(*args)
+    return rc, clef_i4.lib().clef_last_error().decode()
+
+
+def test_sizes():
+    lib = clef_i4.lib()
+    assert lib.clef_f8_prepared_bytes(5, 128) == 5 * 128 + 5 * 4
+    assert lib.clef_f8_prepared_bytes(5, 136) == 5 * 256 + 2 * 5 * 4
+    assert lib.clef_f8_prepared_bytes(0, 136) == 0
+    assert lib.clef_f8_prepared_bytes(1 << 20, 32768) == (1 << 20) * (32768 + 1024)
+    assert lib.clef_f8_prepared_bytes(5, 130) == -1 and lib.clef_f8_prepared_bytes(5, 32776) == -1
+    assert lib.clef_f8_weight_bytes(3, 136, 264) == 3 * 2 * 3 * 16384
+    assert lib.clef_f8_weight_bytes(0, 136, 264) == -1 and lib.clef_f8_weight_bytes(1, 136, 0) == -1
+    assert lib.clef_f8_project_workspace_bytes(0, 256, 256) == 0
+    assert lib.clef_f8_project_workspace_bytes(4096, 256, 264) == 4096 * (384 + 12)
+    assert lib.clef_moe_group_slots_workspace_bytes(1 << 20, 16, 1024) > 0
+    assert lib.clef_moe_group_slots_workspace_bytes(1, 8, 128) == 0
+
+
+@pytest.mark.parametrize("rows,width,stride", [(4, 0, 8), (4, 12, 16), (4, 32776, 32776), (4, 256, 248), (4, 256, 260),
+                                               (-1, 256, 256), ((1 << 27) + 1, 256, 256)])
+def test_prepare_rejects(rows, width, stride):
+    rc, msg = call("clef_f8_prepare", FAKE, rows, width, stride, FAKE, None)
+    assert rc == -1 and msg == SHAPE
+
+
+def test_prepare_pointers_and_no_rows():
+    assert call("clef_f8_prepare", None, 0, 256, 256, None, None)[0] == 0
+    for x, out in [(None, FAKE), (FAKE + 2, FAKE), (FAKE, FAKE + 8)]:
+        rc, msg = call("clef_f8_prepare", x, 4, 256, 256, out, None)
+        assert rc == -1 and "aligned" in msg
+
+
+@pytest.mark.parametrize("matrices,n,k", [(0, 128, 128), (1025, 128, 128), (1, 0, 128), (1, 12, 128), (1, 128, 4),
+                                          (1, 128, 32776), (1, 1048584, 128), (1024, 1048576, 32768)])
+def test_weight_rejects(matrices, n, k):
+    rc, msg = call("clef_f8_pack_weight", FAKE, matrices, n, k, FAKE, FAKE, None)
+    assert rc == -1 and msg == SHAPE
+    rc, msg = call("clef_f8_retile", FAKE, matrices, n, k, FAKE, None)
+    assert rc == -1 and msg == SHAPE
+
+
+@pytest.mark.parametrize("m,n,k", [(-1, 128, 128), ((1 << 20) + 1, 128, 128), (4, 0, 128), (4, 100, 128), (4, 128, 12)])
+def test_products_reject(m, n, k):
+    assert call("clef_f8_gemm", FAKE, FAKE, FAKE, FAKE, m, n, k, None, FAKE, None) == (-1, SHAPE)
+    assert call("clef_f8_gemm_gate_up", FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, m, n, k, FAKE, None) == (-1, SHAPE)
+    assert call("clef_f8_project", FAKE, m, k, max(k, 16), FAKE, FAKE, n, None, FAKE, FAKE, 1 << 40, None) == (-1, SHAPE)
+
+
+def test_products_pointers_workspace_and_no_rows():
+    assert call("clef_f8_gemm", None, None, None, None, 0, 128, 128, None, None, None)[0] == 0
+    assert call("clef_f8_gemm_gate_up", *[None] * 6, 0, 128, 128, None, None)[0] == 0
+    assert call("clef_f8_project", None, 0, 128, 128, None, None, 128, None, None, None, 0, None)[0] == 0
+    good = [FAKE] * 4
+    for i in range(4):
+        bad = list(good)
+        bad[i] = FAKE + 4
+        rc, msg = call("clef_f8_gemm", *bad, 4, 128, 128, None, FAKE, None)
+        assert rc == -1 and "aligned" in msg
+    rc, msg = call("clef_f8_gemm", *good, 4, 128, 128, FAKE + 2, FAKE, None)
+    assert rc == -1 and "aligned" in msg
+    need = clef_i4.lib().clef_f8_project_workspace_bytes(4096, 256, 256)
+    rc, msg = call("clef_f8_project", FAKE, 4096, 256, 256, FAKE, FAKE, 256, None, FAKE, FAKE, need - 1, None)
+    assert rc == -1 and msg == "workspace too small"
+    rc, msg = call("clef_f8_project", FAKE, 4096, 256, 252, FAKE, FAKE, 256, None, FAKE, FAKE, need, None)
+    assert rc == -1 and msg == SHAPE
+
+
+def test_group_slots_rejects():
+    args = (FAKE, FAKE, FAKE, 1 << 30, None)
+    assert call("clef_moe_group_slots", FAKE, (1 << 20) + 1, 8, 128, *args)[1] == "unsupported Omni route grouping shape"
+    assert call("clef_moe_group_slots", FAKE, 1 << 20, 17, 128, *args)[1] == "unsupported Omni route grouping shape"
+    for experts in (0, 1025):
+        assert call("clef_moe_group_slots", FAKE, 4, 8, experts, *args)[1] == "invalid grouped expert lists"
+    assert call("clef_moe_group_slots", FAKE, 4, 8, 128, None, FAKE, FAKE, 1 << 30, None)[0] == -1
+    assert call("clef_moe_group_slots", FAKE, 4, 8, 128, FAKE, None, FAKE, 1 << 30, None)[0] == -1
+    need = clef_i4.lib().clef_moe_group_slots_workspace_bytes(65536, 8, 128)
+    rc, msg = call("clef_moe_group_slots", FAKE, 65536, 8, 128, FAKE, FAKE, FAKE, need - 1, None)
+    assert rc == -1 and msg == "workspace too small"
+
+
+@pytest.mark.parametrize("a_rows,experts,total,topk,routed,k,n,message", [
+    (4, 0, 8, 2, 0, 128, 128, "invalid grouped expert lists"),
+    (4, 1025, 8, 2, 0, 128, 128, "invalid grouped expert lists"),
+    (4, 8, -1, 2, 0, 128, 128, "invalid grouped expert lists"),
+    (4, 8, 1 << 25, 2, 0, 128, 128, "invalid grouped expert lists"),
+    (4, 8, 8, 0, 0, 128, 128, "invalid grouped expert lists"),
+    (4, 8, 8, 129, 0, 128, 128, "invalid grouped expert lists"),
+    (4, 8, 8, 2, 0, 130, 128, SHAPE),
+    (4, 8, 8, 2, 0, 128, 130, SHAPE),
+    (3, 8, 8, 2, 0, 128, 128, "expert lists name more rows than the activation has"),
+    (7, 8, 8, 2, 1, 128, 128, "expert lists name more rows than the activation has"),
+    (131073, 8, 8, 2, 0, 32768, 128, "expert activation operand of 4 GiB or more (split the tokens into chunks)"),
+])
+def test_experts_reject(a_rows, experts, total, topk, routed, k, n, message):
+    rest = (FAKE, FAKE, experts, total, topk, routed, k, n, FAKE, None)
+    assert call("clef_moe_expert_f8", FAKE, FAKE, a_rows, FAKE, FAKE, *rest) == (-1, message)
+    assert call("clef_moe_expert_gate_up_f8", FAKE, FAKE, a_rows, FAKE, FAKE, FAKE, FAKE, *rest) == (-1, message)
+
+
+def test_experts_pointers_and_no_slots():
+    none = (None, None, 4, None, None, None, None, 8, 0, 2, 0, 128, 128, None, None)
+    assert call("clef_moe_expert_f8", *none)[0] == 0
+    rc, msg = call("clef_moe_expert_f8", FAKE, FAKE, 4, FAKE, FAKE, None, FAKE, 8, 8, 2, 0, 128, 128, FAKE, None)
+    assert rc == -1 and "list pointer" in msg
+    rc, msg = call("clef_moe_expert_f8", FAKE, FAKE, 4, FAKE, FAKE, FAKE, FAKE + 2, 8, 8, 2, 0, 128, 128, FAKE, None)
+    assert rc == -1 and "list pointer" in msg
+    rc, msg = call("clef_moe_expert_f8", FAKE, FAKE, 4, FAKE, None, FAKE, FAKE, 8, 8, 2, 0, 128, 128, FAKE, None)
+    assert rc == -1 and "aligned" in msg
+
+
+def test_operand_order_is_a_permutation():
+    """The byte formula of a weight block (include/clef_i4.h) names each of the
+    16384 bytes once, and a lane's 16 bytes are 16 consecutive k of one row."""
+    r, k = np.meshgrid(np.arange(128), np.arange(128), indexing="ij")
+    at = (r // 16) * 2048 + (k // 64) * 1024 + ((k // 16) % 4 * 16 + r % 16) * 16 + k % 16
+    assert np.array_equal(np.sort(at.ravel()), np.arange(16384))
+    assert (np.diff(at.reshape(128, 8, 16), axis=2) == 1).all()

@@ -1,0 +1,515 @@
+"""Block-scaled FP8 on the GPU against plain implementations in 64 bits.
+
+Tolerances. Whole-number results (codes, scales, lists) are equal. A product's
+sum differs from the 64-bit one in two ways.
+* The FP8 matrix instruction adds eight neighbouring products at a time, each
+  cut (towards zero) to a multiple of 2^(E - 13), E the largest sum of the two
+  exponents among the eight (measured on the device with single products beside
+  a large pair that cancels). The largest of them is at least 2^E and an exact
+  multiple, so eight products are off by less than 7 * 2^-13 of the largest:
+  C = 7 * 2^-13 * (sum over the eights of the largest magnitude).
+* The eights of a block, and the blocks, are added in f32: at most G = (16 +
+  blocks + 4) * 2^-23 times the sum of the terms' magnitudes, each addition
+  taken as off by a whole unit in case it is cut, the scales' product and its
+  fma two more.
+bf16 then rounds by at most 2^-8 of the value. SwiGLU passes a gate error on by
+at most 1.1 |u| (the largest slope of silu is below 1.1) and an up error by
+|silu(g)|, and its own exp2, reciprocal and products add less than 2^-20 of the
+value. Products of small whole numbers lose nothing in any of these steps and
+are compared bit for bit.
+"""
+import pytest
+import torch
+
+import clef_i4
+
+pytestmark = pytest.mark.gpu
+F8 = torch.float8_e4m3fn
+BF = torch.bfloat16
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(shape, std, seed, dtype=BF):
+    return (torch.randn(shape, generator=gen(seed), device="cuda") * std).to(dtype)
+
+
+def quantize64(x):
+    """(codes as f64 values [rows][width], scales f64 [rows][kb]) of bf16 rows."""
+    rows, width = x.shape
+    v = torch.nn.functional.pad(x.cpu().double(), (0, -width % 128)).unflatten(1, (-1, 128))
+    mag = v.abs()
+    mag = torch.where(torch.isfinite(mag), mag, torch.zeros_like(mag))
+    part, e = torch.frexp(mag.amax(-1).clamp(min=2.0 ** -118) / 448.0)
+    e = torch.where(part == 0.5, e - 1, e)
+    scale = torch.ldexp(torch.ones_like(part), e)
+    q = (v / scale[..., None]).float()  # exact: a power of two
+    q = torch.where(torch.isfinite(v), q, torch.full_like(q, float("nan")))
+    return q.flatten(1)[:, :width].to(F8).double(), scale
+
+
+def weight(matrices, n, k, kind, seed):
+    """e4m3 codes [matrices][n][k] and scales as a checkpoint holds them."""
+    codes = randn((matrices, n, k), 60.0, seed, torch.float32).clamp(-448, 448).to(F8)
+    scales = torch.exp(torch.randn((matrices, -(-n // 128), -(-k // 128)), generator=gen(seed + 1), device="cuda") - 6)
+    if kind == "e8m0":
+        scales = torch.exp2(torch.round(torch.log2(scales))).to(torch.float8_e8m0fnu)
+    return codes, scales
+
+
+def weight64(codes, scales):
+    m, n, k = codes.shape
+    wide = scales.float().double().repeat_interleave(128, 1)[:, :n].repeat_interleave(128, 2)[:, :, :k]
+    return codes.double() * wide
+
+
+def rows64(a):
+    return a.codes.double() * a.scales.double().repeat_interleave(128, 1)[:, : a.width]
+
+
+def check(got, want, slack):
+    """|got - want| <= 2^-8 |want| + slack (1 + 2^-8), elementwise."""
+    got, want = got.double(), want.double()
+    off = (got - want).abs() - (2.0 ** -8 * want.abs() + slack * (1 + 2.0 ** -8))
+    assert torch.isfinite(got).all()
+    assert (off <= 0).all(), f"{(off > 0).sum().item()} of {off.numel()} off, worst by {off.max().item()}"
+
+
+def product64(x, w):
+    """x [m][k] times w [n][k] in f64, and how far off an f32 sum by FP8
+    matrix instructions may be (C + G above)."""
+    m, k = x.shape
+    n = w.shape[0]
+    pad = (0, -k % 8)
+    xe = torch.nn.functional.pad(x.abs().float(), pad).unflatten(1, (-1, 8))
+    we = torch.nn.functional.pad(w.abs().float(), pad).unflatten(1, (-1, 8))
+    largest = torch.zeros((m, n), device="cuda")
+    step = max(1, (1 << 27) // (8 * max(m * n, 1)))
+    for c in range(0, xe.shape[1], step):
+        largest += (xe[:, None, c: c + step] * we[None, :, c: c + step]).amax(-1).sum(-1)
+    mag = x.abs() @ w.abs().t()
+    return x @ w.t(), 7 * 2.0 ** -13 * largest.double() * (1 + 2.0 ** -10) + (20 + -(-k // 128)) * 2.0 ** -23 * mag
+
+
+def swiglu64(x, wg, wu):
+    (g, dg), (u, du) = product64(x, wg), product64(x, wu)
+    s = g * torch.sigmoid(g)
+    h = s * u
+    return h, 1.1 * dg * (u.abs() + du) + s.abs() * du + 2.0 ** -20 * h.abs()
+
+
+# ---------------------------------------------------------------- quantizer
+
+@pytest.mark.parametrize("rows,width", [(0, 128), (1, 8), (1, 2048), (2, 136), (3, 768), (7, 1000), (8, 128), (9, 4160),
+                                        (37, 264), (130, 2176), (16, 32768)])
+def test_prepare_matches_definition(rows, width):
+    x = randn((rows, width), 3.0, rows * 7 + width)
+    if rows:
+        x[0, : width // 2] = 0
+        x[-1] *= 1e-3
+    a = clef_i4.prepare_f8(x)
+    codes, scales = quantize64(x)
+    assert torch.equal(a.codes.cpu().double(), codes)
+    assert torch.equal(a.scales.cpu().double(), scales)
+    pad = a.storage[: rows * a.pitch].view(rows, a.pitch)[:, width:]
+    assert (pad == 0).all()
+
+
+def test_prepare_every_bf16_value():
+    """Every bf16 bit pattern, in blocks whose largest finite magnitude is each
+    binade's: normal, subnormal, zero, infinite, NaN."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(BF)
+    x = torch.cat([bits.view(512, 128), bits.view(128, 512).t().contiguous()]).cuda().contiguous()
+    a = clef_i4.prepare_f8(x[:, :128])
+    codes, scales = quantize64(x[:, :128])
+    assert torch.equal(a.scales.cpu().double(), scales)
+    got = a.codes.cpu().double()
+    assert torch.equal(torch.isnan(got), torch.isnan(codes))
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(codes))
+
+
+def test_prepare_edges_of_the_scale():
+    """amax at, just below and just above 448 * 2^e, ties of e4m3, e4m3
+    subnormals, blocks of nothing but zeros or non-finite values."""
+    x = torch.zeros((8, 256), dtype=BF, device="cuda")
+    x[0, 0], x[0, 1:5] = 448.0, torch.tensor([17.0, 19.0, 2.0 ** -9, 3 * 2.0 ** -10])
+    x[1, 0], x[1, 1] = 450.0, 1.0
+    x[2, 0], x[2, 1] = 446.0, 2.0 ** -10
+    x[3, 5] = float("inf")
+    x[4, 7], x[4, 9] = float("nan"), 5.0
+    x[5, :128] = float("-inf")
+    x[6, 0] = 3.3895313892515355e38
+    x[7, 0] = 1e-40
+    a = clef_i4.prepare_f8(x)
+    codes, scales = quantize64(x)
+    assert torch.equal(a.scales.cpu().double(), scales)
+    got = a.codes.cpu().double()
+    assert torch.equal(torch.isnan(got), torch.isnan(codes)) and torch.equal(torch.nan_to_num(got), torch.nan_to_num(codes))
+
+
+def test_prepare_strided_rows_and_reused_buffer():
+    wide = randn((19, 1024), 2.0, 5)
+    buffer = torch.full((100000,), 0xAB, dtype=torch.uint8, device="cuda")
+    for first, width in [(0, 512), (8, 520), (256, 768)]:
+        x = wide[:, first: first + width]
+        a = clef_i4.prepare_f8(x, out=buffer)
+        b = clef_i4.prepare_f8(x.contiguous())
+        n = b.storage.numel()
+        assert torch.equal(a.storage[:n], b.storage) and (a.storage[n:] == 0xAB).all()
+
+
+# ---------------------------------------------------------------- weights
+
+@pytest.mark.parametrize("matrices,n,k", [(1, 8, 8), (1, 128, 128), (2, 264, 392), (3, 40, 136)])
+def test_weight_layout(matrices, n, k):
+    """Tiled codes byte by byte, and the quantizer's rule on 128 x 128 blocks."""
+    nb, kb = -(-n // 128), -(-k // 128)
+    r, c = torch.meshgrid(torch.arange(nb * 128), torch.arange(kb * 128), indexing="ij")
+    at = ((r // 128 * kb + c // 128) * 16384 + r % 128 // 16 * 2048 + c % 128 // 64 * 1024 +
+          (c // 16 % 4 * 16 + r % 16) * 16 + c % 16)
+
+    def tiled(codes):
+        wide = torch.zeros((matrices, nb * 128, kb * 128), dtype=torch.uint8)
+        wide[:, :n, :k] = codes.view(torch.uint8).cpu()
+        out = torch.empty((matrices, nb * kb * 16384), dtype=torch.uint8)
+        out[:, at.reshape(-1)] = wide.view(matrices, -1)
+        return out.view(-1)
+
+    codes, scales = weight(matrices, n, k, "f32", 3)
+    w = clef_i4.f8_weight(codes, scales)
+    assert torch.equal(w.codes.cpu(), tiled(codes)) and torch.equal(w.scales, scales)
+    dense = randn((matrices, n, k), 0.05, 9)
+    w = clef_i4.load_f8_weight(dense)
+    blocks = torch.zeros((matrices, nb * 128, kb * 128))
+    blocks[:, :n, :k] = dense.float().cpu()
+    blocks = blocks.view(matrices, nb, 128, kb, 128).permute(0, 1, 3, 2, 4).reshape(-1, 128 * 128)
+    part, e = torch.frexp(blocks.double().abs().amax(-1).clamp(min=2.0 ** -118) / 448.0)
+    e = torch.where(part == 0.5, e - 1, e)
+    scale = torch.ldexp(torch.ones_like(part), e)
+    q = (blocks.double() / scale[:, None]).float().to(F8)
+    q = q.view(matrices, nb, kb, 128, 128).permute(0, 1, 3, 2, 4).reshape(matrices, nb * 128, kb * 128)[:, :n, :k]
+    assert torch.equal(w.codes.cpu(), tiled(q.contiguous()))
+    assert torch.equal(w.scales.cpu().view(-1).double(), scale)
+
+
+# ---------------------------------------------------------------- projections
+
+SHAPES = [(1, 128, 128), (1, 4096, 1024), (3, 136, 8), (16, 1000, 264), (17, 264, 1352), (37, 4160, 1352),
+          (64, 512, 128), (65, 2048, 520), (129, 1024, 2048), (257, 768, 1288), (300, 17408, 256), (700, 384, 4104),
+          (1030, 1152, 1032)]
+
+
+@pytest.mark.parametrize("m,k,n", SHAPES)
+@pytest.mark.parametrize("kind,res", [("f32", False), ("e8m0", True)])
+def test_project_matches_64_bits(m, k, n, kind, res):
+    x = randn((m, k), 1.0, m + k)
+    codes, scales = weight(1, n, k, kind, n)
+    w = clef_i4.f8_weight(codes[0], scales[0])
+    residual = randn((m, n), 30.0, 4) if res else None
+    a = clef_i4.prepare_f8(x)
+    want, slack = product64(rows64(a), weight64(codes, scales)[0])
+    if res:
+        want = want + residual.double()
+        slack += 2.0 ** -23 * want.abs()
+    out = torch.full((m + 1, n), 7.0, dtype=BF, device="cuda")
+    got = clef_i4.project_f8(a, w, residual, out=out[:m])
+    check(got, want, slack)
+    assert (out[m:] == 7.0).all()
+    again = clef_i4.project_quantized_f8(x, w, residual)
+    check(again, want, slack)
+    assert torch.equal(again, clef_i4.project_quantized_f8(x, w, residual))
+
+
+@pytest.mark.parametrize("m,k,n", SHAPES)
+def test_project_gate_up_matches_64_bits(m, k, n):
+    x = randn((m, k), 1.0, m + k)
+    (gc, gs), (uc, us) = weight(1, n, k, "f32", n), weight(1, n, k, "e8m0", n + 2)
+    a = clef_i4.prepare_f8(x)
+    want, slack = swiglu64(rows64(a), weight64(gc, gs)[0] * 0.02, weight64(uc, us)[0])
+    gate, up = clef_i4.f8_weight(gc[0], gs[0] * 0.02), clef_i4.f8_weight(uc[0], us[0])
+    out = torch.full((m + 1, n), 7.0, dtype=BF, device="cuda")
+    # the scales' product with 0.02 is rounded to f32 in the one, not the other
+    check(clef_i4.project_gate_up_f8(a, gate, up, out=out[:m]), want, slack + 2.0 ** -22 * want.abs() + 2.0 ** -22 * slack)
+    assert (out[m:] == 7.0).all()
+
+
+def whole(shape, top, seed):
+    return torch.randint(-top, top + 1, shape, generator=gen(seed), device="cuda").float()
+
+
+@pytest.mark.parametrize("m,k,n", SHAPES)
+def test_project_of_whole_numbers_is_exact(m, k, n):
+    """Whole numbers up to 15: products at most 2^8 apart, sums below 2^24, so
+    nothing is lost before the rounding to bf16."""
+    x = whole((m, k), 15, m + k)
+    w = whole((n, k), 15, n)
+    x[:, ::128] = 15.0
+    nb, kb = -(-n // 128), -(-k // 128)
+    scales = torch.exp2(torch.randint(-3, 1, (nb, kb), generator=gen(3), device="cuda").float())
+    packed = clef_i4.f8_weight(w.to(F8), scales)
+    res = whole((m, n), 255, 5)
+    wide = w.double() * scales.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+    want = x.double() @ wide.t()
+    assert torch.equal(clef_i4.project_quantized_f8(x.to(BF), packed), want.float().to(BF))
+    assert torch.equal(clef_i4.project_f8(clef_i4.prepare_f8(x.to(BF)), packed, res.to(BF)),
+                       (want + res.double()).float().to(BF))
+
+
+def test_project_loaded_weight_and_strided_rows():
+    wide = randn((21, 800), 1.0, 1)
+    x = wide[:, 16: 16 + 520]
+    dense = randn((392, 520), 0.05, 2)
+    w = clef_i4.load_f8_weight(dense)
+    got = clef_i4.project_quantized_f8(x, w)
+    assert torch.equal(got, clef_i4.project_quantized_f8(x.contiguous(), w))
+    rel = (got.double() - x.double() @ dense.double().t()).norm() / (x.double() @ dense.double().t()).norm()
+    assert rel < 2 * 2.0 ** -4  # each operand's codes are off by at most 2^-4
+
+
+def test_project_non_finite_rows_and_values():
+    """A row with NaN or infinity gives NaN in its own outputs only; saturated
+    sums become infinite, SwiGLU's far tails its limits."""
+    x = randn((40, 256), 1.0, 1)
+    x[3, 5], x[17, 200] = float("nan"), float("inf")
+    codes, scales = weight(1, 264, 256, "f32", 2)
+    w = clef_i4.f8_weight(codes[0], scales[0])
+    got = clef_i4.project_quantized_f8(x, w)
+    bad = torch.isnan(got).all(1)
+    assert bad.nonzero().flatten().tolist() == [3, 17] and torch.isfinite(got[~bad]).all()
+    big = clef_i4.f8_weight(codes[0].float().abs().clamp(min=1).to(F8), torch.full_like(scales[0], 3e38))
+    assert torch.isinf(clef_i4.project_quantized_f8(torch.ones_like(x), big)).all()
+    eye = torch.zeros((8, 256), device="cuda")
+    eye[:, 0] = torch.tensor([448.0, -448.0, 100, -100, 20, -20, 0, 1])
+    ones = torch.zeros((8, 256), device="cuda")
+    ones[:, 1] = 1.0
+    one = torch.ones((1, 2), device="cuda")
+    v = torch.zeros((1, 256), dtype=BF, device="cuda")
+    v[0, :2] = 1.0
+    a = clef_i4.prepare_f8(v)
+    h = clef_i4.project_gate_up_f8(a, clef_i4.f8_weight(eye.to(F8), one), clef_i4.f8_weight(ones.to(F8), one))
+    g = eye[:, 0].to(F8).double()
+    want = g * torch.sigmoid(g)
+    assert ((h[0].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-30).all()
+
+
+# ---------------------------------------------------------------- lists
+
+@pytest.mark.parametrize("tokens,topk,experts", [(0, 8, 128), (1, 1, 1), (1, 8, 128), (2, 3, 8), (63, 1, 2), (235, 8, 128),
+                                                 (256, 8, 60), (257, 8, 128), (700, 6, 300), (5000, 8, 128),
+                                                 (3000, 4, 1024), (70000, 8, 64)])
+def test_group_slots_is_a_stable_sort(tokens, topk, experts):
+    g = gen(tokens + experts)
+    ids = torch.randint(0, experts, (tokens, topk), generator=g, device="cuda")
+    if tokens > 60:
+        ids[tokens // 2:] = torch.randint(0, max(1, experts // 9), (tokens - tokens // 2, topk), generator=g, device="cuda")
+    ids = ids.float()
+    if tokens > 2:
+        ids[1, 0], ids[2, -1], ids[tokens // 3, 0] = -1.0, float(experts), float("nan")
+    routes = torch.cat([ids, torch.rand((tokens, topk), generator=g, device="cuda")], 1)
+    offsets, slots = clef_i4.omni_group_slots(routes, experts)
+    flat = ids.reshape(-1).cpu()
+    valid = (flat > -1) & (flat < experts)
+    key = torch.where(valid, torch.nan_to_num(flat), torch.tensor(float(experts))).long()
+    order = torch.argsort(key, stable=True)[: int(valid.sum())]
+    counts = torch.bincount(key, minlength=experts + 1)[:experts]
+    assert offsets.cpu().tolist() == [0] + counts.cumsum(0).tolist()
+    assert torch.equal(slots[: order.numel()].cpu().long(), order)
+    assert (slots[order.numel():] == -1).all()
+
+
+# ---------------------------------------------------------------- experts
+
+def lists(tokens, topk, experts, seed, empty=()):
+    """Distinct random experts per token, none of `empty`."""
+    score = torch.rand((tokens, experts), generator=gen(seed), device="cuda")
+    score += 2.0 * torch.rand(experts, generator=gen(seed + 1), device="cuda")
+    for e in empty:
+        score[:, e] = -1
+    ids = score.topk(topk, 1)[1].float()
+    return clef_i4.omni_group_slots(torch.cat([ids, torch.ones_like(ids)], 1), experts), ids.long()
+
+
+EXPERTS = [(1, 8, 128, 256, 136), (1, 1, 1, 8, 8), (5, 2, 4, 384, 200), (37, 8, 60, 264, 136), (235, 4, 16, 768, 264),
+           (300, 1, 3, 1152, 128), (900, 2, 5, 256, 392), (2100, 8, 24, 136, 128)]
+
+
+@pytest.mark.parametrize("tokens,topk,experts,k,n", EXPERTS)
+def test_experts_match_64_bits(tokens, topk, experts, k, n):
+    empty = (0, experts - 1) if experts > topk + 2 else ()
+    (offsets, slots), ids = lists(tokens, topk, experts, tokens + n, empty)
+    total = tokens * topk
+    codes, scales = weight(experts, n, k, "f32", 5)
+    uc, us = weight(experts, n, k, "e8m0", 7)
+    w, up = clef_i4.f8_weight(codes, scales), clef_i4.f8_weight(uc, us)
+    gate = clef_i4.f8_weight(codes, scales * 2.0 ** -6)
+    w64, u64 = weight64(codes, scales), weight64(uc, us)
+    a = clef_i4.prepare_f8(randn((tokens, k), 1.0, 1))
+    routed = clef_i4.prepare_f8(randn((total, k), 1.0, 2))
+    x, xr = rows64(a), rows64(routed)
+    want = torch.empty((total, n), dtype=torch.float64, device="cuda")
+    want_t, want_h = torch.empty_like(want), torch.empty_like(want)
+    slack, slack_t, slack_h = torch.empty_like(want), torch.empty_like(want), torch.empty_like(want)
+    flat = ids.reshape(-1)
+    for e in range(experts):
+        s = (flat == e).nonzero().flatten()
+        want[s], slack[s] = product64(xr[s], w64[e])
+        want_t[s], slack_t[s] = product64(x[s // topk], w64[e])
+        want_h[s], slack_h[s] = swiglu64(x[s // topk], w64[e] * 2.0 ** -6, u64[e])
+    out = torch.full((total + 1, n), 7.0, dtype=BF, device="cuda")
+    check(clef_i4.expert_f8(routed, w, offsets, slots, topk, True, out=out[:total]), want, slack)
+    assert (out[total] == 7.0).all()
+    check(clef_i4.expert_f8(a, w, offsets, slots, topk, False), want_t, slack_t)
+    h = clef_i4.expert_gate_up_f8(a, gate, up, offsets, slots, topk, out=out[:total])
+    check(h, want_h, slack_h)
+    assert (out[total] == 7.0).all()
+    assert torch.equal(h, clef_i4.expert_gate_up_f8(a, gate, up, offsets, slots, topk))
+    # rows sorted by expert, lists without slots
+    order = slots.long()
+    sorted_a = clef_i4.prepare_f8(randn((total, k), 1.0, 2)[order])
+    got = clef_i4.expert_f8(sorted_a, w, offsets, None, 1, True)
+    check(got, want[order], slack[order])
+
+
+def test_experts_leave_unlisted_rows_and_odd_lists():
+    """Rows behind the last list, slots outside the table and offsets outside
+    it or descending: nothing else is written."""
+    k, n, experts, total = 256, 136, 4, 70
+    codes, scales = weight(experts, n, k, "f32", 5)
+    w = clef_i4.f8_weight(codes, scales)
+    a = clef_i4.prepare_f8(randn((total, k), 1.0, 2))
+    w64, x = weight64(codes, scales), rows64(a)
+
+    def run(offsets, slots):
+        out = torch.full((total, n), 7.0, dtype=BF, device="cuda")
+        clef_i4.expert_f8(a, w, torch.tensor(offsets, dtype=torch.int32, device="cuda"),
+                          None if slots is None else torch.tensor(slots, dtype=torch.int32, device="cuda"), 1, True, out)
+        return out
+
+    def same(out, rows):
+        left = torch.ones(total, dtype=torch.bool)
+        for row, e in rows.items():
+            want, slack = product64(x[row: row + 1], w64[e])
+            check(out[row: row + 1], want, slack)
+            left[row] = False
+        assert (out[left.cuda()] == 7.0).all()
+
+    same(run([0, 3, 3, 20, 41], None), {**{r: 0 for r in range(3)}, **{r: 2 for r in range(3, 20)},
+                                        **{r: 3 for r in range(20, 41)}})
+    same(run([0, 0, 0, 0, 0], None), {})
+    slots = list(range(total))
+    slots[1], slots[2], slots[5] = -1, total, 1 << 30
+    same(run([0, 4, 4, 4, 8], slots), {0: 0, 3: 0, 4: 3, 6: 3, 7: 3})
+    same(run([-5, 2, 2, 60, 1 << 30], None), {**{r: 0 for r in range(2)}, **{r: 2 for r in range(2, 60)},
+                                              **{r: 3 for r in range(60, total)}})
+    same(run([10, 5, 8, 8, 8], None), {r: 1 for r in range(5, 8)})
+
+
+# ---------------------------------------------------------------- together
+
+def moe(experts=16, d=264, f=136, topk=4):
+    gate, up = (clef_i4.load_f8_weight(randn((experts, f, d), 0.05, s)) for s in (1, 2))
+    down = clef_i4.load_f8_weight(randn((experts, d, f), 0.05, 3))
+    return clef_i4.MoeLayerF8(gate, up, down, topk), (gate, up, down)
+
+
+@pytest.mark.parametrize("tokens", [1, 30, 500])
+def test_moe_layer_is_its_steps(tokens):
+    """The layer equals its operators called one by one, and stays within the
+    FP8 roundings of the block in 64 bits."""
+    layer, (gate, up, down) = moe()
+    x, logits = randn((tokens, 264), 1.0, 4), randn((tokens, 16), 1.0, 5)
+    got = layer(x, logits)
+    routes = clef_i4.omni_route(logits, 4)
+    offsets, slots = clef_i4.omni_group_slots(routes, 16)
+    a = clef_i4.prepare_f8(x)
+    h = clef_i4.expert_gate_up_f8(a, gate, up, offsets, slots, 4)
+    values = clef_i4.expert_f8(clef_i4.prepare_f8(h), down, offsets, slots, 4, True)
+    assert torch.equal(got, clef_i4.omni_combine(values, routes))
+    wg, wu = (randn((16, 136, 264), 0.05, s).double() for s in (1, 2))
+    wd = randn((16, 264, 136), 0.05, 3).double()
+    want = torch.zeros((tokens, 264), dtype=torch.float64, device="cuda")
+    for r in range(4):
+        e = routes[:, r].long()
+        g = torch.bmm(wg[e], x.double()[:, :, None])[..., 0]
+        u = torch.bmm(wu[e], x.double()[:, :, None])[..., 0]
+        y = torch.bmm(wd[e], (g * torch.sigmoid(g) * u)[:, :, None])[..., 0]
+        want += routes[:, 4 + r, None].double() * y
+    # five codes on the way (x, gate, up, h, down), each off by at most 2^-4
+    assert (got.double() - want).norm() / want.norm() < 5 * 2.0 ** -4
+
+
+@pytest.mark.parametrize("tokens", [3, 200])
+def test_graph_replays_match_eager(tokens):
+    """A captured layer and projections, replayed between eager calls on other
+    inputs; two graphs, each with its own intermediates."""
+    layer, _ = moe()
+    w = clef_i4.load_f8_weight(randn((520, 264), 0.05, 8))
+    gate, up = (clef_i4.load_f8_weight(randn((392, 264), 0.05, s)) for s in (9, 10))
+    inputs = [(randn((tokens, 264), 1.0, 20 + i), randn((tokens, 16), 1.0, 30 + i)) for i in range(4)]
+
+    def step(x, logits):
+        y = layer(x, logits)
+        return y, clef_i4.project_quantized_f8(y, w), clef_i4.project_gate_up_f8(clef_i4.prepare_f8(y), gate, up)
+
+    want = [step(*i) for i in inputs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = step(*inputs[1])
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(on_side, want[1]))
+    graphs = []
+    for _ in range(2):
+        x, logits = (t.clone() for t in inputs[0])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(x, logits)
+        graphs.append((graph, x, logits, out))
+    for i in (0, 1, 2, 3, 1, 0):
+        for g, (graph, x, logits, out) in enumerate(graphs):
+            j = (i + g) % 4
+            x.copy_(inputs[j][0])
+            logits.copy_(inputs[j][1])
+            graph.replay()
+        step(*inputs[(i + 2) % 4])
+        torch.cuda.synchronize()
+        for g, (_, _, _, out) in enumerate(graphs):
+            assert all(torch.equal(a, b) for a, b in zip(out, want[(i + g) % 4]))
+
+
+def test_binding_refusals():
+    x = randn((4, 256), 1.0, 1)
+    a = clef_i4.prepare_f8(x)
+    w = clef_i4.load_f8_weight(randn((128, 256), 0.1, 2))
+    two = clef_i4.load_f8_weight(randn((2, 128, 256), 0.1, 2))
+    other = clef_i4.load_f8_weight(randn((128, 264), 0.1, 2))
+    offsets = torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")
+    refused = [
+        lambda: clef_i4.prepare_f8(x.float()),
+        lambda: clef_i4.prepare_f8(x[:, :252]),
+        lambda: clef_i4.prepare_f8(x[:, 4:252].t()),
+        lambda: clef_i4.prepare_f8(x[:, 4:252]),  # rows that do not start on 16 bytes
+        lambda: clef_i4.prepare_f8(x, out=torch.empty(10, dtype=torch.uint8, device="cuda")),
+        lambda: clef_i4.prepare_f8(x.cpu()),
+        lambda: clef_i4.load_f8_weight(x.float()),
+        lambda: clef_i4.f8_weight(x, torch.ones((1, 2), device="cuda")),
+        lambda: clef_i4.f8_weight(x.to(F8), torch.ones((2, 1), device="cuda")),
+        lambda: clef_i4.project_f8(a, other),
+        lambda: clef_i4.project_f8(a, two),
+        lambda: clef_i4.project_f8(a, w, residual=randn((4, 120), 1.0, 1)),
+        lambda: clef_i4.project_f8(a, w, out=torch.empty((4, 128), device="cuda")),
+        lambda: clef_i4.project_quantized_f8(x, two),
+        lambda: clef_i4.project_gate_up_f8(a, w, other),
+        lambda: clef_i4.expert_f8(a, two, offsets[:2], None, 1, True),
+        lambda: clef_i4.expert_f8(a, two, offsets.long(), None, 1, True),
+        lambda: clef_i4.expert_f8(a, two, offsets, torch.zeros(9, dtype=torch.int32, device="cuda"), 2, False),
+        lambda: clef_i4.expert_f8(a, two, offsets.cpu(), None, 1, True),
+        lambda: clef_i4.omni_group_slots(torch.zeros((4, 3), device="cuda")),
+        lambda: clef_i4.omni_group_slots(torch.zeros((4, 4), device="cuda"), 2000),
+    ]
+    for i, f in enumerate(refused):
+        with pytest.raises(clef_i4.ClefError):
+            f()
+            pytest.fail(f"refusal {i} did not raise")
