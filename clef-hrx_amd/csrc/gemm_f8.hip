@@ -187,8 +187,332 @@ hipError_t launch_stream(const F8Args& x, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// Tile shape of f8_tile_kernel: WAVES_M x WAVES_N waves of WM rows x WN weight
+// rows, NST LDS stages of one block of k each: A rows (128 bytes each, 16-byte
+// chunk c of row r at c ^ ((r >> 1) & 7)), B fragments in the operand order, the
+// rows' scales (per 16 WM / 16-value groups, in the order the lanes read them)
+// and the two weight panels' scales.
+template <int WM_, int WN_, int WAVES_M_, int WAVES_N_, int NST_>
+struct F8Tile {
+  static constexpr int WM = WM_, WN = WN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, NST = NST_;
+  static constexpr int NW = WAVES_M * WAVES_N, THREADS = 64 * NW;
+  static constexpr int BM = WM * WAVES_M, BN = WN * WAVES_N;
+  static constexpr int TM = WM / 16, TN = WN / 16;  // fragments per wave
+  static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, SA_BYTES = BM * 4, SW_BYTES = 256;
+  static constexpr int SA = A_BYTES + B_BYTES, SW = SA + SA_BYTES;
+  static constexpr int STAGE_BYTES = SW + SW_BYTES * (NW - BM / 64);
+  static constexpr int A_SLOTS = A_BYTES / 1024 / NW, B_SLOTS = B_BYTES / 1024 / NW;
+  static constexpr int DMA = A_SLOTS + B_SLOTS + 1;  // instructions per wave and stage
+  static constexpr int ROWS = NST * STAGE_BYTES;     // lists: the tile's output rows
+  static constexpr int LDS = ROWS + BM * 4;
+  static constexpr int EPI = 16 * WN * 2;            // epilogue staging per wave
+  static_assert(NW == 8 && BN == 256 && BM / 64 < NW, "eight waves, two weight panels");
+  static_assert(A_BYTES % (1024 * NW) == 0 && LDS <= 160 * 1024 && TM >= 4 && TN == 4, "whole instructions per wave");
+};
+
+// Many rows: tiles of BM rows x 256 weight rows through a ring of LDS stages
+// filled by DMA.
+//
+// A wave's step (one block of k) is TM rows of fragments times TN weight
+// fragments. It holds the weight fragments of the step, reads an activation
+// fragment one row of MFMAs ahead of its use, and adds a partial sum to its
+// accumulator by four fmas two MFMAs after the MFMA that made it, so the
+// scaling (4 VALU operations per MFMA, half its issue time) runs under the
+// MFMAs. Before the last row of MFMAs one barrier: the next stage has landed for
+// every wave, this one is read by every wave; under that row the first operands
+// of the next step are read, and under it and the next step's first rows the
+// DMA of step kt + NST goes into this stage, one instruction per MFMA.
+template <class T, bool LISTS, bool GU, bool RESID>
+__global__ __launch_bounds__(T::THREADS) void f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  extern __shared__ __align__(16) char lds[];
+  constexpr int TM = T::TM, TN = T::TN, COLS = GU ? T::BN / 2 : T::BN;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, g = lane >> 4;
+  const int wm = wave / T::WAVES_N, wn = wave % T::WAVES_N;
+  const int kb = p.kb, pitch = kb * 128;
+  int tm, tn, expert = 0, first = 0, here;
+  int64_t m0 = 0;
+  if constexpr (LISTS) {
+    // consecutive blocks of an XCD take the columns of one tile of rows, then the
+    // expert's next rows: both operands stay in its L2
+    const int blocks = tiles_m * tiles_n, per = blocks / 8, b = blockIdx.x;
+    const int r = b < 8 * per ? (b % 8) * per + b / 8 : b;
+    tm = r / tiles_n;
+    tn = r - tm * tiles_n;
+    if (!f8_find_tile<T::BM>(p.lists, tm, expert, first, here)) return;
+  } else {
+    tile_of_block(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
+    m0 = (int64_t)tm * T::BM;
+    here = p.rows - m0 < T::BM ? (int)(p.rows - m0) : T::BM;
+  }
+  const int n0 = tn * COLS;
+  int* out_rows = reinterpret_cast<int*>(lds + T::ROWS);
+
+  // this wave's DMA: A instruction q = A_SLOTS wave + s moves rows 8 q .. + 7
+  int a_voff[T::A_SLOTS], s_voff;
+  auto source_row = [&](int r) -> int64_t {  // row of a (dense: from m0); rows past the end repeat the last
+    r = r < here ? r : here - 1;
+    if constexpr (!LISTS) return r;
+    const int slot = p.lists.slots ? p.lists.slots[first + r] : first + r;
+    const int64_t row = slot >= 0 && slot < p.lists.total ? slot / p.lists.div : 0;
+    return row < p.rows ? row : 0;
+  };
+#pragma unroll
+  for (int s = 0; s < T::A_SLOTS; ++s) {
+    const int r = 8 * (T::A_SLOTS * wave + s) + (lane >> 3);
+    a_voff[s] = (int)((uint32_t)source_row(r) * (uint32_t)pitch) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
+  }
+  const __amdgpu_buffer_rsrc_t a_rsrc =
+      make_rsrc(p.a + (LISTS ? 0 : m0 * pitch), (uint32_t)(LISTS ? p.rows * pitch : (int64_t)here * pitch));
+  // B: waves 0-3 the first panel, 4-7 the second (gate/up: the up panel); a
+  // panel past the last column is empty
+  const int panel_of = wave / 4, nb = f8_blocks(p.n);
+  const int panel = n0 / 128 + (GU ? 0 : panel_of);
+  const uint8_t* wbase = GU && panel_of ? p.w2 : p.w;
+  const float* sbase = GU ? p.ws : p.ws;
+  const int64_t first_block = (int64_t)expert * nb * kb;
+  const __amdgpu_buffer_rsrc_t b_rsrc =
+      make_rsrc(wbase + (first_block + (int64_t)panel * kb) * 16384, panel < nb ? (uint32_t)kb * 16384u : 0u);
+  const int b_voff = (wave & 3) * (T::B_SLOTS * 1024) + lane * 16;
+  // scales: the first BM / 64 waves the rows', the others the panels' (lane 0
+  // the first, lane 1 the second)
+  const bool row_scales = wave < T::BM / 64;
+  __amdgpu_buffer_rsrc_t s_rsrc;
+  if (row_scales) {
+    const int word = 64 * wave + lane, r = word / T::WM * T::WM + 16 * (word % TM) + word % T::WM / TM;
+    s_voff = (int)(source_row(r) * 4);
+    s_rsrc = make_rsrc(p.as + m0, (uint32_t)((p.rows * kb - m0) * 4));
+  } else if (GU) {
+    const float* second = wave & 1 ? p.ws2 : p.ws;
+    s_voff = 0;
+    s_rsrc = make_rsrc(second + first_block + (int64_t)(n0 / 128) * kb, (uint32_t)kb * 4u);
+  } else {
+    const int q = n0 / 128 + (wave & 1);
+    s_voff = 0;
+    s_rsrc = make_rsrc(sbase + first_block + (int64_t)q * kb, q < nb ? (uint32_t)kb * 4u : 0u);
+  }
+  const int s_dst = row_scales ? T::SA + wave * 256 : T::SW + (wave - T::BM / 64) * T::SW_BYTES;
+  const int s_step = row_scales ? (int)(p.rows * 4) : 4;
+  if constexpr (LISTS) {
+    for (int r = threadIdx.x; r < T::BM; r += T::THREADS) {
+      int slot = -1;
+      if (r < here) {
+        slot = p.lists.slots ? p.lists.slots[first + r] : first + r;
+        slot = slot < p.lists.total ? slot : -1;
+      }
+      out_rows[r] = slot;
+    }
+  }
+  const __amdgpu_buffer_rsrc_t none = make_rsrc(p.a, 0);
+  // DMA instruction x of stage kt into `stage` (stages past the end: zeros
+  // that nothing reads, so that every step issues and waits alike)
+  auto issue = [&](char* stage, int kt, int x) {
+    const bool in = kt < kb;
+    const int k = in ? kt : 0;
+    if (x < T::A_SLOTS)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? a_rsrc : none,
+                                               (lds_ptr_t)(stage + (T::A_SLOTS * wave + x) * 1024), 16, a_voff[x],
+                                               k * 128, 0, 0);
+    else if (x < T::A_SLOTS + T::B_SLOTS)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          in ? b_rsrc : none, (lds_ptr_t)(stage + T::A_BYTES + (T::B_SLOTS * wave + x - T::A_SLOTS) * 1024), 16,
+          b_voff, k * 16384 + (x - T::A_SLOTS) * 1024, 0, 0);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? s_rsrc : none, (lds_ptr_t)(stage + s_dst), 4, s_voff, k * s_step, 0,
+                                               0);
+  };
+
+  // a fragment's two halves in a stage
+  const int a_at0 = (wm * T::WM + lr) * 128 + ((g ^ (lr >> 1)) << 4), a_at1 = a_at0 ^ 64;
+  const int b_at = T::A_BYTES + (GU ? wn * (TN / 2) : wn * TN) * 2048 + lane * 16;
+  const int sa_at = T::SA + wm * T::WM * 4 + lr * TM * 4;
+  const int sw_at = T::SW + ((GU ? 0 : wn / 2) ^ ((T::BM / 64) & 1)) * T::SW_BYTES;
+  const int sw2_at = T::SW + (1 ^ ((T::BM / 64) & 1)) * T::SW_BYTES;
+
+  v4f acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
+  auto body = [&](char* __restrict__ r0, char* __restrict__ r1, char* __restrict__ r2) {
+    v8i_t av[2], bv[TN];
+    v4f part[4];
+    float sv[TM][GU ? 2 : 1], last[GU ? 2 : 1];  // this step's scales; those of the row before the step's first
+    auto read_a = [&](const char* stage, int i) {
+      const v4i lo = *reinterpret_cast<const v4i*>(stage + a_at0 + i * 2048);
+      const v4i hi = *reinterpret_cast<const v4i*>(stage + a_at1 + i * 2048);
+      return join_halves(lo, hi);
+    };
+    auto read_b = [&](const char* stage, int j) {
+      const char* at = stage + b_at + (GU && j >= TN / 2 ? 16384 + (j - TN / 2) * 2048 : j * 2048);
+      return join_halves(*reinterpret_cast<const v4i*>(at), *reinterpret_cast<const v4i*>(at + 1024));
+    };
+    float sa[TM], sw[2];
+    auto read_scales = [&](const char* stage) {
+#pragma unroll
+      for (int i = 0; i < TM; i += 4) {
+        const v4f v = *reinterpret_cast<const v4f*>(stage + sa_at + i * 4);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sa[i + t] = v[t];
+      }
+      sw[0] = *reinterpret_cast<const float*>(stage + sw_at);
+      if constexpr (GU) sw[1] = *reinterpret_cast<const float*>(stage + sw2_at);
+    };
+    auto take_scales = [&]() {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        sv[i][0] = sa[i] * sw[0];
+        if constexpr (GU) sv[i][1] = sa[i] * sw[1];
+      }
+    };
+    auto add = [&](v4f& c, const v4f& v, float s) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) c[t] = __builtin_fmaf(v[t], s, c[t]);
+    };
+    // `prev` takes the stage before kt + NST (its DMA began in the step before)
+    auto step = [&](char* cur, char* next, char* prev, int kt) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        if (i == TM - 1) {
+          // the next stage has landed (behind it NST - 2 more), this one is read
+          wait_vmcnt<(T::NST - 2) * T::DMA>();
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+          __builtin_amdgcn_sched_barrier(0);
+          read_scales(next);
+        }
+        av[(i + 1) & 1] = i + 1 < TM ? read_a(cur, i + 1) : read_a(next, 0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          part[j] = mfma_f8(bv[j], av[i & 1], v4f{0, 0, 0, 0});
+          __builtin_amdgcn_sched_barrier(0);
+          // the MFMA two before
+          const int jj = (j + TN - 2) % TN, ii = j >= 2 ? i : i - 1;
+          const int mat = GU && jj >= TN / 2 ? 1 : 0;
+          if (ii >= 0)
+            add(acc[ii][jj], part[jj], sv[ii][mat]);
+          else
+            add(acc[TM - 1][jj], part[jj], last[mat]);
+          if (i == TM - 1) {
+            bv[j] = read_b(next, j);
+            issue(cur, kt + T::NST, j);
+          }
+          if (i * TN + j + TN < T::DMA) issue(prev, kt + T::NST - 1, i * TN + j + TN);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < (GU ? 2 : 1); ++t) last[t] = sv[TM - 1][t];
+      take_scales();
+    };
+    // stages 0 .. NST - 1; of the last the first TN instructions, the rest go
+    // out in step 0
+#pragma unroll
+    for (int x = 0; x < T::DMA; ++x) issue(r0, 0, x);
+    if constexpr (T::NST == 3)
+#pragma unroll
+      for (int x = 0; x < T::DMA; ++x) issue(r1, 1, x);
+#pragma unroll
+    for (int x = 0; x < TN; ++x) issue(T::NST == 3 ? r2 : r1, T::NST - 1, x);
+    wait_vmcnt<(T::NST - 2) * T::DMA + TN>();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    read_scales(r0);
+    av[0] = read_a(r0, 0);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) bv[j] = read_b(r0, j);
+    take_scales();
+#pragma unroll
+    for (int j = 0; j < TN; ++j) part[j] = v4f{0, 0, 0, 0};
+#pragma unroll
+    for (int t = 0; t < (GU ? 2 : 1); ++t) last[t] = 0.0f;
+    for (int kt = 0; kt < kb; kt += T::NST) {
+      if constexpr (T::NST == 3) {
+        step(r0, r1, r2, kt);
+        if (kt + 1 < kb) step(r1, r2, r0, kt + 1);
+        if (kt + 2 < kb) step(r2, r0, r1, kt + 2);
+      } else {
+        step(r0, r1, r1, kt);
+        if (kt + 1 < kb) step(r1, r0, r0, kt + 1);
+      }
+    }
+    // the last two partial sums
+    add(acc[TM - 1][TN - 2], part[TN - 2], last[GU ? 1 : 0]);
+    add(acc[TM - 1][TN - 1], part[TN - 1], last[GU ? 1 : 0]);
+  };
+  body(lds, lds + T::STAGE_BYTES, lds + (T::NST == 3 ? 2 : 0) * T::STAGE_BYTES);
+
+  // epilogue: 16 rows at a time through the wave's own LDS (16-byte chunk c of
+  // row r at c ^ (r & 7)), stored as 16-byte pieces of whole row segments
+  wait_vmcnt<0>();
+  __syncthreads();
+  constexpr int WC = GU ? T::WN / 2 : T::WN, ROW = WC * 2, CH = WC / 8;  // columns, bytes, chunks of a row
+  constexpr int PER = 64 / CH;                                           // rows per store
+  char* own = lds + wave * T::EPI;
+  const int c0 = n0 + wn * WC;
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int r0 = wm * T::WM + 16 * i;
+#pragma unroll
+    for (int j = 0; j < (GU ? TN / 2 : TN); ++j) {
+      v4f y = acc[i][j];
+      if constexpr (GU) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) y[t] = f8_swiglu(y[t], acc[i][j + TN / 2][t]);
+      }
+      if constexpr (RESID) {
+        const int col = c0 + 16 * j + 4 * g;
+        if (r0 + lr < here && col < p.n) {
+          const uint2 rv = *reinterpret_cast<const uint2*>(p.residual + (m0 + r0 + lr) * p.n + col);
+          y[0] += bf16_lo(rv.x);
+          y[1] += bf16_hi(rv.x);
+          y[2] += bf16_lo(rv.y);
+          y[3] += bf16_hi(rv.y);
+        }
+      }
+      const int chunk = 2 * j + (g >> 1);
+      *reinterpret_cast<uint2*>(own + lr * ROW + ((chunk ^ (lr & (CH - 1))) << 4) + 8 * (g & 1)) =
+          uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+    }
+#pragma unroll
+    for (int q = 0; q < 16 / PER; ++q) {
+      const int r = q * PER + lane / CH, chunk = lane % CH, col = c0 + 8 * chunk;
+      const uint4 v = *reinterpret_cast<const uint4*>(own + r * ROW + ((chunk ^ (r & (CH - 1))) << 4));
+      if (r0 + r >= here || col >= p.n) continue;
+      int64_t row = m0 + r0 + r;
+      if constexpr (LISTS) {
+        row = out_rows[r0 + r];
+        if (row < 0) continue;
+      }
+      *reinterpret_cast<uint4*>(p.out + row * p.n + col) = v;
+    }
+    asm volatile("" ::: "memory");
+  }
+#endif
+}
+
+using F8Tile256 = F8Tile<128, 64, 2, 4, 2>;  // 256 x 256
+using F8Tile128 = F8Tile<64, 64, 2, 4, 3>;   // 128 x 256
+
+template <class T, bool LISTS, bool GU, bool RESID>
+hipError_t launch_tile(const F8Args& x, hipStream_t stream) {
+  static LaunchCache cache;
+  auto* kernel = &f8_tile_kernel<T, LISTS, GU, RESID>;
+  if (hipError_t e = ensure_dynamic_lds(cache, reinterpret_cast<const void*>(kernel), T::LDS)) return e;
+  constexpr int COLS = GU ? T::BN / 2 : T::BN;
+  const int64_t tiles_m = LISTS ? f8_most_tiles(x.lists.total, x.lists.experts, T::BM) : (x.rows + T::BM - 1) / T::BM;
+  const int tiles_n = (x.n + COLS - 1) / COLS;
+  if (tiles_m * tiles_n > kMaxTiles) return hipErrorInvalidValue;
+  kernel<<<(unsigned)(tiles_m * tiles_n), T::THREADS, T::LDS, stream>>>(x, (int)tiles_m, tiles_n);
+  return hipGetLastError();
+}
+
 template <bool LISTS, bool GU, bool RESID>
 hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
+  const int64_t rows = LISTS ? x.lists.total / x.lists.experts : x.rows;
+  if (rows > 768) return launch_tile<F8Tile256, LISTS, GU, RESID>(x, stream);
+  if (rows > 64) return launch_tile<F8Tile128, LISTS, GU, RESID>(x, stream);
   return launch_stream<4, 4, 1, LISTS, GU, RESID>(x, stream);
 }
 
