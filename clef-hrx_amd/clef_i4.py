@@ -86,15 +86,16 @@ SIGNATURES = {
     "clef_f8_prepare": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _P]),
     "clef_f8_pack_weight": (ctypes.c_int, [_P, _I64, _I32, _I32, _P, _P, _P]),
     "clef_f8_retile": (ctypes.c_int, [_P, _I64, _I32, _I32, _P, _P]),
-    "clef_f8_gemm": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I32, _I32, _P, _P, _P]),
-    "clef_f8_gemm_gate_up": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _P, _P]),
+    "clef_f8_gemm": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P, _P]),
+    "clef_f8_gemm_gate_up": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P]),
     "clef_f8_project_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
-    "clef_f8_project": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _P, _I32, _P, _P, _P, _SZ, _P]),
+    "clef_f8_project": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _P, _I32, _I32, _P, _P, _P, _SZ, _P]),
     "clef_moe_group_slots_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
     "clef_moe_group_slots": (ctypes.c_int, [_P, _I64, _I32, _I32, _P, _P, _P, _SZ, _P]),
-    "clef_moe_expert_f8": (ctypes.c_int, [_P, _P, _I64, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _I32, _P, _P]),
+    "clef_moe_expert_f8": (ctypes.c_int, [_P, _P, _I64, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _I32, _I32, _P,
+                                          _P]),
     "clef_moe_expert_gate_up_f8": (ctypes.c_int, [_P, _P, _I64, _P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32,
-                                                  _I32, _P, _P]),
+                                                  _I32, _I32, _P, _P]),
     "clef_pack_cache_path": (ctypes.c_int, [_P, _P, _P, _SZ]),
     "clef_pack_cache_read": (ctypes.c_int, [_P, _P, _P, _SZ, _P, _SZ, _P]),
     "clef_pack_cache_write": (ctypes.c_int, [_P, _P, _P, _SZ, _P, _SZ]),
@@ -954,6 +955,7 @@ class F8Weight:
     rows: int
     cols: int
     matrices: int = 1
+    pow2: bool = False    # every scale is a power of two: the matrix unit may apply them
 
 
 def _f8_weight_storage(w: torch.Tensor):
@@ -965,7 +967,8 @@ def _f8_weight_storage(w: torch.Tensor):
         raise ClefError(-1, _BAD_F8)
     _on_current(w)
     scales = torch.empty((matrices, (rows + 127) // 128, (cols + 127) // 128), dtype=torch.float32, device=w.device)
-    return F8Weight(torch.empty(nbytes, dtype=torch.uint8, device=w.device), scales, rows, cols, matrices)
+    return F8Weight(torch.empty(nbytes, dtype=torch.uint8, device=w.device), scales, rows, cols, matrices,
+                    w.dtype == torch.bfloat16)  # the quantizer's scales are powers of two
 
 
 def load_f8_weight(w: torch.Tensor) -> F8Weight:
@@ -991,6 +994,7 @@ def f8_weight(codes: torch.Tensor, scales: torch.Tensor) -> F8Weight:
     _on_current(scales)
     _n.launch(_n.clef_f8_retile, codes.contiguous(), out.matrices, out.rows, out.cols, out.codes)
     out.scales.copy_(scales.float().view(out.scales.shape))
+    out.pow2 = scales.dtype == torch.float8_e8m0fnu
     return out
 
 
@@ -1003,7 +1007,8 @@ def project_f8(a: PreparedF8, w: F8Weight, residual: torch.Tensor | None = None,
     _check_residual(residual, a.rows, w.rows)
     out = _f8_out(a.storage, a.rows, w.rows, out)
     codes, scales = a.call_args()
-    _n.launch(_n.clef_f8_gemm, codes, scales, w.codes, w.scales, a.rows, w.rows, w.cols, residual, out)
+    _n.launch(_n.clef_f8_gemm, codes, scales, w.codes, w.scales, a.rows, w.rows, w.cols, int(w.pow2), residual,
+              out)
     return out
 
 
@@ -1023,7 +1028,8 @@ def project_quantized_f8(x: torch.Tensor, w: F8Weight, residual: torch.Tensor | 
     out = _f8_out(x, m, w.rows, out)
     nbytes = _n.value(_n.clef_f8_project_workspace_bytes, m, w.rows, k)
     ws = _n.empty(x, torch.uint8, nbytes) if nbytes > 0 else None
-    _n.launch(_n.clef_f8_project, address, m, k, pitch, w.codes, w.scales, w.rows, residual, out, ws, nbytes)
+    _n.launch(_n.clef_f8_project, address, m, k, pitch, w.codes, w.scales, w.rows, int(w.pow2), residual, out, ws,
+              nbytes)
     return out
 
 
@@ -1036,7 +1042,7 @@ def project_gate_up_f8(a: PreparedF8, gate: F8Weight, up: F8Weight, out: torch.T
     out = _f8_out(a.storage, a.rows, gate.rows, out)
     codes, scales = a.call_args()
     _n.launch(_n.clef_f8_gemm_gate_up, codes, scales, gate.codes, gate.scales, up.codes, up.scales, a.rows, gate.rows,
-              gate.cols, out)
+              gate.cols, int(gate.pow2 and up.pow2), out)
     return out
 
 
@@ -1082,7 +1088,7 @@ def expert_f8(a: PreparedF8, w: F8Weight, offsets: torch.Tensor, slots: torch.Te
     out = _f8_out(a.storage, total, w.rows, out)
     codes, scales = a.call_args()
     _n.launch(_n.clef_moe_expert_f8, codes, scales, a.rows, w.codes, w.scales, offsets, slots, w.matrices, total, topk,
-              int(input_routed), w.cols, w.rows, out)
+              int(input_routed), w.cols, w.rows, int(w.pow2), out)
     return out
 
 
@@ -1098,7 +1104,8 @@ def expert_gate_up_f8(a: PreparedF8, gate: F8Weight, up: F8Weight, offsets: torc
     out = _f8_out(a.storage, total, gate.rows, out)
     codes, scales = a.call_args()
     _n.launch(_n.clef_moe_expert_gate_up_f8, codes, scales, a.rows, gate.codes, gate.scales, up.codes, up.scales,
-              offsets, slots, gate.matrices, total, topk, int(input_routed), gate.cols, gate.rows, out)
+              offsets, slots, gate.matrices, total, topk, int(input_routed), gate.cols, gate.rows,
+              int(gate.pow2 and up.pow2), out)
     return out
 
 

@@ -901,7 +901,7 @@ int clef_f8_retile(const uint8_t* w, int64_t matrices, int32_t n, int32_t k, uin
 }
 
 int clef_f8_gemm(const uint8_t* a, const float* a_scales, const uint8_t* w, const float* w_scales, int64_t m,
-                 int32_t n, int32_t k, const uint16_t* residual, uint16_t* out, clef_stream_t stream) {
+                 int32_t n, int32_t k, int32_t pow2, const uint16_t* residual, uint16_t* out, clef_stream_t stream) {
   if (int rc = check_f8_gemm(m, n, k)) return rc;
   if (m == 0) return CLEF_OK;
   if (!aligned(a, 16) || !aligned(a_scales, 16) || !aligned(w, 16) || !aligned(w_scales, 16) || !aligned(out, 16) ||
@@ -909,13 +909,13 @@ int clef_f8_gemm(const uint8_t* a, const float* a_scales, const uint8_t* w, cons
     return fail(kAlign);
   clef::F8Args x{};
   x.a = a, x.as = a_scales, x.rows = m, x.w = w, x.ws = w_scales, x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
-  x.residual = residual, x.out = out;
+  x.pow2 = pow2 != 0, x.residual = residual, x.out = out;
   return hip_status(clef::launch_f8_gemm(x, false, hs(stream)));
 }
 
 int clef_f8_gemm_gate_up(const uint8_t* a, const float* a_scales, const uint8_t* gate, const float* gate_scales,
-                         const uint8_t* up, const float* up_scales, int64_t m, int32_t n, int32_t k, uint16_t* h,
-                         clef_stream_t stream) {
+                         const uint8_t* up, const float* up_scales, int64_t m, int32_t n, int32_t k, int32_t pow2,
+                         uint16_t* h, clef_stream_t stream) {
   if (int rc = check_f8_gemm(m, n, k)) return rc;
   if (m == 0) return CLEF_OK;
   if (!aligned(a, 16) || !aligned(a_scales, 16) || !aligned(gate, 16) || !aligned(gate_scales, 16) ||
@@ -923,7 +923,7 @@ int clef_f8_gemm_gate_up(const uint8_t* a, const float* a_scales, const uint8_t*
     return fail(kAlign);
   clef::F8Args x{};
   x.a = a, x.as = a_scales, x.rows = m, x.w = gate, x.ws = gate_scales, x.w2 = up, x.ws2 = up_scales;
-  x.n = n, x.kb = clef::f8_blocks(k), x.k = k, x.out = h;
+  x.n = n, x.kb = clef::f8_blocks(k), x.k = k, x.pow2 = pow2 != 0, x.out = h;
   return hip_status(clef::launch_f8_gemm(x, true, hs(stream)));
 }
 
@@ -933,8 +933,8 @@ size_t clef_f8_project_workspace_bytes(int64_t m, int32_t n, int32_t k) {
 }
 
 int clef_f8_project(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint8_t* w, const float* w_scales,
-                    int32_t n, const uint16_t* residual, uint16_t* out, void* workspace, size_t workspace_bytes,
-                    clef_stream_t stream) {
+                    int32_t n, int32_t pow2, const uint16_t* residual, uint16_t* out, void* workspace,
+                    size_t workspace_bytes, clef_stream_t stream) {
   if (int rc = check_f8_gemm(m, n, k)) return rc;
   if (!(x_stride >= k && x_stride % 8 == 0)) return fail(kF8Shape);
   if (m == 0) return CLEF_OK;
@@ -944,15 +944,15 @@ int clef_f8_project(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, c
   if (clef::f8_project_fusable(m, n, k)) {
     clef::F8Args y{};
     y.x = x, y.x_stride = x_stride, y.k = k, y.rows = m, y.w = w, y.ws = w_scales, y.n = n;
-    y.kb = clef::f8_blocks(k), y.residual = residual, y.out = out;
+    y.kb = clef::f8_blocks(k), y.pow2 = pow2 != 0, y.residual = residual, y.out = out;
     return hip_status(clef::launch_f8_gemm(y, false, hs(stream)));
   }
   if (!aligned(workspace, 16)) return fail(kAlign);
   if (workspace_bytes < clef_f8_project_workspace_bytes(m, n, k)) return fail(kWorkspace);
   uint8_t* a = static_cast<uint8_t*>(workspace);
   if (int rc = clef_f8_prepare(x, m, k, x_stride, a, stream)) return rc;
-  return clef_f8_gemm(a, reinterpret_cast<const float*>(a + m * clef::f8_pitch(k)), w, w_scales, m, n, k, residual, out,
-                      stream);
+  return clef_f8_gemm(a, reinterpret_cast<const float*>(a + m * clef::f8_pitch(k)), w, w_scales, m, n, k, pow2, residual,
+                      out, stream);
 }
 
 size_t clef_moe_group_slots_workspace_bytes(int64_t tokens, int32_t topk, int32_t experts) {
@@ -974,21 +974,21 @@ int clef_moe_group_slots(const float* routes, int64_t tokens, int32_t topk, int3
 
 int clef_moe_expert_f8(const uint8_t* a, const float* a_scales, int64_t a_rows, const uint8_t* w, const float* w_scales,
                        const int32_t* offsets, const int32_t* slots, int32_t experts, int64_t total, int32_t topk,
-                       int32_t input_routed, int32_t k, int32_t n, uint16_t* out, clef_stream_t stream) {
+                       int32_t input_routed, int32_t k, int32_t n, int32_t pow2, uint16_t* out, clef_stream_t stream) {
   if (int rc = check_f8_lists(a_rows, offsets, slots, experts, total, topk, input_routed, k, n)) return rc;
   if (total == 0) return CLEF_OK;
   if (!aligned(a, 16) || !aligned(a_scales, 16) || !aligned(w, 16) || !aligned(w_scales, 16) || !aligned(out, 16))
     return fail(kAlign);
   clef::F8Args x{};
   x.a = a, x.as = a_scales, x.rows = a_rows, x.w = w, x.ws = w_scales, x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
-  x.out = out, x.lists = {offsets, slots, experts, (int)total, input_routed ? 1 : topk};
+  x.pow2 = pow2 != 0, x.out = out, x.lists = {offsets, slots, experts, (int)total, input_routed ? 1 : topk};
   return hip_status(clef::launch_f8_experts(x, false, hs(stream)));
 }
 
 int clef_moe_expert_gate_up_f8(const uint8_t* a, const float* a_scales, int64_t a_rows, const uint8_t* gate,
                                const float* gate_scales, const uint8_t* up, const float* up_scales,
                                const int32_t* offsets, const int32_t* slots, int32_t experts, int64_t total,
-                               int32_t topk, int32_t input_routed, int32_t k, int32_t n, uint16_t* h,
+                               int32_t topk, int32_t input_routed, int32_t k, int32_t n, int32_t pow2, uint16_t* h,
                                clef_stream_t stream) {
   if (int rc = check_f8_lists(a_rows, offsets, slots, experts, total, topk, input_routed, k, n)) return rc;
   if (total == 0) return CLEF_OK;
@@ -998,7 +998,7 @@ int clef_moe_expert_gate_up_f8(const uint8_t* a, const float* a_scales, int64_t 
   clef::F8Args x{};
   x.a = a, x.as = a_scales, x.rows = a_rows, x.w = gate, x.ws = gate_scales, x.w2 = up, x.ws2 = up_scales;
   x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
-  x.out = h, x.lists = {offsets, slots, experts, (int)total, input_routed ? 1 : topk};
+  x.pow2 = pow2 != 0, x.out = h, x.lists = {offsets, slots, experts, (int)total, input_routed ? 1 : topk};
   return hip_status(clef::launch_f8_experts(x, true, hs(stream)));
 }
 

@@ -57,6 +57,7 @@ struct F8Args {
   const uint8_t* w2;
   const float* ws2;
   int n, kb;  // output columns, blocks of 128 along k
+  bool pow2;  // every scale of a and w is a power of two
   const uint16_t* residual;
   uint16_t* out;
   F8Lists lists;
@@ -92,6 +93,12 @@ typedef int v8i_t __attribute__((ext_vector_type(8)));
 // scales 127 (e8m0) = 1.
 __device__ __forceinline__ v4f mfma_f8(v8i_t w, v8i_t a, v4f c) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 0, 127, 0, 127);
+}
+
+// The same with the scales in the MFMA: e8m0 exponents in the top bytes of sw
+// (of w's rows) and sa (of a's rows; lane l's row l % 16).
+__device__ __forceinline__ v4f mfma_f8_scaled(v8i_t w, v8i_t a, v4f c, int sw, int sa) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 3, sw, 3, sa);
 }
 
 __device__ __forceinline__ v8i_t join_halves(v4i lo, v4i hi) {
@@ -132,44 +139,81 @@ __device__ __forceinline__ uint32_t f8_amax2(uint32_t m, uint32_t pair) {
   return m > c ? m : c;
 }
 
-// Tile `tile` of the experts' lists cut into tiles of BM slots, experts
-// ascending: its expert, first place and slots; false when there are fewer
-// tiles. Offsets outside 0 .. total or descending are clamped, so every place
-// is a slot. Each wave finds it by itself (a scan over 64 experts at a time).
-template <int BM>
-__device__ __forceinline__ bool f8_find_tile(const F8Lists& l, int tile, int& expert, int& first, int& count) {
-  const int lane = threadIdx.x & 63;
-  int before = 0;
-  for (int c = 0; c < l.experts; c += 64) {
-    const int e = c + lane;
-    int lo = 0, hi = 0;
-    if (e < l.experts) {
-      lo = l.offsets[e];
-      hi = l.offsets[e + 1];
-    }
-    lo = lo < 0 ? 0 : lo > l.total ? l.total : lo;
-    hi = hi < lo ? lo : hi > l.total ? l.total : hi;
-    const int n = (hi - lo + BM - 1) / BM;
-    int incl = n;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(incl, off, 64);
-      if (lane >= off) incl += o;
-    }
-    const unsigned long long mask = __ballot(before + incl > tile);
-    if (mask != 0ull) {
-      const int at = __builtin_ctzll(mask);
-      expert = c + at;
-      const int begin = __builtin_amdgcn_readlane(lo, at), end = __builtin_amdgcn_readlane(hi, at);
-      const int tiles = __builtin_amdgcn_readlane(n, at), upto = __builtin_amdgcn_readlane(incl, at);
-      first = begin + (tile - before - (upto - tiles)) * BM;
-      count = end - first < BM ? end - first : BM;
-      return true;
-    }
-    before += __builtin_amdgcn_readlane(incl, 63);
-  }
-  return false;
+// Inclusive sum over the wave's lanes (DPP: shifts within the rows of 16, then
+// the rows' last lanes handed on).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true);
+  return v;
 }
+
+// The experts' lists cut into tiles of BM slots, experts ascending. find(tile)
+// gives a tile's expert, first place and slots; `total` is the number of
+// tiles. Offsets outside 0 .. total or descending are clamped, so every place is a
+// slot. Each wave looks by itself, 64 experts at a time; the first 128 stay in
+// registers between the count and the search.
+template <int BM>
+struct F8Tiles {
+  const F8Lists& l;
+  int lo[2], hi[2], incl[2], total;
+
+  __device__ __forceinline__ explicit F8Tiles(const F8Lists& lists) : l(lists), total(0) {
+    load(0, lo[0], hi[0]);
+    load(64, lo[1], hi[1]);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      incl[c] = wave_scan((hi[c] - lo[c] + BM - 1) / BM) + total;
+      total = __builtin_amdgcn_readlane(incl[c], 63);
+    }
+    for (int c = 128; c < l.experts; c += 64) {
+      int x, y;
+      load(c, x, y);
+      total += __builtin_amdgcn_readlane(wave_scan((y - x + BM - 1) / BM), 63);
+    }
+  }
+
+  __device__ __forceinline__ void load(int c, int& x, int& y) const {
+    const int e = c + (int)(threadIdx.x & 63);
+    x = y = 0;
+    if (e < l.experts) {
+      x = l.offsets[e];
+      y = l.offsets[e + 1];
+    }
+    x = x < 0 ? 0 : x > l.total ? l.total : x;
+    y = y < x ? x : y > l.total ? l.total : y;
+  }
+
+  __device__ __forceinline__ bool at(int c, int tile, int x, int y, int upto, int& expert, int& first,
+                                     int& count) const {
+    const unsigned long long mask = __ballot(upto > tile);
+    if (mask == 0ull) return false;
+    const int lane = __builtin_ctzll(mask);
+    const int begin = __builtin_amdgcn_readlane(x, lane), end = __builtin_amdgcn_readlane(y, lane);
+    const int before = __builtin_amdgcn_readlane(upto, lane) - (end - begin + BM - 1) / BM;
+    expert = c + lane;
+    first = begin + (tile - before) * BM;
+    count = end - first < BM ? end - first : BM;
+    return true;
+  }
+
+  // tile < total
+  __device__ __forceinline__ void find(int tile, int& expert, int& first, int& count) const {
+    if (at(0, tile, lo[0], hi[0], incl[0], expert, first, count)) return;
+    if (at(64, tile, lo[1], hi[1], incl[1], expert, first, count)) return;
+    int before = __builtin_amdgcn_readlane(incl[1], 63);
+    for (int c = 128; c < l.experts; c += 64) {
+      int x, y;
+      load(c, x, y);
+      const int upto = wave_scan((y - x + BM - 1) / BM) + before;
+      if (at(c, tile, x, y, upto, expert, first, count)) return;
+      before = __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+};
 
 // The most tiles of bm slots that lists over `total` slots can have.
 inline int64_t f8_most_tiles(int64_t total, int experts, int bm) {

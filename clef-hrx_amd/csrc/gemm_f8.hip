@@ -34,7 +34,9 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
   int expert = 0, first = 0, here = 0;
   int64_t m0 = 0;
   if constexpr (LISTS) {
-    if (!f8_find_tile<BM>(p.lists, blockIdx.y, expert, first, here)) return;
+    const F8Tiles<BM> tiles(p.lists);
+    if ((int)blockIdx.y >= tiles.total) return;
+    tiles.find(blockIdx.y, expert, first, here);
   } else {
     m0 = (int64_t)blockIdx.y * BM;
     here = p.rows - m0 < BM ? (int)(p.rows - m0) : BM;
@@ -102,7 +104,8 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
       b.sa[i] = as_float(__builtin_amdgcn_raw_buffer_load_b32(sr, s_voff[i], (int)(k * p.rows * 4), 0));
     }
 #pragma unroll
-    for (int m = 0; m < MATS; ++m) b.sw[m] = in ? wsp[m][k] : 0.0f;
+    for (int m = 0; m < MATS; ++m)
+      b.sw[m] = as_float(__builtin_amdgcn_raw_buffer_load_b32(make_rsrc(wsp[m], in ? (uint32_t)kb * 4u : 0u), 0, k * 4, 0));
   };
   v4f acc[MT][NT];
 #pragma unroll
@@ -126,7 +129,11 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
           for (int t = 0; t < 4; ++t) acc[i][j][t] = __builtin_fmaf(part[t], s, acc[i][j][t]);
         }
       }
+      // the order as written: loads drawn up to here would need registers of
+      // their own for every block in flight
+      __builtin_amdgcn_sched_barrier(0);
       load(buf[d], k0 + NW * (D + d));
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   // the waves' sums: fragment (i, j) of wave w at ((w MT + i) NT + j) KiB
@@ -192,8 +199,9 @@ hipError_t launch_stream(const F8Args& x, hipStream_t stream) {
 // chunk c of row r at c ^ ((r >> 1) & 7)), B fragments in the operand order, the
 // rows' scales (per 16 WM / 16-value groups, in the order the lanes read them)
 // and the two weight panels' scales.
-template <int WM_, int WN_, int WAVES_M_, int WAVES_N_, int NST_>
+template <int WM_, int WN_, int WAVES_M_, int WAVES_N_, int NST_, int GROUPS_ = 1>
 struct F8Tile {
+  static constexpr int GROUPS = GROUPS_;  // workgroups per CU
   static constexpr int WM = WM_, WN = WN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, NST = NST_;
   static constexpr int NW = WAVES_M * WAVES_N, THREADS = 64 * NW;
   static constexpr int BM = WM * WAVES_M, BN = WN * WAVES_N;
@@ -202,28 +210,38 @@ struct F8Tile {
   static constexpr int SA = A_BYTES + B_BYTES, SW = SA + SA_BYTES;
   static constexpr int STAGE_BYTES = SW + SW_BYTES * (NW - BM / 64);
   static constexpr int A_SLOTS = A_BYTES / 1024 / NW, B_SLOTS = B_BYTES / 1024 / NW;
-  static constexpr int DMA = A_SLOTS + B_SLOTS + 1;  // instructions per wave and stage
+  // a wave's DMA instructions per stage: first (X) the weight fragments, the
+  // rows of its first TM / 2 activation fragments and the scales, then (Y) the
+  // other rows
+  static constexpr int Y = A_SLOTS / 2, X = B_SLOTS + A_SLOTS - Y + 1, DMA = X + Y;
   static constexpr int ROWS = NST * STAGE_BYTES;     // lists: the tile's output rows
   static constexpr int LDS = ROWS + BM * 4;
   static constexpr int EPI = 16 * WN * 2;            // epilogue staging per wave
-  static_assert(NW == 8 && BN == 256 && BM / 64 < NW, "eight waves, two weight panels");
-  static_assert(A_BYTES % (1024 * NW) == 0 && LDS <= 160 * 1024 && TM >= 4 && TN == 4, "whole instructions per wave");
+  static_assert(NW == 8 && (BN == 256 || BN == 128) && BM / 64 + 2 <= NW, "eight waves, one or two weight panels");
+  static_assert(A_BYTES % (2048 * NW) == 0 && B_BYTES % (2048 * NW) == 0 && LDS <= 160 * 1024, "whole instructions per wave");
+  static_assert(TM * TN % 4 == 0 && TM % 4 == 0 && TN % 2 == 0 && NST >= 2 && NST <= 4, "step");
+  static_assert(X <= TM / 2 * TN && Y <= TN, "one DMA instruction per MFMA behind each barrier");
 };
 
-// Many rows: tiles of BM rows x 256 weight rows through a ring of LDS stages
+// Many rows: tiles of BM rows x BN weight rows through a ring of LDS stages
 // filled by DMA.
 //
 // A wave's step (one block of k) is TM rows of fragments times TN weight
-// fragments. It holds the weight fragments of the step, reads an activation
-// fragment one row of MFMAs ahead of its use, and adds a partial sum to its
-// accumulator by four fmas two MFMAs after the MFMA that made it, so the
-// scaling (4 VALU operations per MFMA, half its issue time) runs under the
-// MFMAs. Before the last row of MFMAs one barrier: the next stage has landed for
-// every wave, this one is read by every wave; under that row the first operands
-// of the next step are read, and under it and the next step's first rows the
-// DMA of step kt + NST goes into this stage, one instruction per MFMA.
-template <class T, bool LISTS, bool GU, bool RESID>
-__global__ __launch_bounds__(T::THREADS) void f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
+// fragments. It holds the weight fragments of the step and reads an activation
+// fragment one row of MFMAs ahead of its use. Scales that are powers of two
+// (HW) go into the MFMA, which adds to the accumulator itself; other scales are
+// applied by four fmas to a partial sum two MFMAs after the MFMA that made it
+// (half the MFMAs' issue time, run under them).
+//
+// A stage of LDS is filled in two parts: X (weights, scales, the first half of
+// each wave's activation rows) and Y (the other half). Behind a barrier in the
+// middle of a step X has been read by every wave and is loaded for NST steps
+// on, behind one before the step's last row of MFMAs the same goes for Y; each
+// barrier also waits for the part that the MFMAs behind it read. So every load
+// has NST - 1/2 steps to land, where loading a stage as a whole behind one
+// barrier left NST - 1, with one DMA instruction per MFMA.
+template <class T, bool HW, bool LISTS, bool GU, bool RESID>
+__global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __align__(16) char lds[];
   constexpr int TM = T::TM, TN = T::TN, COLS = GU ? T::BN / 2 : T::BN;
@@ -235,12 +253,15 @@ __global__ __launch_bounds__(T::THREADS) void f8_tile_kernel(const F8Args p, int
   int64_t m0 = 0;
   if constexpr (LISTS) {
     // consecutive blocks of an XCD take the columns of one tile of rows, then the
-    // expert's next rows: both operands stay in its L2
-    const int blocks = tiles_m * tiles_n, per = blocks / 8, b = blockIdx.x;
+    // expert's next rows: both operands stay in its L2. The grid has blocks for
+    // the most tiles that such lists can have; those there are shared evenly.
+    const F8Tiles<T::BM> tiles(p.lists);
+    const int blocks = tiles.total * tiles_n, per = blocks / 8, b = blockIdx.x;
+    if (b >= blocks) return;
     const int r = b < 8 * per ? (b % 8) * per + b / 8 : b;
     tm = r / tiles_n;
     tn = r - tm * tiles_n;
-    if (!f8_find_tile<T::BM>(p.lists, tm, expert, first, here)) return;
+    tiles.find(tm, expert, first, here);
   } else {
     tile_of_block(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
     m0 = (int64_t)tm * T::BM;
@@ -249,8 +270,15 @@ __global__ __launch_bounds__(T::THREADS) void f8_tile_kernel(const F8Args p, int
   const int n0 = tn * COLS;
   int* out_rows = reinterpret_cast<int*>(lds + T::ROWS);
 
-  // this wave's DMA: A instruction q = A_SLOTS wave + s moves rows 8 q .. + 7
+  // this wave's DMA: A instruction s moves 8 rows, the first half of a wave's
+  // instructions rows of the first TM / 2 fragments of either row of waves
   int a_voff[T::A_SLOTS], s_voff;
+  auto a_piece = [&](int s) {  // KiB of the stage
+    constexpr int H = T::A_SLOTS / 2;
+    constexpr int PER = T::WM / 16;  // KiB of half of a row of waves' rows
+    const int hi = s >= H, q = wave * H + s % H;
+    return q / PER * (2 * PER) + hi * PER + q % PER;
+  };
   auto source_row = [&](int r) -> int64_t {  // row of a (dense: from m0); rows past the end repeat the last
     r = r < here ? r : here - 1;
     if constexpr (!LISTS) return r;
@@ -260,21 +288,22 @@ __global__ __launch_bounds__(T::THREADS) void f8_tile_kernel(const F8Args p, int
   };
 #pragma unroll
   for (int s = 0; s < T::A_SLOTS; ++s) {
-    const int r = 8 * (T::A_SLOTS * wave + s) + (lane >> 3);
+    const int r = 8 * a_piece(s) + (lane >> 3);
     a_voff[s] = (int)((uint32_t)source_row(r) * (uint32_t)pitch) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
   }
   const __amdgpu_buffer_rsrc_t a_rsrc =
       make_rsrc(p.a + (LISTS ? 0 : m0 * pitch), (uint32_t)(LISTS ? p.rows * pitch : (int64_t)here * pitch));
-  // B: waves 0-3 the first panel, 4-7 the second (gate/up: the up panel); a
-  // panel past the last column is empty
-  const int panel_of = wave / 4, nb = f8_blocks(p.n);
-  const int panel = n0 / 128 + (GU ? 0 : panel_of);
-  const uint8_t* wbase = GU && panel_of ? p.w2 : p.w;
-  const float* sbase = GU ? p.ws : p.ws;
+  // B: this wave's weight fragments, consecutive ones of one panel (gate/up: the
+  // first half of the waves the gate's, the second the up's); a panel past the
+  // last column is empty
+  constexpr int FRAGS = T::B_SLOTS / 2;
+  const int nb = f8_blocks(p.n);
+  const bool up = GU && wave >= T::NW / 2;
+  const int frag = n0 / 16 + (up ? wave - T::NW / 2 : wave) * FRAGS, panel = frag / 8;
   const int64_t first_block = (int64_t)expert * nb * kb;
-  const __amdgpu_buffer_rsrc_t b_rsrc =
-      make_rsrc(wbase + (first_block + (int64_t)panel * kb) * 16384, panel < nb ? (uint32_t)kb * 16384u : 0u);
-  const int b_voff = (wave & 3) * (T::B_SLOTS * 1024) + lane * 16;
+  const __amdgpu_buffer_rsrc_t b_rsrc = make_rsrc((up ? p.w2 : p.w) + (first_block + (int64_t)panel * kb) * 16384,
+                                                  panel < nb ? (uint32_t)kb * 16384u : 0u);
+  const int b_voff = frag % 8 * 2048 + lane * 16;
   // scales: the first BM / 64 waves the rows', the others the panels' (lane 0
   // the first, lane 1 the second)
   const bool row_scales = wave < T::BM / 64;
@@ -290,7 +319,7 @@ __global__ __launch_bounds__(T::THREADS) void f8_tile_kernel(const F8Args p, int
   } else {
     const int q = n0 / 128 + (wave & 1);
     s_voff = 0;
-    s_rsrc = make_rsrc(sbase + first_block + (int64_t)q * kb, q < nb ? (uint32_t)kb * 4u : 0u);
+    s_rsrc = make_rsrc(p.ws + first_block + (int64_t)q * kb, q < nb ? (uint32_t)kb * 4u : 0u);
   }
   const int s_dst = row_scales ? T::SA + wave * 256 : T::SW + (wave - T::BM / 64) * T::SW_BYTES;
   const int s_step = row_scales ? (int)(p.rows * 4) : 4;
@@ -305,29 +334,31 @@ __global__ __launch_bounds__(T::THREADS) void f8_tile_kernel(const F8Args p, int
     }
   }
   const __amdgpu_buffer_rsrc_t none = make_rsrc(p.a, 0);
-  // DMA instruction x of stage kt into `stage` (stages past the end: zeros
-  // that nothing reads, so that every step issues and waits alike)
+  // DMA instruction x of stage kt into `stage`, X first (stages past the end:
+  // zeros that nothing reads, so that every step issues and waits alike)
   auto issue = [&](char* stage, int kt, int x) {
     const bool in = kt < kb;
     const int k = in ? kt : 0;
-    if (x < T::A_SLOTS)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? a_rsrc : none,
-                                               (lds_ptr_t)(stage + (T::A_SLOTS * wave + x) * 1024), 16, a_voff[x],
-                                               k * 128, 0, 0);
-    else if (x < T::A_SLOTS + T::B_SLOTS)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          in ? b_rsrc : none, (lds_ptr_t)(stage + T::A_BYTES + (T::B_SLOTS * wave + x - T::A_SLOTS) * 1024), 16,
-          b_voff, k * 16384 + (x - T::A_SLOTS) * 1024, 0, 0);
-    else
+    constexpr int H = T::A_SLOTS / 2;
+    if (x < T::B_SLOTS) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? b_rsrc : none,
+                                               (lds_ptr_t)(stage + T::A_BYTES + (T::B_SLOTS * wave + x) * 1024), 16,
+                                               b_voff, k * 16384 + x * 1024, 0, 0);
+    } else if (x == T::B_SLOTS + H) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? s_rsrc : none, (lds_ptr_t)(stage + s_dst), 4, s_voff, k * s_step, 0,
                                                0);
+    } else {
+      const int q = x < T::B_SLOTS + H ? x - T::B_SLOTS : x - T::B_SLOTS - 1;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? a_rsrc : none, (lds_ptr_t)(stage + a_piece(q) * 1024), 16, a_voff[q],
+                                               k * 128, 0, 0);
+    }
   };
 
   // a fragment's two halves in a stage
   const int a_at0 = (wm * T::WM + lr) * 128 + ((g ^ (lr >> 1)) << 4), a_at1 = a_at0 ^ 64;
   const int b_at = T::A_BYTES + (GU ? wn * (TN / 2) : wn * TN) * 2048 + lane * 16;
   const int sa_at = T::SA + wm * T::WM * 4 + lr * TM * 4;
-  const int sw_at = T::SW + ((GU ? 0 : wn / 2) ^ ((T::BM / 64) & 1)) * T::SW_BYTES;
+  const int sw_at = T::SW + ((GU ? 0 : wn * T::WN / 128) ^ ((T::BM / 64) & 1)) * T::SW_BYTES;
   const int sw2_at = T::SW + (1 ^ ((T::BM / 64) & 1)) * T::SW_BYTES;
 
   v4f acc[TM][TN];
@@ -335,20 +366,22 @@ __global__ __launch_bounds__(T::THREADS) void f8_tile_kernel(const F8Args p, int
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
-  auto body = [&](char* __restrict__ r0, char* __restrict__ r1, char* __restrict__ r2) {
+  auto body = [&](char* __restrict__ r0, char* __restrict__ r1, char* __restrict__ r2, char* __restrict__ r3) {
+    constexpr int MATS = GU ? 2 : 1;
     v8i_t av[2], bv[TN];
-    v4f part[4];
-    float sv[TM][GU ? 2 : 1], last[GU ? 2 : 1];  // this step's scales; those of the row before the step's first
+    v4f part[4];               // !HW: partial sums on their way
+    float sv[TM][MATS], last[MATS];  // !HW: this step's scales; those of the row before the step's first
+    int sa_bits[TM], sw_bits[MATS];  // HW: the scales' bits, exponent in the top byte
     auto read_a = [&](const char* stage, int i) {
       const v4i lo = *reinterpret_cast<const v4i*>(stage + a_at0 + i * 2048);
       const v4i hi = *reinterpret_cast<const v4i*>(stage + a_at1 + i * 2048);
       return join_halves(lo, hi);
     };
     auto read_b = [&](const char* stage, int j) {
-      const char* at = stage + b_at + (GU && j >= TN / 2 ? 16384 + (j - TN / 2) * 2048 : j * 2048);
+      const char* at = stage + b_at + (GU && j >= TN / 2 ? T::B_BYTES / 2 + (j - TN / 2) * 2048 : j * 2048);
       return join_halves(*reinterpret_cast<const v4i*>(at), *reinterpret_cast<const v4i*>(at + 1024));
     };
-    float sa[TM], sw[2];
+    float sa[TM], sw[MATS];
     auto read_scales = [&](const char* stage) {
 #pragma unroll
       for (int i = 0; i < TM; i += 4) {
@@ -360,62 +393,76 @@ __global__ __launch_bounds__(T::THREADS) void f8_tile_kernel(const F8Args p, int
       if constexpr (GU) sw[1] = *reinterpret_cast<const float*>(stage + sw2_at);
     };
     auto take_scales = [&]() {
+      if constexpr (HW) {
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        sv[i][0] = sa[i] * sw[0];
-        if constexpr (GU) sv[i][1] = sa[i] * sw[1];
+        for (int i = 0; i < TM; ++i) sa_bits[i] = (int)(as_uint(sa[i]) << 1);
+#pragma unroll
+        for (int t = 0; t < MATS; ++t) sw_bits[t] = (int)(as_uint(sw[t]) << 1);
+      } else {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int t = 0; t < MATS; ++t) sv[i][t] = sa[i] * sw[t];
       }
     };
     auto add = [&](v4f& c, const v4f& v, float s) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) c[t] = __builtin_fmaf(v[t], s, c[t]);
     };
-    // `prev` takes the stage before kt + NST (its DMA began in the step before)
-    auto step = [&](char* cur, char* next, char* prev, int kt) {
+    // at most (NST - 1) stages' DMA behind what is waited for
+    auto landed = [&]() {
+      wait_vmcnt<(T::NST - 1) * T::DMA>();
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto step = [&](char* cur, const char* next, int kt) {
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
+        if (i == TM / 2 - 1) landed();  // this stage's Y; its X has been read
         if (i == TM - 1) {
-          // the next stage has landed (behind it NST - 2 more), this one is read
-          wait_vmcnt<(T::NST - 2) * T::DMA>();
-          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-          __builtin_amdgcn_sched_barrier(0);
+          landed();  // the next stage's X; this stage has been read
           read_scales(next);
         }
         av[(i + 1) & 1] = i + 1 < TM ? read_a(cur, i + 1) : read_a(next, 0);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-          part[j] = mfma_f8(bv[j], av[i & 1], v4f{0, 0, 0, 0});
-          __builtin_amdgcn_sched_barrier(0);
-          // the MFMA two before
-          const int jj = (j + TN - 2) % TN, ii = j >= 2 ? i : i - 1;
-          const int mat = GU && jj >= TN / 2 ? 1 : 0;
-          if (ii >= 0)
-            add(acc[ii][jj], part[jj], sv[ii][mat]);
-          else
-            add(acc[TM - 1][jj], part[jj], last[mat]);
-          if (i == TM - 1) {
-            bv[j] = read_b(next, j);
-            issue(cur, kt + T::NST, j);
+          if constexpr (HW) {
+            acc[i][j] = mfma_f8_scaled(bv[j], av[i & 1], acc[i][j], sw_bits[GU && j >= TN / 2 ? 1 : 0], sa_bits[i]);
+            __builtin_amdgcn_sched_barrier(0);
+          } else {
+            part[(i * TN + j) % 4] = mfma_f8(bv[j], av[i & 1], v4f{0, 0, 0, 0});
+            __builtin_amdgcn_sched_barrier(0);
+            // the MFMA two before
+            const int before = i * TN + j - 2, ii = (before + TM * TN) / TN % TM, jj = (before + TN) % TN;
+            const int mat = GU && jj >= TN / 2 ? 1 : 0;
+            add(acc[ii][jj], part[(before + 4) % 4], before >= 0 ? sv[ii][mat] : last[mat]);
           }
-          if (i * TN + j + TN < T::DMA) issue(prev, kt + T::NST - 1, i * TN + j + TN);
+          if (i == TM - 1) bv[j] = read_b(next, j);
+          // X behind the first barrier, Y behind the second
+          constexpr int SPAN = TM / 2 * TN;
+          const int u = (i - (TM / 2 - 1)) * TN + j;
+          if (u >= 0 && u < SPAN) {
+#pragma unroll
+            for (int x = u * T::X / SPAN; x < (u + 1) * T::X / SPAN; ++x) issue(cur, kt + T::NST, x);
+          } else if (i == TM - 1 && j < T::Y) {
+            issue(cur, kt + T::NST, T::X + j);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+      if constexpr (!HW) {
 #pragma unroll
-      for (int t = 0; t < (GU ? 2 : 1); ++t) last[t] = sv[TM - 1][t];
+        for (int t = 0; t < MATS; ++t) last[t] = sv[TM - 1][t];
+      }
       take_scales();
     };
-    // stages 0 .. NST - 1; of the last the first TN instructions, the rest go
-    // out in step 0
+    char* const ring[4] = {r0, r1, r2, r3};
 #pragma unroll
-    for (int x = 0; x < T::DMA; ++x) issue(r0, 0, x);
-    if constexpr (T::NST == 3)
+    for (int n = 0; n < T::NST; ++n)
 #pragma unroll
-      for (int x = 0; x < T::DMA; ++x) issue(r1, 1, x);
-#pragma unroll
-    for (int x = 0; x < TN; ++x) issue(T::NST == 3 ? r2 : r1, T::NST - 1, x);
-    wait_vmcnt<(T::NST - 2) * T::DMA + TN>();
+      for (int x = 0; x < T::DMA; ++x) issue(ring[n], n, x);
+    wait_vmcnt<T::NST * T::DMA - T::X>();
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     read_scales(r0);
@@ -423,25 +470,30 @@ __global__ __launch_bounds__(T::THREADS) void f8_tile_kernel(const F8Args p, int
 #pragma unroll
     for (int j = 0; j < TN; ++j) bv[j] = read_b(r0, j);
     take_scales();
+    if constexpr (!HW) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j) part[j] = v4f{0, 0, 0, 0};
+      for (int t = 0; t < 4; ++t) part[t] = v4f{0, 0, 0, 0};
 #pragma unroll
-    for (int t = 0; t < (GU ? 2 : 1); ++t) last[t] = 0.0f;
+      for (int t = 0; t < MATS; ++t) last[t] = 0.0f;
+    }
     for (int kt = 0; kt < kb; kt += T::NST) {
-      if constexpr (T::NST == 3) {
-        step(r0, r1, r2, kt);
-        if (kt + 1 < kb) step(r1, r2, r0, kt + 1);
-        if (kt + 2 < kb) step(r2, r0, r1, kt + 2);
+      step(r0, r1, kt);
+      if constexpr (T::NST == 2) {
+        if (kt + 1 < kb) step(r1, r0, kt + 1);
       } else {
-        step(r0, r1, r1, kt);
-        if (kt + 1 < kb) step(r1, r0, r0, kt + 1);
+        if (kt + 1 < kb) step(r1, r2, kt + 1);
+        if (kt + 2 < kb) step(r2, T::NST == 3 ? r0 : r3, kt + 2);
+        if constexpr (T::NST == 4)
+          if (kt + 3 < kb) step(r3, r0, kt + 3);
       }
     }
-    // the last two partial sums
-    add(acc[TM - 1][TN - 2], part[TN - 2], last[GU ? 1 : 0]);
-    add(acc[TM - 1][TN - 1], part[TN - 1], last[GU ? 1 : 0]);
+    if constexpr (!HW) {
+      // the last two partial sums
+      add(acc[TM - 1][TN - 2], part[2], last[GU && TN > 2 ? 1 : 0]);
+      add(acc[TM - 1][TN - 1], part[3], last[GU ? 1 : 0]);
+    }
   };
-  body(lds, lds + T::STAGE_BYTES, lds + (T::NST == 3 ? 2 : 0) * T::STAGE_BYTES);
+  body(lds, lds + T::STAGE_BYTES, lds + 2 % T::NST * T::STAGE_BYTES, lds + 3 % T::NST * T::STAGE_BYTES);
 
   // epilogue: 16 rows at a time through the wave's own LDS (16-byte chunk c of
   // row r at c ^ (r & 7)), stored as 16-byte pieces of whole row segments
@@ -476,8 +528,9 @@ __global__ __launch_bounds__(T::THREADS) void f8_tile_kernel(const F8Args p, int
           uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
     }
 #pragma unroll
-    for (int q = 0; q < 16 / PER; ++q) {
+    for (int q = 0; q < (16 + PER - 1) / PER; ++q) {
       const int r = q * PER + lane / CH, chunk = lane % CH, col = c0 + 8 * chunk;
+      if (PER > 16 && r >= 16) continue;
       const uint4 v = *reinterpret_cast<const uint4*>(own + r * ROW + ((chunk ^ (r & (CH - 1))) << 4));
       if (r0 + r >= here || col >= p.n) continue;
       int64_t row = m0 + r0 + r;
@@ -492,13 +545,13 @@ __global__ __launch_bounds__(T::THREADS) void f8_tile_kernel(const F8Args p, int
 #endif
 }
 
-using F8Tile256 = F8Tile<128, 64, 2, 4, 2>;  // 256 x 256
-using F8Tile128 = F8Tile<64, 64, 2, 4, 3>;   // 128 x 256
+using F8Tile256 = F8Tile<128, 64, 2, 4, 2>;     // 256 x 256
+using F8Tile128 = F8Tile<64, 32, 2, 4, 2, 2>;   // 128 x 128, two workgroups per CU
 
-template <class T, bool LISTS, bool GU, bool RESID>
+template <class T, bool HW, bool LISTS, bool GU, bool RESID>
 hipError_t launch_tile(const F8Args& x, hipStream_t stream) {
   static LaunchCache cache;
-  auto* kernel = &f8_tile_kernel<T, LISTS, GU, RESID>;
+  auto* kernel = &f8_tile_kernel<T, HW, LISTS, GU, RESID>;
   if (hipError_t e = ensure_dynamic_lds(cache, reinterpret_cast<const void*>(kernel), T::LDS)) return e;
   constexpr int COLS = GU ? T::BN / 2 : T::BN;
   const int64_t tiles_m = LISTS ? f8_most_tiles(x.lists.total, x.lists.experts, T::BM) : (x.rows + T::BM - 1) / T::BM;
@@ -508,12 +561,57 @@ hipError_t launch_tile(const F8Args& x, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// The kernel of a shape. From the smallest tiles up: 16 x 32, 16 x 64, 32 x 64
+// and 64 x 64 of the split-k kernel while they are at most one per CU (m x k x n
+// in us: 256 x 2048 x 512 4.1 on 16 x 32 tiles, 5.0, 6.3, 8.0 on the larger
+// ones; 384 x 512 x 2048 8.6, 6.5, 6.8 and 4.7); beyond, 128 x 128 tiles, two
+// workgroups per CU (256 x 4096 x 12288: 20 against 39 on 64 x 64), and 256 x
+// 256 tiles from three times their rounds over the CUs up, a 256 x 256 round
+// taking about three of 128 x 128 (1024 x 4096 x 12288, 1 and 3 rounds: 49
+// against 52; 1536, 2 and 5: 97 against 81; 4096, 3 and 12: 175 against 220).
+// One tile of 16 rows against more columns than 256 tiles cover stays on 16 x
+// 32 (16 x 5120 x 2 17408: 39 against 45 on 128 x 128).
 template <bool LISTS, bool GU, bool RESID>
 hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
-  const int64_t rows = LISTS ? x.lists.total / x.lists.experts : x.rows;
-  if (rows > 768) return launch_tile<F8Tile256, LISTS, GU, RESID>(x, stream);
-  if (rows > 64) return launch_tile<F8Tile128, LISTS, GU, RESID>(x, stream);
-  return launch_stream<4, 4, 1, LISTS, GU, RESID>(x, stream);
+  constexpr int64_t kCus = 256;
+  const int64_t rows_of_w = (int64_t)x.n * (GU ? 2 : 1);
+  // tiles of bm rows; experts' lists as if evenly filled (a little more, for
+  // those above the mean)
+  auto tiles = [&](int bm, int bn) {
+    int64_t down;
+    if constexpr (LISTS) {
+      const int64_t named = x.lists.total < x.lists.experts ? x.lists.total : x.lists.experts;
+      const int64_t rows = x.lists.total * 21 / 20 / named;
+      down = named * ((rows + bm - 1) / bm > 0 ? (rows + bm - 1) / bm : 1);
+    } else {
+      down = (x.rows + bm - 1) / bm;
+    }
+    return down * ((rows_of_w + bn - 1) / bn);
+  };
+  if constexpr (LISTS) {
+    // The experts' weights are read once whatever the tile: 16 x 64 tiles for a
+    // few slots (8 slots: 4.7 / 5.3 us down / gate/up against 6.1 / 10.0 on 128 x
+    // 128) and for up to 8 rows per expert over at least 16 blocks of k (60
+    // tokens of 128 experts top-8, gate/up 71 against 75; 240 tokens 91 against
+    // 79; down, 6 blocks of k, 43 against 36).
+    const int64_t rows = x.lists.total / x.lists.experts;
+    if (x.lists.total <= 16 || (rows < 8 && x.kb >= 16)) {
+      if (f8_most_tiles(x.lists.total, x.lists.experts, 16) <= 65535)
+        return launch_stream<1, 4, 2, LISTS, GU, RESID>(x, stream);
+    }
+  } else {
+    if (tiles(16, 32) <= kCus || (x.rows <= 16 && tiles(16, 64) > kCus))
+      return launch_stream<1, 2, 2, LISTS, GU, RESID>(x, stream);
+    if (tiles(16, 64) <= kCus) return launch_stream<1, 4, 2, LISTS, GU, RESID>(x, stream);
+    if (tiles(32, 64) <= kCus) return launch_stream<2, 4, 2, LISTS, GU, RESID>(x, stream);
+    if (tiles(64, 64) <= kCus) return launch_stream<4, 4, 1, LISTS, GU, RESID>(x, stream);
+  }
+  const int64_t small = (tiles(128, 128) + kCus - 1) / kCus, large = (tiles(256, 256) + kCus - 1) / kCus;
+  if (small >= 3 * large)
+    return x.pow2 ? launch_tile<F8Tile256, true, LISTS, GU, RESID>(x, stream)
+                  : launch_tile<F8Tile256, false, LISTS, GU, RESID>(x, stream);
+  return x.pow2 ? launch_tile<F8Tile128, true, LISTS, GU, RESID>(x, stream)
+                : launch_tile<F8Tile128, false, LISTS, GU, RESID>(x, stream);
 }
 
 }  // namespace

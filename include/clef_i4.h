@@ -525,21 +525,25 @@ int clef_f8_pack_weight(const uint16_t* w, int64_t matrices, int32_t n, int32_t 
  * (their scales are used as they are). 1 <= matrices <= 1024. */
 int clef_f8_retile(const uint8_t* w, int64_t matrices, int32_t n, int32_t k, uint8_t* codes, clef_stream_t stream);
 
-/* Projection of a prepared activation; residual bf16 [m][n], nullable. */
+/* Projection of a prepared activation; residual bf16 [m][n], nullable. pow2
+ * (here and below) nonzero: every scale of a and w is a power of two between
+ * 2^-126 and 2^127, as clef_f8_prepare, clef_f8_pack_weight and e8m0
+ * checkpoints make them; the matrix unit may then apply them (with other
+ * scales it would drop their mantissas). The same sums within f32 rounding. */
 int clef_f8_gemm(const uint8_t* a, const float* a_scales, const uint8_t* w, const float* w_scales, int64_t m,
-                 int32_t n, int32_t k, const uint16_t* residual, uint16_t* out, clef_stream_t stream);
+                 int32_t n, int32_t k, int32_t pow2, const uint16_t* residual, uint16_t* out, clef_stream_t stream);
 
 /* h[m][n] = silu(g) * u of the two projections' f32 sums, bf16 once. */
 int clef_f8_gemm_gate_up(const uint8_t* a, const float* a_scales, const uint8_t* gate, const float* gate_scales,
-                         const uint8_t* up, const float* up_scales, int64_t m, int32_t n, int32_t k, uint16_t* h,
-                         clef_stream_t stream);
+                         const uint8_t* up, const float* up_scales, int64_t m, int32_t n, int32_t k, int32_t pow2,
+                         uint16_t* h, clef_stream_t stream);
 
 /* clef_f8_prepare and clef_f8_gemm in one call; the workspace (bytes below, 0
  * where a few rows are quantized by the product itself) takes the activation. */
 size_t clef_f8_project_workspace_bytes(int64_t m, int32_t n, int32_t k);
 int clef_f8_project(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint8_t* w, const float* w_scales,
-                    int32_t n, const uint16_t* residual, uint16_t* out, void* workspace, size_t workspace_bytes,
-                    clef_stream_t stream);
+                    int32_t n, int32_t pow2, const uint16_t* residual, uint16_t* out, void* workspace,
+                    size_t workspace_bytes, clef_stream_t stream);
 
 /* Routes (as clef_moe_route writes them, any number of experts up to 1024)
  * listed by expert: offsets [experts + 1], slots [tokens * topk]: the route
@@ -564,13 +568,13 @@ int clef_moe_group_slots(const float* routes, int64_t tokens, int32_t topk, int3
  * 2 GiB. */
 int clef_moe_expert_f8(const uint8_t* a, const float* a_scales, int64_t a_rows, const uint8_t* w, const float* w_scales,
                        const int32_t* offsets, const int32_t* slots, int32_t experts, int64_t total, int32_t topk,
-                       int32_t input_routed, int32_t k, int32_t n, uint16_t* out, clef_stream_t stream);
+                       int32_t input_routed, int32_t k, int32_t n, int32_t pow2, uint16_t* out, clef_stream_t stream);
 
 /* h = silu(gate) * up over the same lists, as clef_f8_gemm_gate_up. */
 int clef_moe_expert_gate_up_f8(const uint8_t* a, const float* a_scales, int64_t a_rows, const uint8_t* gate,
                                const float* gate_scales, const uint8_t* up, const float* up_scales,
                                const int32_t* offsets, const int32_t* slots, int32_t experts, int64_t total,
-                               int32_t topk, int32_t input_routed, int32_t k, int32_t n, uint16_t* h,
+                               int32_t topk, int32_t input_routed, int32_t k, int32_t n, int32_t pow2, uint16_t* h,
                                clef_stream_t stream);
 
 /* ------------------------------------------------------- packed cache */

@@ -53,27 +53,27 @@ def test_weight_rejects(matrices, n, k):
 
 @pytest.mark.parametrize("m,n,k", [(-1, 128, 128), ((1 << 20) + 1, 128, 128), (4, 0, 128), (4, 100, 128), (4, 128, 12)])
 def test_products_reject(m, n, k):
-    assert call("clef_f8_gemm", FAKE, FAKE, FAKE, FAKE, m, n, k, None, FAKE, None) == (-1, SHAPE)
-    assert call("clef_f8_gemm_gate_up", FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, m, n, k, FAKE, None) == (-1, SHAPE)
-    assert call("clef_f8_project", FAKE, m, k, max(k, 16), FAKE, FAKE, n, None, FAKE, FAKE, 1 << 40, None) == (-1, SHAPE)
+    assert call("clef_f8_gemm", FAKE, FAKE, FAKE, FAKE, m, n, k, 0, None, FAKE, None) == (-1, SHAPE)
+    assert call("clef_f8_gemm_gate_up", FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, m, n, k, 0, FAKE, None) == (-1, SHAPE)
+    assert call("clef_f8_project", FAKE, m, k, max(k, 16), FAKE, FAKE, n, 0, None, FAKE, FAKE, 1 << 40, None) == (-1, SHAPE)
 
 
 def test_products_pointers_workspace_and_no_rows():
-    assert call("clef_f8_gemm", None, None, None, None, 0, 128, 128, None, None, None)[0] == 0
-    assert call("clef_f8_gemm_gate_up", *[None] * 6, 0, 128, 128, None, None)[0] == 0
-    assert call("clef_f8_project", None, 0, 128, 128, None, None, 128, None, None, None, 0, None)[0] == 0
+    assert call("clef_f8_gemm", None, None, None, None, 0, 128, 128, 1, None, None, None)[0] == 0
+    assert call("clef_f8_gemm_gate_up", *[None] * 6, 0, 128, 128, 1, None, None)[0] == 0
+    assert call("clef_f8_project", None, 0, 128, 128, None, None, 128, 1, None, None, None, 0, None)[0] == 0
     good = [FAKE] * 4
     for i in range(4):
         bad = list(good)
         bad[i] = FAKE + 4
-        rc, msg = call("clef_f8_gemm", *bad, 4, 128, 128, None, FAKE, None)
+        rc, msg = call("clef_f8_gemm", *bad, 4, 128, 128, 0, None, FAKE, None)
         assert rc == -1 and "aligned" in msg
-    rc, msg = call("clef_f8_gemm", *good, 4, 128, 128, FAKE + 2, FAKE, None)
+    rc, msg = call("clef_f8_gemm", *good, 4, 128, 128, 0, FAKE + 2, FAKE, None)
     assert rc == -1 and "aligned" in msg
     need = clef_i4.lib().clef_f8_project_workspace_bytes(4096, 256, 256)
-    rc, msg = call("clef_f8_project", FAKE, 4096, 256, 256, FAKE, FAKE, 256, None, FAKE, FAKE, need - 1, None)
+    rc, msg = call("clef_f8_project", FAKE, 4096, 256, 256, FAKE, FAKE, 256, 0, None, FAKE, FAKE, need - 1, None)
     assert rc == -1 and msg == "workspace too small"
-    rc, msg = call("clef_f8_project", FAKE, 4096, 256, 252, FAKE, FAKE, 256, None, FAKE, FAKE, need, None)
+    rc, msg = call("clef_f8_project", FAKE, 4096, 256, 252, FAKE, FAKE, 256, 0, None, FAKE, FAKE, need, None)
     assert rc == -1 and msg == SHAPE
 
 
@@ -104,19 +104,19 @@ def test_group_slots_rejects():
     (131073, 8, 8, 2, 0, 32768, 128, "expert activation operand of 4 GiB or more (split the tokens into chunks)"),
 ])
 def test_experts_reject(a_rows, experts, total, topk, routed, k, n, message):
-    rest = (FAKE, FAKE, experts, total, topk, routed, k, n, FAKE, None)
+    rest = (FAKE, FAKE, experts, total, topk, routed, k, n, 0, FAKE, None)
     assert call("clef_moe_expert_f8", FAKE, FAKE, a_rows, FAKE, FAKE, *rest) == (-1, message)
     assert call("clef_moe_expert_gate_up_f8", FAKE, FAKE, a_rows, FAKE, FAKE, FAKE, FAKE, *rest) == (-1, message)
 
 
 def test_experts_pointers_and_no_slots():
-    none = (None, None, 4, None, None, None, None, 8, 0, 2, 0, 128, 128, None, None)
+    none = (None, None, 4, None, None, None, None, 8, 0, 2, 0, 128, 128, 1, None, None)
     assert call("clef_moe_expert_f8", *none)[0] == 0
-    rc, msg = call("clef_moe_expert_f8", FAKE, FAKE, 4, FAKE, FAKE, None, FAKE, 8, 8, 2, 0, 128, 128, FAKE, None)
+    rc, msg = call("clef_moe_expert_f8", FAKE, FAKE, 4, FAKE, FAKE, None, FAKE, 8, 8, 2, 0, 128, 128, 0, FAKE, None)
     assert rc == -1 and "list pointer" in msg
-    rc, msg = call("clef_moe_expert_f8", FAKE, FAKE, 4, FAKE, FAKE, FAKE, FAKE + 2, 8, 8, 2, 0, 128, 128, FAKE, None)
+    rc, msg = call("clef_moe_expert_f8", FAKE, FAKE, 4, FAKE, FAKE, FAKE, FAKE + 2, 8, 8, 2, 0, 128, 128, 0, FAKE, None)
     assert rc == -1 and "list pointer" in msg
-    rc, msg = call("clef_moe_expert_f8", FAKE, FAKE, 4, FAKE, None, FAKE, FAKE, 8, 8, 2, 0, 128, 128, FAKE, None)
+    rc, msg = call("clef_moe_expert_f8", FAKE, FAKE, 4, FAKE, None, FAKE, FAKE, 8, 8, 2, 0, 128, 128, 0, FAKE, None)
     assert rc == -1 and "aligned" in msg
 
 

@@ -197,8 +197,11 @@ def test_weight_layout(matrices, n, k):
 # ---------------------------------------------------------------- projections
 
 SHAPES = [(1, 128, 128), (1, 4096, 1024), (3, 136, 8), (16, 1000, 264), (17, 264, 1352), (37, 4160, 1352),
-          (64, 512, 128), (65, 2048, 520), (129, 1024, 2048), (257, 768, 1288), (300, 17408, 256), (700, 384, 4104),
-          (1030, 1152, 1032)]
+          (64, 512, 128), (65, 2048, 520), (129, 1024, 2048), (257, 768, 1288), (300, 17408, 256),
+          # 128 x 128 tiles: one, two, three and nine blocks of k
+          (700, 128, 4104), (700, 256, 4104), (700, 384, 4104), (1030, 1152, 1032),
+          # 256 x 256 tiles: one, two, three and eight blocks
+          (2300, 128, 3608), (2300, 256, 3608), (2300, 392, 3608), (2060, 1000, 4104)]
 
 
 @pytest.mark.parametrize("m,k,n", SHAPES)
@@ -223,15 +226,16 @@ def test_project_matches_64_bits(m, k, n, kind, res):
 
 
 @pytest.mark.parametrize("m,k,n", SHAPES)
-def test_project_gate_up_matches_64_bits(m, k, n):
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+def test_project_gate_up_matches_64_bits(m, k, n, kind):
     x = randn((m, k), 1.0, m + k)
-    (gc, gs), (uc, us) = weight(1, n, k, "f32", n), weight(1, n, k, "e8m0", n + 2)
+    (gc, gs), (uc, us) = weight(1, n, k, kind, n), weight(1, n, k, "e8m0", n + 2)
+    gs = (gs.float() * 2.0 ** -6).to(gs.dtype)
     a = clef_i4.prepare_f8(x)
-    want, slack = swiglu64(rows64(a), weight64(gc, gs)[0] * 0.02, weight64(uc, us)[0])
-    gate, up = clef_i4.f8_weight(gc[0], gs[0] * 0.02), clef_i4.f8_weight(uc[0], us[0])
+    want, slack = swiglu64(rows64(a), weight64(gc, gs)[0], weight64(uc, us)[0])
+    gate, up = clef_i4.f8_weight(gc[0], gs[0]), clef_i4.f8_weight(uc[0], us[0])
     out = torch.full((m + 1, n), 7.0, dtype=BF, device="cuda")
-    # the scales' product with 0.02 is rounded to f32 in the one, not the other
-    check(clef_i4.project_gate_up_f8(a, gate, up, out=out[:m]), want, slack + 2.0 ** -22 * want.abs() + 2.0 ** -22 * slack)
+    check(clef_i4.project_gate_up_f8(a, gate, up, out=out[:m]), want, slack)
     assert (out[m:] == 7.0).all()
 
 
@@ -239,8 +243,9 @@ def whole(shape, top, seed):
     return torch.randint(-top, top + 1, shape, generator=gen(seed), device="cuda").float()
 
 
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
 @pytest.mark.parametrize("m,k,n", SHAPES)
-def test_project_of_whole_numbers_is_exact(m, k, n):
+def test_project_of_whole_numbers_is_exact(m, k, n, kind):
     """Whole numbers up to 15: products at most 2^8 apart, sums below 2^24, so
     nothing is lost before the rounding to bf16."""
     x = whole((m, k), 15, m + k)
@@ -248,7 +253,8 @@ def test_project_of_whole_numbers_is_exact(m, k, n):
     x[:, ::128] = 15.0
     nb, kb = -(-n // 128), -(-k // 128)
     scales = torch.exp2(torch.randint(-3, 1, (nb, kb), generator=gen(3), device="cuda").float())
-    packed = clef_i4.f8_weight(w.to(F8), scales)
+    packed = clef_i4.f8_weight(w.to(F8), scales.to(torch.float8_e8m0fnu) if kind == "e8m0" else scales)
+    assert packed.pow2 == (kind == "e8m0")
     res = whole((m, n), 255, 5)
     wide = w.double() * scales.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
     want = x.double() @ wide.t()
@@ -332,18 +338,20 @@ def lists(tokens, topk, experts, seed, empty=()):
 
 
 EXPERTS = [(1, 8, 128, 256, 136), (1, 1, 1, 8, 8), (5, 2, 4, 384, 200), (37, 8, 60, 264, 136), (235, 4, 16, 768, 264),
-           (300, 1, 3, 1152, 128), (900, 2, 5, 256, 392), (2100, 8, 24, 136, 128)]
+           (300, 1, 3, 1152, 128), (900, 2, 5, 256, 392), (2100, 8, 24, 136, 128), (900, 1, 200, 264, 136),
+           (3000, 1, 4, 264, 3000), (3000, 1, 4, 128, 3000)]
 
 
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
 @pytest.mark.parametrize("tokens,topk,experts,k,n", EXPERTS)
-def test_experts_match_64_bits(tokens, topk, experts, k, n):
+def test_experts_match_64_bits(tokens, topk, experts, k, n, kind):
     empty = (0, experts - 1) if experts > topk + 2 else ()
     (offsets, slots), ids = lists(tokens, topk, experts, tokens + n, empty)
     total = tokens * topk
-    codes, scales = weight(experts, n, k, "f32", 5)
+    codes, scales = weight(experts, n, k, kind, 5)
     uc, us = weight(experts, n, k, "e8m0", 7)
     w, up = clef_i4.f8_weight(codes, scales), clef_i4.f8_weight(uc, us)
-    gate = clef_i4.f8_weight(codes, scales * 2.0 ** -6)
+    gate = clef_i4.f8_weight(codes, (scales.float() * 2.0 ** -6).to(scales.dtype))
     w64, u64 = weight64(codes, scales), weight64(uc, us)
     a = clef_i4.prepare_f8(randn((tokens, k), 1.0, 1))
     routed = clef_i4.prepare_f8(randn((total, k), 1.0, 2))
