@@ -86,15 +86,15 @@ SIGNATURES = {
     "clef_f8_prepare": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _P]),
     "clef_f8_pack_weight": (ctypes.c_int, [_P, _I64, _I32, _I32, _P, _P, _P]),
     "clef_f8_retile": (ctypes.c_int, [_P, _I64, _I32, _I32, _P, _P]),
-    "clef_f8_gemm": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P, _P]),
-    "clef_f8_gemm_gate_up": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P]),
+    "clef_f8_gemm": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _I32, _I32, _P, _P, _P]),
+    "clef_f8_gemm_gate_up": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P]),
     "clef_f8_project_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
     "clef_f8_project": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _P, _I32, _I32, _P, _P, _P, _SZ, _P]),
     "clef_moe_group_slots_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
     "clef_moe_group_slots": (ctypes.c_int, [_P, _I64, _I32, _I32, _P, _P, _P, _SZ, _P]),
-    "clef_moe_expert_f8": (ctypes.c_int, [_P, _P, _I64, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _I32, _I32, _P,
+    "clef_moe_expert_f8": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _I32, _I32, _P,
                                           _P]),
-    "clef_moe_expert_gate_up_f8": (ctypes.c_int, [_P, _P, _I64, _P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32,
+    "clef_moe_expert_gate_up_f8": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32,
                                                   _I32, _I32, _P, _P]),
     "clef_pack_cache_path": (ctypes.c_int, [_P, _P, _P, _SZ]),
     "clef_pack_cache_read": (ctypes.c_int, [_P, _P, _P, _SZ, _P, _SZ, _P]),
@@ -897,7 +897,8 @@ def _f8_out(like: torch.Tensor, rows: int, cols: int, out: torch.Tensor | None) 
 @dataclass
 class PreparedF8:
     """prepare_f8 output: one uint8 buffer, e4m3 codes [rows][pitch] (pitch =
-    width rounded up to 128), then f32 scales [pitch / 128][rows]."""
+    width rounded up to 128), then the scales as e8m0 [rows][blocks rounded up
+    to 16] and as f32 [blocks][rows], blocks = pitch / 128."""
     storage: torch.Tensor
     rows: int
     width: int
@@ -913,18 +914,21 @@ class PreparedF8:
         return codes.view(self.rows, self.pitch)[:, : self.width]
 
     @property
+    def _scales_at(self) -> int:
+        return self.rows * (self.pitch + (self.pitch // 128 + 15) // 16 * 16)
+
+    @property
     def scales(self) -> torch.Tensor:
-        """f32 [rows][ceil(width / 128)], a view (k-block major in memory)."""
-        start = self.rows * self.pitch
+        """f32 [rows][ceil(width / 128)], a view."""
+        start = self._scales_at
         scales = self.storage[start: start + self.rows * self.pitch // 32].view(torch.float32)
         return scales.view(self.pitch // 128, self.rows).t()
 
-    def call_args(self):
-        """codes and scales as call arguments: addresses, without views."""
-        if self.storage.dtype != torch.uint8 or self.storage.numel() < self.rows * self.pitch * 33 // 32:
+    def call_arg(self) -> torch.Tensor:
+        """The buffer, as large as its rows need."""
+        if self.storage.dtype != torch.uint8 or self.storage.numel() < self._scales_at + self.rows * self.pitch // 32:
             raise ClefError(-1, "FP8 activation buffer too small")
-        base = _n.pointer(self.storage)
-        return base, base + self.rows * self.pitch
+        return self.storage
 
 
 def prepare_f8(x: torch.Tensor, out: torch.Tensor | None = None) -> PreparedF8:
@@ -1006,8 +1010,7 @@ def project_f8(a: PreparedF8, w: F8Weight, residual: torch.Tensor | None = None,
     _on_current(a.storage, w.codes, residual)
     _check_residual(residual, a.rows, w.rows)
     out = _f8_out(a.storage, a.rows, w.rows, out)
-    codes, scales = a.call_args()
-    _n.launch(_n.clef_f8_gemm, codes, scales, w.codes, w.scales, a.rows, w.rows, w.cols, int(w.pow2), residual,
+    _n.launch(_n.clef_f8_gemm, a.call_arg(), w.codes, w.scales, a.rows, w.rows, w.cols, int(w.pow2), residual,
               out)
     return out
 
@@ -1040,8 +1043,7 @@ def project_gate_up_f8(a: PreparedF8, gate: F8Weight, up: F8Weight, out: torch.T
         raise ClefError(-1, _BAD_F8)
     _on_current(a.storage, gate.codes, up.codes)
     out = _f8_out(a.storage, a.rows, gate.rows, out)
-    codes, scales = a.call_args()
-    _n.launch(_n.clef_f8_gemm_gate_up, codes, scales, gate.codes, gate.scales, up.codes, up.scales, a.rows, gate.rows,
+    _n.launch(_n.clef_f8_gemm_gate_up, a.call_arg(), gate.codes, gate.scales, up.codes, up.scales, a.rows, gate.rows,
               gate.cols, int(gate.pow2 and up.pow2), out)
     return out
 
@@ -1086,8 +1088,7 @@ def expert_f8(a: PreparedF8, w: F8Weight, offsets: torch.Tensor, slots: torch.Te
     as they were in `out`, undefined in a new output."""
     total = _check_lists(a, w, offsets, slots, topk, input_routed)
     out = _f8_out(a.storage, total, w.rows, out)
-    codes, scales = a.call_args()
-    _n.launch(_n.clef_moe_expert_f8, codes, scales, a.rows, w.codes, w.scales, offsets, slots, w.matrices, total, topk,
+    _n.launch(_n.clef_moe_expert_f8, a.call_arg(), a.rows, w.codes, w.scales, offsets, slots, w.matrices, total, topk,
               int(input_routed), w.cols, w.rows, int(w.pow2), out)
     return out
 
@@ -1102,8 +1103,7 @@ def expert_gate_up_f8(a: PreparedF8, gate: F8Weight, up: F8Weight, offsets: torc
     total = _check_lists(a, gate, offsets, slots, topk, input_routed)
     _on_current(up.codes)
     out = _f8_out(a.storage, total, gate.rows, out)
-    codes, scales = a.call_args()
-    _n.launch(_n.clef_moe_expert_gate_up_f8, codes, scales, a.rows, gate.codes, gate.scales, up.codes, up.scales,
+    _n.launch(_n.clef_moe_expert_gate_up_f8, a.call_arg(), a.rows, gate.codes, gate.scales, up.codes, up.scales,
               offsets, slots, gate.matrices, total, topk, int(input_routed), gate.cols, gate.rows,
               int(gate.pow2 and up.pow2), out)
     return out

@@ -847,6 +847,14 @@ int check_f8_weight(int64_t matrices, int32_t n, int32_t k) {
   return CLEF_OK;
 }
 
+// The parts of a prepared activation (f8.hpp).
+void set_f8_activation(clef::F8Args& x, const uint8_t* a, int64_t rows, int32_t k) {
+  x.a = a;
+  x.ae = a + rows * clef::f8_pitch(k);
+  x.as = reinterpret_cast<const float*>(x.ae + rows * clef::f8_scale_pitch(k));
+  x.rows = rows;
+}
+
 int check_f8_lists(int64_t a_rows, const int32_t* offsets, const int32_t* slots, int64_t experts, int64_t total,
                    int32_t topk, int32_t input_routed, int32_t k, int32_t n) {
   if (!(experts >= 1 && experts <= kF8MostExperts && total >= 0 && total <= 16777216 && topk >= 1 && topk <= 128))
@@ -857,8 +865,6 @@ int check_f8_lists(int64_t a_rows, const int32_t* offsets, const int32_t* slots,
     return fail("expert lists name more rows than the activation has");
   if (a_rows > kF8MostRows * (int64_t)128 || a_rows * clef::f8_pitch(k) > (int64_t)0xFFFFFFFF)
     return fail("expert activation operand of 4 GiB or more (split the tokens into chunks)");
-  if (a_rows * clef::f8_blocks(k) * 4 > (int64_t)0x7FFFFFFF)
-    return fail("expert activation scales of 2 GiB or more (split the tokens into chunks)");
   if (!aligned(offsets, 4) || (slots && !aligned(slots, 4))) return fail("expert list pointer is NULL or not aligned");
   return CLEF_OK;
 }
@@ -883,8 +889,9 @@ int clef_f8_prepare(const uint16_t* x, int64_t rows, int32_t width, int64_t x_st
     return fail(kF8Shape);
   if (rows == 0) return CLEF_OK;
   if (!aligned(x, 16) || !aligned(out, 16)) return fail(kAlign);
-  float* scales = reinterpret_cast<float*>(out + rows * clef::f8_pitch(width));
-  return hip_status(clef::launch_f8_prepare(x, rows, width, x_stride, out, scales, hs(stream)));
+  uint8_t* exponents = out + rows * clef::f8_pitch(width);
+  float* scales = reinterpret_cast<float*>(exponents + rows * clef::f8_scale_pitch(width));
+  return hip_status(clef::launch_f8_prepare(x, rows, width, x_stride, out, exponents, scales, hs(stream)));
 }
 
 int clef_f8_pack_weight(const uint16_t* w, int64_t matrices, int32_t n, int32_t k, uint8_t* codes, float* scales,
@@ -900,29 +907,31 @@ int clef_f8_retile(const uint8_t* w, int64_t matrices, int32_t n, int32_t k, uin
   return hip_status(clef::launch_f8_retile(w, matrices, n, k, codes, hs(stream)));
 }
 
-int clef_f8_gemm(const uint8_t* a, const float* a_scales, const uint8_t* w, const float* w_scales, int64_t m,
+int clef_f8_gemm(const uint8_t* a, const uint8_t* w, const float* w_scales, int64_t m,
                  int32_t n, int32_t k, int32_t pow2, const uint16_t* residual, uint16_t* out, clef_stream_t stream) {
   if (int rc = check_f8_gemm(m, n, k)) return rc;
   if (m == 0) return CLEF_OK;
-  if (!aligned(a, 16) || !aligned(a_scales, 16) || !aligned(w, 16) || !aligned(w_scales, 16) || !aligned(out, 16) ||
+  if (!aligned(a, 16) || !aligned(w, 16) || !aligned(w_scales, 16) || !aligned(out, 16) ||
       (residual && !aligned(residual, 16)))
     return fail(kAlign);
   clef::F8Args x{};
-  x.a = a, x.as = a_scales, x.rows = m, x.w = w, x.ws = w_scales, x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
+  set_f8_activation(x, a, m, k);
+  x.w = w, x.ws = w_scales, x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
   x.pow2 = pow2 != 0, x.residual = residual, x.out = out;
   return hip_status(clef::launch_f8_gemm(x, false, hs(stream)));
 }
 
-int clef_f8_gemm_gate_up(const uint8_t* a, const float* a_scales, const uint8_t* gate, const float* gate_scales,
+int clef_f8_gemm_gate_up(const uint8_t* a, const uint8_t* gate, const float* gate_scales,
                          const uint8_t* up, const float* up_scales, int64_t m, int32_t n, int32_t k, int32_t pow2,
                          uint16_t* h, clef_stream_t stream) {
   if (int rc = check_f8_gemm(m, n, k)) return rc;
   if (m == 0) return CLEF_OK;
-  if (!aligned(a, 16) || !aligned(a_scales, 16) || !aligned(gate, 16) || !aligned(gate_scales, 16) ||
+  if (!aligned(a, 16) || !aligned(gate, 16) || !aligned(gate_scales, 16) ||
       !aligned(up, 16) || !aligned(up_scales, 16) || !aligned(h, 16))
     return fail(kAlign);
   clef::F8Args x{};
-  x.a = a, x.as = a_scales, x.rows = m, x.w = gate, x.ws = gate_scales, x.w2 = up, x.ws2 = up_scales;
+  set_f8_activation(x, a, m, k);
+  x.w = gate, x.ws = gate_scales, x.w2 = up, x.ws2 = up_scales;
   x.n = n, x.kb = clef::f8_blocks(k), x.k = k, x.pow2 = pow2 != 0, x.out = h;
   return hip_status(clef::launch_f8_gemm(x, true, hs(stream)));
 }
@@ -951,7 +960,7 @@ int clef_f8_project(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, c
   if (workspace_bytes < clef_f8_project_workspace_bytes(m, n, k)) return fail(kWorkspace);
   uint8_t* a = static_cast<uint8_t*>(workspace);
   if (int rc = clef_f8_prepare(x, m, k, x_stride, a, stream)) return rc;
-  return clef_f8_gemm(a, reinterpret_cast<const float*>(a + m * clef::f8_pitch(k)), w, w_scales, m, n, k, pow2, residual,
+  return clef_f8_gemm(a, w, w_scales, m, n, k, pow2, residual,
                       out, stream);
 }
 
@@ -972,31 +981,33 @@ int clef_moe_group_slots(const float* routes, int64_t tokens, int32_t topk, int3
   return hip_status(clef::launch_group_slots(routes, tokens, topk, experts, offsets, slots, workspace, hs(stream)));
 }
 
-int clef_moe_expert_f8(const uint8_t* a, const float* a_scales, int64_t a_rows, const uint8_t* w, const float* w_scales,
+int clef_moe_expert_f8(const uint8_t* a, int64_t a_rows, const uint8_t* w, const float* w_scales,
                        const int32_t* offsets, const int32_t* slots, int32_t experts, int64_t total, int32_t topk,
                        int32_t input_routed, int32_t k, int32_t n, int32_t pow2, uint16_t* out, clef_stream_t stream) {
   if (int rc = check_f8_lists(a_rows, offsets, slots, experts, total, topk, input_routed, k, n)) return rc;
   if (total == 0) return CLEF_OK;
-  if (!aligned(a, 16) || !aligned(a_scales, 16) || !aligned(w, 16) || !aligned(w_scales, 16) || !aligned(out, 16))
+  if (!aligned(a, 16) || !aligned(w, 16) || !aligned(w_scales, 16) || !aligned(out, 16))
     return fail(kAlign);
   clef::F8Args x{};
-  x.a = a, x.as = a_scales, x.rows = a_rows, x.w = w, x.ws = w_scales, x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
+  set_f8_activation(x, a, a_rows, k);
+  x.w = w, x.ws = w_scales, x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
   x.pow2 = pow2 != 0, x.out = out, x.lists = {offsets, slots, experts, (int)total, input_routed ? 1 : topk};
   return hip_status(clef::launch_f8_experts(x, false, hs(stream)));
 }
 
-int clef_moe_expert_gate_up_f8(const uint8_t* a, const float* a_scales, int64_t a_rows, const uint8_t* gate,
+int clef_moe_expert_gate_up_f8(const uint8_t* a, int64_t a_rows, const uint8_t* gate,
                                const float* gate_scales, const uint8_t* up, const float* up_scales,
                                const int32_t* offsets, const int32_t* slots, int32_t experts, int64_t total,
                                int32_t topk, int32_t input_routed, int32_t k, int32_t n, int32_t pow2, uint16_t* h,
                                clef_stream_t stream) {
   if (int rc = check_f8_lists(a_rows, offsets, slots, experts, total, topk, input_routed, k, n)) return rc;
   if (total == 0) return CLEF_OK;
-  if (!aligned(a, 16) || !aligned(a_scales, 16) || !aligned(gate, 16) || !aligned(gate_scales, 16) ||
+  if (!aligned(a, 16) || !aligned(gate, 16) || !aligned(gate_scales, 16) ||
       !aligned(up, 16) || !aligned(up_scales, 16) || !aligned(h, 16))
     return fail(kAlign);
   clef::F8Args x{};
-  x.a = a, x.as = a_scales, x.rows = a_rows, x.w = gate, x.ws = gate_scales, x.w2 = up, x.ws2 = up_scales;
+  set_f8_activation(x, a, a_rows, k);
+  x.w = gate, x.ws = gate_scales, x.w2 = up, x.ws2 = up_scales;
   x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
   x.pow2 = pow2 != 0, x.out = h, x.lists = {offsets, slots, experts, (int)total, input_routed ? 1 : topk};
   return hip_status(clef::launch_f8_experts(x, true, hs(stream)));

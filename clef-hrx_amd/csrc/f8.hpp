@@ -3,8 +3,12 @@
 // along k: y[m][n] = sum_b sa[m][b] sw[n / 128][b] sum_{k in block b} qa[m][k] qw[n][k].
 //
 // Activation ("prepared"): codes row-major [rows][pitch], pitch the width
-// rounded up to 128 (the rest zeros), then f32 scales [pitch / 128][rows]: the
-// scales that a tile needs in one k-step lie side by side.
+// rounded up to 128 (the rest zeros), then its scales in two forms: as e8m0
+// bytes [rows][kb rounded up to 16] (bits 23..30 of the f32), 16 blocks of k of
+// a row in one 16-byte load, which the tiled products keep in LDS, and as f32
+// [kb][rows], the rows of a fragment side by side, which the split-k products
+// load as they go (with the bytes instead, 64 x 64 tiles took 724 us, not 584,
+// at 4096 x 4096 x 12288).
 //
 // Weight: blocks of 128 rows x 128 k (16 KiB), block (r / 128, k / 128) of one
 // matrix at ((r / 128) * kb + k / 128) * 16384; rows and columns past the end
@@ -28,8 +32,9 @@ namespace clef {
 
 constexpr int f8_blocks(int64_t width) { return (int)((width + 127) / 128); }
 constexpr int64_t f8_pitch(int64_t width) { return (width + 127) / 128 * 128; }
+constexpr int64_t f8_scale_pitch(int64_t width) { return (f8_blocks(width) + 15) / 16 * 16; }
 constexpr int64_t f8_prepared_bytes(int64_t rows, int64_t width) {
-  return rows * f8_pitch(width) + 4 * rows * f8_blocks(width);
+  return rows * (f8_pitch(width) + f8_scale_pitch(width) + 4 * f8_blocks(width));
 }
 constexpr int64_t f8_weight_bytes(int64_t matrices, int64_t rows, int64_t cols) {
   return matrices * f8_blocks(rows) * f8_blocks(cols) * 16384;
@@ -50,14 +55,15 @@ struct F8Lists {
 // gate, w2 the up matrices, n the width of h.
 struct F8Args {
   const uint8_t* a;
-  const float* as;  // [kb][rows]
+  const uint8_t* ae;  // its scales: e8m0 [rows][kb rounded up to 16]
+  const float* as;    // and f32 [kb][rows]
   int64_t rows;     // rows of a
   const uint8_t* w;
   const float* ws;
   const uint8_t* w2;
   const float* ws2;
   int n, kb;  // output columns, blocks of 128 along k
-  bool pow2;  // every scale of a and w is a power of two
+  bool pow2;  // every scale of w is a power of two
   const uint16_t* residual;
   uint16_t* out;
   F8Lists lists;
@@ -68,7 +74,7 @@ struct F8Args {
 };
 
 hipError_t launch_f8_prepare(const uint16_t* x, int64_t rows, int width, int64_t x_stride, uint8_t* codes,
-                             float* scales, hipStream_t stream);
+                             uint8_t* exponents, float* scales, hipStream_t stream);
 hipError_t launch_f8_pack(const uint16_t* w, int64_t matrices, int n, int k, uint8_t* codes, float* scales,
                           hipStream_t stream);
 hipError_t launch_f8_retile(const uint8_t* w, int64_t matrices, int n, int k, uint8_t* codes, hipStream_t stream);
@@ -84,6 +90,7 @@ hipError_t launch_group_slots(const float* routes, int64_t tokens, int topk, int
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef int v8i_t __attribute__((ext_vector_type(8)));
 
 // D = W A^T of a 16 x 16 tile over 128 k, added to c. Lane l holds weight row
@@ -95,10 +102,20 @@ __device__ __forceinline__ v4f mfma_f8(v8i_t w, v8i_t a, v4f c) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 0, 127, 0, 127);
 }
 
-// The same with the scales in the MFMA: e8m0 exponents in the top bytes of sw
-// (of w's rows) and sa (of a's rows; lane l's row l % 16).
-__device__ __forceinline__ v4f mfma_f8_scaled(v8i_t w, v8i_t a, v4f c, int sw, int sa) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 3, sw, 3, sa);
+// The same with the scales in the MFMA: e8m0 exponents, in byte 3 of sw (of w's
+// rows) and byte `byte` (known when compiled) of sa (of a's rows; lane l's row l % 16).
+__device__ __forceinline__ v4f mfma_f8_scaled(v8i_t w, v8i_t a, v4f c, int sw, uint32_t sa, int byte) {
+  switch (byte) {
+    case 0: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 3, sw, 0, (int)sa);
+    case 1: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 3, sw, 1, (int)sa);
+    case 2: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 3, sw, 2, (int)sa);
+    default: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 3, sw, 3, (int)sa);
+  }
+}
+
+// The power of two whose e8m0 exponent is byte `byte` of v.
+__device__ __forceinline__ float e8m0_byte(uint32_t v, int byte) {
+  return as_float((byte < 3 ? v << (23 - 8 * byte) : v >> 1) & 0x7F800000u);
 }
 
 __device__ __forceinline__ v8i_t join_halves(v4i lo, v4i hi) {

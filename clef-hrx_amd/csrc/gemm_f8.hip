@@ -59,18 +59,16 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
   for (int i = 0; i < MT; ++i) {
     int r = 16 * i + lr;
     r = r < here ? r : here - 1;
-    int64_t row = m0 + r;
+    int64_t row = r;
     if constexpr (LISTS) {
       const int place = first + r;
       const int slot = p.lists.slots ? p.lists.slots[place] : place;
       // a slot outside the table reads nothing (it is not stored either)
       row = slot >= 0 && slot < p.lists.total ? slot / p.lists.div : 0;
       row = row < p.rows ? row : 0;
-      a_voff[i] = (int)((uint32_t)row * (uint32_t)pitch) + 16 * g;
-    } else {
-      a_voff[i] = r * pitch + 16 * g;
     }
-    s_voff[i] = (int)(row * 4);
+    a_voff[i] = (int)((uint32_t)row * (uint32_t)pitch) + 16 * g;
+    s_voff[i] = (int)((m0 + row) * 4);
   }
   const int nb = f8_blocks(p.n);
   const int64_t panel = ((int64_t)expert * nb + n0 / 128) * kb;
@@ -196,9 +194,11 @@ hipError_t launch_stream(const F8Args& x, hipStream_t stream) {
 
 // Tile shape of f8_tile_kernel: WAVES_M x WAVES_N waves of WM rows x WN weight
 // rows, NST LDS stages of one block of k each: A rows (128 bytes each, 16-byte
-// chunk c of row r at c ^ ((r >> 1) & 7)), B fragments in the operand order, the
-// rows' scales (per 16 WM / 16-value groups, in the order the lanes read them)
-// and the two weight panels' scales.
+// chunk c of row r at c ^ ((r >> 1) & 7)) and B fragments in the operand order.
+// Behind the stages the rows' e8m0 scales of 16 blocks of k, as loaded (16 bytes
+// per row) and, twice, turned into the order of use (per block of k a lane's TM
+// rows side by side), the scales of the tile's one or two weight panels (256 f32
+// each) and, with lists, the tile's output rows.
 template <int WM_, int WN_, int WAVES_M_, int WAVES_N_, int NST_, int GROUPS_ = 1>
 struct F8Tile {
   static constexpr int GROUPS = GROUPS_;  // workgroups per CU
@@ -206,20 +206,18 @@ struct F8Tile {
   static constexpr int NW = WAVES_M * WAVES_N, THREADS = 64 * NW;
   static constexpr int BM = WM * WAVES_M, BN = WN * WAVES_N;
   static constexpr int TM = WM / 16, TN = WN / 16;  // fragments per wave
-  static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, SA_BYTES = BM * 4, SW_BYTES = 256;
-  static constexpr int SA = A_BYTES + B_BYTES, SW = SA + SA_BYTES;
-  static constexpr int STAGE_BYTES = SW + SW_BYTES * (NW - BM / 64);
+  static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int A_SLOTS = A_BYTES / 1024 / NW, B_SLOTS = B_BYTES / 1024 / NW;
-  // a wave's DMA instructions per stage: first (X) the weight fragments, the
-  // rows of its first TM / 2 activation fragments and the scales, then (Y) the
-  // other rows
-  static constexpr int Y = A_SLOTS / 2, X = B_SLOTS + A_SLOTS - Y + 1, DMA = X + Y;
-  static constexpr int ROWS = NST * STAGE_BYTES;     // lists: the tile's output rows
+  // a wave's DMA instructions per stage: first (X) the weight fragments and the
+  // rows of its first TM / 2 activation fragments, then (Y) the other rows
+  static constexpr int Y = A_SLOTS / 2, X = B_SLOTS + A_SLOTS - Y, DMA = X + Y;
+  static constexpr int SA_BYTES = BM * 16, SA = NST * STAGE_BYTES, ST = SA + SA_BYTES, SW = ST + 2 * SA_BYTES;
+  static constexpr int ROWS = SW + 2 * 1024;
   static constexpr int LDS = ROWS + BM * 4;
   static constexpr int EPI = 16 * WN * 2;            // epilogue staging per wave
-  static_assert(NW == 8 && (BN == 256 || BN == 128) && BM / 64 + 2 <= NW, "eight waves, one or two weight panels");
+  static_assert(NW == 8 && (BN == 256 || BN == 128) && BM / 64 <= NW, "eight waves, one or two weight panels");
   static_assert(A_BYTES % (2048 * NW) == 0 && B_BYTES % (2048 * NW) == 0 && LDS <= 160 * 1024, "whole instructions per wave");
-  static_assert(TM * TN % 4 == 0 && TM % 4 == 0 && TN % 2 == 0 && NST >= 2 && NST <= 4, "step");
+  static_assert(TM * TN % 4 == 0 && TM % 4 == 0 && TN % 2 == 0 && (NST == 2 || NST == 4), "step");
   static_assert(X <= TM / 2 * TN && Y <= TN, "one DMA instruction per MFMA behind each barrier");
 };
 
@@ -248,7 +246,7 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, g = lane >> 4;
   const int wm = wave / T::WAVES_N, wn = wave % T::WAVES_N;
-  const int kb = p.kb, pitch = kb * 128;
+  const int kb = p.kb, pitch = kb * 128, kp = (kb + 15) / 16 * 16;
   int tm, tn, expert = 0, first = 0, here;
   int64_t m0 = 0;
   if constexpr (LISTS) {
@@ -272,7 +270,7 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
 
   // this wave's DMA: A instruction s moves 8 rows, the first half of a wave's
   // instructions rows of the first TM / 2 fragments of either row of waves
-  int a_voff[T::A_SLOTS], s_voff;
+  int a_voff[T::A_SLOTS];
   auto a_piece = [&](int s) {  // KiB of the stage
     constexpr int H = T::A_SLOTS / 2;
     constexpr int PER = T::WM / 16;  // KiB of half of a row of waves' rows
@@ -304,25 +302,35 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
   const __amdgpu_buffer_rsrc_t b_rsrc = make_rsrc((up ? p.w2 : p.w) + (first_block + (int64_t)panel * kb) * 16384,
                                                   panel < nb ? (uint32_t)kb * 16384u : 0u);
   const int b_voff = frag % 8 * 2048 + lane * 16;
-  // scales: the first BM / 64 waves the rows', the others the panels' (lane 0
-  // the first, lane 1 the second)
-  const bool row_scales = wave < T::BM / 64;
-  __amdgpu_buffer_rsrc_t s_rsrc;
-  if (row_scales) {
-    const int word = 64 * wave + lane, r = word / T::WM * T::WM + 16 * (word % TM) + word % T::WM / TM;
-    s_voff = (int)(source_row(r) * 4);
-    s_rsrc = make_rsrc(p.as + m0, (uint32_t)((p.rows * kb - m0) * 4));
-  } else if (GU) {
-    const float* second = wave & 1 ? p.ws2 : p.ws;
-    s_voff = 0;
-    s_rsrc = make_rsrc(second + first_block + (int64_t)(n0 / 128) * kb, (uint32_t)kb * 4u);
-  } else {
-    const int q = n0 / 128 + (wave & 1);
-    s_voff = 0;
-    s_rsrc = make_rsrc(p.ws + first_block + (int64_t)q * kb, q < nb ? (uint32_t)kb * 4u : 0u);
+  // scales: of the rows, 16 blocks of k at a time by the first BM / 64 waves
+  const __amdgpu_buffer_rsrc_t s_rsrc =
+      make_rsrc(p.ae + m0 * kp, (uint32_t)(LISTS ? p.rows * kp : (int64_t)here * kp));
+  const int s_voff = (int)((uint32_t)source_row(64 * wave + lane) * (uint32_t)kp);
+  auto issue_scales = [&](int chunk) {
+    if (wave < T::BM / 64)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(s_rsrc, (lds_ptr_t)(lds + T::SA + wave * 1024), 16, s_voff, chunk * 16, 0,
+                                               0);
+  };
+  // into the order of use, each row by the lane that loaded it: row wm WM + 16 i
+  // + l of block kt at kt BM + wm WM + l TM + i
+  auto turn_scales = [&](int chunk) {
+    if (wave < T::BM / 64) {
+      const int r = 64 * wave + lane;
+      const v4u v = *reinterpret_cast<const v4u*>(lds + T::SA + r * 16);
+      char* to = lds + T::ST + (chunk & 1) * T::SA_BYTES + r / T::WM * T::WM + r % 16 * TM + r % T::WM / 16;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) to[k * T::BM] = (char)(v[k / 4] >> (8 * (k % 4)));
+    }
+  };
+  issue_scales(0);
+  // and of the panels (gate/up: gate, up), as f32
+  {
+    const int q = threadIdx.x >> 8, k = threadIdx.x & 255;
+    const int of = n0 / 128 + (GU ? 0 : q);
+    float v = 0.0f;
+    if (k < kb && of < nb) v = (GU && q ? p.ws2 : p.ws)[first_block + (int64_t)of * kb + k];
+    reinterpret_cast<float*>(lds + T::SW)[threadIdx.x] = v;
   }
-  const int s_dst = row_scales ? T::SA + wave * 256 : T::SW + (wave - T::BM / 64) * T::SW_BYTES;
-  const int s_step = row_scales ? (int)(p.rows * 4) : 4;
   if constexpr (LISTS) {
     for (int r = threadIdx.x; r < T::BM; r += T::THREADS) {
       int slot = -1;
@@ -339,27 +347,21 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
   auto issue = [&](char* stage, int kt, int x) {
     const bool in = kt < kb;
     const int k = in ? kt : 0;
-    constexpr int H = T::A_SLOTS / 2;
-    if (x < T::B_SLOTS) {
+    if (x < T::B_SLOTS)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? b_rsrc : none,
                                                (lds_ptr_t)(stage + T::A_BYTES + (T::B_SLOTS * wave + x) * 1024), 16,
                                                b_voff, k * 16384 + x * 1024, 0, 0);
-    } else if (x == T::B_SLOTS + H) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? s_rsrc : none, (lds_ptr_t)(stage + s_dst), 4, s_voff, k * s_step, 0,
-                                               0);
-    } else {
-      const int q = x < T::B_SLOTS + H ? x - T::B_SLOTS : x - T::B_SLOTS - 1;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? a_rsrc : none, (lds_ptr_t)(stage + a_piece(q) * 1024), 16, a_voff[q],
-                                               k * 128, 0, 0);
-    }
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? a_rsrc : none,
+                                               (lds_ptr_t)(stage + a_piece(x - T::B_SLOTS) * 1024), 16,
+                                               a_voff[x - T::B_SLOTS], k * 128, 0, 0);
   };
 
   // a fragment's two halves in a stage
   const int a_at0 = (wm * T::WM + lr) * 128 + ((g ^ (lr >> 1)) << 4), a_at1 = a_at0 ^ 64;
   const int b_at = T::A_BYTES + (GU ? wn * (TN / 2) : wn * TN) * 2048 + lane * 16;
-  const int sa_at = T::SA + wm * T::WM * 4 + lr * TM * 4;
-  const int sw_at = T::SW + ((GU ? 0 : wn * T::WN / 128) ^ ((T::BM / 64) & 1)) * T::SW_BYTES;
-  const int sw2_at = T::SW + (1 ^ ((T::BM / 64) & 1)) * T::SW_BYTES;
+  const char* const sa_at = lds + T::ST + wm * T::WM + lr * TM;
+  const float* const sw_at = reinterpret_cast<const float*>(lds + T::SW) + (GU ? 0 : wn * T::WN / 128) * 256;
 
   v4f acc[TM][TN];
 #pragma unroll
@@ -370,8 +372,9 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
     constexpr int MATS = GU ? 2 : 1;
     v8i_t av[2], bv[TN];
     v4f part[4];               // !HW: partial sums on their way
-    float sv[TM][MATS], last[MATS];  // !HW: this step's scales; those of the row before the step's first
-    int sa_bits[TM], sw_bits[MATS];  // HW: the scales' bits, exponent in the top byte
+    float sv[MATS], last[MATS];  // !HW: scales of the row of MFMAs and of the row before
+    uint32_t sa[TM / 4], sa_next[TM / 4];  // the rows' exponents, four in each
+    int sw_bits[MATS];         // HW: the panels' scales, exponent in the top byte
     auto read_a = [&](const char* stage, int i) {
       const v4i lo = *reinterpret_cast<const v4i*>(stage + a_at0 + i * 2048);
       const v4i hi = *reinterpret_cast<const v4i*>(stage + a_at1 + i * 2048);
@@ -381,28 +384,23 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
       const char* at = stage + b_at + (GU && j >= TN / 2 ? T::B_BYTES / 2 + (j - TN / 2) * 2048 : j * 2048);
       return join_halves(*reinterpret_cast<const v4i*>(at), *reinterpret_cast<const v4i*>(at + 1024));
     };
-    float sa[TM], sw[MATS];
-    auto read_scales = [&](const char* stage) {
+    float sw[MATS];
+    // of step kt (the step before still takes sa)
+    auto read_scales = [&](int kt) {
 #pragma unroll
-      for (int i = 0; i < TM; i += 4) {
-        const v4f v = *reinterpret_cast<const v4f*>(stage + sa_at + i * 4);
+      for (int t = 0; t < MATS; ++t) sw[t] = sw_at[t * 256 + (kt < kb ? kt : 0)];
+      const char* at = sa_at + (kt >> 4 & 1) * T::SA_BYTES + (kt & 15) * T::BM;
+      typedef uint32_t pack __attribute__((ext_vector_type(TM / 4)));
+      const pack v = *reinterpret_cast<const pack*>(at);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) sa[i + t] = v[t];
-      }
-      sw[0] = *reinterpret_cast<const float*>(stage + sw_at);
-      if constexpr (GU) sw[1] = *reinterpret_cast<const float*>(stage + sw2_at);
+      for (int i = 0; i < TM / 4; ++i) sa_next[i] = v[i];
     };
     auto take_scales = [&]() {
+#pragma unroll
+      for (int i = 0; i < TM / 4; ++i) sa[i] = sa_next[i];
       if constexpr (HW) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) sa_bits[i] = (int)(as_uint(sa[i]) << 1);
-#pragma unroll
         for (int t = 0; t < MATS; ++t) sw_bits[t] = (int)(as_uint(sw[t]) << 1);
-      } else {
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int t = 0; t < MATS; ++t) sv[i][t] = sa[i] * sw[t];
       }
     };
     auto add = [&](v4f& c, const v4f& v, float s) {
@@ -418,17 +416,24 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
     auto step = [&](char* cur, const char* next, int kt) {
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
+        if constexpr (!HW) {
+#pragma unroll
+          for (int t = 0; t < MATS; ++t) {
+            last[t] = sv[t];
+            sv[t] = e8m0_byte(sa[i / 4], i % 4) * sw[t];
+          }
+        }
         if (i == TM / 2 - 1) landed();  // this stage's Y; its X has been read
         if (i == TM - 1) {
           landed();  // the next stage's X; this stage has been read
-          read_scales(next);
+          read_scales(kt + 1);
         }
         av[(i + 1) & 1] = i + 1 < TM ? read_a(cur, i + 1) : read_a(next, 0);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
           if constexpr (HW) {
-            acc[i][j] = mfma_f8_scaled(bv[j], av[i & 1], acc[i][j], sw_bits[GU && j >= TN / 2 ? 1 : 0], sa_bits[i]);
+            acc[i][j] = mfma_f8_scaled(bv[j], av[i & 1], acc[i][j], sw_bits[GU && j >= TN / 2 ? 1 : 0], sa[i / 4], i % 4);
             __builtin_amdgcn_sched_barrier(0);
           } else {
             part[(i * TN + j) % 4] = mfma_f8(bv[j], av[i & 1], v4f{0, 0, 0, 0});
@@ -436,7 +441,7 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
             // the MFMA two before
             const int before = i * TN + j - 2, ii = (before + TM * TN) / TN % TM, jj = (before + TN) % TN;
             const int mat = GU && jj >= TN / 2 ? 1 : 0;
-            add(acc[ii][jj], part[(before + 4) % 4], before >= 0 ? sv[ii][mat] : last[mat]);
+            add(acc[ii][jj], part[(before + 4) % 4], j >= 2 ? sv[mat] : last[mat]);
           }
           if (i == TM - 1) bv[j] = read_b(next, j);
           // X behind the first barrier, Y behind the second
@@ -451,10 +456,6 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if constexpr (!HW) {
-#pragma unroll
-        for (int t = 0; t < MATS; ++t) last[t] = sv[TM - 1][t];
-      }
       take_scales();
     };
     char* const ring[4] = {r0, r1, r2, r3};
@@ -462,10 +463,12 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
     for (int n = 0; n < T::NST; ++n)
 #pragma unroll
       for (int x = 0; x < T::DMA; ++x) issue(ring[n], n, x);
+    wait_vmcnt<T::NST * T::DMA>();  // the first scales were issued before
+    turn_scales(0);
     wait_vmcnt<T::NST * T::DMA - T::X>();
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    read_scales(r0);
+    read_scales(0);
     av[0] = read_a(r0, 0);
 #pragma unroll
     for (int j = 0; j < TN; ++j) bv[j] = read_b(r0, j);
@@ -474,23 +477,35 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
 #pragma unroll
       for (int t = 0; t < 4; ++t) part[t] = v4f{0, 0, 0, 0};
 #pragma unroll
-      for (int t = 0; t < MATS; ++t) last[t] = 0.0f;
+      for (int t = 0; t < MATS; ++t) sv[t] = 0.0f;
     }
-    for (int kt = 0; kt < kb; kt += T::NST) {
-      step(r0, r1, kt);
-      if constexpr (T::NST == 2) {
-        if (kt + 1 < kb) step(r1, r0, kt + 1);
-      } else {
-        if (kt + 1 < kb) step(r1, r2, kt + 1);
-        if (kt + 2 < kb) step(r2, T::NST == 3 ? r0 : r3, kt + 2);
-        if constexpr (T::NST == 4)
+    // The scales of the next 16 blocks of k are loaded under 8 steps and turned
+    // before the other 8 (a branch inside a step instead made the compiler spill).
+    for (int k0 = 0; k0 < kb; k0 += 8) {
+      if ((k0 | 8) + 8 < kb) {
+        if (k0 & 8) {
+          wait_vmcnt<T::NST * T::DMA>();
+          turn_scales(k0 / 16 + 1);
+        } else {
+          issue_scales(k0 / 16 + 1);
+        }
+      }
+      const int k1 = k0 + 8 < kb ? k0 + 8 : kb;
+      for (int kt = k0; kt < k1; kt += T::NST) {
+        step(r0, r1, kt);
+        if constexpr (T::NST == 2) {
+          if (kt + 1 < kb) step(r1, r0, kt + 1);
+        } else {
+          if (kt + 1 < kb) step(r1, r2, kt + 1);
+          if (kt + 2 < kb) step(r2, r3, kt + 2);
           if (kt + 3 < kb) step(r3, r0, kt + 3);
+        }
       }
     }
     if constexpr (!HW) {
       // the last two partial sums
-      add(acc[TM - 1][TN - 2], part[2], last[GU && TN > 2 ? 1 : 0]);
-      add(acc[TM - 1][TN - 1], part[3], last[GU ? 1 : 0]);
+      add(acc[TM - 1][TN - 2], part[2], sv[GU && TN > 2 ? 1 : 0]);
+      add(acc[TM - 1][TN - 1], part[3], sv[GU ? 1 : 0]);
     }
   };
   body(lds, lds + T::STAGE_BYTES, lds + 2 % T::NST * T::STAGE_BYTES, lds + 3 % T::NST * T::STAGE_BYTES);

@@ -8,14 +8,16 @@ namespace clef {
 namespace {
 
 // x bf16 [rows][width] (row pitch x_stride) -> codes [rows][pitch], scales
-// [kb][rows]. 16 lanes hold a block of 128 columns, 8 values each: one 16-byte
+// as e8m0 [rows][kp] and f32 [kb][rows]. 16 lanes hold a block of 128 columns, 8 values each: one 16-byte
 // load, the maximum over the 16 lanes by DPP, one 8-byte store of codes (a
 // whole line per block). A workgroup covers 2^RLOG rows x CPW * STEPS blocks, so
-// that the scales of neighbouring rows go out together, with STEPS loads in
+// that the f32 scales of neighbouring rows go out together, with STEPS loads in
 // flight per lane. Bound by HBM: 2 bytes read and 1 written per value.
 template <int RLOG, int STEPS>
 __global__ __launch_bounds__(256) void f8_prepare_kernel(const uint16_t* __restrict__ x, int64_t rows, int width,
-                                                         int64_t x_stride, int kb, uint8_t* __restrict__ codes,
+                                                         int64_t x_stride, int kb, int kp,
+                                                         uint8_t* __restrict__ codes,
+                                                         uint8_t* __restrict__ exponents,
                                                          float* __restrict__ scales) {
   constexpr int R = 1 << RLOG, CPW = 16 / R;
   const int group = threadIdx.x >> 4, l = threadIdx.x & 15;
@@ -35,14 +37,21 @@ __global__ __launch_bounds__(256) void f8_prepare_kernel(const uint16_t* __restr
     const int b = b0 + s * CPW;
     uint32_t m = f8_amax2(f8_amax2(f8_amax2(f8_amax2(0u, v[s].x), v[s].y), v[s].z), v[s].w);
     m = group_max16(m);
-    if (!row_here || b >= kb) continue;
+    if (!row_here || b >= kp) continue;
+    if (b >= kb) {  // the row's bytes behind its exponents: zeros
+      if (l == 0) exponents[row * kp + b] = 0;
+      continue;
+    }
     const uint32_t field = f8_scale_field(m);
     const float inv = as_float((254u - field) << 23);
     uint2 q;
     q.x = f8_codes(v[s].x, v[s].y, inv);
     q.y = f8_codes(v[s].z, v[s].w, inv);
     *reinterpret_cast<uint2*>(codes + row * ((int64_t)kb * 128) + b * 128 + 8 * l) = q;
-    if (l == 0) scales[(int64_t)b * rows + row] = as_float(field << 23);
+    if (l == 0) {
+      exponents[row * kp + b] = (uint8_t)field;
+      scales[(int64_t)b * rows + row] = as_float(field << 23);
+    }
   }
 }
 
@@ -121,14 +130,14 @@ __global__ __launch_bounds__(256) void f8_retile_kernel(const uint8_t* __restric
 }  // namespace
 
 hipError_t launch_f8_prepare(const uint16_t* x, int64_t rows, int width, int64_t x_stride, uint8_t* codes,
-                             float* scales, hipStream_t stream) {
-  const int kb = f8_blocks(width);
+                             uint8_t* exponents, float* scales, hipStream_t stream) {
+  const int kb = f8_blocks(width), kp = (int)f8_scale_pitch(width);
   constexpr int STEPS = 4;
   auto run = [&](auto rlog) {
     constexpr int R = 1 << decltype(rlog)::value, per = 16 / R * STEPS;
-    const dim3 grid((unsigned)((rows + R - 1) / R), (unsigned)((kb + per - 1) / per));
+    const dim3 grid((unsigned)((rows + R - 1) / R), (unsigned)((kp + per - 1) / per));
     f8_prepare_kernel<decltype(rlog)::value, STEPS>
-        <<<grid, 256, 0, stream>>>(x, rows, width, x_stride, kb, codes, scales);
+        <<<grid, 256, 0, stream>>>(x, rows, width, x_stride, kb, kp, codes, exponents, scales);
   };
   // rows per workgroup: 8 where there are rows, else as many as there are
   if (rows >= 8)

@@ -492,8 +492,11 @@ int clef_moe_router_logits(const uint16_t* x, const uint16_t* gate_w, int64_t to
  *   y[m][n] = sum_b sa[m][b] * sw[n/128][b] * sum_{k in block b} qa[m][k] * qw[n][k]
  * in f32, rounded to bf16 once (behind the residual or SwiGLU). Widths and
  * column counts are multiples of 8; blocks may end inside.
- *   activation      codes [rows][pitch], pitch = width rounded up to 128 (the
- *                   rest zeros), then f32 scales [pitch/128][rows]
+ *   activation      one buffer: codes [rows][pitch], pitch = width rounded up
+ *                   to 128 (the rest zeros), then its scales, powers of two,
+ *                   as e8m0 bytes [rows][blocks rounded up to 16] (zeros
+ *                   behind a row's blocks) and again as f32 [blocks][rows],
+ *                   blocks = pitch/128
  *   tiled weight    128-row x 128-k blocks of 16 KiB, block (r/128, k/128) of
  *                   a matrix at ((r/128)*ceil(cols/128) + k/128)*16384, byte
  *                   (r, k) of a block at (r/16)*2048 + (k/64)*1024 +
@@ -526,15 +529,15 @@ int clef_f8_pack_weight(const uint16_t* w, int64_t matrices, int32_t n, int32_t 
 int clef_f8_retile(const uint8_t* w, int64_t matrices, int32_t n, int32_t k, uint8_t* codes, clef_stream_t stream);
 
 /* Projection of a prepared activation; residual bf16 [m][n], nullable. pow2
- * (here and below) nonzero: every scale of a and w is a power of two between
- * 2^-126 and 2^127, as clef_f8_prepare, clef_f8_pack_weight and e8m0
- * checkpoints make them; the matrix unit may then apply them (with other
+ * (here and below) nonzero: every scale of w is a power of two between 2^-126
+ * and 2^127, as clef_f8_pack_weight and e8m0 checkpoints make them; the matrix
+ * unit may then apply them (with other
  * scales it would drop their mantissas). The same sums within f32 rounding. */
-int clef_f8_gemm(const uint8_t* a, const float* a_scales, const uint8_t* w, const float* w_scales, int64_t m,
+int clef_f8_gemm(const uint8_t* a, const uint8_t* w, const float* w_scales, int64_t m,
                  int32_t n, int32_t k, int32_t pow2, const uint16_t* residual, uint16_t* out, clef_stream_t stream);
 
 /* h[m][n] = silu(g) * u of the two projections' f32 sums, bf16 once. */
-int clef_f8_gemm_gate_up(const uint8_t* a, const float* a_scales, const uint8_t* gate, const float* gate_scales,
+int clef_f8_gemm_gate_up(const uint8_t* a, const uint8_t* gate, const float* gate_scales,
                          const uint8_t* up, const float* up_scales, int64_t m, int32_t n, int32_t k, int32_t pow2,
                          uint16_t* h, clef_stream_t stream);
 
@@ -564,14 +567,13 @@ int clef_moe_group_slots(const float* routes, int64_t tokens, int32_t topk, int3
  * write one row). Preconditions: 1 <= experts <= 1024, total <= 16777216, 1 <=
  * topk <= 128 -> "invalid grouped expert lists"; the shapes above; a_rows >=
  * the rows that total slots need -> "expert lists name more rows than the
- * activation has"; codes of the activation below 4 GiB and its scales below
- * 2 GiB. */
-int clef_moe_expert_f8(const uint8_t* a, const float* a_scales, int64_t a_rows, const uint8_t* w, const float* w_scales,
+ * activation has"; codes of the activation below 4 GiB. */
+int clef_moe_expert_f8(const uint8_t* a, int64_t a_rows, const uint8_t* w, const float* w_scales,
                        const int32_t* offsets, const int32_t* slots, int32_t experts, int64_t total, int32_t topk,
                        int32_t input_routed, int32_t k, int32_t n, int32_t pow2, uint16_t* out, clef_stream_t stream);
 
 /* h = silu(gate) * up over the same lists, as clef_f8_gemm_gate_up. */
-int clef_moe_expert_gate_up_f8(const uint8_t* a, const float* a_scales, int64_t a_rows, const uint8_t* gate,
+int clef_moe_expert_gate_up_f8(const uint8_t* a, int64_t a_rows, const uint8_t* gate,
                                const float* gate_scales, const uint8_t* up, const float* up_scales,
                                const int32_t* offsets, const int32_t* slots, int32_t experts, int64_t total,
                                int32_t topk, int32_t input_routed, int32_t k, int32_t n, int32_t pow2, uint16_t* h,

@@ -15,15 +15,16 @@ def call(name, *args):
 
 def test_sizes():
     lib = clef_i4.lib()
-    assert lib.clef_f8_prepared_bytes(5, 128) == 5 * 128 + 5 * 4
-    assert lib.clef_f8_prepared_bytes(5, 136) == 5 * 256 + 2 * 5 * 4
+    assert lib.clef_f8_prepared_bytes(5, 128) == 5 * (128 + 16 + 4)
+    assert lib.clef_f8_prepared_bytes(5, 136) == 5 * (256 + 16 + 2 * 4)
+    assert lib.clef_f8_prepared_bytes(5, 2056) == 5 * (17 * 128 + 32 + 17 * 4)
     assert lib.clef_f8_prepared_bytes(0, 136) == 0
-    assert lib.clef_f8_prepared_bytes(1 << 20, 32768) == (1 << 20) * (32768 + 1024)
+    assert lib.clef_f8_prepared_bytes(1 << 20, 32768) == (1 << 20) * (32768 + 256 + 1024)
     assert lib.clef_f8_prepared_bytes(5, 130) == -1 and lib.clef_f8_prepared_bytes(5, 32776) == -1
     assert lib.clef_f8_weight_bytes(3, 136, 264) == 3 * 2 * 3 * 16384
     assert lib.clef_f8_weight_bytes(0, 136, 264) == -1 and lib.clef_f8_weight_bytes(1, 136, 0) == -1
     assert lib.clef_f8_project_workspace_bytes(0, 256, 256) == 0
-    assert lib.clef_f8_project_workspace_bytes(4096, 256, 264) == 4096 * (384 + 12)
+    assert lib.clef_f8_project_workspace_bytes(4096, 256, 264) == 4096 * (384 + 16 + 12)
     assert lib.clef_moe_group_slots_workspace_bytes(1 << 20, 16, 1024) > 0
     assert lib.clef_moe_group_slots_workspace_bytes(1, 8, 128) == 0
 
@@ -53,17 +54,17 @@ def test_weight_rejects(matrices, n, k):
 
 @pytest.mark.parametrize("m,n,k", [(-1, 128, 128), ((1 << 20) + 1, 128, 128), (4, 0, 128), (4, 100, 128), (4, 128, 12)])
 def test_products_reject(m, n, k):
-    assert call("clef_f8_gemm", FAKE, FAKE, FAKE, FAKE, m, n, k, 0, None, FAKE, None) == (-1, SHAPE)
-    assert call("clef_f8_gemm_gate_up", FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, m, n, k, 0, FAKE, None) == (-1, SHAPE)
+    assert call("clef_f8_gemm", FAKE, FAKE, FAKE, m, n, k, 0, None, FAKE, None) == (-1, SHAPE)
+    assert call("clef_f8_gemm_gate_up", FAKE, FAKE, FAKE, FAKE, FAKE, m, n, k, 0, FAKE, None) == (-1, SHAPE)
     assert call("clef_f8_project", FAKE, m, k, max(k, 16), FAKE, FAKE, n, 0, None, FAKE, FAKE, 1 << 40, None) == (-1, SHAPE)
 
 
 def test_products_pointers_workspace_and_no_rows():
-    assert call("clef_f8_gemm", None, None, None, None, 0, 128, 128, 1, None, None, None)[0] == 0
-    assert call("clef_f8_gemm_gate_up", *[None] * 6, 0, 128, 128, 1, None, None)[0] == 0
+    assert call("clef_f8_gemm", None, None, None, 0, 128, 128, 1, None, None, None)[0] == 0
+    assert call("clef_f8_gemm_gate_up", *[None] * 5, 0, 128, 128, 1, None, None)[0] == 0
     assert call("clef_f8_project", None, 0, 128, 128, None, None, 128, 1, None, None, None, 0, None)[0] == 0
-    good = [FAKE] * 4
-    for i in range(4):
+    good = [FAKE] * 3
+    for i in range(3):
         bad = list(good)
         bad[i] = FAKE + 4
         rc, msg = call("clef_f8_gemm", *bad, 4, 128, 128, 0, None, FAKE, None)
@@ -105,18 +106,18 @@ def test_group_slots_rejects():
 ])
 def test_experts_reject(a_rows, experts, total, topk, routed, k, n, message):
     rest = (FAKE, FAKE, experts, total, topk, routed, k, n, 0, FAKE, None)
-    assert call("clef_moe_expert_f8", FAKE, FAKE, a_rows, FAKE, FAKE, *rest) == (-1, message)
-    assert call("clef_moe_expert_gate_up_f8", FAKE, FAKE, a_rows, FAKE, FAKE, FAKE, FAKE, *rest) == (-1, message)
+    assert call("clef_moe_expert_f8", FAKE, a_rows, FAKE, FAKE, *rest) == (-1, message)
+    assert call("clef_moe_expert_gate_up_f8", FAKE, a_rows, FAKE, FAKE, FAKE, FAKE, *rest) == (-1, message)
 
 
 def test_experts_pointers_and_no_slots():
-    none = (None, None, 4, None, None, None, None, 8, 0, 2, 0, 128, 128, 1, None, None)
+    none = (None, 4, None, None, None, None, 8, 0, 2, 0, 128, 128, 1, None, None)
     assert call("clef_moe_expert_f8", *none)[0] == 0
-    rc, msg = call("clef_moe_expert_f8", FAKE, FAKE, 4, FAKE, FAKE, None, FAKE, 8, 8, 2, 0, 128, 128, 0, FAKE, None)
+    rc, msg = call("clef_moe_expert_f8", FAKE, 4, FAKE, FAKE, None, FAKE, 8, 8, 2, 0, 128, 128, 0, FAKE, None)
     assert rc == -1 and "list pointer" in msg
-    rc, msg = call("clef_moe_expert_f8", FAKE, FAKE, 4, FAKE, FAKE, FAKE, FAKE + 2, 8, 8, 2, 0, 128, 128, 0, FAKE, None)
+    rc, msg = call("clef_moe_expert_f8", FAKE, 4, FAKE, FAKE, FAKE, FAKE + 2, 8, 8, 2, 0, 128, 128, 0, FAKE, None)
     assert rc == -1 and "list pointer" in msg
-    rc, msg = call("clef_moe_expert_f8", FAKE, FAKE, 4, FAKE, None, FAKE, FAKE, 8, 8, 2, 0, 128, 128, 0, FAKE, None)
+    rc, msg = call("clef_moe_expert_f8", FAKE, 4, FAKE, None, FAKE, FAKE, 8, 8, 2, 0, 128, 128, 0, FAKE, None)
     assert rc == -1 and "aligned" in msg
 
 

@@ -113,6 +113,9 @@ def test_prepare_matches_definition(rows, width):
     codes, scales = quantize64(x)
     assert torch.equal(a.codes.cpu().double(), codes)
     assert torch.equal(a.scales.cpu().double(), scales)
+    blocks = -(-width // 128)
+    exps = a.storage[rows * a.pitch:].view(-1)[: rows * (-(-blocks // 16) * 16)].view(rows, -(-blocks // 16) * 16)
+    assert torch.equal(torch.ldexp(torch.ones((), dtype=torch.float64), exps[:, :blocks].cpu().int() - 127), scales)
     pad = a.storage[: rows * a.pitch].view(rows, a.pitch)[:, width:]
     assert (pad == 0).all()
 
