@@ -910,8 +910,7 @@ class PreparedF8:
     @property
     def codes(self) -> torch.Tensor:
         """float8_e4m3fn [rows][width], a view."""
-        codes = self.storage[: self.rows * self.pitch].view(torch.float8_e4m3fn)
-        return codes.view(self.rows, self.pitch)[:, : self.width]
+        return self.storage.view(torch.float8_e4m3fn).as_strided((self.rows, self.width), (self.pitch, 1))
 
     @property
     def _scales_at(self) -> int:
@@ -920,9 +919,10 @@ class PreparedF8:
     @property
     def scales(self) -> torch.Tensor:
         """f32 [rows][ceil(width / 128)], a view."""
-        start = self._scales_at
-        scales = self.storage[start: start + self.rows * self.pitch // 32].view(torch.float32)
-        return scales.view(self.pitch // 128, self.rows).t()
+        words = self.storage.numel() // 4 * 4
+        held = self.storage if words == self.storage.numel() else self.storage[:words]
+        return held.view(torch.float32).as_strided((self.rows, self.pitch // 128), (1, max(self.rows, 1)),
+                                                   self._scales_at // 4)
 
     def call_arg(self) -> torch.Tensor:
         """The buffer, as large as its rows need."""

@@ -15,6 +15,10 @@ namespace clef {
 
 namespace {
 
+// Rows that a split-k workgroup quantizes itself: as many values as its threads
+// take in kQxPasses passes of 8.
+constexpr int kQxPasses = 4, kQxValues = 512 * 8 * kQxPasses;
+
 // Few rows: each workgroup owns 16 MT rows x 16 NT weight rows (gate/up: NT / 2
 // fragments of gate rows and the same of up), its eight waves split the
 // blocks of k (wave w: blocks w, w + 8, ..). Operands go straight into
@@ -22,11 +26,16 @@ namespace {
 // used by this workgroup's rows only, so LDS would add a trip and nothing
 // else. D blocks are in flight per wave. The waves' sums meet in LDS and are
 // added in wave order (the result does not depend on timing).
-template <int MT, int NT, int D, bool LISTS, bool GU, bool RESID>
+//
+// QX: the rows come in bf16 (p.x) and every workgroup quantizes them into LDS
+// first, by the quantizer's rule, while its first weights are on their way:
+// for the few rows where that is shorter than a launch (f8_project_fusable).
+template <int MT, int NT, int D, bool QX, bool LISTS, bool GU, bool RESID>
 __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int NW = 8, BM = 16 * MT, COLS = 16 * NT / (GU ? 2 : 1), NG = GU ? NT / 2 : NT;
   static_assert(!GU || NT % 2 == 0, "gate and up fragments");
+  static_assert(!QX || (MT == 1 && !LISTS && !GU), "rows quantized here");
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, g = lane >> 4;
@@ -78,6 +87,19 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
   const float* wsp[2] = {p.ws + panel, GU ? p.ws2 + panel : nullptr};
   constexpr int MATS = GU ? 2 : 1;
 
+  // QX: codes [rows][pitch] and scales [rows][kb] behind the waves' sums
+  char* const q_codes = lds + NW * MT * NT * 1024;
+  float* const q_scales = reinterpret_cast<float*>(q_codes + p.rows * pitch);
+  uint4 xv[kQxPasses];
+  if constexpr (QX) {
+#pragma unroll
+    for (int s = 0; s < kQxPasses; ++s) {
+      const int c = threadIdx.x + s * 512, per = pitch / 8, row = c / per, col = (c - row * per) * 8;
+      xv[s] = uint4{0, 0, 0, 0};
+      if (row < here && col < p.k) xv[s] = *reinterpret_cast<const uint4*>(p.x + row * p.x_stride + col);
+    }
+  }
+
   struct Block {
     v4i w[NT][2], a[MT][2];
     float sa[MT], sw[MATS];
@@ -96,7 +118,7 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
         b.w[j][h] = __builtin_amdgcn_raw_buffer_load_b128(wr, w_voff + (j % NG) * 2048 + h * 1024, k * 16384, 0);
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int i = 0; i < (QX ? 0 : MT); ++i) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) b.a[i][h] = __builtin_amdgcn_raw_buffer_load_b128(ar, a_voff[i] + 64 * h, k * 128, 0);
       b.sa[i] = as_float(__builtin_amdgcn_raw_buffer_load_b32(sr, s_voff[i], (int)(k * p.rows * 4), 0));
@@ -112,10 +134,36 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
     for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0, 0, 0, 0};
 #pragma unroll
   for (int d = 0; d < D; ++d) load(buf[d], wave + NW * d);
+  if constexpr (QX) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int s = 0; s < kQxPasses; ++s) {
+      if (s * 512 * 8 >= here * pitch) break;
+      const int c = threadIdx.x + s * 512, per = pitch / 8, row = c / per, col = (c - row * per) * 8;
+      uint32_t m = f8_amax2(f8_amax2(f8_amax2(f8_amax2(0u, xv[s].x), xv[s].y), xv[s].z), xv[s].w);
+      m = group_max16(m);  // 16 lanes hold a block
+      const uint32_t field = f8_scale_field(m);
+      const float inv = as_float((254u - field) << 23);
+      if (row < here) {
+        *reinterpret_cast<uint2*>(q_codes + row * pitch + col) =
+            uint2{f8_codes(xv[s].x, xv[s].y, inv), f8_codes(xv[s].z, xv[s].w, inv)};
+        if (threadIdx.x % 16 == 0) q_scales[row * kb + col / 128] = as_float(field << 23);
+      }
+    }
+    __syncthreads();
+  }
   for (int k0 = wave; k0 < kb; k0 += NW * D) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
-      const Block& b = buf[d];
+      Block& b = buf[d];
+      if constexpr (QX) {
+        // (blocks past the end multiply zeros)
+        const int k = k0 + NW * d < kb ? k0 + NW * d : 0, row = lr < here ? lr : here - 1;
+        const char* at = q_codes + row * pitch + k * 128 + 16 * g;
+        b.a[0][0] = *reinterpret_cast<const v4i*>(at);
+        b.a[0][1] = *reinterpret_cast<const v4i*>(at + 64);
+        b.sa[0] = k0 + NW * d < kb ? q_scales[row * kb + k] : 0.0f;
+      }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const v8i_t av = join_halves(b.a[i][0], b.a[i][1]);
@@ -177,14 +225,16 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
 #endif
 }
 
-template <int MT, int NT, int D, bool LISTS, bool GU, bool RESID>
+template <int MT, int NT, int D, bool QX, bool LISTS, bool GU, bool RESID>
 hipError_t launch_stream(const F8Args& x, hipStream_t stream) {
-  constexpr int BM = 16 * MT, COLS = 16 * NT / (GU ? 2 : 1), lds = 8 * MT * NT * 1024;
+  constexpr int BM = 16 * MT, COLS = 16 * NT / (GU ? 2 : 1), sums = 8 * MT * NT * 1024;
   static_assert(128 % COLS == 0, "a tile's columns lie in one weight block");
+  static_assert(!QX || sums + kQxValues + kQxValues / 32 <= 64 * 1024, "LDS without raising the limit");
   static LaunchCache cache;
-  auto* kernel = &f8_stream_kernel<MT, NT, D, LISTS, GU, RESID>;
-  if (lds > 64 * 1024)
-    if (hipError_t e = ensure_dynamic_lds(cache, reinterpret_cast<const void*>(kernel), lds)) return e;
+  auto* kernel = &f8_stream_kernel<MT, NT, D, QX, LISTS, GU, RESID>;
+  if (sums > 64 * 1024)
+    if (hipError_t e = ensure_dynamic_lds(cache, reinterpret_cast<const void*>(kernel), sums)) return e;
+  const int lds = sums + (QX ? (int)x.rows * x.kb * 132 : 0);
   const int64_t tiles_m = LISTS ? f8_most_tiles(x.lists.total, x.lists.experts, BM) : (x.rows + BM - 1) / BM;
   if (tiles_m > 65535) return hipErrorInvalidValue;
   const dim3 grid((unsigned)((x.n + COLS - 1) / COLS), (unsigned)tiles_m);
@@ -612,14 +662,18 @@ hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
     const int64_t rows = x.lists.total / x.lists.experts;
     if (x.lists.total <= 16 || (rows < 8 && x.kb >= 16)) {
       if (f8_most_tiles(x.lists.total, x.lists.experts, 16) <= 65535)
-        return launch_stream<1, 4, 2, LISTS, GU, RESID>(x, stream);
+        return launch_stream<1, 4, 2, false, LISTS, GU, RESID>(x, stream);
     }
   } else {
+    if constexpr (!GU)
+      if (x.x != nullptr)  // f8_project_fusable
+        return tiles(16, 32) <= kCus || tiles(16, 64) > kCus ? launch_stream<1, 2, 2, true, false, false, RESID>(x, stream)
+                                                             : launch_stream<1, 4, 2, true, false, false, RESID>(x, stream);
     if (tiles(16, 32) <= kCus || (x.rows <= 16 && tiles(16, 64) > kCus))
-      return launch_stream<1, 2, 2, LISTS, GU, RESID>(x, stream);
-    if (tiles(16, 64) <= kCus) return launch_stream<1, 4, 2, LISTS, GU, RESID>(x, stream);
-    if (tiles(32, 64) <= kCus) return launch_stream<2, 4, 2, LISTS, GU, RESID>(x, stream);
-    if (tiles(64, 64) <= kCus) return launch_stream<4, 4, 1, LISTS, GU, RESID>(x, stream);
+      return launch_stream<1, 2, 2, false, LISTS, GU, RESID>(x, stream);
+    if (tiles(16, 64) <= kCus) return launch_stream<1, 4, 2, false, LISTS, GU, RESID>(x, stream);
+    if (tiles(32, 64) <= kCus) return launch_stream<2, 4, 2, false, LISTS, GU, RESID>(x, stream);
+    if (tiles(64, 64) <= kCus) return launch_stream<4, 4, 1, false, LISTS, GU, RESID>(x, stream);
   }
   const int64_t small = (tiles(128, 128) + kCus - 1) / kCus, large = (tiles(256, 256) + kCus - 1) / kCus;
   if (small >= 3 * large)
@@ -636,7 +690,7 @@ hipError_t launch_f8_gemm(const F8Args& x, bool gate_up, hipStream_t stream) {
   return x.residual ? launch_rows<false, false, true>(x, stream) : launch_rows<false, false, false>(x, stream);
 }
 
-bool f8_project_fusable(int64_t, int, int) { return false; }
+bool f8_project_fusable(int64_t m, int, int k) { return m <= 4 && m * f8_pitch(k) <= kQxValues; }
 
 hipError_t launch_f8_experts(const F8Args& x, bool gate_up, hipStream_t stream) {
   return gate_up ? launch_rows<true, true, false>(x, stream) : launch_rows<true, false, false>(x, stream);
