@@ -242,21 +242,23 @@ hipError_t launch_stream(const F8Args& x, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Tile shape of f8_tile_kernel: WAVES_M x WAVES_N waves of WM rows x WN weight
-// rows, NST LDS stages of one block of k each: A rows (128 bytes each, 16-byte
+// Tile shape of f8_tile_kernel: KG groups of WAVES_M x WAVES_N waves of WM rows x
+// WN weight rows, group g multiplying block g of each step's KG blocks of k; NST
+// LDS stages of one step each, for each block A rows (128 bytes each, 16-byte
 // chunk c of row r at c ^ ((r >> 1) & 7)) and B fragments in the operand order.
 // Behind the stages the rows' e8m0 scales of 16 blocks of k, as loaded (16 bytes
 // per row) and, twice, turned into the order of use (per block of k a lane's TM
 // rows side by side), the scales of the tile's one or two weight panels (256 f32
 // each) and, with lists, the tile's output rows.
-template <int WM_, int WN_, int WAVES_M_, int WAVES_N_, int NST_, int GROUPS_ = 1>
+template <int WM_, int WN_, int WAVES_M_, int WAVES_N_, int NST_, int GROUPS_ = 1, int KG_ = 1>
 struct F8Tile {
   static constexpr int GROUPS = GROUPS_;  // workgroups per CU
   static constexpr int WM = WM_, WN = WN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, NST = NST_;
-  static constexpr int NW = WAVES_M * WAVES_N, THREADS = 64 * NW;
+  static constexpr int KG = KG_, NWB = WAVES_M * WAVES_N, NW = NWB * KG, THREADS = 64 * NW;
   static constexpr int BM = WM * WAVES_M, BN = WN * WAVES_N;
   static constexpr int TM = WM / 16, TN = WN / 16;  // fragments per wave
-  static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int A_BLOCK = BM * 128, B_BLOCK = BN * 128;
+  static constexpr int A_BYTES = KG * A_BLOCK, B_BYTES = KG * B_BLOCK, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int A_SLOTS = A_BYTES / 1024 / NW, B_SLOTS = B_BYTES / 1024 / NW;
   // a wave's DMA instructions per stage: first (X) the weight fragments and the
   // rows of its first TM / 2 activation fragments, then (Y) the other rows
@@ -267,7 +269,8 @@ struct F8Tile {
   static constexpr int EPI = 16 * WN * 2;            // epilogue staging per wave
   static_assert(NW == 8 && (BN == 256 || BN == 128) && BM / 64 <= NW, "eight waves, one or two weight panels");
   static_assert(A_BYTES % (2048 * NW) == 0 && B_BYTES % (2048 * NW) == 0 && LDS <= 160 * 1024, "whole instructions per wave");
-  static_assert(TM * TN % 4 == 0 && TM % 4 == 0 && TN % 2 == 0 && (NST == 2 || NST == 4), "step");
+  static_assert(TM * TN % 4 == 0 && TM % 4 == 0 && TN % 2 == 0 && (NST == 2 || NST == 4) && TM % KG == 0, "step");
+  static_assert(NW * (TM - TM / KG) * TN * 1024 <= NST * STAGE_BYTES, "the groups' sums meet in the stages");
   static_assert(X <= TM / 2 * TN && Y <= TN, "one DMA instruction per MFMA behind each barrier");
 };
 
@@ -296,17 +299,20 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
   constexpr int TM = T::TM, TN = T::TN;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, g = lane >> 4;
-  const int wm = wave / T::WAVES_N, wn = wave % T::WAVES_N;
+  const int kg = T::KG == 1 ? 0 : wave / T::NWB, wb = wave % T::NWB;  // group, wave in it
+  const int wm = wb / T::WAVES_N, wn = wb % T::WAVES_N;
   const int kb = p.kb, pitch = kb * 128, kp = (kb + 15) / 16 * 16;
+  const int steps = (kb + T::KG - 1) / T::KG;
   int* out_rows = reinterpret_cast<int*>(lds + T::ROWS);
 
-  // this wave's DMA: A instruction s moves 8 rows, the first half of a wave's
-  // instructions rows of the first TM / 2 fragments of either row of waves
+  // this wave's DMA, of its group's blocks: A instruction s moves 8 rows, the
+  // first half of a wave's instructions rows of the first TM / 2 fragments of
+  // either row of waves
   int a_voff[T::A_SLOTS];
-  auto a_piece = [&](int s) {  // KiB of the stage
+  auto a_piece = [&](int s) {  // KiB of the block
     constexpr int H = T::A_SLOTS / 2;
     constexpr int PER = T::WM / 16;  // KiB of half of a row of waves' rows
-    const int hi = s >= H, q = wave * H + s % H;
+    const int hi = s >= H, q = wb * H + s % H;
     return q / PER * (2 * PER) + hi * PER + q % PER;
   };
   auto source_row = [&](int r) -> int64_t {  // row of a (dense: from m0); rows past the end repeat the last
@@ -328,8 +334,8 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
   // last column is empty
   constexpr int FRAGS = T::B_SLOTS / 2;
   const int nb = f8_blocks(p.n);
-  const bool up = GU && wave >= T::NW / 2;
-  const int frag = n0 / 16 + (up ? wave - T::NW / 2 : wave) * FRAGS, panel = frag / 8;
+  const bool up = GU && wb >= T::NWB / 2;
+  const int frag = n0 / 16 + (up ? wb - T::NWB / 2 : wb) * FRAGS, panel = frag / 8;
   const int64_t first_block = (int64_t)expert * nb * kb;
   const __amdgpu_buffer_rsrc_t b_rsrc = make_rsrc((up ? p.w2 : p.w) + (first_block + (int64_t)panel * kb) * 16384,
                                                   panel < nb ? (uint32_t)kb * 16384u : 0u);
@@ -374,24 +380,25 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
     }
   }
   const __amdgpu_buffer_rsrc_t none = make_rsrc(p.a, 0);
-  // DMA instruction x of stage kt into `stage`, X first (stages past the end:
+  // DMA instruction x of step kt into `stage`, X first (stages past the end:
   // zeros that nothing reads, so that every step issues and waits alike)
   auto issue = [&](char* stage, int kt, int x) {
-    const bool in = kt < kb;
-    const int k = in ? kt : 0;
+    const int block = T::KG * kt + kg;
+    const bool in = block < kb;
+    const int k = in ? block : 0;
     if (x < T::B_SLOTS)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? b_rsrc : none,
                                                (lds_ptr_t)(stage + T::A_BYTES + (T::B_SLOTS * wave + x) * 1024), 16,
                                                b_voff, k * 16384 + x * 1024, 0, 0);
     else
       __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? a_rsrc : none,
-                                               (lds_ptr_t)(stage + a_piece(x - T::B_SLOTS) * 1024), 16,
+                                               (lds_ptr_t)(stage + kg * T::A_BLOCK + a_piece(x - T::B_SLOTS) * 1024), 16,
                                                a_voff[x - T::B_SLOTS], k * 128, 0, 0);
   };
 
   // a fragment's two halves in a stage
-  const int a_at0 = (wm * T::WM + lr) * 128 + ((g ^ (lr >> 1)) << 4), a_at1 = a_at0 ^ 64;
-  const int b_at = T::A_BYTES + (GU ? wn * (TN / 2) : wn * TN) * 2048 + lane * 16;
+  const int a_at0 = kg * T::A_BLOCK + (wm * T::WM + lr) * 128 + ((g ^ (lr >> 1)) << 4), a_at1 = a_at0 ^ 64;
+  const int b_at = T::A_BYTES + kg * T::B_BLOCK + (GU ? wn * (TN / 2) : wn * TN) * 2048 + lane * 16;
   const char* const sa_at = lds + T::ST + wm * T::WM + lr * TM;
   const float* const sw_at = reinterpret_cast<const float*>(lds + T::SW) + (GU ? 0 : wn * T::WN / 128) * 256;
 
@@ -413,15 +420,16 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
       return join_halves(lo, hi);
     };
     auto read_b = [&](const char* stage, int j) {
-      const char* at = stage + b_at + (GU && j >= TN / 2 ? T::B_BYTES / 2 + (j - TN / 2) * 2048 : j * 2048);
+      const char* at = stage + b_at + (GU && j >= TN / 2 ? T::B_BLOCK / 2 + (j - TN / 2) * 2048 : j * 2048);
       return join_halves(*reinterpret_cast<const v4i*>(at), *reinterpret_cast<const v4i*>(at + 1024));
     };
     float sw[MATS];
     // of step kt (the step before still takes sa)
     auto read_scales = [&](int kt) {
+      const int block = T::KG * kt + kg;  // (a block past the last: its products are zeros)
 #pragma unroll
-      for (int t = 0; t < MATS; ++t) sw[t] = sw_at[t * 256 + (kt < kb ? kt : 0)];
-      const char* at = sa_at + (kt >> 4 & 1) * T::SA_BYTES + (kt & 15) * T::BM;
+      for (int t = 0; t < MATS; ++t) sw[t] = sw_at[t * 256 + (block < kb ? block : 0)];
+      const char* at = sa_at + (block >> 4 & 1) * T::SA_BYTES + (block & 15) * T::BM;
       typedef uint32_t pack __attribute__((ext_vector_type(TM / 4)));
       const pack v = *reinterpret_cast<const pack*>(at);
 #pragma unroll
@@ -511,26 +519,30 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
 #pragma unroll
       for (int t = 0; t < MATS; ++t) sv[t] = 0.0f;
     }
-    // The scales of the next 16 blocks of k are loaded under 8 steps and turned
-    // before the other 8 (a branch inside a step instead made the compiler spill).
-    for (int k0 = 0; k0 < kb; k0 += 8) {
-      if ((k0 | 8) + 8 < kb) {
-        if (k0 & 8) {
+    // The scales of the next 16 blocks of k are loaded in the first half of these
+    // and turned before the second (a branch inside a step instead made the
+    // compiler spill).
+    constexpr int HALF_STEPS = 8 / T::KG;
+    for (int k0 = 0; k0 < steps; k0 += HALF_STEPS) {
+      const bool second = k0 & HALF_STEPS;
+      const int next = (k0 / (2 * HALF_STEPS) + 1) * 2 * HALF_STEPS;  // first step of the next 16 blocks
+      if (next < steps) {
+        if (second) {
           wait_vmcnt<T::NST * T::DMA>();
-          turn_scales(k0 / 16 + 1);
+          turn_scales(next / (2 * HALF_STEPS));
         } else {
-          issue_scales(k0 / 16 + 1);
+          issue_scales(next / (2 * HALF_STEPS));
         }
       }
-      const int k1 = k0 + 8 < kb ? k0 + 8 : kb;
+      const int k1 = k0 + HALF_STEPS < steps ? k0 + HALF_STEPS : steps;
       for (int kt = k0; kt < k1; kt += T::NST) {
         step(r0, r1, kt);
         if constexpr (T::NST == 2) {
-          if (kt + 1 < kb) step(r1, r0, kt + 1);
+          if (kt + 1 < steps) step(r1, r0, kt + 1);
         } else {
-          if (kt + 1 < kb) step(r1, r2, kt + 1);
-          if (kt + 2 < kb) step(r2, r3, kt + 2);
-          if (kt + 3 < kb) step(r3, r0, kt + 3);
+          if (kt + 1 < steps) step(r1, r2, kt + 1);
+          if (kt + 2 < steps) step(r2, r3, kt + 2);
+          if (kt + 3 < steps) step(r3, r0, kt + 3);
         }
       }
     }
@@ -545,32 +557,62 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
   // epilogue: 16 rows at a time through the wave's own LDS (16-byte chunk c of
   // row r at c ^ (r & 7)), stored as 16-byte pieces of whole row segments; the
   // residual's loads all go out first
-  uint2 res[RESID ? TM : 1][RESID ? TN : 1];
+  constexpr int EM = TM / T::KG;  // rows of fragments that this wave stores, from fragment kg EM
+  const int w0 = wm * T::WM + kg * EM * 16;
+  uint2 res[RESID ? EM : 1][RESID ? TN : 1];
   if constexpr (RESID) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int i = 0; i < EM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
-        const int r = wm * T::WM + 16 * i + lr, col = n0 + wn * T::WN + 16 * j + 4 * g;
+        const int r = w0 + 16 * i + lr, col = n0 + wn * T::WN + 16 * j + 4 * g;
         res[i][j] = uint2{0, 0};
         if (r < here && col < p.n) res[i][j] = *reinterpret_cast<const uint2*>(p.residual + (m0 + r) * p.n + col);
       }
   }
   wait_vmcnt<0>();
   __syncthreads();
+  v4f sum[EM][TN];
+  if constexpr (T::KG == 1) {
+#pragma unroll
+    for (int i = 0; i < EM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) sum[i][j] = acc[i][j];
+  } else {
+    // two groups: each gives the other its part of the rows that the other stores
+    static_assert(T::KG <= 2, "a pair of groups");
+    v4f* const mine = reinterpret_cast<v4f*>(lds) + wave * (EM * TN * 64) + lane;
+    const v4f* const theirs = reinterpret_cast<v4f*>(lds) + (wave ^ T::NWB) * (EM * TN * 64) + lane;
+#pragma unroll
+    for (int i = 0; i < EM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sum[i][j][t] = kg ? acc[i][j][t] : acc[EM + i][j][t];
+        mine[(i * TN + j) * 64] = sum[i][j];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sum[i][j][t] = kg ? acc[EM + i][j][t] : acc[i][j][t];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) sum[i][j] += theirs[(i * TN + j) * 64];
+    __syncthreads();
+  }
   constexpr int WC = GU ? T::WN / 2 : T::WN, ROW = WC * 2, CH = WC / 8;  // columns, bytes, chunks of a row
   constexpr int PER = 64 / CH;                                           // rows per store
   char* own = lds + wave * T::EPI;
   const int c0 = n0 + wn * WC;
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int r0 = wm * T::WM + 16 * i;
+  for (int i = 0; i < EM; ++i) {
+    const int r0 = w0 + 16 * i;
 #pragma unroll
     for (int j = 0; j < (GU ? TN / 2 : TN); ++j) {
-      v4f y = acc[i][j];
+      v4f y = sum[i][j];
       if constexpr (GU) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) y[t] = f8_swiglu(y[t], acc[i][j + TN / 2][t]);
+        for (int t = 0; t < 4; ++t) y[t] = f8_swiglu(y[t], sum[i][j + TN / 2][t]);
       }
       if constexpr (RESID) {
         y[0] += bf16_lo(res[i][j].x);
@@ -636,6 +678,7 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
 using F8Tile256 = F8Tile<128, 64, 2, 4, 2>;     // 256 x 256
 using F8Tile256H = F8Tile<64, 64, 2, 4, 2>;     // 128 x 256
 using F8Tile128 = F8Tile<64, 32, 2, 4, 2, 2>;   // 128 x 128, two workgroups per CU
+using F8Tile128K = F8Tile<64, 64, 2, 2, 2, 1, 2>;  // 128 x 128, two blocks of k at a time
 
 template <class T, class HALF, bool HW, bool LISTS, bool GU, bool RESID>
 hipError_t launch_tile(const F8Args& x, hipStream_t stream) {
@@ -703,6 +746,13 @@ hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
   if (small >= 3 * large)
     return x.pow2 ? launch_tile<F8Tile256, F8Tile256H, true, LISTS, GU, RESID>(x, stream)
                   : launch_tile<F8Tile256, F8Tile256H, false, LISTS, GU, RESID>(x, stream);
+  // One tile per CU with f32 scales: two blocks of k at a time on two groups of
+  // waves, which read less LDS per MFMA (620 x 17408 x 5120 82 -> 74 us, 512 x 4096
+  // x 4096 19.1 -> 17.3; 768 x 512 x 4096, 4 blocks of k, 6.0 -> 7.0; with
+  // power-of-two scales no gain: 15.9 and 15.9 at 512 x 4096 x 4096).
+  if constexpr (!LISTS)
+    if (small <= 1 && !x.pow2 && x.kb >= 16)
+      return launch_tile<F8Tile128K, F8Tile128K, false, LISTS, GU, RESID>(x, stream);
   return x.pow2 ? launch_tile<F8Tile128, F8Tile128, true, LISTS, GU, RESID>(x, stream)
                 : launch_tile<F8Tile128, F8Tile128, false, LISTS, GU, RESID>(x, stream);
 }
