@@ -243,17 +243,18 @@ hipError_t launch_stream(const F8Args& x, hipStream_t stream) {
 }
 
 // Tile shape of f8_tile_kernel: KG groups of WAVES_M x WAVES_N waves of WM rows x
-// WN weight rows, group g multiplying block g of each step's KG blocks of k; NST
+// WN weight rows, group g multiplying block g of each step's KG blocks of k; two
 // LDS stages of one step each, for each block A rows (128 bytes each, 16-byte
 // chunk c of row r at c ^ ((r >> 1) & 7)) and B fragments in the operand order.
 // Behind the stages the rows' e8m0 scales of 16 blocks of k, as loaded (16 bytes
 // per row) and, twice, turned into the order of use (per block of k a lane's TM
 // rows side by side), the scales of the tile's one or two weight panels (256 f32
 // each) and, with lists, the tile's output rows.
-template <int WM_, int WN_, int WAVES_M_, int WAVES_N_, int NST_, int GROUPS_ = 1, int KG_ = 1>
+template <int WM_, int WN_, int WAVES_M_, int WAVES_N_, int GROUPS_ = 1, int KG_ = 1>
 struct F8Tile {
   static constexpr int GROUPS = GROUPS_;  // workgroups per CU
-  static constexpr int WM = WM_, WN = WN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, NST = NST_;
+  static constexpr int WM = WM_, WN = WN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_;
+  static constexpr int NST = 2;  // LDS stages
   static constexpr int KG = KG_, NWB = WAVES_M * WAVES_N, NW = NWB * KG, THREADS = 64 * NW;
   static constexpr int BM = WM * WAVES_M, BN = WN * WAVES_N;
   static constexpr int TM = WM / 16, TN = WN / 16;  // fragments per wave
@@ -269,7 +270,7 @@ struct F8Tile {
   static constexpr int EPI = 16 * WN * 2;            // epilogue staging per wave
   static_assert(NW == 8 && (BN == 256 || BN == 128) && BM / 64 <= NW, "eight waves, one or two weight panels");
   static_assert(A_BYTES % (2048 * NW) == 0 && B_BYTES % (2048 * NW) == 0 && LDS <= 160 * 1024, "whole instructions per wave");
-  static_assert(TM * TN % 4 == 0 && TM % 4 == 0 && TN % 2 == 0 && (NST == 2 || NST == 4) && TM % KG == 0, "step");
+  static_assert(TM * TN % 4 == 0 && TM % 4 == 0 && TN % 2 == 0 && TM % KG == 0, "step");
   static_assert(NW * (TM - TM / KG) * TN * 1024 <= NST * STAGE_BYTES, "the groups' sums meet in the stages");
   static_assert(X <= TM / 2 * TN && Y <= TN, "one DMA instruction per MFMA behind each barrier");
 };
@@ -286,11 +287,12 @@ struct F8Tile {
 //
 // A stage of LDS is filled in two parts: X (weights, scales, the first half of
 // each wave's activation rows) and Y (the other half). Behind a barrier in the
-// middle of a step X has been read by every wave and is loaded for NST steps
+// middle of a step X has been read by every wave and is loaded for two steps
 // on, behind one before the step's last row of MFMAs the same goes for Y; each
 // barrier also waits for the part that the MFMAs behind it read. So every load
-// has NST - 1/2 steps to land, where loading a stage as a whole behind one
-// barrier left NST - 1, with one DMA instruction per MFMA.
+// has a step and a half to land, where loading a stage as a whole behind one
+// barrier left one, with one DMA instruction per MFMA or less (all of them at
+// once: 4 % slower). Four stages gained nothing on 128 x 128 tiles.
 //
 // The tile: `here` rows from m0 (lists: the expert's, from place first) and COLS
 // columns from n0.
@@ -304,6 +306,31 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
   const int kb = p.kb, pitch = kb * 128, kp = (kb + 15) / 16 * 16;
   const int steps = (kb + T::KG - 1) / T::KG;
   int* out_rows = reinterpret_cast<int*>(lds + T::ROWS);
+
+  // B: this wave's weight fragments, consecutive ones of one panel (gate/up: the
+  // first half of the waves the gate's, the second the up's); a panel past the
+  // last column is empty
+  constexpr int FRAGS = T::B_SLOTS / 2;
+  const int nb = f8_blocks(p.n);
+  const bool up = GU && wb >= T::NWB / 2;
+  const int frag = n0 / 16 + (up ? wb - T::NWB / 2 : wb) * FRAGS, panel = frag / 8;
+  const int64_t first_block = (int64_t)expert * nb * kb;
+  const __amdgpu_buffer_rsrc_t b_rsrc = make_rsrc((up ? p.w2 : p.w) + (first_block + (int64_t)panel * kb) * 16384,
+                                                  panel < nb ? (uint32_t)kb * 16384u : 0u);
+  const int b_voff = frag % 8 * 2048 + lane * 16;
+  const __amdgpu_buffer_rsrc_t none = make_rsrc(p.a, 0);
+  auto issue_b = [&](char* stage, int kt, int x) {
+    const int block = T::KG * kt + kg;
+    const bool in = block < kb;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? b_rsrc : none,
+                                             (lds_ptr_t)(stage + T::A_BYTES + (T::B_SLOTS * wave + x) * 1024), 16, b_voff,
+                                             (in ? block : 0) * 16384 + x * 1024, 0, 0);
+  };
+  // the first weights, before the rows are known (lists: two loads later)
+#pragma unroll
+  for (int x = 0; x < T::B_SLOTS; ++x) issue_b(lds, 0, x);
+#pragma unroll
+  for (int x = 0; x < T::B_SLOTS; ++x) issue_b(lds + T::STAGE_BYTES, 1, x);
 
   // this wave's DMA, of its group's blocks: A instruction s moves 8 rows, the
   // first half of a wave's instructions rows of the first TM / 2 fragments of
@@ -329,17 +356,6 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
   }
   const __amdgpu_buffer_rsrc_t a_rsrc =
       make_rsrc(p.a + (LISTS ? 0 : m0 * pitch), (uint32_t)(LISTS ? p.rows * pitch : (int64_t)here * pitch));
-  // B: this wave's weight fragments, consecutive ones of one panel (gate/up: the
-  // first half of the waves the gate's, the second the up's); a panel past the
-  // last column is empty
-  constexpr int FRAGS = T::B_SLOTS / 2;
-  const int nb = f8_blocks(p.n);
-  const bool up = GU && wb >= T::NWB / 2;
-  const int frag = n0 / 16 + (up ? wb - T::NWB / 2 : wb) * FRAGS, panel = frag / 8;
-  const int64_t first_block = (int64_t)expert * nb * kb;
-  const __amdgpu_buffer_rsrc_t b_rsrc = make_rsrc((up ? p.w2 : p.w) + (first_block + (int64_t)panel * kb) * 16384,
-                                                  panel < nb ? (uint32_t)kb * 16384u : 0u);
-  const int b_voff = frag % 8 * 2048 + lane * 16;
   // scales: of the rows, 16 blocks of k at a time by the first BM / 64 waves
   const __amdgpu_buffer_rsrc_t s_rsrc =
       make_rsrc(p.ae + m0 * kp, (uint32_t)(LISTS ? p.rows * kp : (int64_t)here * kp));
@@ -379,7 +395,6 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
       out_rows[r] = slot;
     }
   }
-  const __amdgpu_buffer_rsrc_t none = make_rsrc(p.a, 0);
   // DMA instruction x of step kt into `stage`, X first (stages past the end:
   // zeros that nothing reads, so that every step issues and waits alike)
   auto issue = [&](char* stage, int kt, int x) {
@@ -387,9 +402,7 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
     const bool in = block < kb;
     const int k = in ? block : 0;
     if (x < T::B_SLOTS)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? b_rsrc : none,
-                                               (lds_ptr_t)(stage + T::A_BYTES + (T::B_SLOTS * wave + x) * 1024), 16,
-                                               b_voff, k * 16384 + x * 1024, 0, 0);
+      issue_b(stage, kt, x);
     else
       __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? a_rsrc : none,
                                                (lds_ptr_t)(stage + kg * T::A_BLOCK + a_piece(x - T::B_SLOTS) * 1024), 16,
@@ -407,7 +420,7 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
-  auto body = [&](char* __restrict__ r0, char* __restrict__ r1, char* __restrict__ r2, char* __restrict__ r3) {
+  auto body = [&](char* __restrict__ r0, char* __restrict__ r1) {
     constexpr int MATS = GU ? 2 : 1;
     v8i_t av[2], bv[TN];
     v4f part[4];               // !HW: partial sums on their way
@@ -447,9 +460,9 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
 #pragma unroll
       for (int t = 0; t < 4; ++t) c[t] = __builtin_fmaf(v[t], s, c[t]);
     };
-    // at most (NST - 1) stages' DMA behind what is waited for
+    // at most one stage's DMA behind what is waited for
     auto landed = [&]() {
-      wait_vmcnt<(T::NST - 1) * T::DMA>();
+      wait_vmcnt<T::DMA>();
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
     };
@@ -498,14 +511,15 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
       }
       take_scales();
     };
-    char* const ring[4] = {r0, r1, r2, r3};
+    // the weights of both stages are on their way; then the first scales (turned
+    // once they have landed) and the rows
 #pragma unroll
-    for (int n = 0; n < T::NST; ++n)
+    for (int x = T::B_SLOTS; x < T::DMA; ++x) issue(r0, 0, x);
 #pragma unroll
-      for (int x = 0; x < T::DMA; ++x) issue(ring[n], n, x);
-    wait_vmcnt<T::NST * T::DMA>();  // the first scales were issued before
+    for (int x = T::B_SLOTS; x < T::DMA; ++x) issue(r1, 1, x);
+    wait_vmcnt<2 * T::A_SLOTS>();
     turn_scales(0);
-    wait_vmcnt<T::NST * T::DMA - T::X>();
+    wait_vmcnt<T::A_SLOTS>();
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     read_scales(0);
@@ -537,13 +551,7 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
       const int k1 = k0 + HALF_STEPS < steps ? k0 + HALF_STEPS : steps;
       for (int kt = k0; kt < k1; kt += T::NST) {
         step(r0, r1, kt);
-        if constexpr (T::NST == 2) {
-          if (kt + 1 < steps) step(r1, r0, kt + 1);
-        } else {
-          if (kt + 1 < steps) step(r1, r2, kt + 1);
-          if (kt + 2 < steps) step(r2, r3, kt + 2);
-          if (kt + 3 < steps) step(r3, r0, kt + 3);
-        }
+        if (kt + 1 < steps) step(r1, r0, kt + 1);
       }
     }
     if constexpr (!HW) {
@@ -552,7 +560,7 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
       add(acc[TM - 1][TN - 1], part[3], sv[GU ? 1 : 0]);
     }
   };
-  body(lds, lds + T::STAGE_BYTES, lds + 2 % T::NST * T::STAGE_BYTES, lds + 3 % T::NST * T::STAGE_BYTES);
+  body(lds, lds + T::STAGE_BYTES);
 
   // epilogue: 16 rows at a time through the wave's own LDS (16-byte chunk c of
   // row r at c ^ (r & 7)), stored as 16-byte pieces of whole row segments; the
@@ -675,10 +683,10 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
 #endif
 }
 
-using F8Tile256 = F8Tile<128, 64, 2, 4, 2>;     // 256 x 256
-using F8Tile256H = F8Tile<64, 64, 2, 4, 2>;     // 128 x 256
-using F8Tile128 = F8Tile<64, 32, 2, 4, 2, 2>;   // 128 x 128, two workgroups per CU
-using F8Tile128K = F8Tile<64, 64, 2, 2, 2, 1, 2>;  // 128 x 128, two blocks of k at a time
+using F8Tile256 = F8Tile<128, 64, 2, 4>;           // 256 x 256
+using F8Tile256H = F8Tile<64, 64, 2, 4>;           // 128 x 256
+using F8Tile128 = F8Tile<64, 32, 2, 4, 2>;         // 128 x 128, two workgroups per CU
+using F8Tile128K = F8Tile<64, 64, 2, 2, 1, 2>;     // 128 x 128, two blocks of k at a time
 
 template <class T, class HALF, bool HW, bool LISTS, bool GU, bool RESID>
 hipError_t launch_tile(const F8Args& x, hipStream_t stream) {
