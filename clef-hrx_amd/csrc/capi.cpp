@@ -828,6 +828,7 @@ int clef_moe_layer_static(const uint16_t* x, const void* logits, int32_t logits_
 namespace {
 
 constexpr const char* kF8Shape = "unsupported FP8 block shape";
+constexpr const char* kF8Overlap = "FP8 output overlaps its input rows";
 constexpr int32_t kF8Widest = 32768, kF8MostRows = 1048576, kF8MostExperts = 1024;
 
 bool f8_width(int32_t v) { return v >= 8 && v <= kF8Widest && v % 8 == 0; }
@@ -950,7 +951,9 @@ int clef_f8_project(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, c
   if (!aligned(x, 16) || !aligned(w, 16) || !aligned(w_scales, 16) || !aligned(out, 16) ||
       (residual && !aligned(residual, 16)))
     return fail(kAlign);
+  const bool apart = !overlap(x, (size_t)((m - 1) * x_stride + k) * 2, out, (size_t)m * n * 2);
   if (clef::f8_project_fusable(m, n, k)) {
+    if (!apart) return fail(kF8Overlap);
     clef::F8Args y{};
     y.x = x, y.x_stride = x_stride, y.k = k, y.rows = m, y.w = w, y.ws = w_scales, y.n = n;
     y.kb = clef::f8_blocks(k), y.pow2 = pow2 != 0, y.residual = residual, y.out = out;
@@ -958,10 +961,10 @@ int clef_f8_project(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, c
   }
   if (!aligned(workspace, 16)) return fail(kAlign);
   if (workspace_bytes < clef_f8_project_workspace_bytes(m, n, k)) return fail(kWorkspace);
+  if (!apart) return fail(kF8Overlap);
   uint8_t* a = static_cast<uint8_t*>(workspace);
   if (int rc = clef_f8_prepare(x, m, k, x_stride, a, stream)) return rc;
-  return clef_f8_gemm(a, w, w_scales, m, n, k, pow2, residual,
-                      out, stream);
+  return clef_f8_gemm(a, w, w_scales, m, n, k, pow2, residual, out, stream);
 }
 
 size_t clef_moe_group_slots_workspace_bytes(int64_t tokens, int32_t topk, int32_t experts) {

@@ -139,21 +139,40 @@ __device__ __forceinline__ uint32_t f8_scale_field(uint32_t amax_bits) {
   return (uint32_t)(f > 1 ? f : 1);
 }
 
-// Four e4m3 codes of two bf16 pairs times `inv` (a power of two: exact), each
-// rounded to nearest even once. |value| <= 448 by the choice of the scale;
-// infinities are made NaN, which e4m3 has (0x7F) where it has no infinity.
-__device__ __forceinline__ uint32_t f8_codes(uint32_t p0, uint32_t p1, float inv) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(p0) * inv, bf16_hi(p0) * inv, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(p1) * inv, bf16_hi(p1) * inv, w, true);
+// Eight e4m3 codes of bf16 values over `scale` (a power of two: exact), each
+// rounded to nearest even once. |value| <= 448 scale by the choice of the scale;
+// infinities and NaN become NaN (0x7F; e4m3 has no infinity).
+__device__ __forceinline__ uint2 f8_codes8(uint4 v, float scale) {
+  using s2 = __attribute__((ext_vector_type(2))) short;
+  using b2 = __attribute__((ext_vector_type(2))) __bf16;
+  auto two = [&](uint32_t lo, uint32_t hi) {
+    s2 w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(s2{0, 0}, __builtin_bit_cast(b2, lo), scale, false);
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(b2, hi), scale, true));
+  };
+  return uint2{two(v.x, v.y), two(v.z, v.w)};
 }
 
-// The largest finite magnitude of a bf16 pair against the halves of `m`, as
-// bf16 bits; non-finite values count as zero (they stay NaN in the codes).
-__device__ __forceinline__ uint32_t f8_amax2(uint32_t m, uint32_t pair) {
-  const uint32_t lo = pair & 0x7FFFu, hi = (pair >> 16) & 0x7FFFu;
-  const uint32_t a = lo < 0x7F80u ? lo : 0u, b = hi < 0x7F80u ? hi : 0u;
-  const uint32_t c = a > b ? a : b;
-  return m > c ? m : c;
+// The largest magnitude of eight bf16 values as bf16 bits, infinities and NaN
+// above 0x7F7F (two 16-bit maxima per instruction); FINITE: those as zero.
+template <bool FINITE>
+__device__ __forceinline__ uint32_t f8_amax8(uint4 v) {
+  using u2 = __attribute__((ext_vector_type(2))) unsigned short;
+  auto mag = [](uint32_t p) {
+    u2 m = __builtin_bit_cast(u2, p & 0x7FFF7FFFu);
+    if (FINITE) m = u2{m[0] < 0x7F80 ? m[0] : (unsigned short)0, m[1] < 0x7F80 ? m[1] : (unsigned short)0};
+    return m;
+  };
+  const u2 m = __builtin_elementwise_max(__builtin_elementwise_max(mag(v.x), mag(v.y)),
+                                         __builtin_elementwise_max(mag(v.z), mag(v.w)));
+  return m[0] > m[1] ? m[0] : m[1];
+}
+
+// The largest finite magnitude of the values that 16 lanes hold, 8 each, as bf16
+// bits (non-finite ones stay NaN in the codes). Every lane of the wave is here.
+__device__ __forceinline__ uint32_t f8_block_amax(uint4 v) {
+  uint32_t m = group_max16(f8_amax8<false>(v));
+  if (__builtin_expect(__any(m >= 0x7F80u), 0)) m = group_max16(f8_amax8<true>(v));
+  return m;
 }
 
 // Inclusive sum over the wave's lanes (DPP: shifts within the rows of 16, then

@@ -15,9 +15,13 @@ namespace clef {
 
 namespace {
 
-// Rows that a split-k workgroup quantizes itself: as many values as its threads
-// take in kQxPasses passes of 8.
-constexpr int kQxPasses = 4, kQxValues = 512 * 8 * kQxPasses;
+// The most values of a tile's rows that a split-k workgroup quantizes itself: ten
+// passes of its threads, 0.3 us each (instructions, and loads of rows that every
+// workgroup reads), against the quantizer's launch (m x k x n, us for both ways:
+// 64 x 512 x 2048 3.6 and 5.1, 8 x 4096 x 2048 5.9 and 7.0, 16 x 2560 x 2048 6.4
+// and 6.8, twelve passes 12 x 4096 x 2048 7.2 and 7.4, 6 x 8192 x 8192 15.2 and
+// 14.3) and the 4 us that its call takes the host.
+constexpr int kQxValues = 10 * 512 * 8;
 
 // Few rows: each workgroup owns 16 MT rows x 16 NT weight rows (gate/up: NT / 2
 // fragments of gate rows and the same of up), its eight waves split the
@@ -27,15 +31,14 @@ constexpr int kQxPasses = 4, kQxValues = 512 * 8 * kQxPasses;
 // else. D blocks are in flight per wave. The waves' sums meet in LDS and are
 // added in wave order (the result does not depend on timing).
 //
-// QX: the rows come in bf16 (p.x) and every workgroup quantizes them into LDS
-// first, by the quantizer's rule, while its first weights are on their way:
-// for the few rows where that is shorter than a launch (f8_project_fusable).
+// QX: the rows come in bf16 (p.x) and every workgroup quantizes its tile's into
+// LDS first, by the quantizer's rule, while its first weights are on their way.
 template <int MT, int NT, int D, bool QX, bool LISTS, bool GU, bool RESID>
 __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int NW = 8, BM = 16 * MT, COLS = 16 * NT / (GU ? 2 : 1), NG = GU ? NT / 2 : NT;
   static_assert(!GU || NT % 2 == 0, "gate and up fragments");
-  static_assert(!QX || (MT == 1 && !LISTS && !GU), "rows quantized here");
+  static_assert(!QX || (!LISTS && !GU), "rows quantized here");
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, g = lane >> 4;
@@ -87,18 +90,48 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
   const float* wsp[2] = {p.ws + panel, GU ? p.ws2 + panel : nullptr};
   constexpr int MATS = GU ? 2 : 1;
 
-  // QX: codes [rows][pitch] and scales [rows][kb] behind the waves' sums
+  // QX, behind the waves' sums: codes (rows 16 bytes apart beyond the pitch, so
+  // that a fragment's 16 rows lie in different banks) and scales [rows][kb]
+  const int q_pitch = pitch + 16, q_blocks = here * kb;
   char* const q_codes = lds + NW * MT * NT * 1024;
-  float* const q_scales = reinterpret_cast<float*>(q_codes + p.rows * pitch);
-  uint4 xv[kQxPasses];
-  if constexpr (QX) {
+  float* const q_scales = reinterpret_cast<float*>(q_codes + (int)(p.rows < BM ? p.rows : BM) * q_pitch);
+  // 16 lanes take a block, the workgroup 32 blocks in a pass; where the lanes'
+  // block of the pass to be loaded, and of the one to be stored, lies
+  struct Place {
+    int row, block;
+  };
+  constexpr int QA = 4;  // passes loaded ahead
+  uint4 xv[QA];
+  const int q_col = (threadIdx.x & 15) * 8, q_rows = 32 / kb, q_rest = 32 - q_rows * kb;
+  Place q_in{(int)(threadIdx.x >> 4) / kb, (int)(threadIdx.x >> 4) % kb}, q_out = q_in;
+  auto q_next = [&](Place& at) {
+    at.block += q_rest;
+    at.row += q_rows + (at.block >= kb);
+    at.block -= at.block >= kb ? kb : 0;
+  };
+  auto q_load = [&](int b0) {
 #pragma unroll
-    for (int s = 0; s < kQxPasses; ++s) {
-      const int c = threadIdx.x + s * 512, per = pitch / 8, row = c / per, col = (c - row * per) * 8;
+    for (int s = 0; s < QA; ++s) {
+      if (b0 + s * 32 >= q_blocks) break;
+      const int col = q_in.block * 128 + q_col;
       xv[s] = uint4{0, 0, 0, 0};
-      if (row < here && col < p.k) xv[s] = *reinterpret_cast<const uint4*>(p.x + row * p.x_stride + col);
+      if (q_in.row < here && col < p.k) xv[s] = *reinterpret_cast<const uint4*>(p.x + (m0 + q_in.row) * p.x_stride + col);
+      q_next(q_in);
     }
-  }
+  };
+  auto q_store = [&](int b0) {
+#pragma unroll
+    for (int s = 0; s < QA; ++s) {
+      if (b0 + s * 32 >= q_blocks) break;
+      const float scale = as_float(f8_scale_field(f8_block_amax(xv[s])) << 23);
+      if (q_out.row < here) {
+        *reinterpret_cast<uint2*>(q_codes + q_out.row * q_pitch + q_out.block * 128 + q_col) = f8_codes8(xv[s], scale);
+        if (q_col == 0) q_scales[q_out.row * kb + q_out.block] = scale;
+      }
+      q_next(q_out);
+    }
+  };
+  if constexpr (QX) q_load(0);
 
   struct Block {
     v4i w[NT][2], a[MT][2];
@@ -136,19 +169,10 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
   for (int d = 0; d < D; ++d) load(buf[d], wave + NW * d);
   if constexpr (QX) {
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int s = 0; s < kQxPasses; ++s) {
-      if (s * 512 * 8 >= here * pitch) break;
-      const int c = threadIdx.x + s * 512, per = pitch / 8, row = c / per, col = (c - row * per) * 8;
-      uint32_t m = f8_amax2(f8_amax2(f8_amax2(f8_amax2(0u, xv[s].x), xv[s].y), xv[s].z), xv[s].w);
-      m = group_max16(m);  // 16 lanes hold a block
-      const uint32_t field = f8_scale_field(m);
-      const float inv = as_float((254u - field) << 23);
-      if (row < here) {
-        *reinterpret_cast<uint2*>(q_codes + row * pitch + col) =
-            uint2{f8_codes(xv[s].x, xv[s].y, inv), f8_codes(xv[s].z, xv[s].w, inv)};
-        if (threadIdx.x % 16 == 0) q_scales[row * kb + col / 128] = as_float(field << 23);
-      }
+    q_store(0);
+    for (int b0 = QA * 32; b0 < q_blocks; b0 += QA * 32) {
+      q_load(b0);
+      q_store(b0);
     }
     __syncthreads();
   }
@@ -158,11 +182,15 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
       Block& b = buf[d];
       if constexpr (QX) {
         // (blocks past the end multiply zeros)
-        const int k = k0 + NW * d < kb ? k0 + NW * d : 0, row = lr < here ? lr : here - 1;
-        const char* at = q_codes + row * pitch + k * 128 + 16 * g;
-        b.a[0][0] = *reinterpret_cast<const v4i*>(at);
-        b.a[0][1] = *reinterpret_cast<const v4i*>(at + 64);
-        b.sa[0] = k0 + NW * d < kb ? q_scales[row * kb + k] : 0.0f;
+        const int k = k0 + NW * d < kb ? k0 + NW * d : 0;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int r = 16 * i + lr, row = r < here ? r : here - 1;
+          const char* at = q_codes + row * q_pitch + k * 128 + 16 * g;
+          b.a[i][0] = *reinterpret_cast<const v4i*>(at);
+          b.a[i][1] = *reinterpret_cast<const v4i*>(at + 64);
+          b.sa[i] = k0 + NW * d < kb ? q_scales[row * kb + k] : 0.0f;
+        }
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
@@ -229,12 +257,15 @@ template <int MT, int NT, int D, bool QX, bool LISTS, bool GU, bool RESID>
 hipError_t launch_stream(const F8Args& x, hipStream_t stream) {
   constexpr int BM = 16 * MT, COLS = 16 * NT / (GU ? 2 : 1), sums = 8 * MT * NT * 1024;
   static_assert(128 % COLS == 0, "a tile's columns lie in one weight block");
-  static_assert(!QX || sums + kQxValues + kQxValues / 32 <= 64 * 1024, "LDS without raising the limit");
+  // the most that kQxValues of codes, their padding and scales take
+  constexpr int most = sums + (QX ? kQxValues + 16 * BM + kQxValues / 32 : 0);
+  static_assert(most <= 160 * 1024, "LDS of a workgroup");
   static LaunchCache cache;
   auto* kernel = &f8_stream_kernel<MT, NT, D, QX, LISTS, GU, RESID>;
-  if (sums > 64 * 1024)
-    if (hipError_t e = ensure_dynamic_lds(cache, reinterpret_cast<const void*>(kernel), sums)) return e;
-  const int lds = sums + (QX ? (int)x.rows * x.kb * 132 : 0);
+  if (most > 64 * 1024)
+    if (hipError_t e = ensure_dynamic_lds(cache, reinterpret_cast<const void*>(kernel), most)) return e;
+  const int lds = sums + (QX ? (int)(x.rows < BM ? x.rows : BM) * (x.kb * 132 + 16) : 0);
+  if (lds > most) return hipErrorInvalidValue;
   const int64_t tiles_m = LISTS ? f8_most_tiles(x.lists.total, x.lists.experts, BM) : (x.rows + BM - 1) / BM;
   if (tiles_m > 65535) return hipErrorInvalidValue;
   const dim3 grid((unsigned)((x.n + COLS - 1) / COLS), (unsigned)tiles_m);
@@ -701,6 +732,18 @@ hipError_t launch_tile(const F8Args& x, hipStream_t stream) {
   return hipGetLastError();
 }
 
+constexpr int64_t kCus = 256;
+
+// Tiles of the split-k kernel for m rows against n weight rows (gate/up: both).
+enum class StreamShape { kNone, k16x32, k16x64, k32x64, k64x64 };
+StreamShape stream_shape(int64_t m, int64_t n) {
+  auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); };
+  if (tiles(16, 32) <= kCus || (m <= 16 && tiles(16, 64) > kCus)) return StreamShape::k16x32;
+  if (tiles(16, 64) <= kCus) return StreamShape::k16x64;
+  if (tiles(32, 64) <= kCus) return StreamShape::k32x64;
+  return tiles(64, 64) <= kCus ? StreamShape::k64x64 : StreamShape::kNone;
+}
+
 // The kernel of a shape. From the smallest tiles up: 16 x 32, 16 x 64, 32 x 64
 // and 64 x 64 of the split-k kernel while they are at most one per CU (m x k x n
 // in us: 256 x 2048 x 512 4.1 on 16 x 32 tiles, 5.0, 6.3, 8.0 on the larger
@@ -713,7 +756,6 @@ hipError_t launch_tile(const F8Args& x, hipStream_t stream) {
 // 32 (16 x 5120 x 2 17408: 39 against 45 on 128 x 128).
 template <bool LISTS, bool GU, bool RESID>
 hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
-  constexpr int64_t kCus = 256;
   const int64_t rows_of_w = (int64_t)x.n * (GU ? 2 : 1);
   // tiles of bm rows; experts' lists as if evenly filled (a little more, for
   // those above the mean)
@@ -740,15 +782,21 @@ hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
         return launch_stream<1, 4, 2, false, LISTS, GU, RESID>(x, stream);
     }
   } else {
+    const StreamShape shape = stream_shape(x.rows, rows_of_w);
     if constexpr (!GU)
-      if (x.x != nullptr)  // f8_project_fusable
-        return tiles(16, 32) <= kCus || tiles(16, 64) > kCus ? launch_stream<1, 2, 2, true, false, false, RESID>(x, stream)
-                                                             : launch_stream<1, 4, 2, true, false, false, RESID>(x, stream);
-    if (tiles(16, 32) <= kCus || (x.rows <= 16 && tiles(16, 64) > kCus))
-      return launch_stream<1, 2, 2, false, LISTS, GU, RESID>(x, stream);
-    if (tiles(16, 64) <= kCus) return launch_stream<1, 4, 2, false, LISTS, GU, RESID>(x, stream);
-    if (tiles(32, 64) <= kCus) return launch_stream<2, 4, 2, false, LISTS, GU, RESID>(x, stream);
-    if (tiles(64, 64) <= kCus) return launch_stream<4, 4, 1, false, LISTS, GU, RESID>(x, stream);
+      if (x.x != nullptr) switch (shape) {  // f8_project_fusable
+          case StreamShape::k16x32: return launch_stream<1, 2, 2, true, false, false, RESID>(x, stream);
+          case StreamShape::k16x64: return launch_stream<1, 4, 2, true, false, false, RESID>(x, stream);
+          case StreamShape::k32x64: return launch_stream<2, 4, 2, true, false, false, RESID>(x, stream);
+          default: return hipErrorInvalidValue;
+        }
+    switch (shape) {
+      case StreamShape::k16x32: return launch_stream<1, 2, 2, false, LISTS, GU, RESID>(x, stream);
+      case StreamShape::k16x64: return launch_stream<1, 4, 2, false, LISTS, GU, RESID>(x, stream);
+      case StreamShape::k32x64: return launch_stream<2, 4, 2, false, LISTS, GU, RESID>(x, stream);
+      case StreamShape::k64x64: return launch_stream<4, 4, 1, false, LISTS, GU, RESID>(x, stream);
+      default: break;
+    }
   }
   const int64_t small = (tiles(128, 128) + kCus - 1) / kCus, large = (tiles(256, 256) + kCus - 1) / kCus;
   if (small >= 3 * large)
@@ -772,7 +820,13 @@ hipError_t launch_f8_gemm(const F8Args& x, bool gate_up, hipStream_t stream) {
   return x.residual ? launch_rows<false, false, true>(x, stream) : launch_rows<false, false, false>(x, stream);
 }
 
-bool f8_project_fusable(int64_t m, int, int k) { return m <= 4 && m * f8_pitch(k) <= kQxValues; }
+bool f8_project_fusable(int64_t m, int n, int k) {
+  const StreamShape shape = stream_shape(m, n);
+  const int rows = shape == StreamShape::k16x32 || shape == StreamShape::k16x64 ? 16
+                   : shape == StreamShape::k32x64                               ? 32
+                                                                                : 0;
+  return rows > 0 && (m < rows ? m : rows) * f8_pitch(k) <= kQxValues;
+}
 
 hipError_t launch_f8_experts(const F8Args& x, bool gate_up, hipStream_t stream) {
   return gate_up ? launch_rows<true, true, false>(x, stream) : launch_rows<true, false, false>(x, stream);

@@ -36,22 +36,18 @@ __global__ __launch_bounds__(256) void f8_prepare_kernel(const uint16_t* __restr
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
     const int b = b0 + s * CPW;
-    uint32_t m = f8_amax2(f8_amax2(f8_amax2(f8_amax2(0u, v[s].x), v[s].y), v[s].z), v[s].w);
-    m = group_max16(m);
+    const uint32_t m = f8_block_amax(v[s]);
     if (!row_here || b >= kp) continue;
     if (b >= kb) {  // the row's bytes behind its exponents: zeros
       if (l == 0) exponents[row * kp + b] = 0;
       continue;
     }
     const uint32_t field = f8_scale_field(m);
-    const float inv = as_float((254u - field) << 23);
-    uint2 q;
-    q.x = f8_codes(v[s].x, v[s].y, inv);
-    q.y = f8_codes(v[s].z, v[s].w, inv);
-    *reinterpret_cast<uint2*>(codes + row * ((int64_t)kb * 128) + b * 128 + 8 * l) = q;
+    const float scale = as_float(field << 23);
+    *reinterpret_cast<uint2*>(codes + row * ((int64_t)kb * 128) + b * 128 + 8 * l) = f8_codes8(v[s], scale);
     if (l == 0) {
       exponents[row * kp + b] = (uint8_t)field;
-      scales[(int64_t)b * rows + row] = as_float(field << 23);
+      scales[(int64_t)b * rows + row] = scale;
     }
   }
 }
@@ -83,7 +79,8 @@ __global__ __launch_bounds__(256) void f8_pack_kernel(const uint16_t* __restrict
     const int row = rb * 128 + r0 + 16 * i;
     v[i] = uint4{0, 0, 0, 0};
     if (row < n && col < k) v[i] = *reinterpret_cast<const uint4*>(w + (e * n + row) * (int64_t)k + col);
-    m = f8_amax2(f8_amax2(f8_amax2(f8_amax2(m, v[i].x), v[i].y), v[i].z), v[i].w);
+    const uint32_t o = f8_amax8<true>(v[i]);
+    m = m > o ? m : o;
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
@@ -95,16 +92,13 @@ __global__ __launch_bounds__(256) void f8_pack_kernel(const uint16_t* __restrict
 #pragma unroll
   for (int i = 0; i < 4; ++i) m = m > wave_max[i] ? m : wave_max[i];
   const uint32_t field = f8_scale_field(m);
-  const float inv = as_float((254u - field) << 23);
+  const float scale = as_float(field << 23);
   uint8_t* out = codes + block * 16384;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    uint2 q;
-    q.x = f8_codes(v[i].x, v[i].y, inv);
-    q.y = f8_codes(v[i].z, v[i].w, inv);
-    *reinterpret_cast<uint2*>(out + f8_block_byte(r0 + 16 * i, 8 * l)) = q;
+    *reinterpret_cast<uint2*>(out + f8_block_byte(r0 + 16 * i, 8 * l)) = f8_codes8(v[i], scale);
   }
-  if (threadIdx.x == 0) scales[block] = as_float(field << 23);
+  if (threadIdx.x == 0) scales[block] = scale;
 }
 
 // e4m3 rows [matrices][n][k] -> blocks in the operand order; one workgroup per

@@ -532,7 +532,9 @@ int clef_f8_retile(const uint8_t* w, int64_t matrices, int32_t n, int32_t k, uin
  * (here and below) nonzero: every scale of w is a power of two between 2^-126
  * and 2^127, as clef_f8_pack_weight and e8m0 checkpoints make them; the matrix
  * unit may then apply them (with other
- * scales it would drop their mantissas). The same sums within f32 rounding. */
+ * scales it would drop their mantissas). The same sums within f32 rounding.
+ * Products of an activation's scale and a weight's are formed in f32. The
+ * output may be the residual itself and overlaps no other input. */
 int clef_f8_gemm(const uint8_t* a, const uint8_t* w, const float* w_scales, int64_t m,
                  int32_t n, int32_t k, int32_t pow2, const uint16_t* residual, uint16_t* out, clef_stream_t stream);
 
@@ -542,7 +544,9 @@ int clef_f8_gemm_gate_up(const uint8_t* a, const uint8_t* gate, const float* gat
                          uint16_t* h, clef_stream_t stream);
 
 /* clef_f8_prepare and clef_f8_gemm in one call; the workspace (bytes below, 0
- * where a few rows are quantized by the product itself) takes the activation. */
+ * where the product quantizes the rows itself: then each of its workgroups reads
+ * its rows of x) takes the activation. An output that overlaps x -> "FP8 output
+ * overlaps its input rows". */
 size_t clef_f8_project_workspace_bytes(int64_t m, int32_t n, int32_t k);
 int clef_f8_project(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint8_t* w, const float* w_scales,
                     int32_t n, int32_t pow2, const uint16_t* residual, uint16_t* out, void* workspace,

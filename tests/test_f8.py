@@ -78,6 +78,14 @@ def test_products_pointers_workspace_and_no_rows():
     assert rc == -1 and msg == SHAPE
 
 
+@pytest.mark.parametrize("m", [4, 4096])
+def test_project_rejects_an_output_over_its_rows(m):
+    far = FAKE + (1 << 40)
+    for x, out in ((FAKE, FAKE), (FAKE, FAKE + (m - 1) * 1024 + 496), (FAKE + 512 * m - 16, FAKE)):
+        rc, msg = call("clef_f8_project", x, m, 256, 512, far, far, 256, 0, None, out, far, 1 << 40, None)
+        assert rc == -1 and msg == "FP8 output overlaps its input rows"
+
+
 def test_group_slots_rejects():
     args = (FAKE, FAKE, FAKE, 1 << 30, None)
     assert call("clef_moe_group_slots", FAKE, (1 << 20) + 1, 8, 128, *args)[1] == "unsupported Omni route grouping shape"

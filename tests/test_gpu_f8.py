@@ -268,6 +268,35 @@ def test_project_of_whole_numbers_is_exact(m, k, n, kind):
                        (want + res.double()).float().to(BF))
 
 
+@pytest.mark.parametrize("m,k,n", [
+    # one launch on 16 x 32, 16 x 64 and 32 x 64 tiles: one row to many tiles of
+    # rows, the last of them short; blocks that end inside; one pass to ten
+    (1, 8, 8), (1, 16384, 256), (2, 20480, 264), (3, 12288, 520), (5, 8192, 136), (9, 4104, 1000), (10, 4096, 2048),
+    (16, 2560, 32), (17, 2560, 392), (33, 128, 3992), (130, 1000, 520), (250, 512, 1096), (255, 1280, 1016),
+    (513, 1032, 1000), (1000, 264, 520), (4095, 128, 64),
+    # and rows or widths just past it
+    (11, 4096, 2048), (16, 2568, 32), (3, 20480, 264), (64, 1400, 5000)])
+@pytest.mark.parametrize("res", [False, True])
+def test_project_quantizing_rows_itself_is_the_two_steps(m, k, n, res):
+    """The same codes, scales and order of sums whether the rows are quantized
+    by the product or before it, non-finite values and column ranges included."""
+    wide = randn((m, k + 24), 1.0, m + k)
+    wide *= torch.exp2(torch.randint(-140, 100, (m, 1), generator=gen(3), device="cuda").float()).to(BF)
+    wide[m // 2, 8 + k // 2] = float("nan")
+    wide[-1, 8 + k - 1] = float("-inf")
+    codes, scales = weight(1, n, k, "f32", n)
+    w = clef_i4.f8_weight(codes[0], scales[0])
+    residual = randn((m, n), 3.0, 4) if res else None
+    for x in (wide[:, 8: 8 + k], wide[:, 8: 8 + k].contiguous()):
+        want = clef_i4.project_f8(clef_i4.prepare_f8(x), w, residual)
+        out = torch.full((m + 1, n), 7.0, dtype=BF, device="cuda")
+        clef_i4.project_quantized_f8(x, w, residual, out=out[:m])
+        assert torch.equal(out[:m].view(torch.int16), want.view(torch.int16)) and (out[m:] == 7.0).all()
+    if res:  # the output may be the residual itself
+        clef_i4.project_quantized_f8(x, w, residual, out=residual)
+        assert torch.equal(residual.view(torch.int16), want.view(torch.int16))
+
+
 def test_project_loaded_weight_and_strided_rows():
     wide = randn((21, 800), 1.0, 1)
     x = wide[:, 16: 16 + 520]
