@@ -696,7 +696,8 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void f8_tile_kernel(cons
     // expert's next rows: both operands stay in its L2. The grid has blocks for
     // the most tiles that such lists can have; those there are shared evenly.
     const F8Tiles<T::BM> tiles(p.lists);
-    const int blocks = tiles.total * tiles_n, per = blocks / 8, b = blockIdx.x;
+    // (lists that overlap can make more than the grid has blocks for)
+    const int blocks = (tiles.total < tiles_m ? tiles.total : tiles_m) * tiles_n, per = blocks / 8, b = blockIdx.x;
     if (b >= blocks) return;
     const int r = b < 8 * per ? (b % 8) * per + b / 8 : b;
     tm = r / tiles_n;

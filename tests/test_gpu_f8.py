@@ -334,6 +334,77 @@ def test_project_non_finite_rows_and_values():
     assert ((h[0].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-30).all()
 
 
+@pytest.mark.parametrize("m,k,n", [(5, 4104, 264), (64, 512, 2000), (700, 256, 4104), (620, 5120, 2504),
+                                   (2300, 392, 3608)])
+def test_project_onto_its_residual(m, k, n):
+    x, residual = randn((m, k), 1.0, m), randn((m, n), 30.0, 4)
+    codes, scales = weight(1, n, k, "f32", n)
+    w = clef_i4.f8_weight(codes[0], scales[0])
+    want = clef_i4.project_quantized_f8(x, w, residual)
+    assert torch.equal(clef_i4.project_quantized_f8(x, w, residual, out=residual), want)
+
+
+@pytest.mark.parametrize("m", [3, 300, 1030, 8200])
+def test_project_scales_at_their_limits(m):
+    """e8m0 from 2^-127 to 2^127 and NaN. One product of ones per output: exact."""
+    k, n = 384, 1280
+    exponents = torch.tensor([0, 1, 2, 120, 127, 140, 252, 253, 254, 255], dtype=torch.uint8, device="cuda")
+    scales = exponents[:, None].expand(10, 3).contiguous().view(torch.float8_e8m0fnu)
+    w = clef_i4.f8_weight(torch.ones((n, k), device="cuda").to(F8), scales)
+    x = torch.zeros((m, k), dtype=BF, device="cuda")
+    x[torch.arange(m, device="cuda"), torch.arange(m, device="cuda") * 37 % k] = 448.0  # a row scale of one
+    got = clef_i4.project_quantized_f8(x, w).double()
+    want = 448.0 * scales[:, 0].double().repeat_interleave(128)
+    want = want.float().to(BF).double().expand(m, n)  # past the largest bf16: infinity
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
+def test_rows_and_slots_beyond_4_gib():
+    """Activations whose bytes do not fit 32 bits (rows of a projection) or
+    just do (an expert's), read at their end."""
+    n, k, m = 8, 4224, 1048576
+    codes, scales = weight(2, n, k, "f32", 3)
+    last = randn((300, k), 1.0, 7)
+    x = torch.zeros((m, k), dtype=BF, device="cuda")
+    x[-300:] = last
+    want, slack = product64(rows64(clef_i4.prepare_f8(last)), weight64(codes, scales)[0])
+    w = clef_i4.f8_weight(codes[0], scales[0])
+    got = clef_i4.project_quantized_f8(x, w)
+    check(got[-300:], want, slack)
+    assert not got[:-300].any()
+    del got
+    rows = 1000000  # 4.22e9 bytes of codes
+    a = clef_i4.prepare_f8(x[-rows:])
+    two = clef_i4.f8_weight(codes, scales)
+    count = 250
+    slots = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
+    slots[:count] = torch.arange(rows - count, rows, dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([0, 0, count], dtype=torch.int32, device="cuda")
+    out = clef_i4.expert_f8(a, two, offsets, slots, 1, True, out=torch.full((rows, n), 7.0, dtype=BF, device="cuda"))
+    want, slack = product64(rows64(clef_i4.prepare_f8(last[-count:])), weight64(codes, scales)[1])
+    check(out[-count:], want, slack)
+    assert (out[:-count] == 7.0).all()
+    with pytest.raises(clef_i4.ClefError):
+        clef_i4.expert_f8(clef_i4.prepare_f8(x), two, offsets, slots, 1, True)
+
+
+def test_two_streams_at_once():
+    """Calls in flight side by side have workspaces of their own."""
+    w = clef_i4.load_f8_weight(randn((2048, 1032), 0.05, 8))
+    inputs = [randn((700, 1032), 1.0, 20 + i) for i in range(6)] + [randn((9, 1032), 1.0, 40 + i) for i in range(6)]
+    want = [clef_i4.project_quantized_f8(x, w) for x in inputs]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for i, x in enumerate(inputs):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append(clef_i4.project_quantized_f8(x, w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ---------------------------------------------------------------- lists
 
 @pytest.mark.parametrize("tokens,topk,experts", [(0, 8, 128), (1, 1, 1), (1, 8, 128), (2, 3, 8), (63, 1, 2), (235, 8, 128),
@@ -446,6 +517,38 @@ def test_experts_leave_unlisted_rows_and_odd_lists():
     same(run([-5, 2, 2, 60, 1 << 30], None), {**{r: 0 for r in range(2)}, **{r: 2 for r in range(2, 60)},
                                               **{r: 3 for r in range(60, total)}})
     same(run([10, 5, 8, 8, 8], None), {r: 1 for r in range(5, 8)})
+
+
+@pytest.mark.parametrize("tokens,experts", [(12, 1024), (5000, 1024), (20000, 130)])
+def test_experts_past_the_first_128(tokens, experts):
+    """Whole numbers, each expert's weight its number: exact."""
+    k, n = 136, 8
+    ids = torch.randint(0, experts, (tokens, 1), generator=gen(experts), device="cuda")
+    ids[0], ids[-1] = 128, experts - 1
+    offsets, slots = clef_i4.omni_group_slots(torch.cat([ids, torch.ones_like(ids)], 1).float(), experts)
+    codes = torch.zeros((experts, n, k), device="cuda")
+    codes[:, :, 0] = (torch.arange(experts, device="cuda") // 64)[:, None]
+    codes[:, :, 130] = (torch.arange(experts, device="cuda") % 64 // 4)[:, None]
+    w = clef_i4.f8_weight(codes.to(F8), torch.ones((experts, 1, 2), device="cuda"))
+    assert torch.equal(codes.to(F8).float(), codes)
+    x = torch.zeros((tokens, k), dtype=BF, device="cuda")
+    x[:, 0], x[:, 130] = 16.0, 1.0
+    got = clef_i4.expert_f8(clef_i4.prepare_f8(x), w, offsets, slots, 1, True)
+    assert torch.equal(got.float(), (ids // 64 * 16 + ids % 64 // 4).float().expand(tokens, n).to(BF).float())
+
+
+def test_experts_overlapping_lists_stay_inside():
+    """Lists that name places twice make more tiles than sound ones can: a row
+    is one of its experts', nothing else is written."""
+    k, n, total = 128, 136, 1000
+    w = clef_i4.f8_weight(torch.ones((6, n, k), device="cuda").to(F8),
+                          torch.arange(1, 7, device="cuda").float()[:, None, None].expand(6, 2, 1).contiguous())
+    x = torch.zeros((total, k), dtype=BF, device="cuda")
+    x[:, 3] = 1.0
+    offsets = torch.tensor([0, total, 0, total, 0, total, 1], dtype=torch.int32, device="cuda")
+    out = torch.full((total + 1, n), 7.0, dtype=BF, device="cuda")
+    clef_i4.expert_f8(clef_i4.prepare_f8(x), w, offsets, None, 1, True, out=out[:total])
+    assert torch.isin(out, torch.tensor([1.0, 3.0, 5.0, 7.0], dtype=BF, device="cuda")).all() and (out[total] == 7.0).all()
 
 
 # ---------------------------------------------------------------- together
