@@ -113,11 +113,6 @@ __device__ __forceinline__ v4f mfma_f8_scaled(v8i_t w, v8i_t a, v4f c, int sw, u
   }
 }
 
-// The power of two whose e8m0 exponent is byte `byte` of v.
-__device__ __forceinline__ float e8m0_byte(uint32_t v, int byte) {
-  return as_float((byte < 3 ? v << (23 - 8 * byte) : v >> 1) & 0x7F800000u);
-}
-
 __device__ __forceinline__ v8i_t join_halves(v4i lo, v4i hi) {
   return v8i_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }

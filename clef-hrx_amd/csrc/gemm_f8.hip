@@ -311,10 +311,12 @@ struct F8Tile {
 //
 // A wave's step (one block of k) is TM rows of fragments times TN weight
 // fragments. It holds the weight fragments of the step and reads an activation
-// fragment one row of MFMAs ahead of its use. Scales that are powers of two
-// (HW) go into the MFMA, which adds to the accumulator itself; other scales are
-// applied by four fmas to a partial sum two MFMAs after the MFMA that made it
-// (half the MFMAs' issue time, run under them).
+// fragment one row of MFMAs ahead of its use. The rows' scales,
+// powers of two, go into the MFMA. So do the weight's where they are (HW), and
+// the MFMA adds to the accumulator itself; other weight scales are applied by
+// four fmas to a partial sum two MFMAs after the MFMA that made it (half the
+// MFMAs' issue time, run under them; with the rows' scales in those fmas 1711 x
+// 5120 x 2 17408 took 295 us, not 288).
 //
 // A stage of LDS is filled in two parts: X (weights, scales, the first half of
 // each wave's activation rows) and Y (the other half). Behind a barrier in the
@@ -455,7 +457,7 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
     constexpr int MATS = GU ? 2 : 1;
     v8i_t av[2], bv[TN];
     v4f part[4];               // !HW: partial sums on their way
-    float sv[MATS], last[MATS];  // !HW: scales of the row of MFMAs and of the row before
+    float sv[MATS], last[MATS];  // !HW: the panels' scales in this step and in the one before
     uint32_t sa[TM / 4], sa_next[TM / 4];  // the rows' exponents, four in each
     int sw_bits[MATS];         // HW: the panels' scales, exponent in the top byte
     auto read_a = [&](const char* stage, int i) {
@@ -482,9 +484,14 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
     auto take_scales = [&]() {
 #pragma unroll
       for (int i = 0; i < TM / 4; ++i) sa[i] = sa_next[i];
-      if constexpr (HW) {
 #pragma unroll
-        for (int t = 0; t < MATS; ++t) sw_bits[t] = (int)(as_uint(sw[t]) << 1);
+      for (int t = 0; t < MATS; ++t) {
+        if constexpr (HW) {
+          sw_bits[t] = (int)(as_uint(sw[t]) << 1);
+        } else {
+          last[t] = sv[t];
+          sv[t] = sw[t];
+        }
       }
     };
     auto add = [&](v4f& c, const v4f& v, float s) {
@@ -500,13 +507,6 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
     auto step = [&](char* cur, const char* next, int kt) {
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        if constexpr (!HW) {
-#pragma unroll
-          for (int t = 0; t < MATS; ++t) {
-            last[t] = sv[t];
-            sv[t] = e8m0_byte(sa[i / 4], i % 4) * sw[t];
-          }
-        }
         if (i == TM / 2 - 1) landed();  // this stage's Y; its X has been read
         if (i == TM - 1) {
           landed();  // the next stage's X; this stage has been read
@@ -520,12 +520,12 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
             acc[i][j] = mfma_f8_scaled(bv[j], av[i & 1], acc[i][j], sw_bits[GU && j >= TN / 2 ? 1 : 0], sa[i / 4], i % 4);
             __builtin_amdgcn_sched_barrier(0);
           } else {
-            part[(i * TN + j) % 4] = mfma_f8(bv[j], av[i & 1], v4f{0, 0, 0, 0});
+            part[(i * TN + j) % 4] = mfma_f8_scaled(bv[j], av[i & 1], v4f{0, 0, 0, 0}, 127 << 24, sa[i / 4], i % 4);
             __builtin_amdgcn_sched_barrier(0);
             // the MFMA two before
             const int before = i * TN + j - 2, ii = (before + TM * TN) / TN % TM, jj = (before + TN) % TN;
             const int mat = GU && jj >= TN / 2 ? 1 : 0;
-            add(acc[ii][jj], part[(before + 4) % 4], j >= 2 ? sv[mat] : last[mat]);
+            add(acc[ii][jj], part[(before + 4) % 4], before >= 0 ? sv[mat] : last[mat]);
           }
           if (i == TM - 1) bv[j] = read_b(next, j);
           // X behind the first barrier, Y behind the second
@@ -557,13 +557,13 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
     av[0] = read_a(r0, 0);
 #pragma unroll
     for (int j = 0; j < TN; ++j) bv[j] = read_b(r0, j);
-    take_scales();
     if constexpr (!HW) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) part[t] = v4f{0, 0, 0, 0};
 #pragma unroll
       for (int t = 0; t < MATS; ++t) sv[t] = 0.0f;
     }
+    take_scales();
     // The scales of the next 16 blocks of k are loaded in the first half of these
     // and turned before the second (a branch inside a step instead made the
     // compiler spill).
@@ -587,8 +587,8 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
     }
     if constexpr (!HW) {
       // the last two partial sums
-      add(acc[TM - 1][TN - 2], part[2], sv[GU && TN > 2 ? 1 : 0]);
-      add(acc[TM - 1][TN - 1], part[3], sv[GU ? 1 : 0]);
+      add(acc[TM - 1][TN - 2], part[2], last[GU && TN > 2 ? 1 : 0]);
+      add(acc[TM - 1][TN - 1], part[3], last[GU ? 1 : 0]);
     }
   };
   body(lds, lds + T::STAGE_BYTES);
