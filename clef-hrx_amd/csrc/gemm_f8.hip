@@ -749,12 +749,12 @@ StreamShape stream_shape(int64_t m, int64_t n) {
 // and 64 x 64 of the split-k kernel while they are at most one per CU (m x k x n
 // in us: 256 x 2048 x 512 4.1 on 16 x 32 tiles, 5.0, 6.3, 8.0 on the larger
 // ones; 384 x 512 x 2048 8.6, 6.5, 6.8 and 4.7); beyond, 128 x 128 tiles, two
-// workgroups per CU (256 x 4096 x 12288: 20 against 39 on 64 x 64), and 256 x
+// workgroups per CU (256 x 4096 x 12288: 19 against 39 on 64 x 64), and 256 x
 // 256 tiles from three times their rounds over the CUs up, a 256 x 256 round
 // taking about three of 128 x 128 (1024 x 4096 x 12288, 1 and 3 rounds: 49
-// against 52; 1536, 2 and 5: 97 against 81; 4096, 3 and 12: 175 against 220).
+// against 52; 1536, 2 and 5: 95 against 81; 4096, 3 and 12: 174 against 218).
 // One tile of 16 rows against more columns than 256 tiles cover stays on 16 x
-// 32 (16 x 5120 x 2 17408: 39 against 45 on 128 x 128).
+// 32 (16 x 5120 x 2 17408: 39 against 44 on 128 x 128).
 template <bool LISTS, bool GU, bool RESID>
 hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
   const int64_t rows_of_w = (int64_t)x.n * (GU ? 2 : 1);
@@ -773,10 +773,10 @@ hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
   };
   if constexpr (LISTS) {
     // The experts' weights are read once whatever the tile: 16 x 64 tiles for a
-    // few slots (8 slots: 4.7 / 5.3 us down / gate/up against 6.1 / 10.0 on 128 x
+    // few slots (8 slots: 4.7 / 5.3 us down / gate/up against 6.2 / 9.8 on 128 x
     // 128) and for up to 8 rows per expert over at least 16 blocks of k (60
-    // tokens of 128 experts top-8, gate/up 71 against 75; 240 tokens 91 against
-    // 79; down, 6 blocks of k, 43 against 36).
+    // tokens of 128 experts top-8, gate/up 71 against 74; 240 tokens 92 against
+    // 78; down, 6 blocks of k, 43 against 39).
     const int64_t rows = x.lists.total / x.lists.experts;
     if (x.lists.total <= 16 || (rows < 8 && x.kb >= 16)) {
       if (f8_most_tiles(x.lists.total, x.lists.experts, 16) <= 65535)
@@ -803,13 +803,17 @@ hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
   if (small >= 3 * large)
     return x.pow2 ? launch_tile<F8Tile256, F8Tile256H, true, LISTS, GU, RESID>(x, stream)
                   : launch_tile<F8Tile256, F8Tile256H, false, LISTS, GU, RESID>(x, stream);
-  // One tile per CU with f32 scales: two blocks of k at a time on two groups of
-  // waves, which read less LDS per MFMA (620 x 17408 x 5120 82 -> 74 us, 512 x 4096
-  // x 4096 19.1 -> 17.3; 768 x 512 x 4096, 4 blocks of k, 6.0 -> 7.0; with
-  // power-of-two scales no gain: 15.9 and 15.9 at 512 x 4096 x 4096).
+  // One tile per CU: two blocks of k at a time on two groups of waves, which read
+  // less LDS per MFMA and have more loads on their way, against a longer start and
+  // the groups' sums (f32 scales, us for 128 x 128 tiles and these: 620 x 17408 x
+  // 5120 80 and 72, 512 x 4096 x 4096 18.4 and 17.1, 768 x 512 x 4096, 4 blocks of
+  // k, 5.9 and 6.8; powers of two: 620 x 17408 x 5120 76.7 and 72.2, 300 x 8192 x
+  // 8192 36.8 and 35.0, 300 x 5120 x 2 5120 22.0 and 21.5, 256 x 4096 x 12288 16.8
+  // and 16.7, 640 x 2048 x 2048 9.4 and 10.3).
   if constexpr (!LISTS)
-    if (small <= 1 && !x.pow2 && x.kb >= 16)
-      return launch_tile<F8Tile128K, F8Tile128K, false, LISTS, GU, RESID>(x, stream);
+    if (small <= 1 && x.kb >= (x.pow2 ? 40 : 16))
+      return x.pow2 ? launch_tile<F8Tile128K, F8Tile128K, true, LISTS, GU, RESID>(x, stream)
+                    : launch_tile<F8Tile128K, F8Tile128K, false, LISTS, GU, RESID>(x, stream);
   return x.pow2 ? launch_tile<F8Tile128, F8Tile128, true, LISTS, GU, RESID>(x, stream)
                 : launch_tile<F8Tile128, F8Tile128, false, LISTS, GU, RESID>(x, stream);
 }

@@ -201,10 +201,11 @@ def test_weight_layout(matrices, n, k):
 
 SHAPES = [(1, 128, 128), (1, 4096, 1024), (3, 136, 8), (16, 1000, 264), (17, 264, 1352), (37, 4160, 1352),
           (64, 512, 128), (65, 2048, 520), (129, 1024, 2048), (257, 768, 1288), (300, 17408, 256),
-          # 128 x 128 tiles: one, two, three and nine blocks of k, and (with f32
-          # scales two at a time) 16, 17, 33 and 40
+          # 128 x 128 tiles: one, two, three and nine blocks of k, and (two
+          # at a time) 16, 17, 33, 40 and 43
           (700, 128, 4104), (700, 256, 4104), (700, 384, 4104), (1030, 1152, 1032),
           (700, 2048, 1544), (650, 2064, 2056), (140, 4224, 8200), (620, 5120, 2504),
+          (600, 5384, 2504),
           # 256 x 256 tiles: one, two, three and eight blocks
           (2300, 128, 3608), (2300, 256, 3608), (2300, 392, 3608), (2060, 1000, 4104)]
 
