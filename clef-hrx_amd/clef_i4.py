@@ -142,7 +142,7 @@ def _check(rc: int) -> None:
 
 
 class _Native:
-    """The call module (csrc/host_call.cpp: launch, value, pointer, empty) and
+    """The call module (csrc/host_call.cpp: launch, value, pointer, empty, matrix) and
     its handle of every entry point, as attributes; filled on first use."""
 
     def __getattr__(self, name):
@@ -157,7 +157,7 @@ class _Native:
         found = {entry: host.entry(ctypes.cast(getattr(handle, entry), ctypes.c_void_p).value,
                                    "".join("p" if a is _P else "i" for a in args))
                  for entry, (_, args) in SIGNATURES.items()}
-        found.update(launch=host.launch, value=host.value, pointer=host.pointer, empty=host.empty)
+        found.update(launch=host.launch, value=host.value, pointer=host.pointer, empty=host.empty, matrix=host.matrix)
         if name not in found:
             raise AttributeError(name)
         self.__dict__.update(found)
@@ -909,8 +909,8 @@ class PreparedF8:
 
     @property
     def codes(self) -> torch.Tensor:
-        """float8_e4m3fn [rows][width], a view."""
-        return self.storage.view(torch.float8_e4m3fn).as_strided((self.rows, self.width), (self.pitch, 1))
+        """float8_e4m3fn [rows][width], on the buffer's memory."""
+        return _n.matrix(self.storage, torch.float8_e4m3fn, 0, self.rows, self.width, self.pitch, 1)
 
     @property
     def _scales_at(self) -> int:
@@ -918,11 +918,9 @@ class PreparedF8:
 
     @property
     def scales(self) -> torch.Tensor:
-        """f32 [rows][ceil(width / 128)], a view."""
-        words = self.storage.numel() // 4 * 4
-        held = self.storage if words == self.storage.numel() else self.storage[:words]
-        return held.view(torch.float32).as_strided((self.rows, self.pitch // 128), (1, max(self.rows, 1)),
-                                                   self._scales_at // 4)
+        """f32 [rows][ceil(width / 128)], on the buffer's memory."""
+        return _n.matrix(self.storage, torch.float32, self._scales_at, self.rows, self.pitch // 128, 1,
+                         max(self.rows, 1))
 
     def call_arg(self) -> torch.Tensor:
         """The buffer, as large as its rows need."""

@@ -163,6 +163,29 @@ def test_prepare_strided_rows_and_reused_buffer():
         assert torch.equal(a.storage[:n], b.storage) and (a.storage[n:] == 0xAB).all()
 
 
+def test_views_of_a_prepared_activation():
+    """On the buffer's memory, which they keep; refused where they do not fit."""
+    buffer = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    a = clef_i4.prepare_f8(randn((5, 264), 1.0, 1), out=buffer[4096:])
+    codes, scales = a.codes, a.scales
+    assert codes.shape == (5, 264) and codes.stride() == (384, 1) and codes.dtype == F8 and not codes.requires_grad
+    assert scales.shape == (5, 3) and scales.stride() == (1, 5) and scales.dtype == torch.float32
+    assert codes.data_ptr() == buffer.data_ptr() + 4096
+    assert scales.data_ptr() == buffer.data_ptr() + 4096 + 5 * (384 + 16)
+    at = 4096 + torch.arange(5, device="cuda")[:, None] * 384 + torch.arange(264, device="cuda")
+    assert torch.equal(codes.view(torch.uint8), buffer[at])
+    want = buffer[4096 + 5 * 400: 4096 + 5 * 400 + 60].view(torch.float32).view(3, 5).t()
+    assert torch.equal(scales, want)
+    kept = scales.clone()
+    del buffer, a
+    torch.full((1 << 16,), 0xAB, dtype=torch.uint8, device="cuda")
+    assert torch.equal(scales, kept)
+    for wrong in (clef_i4.PreparedF8(codes.view(torch.uint8), 5, 264), clef_i4.PreparedF8(torch.zeros(2000, dtype=torch.uint8, device="cuda"), 5, 264),
+                  clef_i4.PreparedF8(torch.empty(4099, dtype=torch.uint8, device="cuda")[3:], 1, 1280)):
+        with pytest.raises(ValueError):
+            wrong.scales
+
+
 # ---------------------------------------------------------------- weights
 
 @pytest.mark.parametrize("matrices,n,k", [(1, 8, 8), (1, 128, 128), (2, 264, 392), (3, 40, 136)])
