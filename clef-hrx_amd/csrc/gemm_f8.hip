@@ -772,14 +772,21 @@ hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
     return down * ((rows_of_w + bn - 1) / bn);
   };
   if constexpr (LISTS) {
-    // The experts' weights are read once whatever the tile: 16 x 64 tiles for a
-    // few slots (8 slots: 4.7 / 5.3 us down / gate/up against 6.2 / 9.8 on 128 x
-    // 128) and for up to 8 rows per expert over at least 16 blocks of k (60
-    // tokens of 128 experts top-8, gate/up 71 against 74; 240 tokens 92 against
-    // 78; down, 6 blocks of k, 43 against 39).
-    const int64_t rows = x.lists.total / x.lists.experts;
-    if (x.lists.total <= 16 || (rows < 8 && x.kb >= 16)) {
-      if (f8_most_tiles(x.lists.total, x.lists.experts, 16) <= 65535)
+    // Experts with few rows, whose weights are read once whatever the tile. As
+    // many tiles as CUs: 16 x 32, then 16 x 64 (8 slots of 128 experts, down 768 x
+    // 2048: 4.7 us on 16 x 64 against 6.2 on 128 x 128; 46 of 8, 272 x 512: 3.1 on 16
+    // x 32, 3.5, 5.2). More: 16 x 64 up to twelve rows per expert where k has eight
+    // blocks (gate/up 23 blocks x 2 1048, 5.5 rows each of 64: 76 against 83 to 86;
+    // 11 rows: 69 and 69 to 71; 13 rows, 20 blocks: 47 against 41 to 44) or where
+    // the tiles are few (3 blocks, 1456 tiles: 12.5 against 13.3; 3578: 28.3 and
+    // 28.5; 11632: 88 against 78). The experts named: about total E / (total + E).
+    const int64_t total = x.lists.total, experts = x.lists.experts;
+    const int64_t named = total * experts / (total + experts) > 1 ? total * experts / (total + experts) : 1;
+    const int64_t down = named * ((total * 21 / 20 / (total < experts ? total : experts) + 15) / 16);
+    const int64_t narrow = down * ((rows_of_w + 31) / 32), wide = down * ((rows_of_w + 63) / 64);
+    if (f8_most_tiles(total, (int)experts, 16) <= 65535) {
+      if (narrow <= kCus) return launch_stream<1, 2, 2, false, LISTS, GU, RESID>(x, stream);
+      if (wide <= kCus || (total < 12 * experts && (x.kb >= 8 || wide <= 14 * kCus)))
         return launch_stream<1, 4, 2, false, LISTS, GU, RESID>(x, stream);
     }
   } else {

@@ -509,10 +509,11 @@ def test_experts_match_64_bits(tokens, topk, experts, k, n, kind):
     check(got, want[order], slack[order])
 
 
-def test_experts_leave_unlisted_rows_and_odd_lists():
+@pytest.mark.parametrize("n", [136, 2600, 4104])
+def test_experts_leave_unlisted_rows_and_odd_lists(n):
     """Rows behind the last list, slots outside the table and offsets outside
     it or descending: nothing else is written."""
-    k, n, experts, total = 256, 136, 4, 70
+    k, experts, total = 256, 4, 70
     codes, scales = weight(experts, n, k, "f32", 5)
     w = clef_i4.f8_weight(codes, scales)
     a = clef_i4.prepare_f8(randn((total, k), 1.0, 2))
@@ -561,12 +562,13 @@ def test_experts_past_the_first_128(tokens, experts):
     assert torch.equal(got.float(), (ids // 64 * 16 + ids % 64 // 4).float().expand(tokens, n).to(BF).float())
 
 
-def test_experts_overlapping_lists_stay_inside():
+@pytest.mark.parametrize("n", [136, 2048])
+def test_experts_overlapping_lists_stay_inside(n):
     """Lists that name places twice make more tiles than sound ones can: a row
     is one of its experts', nothing else is written."""
-    k, n, total = 128, 136, 1000
+    k, total = 128, 1000
     w = clef_i4.f8_weight(torch.ones((6, n, k), device="cuda").to(F8),
-                          torch.arange(1, 7, device="cuda").float()[:, None, None].expand(6, 2, 1).contiguous())
+                          torch.arange(1, 7, device="cuda").float()[:, None, None].expand(6, -(-n // 128), 1).contiguous())
     x = torch.zeros((total, k), dtype=BF, device="cuda")
     x[:, 3] = 1.0
     offsets = torch.tensor([0, total, 0, total, 0, total, 1], dtype=torch.int32, device="cuda")
