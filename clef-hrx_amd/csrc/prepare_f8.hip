@@ -7,13 +7,13 @@ namespace clef {
 
 namespace {
 
-// x bf16 [rows][width] (row pitch x_stride) -> codes [rows][pitch], scales
-// as e8m0 [rows][kp] and f32 [kb][rows]. 16 lanes hold a block of 128 columns, 8 values each: one 16-byte
-// load, the maximum over the 16 lanes by DPP, one 8-byte store of codes (a
-// whole line per block). A workgroup covers 2^RLOG rows x CPW * STEPS blocks, so
-// that the f32 scales of neighbouring rows go out together, with STEPS loads in
-// flight per lane. Bound by HBM: 2 bytes read and 1 written per value, 5.3 TB/s at
-// 4096 x 12288 (28.4 us).
+// x bf16 [rows][width] (row pitch x_stride) -> codes [rows][pitch], scales as
+// e8m0 [rows][kp] and f32 [kb][rows]. 16 lanes hold a block of 128 columns, 8
+// values each: one 16-byte load, the maximum over the 16 lanes by DPP, one 8-byte
+// store of codes (a whole line per block). A workgroup covers 2^RLOG rows x CPW *
+// STEPS blocks, so that the f32 scales of neighbouring rows go out together, with
+// STEPS loads in flight per lane. Bound by HBM: 2 bytes read and 1 written per
+// value, 5.5 TB/s at 4096 x 12288 (27.6 us).
 template <int RLOG, int STEPS>
 __global__ __launch_bounds__(256) void f8_prepare_kernel(const uint16_t* __restrict__ x, int64_t rows, int width,
                                                          int64_t x_stride, int kb, int kp,
@@ -134,9 +134,9 @@ hipError_t launch_f8_prepare(const uint16_t* x, int64_t rows, int width, int64_t
         <<<grid, 256, 0, stream>>>(x, rows, width, x_stride, kb, kp, codes, exponents, scales);
   };
   using std::integral_constant;
-  // Four loads ahead from 16M values up (4096 x 4096 9.6 us against 10.0 with
-  // two, 32768 x 768 15.4 against 18.1), two below (620 x 17408 7.3 against 8.2).
-  // Four rows per workgroup (4096 x 4096 with 1, 2 or 8: 11.8, 10.0, 11.0), one
+  // Four loads ahead from 16M values up (4096 x 4096 9.0 us against 9.7 with
+  // two, 32768 x 768 13.4 against 15.8), two below (620 x 17408 7.1 against 7.4).
+  // Four rows per workgroup (4096 x 4096 with 1, 2 or 8: 10.4, 9.6, 10.7), one
   // where there are fewer.
   if (rows >= 3 && rows * width >= (1 << 24))
     run(integral_constant<int, 2>{}, integral_constant<int, 4>{});
