@@ -17,10 +17,10 @@ namespace {
 
 // The most values of a tile's rows that a split-k workgroup quantizes itself: ten
 // passes of its threads, 0.3 us each (instructions, and loads of rows that every
-// workgroup reads), against the quantizer's launch (m x k x n, us for both ways:
-// 64 x 512 x 2048 3.6 and 5.1, 8 x 4096 x 2048 5.9 and 7.0, 16 x 2560 x 2048 6.4
-// and 6.8, twelve passes 12 x 4096 x 2048 7.2 and 7.4, 6 x 8192 x 8192 15.2 and
-// 14.3) and the 4 us that its call takes the host.
+// workgroup reads), against the quantizer's launch (m x k x n, us for one launch
+// and for two: 64 x 1536 x 2048, six passes, 4.9 and 5.5; 8 x 4096 x 2048, eight,
+// 5.9 and 6.5; 16 x 2560 x 2048, ten, 6.2 and 6.1, and 8 x 5120 x 8192 11.4 and
+// 10.5) and the 2.5 to 4 us more that two launches take the host (6.3 and 9.0).
 constexpr int kQxValues = 10 * 512 * 8;
 
 // Few rows: each workgroup owns 16 MT rows x 16 NT weight rows (gate/up: NT / 2
@@ -28,12 +28,19 @@ constexpr int kQxValues = 10 * 512 * 8;
 // blocks of k (wave w: blocks w, w + 8, ..). Operands go straight into
 // registers: a weight fragment is two contiguous KiB in the operand order and is
 // used by this workgroup's rows only, so LDS would add a trip and nothing
-// else. D blocks are in flight per wave. The waves' sums meet in LDS and are
-// added in wave order (the result does not depend on timing).
+// else. The waves' sums meet in LDS and are added in wave order (the result does
+// not depend on timing).
+//
+// A wave has one block of k on its way: a second or third costs registers, and
+// with them workgroups per CU, and gained nothing anywhere (16 x 32 tiles, 1, 2
+// and 3 blocks in us: 37 x 4160 x 1352 5.4, 5.8, 5.7; 3 x 15208 x 1960 9.4, 9.5,
+// 10.1; 16 x 64, 60 tokens of 60 experts top-1 gate/up 408 x 2 2968 46, 55, 67). Waves
+// without a block issue nothing: loads through empty resources took as long as
+// others (1 x 448 x 2 1336 with two blocks 3.1 us, 2.6 without them).
 //
 // QX: the rows come in bf16 (p.x) and every workgroup quantizes its tile's into
 // LDS first, by the quantizer's rule, while its first weights are on their way.
-template <int MT, int NT, int D, bool QX, bool LISTS, bool GU, bool RESID>
+template <int MT, int NT, bool QX, bool LISTS, bool GU, bool RESID>
 __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int NW = 8, BM = 16 * MT, COLS = 16 * NT / (GU ? 2 : 1), NG = GU ? NT / 2 : NT;
@@ -58,14 +65,12 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
   // activation rows of this lane: byte and scale offsets (rows past the end
   // read the tile's last row; their sums are not stored)
   int a_voff[MT], s_voff[MT];
-  __amdgpu_buffer_rsrc_t a_rsrc, a_none, s_rsrc, s_none;
+  __amdgpu_buffer_rsrc_t a_rsrc, s_rsrc;
   {
     const uint8_t* base = p.a + (LISTS ? 0 : m0 * pitch);
     const uint32_t bytes = (uint32_t)(LISTS ? p.rows * pitch : (int64_t)here * pitch);
     a_rsrc = make_rsrc(base, bytes);
-    a_none = make_rsrc(base, 0);
     s_rsrc = make_rsrc(p.as, (uint32_t)(p.rows * kb * 4));
-    s_none = make_rsrc(p.as, 0);
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
@@ -136,37 +141,33 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
   struct Block {
     v4i w[NT][2], a[MT][2];
     float sa[MT], sw[MATS];
-  } buf[D];
-  auto load = [&](Block& b, int kt) {
-    // blocks past the end: empty resources, zeros without a request
-    const bool in = kt < kb;
-    const int k = in ? kt : 0;
-    const __amdgpu_buffer_rsrc_t ar = in ? a_rsrc : a_none, sr = in ? s_rsrc : s_none;
+  } b;
+  auto load = [&](int kt) {
+    if (kt >= kb) return;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int mat = j / NG;
-      const __amdgpu_buffer_rsrc_t wr = make_rsrc(wp[mat], in ? panel_bytes : 0u);
+      const __amdgpu_buffer_rsrc_t wr = make_rsrc(wp[mat], panel_bytes);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        b.w[j][h] = __builtin_amdgcn_raw_buffer_load_b128(wr, w_voff + (j % NG) * 2048 + h * 1024, k * 16384, 0);
+        b.w[j][h] = __builtin_amdgcn_raw_buffer_load_b128(wr, w_voff + (j % NG) * 2048 + h * 1024, kt * 16384, 0);
     }
 #pragma unroll
     for (int i = 0; i < (QX ? 0 : MT); ++i) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) b.a[i][h] = __builtin_amdgcn_raw_buffer_load_b128(ar, a_voff[i] + 64 * h, k * 128, 0);
-      b.sa[i] = as_float(__builtin_amdgcn_raw_buffer_load_b32(sr, s_voff[i], (int)(k * p.rows * 4), 0));
+      for (int h = 0; h < 2; ++h) b.a[i][h] = __builtin_amdgcn_raw_buffer_load_b128(a_rsrc, a_voff[i] + 64 * h, kt * 128, 0);
+      b.sa[i] = as_float(__builtin_amdgcn_raw_buffer_load_b32(s_rsrc, s_voff[i], (int)(kt * p.rows * 4), 0));
     }
 #pragma unroll
     for (int m = 0; m < MATS; ++m)
-      b.sw[m] = as_float(__builtin_amdgcn_raw_buffer_load_b32(make_rsrc(wsp[m], in ? (uint32_t)kb * 4u : 0u), 0, k * 4, 0));
+      b.sw[m] = as_float(__builtin_amdgcn_raw_buffer_load_b32(make_rsrc(wsp[m], (uint32_t)kb * 4u), 0, kt * 4, 0));
   };
   v4f acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0, 0, 0, 0};
-#pragma unroll
-  for (int d = 0; d < D; ++d) load(buf[d], wave + NW * d);
+  load(wave);
   if constexpr (QX) {
     __builtin_amdgcn_sched_barrier(0);
     q_store(0);
@@ -176,39 +177,33 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
     }
     __syncthreads();
   }
-  for (int k0 = wave; k0 < kb; k0 += NW * D) {
-#pragma unroll
-    for (int d = 0; d < D; ++d) {
-      Block& b = buf[d];
-      if constexpr (QX) {
-        // (blocks past the end multiply zeros)
-        const int k = k0 + NW * d < kb ? k0 + NW * d : 0;
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const int r = 16 * i + lr, row = r < here ? r : here - 1;
-          const char* at = q_codes + row * q_pitch + k * 128 + 16 * g;
-          b.a[i][0] = *reinterpret_cast<const v4i*>(at);
-          b.a[i][1] = *reinterpret_cast<const v4i*>(at + 64);
-          b.sa[i] = k0 + NW * d < kb ? q_scales[row * kb + k] : 0.0f;
-        }
-      }
+  for (int k = wave; k < kb; k += NW) {
+    if constexpr (QX) {
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const v8i_t av = join_halves(b.a[i][0], b.a[i][1]);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const v4f part = mfma_f8(join_halves(b.w[j][0], b.w[j][1]), av, v4f{0, 0, 0, 0});
-          const float s = b.sa[i] * b.sw[j / NG];
-#pragma unroll
-          for (int t = 0; t < 4; ++t) acc[i][j][t] = __builtin_fmaf(part[t], s, acc[i][j][t]);
-        }
+        const int r = 16 * i + lr, row = r < here ? r : here - 1;
+        const char* at = q_codes + row * q_pitch + k * 128 + 16 * g;
+        b.a[i][0] = *reinterpret_cast<const v4i*>(at);
+        b.a[i][1] = *reinterpret_cast<const v4i*>(at + 64);
+        b.sa[i] = q_scales[row * kb + k];
       }
-      // the order as written: loads drawn up to here would need registers of
-      // their own for every block in flight
-      __builtin_amdgcn_sched_barrier(0);
-      load(buf[d], k0 + NW * (D + d));
-      __builtin_amdgcn_sched_barrier(0);
     }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const v8i_t av = join_halves(b.a[i][0], b.a[i][1]);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const v4f part = mfma_f8(join_halves(b.w[j][0], b.w[j][1]), av, v4f{0, 0, 0, 0});
+        const float s = b.sa[i] * b.sw[j / NG];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[i][j][t] = __builtin_fmaf(part[t], s, acc[i][j][t]);
+      }
+    }
+    // the order as written: loads drawn up to here would need registers of
+    // their own for another block
+    __builtin_amdgcn_sched_barrier(0);
+    load(k + NW);
+    __builtin_amdgcn_sched_barrier(0);
   }
   // the waves' sums: fragment (i, j) of wave w at ((w MT + i) NT + j) KiB
   v4f* sums = reinterpret_cast<v4f*>(lds);
@@ -253,7 +248,7 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8Args p) {
 #endif
 }
 
-template <int MT, int NT, int D, bool QX, bool LISTS, bool GU, bool RESID>
+template <int MT, int NT, bool QX, bool LISTS, bool GU, bool RESID>
 hipError_t launch_stream(const F8Args& x, hipStream_t stream) {
   constexpr int BM = 16 * MT, COLS = 16 * NT / (GU ? 2 : 1), sums = 8 * MT * NT * 1024;
   static_assert(128 % COLS == 0, "a tile's columns lie in one weight block");
@@ -261,7 +256,7 @@ hipError_t launch_stream(const F8Args& x, hipStream_t stream) {
   constexpr int most = sums + (QX ? kQxValues + 16 * BM + kQxValues / 32 : 0);
   static_assert(most <= 160 * 1024, "LDS of a workgroup");
   static LaunchCache cache;
-  auto* kernel = &f8_stream_kernel<MT, NT, D, QX, LISTS, GU, RESID>;
+  auto* kernel = &f8_stream_kernel<MT, NT, QX, LISTS, GU, RESID>;
   if (most > 64 * 1024)
     if (hipError_t e = ensure_dynamic_lds(cache, reinterpret_cast<const void*>(kernel), most)) return e;
   const int lds = sums + (QX ? (int)(x.rows < BM ? x.rows : BM) * (x.kb * 132 + 16) : 0);
@@ -736,10 +731,11 @@ hipError_t launch_tile(const F8Args& x, hipStream_t stream) {
 constexpr int64_t kCus = 256;
 
 // Tiles of the split-k kernel for m rows against n weight rows (gate/up: both).
-enum class StreamShape { kNone, k16x32, k16x64, k32x64, k64x64 };
+enum class StreamShape { kNone, k16x32, k32x32, k16x64, k32x64, k64x64 };
 StreamShape stream_shape(int64_t m, int64_t n) {
   auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); };
   if (tiles(16, 32) <= kCus || (m <= 16 && tiles(16, 64) > kCus)) return StreamShape::k16x32;
+  if (m <= 32 && tiles(32, 32) <= kCus) return StreamShape::k32x32;
   if (tiles(16, 64) <= kCus) return StreamShape::k16x64;
   if (tiles(32, 64) <= kCus) return StreamShape::k32x64;
   return tiles(64, 64) <= kCus ? StreamShape::k64x64 : StreamShape::kNone;
@@ -747,8 +743,10 @@ StreamShape stream_shape(int64_t m, int64_t n) {
 
 // The kernel of a shape. From the smallest tiles up: 16 x 32, 16 x 64, 32 x 64
 // and 64 x 64 of the split-k kernel while they are at most one per CU (m x k x n
-// in us: 256 x 2048 x 512 4.1 on 16 x 32 tiles, 5.0, 6.3, 8.0 on the larger
-// ones; 384 x 512 x 2048 8.6, 6.5, 6.8 and 4.7); beyond, 128 x 128 tiles, two
+// in us: 133 x 5784 x 288 6.3 on 16 x 32 tiles, 7.9, 10.7, 16.3 on the larger
+// ones; 170 x 3600 x 3808 24.8, 14.1, 15.2 and 12.5), and 32 x 32 where one tile
+// has all rows and reads the weights once (20 x 14512 x 6848 20.8 against 29.5 on
+// 16 x 64, 29 x 1072 x 7976 3.7 against 5.1); beyond, 128 x 128 tiles, two
 // workgroups per CU (256 x 4096 x 12288: 19 against 39 on 64 x 64), and 256 x
 // 256 tiles from three times their rounds over the CUs up, a 256 x 256 round
 // taking about three of 128 x 128 (1024 x 4096 x 12288, 1 and 3 rounds: 49
@@ -773,36 +771,36 @@ hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
   };
   if constexpr (LISTS) {
     // Experts with few rows, whose weights are read once whatever the tile. As
-    // many tiles as CUs: 16 x 32, then 16 x 64 (8 slots of 128 experts, down 768 x
-    // 2048: 4.7 us on 16 x 64 against 6.2 on 128 x 128; 46 of 8, 272 x 512: 3.1 on 16
-    // x 32, 3.5, 5.2). More: 16 x 64 up to twelve rows per expert where k has eight
-    // blocks (gate/up 23 blocks x 2 1048, 5.5 rows each of 64: 76 against 83 to 86;
-    // 11 rows: 69 and 69 to 71; 13 rows, 20 blocks: 47 against 41 to 44) or where
-    // the tiles are few (3 blocks, 1456 tiles: 12.5 against 13.3; 3578: 28.3 and
-    // 28.5; 11632: 88 against 78). The experts named: about total E / (total + E).
+    // many tiles as CUs: 16 x 32, then 16 x 64 (8 slots of 128 experts, gate/up 2048
+    // x 2 768: 4.6 us on 16 x 64, 4.7 on 16 x 32 and 9.8 on 128 x 128; 57 of 8, 2928 x
+    // 464: 4.8 on 16 x 32, 5.6, 12.9). More: 16 x 64 below sixteen rows per expert
+    // (gate/up, 540 slots of 128 568 x 2 1440 40.6 against 51.7 on 128 x 128, 793 of
+    // 60 3112 x 2 712 51.7 against 53.5; 1063 of 64 584 x 2 256, 16.6 rows each, 8.9
+    // against 7.9). The experts named: about total E / (total + E).
     const int64_t total = x.lists.total, experts = x.lists.experts;
     const int64_t named = total * experts / (total + experts) > 1 ? total * experts / (total + experts) : 1;
     const int64_t down = named * ((total * 21 / 20 / (total < experts ? total : experts) + 15) / 16);
     const int64_t narrow = down * ((rows_of_w + 31) / 32), wide = down * ((rows_of_w + 63) / 64);
     if (f8_most_tiles(total, (int)experts, 16) <= 65535) {
-      if (narrow <= kCus) return launch_stream<1, 2, 2, false, LISTS, GU, RESID>(x, stream);
-      if (wide <= kCus || (total < 12 * experts && (x.kb >= 8 || wide <= 14 * kCus)))
-        return launch_stream<1, 4, 2, false, LISTS, GU, RESID>(x, stream);
+      if (narrow <= kCus) return launch_stream<1, 2, false, LISTS, GU, RESID>(x, stream);
+      if (wide <= kCus || total < 16 * experts) return launch_stream<1, 4, false, LISTS, GU, RESID>(x, stream);
     }
   } else {
     const StreamShape shape = stream_shape(x.rows, rows_of_w);
     if constexpr (!GU)
       if (x.x != nullptr) switch (shape) {  // f8_project_fusable
-          case StreamShape::k16x32: return launch_stream<1, 2, 2, true, false, false, RESID>(x, stream);
-          case StreamShape::k16x64: return launch_stream<1, 4, 2, true, false, false, RESID>(x, stream);
-          case StreamShape::k32x64: return launch_stream<2, 4, 2, true, false, false, RESID>(x, stream);
+          case StreamShape::k16x32: return launch_stream<1, 2, true, false, false, RESID>(x, stream);
+          case StreamShape::k32x32: return launch_stream<2, 2, true, false, false, RESID>(x, stream);
+          case StreamShape::k16x64: return launch_stream<1, 4, true, false, false, RESID>(x, stream);
+          case StreamShape::k32x64: return launch_stream<2, 4, true, false, false, RESID>(x, stream);
           default: return hipErrorInvalidValue;
         }
     switch (shape) {
-      case StreamShape::k16x32: return launch_stream<1, 2, 2, false, LISTS, GU, RESID>(x, stream);
-      case StreamShape::k16x64: return launch_stream<1, 4, 2, false, LISTS, GU, RESID>(x, stream);
-      case StreamShape::k32x64: return launch_stream<2, 4, 2, false, LISTS, GU, RESID>(x, stream);
-      case StreamShape::k64x64: return launch_stream<4, 4, 1, false, LISTS, GU, RESID>(x, stream);
+      case StreamShape::k16x32: return launch_stream<1, 2, false, LISTS, GU, RESID>(x, stream);
+      case StreamShape::k32x32: return launch_stream<2, 2, false, LISTS, GU, RESID>(x, stream);
+      case StreamShape::k16x64: return launch_stream<1, 4, false, LISTS, GU, RESID>(x, stream);
+      case StreamShape::k32x64: return launch_stream<2, 4, false, LISTS, GU, RESID>(x, stream);
+      case StreamShape::k64x64: return launch_stream<4, 4, false, LISTS, GU, RESID>(x, stream);
       default: break;
     }
   }
@@ -834,9 +832,9 @@ hipError_t launch_f8_gemm(const F8Args& x, bool gate_up, hipStream_t stream) {
 
 bool f8_project_fusable(int64_t m, int n, int k) {
   const StreamShape shape = stream_shape(m, n);
-  const int rows = shape == StreamShape::k16x32 || shape == StreamShape::k16x64 ? 16
-                   : shape == StreamShape::k32x64                               ? 32
-                                                                                : 0;
+  const int rows = shape == StreamShape::k16x32 || shape == StreamShape::k16x64   ? 16
+                   : shape == StreamShape::k32x32 || shape == StreamShape::k32x64 ? 32
+                                                                                  : 0;
   return rows > 0 && (m < rows ? m : rows) * f8_pitch(k) <= kQxValues;
 }
 

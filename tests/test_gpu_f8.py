@@ -224,6 +224,7 @@ def test_weight_layout(matrices, n, k):
 
 SHAPES = [(1, 128, 128), (1, 4096, 1024), (3, 136, 8), (16, 1000, 264), (17, 264, 1352), (37, 4160, 1352),
           (64, 512, 128), (65, 2048, 520), (129, 1024, 2048), (257, 768, 1288), (300, 17408, 256),
+          (20, 1200, 6848), (31, 392, 4104), (24, 520, 4000),
           # 128 x 128 tiles: one, two, three and nine blocks of k, and (two
           # at a time) 16, 17, 33, 40 and 43
           (700, 128, 4104), (700, 256, 4104), (700, 384, 4104), (1030, 1152, 1032),
@@ -293,11 +294,11 @@ def test_project_of_whole_numbers_is_exact(m, k, n, kind):
 
 
 @pytest.mark.parametrize("m,k,n", [
-    # one launch on 16 x 32, 16 x 64 and 32 x 64 tiles: one row to many tiles of
+    # one launch on 16 x 32, 32 x 32, 16 x 64 and 32 x 64 tiles: one row to many tiles of
     # rows, the last of them short; blocks that end inside; one pass to ten
     (1, 8, 8), (1, 16384, 256), (2, 20480, 264), (3, 12288, 520), (5, 8192, 136), (9, 4104, 1000), (10, 4096, 2048),
     (16, 2560, 32), (17, 2560, 392), (33, 128, 3992), (130, 1000, 520), (250, 512, 1096), (255, 1280, 1016),
-    (513, 1032, 1000), (1000, 264, 520), (4095, 128, 64),
+    (513, 1032, 1000), (1000, 264, 520), (4095, 128, 64), (20, 1200, 6848), (31, 1280, 4104),
     # and rows or widths just past it
     (11, 4096, 2048), (16, 2568, 32), (3, 20480, 264), (64, 1400, 5000)])
 @pytest.mark.parametrize("res", [False, True])
