@@ -90,6 +90,7 @@ hipError_t launch_group_slots(const float* routes, int64_t tokens, int topk, int
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef int v8i_t __attribute__((ext_vector_type(8)));
 
@@ -111,6 +112,21 @@ __device__ __forceinline__ v4f mfma_f8_scaled(v8i_t w, v8i_t a, v4f c, int sw, u
     case 2: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 3, sw, 2, (int)sa);
     default: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 3, sw, 3, (int)sa);
   }
+}
+
+// Any f32 scale as 2^e for the MFMA (e8m0 in byte 3) and a factor of magnitude
+// 1 .. 2 for the fma behind it: with both powers of two in the MFMA a block's
+// partial sum leaves f32's range only where the product itself does. Scales
+// below 2^-126 (zero among them) take 2^-127, the least there is, and a
+// smaller factor; infinities and NaN are the factor themselves.
+struct F8Split {
+  int exponent;
+  float factor;
+};
+__device__ __forceinline__ F8Split f8_split_scale(float s) {
+  const uint32_t bits = as_uint(s), field = bits >> 23 & 0xFFu;
+  if (field == 255u) return {127 << 24, s};
+  return {(int)(bits << 1), field == 0u ? s * 0x1p127f : as_float((bits & 0x807FFFFFu) | 0x3F800000u)};
 }
 
 __device__ __forceinline__ v8i_t join_halves(v4i lo, v4i hi) {

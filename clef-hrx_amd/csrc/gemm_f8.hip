@@ -1,10 +1,12 @@
 // Block-scaled FP8 products for gfx950 (layouts and the formula in f8.hpp).
 //
 // A block's codes are multiplied by v_mfma_scale_f32_16x16x128_f8f6f4 (one
-// instruction covers a block's 128 k, accumulating in f32), and the partial
-// sum enters the f32 accumulator by one fma with sa[m] sw: a scale pair is
-// rounded once, a block's sum once more in the fma. Output values are rounded
-// to bf16 once, behind the residual or SwiGLU. Inside the instruction the
+// instruction covers a block's 128 k, accumulating in f32). The split-k kernel
+// adds the partial sum to the f32 accumulator by one fma with sa[m] sw; the
+// tiled kernel has the powers of two of both scales in the instruction, which
+// adds to the accumulator itself where that is all of them, and else leaves an
+// fma with the rest of sw. A block's sum is rounded once more on the way. Output
+// values are rounded to bf16 once, behind the residual or SwiGLU. Inside the instruction the
 // products of eight neighbouring k are cut to 2^-13 of the largest of them (a
 // property of the FP8 matrix unit, measured with single products beside a pair
 // that cancels); the eights and everything behind them add in f32. Against 64
@@ -274,8 +276,9 @@ hipError_t launch_stream(const F8Args& x, hipStream_t stream) {
 // chunk c of row r at c ^ ((r >> 1) & 7)) and B fragments in the operand order.
 // Behind the stages the rows' e8m0 scales of 16 blocks of k, as loaded (16 bytes
 // per row) and, twice, turned into the order of use (per block of k a lane's TM
-// rows side by side), the scales of the tile's one or two weight panels (256 f32
-// each) and, with lists, the tile's output rows.
+// rows side by side), the scales of the tile's one or two weight panels (256
+// each, as they are or as pairs of the MFMA's exponent and the fma's factor) and, with lists, the
+// tile's output rows.
 template <int WM_, int WN_, int WAVES_M_, int WAVES_N_, int GROUPS_ = 1, int KG_ = 1>
 struct F8Tile {
   static constexpr int GROUPS = GROUPS_;  // workgroups per CU
@@ -291,7 +294,7 @@ struct F8Tile {
   // rows of its first TM / 2 activation fragments, then (Y) the other rows
   static constexpr int Y = A_SLOTS / 2, X = B_SLOTS + A_SLOTS - Y, DMA = X + Y;
   static constexpr int SA_BYTES = BM * 16, SA = NST * STAGE_BYTES, ST = SA + SA_BYTES, SW = ST + 2 * SA_BYTES;
-  static constexpr int ROWS = SW + 2 * 1024;
+  static constexpr int ROWS = SW + 2 * 2048;
   static constexpr int LDS = ROWS + BM * 4;
   static constexpr int EPI = 16 * WN * 2;            // epilogue staging per wave
   static_assert(NW == 8 && (BN == 256 || BN == 128) && BM / 64 <= NW, "eight waves, one or two weight panels");
@@ -308,10 +311,12 @@ struct F8Tile {
 // fragments. It holds the weight fragments of the step and reads an activation
 // fragment one row of MFMAs ahead of its use. The rows' scales,
 // powers of two, go into the MFMA. So do the weight's where they are (HW), and
-// the MFMA adds to the accumulator itself; other weight scales are applied by
-// four fmas to a partial sum two MFMAs after the MFMA that made it (half the
-// MFMAs' issue time, run under them; with the rows' scales in those fmas 1711 x
-// 5120 x 2 17408 took 295 us, not 288).
+// the MFMA adds to the accumulator itself. Of other weight scales the power of
+// two goes there too (f8_split_scale), and the factor that is left is applied by four
+// fmas to a partial sum two MFMAs after the MFMA that made it (half the MFMAs'
+// issue time, run under them; with the rows' scales in those fmas 1711 x 5120 x 2
+// 17408 took 295 us, not 288, and with all of the weight's 273, not 275, but
+// partial sums of rows of 1e35 and more overflowed).
 //
 // A stage of LDS is filled in two parts: X (weights, the first half of each
 // wave's activation rows) and Y (the other half). Behind a barrier in the
@@ -406,13 +411,12 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
     }
   };
   issue_scales(0);
-  // and of the panels (gate/up: gate, up), as f32
+  // and of the panels (gate/up: gate, up), a thread each
+  float panel_scale = 0.0f;
   {
     const int q = threadIdx.x >> 8, k = threadIdx.x & 255;
     const int of = n0 / 128 + (GU ? 0 : q);
-    float v = 0.0f;
-    if (k < kb && of < nb) v = (GU && q ? p.ws2 : p.ws)[first_block + (int64_t)of * kb + k];
-    reinterpret_cast<float*>(lds + T::SW)[threadIdx.x] = v;
+    if (k < kb && of < nb) panel_scale = (GU && q ? p.ws2 : p.ws)[first_block + (int64_t)of * kb + k];
   }
   if constexpr (LISTS) {
     for (int r = threadIdx.x; r < T::BM; r += T::THREADS) {
@@ -442,7 +446,8 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
   const int a_at0 = kg * T::A_BLOCK + (wm * T::WM + lr) * 128 + ((g ^ (lr >> 1)) << 4), a_at1 = a_at0 ^ 64;
   const int b_at = T::A_BYTES + kg * T::B_BLOCK + (GU ? wn * (TN / 2) : wn * TN) * 2048 + lane * 16;
   const char* const sa_at = lds + T::ST + wm * T::WM + lr * TM;
-  const float* const sw_at = reinterpret_cast<const float*>(lds + T::SW) + (GU ? 0 : wn * T::WN / 128) * 256;
+  using Panel = std::conditional_t<HW, float, v2f>;
+  const Panel* const sw_at = reinterpret_cast<const Panel*>(lds + T::SW) + (GU ? 0 : wn * T::WN / 128) * 256;
 
   v4f acc[TM][TN];
 #pragma unroll
@@ -453,9 +458,9 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
     constexpr int MATS = GU ? 2 : 1;
     v8i_t av[2], bv[TN];
     v4f part[4];               // !HW: partial sums on their way
-    float sv[MATS], last[MATS];  // !HW: the panels' scales in this step and in the one before
+    float sv[MATS], last[MATS];  // !HW: the panels' factors in this step and in the one before
     uint32_t sa[TM / 4], sa_next[TM / 4];  // the rows' exponents, four in each
-    int sw_bits[MATS];         // HW: the panels' scales, exponent in the top byte
+    int sw_bits[MATS];         // the panels' exponents, in the top byte
     auto read_a = [&](const char* stage, int i) {
       const v4i lo = *reinterpret_cast<const v4i*>(stage + a_at0 + i * 2048);
       const v4i hi = *reinterpret_cast<const v4i*>(stage + a_at1 + i * 2048);
@@ -465,7 +470,7 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
       const char* at = stage + b_at + (GU && j >= TN / 2 ? T::B_BLOCK / 2 + (j - TN / 2) * 2048 : j * 2048);
       return join_halves(*reinterpret_cast<const v4i*>(at), *reinterpret_cast<const v4i*>(at + 1024));
     };
-    float sw[MATS];
+    Panel sw[MATS];
     // of step kt (the step before still takes sa)
     auto read_scales = [&](int kt) {
       const int block = T::KG * kt + kg;  // (a block past the last: its products are zeros)
@@ -485,8 +490,9 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
         if constexpr (HW) {
           sw_bits[t] = (int)(as_uint(sw[t]) << 1);
         } else {
+          sw_bits[t] = (int)as_uint(sw[t][0]);
           last[t] = sv[t];
-          sv[t] = sw[t];
+          sv[t] = sw[t][1];
         }
       }
     };
@@ -512,11 +518,12 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
+          const int bits = sw_bits[GU && j >= TN / 2 ? 1 : 0];
           if constexpr (HW) {
-            acc[i][j] = mfma_f8_scaled(bv[j], av[i & 1], acc[i][j], sw_bits[GU && j >= TN / 2 ? 1 : 0], sa[i / 4], i % 4);
+            acc[i][j] = mfma_f8_scaled(bv[j], av[i & 1], acc[i][j], bits, sa[i / 4], i % 4);
             __builtin_amdgcn_sched_barrier(0);
           } else {
-            part[(i * TN + j) % 4] = mfma_f8_scaled(bv[j], av[i & 1], v4f{0, 0, 0, 0}, 127 << 24, sa[i / 4], i % 4);
+            part[(i * TN + j) % 4] = mfma_f8_scaled(bv[j], av[i & 1], v4f{0, 0, 0, 0}, bits, sa[i / 4], i % 4);
             __builtin_amdgcn_sched_barrier(0);
             // the MFMA two before
             const int before = i * TN + j - 2, ii = (before + TM * TN) / TN % TM, jj = (before + TN) % TN;
@@ -539,12 +546,18 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
       take_scales();
     };
     // the weights of both stages are on their way; then the first scales (turned
-    // once they have landed) and the rows
+    // and split once they have landed) and the rows
 #pragma unroll
     for (int x = T::B_SLOTS; x < T::DMA; ++x) issue(r0, 0, x);
 #pragma unroll
     for (int x = T::B_SLOTS; x < T::DMA; ++x) issue(r1, 1, x);
     wait_vmcnt<2 * T::A_SLOTS>();
+    if constexpr (HW) {
+      reinterpret_cast<float*>(lds + T::SW)[threadIdx.x] = panel_scale;
+    } else {
+      const F8Split split = f8_split_scale(panel_scale);
+      reinterpret_cast<v2f*>(lds + T::SW)[threadIdx.x] = v2f{as_float((uint32_t)split.exponent), split.factor};
+    }
     turn_scales(0);
     wait_vmcnt<T::A_SLOTS>();
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");

@@ -385,6 +385,62 @@ def test_project_scales_at_their_limits(m):
     assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
 
 
+# one of each kernel: quantizing its rows itself, few rows, 128 x 128 tiles (two
+# blocks of k at a time, one at a time), 256 x 256 tiles and their shape of half the rows
+ENDS = [(5, 4104, 264), (64, 512, 2000), (700, 2064, 1544), (700, 256, 4104), (2300, 392, 3608), (2100, 392, 4104)]
+
+
+def scaled_weight(matrices, n, k, kind, p, seed):
+    """The same codes for every p, scales (of full mantissas in f32) times 2^p."""
+    codes = randn((matrices, n, k), 60.0, seed, torch.float32).clamp(-448, 448).to(F8)
+    scales = torch.rand((matrices, -(-n // 128), -(-k // 128)), generator=gen(seed + 1), device="cuda")
+    scales = torch.exp2(-torch.floor(4 * scales)) if kind == "e8m0" else 0.6 + 0.9 * scales
+    scales = torch.ldexp(scales * 2.0 ** -6, torch.tensor(p + 6, device="cuda"))
+    return clef_i4.f8_weight(codes, scales.to(torch.float8_e8m0fnu) if kind == "e8m0" else scales)
+
+
+def one(w):
+    return clef_i4.F8Weight(w.codes, w.scales[0], w.rows, w.cols, 1, w.pow2)
+
+
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+@pytest.mark.parametrize("p", [123, -118])
+@pytest.mark.parametrize("m,k,n", ENDS)
+def test_project_rows_at_the_ends_of_bf16(m, k, n, p, kind):
+    """Rows times 2^p against weights times 2^-p: the same bits as without, since
+    every step only multiplies by powers of two in between, while a row's scale
+    times a sum of codes is far outside f32 (p = 123) or the weight's scale large."""
+    x = whole((m, k), 15, m + k)
+    far = torch.ldexp(x, torch.tensor(p, device="cuda")).to(BF)
+    assert torch.equal(torch.ldexp(far.double(), torch.tensor(-p, device="cuda")).float(), x)
+    x, res = x.to(BF), randn((m, n), 300.0, 3)
+    near_w, far_w = (one(scaled_weight(1, n, k, kind, e, 5)) for e in (0, -p))
+    want = clef_i4.project_quantized_f8(x, near_w, res)
+    assert torch.isfinite(want).all()
+    assert torch.equal(clef_i4.project_quantized_f8(far, far_w, res), want)
+    near_u, far_u = (one(scaled_weight(1, n, k, kind, e, 7)) for e in (0, -p))
+    want = clef_i4.project_gate_up_f8(clef_i4.prepare_f8(x), near_w, near_u)
+    assert torch.isfinite(want).all()
+    assert torch.equal(clef_i4.project_gate_up_f8(clef_i4.prepare_f8(far), far_w, far_u), want)
+
+
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+@pytest.mark.parametrize("p", [123, -118])
+@pytest.mark.parametrize("tokens,experts,k,n", [(20, 16, 264, 520), (900, 5, 256, 392), (3000, 4, 264, 3000)])
+def test_experts_rows_at_the_ends_of_bf16(tokens, experts, k, n, p, kind):
+    """The same over lists."""
+    (offsets, slots), _ = lists(tokens, 1, experts, tokens)
+    x = whole((tokens, k), 15, tokens + k)
+    far = clef_i4.prepare_f8(torch.ldexp(x, torch.tensor(p, device="cuda")).to(BF))
+    near = clef_i4.prepare_f8(x.to(BF))
+    near_w, far_w = (scaled_weight(experts, n, k, kind, e, 5) for e in (0, -p))
+    want = clef_i4.expert_f8(near, near_w, offsets, slots, 1, True)
+    assert torch.isfinite(want).all()
+    assert torch.equal(clef_i4.expert_f8(far, far_w, offsets, slots, 1, True), want)
+    want = clef_i4.expert_gate_up_f8(near, near_w, near_w, offsets, slots, 1, True)
+    assert torch.equal(clef_i4.expert_gate_up_f8(far, far_w, far_w, offsets, slots, 1, True), want)
+
+
 def test_rows_and_slots_beyond_4_gib():
     """Activations whose bytes do not fit 32 bits (rows of a projection) or
     just do (an expert's), read at their end."""
