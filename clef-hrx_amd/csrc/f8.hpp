@@ -97,14 +97,9 @@ typedef int v8i_t __attribute__((ext_vector_type(8)));
 // D = W A^T of a 16 x 16 tile over 128 k, added to c. Lane l holds weight row
 // l % 16 in w and activation row l % 16 in a, the 32 values of its k-group
 // l / 16 (any order of k that both share); D's lane l holds activation row
-// l % 16 and weight rows 4 (l / 16) .. + 3. cbsz = blgp = 0: e4m3 both, block
-// scales 127 (e8m0) = 1.
-__device__ __forceinline__ v4f mfma_f8(v8i_t w, v8i_t a, v4f c) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 0, 127, 0, 127);
-}
-
-// The same with the scales in the MFMA: e8m0 exponents, in byte 3 of sw (of w's
-// rows) and byte `byte` (known when compiled) of sa (of a's rows; lane l's row l % 16).
+// l % 16 and weight rows 4 (l / 16) .. + 3. cbsz = blgp = 0: e4m3 both. The
+// scales are e8m0 exponents, in byte 3 of sw (of w's rows) and byte `byte`
+// (known when compiled) of sa (of a's rows; lane l's row l % 16).
 __device__ __forceinline__ v4f mfma_f8_scaled(v8i_t w, v8i_t a, v4f c, int sw, uint32_t sa, int byte) {
   switch (byte) {
     case 0: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 3, sw, 0, (int)sa);
@@ -117,16 +112,16 @@ __device__ __forceinline__ v4f mfma_f8_scaled(v8i_t w, v8i_t a, v4f c, int sw, u
 // Any f32 scale as 2^e for the MFMA (e8m0 in byte 3) and a factor of magnitude
 // 1 .. 2 for the fma behind it: with both powers of two in the MFMA a block's
 // partial sum leaves f32's range only where the product itself does. Scales
-// below 2^-126 (zero among them) take 2^-127, the least there is, and a
-// smaller factor; infinities and NaN are the factor themselves.
+// below 2^-126 take 2^-127, the least there is, and a smaller factor; zero,
+// infinities and NaN are the factor themselves.
 struct F8Split {
   int exponent;
   float factor;
 };
 __device__ __forceinline__ F8Split f8_split_scale(float s) {
-  const uint32_t bits = as_uint(s), field = bits >> 23 & 0xFFu;
-  if (field == 255u) return {127 << 24, s};
-  return {(int)(bits << 1), field == 0u ? s * 0x1p127f : as_float((bits & 0x807FFFFFu) | 0x3F800000u)};
+  const int e = __builtin_amdgcn_frexp_expf(s);  // |s| in 2^(e - 1) .. 2^e; 0 for zero, infinities and NaN
+  const int up = e < -126 ? -126 : e;
+  return {(up + 126) << 24, __builtin_ldexpf(s, 1 - up)};
 }
 
 __device__ __forceinline__ v8i_t join_halves(v4i lo, v4i hi) {

@@ -533,8 +533,9 @@ int clef_f8_retile(const uint8_t* w, int64_t matrices, int32_t n, int32_t k, uin
  * and 2^127, as clef_f8_pack_weight and e8m0 checkpoints make them; the matrix
  * unit may then apply them (with other
  * scales it would drop their mantissas). The same sums within f32 rounding.
- * Products of an activation's scale and a weight's are formed in f32. The
- * output may be the residual itself and overlaps no other input. */
+ * Scales of any size: a block's sum leaves f32's range only where it does with
+ * both of its scales applied. The output may be the residual itself and overlaps
+ * no other input. */
 int clef_f8_gemm(const uint8_t* a, const uint8_t* w, const float* w_scales, int64_t m,
                  int32_t n, int32_t k, int32_t pow2, const uint16_t* residual, uint16_t* out, clef_stream_t stream);
 

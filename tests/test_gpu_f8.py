@@ -424,6 +424,44 @@ def test_project_rows_at_the_ends_of_bf16(m, k, n, p, kind):
     assert torch.equal(clef_i4.project_gate_up_f8(clef_i4.prepare_f8(far), far_w, far_u), want)
 
 
+def same_bits(got, want64):
+    """want64 has at most 24 bits: f32 holds it, and bf16 rounds it once."""
+    assert torch.equal(want64.float().double(), want64)
+    assert torch.equal(got.view(torch.int16), want64.float().to(BF).view(torch.int16))
+
+
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+@pytest.mark.parametrize("m,k,n", ENDS)
+def test_project_scales_whose_product_leaves_f32(m, k, n, kind):
+    """Sums in f32's range whose scales multiply to more than its largest value
+    (2^119 times 2^10: each block's largest value meets a weight of zero) or to
+    less than its smallest normal (2^-126 times 2^-18). Whole numbers, blocks and
+    rows chosen so that f32 loses nothing: bit for bit."""
+    nb, kb = -(-n // 128), -(-k // 128)
+
+    def product(x, w, scale):
+        scales = torch.full((nb, kb), scale, device="cuda")
+        packed = clef_i4.f8_weight(w.to(F8), scales.to(torch.float8_e8m0fnu) if kind == "e8m0" else scales)
+        want = x.double() @ w.to(F8).double().t() * scales[0, 0].double()
+        same_bits(clef_i4.project_quantized_f8(x.to(BF), packed), want)
+        h = clef_i4.project_gate_up_f8(clef_i4.prepare_f8(x.to(BF)), packed, packed)
+        assert not torch.isnan(h).any()
+
+    # two of a block's values count, in an eight of their own: sums of few bits
+    x = torch.zeros((m, k), device="cuda")
+    x[:, 9::128] = whole((m, x[:, 9::128].shape[1]), 7, m) * 2.0 ** 110
+    x[:, 13::128] = whole((m, x[:, 13::128].shape[1]), 7, m + 1) * 2.0 ** 110
+    x[:, 0::128] = 2.0 ** 127
+    w = whole((n, k), 7, n) * 2.0 ** -9
+    w[:, 0::128] = 0
+    product(x, w, 1.375 * 2.0 ** 10 if kind == "f32" else 2.0 ** 10)
+    x = (7.5 + whole((m, k), 7, m) / 2).floor() * 2.0 ** -122  # 4 .. 11
+    x[:, 0::128] = 15 * 2.0 ** -122
+    w = 32 * (12 + whole((n, k), 2, n))  # 320 .. 448
+    w = w * (torch.arange(k, device="cuda") % 128 < 8)
+    product(x, w, 85 * 2.0 ** -24 if kind == "f32" else 2.0 ** -18)
+
+
 @pytest.mark.parametrize("kind", ["f32", "e8m0"])
 @pytest.mark.parametrize("p", [123, -118])
 @pytest.mark.parametrize("tokens,experts,k,n", [(20, 16, 264, 520), (900, 5, 256, 392), (3000, 4, 264, 3000)])
