@@ -112,16 +112,17 @@ __device__ __forceinline__ v4f mfma_f8_scaled(v8i_t w, v8i_t a, v4f c, int sw, u
 // Any f32 scale as 2^e for the MFMA (e8m0 in byte 3) and a factor of magnitude
 // 1 .. 2 for the fma behind it: with both powers of two in the MFMA a block's
 // partial sum leaves f32's range only where the product itself does. Scales
-// below 2^-126 take 2^-127, the least there is, and a smaller factor; zero,
-// infinities and NaN are the factor themselves.
+// below 2^-126 take 2^-127, the least there is, and a smaller factor (zero
+// itself: no partial sum becomes infinite in front of it), infinities and NaN
+// 2^127 and themselves.
 struct F8Split {
   int exponent;
   float factor;
 };
 __device__ __forceinline__ F8Split f8_split_scale(float s) {
-  const int e = __builtin_amdgcn_frexp_expf(s);  // |s| in 2^(e - 1) .. 2^e; 0 for zero, infinities and NaN
-  const int up = e < -126 ? -126 : e;
-  return {(up + 126) << 24, __builtin_ldexpf(s, 1 - up)};
+  const uint32_t field = as_uint(s) >> 23 & 0xFFu;
+  const int e = field < 254u ? (int)field : 254;
+  return {e << 24, __builtin_ldexpf(s, 127 - e)};
 }
 
 __device__ __forceinline__ v8i_t join_halves(v4i lo, v4i hi) {

@@ -462,6 +462,24 @@ def test_project_scales_whose_product_leaves_f32(m, k, n, kind):
     product(x, w, 85 * 2.0 ** -24 if kind == "f32" else 2.0 ** -18)
 
 
+@pytest.mark.parametrize("m,k,n", ENDS)
+def test_project_blocks_with_a_scale_of_zero(m, k, n):
+    """Such blocks add nothing, however large the rows; subnormal scales count."""
+    codes = whole((n, k), 15, n).to(F8)
+    x = whole((m, k), 15, m)
+    x[:, ::128] = 15.0
+    far = torch.ldexp(x, torch.tensor(123, device="cuda")).to(BF)
+    scales = torch.full((-(-n // 128), -(-k // 128)), 85 * 2.0 ** -139, device="cuda")  # 2.66 * 2^-134
+    scales[:, ::2] = 0
+    scales[:, 2::4] = -0.0
+    wide = scales.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+    want = far.double() @ (codes.double() * wide).t()
+    got = clef_i4.project_quantized_f8(far, clef_i4.f8_weight(codes, scales))
+    # sums of whole numbers below 2^24 times 85 and a power of two
+    slack = 2.0 ** -23 * (far.double().abs() @ (codes.double() * wide).abs().t())
+    check(got, want, slack)
+
+
 @pytest.mark.parametrize("kind", ["f32", "e8m0"])
 @pytest.mark.parametrize("p", [123, -118])
 @pytest.mark.parametrize("tokens,experts,k,n", [(20, 16, 264, 520), (900, 5, 256, 392), (3000, 4, 264, 3000)])
