@@ -477,9 +477,11 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
     Panel sw[MATS];
     // of step kt (the step before still takes sa)
     auto read_scales = [&](int kt) {
-      const int block = T::KG * kt + kg;  // (a block past the last: its products are zeros)
+      // (a block past the last in a step that counts: its products and its entry
+      // here are zeros, of an odd number of blocks, so below 256)
+      const int block = T::KG * kt + kg;
 #pragma unroll
-      for (int t = 0; t < MATS; ++t) sw[t] = sw_at[t * 256 + (block < kb ? block : 0)];
+      for (int t = 0; t < MATS; ++t) sw[t] = sw_at[t * 256 + (block & 255)];
       const char* at = sa_at + (block >> 4 & 1) * T::SA_BYTES + (block & 15) * T::BM;
       typedef uint32_t pack __attribute__((ext_vector_type(TM / 4)));
       const pack v = *reinterpret_cast<const pack*>(at);

@@ -480,6 +480,19 @@ def test_project_blocks_with_a_scale_of_zero(m, k, n):
     check(got, want, slack)
 
 
+@pytest.mark.parametrize("m,k,n", ENDS)
+def test_project_infinite_scale(m, k, n):
+    """A block of infinite scale makes its sums infinite with their sign,
+    whatever the number of blocks."""
+    codes = torch.ones((n, k), device="cuda")
+    codes[1::2] = -1.0
+    scales = torch.ones((-(-n // 128), -(-k // 128)), device="cuda")
+    scales[:, 0] = float("inf")
+    w = clef_i4.f8_weight(codes.to(F8), scales)
+    got = clef_i4.project_quantized_f8(torch.ones((m, k), dtype=BF, device="cuda"), w)
+    assert torch.equal(got.float(), (codes[:, 0] * float("inf")).expand(m, n))
+
+
 @pytest.mark.parametrize("kind", ["f32", "e8m0"])
 @pytest.mark.parametrize("p", [123, -118])
 @pytest.mark.parametrize("tokens,experts,k,n", [(20, 16, 264, 520), (900, 5, 256, 392), (3000, 4, 264, 3000)])
