@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256) void f8_prepare_kernel(const uint16_t* __restr
                                                          float* __restrict__ scales) {
   constexpr int R = 1 << RLOG, CPW = 16 / R;
   const int group = threadIdx.x >> 4, l = threadIdx.x & 15;
-  const int64_t row = (int64_t)blockIdx.x * R + (group & (R - 1));
+  const int64_t row = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * R + (group & (R - 1));
   const int b0 = blockIdx.y * (CPW * STEPS) + (group >> RLOG);
   const bool row_here = row < rows;
   const uint16_t* xr = x + row * x_stride;
@@ -129,7 +129,10 @@ hipError_t launch_f8_prepare(const uint16_t* x, int64_t rows, int width, int64_t
   const int kb = f8_blocks(width), kp = (int)f8_scale_pitch(width);
   auto run = [&](auto rlog, auto steps) {
     constexpr int R = 1 << decltype(rlog)::value, per = 16 / R * decltype(steps)::value;
-    const dim3 grid((unsigned)((rows + R - 1) / R), (unsigned)((kp + per - 1) / per));
+    // a dispatch counts the work-items of each dimension in 32 bits: parts of
+    // 2^22 workgroups along z
+    const int64_t down = (rows + R - 1) / R, most = (int64_t)1 << 22, parts = (down + most - 1) / most;
+    const dim3 grid((unsigned)(parts > 1 ? most : down), (unsigned)((kp + per - 1) / per), (unsigned)parts);
     f8_prepare_kernel<decltype(rlog)::value, decltype(steps)::value>
         <<<grid, 256, 0, stream>>>(x, rows, width, x_stride, kb, kp, codes, exponents, scales);
   };

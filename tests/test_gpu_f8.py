@@ -163,6 +163,28 @@ def test_prepare_strided_rows_and_reused_buffer():
         assert torch.equal(a.storage[:n], b.storage) and (a.storage[n:] == 0xAB).all()
 
 
+@pytest.mark.parametrize("rows", [(1 << 24) + 5, 1 << 27])
+def test_prepare_more_rows_than_one_dimension_of_a_launch(rows):
+    """2^27 rows, the most there may be: every row as in a call of its own."""
+    some = randn((4096, 8), 1.0, 5)
+    x = some.repeat(-(-rows // 4096), 1)[:rows]
+    x[-3:] = some[7:10] * 3
+    a = clef_i4.prepare_f8(x)
+    del x
+    want = clef_i4.prepare_f8(some)
+    codes, scales = a.codes.view(torch.uint8), a.scales
+    whole_parts = rows // 4096 - 1  # the last rows differ
+    for first in range(0, whole_parts, 2048):
+        count = min(2048, whole_parts - first)
+        at = slice(first * 4096, (first + count) * 4096)
+        assert (codes[at].view(count, 4096, 8) == want.codes.view(torch.uint8)).all()
+        assert (scales[at].view(count, 4096) == want.scales[:, 0]).all()
+    last = clef_i4.prepare_f8(some[7:10] * 3)
+    assert torch.equal(codes[-3:], last.codes.view(torch.uint8)) and torch.equal(scales[-3:], last.scales)
+    exps = a.storage[rows * 128: rows * 144].view(rows, 16)
+    assert torch.equal(exps[-3:], last.storage[3 * 128: 3 * 144].view(3, 16))
+
+
 def test_views_of_a_prepared_activation():
     """On the buffer's memory, which they keep; refused where they do not fit."""
     buffer = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
