@@ -142,8 +142,8 @@ def _check(rc: int) -> None:
 
 
 class _Native:
-    """The call module (csrc/host_call.cpp: launch, value, pointer, empty, matrix) and
-    its handle of every entry point, as attributes; filled on first use."""
+    """The call module (csrc/host_call.cpp: launch, value, pointer, holds, empty,
+    matrix) and its handle of every entry point, as attributes; filled on first use."""
 
     def __getattr__(self, name):
         handle = lib()
@@ -157,7 +157,8 @@ class _Native:
         found = {entry: host.entry(ctypes.cast(getattr(handle, entry), ctypes.c_void_p).value,
                                    "".join("p" if a is _P else "i" for a in args))
                  for entry, (_, args) in SIGNATURES.items()}
-        found.update(launch=host.launch, value=host.value, pointer=host.pointer, empty=host.empty, matrix=host.matrix)
+        found.update(launch=host.launch, value=host.value, pointer=host.pointer, holds=host.holds, empty=host.empty,
+                     matrix=host.matrix)
         if name not in found:
             raise AttributeError(name)
         self.__dict__.update(found)
@@ -923,9 +924,11 @@ class PreparedF8:
                          max(self.rows, 1))
 
     def call_arg(self) -> torch.Tensor:
-        """The buffer, as large as its rows need."""
-        if self.storage.dtype != torch.uint8 or self.storage.numel() < self._scales_at + self.rows * self.pitch // 32:
-            raise ClefError(-1, "FP8 activation buffer too small")
+        """The buffer, as large as its rows need, on the current device."""
+        blocks = (self.width + 127) // 128
+        nbytes = self.rows * (blocks * 132 + (blocks + 15) // 16 * 16)
+        if not _n.holds(torch._C._cuda_getDevice(), self.storage, torch.uint8, nbytes):
+            raise ClefError(-1, "FP8 activation: buffer too small, of another type or not on the current device")
         return self.storage
 
 
@@ -958,6 +961,14 @@ class F8Weight:
     cols: int
     matrices: int = 1
     pow2: bool = False    # every scale is a power of two: the matrix unit may apply them
+
+    def check(self) -> None:
+        """The kernels know rows, cols and matrices alone: codes and scales are
+        as large as those say, on the current device."""
+        blocks = self.matrices * ((self.rows + 127) // 128) * ((self.cols + 127) // 128)
+        if not _n.holds(torch._C._cuda_getDevice(), self.codes, torch.uint8, blocks * 16384,
+                        self.scales, torch.float32, blocks):
+            raise ClefError(-1, "FP8 weight: codes or scales too small, of another type or not on the current device")
 
 
 def _f8_weight_storage(w: torch.Tensor):
@@ -1005,17 +1016,19 @@ def project_f8(a: PreparedF8, w: F8Weight, residual: torch.Tensor | None = None,
     """Block-scaled FP8 projection (clef_f8_gemm): bf16 [rows][w.rows]."""
     if a.width != w.cols or w.matrices != 1:
         raise ClefError(-1, _BAD_F8)
-    _on_current(a.storage, w.codes, residual)
+    w.check()
     _check_residual(residual, a.rows, w.rows)
-    out = _f8_out(a.storage, a.rows, w.rows, out)
-    _n.launch(_n.clef_f8_gemm, a.call_arg(), w.codes, w.scales, a.rows, w.rows, w.cols, int(w.pow2), residual,
-              out)
+    storage = a.call_arg()
+    out = _f8_out(storage, a.rows, w.rows, out)
+    _n.launch(_n.clef_f8_gemm, storage, w.codes, w.scales, a.rows, w.rows, w.cols, int(w.pow2), residual, out)
     return out
 
 
 def _check_residual(residual: torch.Tensor | None, rows: int, cols: int) -> None:
-    if residual is not None and (tuple(residual.shape) != (rows, cols) or residual.dtype != torch.bfloat16):
-        raise ClefError(-1, "residual shape/dtype mismatch")
+    if residual is not None:
+        if tuple(residual.shape) != (rows, cols) or residual.dtype != torch.bfloat16:
+            raise ClefError(-1, "residual shape/dtype mismatch")
+        _on_current(residual)
 
 
 def project_quantized_f8(x: torch.Tensor, w: F8Weight, residual: torch.Tensor | None = None,
@@ -1024,7 +1037,8 @@ def project_quantized_f8(x: torch.Tensor, w: F8Weight, residual: torch.Tensor | 
     address, m, k, pitch = _f8_rows(x)
     if k != w.cols or w.matrices != 1:
         raise ClefError(-1, _BAD_F8)
-    _on_current(x, w.codes, residual)
+    w.check()
+    _on_current(x)
     _check_residual(residual, m, w.rows)
     out = _f8_out(x, m, w.rows, out)
     nbytes = _n.value(_n.clef_f8_project_workspace_bytes, m, w.rows, k)
@@ -1039,9 +1053,11 @@ def project_gate_up_f8(a: PreparedF8, gate: F8Weight, up: F8Weight, out: torch.T
     (clef_f8_gemm_gate_up): bf16 [rows][gate.rows], rounded once."""
     if a.width != gate.cols or (gate.rows, gate.cols, gate.matrices) != (up.rows, up.cols, 1) or gate.matrices != 1:
         raise ClefError(-1, _BAD_F8)
-    _on_current(a.storage, gate.codes, up.codes)
-    out = _f8_out(a.storage, a.rows, gate.rows, out)
-    _n.launch(_n.clef_f8_gemm_gate_up, a.call_arg(), gate.codes, gate.scales, up.codes, up.scales, a.rows, gate.rows,
+    gate.check()
+    up.check()
+    storage = a.call_arg()
+    out = _f8_out(storage, a.rows, gate.rows, out)
+    _n.launch(_n.clef_f8_gemm_gate_up, storage, gate.codes, gate.scales, up.codes, up.scales, a.rows, gate.rows,
               gate.cols, int(gate.pow2 and up.pow2), out)
     return out
 
@@ -1071,7 +1087,8 @@ def _check_lists(a: PreparedF8, w: F8Weight, offsets: torch.Tensor, slots: torch
     if offsets.dtype != torch.int32 or offsets.numel() != w.matrices + 1 or (slots is not None
                                                                              and slots.dtype != torch.int32):
         raise ClefError(-1, "invalid grouped expert lists")
-    _on_current(a.storage, w.codes, offsets, slots)
+    w.check()
+    _on_current(offsets, slots)
     if slots is not None:
         return slots.numel()
     return a.rows if input_routed else a.rows * topk
@@ -1085,8 +1102,9 @@ def expert_f8(a: PreparedF8, w: F8Weight, offsets: torch.Tensor, slots: torch.Te
     places themselves (rows sorted by expert). Rows that no list names are left
     as they were in `out`, undefined in a new output."""
     total = _check_lists(a, w, offsets, slots, topk, input_routed)
-    out = _f8_out(a.storage, total, w.rows, out)
-    _n.launch(_n.clef_moe_expert_f8, a.call_arg(), a.rows, w.codes, w.scales, offsets, slots, w.matrices, total, topk,
+    storage = a.call_arg()
+    out = _f8_out(storage, total, w.rows, out)
+    _n.launch(_n.clef_moe_expert_f8, storage, a.rows, w.codes, w.scales, offsets, slots, w.matrices, total, topk,
               int(input_routed), w.cols, w.rows, int(w.pow2), out)
     return out
 
@@ -1099,9 +1117,10 @@ def expert_gate_up_f8(a: PreparedF8, gate: F8Weight, up: F8Weight, offsets: torc
     if (gate.rows, gate.cols, gate.matrices) != (up.rows, up.cols, up.matrices):
         raise ClefError(-1, _BAD_F8)
     total = _check_lists(a, gate, offsets, slots, topk, input_routed)
-    _on_current(up.codes)
-    out = _f8_out(a.storage, total, gate.rows, out)
-    _n.launch(_n.clef_moe_expert_gate_up_f8, a.call_arg(), a.rows, gate.codes, gate.scales, up.codes, up.scales,
+    up.check()
+    storage = a.call_arg()
+    out = _f8_out(storage, total, gate.rows, out)
+    _n.launch(_n.clef_moe_expert_gate_up_f8, storage, a.rows, gate.codes, gate.scales, up.codes, up.scales,
               offsets, slots, gate.matrices, total, topk, int(input_routed), gate.cols, gate.rows,
               int(gate.pow2 and up.pow2), out)
     return out

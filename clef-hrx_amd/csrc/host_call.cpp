@@ -12,6 +12,8 @@
 //     the function given to set_check, which raises.
 //   value(entry, *args): entry(args..) as int64 (size functions).
 //   pointer(tensor): its device pointer, checked as an argument is.
+//   holds(device, tensor, dtype, count, ..): whether each is a contiguous tensor of
+//     that dtype and at least count elements on that device (-1: the host).
 //   empty(like, dtype, *sizes): torch.empty on like's device.
 //   matrix(buffer, dtype, byte, rows, cols, row_step, col_step): a 2-d tensor of
 //     dtype on buffer's memory from its byte `byte`, steps in elements; bounds
@@ -182,6 +184,28 @@ PyObject* pointer(PyObject*, PyObject* o) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* holds(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  bool all = n >= 1 && n % 3 == 1;
+  for (Py_ssize_t i = 1; all && i < n; i += 3) all = THPVariable_Check(args[i]) && THPDtype_Check(args[i + 1]);
+  if (!all) {
+    PyErr_SetString(PyExc_TypeError, "holds(device, tensor, dtype, count, ..) expected");
+    return nullptr;
+  }
+  const int64_t device = PyLong_AsLongLong(args[0]);
+  if (device == -1 && PyErr_Occurred()) return nullptr;
+  for (Py_ssize_t i = 1; i < n; i += 3) {
+    const int64_t count = PyLong_AsLongLong(args[i + 2]);
+    if (count == -1 && PyErr_Occurred()) return nullptr;
+    const at::Tensor& t = THPVariable_Unpack(args[i]);
+    const int64_t on = t.is_cuda() ? t.get_device() : t.is_cpu() ? -1 : -2;
+    all = all && t.scalar_type() == reinterpret_cast<THPDtype*>(args[i + 1])->scalar_type && t.numel() >= count &&
+          on == device && t.is_contiguous();
+  }
+  return PyBool_FromLong(all);
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* empty(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n < 3 || n > 6 || !THPVariable_Check(args[0]) || !THPDtype_Check(args[1])) {
@@ -251,6 +275,7 @@ PyMethodDef methods[] = {
     {"launch", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&launch)), METH_FASTCALL, nullptr},
     {"value", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&value)), METH_FASTCALL, nullptr},
     {"pointer", &pointer, METH_O, nullptr},
+    {"holds", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&holds)), METH_FASTCALL, nullptr},
     {"empty", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&empty)), METH_FASTCALL, nullptr},
     {"matrix", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&matrix)), METH_FASTCALL, nullptr},
     {"set_check", &set_check, METH_O, nullptr},

@@ -1,6 +1,9 @@
 """Block-scaled FP8 entry points without a GPU: sizes, refusals."""
+import types
+
 import numpy as np
 import pytest
+import torch
 
 import clef_i4
 
@@ -136,3 +139,55 @@ def test_operand_order_is_a_permutation():
     at = (r // 16) * 2048 + (k // 64) * 1024 + ((k // 16) % 4 * 16 + r % 16) * 16 + k % 16
     assert np.array_equal(np.sort(at.ravel()), np.arange(16384))
     assert (np.diff(at.reshape(128, 8, 16), axis=2) == 1).all()
+
+
+def weight(matrices=1, rows=136, cols=264, codes=None, scales=None, dtype=torch.float32):
+    blocks = matrices * -(-rows // 128) * -(-cols // 128)
+    return clef_i4.F8Weight(torch.zeros(blocks * 16384 if codes is None else codes, dtype=torch.uint8),
+                            torch.zeros(blocks if scales is None else scales, dtype=dtype), rows, cols, matrices)
+
+
+@pytest.mark.parametrize("bad", [dict(codes=6 * 16384 - 1), dict(scales=5), dict(codes=0), dict(scales=0),
+                                 dict(dtype=torch.bfloat16)])
+def test_weights_smaller_than_they_say_do_not_reach_the_library(monkeypatch, bad):
+    """Every call that takes a weight, on host tensors with the library's entry
+    points replaced by one that records."""
+    reached = []
+    holds = clef_i4._n.holds
+    fake = types.SimpleNamespace(holds=holds, value=lambda *a: 0, launch=lambda *a: reached.append(a),
+                                 empty=lambda like, dtype, *size: torch.empty(size, dtype=dtype))
+    for name in clef_i4.SIGNATURES:
+        setattr(fake, name, name)
+    monkeypatch.setattr(clef_i4, "_n", fake)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1)
+    good, wrong = weight(), weight(**bad)
+    goods = weight(2)
+    bad = {k: 2 * v if isinstance(v, int) else v for k, v in bad.items()}
+    wrongs = weight(2, **bad)
+    x = torch.zeros((4, 264), dtype=torch.bfloat16)
+    a = clef_i4.PreparedF8(torch.zeros(clef_i4.lib().clef_f8_prepared_bytes(4, 264), dtype=torch.uint8), 4, 264)
+    offsets = torch.zeros(3, dtype=torch.int32)
+    clef_i4.project_f8(a, good), clef_i4.project_quantized_f8(x, good), clef_i4.project_gate_up_f8(a, good, good)
+    clef_i4.expert_f8(a, goods, offsets, None, 1, True), clef_i4.expert_gate_up_f8(a, goods, goods, offsets, None, 1, True)
+    assert len(reached) == 5
+    for f in (lambda: clef_i4.project_f8(a, wrong), lambda: clef_i4.project_quantized_f8(x, wrong),
+              lambda: clef_i4.project_gate_up_f8(a, wrong, good), lambda: clef_i4.project_gate_up_f8(a, good, wrong),
+              lambda: clef_i4.expert_f8(a, wrongs, offsets, None, 1, True),
+              lambda: clef_i4.expert_gate_up_f8(a, wrongs, goods, offsets, None, 1, True),
+              lambda: clef_i4.expert_gate_up_f8(a, goods, wrongs, offsets, None, 1, True)):
+        with pytest.raises(clef_i4.ClefError):
+            f()
+    assert len(reached) == 5
+
+
+def test_holds():
+    t, u = torch.zeros((4, 6), dtype=torch.int32), torch.zeros(3)
+    holds = clef_i4._n.holds
+    assert holds(-1) and holds(-1, t, torch.int32, 24) and holds(-1, t, torch.int32, -1, u, torch.float32, 3)
+    assert not holds(-1, t, torch.int32, 25) and not holds(-1, t, torch.float32, 24) and not holds(0, t, torch.int32, 24)
+    assert not holds(-1, t.t(), torch.int32, 24) and not holds(-1, t.to("meta"), torch.int32, 24)
+    assert not holds(-1, t, torch.int32, 25, u, torch.float32, 3) and not holds(-1, t, torch.int32, 24, u, torch.float32, 4)
+    for wrong in ((), (-1, t), (-1, t, torch.int32), (-1, None, torch.int32, 0), (-1, t, 4, 24), (-1, t, torch.int32, "24"),
+                  (None, t, torch.int32, 24)):
+        with pytest.raises(TypeError):
+            holds(*wrong)

@@ -832,3 +832,28 @@ def test_binding_refusals():
         with pytest.raises(clef_i4.ClefError):
             f()
             pytest.fail(f"refusal {i} did not raise")
+
+
+def test_weights_smaller_than_they_say_are_refused():
+    x = randn((4, 256), 1.0, 1)
+    a = clef_i4.prepare_f8(x)
+    two = clef_i4.load_f8_weight(randn((2, 136, 256), 0.1, 2))
+    w = one(clef_i4.F8Weight(two.codes[: 4 * 16384], two.scales, 136, 256))
+    clef_i4.project_f8(a, w)
+    offsets = torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")
+    F8Weight = clef_i4.F8Weight
+    for codes, scales in ((w.codes[:-16], w.scales), (w.codes, w.scales[:1]), (w.codes.cpu(), w.scales),
+                          (w.codes, w.scales.cpu()), (w.codes.view(torch.int32), w.scales), (w.codes, w.scales.bfloat16())):
+        bad = F8Weight(codes, scales, 136, 256)
+        for f in (lambda: clef_i4.project_f8(a, bad), lambda: clef_i4.project_quantized_f8(x, bad),
+                  lambda: clef_i4.project_gate_up_f8(a, bad, w), lambda: clef_i4.project_gate_up_f8(a, w, bad)):
+            with pytest.raises(clef_i4.ClefError):
+                f()
+    for bad in (F8Weight(two.codes, two.scales, 136, 264, 2), F8Weight(two.codes, two.scales, 264, 256, 2)):
+        with pytest.raises(clef_i4.ClefError):
+            clef_i4.expert_f8(clef_i4.prepare_f8(randn((4, bad.cols), 1.0, 1)), bad, offsets, None, 1, True)
+    three = F8Weight(two.codes, two.scales, 136, 256, 3)
+    for f in (lambda: clef_i4.expert_f8(a, three, torch.zeros(4, dtype=torch.int32, device="cuda"), None, 1, True),
+              lambda: clef_i4.expert_gate_up_f8(a, two, F8Weight(two.codes, two.scales[:1], 136, 256, 2), offsets, None, 1, True)):
+        with pytest.raises(clef_i4.ClefError):
+            f()
