@@ -7,6 +7,10 @@ namespace clef {
 
 namespace {
 
+// A dispatch counts the work-items of each dimension in 32 bits: workgroups of
+// rows beyond this many go along z.
+constexpr int64_t kPartWorkgroups = (int64_t)1 << 22;
+
 // x bf16 [rows][width] (row pitch x_stride) -> codes [rows][pitch], scales as
 // e8m0 [rows][kp] and f32 [kb][rows]. 16 lanes hold a block of 128 columns, 8
 // values each: one 16-byte load, the maximum over the 16 lanes by DPP, one 8-byte
@@ -22,7 +26,7 @@ __global__ __launch_bounds__(256) void f8_prepare_kernel(const uint16_t* __restr
                                                          float* __restrict__ scales) {
   constexpr int R = 1 << RLOG, CPW = 16 / R;
   const int group = threadIdx.x >> 4, l = threadIdx.x & 15;
-  const int64_t row = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * R + (group & (R - 1));
+  const int64_t row = ((int64_t)blockIdx.z * kPartWorkgroups + blockIdx.x) * R + (group & (R - 1));
   const int b0 = blockIdx.y * (CPW * STEPS) + (group >> RLOG);
   const bool row_here = row < rows;
   const uint16_t* xr = x + row * x_stride;
@@ -129,10 +133,8 @@ hipError_t launch_f8_prepare(const uint16_t* x, int64_t rows, int width, int64_t
   const int kb = f8_blocks(width), kp = (int)f8_scale_pitch(width);
   auto run = [&](auto rlog, auto steps) {
     constexpr int R = 1 << decltype(rlog)::value, per = 16 / R * decltype(steps)::value;
-    // a dispatch counts the work-items of each dimension in 32 bits: parts of
-    // 2^22 workgroups along z
-    const int64_t down = (rows + R - 1) / R, most = (int64_t)1 << 22, parts = (down + most - 1) / most;
-    const dim3 grid((unsigned)(parts > 1 ? most : down), (unsigned)((kp + per - 1) / per), (unsigned)parts);
+    const int64_t down = (rows + R - 1) / R, parts = (down + kPartWorkgroups - 1) / kPartWorkgroups;
+    const dim3 grid((unsigned)(parts > 1 ? kPartWorkgroups : down), (unsigned)((kp + per - 1) / per), (unsigned)parts);
     f8_prepare_kernel<decltype(rlog)::value, decltype(steps)::value>
         <<<grid, 256, 0, stream>>>(x, rows, width, x_stride, kb, kp, codes, exponents, scales);
   };
