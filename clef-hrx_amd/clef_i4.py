@@ -719,10 +719,18 @@ def router_logits(x: torch.Tensor, gate_w: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _logits_dtype(logits: torch.Tensor) -> int:
+    if logits.dtype == torch.bfloat16:
+        return 0
+    if logits.dtype != torch.float32:
+        raise ClefError(-1, "invalid router logits dtype")
+    return 1
+
+
 def omni_route(logits: torch.Tensor, topk: int = 8) -> torch.Tensor:
     """Engine::omni_route (src/omni.rs:170-190)."""
     tokens, experts = logits.shape
-    dtype = 0 if logits.dtype == torch.bfloat16 else 1
+    dtype = _logits_dtype(logits)
     routes = _n.empty(logits, torch.float32, tokens, 2 * topk)
     _n.launch(_n.clef_moe_route, logits, dtype, tokens, experts, topk, routes)
     return routes
@@ -846,10 +854,10 @@ class MoeLayer:
             if self.router is None:
                 raise ClefError(-1, "MoE layer needs router logits or a router gate weight")
             logits = router_logits(x, self.router)  # e.project(norm, "mlp.gate"), src/omni.rs:764
+        dtype = _logits_dtype(logits)
         if out is None:
             out = _n.empty(x, torch.bfloat16, tokens, self.hidden)
         ws = self._scratch(x)
-        dtype = 0 if logits.dtype == torch.bfloat16 else 1
         _n.launch(_n.clef_moe_layer, x, logits, dtype, tokens, self.hidden, self.inter, 128, self.topk,
                   self.gate.codes, self.gate.scales, self.up.codes, self.up.scales, self.down.codes, self.down.scales,
                   routes_out, out, ws, ws.numel())

@@ -191,3 +191,19 @@ def test_holds():
                   (None, t, torch.int32, 24)):
         with pytest.raises(TypeError):
             holds(*wrong)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64, torch.int32, torch.int8])
+def test_router_logits_of_other_types_are_refused(dtype):
+    """The library knows bf16 and f32: logits of a narrower type would be read
+    past their end, wider ones as other values."""
+    logits = torch.zeros((4, 128), dtype=dtype)
+    with pytest.raises(clef_i4.ClefError, match="router logits dtype"):
+        clef_i4.omni_route(logits)
+    x = torch.zeros((4, 264), dtype=torch.bfloat16)
+    gate, down = weight(128, 136, 264), weight(128, 264, 136)
+    with pytest.raises(clef_i4.ClefError, match="router logits dtype"):
+        clef_i4.MoeLayerF8(gate, gate, down)(x, logits)
+    q = clef_i4.QuantizedWeight(torch.zeros(1), torch.zeros(1), 128 * 256, 512, 512, 4)
+    with pytest.raises(clef_i4.ClefError, match="router logits dtype"):
+        clef_i4.MoeLayer(q, q, q)(x, logits)
