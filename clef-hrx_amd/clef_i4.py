@@ -86,6 +86,7 @@ SIGNATURES = {
     "clef_f8_prepare": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _P]),
     "clef_f8_pack_weight": (ctypes.c_int, [_P, _I64, _I32, _I32, _P, _P, _P]),
     "clef_f8_retile": (ctypes.c_int, [_P, _I64, _I32, _I32, _P, _P]),
+    "clef_f8_kernel_name": (ctypes.c_char_p, [_I64, _I32, _I32, _I32, _I32, _I32]),
     "clef_f8_gemm": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _I32, _I32, _P, _P, _P]),
     "clef_f8_gemm_gate_up": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P]),
     "clef_f8_project_workspace_bytes": (_SZ, [_I64, _I32, _I32]),

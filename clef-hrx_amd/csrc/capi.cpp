@@ -908,6 +908,16 @@ int clef_f8_retile(const uint8_t* w, int64_t matrices, int32_t n, int32_t k, uin
   return hip_status(clef::launch_f8_retile(w, matrices, n, k, codes, hs(stream)));
 }
 
+const char* clef_f8_kernel_name(int64_t rows, int32_t n, int32_t k, int32_t gate_up, int32_t pow2, int32_t experts) {
+  static const char* const names[] = {"16x32", "32x32", "16x64", "32x64", "64x64", "128x128", "128x128x2", "256x256"};
+  if (rows < 1 || rows > 16777216 || !f8_columns(n) || !f8_width(k) || experts < 0 || experts > kF8MostExperts ||
+      (experts == 0 && rows > kF8MostRows))
+    return "";
+  const clef::F8Kernel kernel = experts > 0 ? clef::f8_kernel_lists(rows, experts, n, gate_up != 0)
+                                            : clef::f8_kernel(rows, n, clef::f8_blocks(k), gate_up != 0, pow2 != 0);
+  return names[(int)kernel];
+}
+
 int clef_f8_gemm(const uint8_t* a, const uint8_t* w, const float* w_scales, int64_t m,
                  int32_t n, int32_t k, int32_t pow2, const uint16_t* residual, uint16_t* out, clef_stream_t stream) {
   if (int rc = check_f8_gemm(m, n, k)) return rc;

@@ -73,6 +73,14 @@ struct F8Args {
   int k;
 };
 
+// The kernels of the products: tiles of rows x weight rows, the first five of the
+// split-k kernel, the others of the tiled one (k128x128k: two blocks of k at a time).
+enum class F8Kernel { k16x32, k32x32, k16x64, k32x64, k64x64, k128x128, k128x128k, k256x256 };
+// The rule that picks one: a projection of m rows, products over lists of total
+// slots (total, experts >= 1).
+F8Kernel f8_kernel(int64_t m, int n, int kb, bool gate_up, bool pow2);
+F8Kernel f8_kernel_lists(int64_t total, int64_t experts, int n, bool gate_up);
+
 hipError_t launch_f8_prepare(const uint16_t* x, int64_t rows, int width, int64_t x_stride, uint8_t* codes,
                              uint8_t* exponents, float* scales, hipStream_t stream);
 hipError_t launch_f8_pack(const uint16_t* w, int64_t matrices, int n, int k, uint8_t* codes, float* scales,

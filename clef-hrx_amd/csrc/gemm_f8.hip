@@ -750,18 +750,20 @@ hipError_t launch_tile(const F8Args& x, hipStream_t stream) {
 
 constexpr int64_t kCus = 256;
 
-// Tiles of the split-k kernel for m rows against n weight rows (gate/up: both).
-enum class StreamShape { kNone, k16x32, k32x32, k16x64, k32x64, k64x64 };
-StreamShape stream_shape(int64_t m, int64_t n) {
+// Tiles of the split-k kernel for m rows against n weight rows (gate/up: both);
+// k256x256 where they are more than the CUs whatever the shape.
+F8Kernel stream_kernel(int64_t m, int64_t n) {
   auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); };
-  if (tiles(16, 32) <= kCus || (m <= 16 && tiles(16, 64) > kCus)) return StreamShape::k16x32;
-  if (m <= 32 && tiles(32, 32) <= kCus) return StreamShape::k32x32;
-  if (tiles(16, 64) <= kCus) return StreamShape::k16x64;
-  if (tiles(32, 64) <= kCus) return StreamShape::k32x64;
-  return tiles(64, 64) <= kCus ? StreamShape::k64x64 : StreamShape::kNone;
+  if (tiles(16, 32) <= kCus || (m <= 16 && tiles(16, 64) > kCus)) return F8Kernel::k16x32;
+  if (m <= 32 && tiles(32, 32) <= kCus) return F8Kernel::k32x32;
+  if (tiles(16, 64) <= kCus) return F8Kernel::k16x64;
+  if (tiles(32, 64) <= kCus) return F8Kernel::k32x64;
+  return tiles(64, 64) <= kCus ? F8Kernel::k64x64 : F8Kernel::k256x256;
 }
 
-// The kernel of a shape. From the smallest tiles up: 16 x 32, 16 x 64, 32 x 64
+}  // namespace
+
+// From the smallest tiles up: 16 x 32, 16 x 64, 32 x 64
 // and 64 x 64 of the split-k kernel while they are at most one per CU (m x k x n
 // in us: 133 x 5784 x 288 6.3 on 16 x 32 tiles, 7.9, 10.7, 16.3 on the larger
 // ones; 170 x 3600 x 3808 24.8, 14.1, 15.2 and 12.5), and 32 x 32 where one tile
@@ -773,61 +775,13 @@ StreamShape stream_shape(int64_t m, int64_t n) {
 // against 52; 1536, 2 and 5: 95 against 81; 4096, 3 and 12: 174 against 218).
 // One tile of 16 rows against more columns than 256 tiles cover stays on 16 x
 // 32 (16 x 5120 x 2 17408: 39 against 44 on 128 x 128).
-template <bool LISTS, bool GU, bool RESID>
-hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
-  const int64_t rows_of_w = (int64_t)x.n * (GU ? 2 : 1);
-  // tiles of bm rows; experts' lists as if evenly filled (a little more, for
-  // those above the mean)
-  auto tiles = [&](int bm, int bn) {
-    int64_t down;
-    if constexpr (LISTS) {
-      const int64_t named = x.lists.total < x.lists.experts ? x.lists.total : x.lists.experts;
-      const int64_t rows = x.lists.total * 21 / 20 / named;
-      down = named * ((rows + bm - 1) / bm > 0 ? (rows + bm - 1) / bm : 1);
-    } else {
-      down = (x.rows + bm - 1) / bm;
-    }
-    return down * ((rows_of_w + bn - 1) / bn);
-  };
-  if constexpr (LISTS) {
-    // Experts with few rows, whose weights are read once whatever the tile. As
-    // many tiles as CUs: 16 x 32, then 16 x 64 (8 slots of 128 experts, gate/up 2048
-    // x 2 768: 4.6 us on 16 x 64, 4.7 on 16 x 32 and 9.8 on 128 x 128; 57 of 8, 2928 x
-    // 464: 4.8 on 16 x 32, 5.6, 12.9). More: 16 x 64 below sixteen rows per expert
-    // (gate/up, 540 slots of 128 568 x 2 1440 40.6 against 51.7 on 128 x 128, 793 of
-    // 60 3112 x 2 712 51.7 against 53.5; 1063 of 64 584 x 2 256, 16.6 rows each, 8.9
-    // against 7.9). The experts named: about total E / (total + E).
-    const int64_t total = x.lists.total, experts = x.lists.experts;
-    const int64_t named = total * experts / (total + experts) > 1 ? total * experts / (total + experts) : 1;
-    const int64_t down = named * ((total * 21 / 20 / (total < experts ? total : experts) + 15) / 16);
-    const int64_t narrow = down * ((rows_of_w + 31) / 32), wide = down * ((rows_of_w + 63) / 64);
-    if (f8_most_tiles(total, (int)experts, 16) <= 65535) {
-      if (narrow <= kCus) return launch_stream<1, 2, false, LISTS, GU, RESID>(x, stream);
-      if (wide <= kCus || total < 16 * experts) return launch_stream<1, 4, false, LISTS, GU, RESID>(x, stream);
-    }
-  } else {
-    const StreamShape shape = stream_shape(x.rows, rows_of_w);
-    if constexpr (!GU)
-      if (x.x != nullptr) switch (shape) {  // f8_project_fusable
-          case StreamShape::k16x32: return launch_stream<1, 2, true, false, false, RESID>(x, stream);
-          case StreamShape::k32x32: return launch_stream<2, 2, true, false, false, RESID>(x, stream);
-          case StreamShape::k16x64: return launch_stream<1, 4, true, false, false, RESID>(x, stream);
-          case StreamShape::k32x64: return launch_stream<2, 4, true, false, false, RESID>(x, stream);
-          default: return hipErrorInvalidValue;
-        }
-    switch (shape) {
-      case StreamShape::k16x32: return launch_stream<1, 2, false, LISTS, GU, RESID>(x, stream);
-      case StreamShape::k32x32: return launch_stream<2, 2, false, LISTS, GU, RESID>(x, stream);
-      case StreamShape::k16x64: return launch_stream<1, 4, false, LISTS, GU, RESID>(x, stream);
-      case StreamShape::k32x64: return launch_stream<2, 4, false, LISTS, GU, RESID>(x, stream);
-      case StreamShape::k64x64: return launch_stream<4, 4, false, LISTS, GU, RESID>(x, stream);
-      default: break;
-    }
-  }
-  const int64_t small = (tiles(128, 128) + kCus - 1) / kCus, large = (tiles(256, 256) + kCus - 1) / kCus;
-  if (small >= 3 * large)
-    return x.pow2 ? launch_tile<F8Tile256, F8Tile256H, true, LISTS, GU, RESID>(x, stream)
-                  : launch_tile<F8Tile256, F8Tile256H, false, LISTS, GU, RESID>(x, stream);
+F8Kernel f8_kernel(int64_t m, int n, int kb, bool gate_up, bool pow2) {
+  const int64_t rows_of_w = (int64_t)n * (gate_up ? 2 : 1);
+  const F8Kernel few = stream_kernel(m, rows_of_w);
+  if (few != F8Kernel::k256x256) return few;
+  auto rounds = [&](int bm, int bn) { return ((m + bm - 1) / bm * ((rows_of_w + bn - 1) / bn) + kCus - 1) / kCus; };
+  const int64_t small = rounds(128, 128);
+  if (small >= 3 * rounds(256, 256)) return F8Kernel::k256x256;
   // One tile per CU: two blocks of k at a time on two groups of waves, which read
   // less LDS per MFMA and have more loads on their way, against a longer start and
   // the groups' sums (f32 scales, us for 128 x 128 tiles and these: 620 x 17408 x
@@ -835,12 +789,64 @@ hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
   // k, 5.9 and 6.8; powers of two: 620 x 17408 x 5120 76.7 and 72.2, 300 x 8192 x
   // 8192 36.8 and 35.0, 300 x 5120 x 2 5120 22.0 and 21.5, 256 x 4096 x 12288 16.8
   // and 16.7, 640 x 2048 x 2048 9.4 and 10.3).
-  if constexpr (!LISTS)
-    if (small <= 1 && x.kb >= (x.pow2 ? 40 : 16))
-      return x.pow2 ? launch_tile<F8Tile128K, F8Tile128K, true, LISTS, GU, RESID>(x, stream)
-                    : launch_tile<F8Tile128K, F8Tile128K, false, LISTS, GU, RESID>(x, stream);
-  return x.pow2 ? launch_tile<F8Tile128, F8Tile128, true, LISTS, GU, RESID>(x, stream)
-                : launch_tile<F8Tile128, F8Tile128, false, LISTS, GU, RESID>(x, stream);
+  return small <= 1 && kb >= (pow2 ? 40 : 16) ? F8Kernel::k128x128k : F8Kernel::k128x128;
+}
+
+// Experts with few rows, whose weights are read once whatever the tile. As
+// many tiles as CUs: 16 x 32, then 16 x 64 (8 slots of 128 experts, gate/up 2048
+// x 2 768: 4.6 us on 16 x 64, 4.7 on 16 x 32 and 9.8 on 128 x 128; 57 of 8, 2928 x
+// 464: 4.8 on 16 x 32, 5.6, 12.9). More: 16 x 64 below sixteen rows per expert
+// (gate/up, 540 slots of 128 568 x 2 1440 40.6 against 51.7 on 128 x 128, 793 of
+// 60 3112 x 2 712 51.7 against 53.5; 1063 of 64 584 x 2 256, 16.6 rows each, 8.9
+// against 7.9). The experts named: about total E / (total + E). Then as without
+// lists, as if evenly filled (a little more, for those above the mean).
+F8Kernel f8_kernel_lists(int64_t total, int64_t experts, int n, bool gate_up) {
+  const int64_t rows_of_w = (int64_t)n * (gate_up ? 2 : 1), least = total < experts ? total : experts;
+  const int64_t rows = total * 21 / 20 / least;
+  const int64_t named = total * experts / (total + experts) > 1 ? total * experts / (total + experts) : 1;
+  const int64_t down = named * ((rows + 15) / 16);
+  if (f8_most_tiles(total, (int)experts, 16) <= 65535) {
+    if (down * ((rows_of_w + 31) / 32) <= kCus) return F8Kernel::k16x32;
+    if (down * ((rows_of_w + 63) / 64) <= kCus || total < 16 * experts) return F8Kernel::k16x64;
+  }
+  auto rounds = [&](int b) { return (least * ((rows + b - 1) / b) * ((rows_of_w + b - 1) / b) + kCus - 1) / kCus; };
+  return rounds(128) >= 3 * rounds(256) ? F8Kernel::k256x256 : F8Kernel::k128x128;
+}
+
+namespace {
+
+template <bool LISTS, bool GU, bool RESID>
+hipError_t launch_rows(const F8Args& x, hipStream_t stream) {
+  const F8Kernel kernel = LISTS ? f8_kernel_lists(x.lists.total, x.lists.experts, x.n, GU)
+                                : f8_kernel(x.rows, x.n, x.kb, GU, x.pow2);
+  if constexpr (!LISTS && !GU)
+    if (x.x != nullptr) switch (kernel) {  // f8_project_fusable
+        case F8Kernel::k16x32: return launch_stream<1, 2, true, false, false, RESID>(x, stream);
+        case F8Kernel::k32x32: return launch_stream<2, 2, true, false, false, RESID>(x, stream);
+        case F8Kernel::k16x64: return launch_stream<1, 4, true, false, false, RESID>(x, stream);
+        case F8Kernel::k32x64: return launch_stream<2, 4, true, false, false, RESID>(x, stream);
+        default: return hipErrorInvalidValue;
+      }
+  if constexpr (!LISTS) switch (kernel) {
+      case F8Kernel::k32x32: return launch_stream<2, 2, false, false, GU, RESID>(x, stream);
+      case F8Kernel::k32x64: return launch_stream<2, 4, false, false, GU, RESID>(x, stream);
+      case F8Kernel::k64x64: return launch_stream<4, 4, false, false, GU, RESID>(x, stream);
+      case F8Kernel::k128x128k:
+        return x.pow2 ? launch_tile<F8Tile128K, F8Tile128K, true, false, GU, RESID>(x, stream)
+                      : launch_tile<F8Tile128K, F8Tile128K, false, false, GU, RESID>(x, stream);
+      default: break;
+    }
+  switch (kernel) {
+    case F8Kernel::k16x32: return launch_stream<1, 2, false, LISTS, GU, RESID>(x, stream);
+    case F8Kernel::k16x64: return launch_stream<1, 4, false, LISTS, GU, RESID>(x, stream);
+    case F8Kernel::k128x128:
+      return x.pow2 ? launch_tile<F8Tile128, F8Tile128, true, LISTS, GU, RESID>(x, stream)
+                    : launch_tile<F8Tile128, F8Tile128, false, LISTS, GU, RESID>(x, stream);
+    case F8Kernel::k256x256:
+      return x.pow2 ? launch_tile<F8Tile256, F8Tile256H, true, LISTS, GU, RESID>(x, stream)
+                    : launch_tile<F8Tile256, F8Tile256H, false, LISTS, GU, RESID>(x, stream);
+    default: return hipErrorInvalidValue;
+  }
 }
 
 }  // namespace
@@ -851,10 +857,10 @@ hipError_t launch_f8_gemm(const F8Args& x, bool gate_up, hipStream_t stream) {
 }
 
 bool f8_project_fusable(int64_t m, int n, int k) {
-  const StreamShape shape = stream_shape(m, n);
-  const int rows = shape == StreamShape::k16x32 || shape == StreamShape::k16x64   ? 16
-                   : shape == StreamShape::k32x32 || shape == StreamShape::k32x64 ? 32
-                                                                                  : 0;
+  const F8Kernel kernel = stream_kernel(m, n);
+  const int rows = kernel == F8Kernel::k16x32 || kernel == F8Kernel::k16x64   ? 16
+                   : kernel == F8Kernel::k32x32 || kernel == F8Kernel::k32x64 ? 32
+                                                                              : 0;
   return rows > 0 && (m < rows ? m : rows) * f8_pitch(k) <= kQxValues;
 }
 

@@ -528,6 +528,13 @@ int clef_f8_pack_weight(const uint16_t* w, int64_t matrices, int32_t n, int32_t 
  * (their scales are used as they are). 1 <= matrices <= 1024. */
 int clef_f8_retile(const uint8_t* w, int64_t matrices, int32_t n, int32_t k, uint8_t* codes, clef_stream_t stream);
 
+/* The tile (rows x columns of the product's weights) that the library's rule picks for a
+ * product, for tests and profiles: "16x32", "32x32", "16x64", "32x64", "64x64",
+ * "128x128", "128x128x2" (two blocks of k at a time), "256x256". experts 0: a
+ * projection of `rows` rows; else lists of `rows` slots. "" for a shape the
+ * products reject. */
+const char* clef_f8_kernel_name(int64_t rows, int32_t n, int32_t k, int32_t gate_up, int32_t pow2, int32_t experts);
+
 /* Projection of a prepared activation; residual bf16 [m][n], nullable. pow2
  * (here and below) nonzero: every scale of w is a power of two between 2^-126
  * and 2^127, as clef_f8_pack_weight and e8m0 checkpoints make them; the matrix

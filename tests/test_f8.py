@@ -207,3 +207,54 @@ def test_router_logits_of_other_types_are_refused(dtype):
     q = clef_i4.QuantizedWeight(torch.zeros(1), torch.zeros(1), 128 * 256, 512, 512, 4)
     with pytest.raises(clef_i4.ClefError, match="router logits dtype"):
         clef_i4.MoeLayer(q, q, q)(x, logits)
+
+
+SPLIT_K = ("16x32", "32x32", "16x64", "32x64", "64x64")
+TILED = ("128x128", "128x128x2", "256x256")
+
+
+def kernel(rows, n, k, gate_up=0, pow2=0, experts=0):
+    return clef_i4.lib().clef_f8_kernel_name(rows, n, k, gate_up, pow2, experts).decode()
+
+
+def test_kernel_name():
+    assert kernel(1, 128, 128) == "16x32" and kernel(4096, 12288, 4096) == "256x256"
+    assert kernel(620, 5120, 17408) == "128x128x2" and kernel(620, 5120, 4096, pow2=1) == "128x128"
+    for bad in ((0, 128, 128), ((1 << 20) + 1, 128, 128), (4, 100, 128), (4, 128, 12), (4, 128, 32776)):
+        assert kernel(*bad) == ""
+    assert kernel(1 << 24, 128, 128, experts=8) == "128x128" and kernel((1 << 24) + 1, 128, 128, experts=8) == ""
+    assert kernel(4, 128, 128, experts=1025) == "" and kernel(4, 128, 128, experts=-1) == ""
+
+
+@pytest.mark.parametrize("pow2", [0, 1])
+def test_every_kernel_is_compared_with_a_reference(pow2):
+    """The shapes of the GPU tests reach, by the library's rule, every kernel of
+    every product; the tiled ones with up to 16 blocks of k and more, the 256 x
+    256 one with a last tile of at most half the rows and of more."""
+    import test_gpu_f8 as gpu
+
+    def reached(shapes, gate_up, experts=False):
+        found = {}
+        for s in shapes:
+            rows, k, n = (s[0] * s[1], s[3], s[4]) if experts else s
+            found.setdefault(kernel(rows, n, k, gate_up, pow2, s[2] if experts else 0), []).append((rows, k))
+        return found
+
+    for found in (reached(gpu.SHAPES + gpu.MORE, 0), reached(gpu.SHAPES + gpu.MORE_GU, 1)):
+        assert set(found) == set(SPLIT_K + TILED)
+        for name in TILED:
+            blocks = [-(-k // 128) for _, k in found[name]]
+            assert max(blocks) > 16 and (min(blocks) <= 16 or (name == "128x128x2" and pow2))
+        for name in SPLIT_K:  # eight waves, a block each, and a second one
+            assert max(k for _, k in found[name]) > 8 * 128
+        assert {0 < rows % 256 <= 128 for rows, _ in found["256x256"]} == {True, False}
+    for gate_up in (0, 1):
+        found = reached(gpu.EXPERTS + gpu.MORE_EXPERTS, gate_up, experts=True)
+        assert set(found) == {"16x32", "16x64", "128x128", "256x256"}
+        for name, shapes in found.items():
+            assert max(k for _, k in shapes) > 16 * 128
+    # and the rows quantized by the product itself, against the two steps
+    mark = next(m for m in gpu.test_project_quantizing_rows_itself_is_the_two_steps.pytestmark if m.args[0] == "m,k,n")
+    fused = {kernel(m, n, k, 0, pow2) for m, k, n in mark.args[1]
+             if clef_i4.lib().clef_f8_project_workspace_bytes(m, n, k) == 0}
+    assert fused == set(SPLIT_K[:4])

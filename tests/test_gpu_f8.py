@@ -291,6 +291,33 @@ def test_project_gate_up_matches_64_bits(m, k, n, kind):
     assert (out[m:] == 7.0).all()
 
 
+# Shapes of the kernels that SHAPES does not reach, or not with more than 16 blocks
+# of k (whose row scales are loaded anew): test_f8.py holds by the library's
+# rule that every kernel is among these lists.
+MORE = [(40, 264, 5000), (50, 2120, 4000), (130, 264, 5128), (250, 2184, 4072), (60, 2312, 8000), (20, 2312, 6848),
+        (2300, 2312, 3608), (2060, 4232, 4104), (1030, 2312, 4104)]
+MORE_GU = [(40, 264, 2504), (1000, 392, 6136), (1100, 128, 6136), (1100, 2312, 6136), (1000, 4232, 6136),
+           (20, 2312, 3000), (60, 2312, 4000), (130, 2312, 2504)]
+
+
+@pytest.mark.parametrize("m,k,n", MORE)
+@pytest.mark.parametrize("kind,res", [("f32", False), ("e8m0", True)])
+def test_project_matches_64_bits_on_every_kernel(m, k, n, kind, res):
+    test_project_matches_64_bits(m, k, n, kind, res)
+
+
+@pytest.mark.parametrize("m,k,n", MORE_GU)
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+def test_project_gate_up_matches_64_bits_on_every_kernel(m, k, n, kind):
+    test_project_gate_up_matches_64_bits(m, k, n, kind)
+
+
+@pytest.mark.parametrize("m,k,n", MORE)
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+def test_project_of_whole_numbers_is_exact_on_every_kernel(m, k, n, kind):
+    test_project_of_whole_numbers_is_exact(m, k, n, kind)
+
+
 def whole(shape, top, seed):
     return torch.randint(-top, top + 1, shape, generator=gen(seed), device="cuda").float()
 
@@ -655,6 +682,16 @@ def test_experts_match_64_bits(tokens, topk, experts, k, n, kind):
     sorted_a = clef_i4.prepare_f8(randn((total, k), 1.0, 2)[order])
     got = clef_i4.expert_f8(sorted_a, w, offsets, None, 1, True)
     check(got, want[order], slack[order])
+
+
+MORE_EXPERTS = [(1, 8, 128, 2312, 136), (37, 8, 60, 2312, 136), (900, 1, 200, 2312, 136), (900, 2, 5, 2312, 392),
+                (3000, 1, 4, 2312, 3000)]
+
+
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+@pytest.mark.parametrize("tokens,topk,experts,k,n", MORE_EXPERTS)
+def test_experts_match_64_bits_with_more_than_16_blocks(tokens, topk, experts, k, n, kind):
+    test_experts_match_64_bits(tokens, topk, experts, k, n, kind)
 
 
 @pytest.mark.parametrize("n", [136, 2600, 4104])
