@@ -588,6 +588,65 @@ def test_rows_and_slots_beyond_4_gib():
         clef_i4.expert_f8(clef_i4.prepare_f8(x), two, offsets, slots, 1, True)
 
 
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+@pytest.mark.parametrize("m,n", [(3, 264), (60, 2000), (250, 4072), (700, 1544), (1030, 4104), (2100, 3608)])
+def test_project_of_the_widest_rows(m, n, kind):
+    """32768 columns: 256 blocks of k, whole numbers, exact."""
+    test_project_of_whole_numbers_is_exact(m, 32768, n, kind)
+
+
+@pytest.mark.parametrize("m", [1, 40, 700])
+def test_project_onto_the_most_columns(m):
+    """1048576 columns of which a few are looked at, exact."""
+    n, k = 1 << 20, 136
+    x, w = whole((m, k), 7, m).to(BF), whole((n, k), 15, 2)
+    scales = torch.exp2(torch.randint(-3, 1, (n // 128, 2), generator=gen(3), device="cuda").float())
+    packed = clef_i4.f8_weight(w.to(F8), scales)
+    got = clef_i4.project_quantized_f8(x, packed)
+    for at in (slice(0, 300), slice(n // 2 - 130, n // 2 + 130), slice(n - 300, n)):
+        wide = scales.repeat_interleave(128, 0)[at].repeat_interleave(128, 1)[:, :k]
+        want = x.double() @ (w[at] * wide).double().t()
+        assert torch.equal(got[:, at], want.float().to(BF))
+
+
+def test_outputs_beyond_4_gib():
+    """150000 rows of 16384 columns (4.9e9 bytes), projected, onto themselves as
+    the residual, and over lists whose slots run backwards."""
+    m, n, k = 150000, 16384, 8
+    x, w = whole((m, k), 7, 1).to(BF), whole((n, k), 7, 2).to(BF)
+    packed = clef_i4.f8_weight(w.to(F8), torch.ones((n // 128, 1), device="cuda"))
+    a = clef_i4.prepare_f8(x)
+    got = clef_i4.project_f8(a, packed)
+
+    def holds(out, factor):
+        for at in range(0, m, 15000):
+            want = x[at: at + 15000].float() @ w.float().t() * factor
+            assert torch.equal(out[at: at + 15000], want.to(BF))
+
+    holds(got, 1)
+    holds(clef_i4.project_f8(a, packed, got, out=got), 2)
+    two = clef_i4.f8_weight(torch.stack([w.to(F8)] * 2), torch.tensor([1.0, 2.0], device="cuda")[:, None, None].repeat(1, n // 128, 1))
+    slots = torch.arange(m - 1, -1, -1, dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([0, m, m], dtype=torch.int32, device="cuda")
+    holds(clef_i4.expert_f8(a, two, offsets, slots, 1, True, out=got), 1)
+    offsets = torch.tensor([0, 0, m], dtype=torch.int32, device="cuda")
+    holds(clef_i4.expert_f8(a, two, offsets, slots, 1, True, out=got), 2)
+
+
+@pytest.mark.parametrize("m,n", [(2100, 3608), (2100, 264), (9, 264)])
+def test_rows_that_lie_far_apart(m, n):
+    """Row pitches of 2^21 and more elements: addresses past 32 bits."""
+    k = 264
+    pitch = (1 << 21) if m > 9 else (1 << 29) + 8
+    base = torch.empty((m - 1) * pitch + k, dtype=BF, device="cuda")
+    x = base.as_strided((m, k), (pitch, 1))
+    near = randn((m, k), 1.0, 3)
+    x.copy_(near)
+    w = clef_i4.load_f8_weight(randn((n, k), 0.1, 2))
+    assert torch.equal(clef_i4.prepare_f8(x).storage, clef_i4.prepare_f8(near).storage)
+    assert torch.equal(clef_i4.project_quantized_f8(x, w), clef_i4.project_quantized_f8(near, w))
+
+
 def test_two_streams_at_once():
     """Calls in flight side by side have workspaces of their own."""
     w = clef_i4.load_f8_weight(randn((2048, 1032), 0.05, 8))
@@ -627,6 +686,19 @@ def test_group_slots_is_a_stable_sort(tokens, topk, experts):
     assert offsets.cpu().tolist() == [0] + counts.cumsum(0).tolist()
     assert torch.equal(slots[: order.numel()].cpu().long(), order)
     assert (slots[order.numel():] == -1).all()
+
+
+@pytest.mark.parametrize("tokens,topk,experts", [(1 << 20, 16, 1024), (1 << 20, 16, 3), ((1 << 17) - 1, 128, 128)])
+def test_group_slots_of_the_most_routes(tokens, topk, experts):
+    """16777216 slots: chunks of many batches."""
+    ids = torch.randint(-1, experts + 1, (tokens, topk), generator=gen(experts), device="cuda")
+    offsets, slots = clef_i4.omni_group_slots(torch.cat([ids, ids], 1).float(), experts)
+    flat = ids.reshape(-1)
+    key, order = torch.sort(torch.where(flat < 0, experts, flat), stable=True)
+    counts = torch.bincount(key, minlength=experts + 1)[:experts]
+    count = int(counts.sum())
+    assert offsets.tolist() == [0] + counts.cumsum(0).tolist()
+    assert torch.equal(slots[:count].long(), order[:count]) and (slots[count:] == -1).all()
 
 
 # ---------------------------------------------------------------- experts
@@ -747,6 +819,21 @@ def test_experts_past_the_first_128(tokens, experts):
     assert torch.equal(got.float(), (ids // 64 * 16 + ids % 64 // 4).float().expand(tokens, n).to(BF).float())
 
 
+def test_experts_of_the_most_slots():
+    """16777216 slots of 8 experts, each expert's weight its number: exact."""
+    total, experts, k, n = 1 << 24, 8, 8, 8
+    bounds = [0, 5, 5, 1 << 20, (1 << 20) + 129, 1 << 22, 1 << 23, total - 1, total]
+    offsets = torch.tensor(bounds, dtype=torch.int32, device="cuda")
+    values = torch.arange(1, experts + 1, device="cuda").float()
+    w = clef_i4.f8_weight(values[:, None, None].expand(experts, n, k).to(F8), torch.ones((experts, 1, 1), device="cuda"))
+    x = torch.zeros((total, k), dtype=BF, device="cuda")
+    x[:, 5] = (torch.arange(total, device="cuda") % 15 + 1).to(BF)
+    got = clef_i4.expert_f8(clef_i4.prepare_f8(x), w, offsets, None, 1, True)
+    counts = torch.tensor(bounds, device="cuda").diff()
+    want = x[:, 5].float() * torch.repeat_interleave(values, counts)
+    assert (got.float() == want[:, None]).all()
+
+
 @pytest.mark.parametrize("n", [136, 2048])
 def test_experts_overlapping_lists_stay_inside(n):
     """Lists that name places twice make more tiles than sound ones can: a row
@@ -794,6 +881,24 @@ def test_moe_layer_is_its_steps(tokens):
         want += routes[:, 4 + r, None].double() * y
     # five codes on the way (x, gate, up, h, down), each off by at most 2^-4
     assert (got.double() - want).norm() / want.norm() < 5 * 2.0 ** -4
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 600])
+def test_moe_layer_rows_without_experts(tokens):
+    """Tokens whose logits leave fewer experts than topk, or none (all masked,
+    NaN): the other tokens' outputs are as without them."""
+    layer, _ = moe()
+    x, logits = randn((tokens + 4, 264), 1.0, 4), randn((tokens + 4, 16), 1.0, 5)
+    want = layer(x, logits)
+    at = [0, tokens // 2, tokens + 1, tokens + 3]
+    logits[at[0]] = float("nan")
+    logits[at[1]] = float("-inf")
+    logits[at[2], 2:] = torch.finfo(BF).min
+    logits[at[3], 1:] = float("-inf")
+    kept = [i for i in range(tokens + 4) if i not in at]
+    torch.full((tokens * 16 + 64, 264), float("nan"), dtype=BF, device="cuda")  # what the intermediates may find
+    got = layer(x, logits)
+    assert got.shape == want.shape and torch.equal(got[kept], want[kept])
 
 
 @pytest.mark.parametrize("tokens", [3, 200])
