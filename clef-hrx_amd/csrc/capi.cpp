@@ -829,6 +829,7 @@ namespace {
 
 constexpr const char* kF8Shape = "unsupported FP8 block shape";
 constexpr const char* kF8Overlap = "FP8 output overlaps its input rows";
+constexpr const char* kF8WeightOverlap = "FP8 weight output overlaps its input";
 constexpr int32_t kF8Widest = 32768, kF8MostRows = 1048576, kF8MostExperts = 1024;
 
 bool f8_width(int32_t v) { return v >= 8 && v <= kF8Widest && v % 8 == 0; }
@@ -845,6 +846,17 @@ int check_f8_weight(int64_t matrices, int32_t n, int32_t k) {
   if (!(matrices >= 1 && matrices <= kF8MostExperts && f8_columns(n) && f8_width(k) &&
         matrices * clef::f8_blocks(n) * clef::f8_blocks(k) < ((int64_t)1 << 31)))
     return fail(kF8Shape);
+  return CLEF_OK;
+}
+
+// The outputs bf16 [m][n] of a product over `rows` prepared rows lie apart from
+// these, and from the residual unless they are the same memory.
+int check_f8_output(const void* out, int64_t m, int32_t n, const void* a, int64_t rows, int32_t k,
+                    const void* residual) {
+  const size_t bytes = (size_t)m * n * 2;
+  if (a != nullptr && overlap(a, (size_t)clef::f8_prepared_bytes(rows, k), out, bytes)) return fail(kF8Overlap);
+  if (residual != nullptr && residual != out && overlap(residual, bytes, out, bytes))
+    return fail("FP8 output overlaps a part of its residual");
   return CLEF_OK;
 }
 
@@ -890,6 +902,8 @@ int clef_f8_prepare(const uint16_t* x, int64_t rows, int32_t width, int64_t x_st
     return fail(kF8Shape);
   if (rows == 0) return CLEF_OK;
   if (!aligned(x, 16) || !aligned(out, 16)) return fail(kAlign);
+  if (overlap(x, (size_t)((rows - 1) * x_stride + width) * 2, out, (size_t)clef::f8_prepared_bytes(rows, width)))
+    return fail(kF8Overlap);
   uint8_t* exponents = out + rows * clef::f8_pitch(width);
   float* scales = reinterpret_cast<float*>(exponents + rows * clef::f8_scale_pitch(width));
   return hip_status(clef::launch_f8_prepare(x, rows, width, x_stride, out, exponents, scales, hs(stream)));
@@ -899,12 +913,17 @@ int clef_f8_pack_weight(const uint16_t* w, int64_t matrices, int32_t n, int32_t 
                         clef_stream_t stream) {
   if (int rc = check_f8_weight(matrices, n, k)) return rc;
   if (!aligned(w, 16) || !aligned(codes, 16) || !aligned(scales, 16)) return fail(kAlign);
+  const size_t in = (size_t)matrices * n * k * 2, out = (size_t)clef::f8_weight_bytes(matrices, n, k);
+  if (overlap(w, in, codes, out) || overlap(w, in, scales, out / 4096) || overlap(codes, out, scales, out / 4096))
+    return fail(kF8WeightOverlap);
   return hip_status(clef::launch_f8_pack(w, matrices, n, k, codes, scales, hs(stream)));
 }
 
 int clef_f8_retile(const uint8_t* w, int64_t matrices, int32_t n, int32_t k, uint8_t* codes, clef_stream_t stream) {
   if (int rc = check_f8_weight(matrices, n, k)) return rc;
   if (!aligned(w, 16) || !aligned(codes, 16)) return fail(kAlign);
+  if (overlap(w, (size_t)matrices * n * k, codes, (size_t)clef::f8_weight_bytes(matrices, n, k)))
+    return fail(kF8WeightOverlap);
   return hip_status(clef::launch_f8_retile(w, matrices, n, k, codes, hs(stream)));
 }
 
@@ -925,6 +944,7 @@ int clef_f8_gemm(const uint8_t* a, const uint8_t* w, const float* w_scales, int6
   if (!aligned(a, 16) || !aligned(w, 16) || !aligned(w_scales, 16) || !aligned(out, 16) ||
       (residual && !aligned(residual, 16)))
     return fail(kAlign);
+  if (int rc = check_f8_output(out, m, n, a, m, k, residual)) return rc;
   clef::F8Args x{};
   set_f8_activation(x, a, m, k);
   x.w = w, x.ws = w_scales, x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
@@ -940,6 +960,7 @@ int clef_f8_gemm_gate_up(const uint8_t* a, const uint8_t* gate, const float* gat
   if (!aligned(a, 16) || !aligned(gate, 16) || !aligned(gate_scales, 16) ||
       !aligned(up, 16) || !aligned(up_scales, 16) || !aligned(h, 16))
     return fail(kAlign);
+  if (int rc = check_f8_output(h, m, n, a, m, k, nullptr)) return rc;
   clef::F8Args x{};
   set_f8_activation(x, a, m, k);
   x.w = gate, x.ws = gate_scales, x.w2 = up, x.ws2 = up_scales;
@@ -964,6 +985,7 @@ int clef_f8_project(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, c
   const bool apart = !overlap(x, (size_t)((m - 1) * x_stride + k) * 2, out, (size_t)m * n * 2);
   if (clef::f8_project_fusable(m, n, k)) {
     if (!apart) return fail(kF8Overlap);
+    if (int rc = check_f8_output(out, m, n, nullptr, 0, k, residual)) return rc;
     clef::F8Args y{};
     y.x = x, y.x_stride = x_stride, y.k = k, y.rows = m, y.w = w, y.ws = w_scales, y.n = n;
     y.kb = clef::f8_blocks(k), y.pow2 = pow2 != 0, y.residual = residual, y.out = out;
@@ -973,6 +995,9 @@ int clef_f8_project(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, c
   if (workspace_bytes < clef_f8_project_workspace_bytes(m, n, k)) return fail(kWorkspace);
   if (!apart) return fail(kF8Overlap);
   uint8_t* a = static_cast<uint8_t*>(workspace);
+  if (int rc = check_f8_output(out, m, n, a, m, k, residual)) return rc;
+  if (residual && overlap(residual, (size_t)m * n * 2, a, (size_t)clef::f8_prepared_bytes(m, k)))
+    return fail("FP8 workspace overlaps an operand");
   if (int rc = clef_f8_prepare(x, m, k, x_stride, a, stream)) return rc;
   return clef_f8_gemm(a, w, w_scales, m, n, k, pow2, residual, out, stream);
 }
@@ -1001,6 +1026,7 @@ int clef_moe_expert_f8(const uint8_t* a, int64_t a_rows, const uint8_t* w, const
   if (total == 0) return CLEF_OK;
   if (!aligned(a, 16) || !aligned(w, 16) || !aligned(w_scales, 16) || !aligned(out, 16))
     return fail(kAlign);
+  if (int rc = check_f8_output(out, total, n, a, a_rows, k, nullptr)) return rc;
   clef::F8Args x{};
   set_f8_activation(x, a, a_rows, k);
   x.w = w, x.ws = w_scales, x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
@@ -1018,6 +1044,7 @@ int clef_moe_expert_gate_up_f8(const uint8_t* a, int64_t a_rows, const uint8_t* 
   if (!aligned(a, 16) || !aligned(gate, 16) || !aligned(gate_scales, 16) ||
       !aligned(up, 16) || !aligned(up_scales, 16) || !aligned(h, 16))
     return fail(kAlign);
+  if (int rc = check_f8_output(h, total, n, a, a_rows, k, nullptr)) return rc;
   clef::F8Args x{};
   set_f8_activation(x, a, a_rows, k);
   x.w = gate, x.ws = gate_scales, x.w2 = up, x.ws2 = up_scales;

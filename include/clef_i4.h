@@ -515,12 +515,13 @@ int64_t clef_f8_weight_bytes(int64_t matrices, int64_t n, int32_t k);
  * row and block the scale is the least power of two at or above amax / 448
  * (2^-126 at least) and the code e4m3(x / scale), exact but for e4m3's
  * rounding to nearest even. Non-finite values do not count in amax and become
- * NaN codes. */
+ * NaN codes. An output that overlaps x -> "FP8 output overlaps its input rows". */
 int clef_f8_prepare(const uint16_t* x, int64_t rows, int32_t width, int64_t x_stride, uint8_t* out,
                     clef_stream_t stream);
 
 /* bf16 weights [matrices][n][k] -> tiled codes and scales, the quantizer's
- * rule on each 128 x 128 block. */
+ * rule on each 128 x 128 block. Outputs that overlap the input or each other (here
+ * and in clef_f8_retile) -> "FP8 weight output overlaps its input". */
 int clef_f8_pack_weight(const uint16_t* w, int64_t matrices, int32_t n, int32_t k, uint8_t* codes, float* scales,
                         clef_stream_t stream);
 
@@ -541,8 +542,9 @@ const char* clef_f8_kernel_name(int64_t rows, int32_t n, int32_t k, int32_t gate
  * unit may then apply them (with other
  * scales it would drop their mantissas). The same sums within f32 rounding.
  * Scales of any size: a block's sum leaves f32's range only where it does with
- * both of its scales applied. The output may be the residual itself and overlaps
- * no other input. */
+ * both of its scales applied. The output may be the residual itself; over a part
+ * of it -> "FP8 output overlaps a part of its residual", over the activation (in
+ * every product below too) -> "FP8 output overlaps its input rows". */
 int clef_f8_gemm(const uint8_t* a, const uint8_t* w, const float* w_scales, int64_t m,
                  int32_t n, int32_t k, int32_t pow2, const uint16_t* residual, uint16_t* out, clef_stream_t stream);
 
@@ -553,8 +555,9 @@ int clef_f8_gemm_gate_up(const uint8_t* a, const uint8_t* gate, const float* gat
 
 /* clef_f8_prepare and clef_f8_gemm in one call; the workspace (bytes below, 0
  * where the product quantizes the rows itself: then each of its workgroups reads
- * its rows of x) takes the activation. An output that overlaps x -> "FP8 output
- * overlaps its input rows". */
+ * its rows of x) takes the activation. An output that overlaps x or the workspace
+ * -> "FP8 output overlaps its input rows", a residual the workspace -> "FP8
+ * workspace overlaps an operand". */
 size_t clef_f8_project_workspace_bytes(int64_t m, int32_t n, int32_t k);
 int clef_f8_project(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint8_t* w, const float* w_scales,
                     int32_t n, int32_t pow2, const uint16_t* residual, uint16_t* out, void* workspace,

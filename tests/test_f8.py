@@ -258,3 +258,37 @@ def test_every_kernel_is_compared_with_a_reference(pow2):
     fused = {kernel(m, n, k, 0, pow2) for m, k, n in mark.args[1]
              if clef_i4.lib().clef_f8_project_workspace_bytes(m, n, k) == 0}
     assert fused == set(SPLIT_K[:4])
+
+
+APART = 1 << 34
+
+
+def test_outputs_over_their_inputs_are_refused():
+    """Kernels read and write in parallel: an output over what other workgroups
+    still read would hold anything."""
+    rows_message, residual_message = "FP8 output overlaps its input rows", "FP8 output overlaps a part of its residual"
+    weight_message = "FP8 weight output overlaps its input"
+    need = clef_i4.lib().clef_f8_prepared_bytes(64, 256)
+    for out in (FAKE, FAKE + 64 * 512 - 16, FAKE - need + 16):
+        assert call("clef_f8_prepare", FAKE, 64, 256, 256, out, None) == (-1, rows_message)
+    assert call("clef_f8_prepare", FAKE, 64, 256, 1024, FAKE + 63 * 2048, None) == (-1, rows_message)
+    for codes in (FAKE, FAKE + 256 * 256 - 16, FAKE - 4 * 16384 + 16):
+        assert call("clef_f8_retile", FAKE, 1, 256, 256, codes, None) == (-1, weight_message)
+        assert call("clef_f8_pack_weight", FAKE, 1, 256, 256, codes, FAKE + APART, None) == (-1, weight_message)
+    assert call("clef_f8_pack_weight", FAKE, 1, 256, 256, FAKE + APART, FAKE, None) == (-1, weight_message)
+    assert call("clef_f8_pack_weight", FAKE, 1, 256, 256, FAKE + APART, FAKE + APART, None) == (-1, weight_message)
+    a, w, s, far = FAKE, FAKE + APART, FAKE + 2 * APART, FAKE + 3 * APART
+    for out in (a, a + need - 16, a - 64 * 128 * 2 + 16):
+        assert call("clef_f8_gemm", a, w, s, 64, 128, 256, 0, None, out, None) == (-1, rows_message)
+        assert call("clef_f8_gemm_gate_up", a, w, s, w, s, 64, 128, 256, 0, out, None) == (-1, rows_message)
+        assert call("clef_moe_expert_f8", a, 64, w, s, far, far, 8, 64, 1, 1, 256, 128, 0, out, None) == (-1, rows_message)
+        assert call("clef_moe_expert_gate_up_f8", a, 64, w, s, w, s, far, far, 8, 64, 1, 1, 256, 128, 0, out, None) == \
+            (-1, rows_message)
+    for m, n in ((64, 128), (4096, 256)):
+        for shift in (256, -256, m * n * 2 - 16):
+            assert call("clef_f8_gemm", a, w, s, m, n, 256, 0, far + shift, far, None) == (-1, residual_message)
+            assert call("clef_f8_project", a, m, 256, 256, w, s, n, 0, far + shift, far, far + APART, 1 << 30, None) == \
+                (-1, residual_message)
+    assert call("clef_f8_project", a, 4096, 256, 256, w, s, 256, 0, None, far, far, 1 << 30, None) == (-1, rows_message)
+    assert call("clef_f8_project", a, 4096, 256, 256, w, s, 256, 0, far, far + APART, far, 1 << 30, None) == \
+        (-1, "FP8 workspace overlaps an operand")

@@ -999,3 +999,20 @@ def test_weights_smaller_than_they_say_are_refused():
               lambda: clef_i4.expert_gate_up_f8(a, two, F8Weight(two.codes, two.scales[:1], 136, 256, 2), offsets, None, 1, True)):
         with pytest.raises(clef_i4.ClefError):
             f()
+
+
+@pytest.mark.parametrize("m,n", [(4, 128), (700, 2056)])
+def test_outputs_over_their_inputs_are_refused(m, n):
+    """Views of one buffer, as a caller saving memory would pass them."""
+    k = 256
+    x, w = randn((m, k), 1.0, 1), clef_i4.load_f8_weight(randn((n, k), 0.1, 2))
+    a = clef_i4.prepare_f8(x)
+    kept, both = x.clone(), randn((m + 1, n), 1.0, 3)
+    for f in (lambda: clef_i4.prepare_f8(x[: m // 2], out=x.view(torch.uint8).view(-1)),
+              lambda: clef_i4.project_f8(a, w, both[:m], out=both[1:]),
+              lambda: clef_i4.project_quantized_f8(x, w, both[1:], out=both[:m])):
+        with pytest.raises(clef_i4.ClefError):
+            f()
+    assert torch.equal(x, kept)
+    want = clef_i4.project_f8(a, w, both[:m])
+    assert torch.equal(clef_i4.project_f8(a, w, both[:m], out=both[:m]), want)
