@@ -871,6 +871,7 @@ class MoeLayer:
 # "block-scaled FP8"); no counterpart in the reference.
 
 _BAD_F8 = "unsupported FP8 block shape"
+_ELSEWHERE = "operands must be on the current device"
 
 
 def _on_current(*tensors) -> None:
@@ -879,7 +880,7 @@ def _on_current(*tensors) -> None:
     device = torch._C._cuda_getDevice()
     for t in tensors:
         if t is not None and t.get_device() != device:
-            raise ClefError(-1, "operands must be on the current device")
+            raise ClefError(-1, _ELSEWHERE)
 
 
 def _f8_rows(x: torch.Tensor):
@@ -971,13 +972,14 @@ class F8Weight:
     matrices: int = 1
     pow2: bool = False    # every scale is a power of two: the matrix unit may apply them
 
-    def check(self) -> None:
+    def check(self) -> int:
         """The kernels know rows, cols and matrices alone: codes and scales are
-        as large as those say, on the current device."""
+        as large as those say, on the current device, whose index this is."""
         blocks = self.matrices * ((self.rows + 127) // 128) * ((self.cols + 127) // 128)
-        if not _n.holds(torch._C._cuda_getDevice(), self.codes, torch.uint8, blocks * 16384,
-                        self.scales, torch.float32, blocks):
+        device = torch._C._cuda_getDevice()
+        if not _n.holds(device, self.codes, torch.uint8, blocks * 16384, self.scales, torch.float32, blocks):
             raise ClefError(-1, "FP8 weight: codes or scales too small, of another type or not on the current device")
+        return device
 
 
 def _f8_weight_storage(w: torch.Tensor):
@@ -1025,19 +1027,20 @@ def project_f8(a: PreparedF8, w: F8Weight, residual: torch.Tensor | None = None,
     """Block-scaled FP8 projection (clef_f8_gemm): bf16 [rows][w.rows]."""
     if a.width != w.cols or w.matrices != 1:
         raise ClefError(-1, _BAD_F8)
-    w.check()
-    _check_residual(residual, a.rows, w.rows)
+    device = w.check()
+    if residual is not None:
+        _check_residual(residual, a.rows, w.rows, device)
     storage = a.call_arg()
     out = _f8_out(storage, a.rows, w.rows, out)
     _n.launch(_n.clef_f8_gemm, storage, w.codes, w.scales, a.rows, w.rows, w.cols, int(w.pow2), residual, out)
     return out
 
 
-def _check_residual(residual: torch.Tensor | None, rows: int, cols: int) -> None:
-    if residual is not None:
-        if tuple(residual.shape) != (rows, cols) or residual.dtype != torch.bfloat16:
-            raise ClefError(-1, "residual shape/dtype mismatch")
-        _on_current(residual)
+def _check_residual(residual: torch.Tensor, rows: int, cols: int, device: int) -> None:
+    if tuple(residual.shape) != (rows, cols) or residual.dtype != torch.bfloat16:
+        raise ClefError(-1, "residual shape/dtype mismatch")
+    if residual.get_device() != device:
+        raise ClefError(-1, _ELSEWHERE)
 
 
 def project_quantized_f8(x: torch.Tensor, w: F8Weight, residual: torch.Tensor | None = None,
@@ -1046,9 +1049,11 @@ def project_quantized_f8(x: torch.Tensor, w: F8Weight, residual: torch.Tensor | 
     address, m, k, pitch = _f8_rows(x)
     if k != w.cols or w.matrices != 1:
         raise ClefError(-1, _BAD_F8)
-    w.check()
-    _on_current(x)
-    _check_residual(residual, m, w.rows)
+    device = w.check()
+    if x.get_device() != device:
+        raise ClefError(-1, _ELSEWHERE)
+    if residual is not None:
+        _check_residual(residual, m, w.rows, device)
     out = _f8_out(x, m, w.rows, out)
     nbytes = _n.value(_n.clef_f8_project_workspace_bytes, m, w.rows, k)
     ws = _n.empty(x, torch.uint8, nbytes) if nbytes > 0 else None
@@ -1096,8 +1101,9 @@ def _check_lists(a: PreparedF8, w: F8Weight, offsets: torch.Tensor, slots: torch
     if offsets.dtype != torch.int32 or offsets.numel() != w.matrices + 1 or (slots is not None
                                                                              and slots.dtype != torch.int32):
         raise ClefError(-1, "invalid grouped expert lists")
-    w.check()
-    _on_current(offsets, slots)
+    device = w.check()
+    if offsets.get_device() != device or (slots is not None and slots.get_device() != device):
+        raise ClefError(-1, _ELSEWHERE)
     if slots is not None:
         return slots.numel()
     return a.rows if input_routed else a.rows * topk
