@@ -11,6 +11,11 @@
 // property of the FP8 matrix unit, measured with single products beside a pair
 // that cancels); the eights and everything behind them add in f32. Against 64
 // bits the sums are off by about 1e-5 of their size, bf16 by 1.7e-3.
+//
+// Times below are in us. "From memory" means operands in turn that pass the
+// last-level cache together (256 MB), as in a model whose layers follow each
+// other; where two variants are compared, both ran in turn on one card. Cards
+// differ by some percent.
 #include "f8.hpp"
 
 namespace clef {
@@ -19,10 +24,12 @@ namespace {
 
 // The most values of a tile's rows that a split-k workgroup quantizes itself: ten
 // passes of its threads, 0.3 us each (instructions, and loads of rows that every
-// workgroup reads), against the quantizer's launch (m x k x n, us for one launch
-// and for two: 64 x 1536 x 2048, six passes, 4.9 and 5.5; 8 x 4096 x 2048, eight,
-// 5.9 and 6.5; 16 x 2560 x 2048, ten, 6.2 and 6.1, and 8 x 5120 x 8192 11.4 and
-// 10.5) and the 2.5 to 4 us more that two launches take the host (6.3 and 9.0).
+// workgroup reads), against the quantizer's launch. From memory, m x k x n with
+// one launch and with two: 64 x 1024 x 2048, four passes, 4.4 and 5.6; 64 x 1536 x
+// 2048, six, 5.5 and 6.0; 8 x 4096 x 2048, eight, 8.9 and 8.5; 16 x 2560 x 2048,
+// ten, 8.2 and 7.6, and 8 x 5120 x 8192 13.1 and 12.1. From eight passes up the
+// device gains nothing more, but two launches take the host 3.5 us longer (8.6
+// against 5.0 through the binding), which is what such calls wait for.
 constexpr int kQxValues = 10 * 512 * 8;
 
 // Few rows: each workgroup owns 16 MT rows x 16 NT weight rows (gate/up: NT / 2
@@ -35,10 +42,11 @@ constexpr int kQxValues = 10 * 512 * 8;
 //
 // A wave has one block of k on its way: a second or third costs registers, and
 // with them workgroups per CU, and gained nothing anywhere (16 x 32 tiles, 1, 2
-// and 3 blocks in us: 37 x 4160 x 1352 5.4, 5.8, 5.7; 3 x 15208 x 1960 9.4, 9.5,
-// 10.1; 16 x 64, 60 tokens of 60 experts top-1 gate/up 408 x 2 2968 46, 55, 67). Waves
-// without a block issue nothing: loads through empty resources took as long as
-// others (1 x 448 x 2 1336 with two blocks 3.1 us, 2.6 without them).
+// and 3 blocks, three weights in turn, mostly from the last-level cache: 37 x 4160 x
+// 1352 5.4, 5.8, 5.7; 3 x 15208 x 1960 9.4, 9.5, 10.1; 16 x 64, 60 tokens of 60
+// experts top-1 gate/up 408 x 2 2968 46, 55, 67). Waves without a block issue
+// nothing: loads through empty resources took as long as others (1 x 448 x 2 1336
+// with two blocks 3.1, 2.6 without them).
 //
 // QX: the rows come in bf16 (p.x) and every workgroup quantizes its tile's into
 // LDS first, by the quantizer's rule, while its first weights are on their way.
@@ -763,18 +771,20 @@ F8Kernel stream_kernel(int64_t m, int64_t n) {
 
 }  // namespace
 
-// From the smallest tiles up: 16 x 32, 16 x 64, 32 x 64
-// and 64 x 64 of the split-k kernel while they are at most one per CU (m x k x n
-// in us: 133 x 5784 x 288 6.3 on 16 x 32 tiles, 7.9, 10.7, 16.3 on the larger
-// ones; 170 x 3600 x 3808 24.8, 14.1, 15.2 and 12.5), and 32 x 32 where one tile
-// has all rows and reads the weights once (20 x 14512 x 6848 20.8 against 29.5 on
-// 16 x 64, 29 x 1072 x 7976 3.7 against 5.1); beyond, 128 x 128 tiles, two
-// workgroups per CU (256 x 4096 x 12288: 19 against 39 on 64 x 64), and 256 x
+// From the smallest tiles up (all of it measured from memory, f32 scales): 16 x 32,
+// 16 x 64, 32 x 64 and 64 x 64 of the split-k kernel while they are at most one per
+// CU (m x k x n: 133 x 5784 x 288 6.4 on 16 x 32 tiles, 7.9, 10.8, 16.6 on the larger
+// ones; 170 x 3600 x 3808 25.3, 15.1, 16.1 and 13.4), and 32 x 32 where one tile
+// has all rows and reads the weights once (20 x 14512 x 6848 22.6 against 29.7 on
+// 16 x 64, 29 x 1072 x 7976 5.1 against 5.7); beyond, 128 x 128 tiles, two
+// workgroups per CU (256 x 4096 x 12288: 24.6 against 40.7 on 64 x 64), and 256 x
 // 256 tiles from three times their rounds over the CUs up, a 256 x 256 round
-// taking about three of 128 x 128 (1024 x 4096 x 12288, 1 and 3 rounds: 49
-// against 52; 1536, 2 and 5: 95 against 81; 4096, 3 and 12: 174 against 218).
+// taking about three of 128 x 128 (1024 x 4096 x 12288, 1 and 3 rounds: 53
+// against 61; 1536, 2 and 5: 98 against 92; 4096, 3 and 12: 178 against 225).
 // One tile of 16 rows against more columns than 256 tiles cover stays on 16 x
-// 32 (16 x 5120 x 2 17408: 39 against 44 on 128 x 128).
+// 32 (16 x 5120 x 2 17408: 36 against 45.5 on 128 x 128). Where k is long and the
+// 128 x 128 tiles cover a third of the CUs this is not the best: 200 x 17408 x 5120
+// takes 71 on them and 66 on 64 x 64.
 F8Kernel f8_kernel(int64_t m, int n, int kb, bool gate_up, bool pow2) {
   const int64_t rows_of_w = (int64_t)n * (gate_up ? 2 : 1);
   const F8Kernel few = stream_kernel(m, rows_of_w);
@@ -784,21 +794,21 @@ F8Kernel f8_kernel(int64_t m, int n, int kb, bool gate_up, bool pow2) {
   if (small >= 3 * rounds(256, 256)) return F8Kernel::k256x256;
   // One tile per CU: two blocks of k at a time on two groups of waves, which read
   // less LDS per MFMA and have more loads on their way, against a longer start and
-  // the groups' sums (f32 scales, us for 128 x 128 tiles and these: 620 x 17408 x
-  // 5120 80 and 72, 512 x 4096 x 4096 18.4 and 17.1, 768 x 512 x 4096, 4 blocks of
-  // k, 5.9 and 6.8; powers of two: 620 x 17408 x 5120 76.7 and 72.2, 300 x 8192 x
-  // 8192 36.8 and 35.0, 300 x 5120 x 2 5120 22.0 and 21.5, 256 x 4096 x 12288 16.8
-  // and 16.7, 640 x 2048 x 2048 9.4 and 10.3).
+  // the groups' sums (from memory, f32 scales, 128 x 128 tiles and these: 620 x
+  // 17408 x 5120 82.7 and 76.2, 512 x 4096 x 4096 21.0 and 20.6, 768 x 512 x 4096, 4
+  // blocks of k, 7.1 and 8.2; powers of two: 620 x 17408 x 5120 78.8 and 73.8, 300 x
+  // 8192 x 8192 38.6 and 35.1, 300 x 5120 x 2 5120 27.7 and 26.1, 256 x 4096 x
+  // 12288 24.2 and 24.3, 640 x 2048 x 2048 12.2 and 13.0).
   return small <= 1 && kb >= (pow2 ? 40 : 16) ? F8Kernel::k128x128k : F8Kernel::k128x128;
 }
 
 // Experts with few rows, whose weights are read once whatever the tile. As
-// many tiles as CUs: 16 x 32, then 16 x 64 (8 slots of 128 experts, gate/up 2048
-// x 2 768: 4.6 us on 16 x 64, 4.7 on 16 x 32 and 9.8 on 128 x 128; 57 of 8, 2928 x
-// 464: 4.8 on 16 x 32, 5.6, 12.9). More: 16 x 64 below sixteen rows per expert
-// (gate/up, 540 slots of 128 568 x 2 1440 40.6 against 51.7 on 128 x 128, 793 of
-// 60 3112 x 2 712 51.7 against 53.5; 1063 of 64 584 x 2 256, 16.6 rows each, 8.9
-// against 7.9). The experts named: about total E / (total + E). Then as without
+// many tiles as CUs: 16 x 32, then 16 x 64 (from memory: 8 slots of 128 experts,
+// gate/up 2048 x 2 768, 8.3 on 16 x 64, 8.9 on 16 x 32 and 14.3 on 128 x 128; 57 of 8,
+// 2928 x 464, 6.8 on 16 x 32, 8.0, 17.3). More: 16 x 64 below sixteen rows per expert
+// (gate/up, 540 slots of 128 568 x 2 1440 54.6 against 66.2 on 128 x 128, 793 of
+// 60 3112 x 2 712 57.8 against 64.8; 1063 of 64 584 x 2 256, 16.6 rows each, 9.8
+// against 9.4). The experts named: about total E / (total + E). Then as without
 // lists, as if evenly filled (a little more, for those above the mean).
 F8Kernel f8_kernel_lists(int64_t total, int64_t experts, int n, bool gate_up) {
   const int64_t rows_of_w = (int64_t)n * (gate_up ? 2 : 1), least = total < experts ? total : experts;

@@ -17,7 +17,8 @@ constexpr int64_t kPartWorkgroups = (int64_t)1 << 22;
 // store of codes (a whole line per block). A workgroup covers 2^RLOG rows x CPW *
 // STEPS blocks, so that the f32 scales of neighbouring rows go out together, with
 // STEPS loads in flight per lane. Bound by HBM: 2 bytes read and 1 written per
-// value, 5.5 TB/s at 4096 x 12288 (27.6 us).
+// value, 4.6 to 5.2 TB/s at 4096 x 12288 (33 us in a graph of inputs and outputs
+// that pass the last-level cache, 29 called one by one).
 template <int RLOG, int STEPS>
 __global__ __launch_bounds__(256) void f8_prepare_kernel(const uint16_t* __restrict__ x, int64_t rows, int width,
                                                          int64_t x_stride, int kb, int kp,
@@ -65,7 +66,8 @@ __device__ __forceinline__ int f8_block_byte(int row, int k) {
 // One workgroup per 128 x 128 block of a bf16 weight: thread t takes 8 chunks
 // of 8 columns (rows t / 16 + 16 i, columns 8 (t % 16) ..), the block's maximum
 // meets in LDS, and the codes go out in the operand order. Weights are packed
-// once, at load.
+// once, at load. Bound by HBM, 2 bytes read and 1 written per value: 128 x 2048 x
+// 768 112 us (5.4 TB/s), 12288 x 4096 33 us (4.6), 1352 x 4160 6.5 us.
 __global__ __launch_bounds__(256) void f8_pack_kernel(const uint16_t* __restrict__ w, int n, int k, int nb, int kb,
                                                       uint8_t* __restrict__ codes, float* __restrict__ scales) {
   __shared__ uint32_t wave_max[4];
@@ -106,7 +108,9 @@ __global__ __launch_bounds__(256) void f8_pack_kernel(const uint16_t* __restrict
 }
 
 // e4m3 rows [matrices][n][k] -> blocks in the operand order; one workgroup per
-// block, 8 bytes per thread and row (k % 8 == 0).
+// block, 8 bytes per thread and row (k % 8 == 0). Bound by HBM, a byte read and a
+// byte written per value: 128 x 2048 x 768 79 us (5.1 TB/s), 12288 x 4096 25 us
+// (4.1), 1352 x 4160 6.0 us.
 __global__ __launch_bounds__(256) void f8_retile_kernel(const uint8_t* __restrict__ w, int n, int k, int nb, int kb,
                                                         uint8_t* __restrict__ codes) {
   const int64_t block = blockIdx.x;
@@ -139,10 +143,10 @@ hipError_t launch_f8_prepare(const uint16_t* x, int64_t rows, int width, int64_t
         <<<grid, 256, 0, stream>>>(x, rows, width, x_stride, kb, kp, codes, exponents, scales);
   };
   using std::integral_constant;
-  // Four loads ahead from 16M values up (4096 x 4096 9.0 us against 9.7 with
-  // two, 32768 x 768 13.4 against 15.8), two below (620 x 17408 7.1 against 7.4).
-  // Four rows per workgroup (4096 x 4096 with 1, 2 or 8: 10.4, 9.6, 10.7), one
-  // where there are fewer.
+  // Rows and outputs from memory: four loads ahead from 16M values up (4096 x 4096
+  // 13.2 us against 13.5 with two, 32768 x 768 17.2 against 19.4), two below (37 x
+  // 4160 2.3 against 2.8, 620 x 17408 10.1 with both). Four rows per workgroup
+  // (32768 x 768 with 1, 2 or 8: 28.0, 19.3, 18.6), one where there are fewer.
   if (rows >= 3 && rows * width >= (1 << 24))
     run(integral_constant<int, 2>{}, integral_constant<int, 4>{});
   else if (rows >= 3)

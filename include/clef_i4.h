@@ -538,9 +538,9 @@ const char* clef_f8_kernel_name(int64_t rows, int32_t n, int32_t k, int32_t gate
 
 /* Projection of a prepared activation; residual bf16 [m][n], nullable. pow2
  * (here and below) nonzero: every scale of w is a power of two between 2^-126
- * and 2^127, as clef_f8_pack_weight and e8m0 checkpoints make them; the matrix
- * unit may then apply them (with other
- * scales it would drop their mantissas). The same sums within f32 rounding.
+ * and 2^127 (e8m0's 2^-127 and NaN too), as clef_f8_pack_weight and e8m0
+ * checkpoints make them; the matrix unit may then apply them (with other scales
+ * it would drop their mantissas). The same sums within f32 rounding.
  * Scales of any size: a block's sum leaves f32's range only where it does with
  * both of its scales applied. The output may be the residual itself; over a part
  * of it -> "FP8 output overlaps a part of its residual", over the activation (in
@@ -578,8 +578,8 @@ int clef_moe_group_slots(const float* routes, int64_t tokens, int32_t topk, int3
  * slot s takes activation row input_routed ? s : s / topk and writes row s of
  * out bf16 [total][n]. Rows that no list names are left as they were. Offsets
  * are clamped to 0 .. total and slots outside it are passed over. An expert's
- * list may be empty, and a slot may be listed by one expert only (two would
- * write one row). Preconditions: 1 <= experts <= 1024, total <= 16777216, 1 <=
+ * list may be empty, and a slot may be listed by one expert only (else rows of
+ * out hold either's values or what was there). Preconditions: 1 <= experts <= 1024, total <= 16777216, 1 <=
  * topk <= 128 -> "invalid grouped expert lists"; the shapes above; a_rows >=
  * the rows that total slots need -> "expert lists name more rows than the
  * activation has"; codes of the activation below 4 GiB. */
