@@ -1144,8 +1144,9 @@ def expert_gate_up_f8(a: PreparedF8, gate: F8Weight, up: F8Weight, offsets: torc
 class MoeLayerF8:
     """The Omni MoE block on block-scaled FP8 experts: router, routes listed by
     expert, gate/up with SwiGLU, down, combine (the steps of MoeLayer; the router
-    takes up to 128 experts). The weights hold one matrix per expert: gate and up [inter][hidden], down
-    [hidden][inter]. Every call takes its intermediates from torch's allocator.
+    takes up to 128 experts). The weights hold one matrix per expert: gate and
+    up [inter][hidden], down [hidden][inter]. Every call takes its intermediates
+    from torch's allocator.
     A token whose logits name fewer experts than topk (NaN, or all but a few at
     the type's lowest value or below) has an unspecified output, as in MoeLayer;
     the other tokens' are as without it."""

@@ -6,11 +6,11 @@
 // accumulator by one fma with the factor that is left of sw, which rounds it once
 // more. The tiled kernel lets the instruction add to the accumulator itself where
 // every factor is one. Output values are rounded to bf16 once, behind the residual
-// or SwiGLU. Inside the instruction the
-// products of eight neighbouring k are cut to 2^-13 of the largest of them (a
-// property of the FP8 matrix unit, measured with single products beside a pair
-// that cancels); the eights and everything behind them add in f32. Against 64
-// bits the sums are off by about 1e-5 of their size, bf16 by 1.7e-3.
+// or SwiGLU. Inside the instruction the products of eight neighbouring k are cut
+// to 2^-13 of the largest of them (a property of the FP8 matrix unit, measured
+// with single products beside a pair that cancels); the eights and everything
+// behind them add in f32. Against 64 bits the sums are off by about 1e-5 of their
+// size, bf16 by 1.7e-3.
 //
 // Times below are in us. "From memory" means operands in turn that pass the
 // last-level cache together (256 MB), as in a model whose layers follow each
@@ -289,8 +289,8 @@ hipError_t launch_stream(const F8Args& x, hipStream_t stream) {
 // Behind the stages the rows' e8m0 scales of 16 blocks of k, as loaded (16 bytes
 // per row) and, twice, turned into the order of use (per block of k a lane's TM
 // rows side by side), the scales of the tile's one or two weight panels (256
-// each, as they are or as pairs of the MFMA's exponent and the fma's factor) and, with lists, the
-// tile's output rows.
+// each, as they are or as pairs of the MFMA's exponent and the fma's factor)
+// and, with lists, the tile's output rows.
 template <int WM_, int WN_, int WAVES_M_, int WAVES_N_, int GROUPS_ = 1, int KG_ = 1>
 struct F8Tile {
   static constexpr int GROUPS = GROUPS_;  // workgroups per CU
@@ -485,8 +485,8 @@ __device__ __forceinline__ void f8_tile(const F8Args& p, char* lds, int expert, 
     Panel sw[MATS];
     // of step kt (the step before still takes sa)
     auto read_scales = [&](int kt) {
-      // (a block past the last in a step that counts: its products and its entry
-      // here are zeros, of an odd number of blocks, so below 256)
+      // (the block past an odd number of them: its products are zeros, and so is
+      // its entry here, which lies below 256)
       const int block = T::KG * kt + kg;
 #pragma unroll
       for (int t = 0; t < MATS; ++t) sw[t] = sw_at[t * 256 + (block & 255)];
