@@ -97,6 +97,13 @@ SIGNATURES = {
                                           _P]),
     "clef_moe_expert_gate_up_f8": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32,
                                                   _I32, _I32, _P, _P]),
+    "clef_linear": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _I32, _I64, _P, _I32, _I32, _P, _I64, _P, _I32, _I64,
+                                   _P]),
+    "clef_linear_gate_up": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _P, _I32, _I64, _P, _P, _I32, _I32, _P, _I64,
+                                           _P]),
+    "clef_moe_layer_f8_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32]),
+    "clef_moe_layer_f8": (ctypes.c_int, [_P, _I64, _P, _I32, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P,
+                                         _P, _P, _P, _SZ, _P]),
     "clef_pack_cache_path": (ctypes.c_int, [_P, _P, _P, _SZ]),
     "clef_pack_cache_read": (ctypes.c_int, [_P, _P, _P, _SZ, _P, _SZ, _P]),
     "clef_pack_cache_write": (ctypes.c_int, [_P, _P, _P, _SZ, _P, _SZ]),
@@ -1171,3 +1178,155 @@ class MoeLayerF8:
         h = expert_gate_up_f8(prepare_f8(x), self.gate, self.up, offsets, slots, self.topk)
         values = expert_f8(prepare_f8(h), self.down, offsets, slots, self.topk, input_routed=True)
         return omni_combine(values, routes)
+
+    def decode(self, x: torch.Tensor, logits: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """The layer for up to 16 tokens in two launches (clef_moe_layer_f8),
+        three with the router: out = residual + sum of the experts' outputs,
+        bf16 [tokens][hidden]. The activations stay bf16 and the router's logits
+        f32 (or as given, bf16 or f32), everything is summed in f32 and rounded
+        once, so the result lies closer to the weights' own than that of
+        __call__, which quantizes the rows and rounds between its steps. Logits
+        of NaN and -inf take no part: a token without an expert gets its
+        residual, or zeros. x may be a column range of wider rows; x and the
+        residual may be `out` itself."""
+        address, tokens, hidden, pitch = _f8_rows(x)
+        if hidden != self.gate.cols or tokens > 16:
+            raise ClefError(-1, "unsupported MoE shape for few tokens")
+        device = self.gate.check()
+        self.up.check()
+        self.down.check()
+        if x.get_device() != device:
+            raise ClefError(-1, _ELSEWHERE)
+        if logits is None:
+            if self.router is None:
+                raise ClefError(-1, "MoE layer needs router logits or a router gate weight")
+            logits = linear(x, self.router, dtype=torch.float32)
+        if tuple(logits.shape) != (tokens, self.gate.matrices):
+            raise ClefError(-1, "router logits: one per token and expert")
+        dtype = _logits_dtype(logits)
+        if logits.get_device() != device:
+            raise ClefError(-1, _ELSEWHERE)
+        if residual is not None:
+            _check_residual(residual, tokens, hidden, device)
+        out = _f8_out(x, tokens, hidden, out)
+        inter, experts = self.gate.rows, self.gate.matrices
+        nbytes = _n.value(_n.clef_moe_layer_f8_workspace_bytes, tokens, hidden, inter, experts, self.topk)
+        ws = _n.empty(x, torch.uint8, nbytes)
+        _n.launch(_n.clef_moe_layer_f8, address, pitch, logits, dtype, tokens, hidden, inter, experts, self.topk,
+                  self.gate.codes, self.gate.scales, self.up.codes, self.up.scales, self.down.codes, self.down.scales,
+                  residual, out, ws, nbytes)
+        return out
+
+
+# ---------------------------------------------------------------- bf16 weights
+
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "sigmoid": 5}
+
+_BAD_LINEAR = "linear shape/dtype mismatch"
+
+
+def _linear_rows(t: torch.Tensor, cols: int, device: int) -> int:
+    """Row pitch of bf16 rows of `cols` contiguous elements on the current
+    device: a matrix, or a column range of a wider one."""
+    if t.dim() != 2 or t.dtype != torch.bfloat16 or t.shape[1] != cols:
+        raise ClefError(-1, _BAD_LINEAR)
+    if t.get_device() != device:
+        raise ClefError(-1, _ELSEWHERE)
+    if t.is_contiguous():
+        return cols
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        raise ClefError(-1, _BAD_LINEAR)
+    return t.stride(0) if t.shape[0] > 1 else cols
+
+
+def _linear_bias(bias: torch.Tensor | None, n: int, device: int):
+    """(address, dtype) of a bias of n values."""
+    if bias is None:
+        return None, 0
+    if bias.dtype not in (torch.bfloat16, torch.float32) or tuple(bias.shape) != (n,):
+        raise ClefError(-1, _BAD_LINEAR)
+    if bias.get_device() != device:
+        raise ClefError(-1, _ELSEWHERE)
+    return bias, int(bias.dtype == torch.float32)
+
+
+def _linear_out(like: torch.Tensor, rows: int, cols: int, out: torch.Tensor | None, dtype, device: int):
+    """The output and its row pitch."""
+    if out is None:
+        return _n.empty(like, dtype, rows, cols), cols
+    if tuple(out.shape) != (rows, cols) or out.dtype != dtype:
+        raise ClefError(-1, "output shape/dtype mismatch")
+    if out.get_device() != device:
+        raise ClefError(-1, _ELSEWHERE)
+    if out.is_contiguous():
+        return out, cols
+    if (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
+        raise ClefError(-1, "output shape/dtype mismatch")
+    return out, out.stride(0) if rows > 1 else cols
+
+
+def _activation_code(activation: str | None) -> int:
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise ClefError(-1, "unknown activation")
+    return code
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+           residual: torch.Tensor | None = None, out: torch.Tensor | None = None, dtype: torch.dtype | None = None
+           ) -> torch.Tensor:
+    """Projection on a weight that stays bf16 (clef_linear): act(x @ weight.T +
+    bias) + residual, [rows][weight.shape[0]] in bf16 or f32 (`dtype`; out's
+    where given), f32 up to the one rounding. The reference's Engine::linear
+    (src/ops.rs:95-175) with an epilogue. x [rows][k] and weight [n][k] bf16, bias
+    [n] bf16 or f32, residual bf16, activation one of ACTIVATIONS. x, weight,
+    residual and out may be column ranges of wider rows; out may be the residual
+    itself."""
+    if weight.dim() != 2:
+        raise ClefError(-1, _BAD_LINEAR)
+    n, k = weight.shape
+    device = torch._C._cuda_getDevice()
+    x_pitch, w_pitch = _linear_rows(x, k, device), _linear_rows(weight, k, device)
+    bias, bias_dtype = _linear_bias(bias, n, device)
+    m = x.shape[0]
+    if dtype is None:
+        dtype = torch.bfloat16 if out is None else out.dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        raise ClefError(-1, _BAD_LINEAR)
+    residual_pitch = n
+    if residual is not None:
+        if residual.shape[0] != m:
+            raise ClefError(-1, "residual shape/dtype mismatch")
+        residual_pitch = _linear_rows(residual, n, device)
+        residual = residual.data_ptr()
+    code = _activation_code(activation)
+    out, out_pitch = _linear_out(x, m, n, out, dtype, device)
+    _n.launch(_n.clef_linear, x.data_ptr(), m, k, x_pitch, weight.data_ptr(), n, w_pitch, bias, bias_dtype, code,
+              residual, residual_pitch, out.data_ptr(), int(dtype is torch.float32), out_pitch)
+    return out
+
+
+def linear_gate_up(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, activation: str | None = "silu",
+                   gate_bias: torch.Tensor | None = None, up_bias: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """h = act(x @ gate.T + gate_bias) * (x @ up.T + up_bias) on weights that
+    stay bf16, in one product (clef_linear_gate_up): bf16 [rows][gate.shape[0]],
+    rounded once. Operands as in linear; the biases are of one type."""
+    if gate.dim() != 2 or gate.shape != up.shape:
+        raise ClefError(-1, _BAD_LINEAR)
+    n, k = gate.shape
+    device = torch._C._cuda_getDevice()
+    x_pitch, w_pitch = _linear_rows(x, k, device), _linear_rows(gate, k, device)
+    if _linear_rows(up, k, device) != w_pitch:
+        raise ClefError(-1, _BAD_LINEAR)
+    if gate_bias is not None and up_bias is not None and gate_bias.dtype != up_bias.dtype:
+        raise ClefError(-1, _BAD_LINEAR)
+    gate_bias, bias_dtype = _linear_bias(gate_bias, n, device)
+    up_bias, up_dtype = _linear_bias(up_bias, n, device)
+    code = _activation_code(activation)
+    m = x.shape[0]
+    out, out_pitch = _linear_out(x, m, n, out, torch.bfloat16, device)
+    _n.launch(_n.clef_linear_gate_up, x.data_ptr(), m, k, x_pitch, gate.data_ptr(), up.data_ptr(), n, w_pitch,
+              gate_bias, up_bias, bias_dtype | up_dtype, code, out.data_ptr(), out_pitch)
+    return out

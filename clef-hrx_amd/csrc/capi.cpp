@@ -14,6 +14,8 @@
 #include "build_id.inc"  // CLEF_BUILD_ID, generated by the Makefile
 #include "f8.hpp"
 #include "kernels.hpp"
+#include "linear.hpp"
+#include "moe_few_f8.hpp"
 
 namespace {
 
@@ -1051,6 +1053,147 @@ int clef_moe_expert_gate_up_f8(const uint8_t* a, int64_t a_rows, const uint8_t* 
   x.n = n, x.kb = clef::f8_blocks(k), x.k = k;
   x.pow2 = pow2 != 0, x.out = h, x.lists = {offsets, slots, experts, (int)total, input_routed ? 1 : topk};
   return hip_status(clef::launch_f8_experts(x, true, hs(stream)));
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- products with bf16 activations
+
+namespace {
+
+constexpr const char* kLinearShape = "linear shape/dtype mismatch";
+constexpr const char* kLinearAlign = "linear operand is NULL or not aligned";
+constexpr const char* kLinearOverlap = "linear output overlaps an operand";
+constexpr int64_t kMostStride = ((int64_t)1 << 31) - 1;
+
+// `rows` pieces of `width` bytes, `step` apart.
+struct Pieces {
+  const void* at;
+  int64_t rows, step, width;
+  size_t extent() const { return (size_t)((rows - 1) * step + width); }
+};
+
+// Whether pieces of a and b can share a byte. Pieces of one step interleave: those
+// of b lie a fixed distance behind a's.
+bool overlap(const Pieces& a, const Pieces& b) {
+  if (!overlap(a.at, a.extent(), b.at, b.extent())) return false;
+  if (a.step != b.step || a.step == 0) return true;
+  int64_t behind = (int64_t)(reinterpret_cast<uintptr_t>(b.at) - reinterpret_cast<uintptr_t>(a.at)) % a.step;
+  if (behind < 0) behind += a.step;
+  return behind < a.width || behind + b.width > a.step;
+}
+
+int check_linear(const clef::LinearArgs& p, bool gate_up, int32_t bias_dtype, int32_t out_dtype) {
+  constexpr int64_t most = 1048576;
+  auto dtype = [](int32_t d) { return d == 0 || d == 1; };
+  auto stride = [](int64_t s, int64_t width) { return s >= width && s <= kMostStride; };
+  if (!(p.m >= 0 && p.m <= most && p.n >= 1 && p.n <= most && p.k >= 1 && p.k <= most && stride(p.x_stride, p.k) &&
+        stride(p.w_stride, p.k) && stride(p.out_stride, p.n) && (!p.residual || stride(p.residual_stride, p.n)) &&
+        dtype(bias_dtype) && dtype(out_dtype) && p.act >= 0 && p.act < clef::kActs))
+    return fail(kLinearShape);
+  if (p.m == 0) return CLEF_OK;
+  const size_t bias_bytes = bias_dtype ? 4 : 2, out_bytes = out_dtype ? 4 : 2;
+  auto optional = [](const void* q, size_t a) { return !q || aligned(q, a); };
+  if (!aligned(p.x, 2) || !aligned(p.w, 2) || (gate_up && !aligned(p.w2, 2)) || !aligned(p.out, out_bytes) ||
+      !optional(p.bias, bias_bytes) || !optional(p.bias2, bias_bytes) || !optional(p.residual, 2))
+    return fail(kLinearAlign);
+  const Pieces out{p.out, p.m, p.out_stride * (int64_t)out_bytes, p.n * (int64_t)out_bytes};
+  auto over = [&](const void* at, int64_t rows, int64_t step, int64_t width) {
+    return at != nullptr && overlap(out, Pieces{at, rows, step, width});
+  };
+  const bool onto = p.residual == p.out && p.residual_stride == p.out_stride && out_dtype == 0;
+  if (over(p.x, p.m, p.x_stride * 2, p.k * 2ll) || over(p.w, p.n, p.w_stride * 2, p.k * 2ll) ||
+      over(p.w2, p.n, p.w_stride * 2, p.k * 2ll) || over(p.bias, 1, 0, p.n * (int64_t)bias_bytes) ||
+      over(p.bias2, 1, 0, p.n * (int64_t)bias_bytes) ||
+      (!onto && over(p.residual, p.m, p.residual_stride * 2, p.n * 2ll)))
+    return fail(kLinearOverlap);
+  return CLEF_OK;
+}
+
+// Rows of one element size that all start on multiples of `to` bytes.
+bool rows_aligned(const void* p, int64_t stride, int64_t bytes, int64_t to) {
+  return reinterpret_cast<uintptr_t>(p) % to == 0 && stride * bytes % to == 0;
+}
+
+int linear(clef::LinearArgs& p, bool gate_up, int32_t bias_dtype, int32_t out_dtype, clef_stream_t stream) {
+  if (int rc = check_linear(p, gate_up, bias_dtype, out_dtype)) return rc;
+  if (p.m == 0) return CLEF_OK;
+  p.bias_f32 = bias_dtype != 0, p.out_f32 = out_dtype != 0;
+  p.wide = rows_aligned(p.out, p.out_stride, p.out_f32 ? 4 : 2, 16) &&
+           (!p.residual || rows_aligned(p.residual, p.residual_stride, 2, 16)) && rows_aligned(p.bias, 0, 1, 16) &&
+           rows_aligned(p.bias2, 0, 1, 16);
+  return hip_status(clef::launch_linear(p, gate_up, hs(stream)));
+}
+
+constexpr const char* kFewShape = "unsupported MoE shape for few tokens";
+
+bool few_shape(int64_t tokens, int32_t hidden, int32_t inter, int32_t experts, int32_t topk) {
+  return tokens >= 0 && tokens <= clef::kMoeFewTokens && f8_width(hidden) && f8_width(inter) && topk >= 1 &&
+         topk <= experts && experts <= clef::kMoeFewExperts;
+}
+
+}  // namespace
+
+extern "C" {
+
+int clef_linear(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint16_t* w, int32_t n,
+                int64_t w_stride, const void* bias, int32_t bias_dtype, int32_t activation, const uint16_t* residual,
+                int64_t residual_stride, void* out, int32_t out_dtype, int64_t out_stride, clef_stream_t stream) {
+  clef::LinearArgs p{};
+  p.x = x, p.m = m, p.x_stride = x_stride, p.n = n, p.k = k, p.w = w, p.w_stride = w_stride, p.bias = bias;
+  p.act = activation, p.residual = residual, p.residual_stride = residual_stride, p.out = out, p.out_stride = out_stride;
+  return linear(p, false, bias_dtype, out_dtype, stream);
+}
+
+int clef_linear_gate_up(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint16_t* gate,
+                        const uint16_t* up, int32_t n, int64_t w_stride, const void* gate_bias, const void* up_bias,
+                        int32_t bias_dtype, int32_t activation, uint16_t* h, int64_t h_stride, clef_stream_t stream) {
+  clef::LinearArgs p{};
+  p.x = x, p.m = m, p.x_stride = x_stride, p.n = n, p.k = k, p.w = gate, p.w2 = up, p.w_stride = w_stride;
+  p.bias = gate_bias, p.bias2 = up_bias, p.act = activation, p.out = h, p.out_stride = h_stride;
+  return linear(p, true, bias_dtype, 0, stream);
+}
+
+size_t clef_moe_layer_f8_workspace_bytes(int64_t tokens, int32_t hidden, int32_t inter, int32_t experts,
+                                         int32_t topk) {
+  if (tokens < 1 || !few_shape(tokens, hidden, inter, experts, topk)) return 0;
+  return clef::moe_few_workspace_bytes((int)tokens, topk, inter);
+}
+
+int clef_moe_layer_f8(const uint16_t* x, int64_t x_stride, const void* logits, int32_t logits_dtype, int64_t tokens,
+                      int32_t hidden, int32_t inter, int32_t experts, int32_t topk, const uint8_t* gate,
+                      const float* gate_scales, const uint8_t* up, const float* up_scales, const uint8_t* down,
+                      const float* down_scales, const uint16_t* residual, uint16_t* out, void* workspace,
+                      size_t workspace_bytes, clef_stream_t stream) {
+  if (!(few_shape(tokens, hidden, inter, experts, topk) && x_stride >= hidden && x_stride % 8 == 0 &&
+        x_stride <= (1 << 24) && (logits_dtype == 0 || logits_dtype == 1)))
+    return fail(kFewShape);
+  if (tokens == 0) return CLEF_OK;
+  for (const void* p : {(const void*)x, logits, (const void*)gate, (const void*)gate_scales, (const void*)up,
+                        (const void*)up_scales, (const void*)down, (const void*)down_scales, (const void*)out,
+                        (const void*)workspace})
+    if (!aligned(p, 16)) return fail(kAlign);
+  if (residual && !aligned(residual, 16)) return fail(kAlign);
+  const size_t need = clef::moe_few_workspace_bytes((int)tokens, topk, inter);
+  if (workspace_bytes < need) return fail(kWorkspace);
+  const size_t logits_bytes = (size_t)tokens * experts * (logits_dtype ? 4 : 2), rows_bytes = (size_t)tokens * hidden * 2;
+  const Pieces rows{x, tokens, x_stride * 2, hidden * 2ll}, result{out, tokens, hidden * 2ll, hidden * 2ll};
+  const size_t weight = (size_t)clef::f8_weight_bytes(experts, inter, hidden);
+  if (overlap(workspace, need, x, rows.extent()) || overlap(workspace, need, logits, logits_bytes) ||
+      overlap(workspace, need, out, rows_bytes) || (residual && overlap(workspace, need, residual, rows_bytes)) ||
+      overlap(workspace, need, gate, weight) || overlap(workspace, need, up, weight) ||
+      overlap(workspace, need, down, weight))
+    return fail("MoE workspace overlaps an operand");
+  if ((x != out && overlap(result, rows)) || (residual && residual != out && overlap(residual, rows_bytes, out, rows_bytes)) ||
+      overlap(logits, logits_bytes, out, rows_bytes))
+    return fail("MoE output overlaps an operand");
+  clef::MoeFewArgs a{};
+  a.x = x, a.x_stride = x_stride, a.logits = logits, a.logits_f32 = logits_dtype != 0;
+  a.tokens = (int)tokens, a.hidden = hidden, a.inter = inter, a.experts = experts, a.topk = topk;
+  a.gate = gate, a.up = up, a.down = down;
+  a.gate_scales = gate_scales, a.up_scales = up_scales, a.down_scales = down_scales;
+  a.residual = residual, a.out = out;
+  return hip_status(clef::launch_moe_few(a, workspace, hs(stream)));
 }
 
 }  // extern "C"

@@ -1,0 +1,117 @@
+// Products of bf16 rows and bf16 weights with an epilogue: arguments and the
+// device helpers that the kernels share.
+//   y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n]
+//   h[m][n] = act(gate sum + gate bias) * (up sum + up bias)      (gate/up)
+// Everything is f32 up to the one rounding of the output (none for f32).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "common.hpp"
+#include "gemm_dma.hpp"
+#include "launch.hpp"
+
+namespace clef {
+
+enum LinearAct { kActNone, kActRelu, kActGelu, kActGeluTanh, kActSilu, kActSigmoid, kActs };
+
+struct LinearArgs {
+  const uint16_t* x;  // [m][k], rows x_stride elements apart
+  int64_t m, x_stride;
+  int n, k;
+  const uint16_t* w;   // [n][k], rows w_stride apart
+  const uint16_t* w2;  // gate/up: the up weight
+  int64_t w_stride;
+  const void* bias;  // bf16 or f32 [n], or NULL
+  const void* bias2;
+  bool bias_f32;
+  int act;
+  const uint16_t* residual;  // bf16, rows residual_stride apart, or NULL
+  int64_t residual_stride;
+  void* out;  // bf16 or f32, rows out_stride apart
+  int64_t out_stride;
+  bool out_f32;
+  bool wide;  // residual and output rows start on multiples of 16 bytes (bias of 8)
+};
+
+hipError_t launch_linear(const LinearArgs& p, bool gate_up, hipStream_t stream);
+
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// D = W A^T of a 16 x 16 tile over 32 k, added to c. Lane l holds weight row
+// l % 16 in w and activation row l % 16 in a, eight values of k-group l / 16 (any
+// order of k that both share); D's lane l holds activation row l % 16 and weight
+// rows 4 (l / 16) .. + 3.
+__device__ __forceinline__ v4f mfma_bf16(u4 w, u4 a, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, a), c, 0, 0,
+                                                 0);
+}
+
+// 1 / (1 + exp(-v)): the hardware's exp2 and reciprocal, each within 1 ulp; the
+// limits are the function's (exp2 of -inf is 0, 1 / inf is 0).
+__device__ __forceinline__ float sigmoid_f32(float v) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896341f));
+}
+
+// v Phi(v), Phi the normal distribution function: Phi(-a) = exp(-a^2 / 2) t P(t)
+// for a >= 0 with t = 1 / (1 + 0.3 a), P of degree 7 fitted to erfcx(a / sqrt 2) /
+// 2 (1.5e-7 of the value for a in 0 .. 14). The tail keeps its relative accuracy
+// (the square's rounding: 2e-6 at a = 5), which 1 + erf(v) would lose.
+__device__ __forceinline__ float gelu_f32(float v) {
+  const float a = __builtin_fabsf(v), t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.3f, 1.0f));
+  float p = 0.0356752909719944f;
+  p = __builtin_fmaf(p, t, -0.15720513463020325f);
+  p = __builtin_fmaf(p, t, 0.20635683834552765f);
+  p = __builtin_fmaf(p, t, -0.05368649214506149f);
+  p = __builtin_fmaf(p, t, 0.1285630166530609f);
+  p = __builtin_fmaf(p, t, 0.0999131053686142f);
+  p = __builtin_fmaf(p, t, 0.12075401097536087f);
+  p = __builtin_fmaf(p, t, 0.11962929368019104f);
+  const float q = p * t * __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f);
+  return v * (v < 0.0f ? q : 1.0f - q);
+}
+
+// One value; `act` is uniform. NaN stays NaN (relu too).
+__device__ __forceinline__ float linear_act(float v, int act) {
+  switch (act) {
+    case kActRelu: return v < 0.0f ? 0.0f : v;
+    case kActGelu: return gelu_f32(v);
+    // 0.5 v (1 + tanh(z)) = v sigmoid(2 z), z = sqrt(2 / pi) (v + 0.044715 v^3)
+    case kActGeluTanh: return v * sigmoid_f32(v * __builtin_fmaf(v * v, 0.0713548162726f, 1.59576912160573f));
+    case kActSilu: return v * sigmoid_f32(v);
+    case kActSigmoid: return sigmoid_f32(v);
+    default: return v;
+  }
+}
+
+__device__ __forceinline__ float linear_bias(const void* bias, bool f32, int col) {
+  return f32 ? static_cast<const float*>(bias)[col] : bf16_to_f32(static_cast<const uint16_t*>(bias)[col]);
+}
+
+// The epilogue of columns col .. + 3 of one row: sums y (gate/up: y the gate's, y2
+// the up's). Any alignment, any number of columns left.
+template <bool GU>
+__device__ __forceinline__ void linear_store4(const LinearArgs& p, int64_t row, int col, v4f y, v4f y2) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if (col + t >= p.n) return;
+    float v = y[t];
+    if (p.bias) v += linear_bias(p.bias, p.bias_f32, col + t);
+    v = linear_act(v, p.act);
+    if constexpr (GU) v *= y2[t] + (p.bias2 ? linear_bias(p.bias2, p.bias_f32, col + t) : 0.0f);
+    if (p.residual) v += bf16_to_f32(p.residual[row * p.residual_stride + col + t]);
+    const int64_t at = row * p.out_stride + col + t;
+    if (p.out_f32)
+      static_cast<float*>(p.out)[at] = v;
+    else
+      static_cast<uint16_t*>(p.out)[at] = (uint16_t)f32_to_bf16(v);
+  }
+}
+
+}  // namespace
+
+}  // namespace clef

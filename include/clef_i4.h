@@ -594,6 +594,69 @@ int clef_moe_expert_gate_up_f8(const uint8_t* a, int64_t a_rows, const uint8_t* 
                                int32_t topk, int32_t input_routed, int32_t k, int32_t n, int32_t pow2, uint16_t* h,
                                clef_stream_t stream);
 
+/* ------------------------------------------------ products with bf16 activations */
+
+/* What CLEF_ACT_* an epilogue applies: GELU by the normal distribution's
+ * function, by its tanh form, SiLU, the logistic function. */
+#define CLEF_ACT_NONE 0
+#define CLEF_ACT_RELU 1
+#define CLEF_ACT_GELU 2
+#define CLEF_ACT_GELU_TANH 3
+#define CLEF_ACT_SILU 4
+#define CLEF_ACT_SIGMOID 5
+
+/* Projection on bf16 weights, Engine::linear (src/ops.rs:95-175) with an
+ * epilogue (the reference's has none):
+ *   out[m][n] = act(sum_k x[m][k] * w[n][k] + bias[n]) + residual[m][n]
+ * in f32 (bf16 MFMA), rounded once for a bf16 output. x, w, residual and out
+ * are rows of contiguous elements, x_stride, w_stride, residual_stride and
+ * out_stride elements apart; bias (nullable) has n contiguous values,
+ * residual (bf16, nullable) m rows of n. Dtypes: 0 bf16, 1 f32. Preconditions
+ * -> "linear shape/dtype mismatch": 0 <= m <= 1048576, 1 <= n, k <= 1048576,
+ * every stride at least its row and at most 2^31 - 1, dtypes and activation as
+ * above. Any k, n and stride; rows that start on multiples of 16 bytes with k
+ * % 8 == 0 run the fast kernels. Pointers need their element's alignment ->
+ * "linear operand is NULL or not aligned". The output may be the residual
+ * itself (the same rows, bf16); over a part of it, x, w or the bias -> "linear
+ * output overlaps an operand" (columns beside an operand's in rows of one
+ * stride do not overlap). With no rows a call does nothing. */
+int clef_linear(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint16_t* w, int32_t n,
+                int64_t w_stride, const void* bias, int32_t bias_dtype, int32_t activation,
+                const uint16_t* residual, int64_t residual_stride, void* out, int32_t out_dtype,
+                int64_t out_stride, clef_stream_t stream);
+
+/* h[m][n] = act(x gate^T + gate_bias) * (x up^T + up_bias) in f32, bf16 once
+ * (SiLU: SwiGLU); gate and up [n][k] share w_stride. As clef_linear otherwise. */
+int clef_linear_gate_up(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint16_t* gate,
+                        const uint16_t* up, int32_t n, int64_t w_stride, const void* gate_bias,
+                        const void* up_bias, int32_t bias_dtype, int32_t activation, uint16_t* h,
+                        int64_t h_stride, clef_stream_t stream);
+
+/* The Omni MoE block (src/omni.rs:760-857) of up to 16 tokens on block-scaled
+ * FP8 experts (the tiled weights of clef_f8_pack_weight, one matrix per
+ * expert: gate and up [inter][hidden], down [hidden][inter]) in two launches:
+ *   out[t] = sum_{e in S} p_e Down_e (silu(Gate_e x_t) * Up_e x_t) + residual[t]
+ * S the topk largest of the token's logits (ties: the lower id), p the softmax
+ * over them. Logits of NaN and -inf take no part, so a token may have fewer
+ * experts or none (its output is the residual, or zero). Unlike the stages
+ * (clef_moe_route .. clef_moe_combine) nothing is rounded on the way: the rows
+ * stay bf16 as they are, probabilities and the sum over experts f32, h keeps 16
+ * bits, the output is rounded once. residual bf16 [tokens][hidden], nullable; it
+ * and x may be the output itself. Preconditions: 0 <= tokens <= 16, 1 <= topk <=
+ * experts <= 128, hidden and inter as the FP8 widths, x_stride >= hidden, x_stride
+ * % 8 == 0, x_stride <= 2^24 -> "unsupported MoE shape for few tokens"; pointers
+ * 16-byte aligned. The workspace (bytes below; 0 for shapes the call rejects)
+ * lies apart from every operand -> "MoE workspace overlaps an operand"; the
+ * output over a part of x, the residual or the logits -> "MoE output overlaps an
+ * operand". */
+size_t clef_moe_layer_f8_workspace_bytes(int64_t tokens, int32_t hidden, int32_t inter, int32_t experts,
+                                         int32_t topk);
+int clef_moe_layer_f8(const uint16_t* x, int64_t x_stride, const void* logits, int32_t logits_dtype, int64_t tokens,
+                      int32_t hidden, int32_t inter, int32_t experts, int32_t topk, const uint8_t* gate,
+                      const float* gate_scales, const uint8_t* up, const float* up_scales, const uint8_t* down,
+                      const float* down_scales, const uint16_t* residual, uint16_t* out, void* workspace,
+                      size_t workspace_bytes, clef_stream_t stream);
+
 /* ------------------------------------------------------- packed cache */
 
 /* Key of a packed-weight cache entry (src/packed_cache.rs:24-33): the weight

@@ -1,0 +1,113 @@
+"""Products with bf16 activations without a GPU: sizes, refusals."""
+import pytest
+
+import clef_i4
+
+FAKE = 1 << 20  # never dereferenced: every call below fails its checks first
+FAR = 1 << 44
+SHAPE = "linear shape/dtype mismatch"
+OVERLAP = "linear output overlaps an operand"
+FEW = "unsupported MoE shape for few tokens"
+
+
+def call(name, *args):
+    rc = getattr(clef_i4.lib(), name)(*args)
+    return rc, clef_i4.lib().clef_last_error().decode()
+
+
+def linear(x=FAKE, m=4, k=128, xs=None, w=FAR, n=64, ws=None, bias=None, bias_dtype=0, act=0, res=None, rs=None, out=2 * FAR,
+           out_dtype=0, os=None):
+    xs, ws, rs, os = (d if v is None else v for v, d in ((xs, k), (ws, k), (rs, n), (os, n)))
+    return call("clef_linear", x, m, k, xs, w, n, ws, bias, bias_dtype, act, res, rs, out, out_dtype, os, None)
+
+
+def gate_up(x=FAKE, m=4, k=128, xs=None, gate=FAR, up=3 * FAR, n=64, ws=None, gb=None, ub=None, bias_dtype=0, act=4,
+            h=2 * FAR, hs=None):
+    xs, ws, hs = (d if v is None else v for v, d in ((xs, k), (ws, k), (hs, n)))
+    return call("clef_linear_gate_up", x, m, k, xs, gate, up, n, ws, gb, ub, bias_dtype, act, h, hs, None)
+
+
+BAD = [dict(m=-1), dict(m=(1 << 20) + 1), dict(k=0), dict(k=(1 << 20) + 1), dict(n=0), dict(n=(1 << 20) + 1), dict(xs=127),
+       dict(ws=127), dict(xs=1 << 31), dict(ws=1 << 31), dict(bias_dtype=2), dict(bias_dtype=-1), dict(act=-1), dict(act=6)]
+
+
+@pytest.mark.parametrize("bad", BAD + [dict(out_dtype=2), dict(os=63), dict(os=1 << 31), dict(res=FAKE, rs=63)])
+def test_linear_rejects(bad):
+    assert linear(**bad) == (-1, SHAPE)
+
+
+@pytest.mark.parametrize("bad", BAD + [dict(hs=63), dict(hs=1 << 31)])
+def test_gate_up_rejects(bad):
+    assert gate_up(**bad) == (-1, SHAPE)
+
+
+def test_no_rows_do_nothing():
+    assert linear(x=None, w=None, out=None, m=0)[0] == 0
+    assert gate_up(x=None, gate=None, up=None, h=None, m=0)[0] == 0
+
+
+@pytest.mark.parametrize("bad", [dict(x=None), dict(x=FAKE + 1), dict(w=None), dict(w=FAR + 1), dict(out=None),
+                                 dict(out=FAR * 2 + 1), dict(out=FAR * 2 + 2, out_dtype=1), dict(bias=FAR * 3 + 1),
+                                 dict(bias=FAR * 3 + 2, bias_dtype=1), dict(res=FAR * 3 + 1)])
+def test_linear_pointers(bad):
+    rc, msg = linear(**bad)
+    assert rc == -1 and "aligned" in msg
+
+
+def test_gate_up_pointers():
+    for bad in (dict(up=None), dict(gate=FAR + 1), dict(h=FAKE + 1), dict(gb=FAKE * 9 + 1), dict(ub=FAKE * 9 + 2, bias_dtype=1)):
+        rc, msg = gate_up(**bad)
+        assert rc == -1 and "aligned" in msg
+
+
+def test_outputs_over_operands_are_refused():
+    # x: 4 rows of 128 at FAKE; the output 4 rows of 64
+    assert linear(out=FAKE) == (-1, OVERLAP)
+    assert linear(out=FAKE + 4 * 256 - 2) == (-1, OVERLAP)
+    assert linear(out=FAR) == (-1, OVERLAP)
+    assert linear(bias=2 * FAR + 64) == (-1, OVERLAP)
+    assert linear(res=2 * FAR, out_dtype=1) == (-1, OVERLAP)      # f32 over its bf16 residual
+    assert linear(res=2 * FAR, rs=128) == (-1, OVERLAP)           # the same memory in other rows
+    assert linear(res=2 * FAR + 16) == (-1, OVERLAP)
+    assert linear(xs=192, out=FAKE + 254, os=192) == (-1, OVERLAP)  # columns 127 .. of the same wide rows
+    assert linear(xs=192, out=FAKE - 2, os=192) == (-1, OVERLAP)
+    assert gate_up(h=FAKE) == (-1, OVERLAP)
+    assert gate_up(h=3 * FAR + 64 * 256 - 2) == (-1, OVERLAP)
+    assert gate_up(ub=2 * FAR) == (-1, OVERLAP)
+
+
+def few(x=FAKE, xs=None, logits=FAR, dtype=0, t=4, hidden=256, inter=128, experts=8, topk=2, gate=2 * FAR, gs=3 * FAR,
+        up=4 * FAR, us=5 * FAR, down=6 * FAR, ds=7 * FAR, res=None, out=8 * FAR, ws=9 * FAR, nbytes=1 << 30):
+    xs = hidden if xs is None else xs
+    return call("clef_moe_layer_f8", x, xs, logits, dtype, t, hidden, inter, experts, topk, gate, gs, up, us, down, ds, res,
+                out, ws, nbytes, None)
+
+
+@pytest.mark.parametrize("bad", [dict(t=-1), dict(t=17), dict(hidden=0), dict(hidden=12), dict(hidden=32776), dict(inter=0),
+                                 dict(inter=12), dict(inter=32776), dict(experts=129), dict(experts=1), dict(topk=0),
+                                 dict(topk=9), dict(xs=248), dict(xs=260), dict(xs=(1 << 24) + 8), dict(dtype=2)])
+def test_moe_layer_f8_rejects(bad):
+    assert few(**bad) == (-1, FEW)
+
+
+@pytest.mark.parametrize("name", ["x", "logits", "gate", "gs", "up", "us", "down", "ds", "out", "ws", "res"])
+def test_moe_layer_f8_pointers(name):
+    at = dict(x=FAKE, logits=FAR, gate=2 * FAR, gs=3 * FAR, up=4 * FAR, us=5 * FAR, down=6 * FAR, ds=7 * FAR, res=10 * FAR,
+              out=8 * FAR, ws=9 * FAR)[name]
+    for bad in ([] if name == "res" else [None]) + [at + 8]:
+        rc, msg = few(**{name: bad})
+        assert rc == -1 and "aligned" in msg
+
+
+def test_moe_layer_f8_workspace_and_overlaps():
+    need = clef_i4.lib().clef_moe_layer_f8_workspace_bytes(4, 256, 128, 8, 2)
+    assert need >= 4 * 2 * 128 * 4
+    for bad in ((0, 256, 128, 8, 2), (17, 256, 128, 8, 2), (4, 12, 128, 8, 2), (4, 256, 128, 8, 9), (4, 256, 128, 129, 2)):
+        assert clef_i4.lib().clef_moe_layer_f8_workspace_bytes(*bad) == 0
+    assert few(nbytes=need - 1) == (-1, "workspace too small")
+    assert few(t=0, x=None, logits=None, gate=None, out=None, ws=None, nbytes=0)[0] == 0
+    for name in ("x", "logits", "out", "gate", "up", "down", "res"):
+        assert few(**{name: 9 * FAR + 16}) == (-1, "MoE workspace overlaps an operand"), name
+    assert few(out=FAKE + 16) == (-1, "MoE output overlaps an operand")
+    assert few(out=FAR) == (-1, "MoE output overlaps an operand")
+    assert few(res=8 * FAR + 16) == (-1, "MoE output overlaps an operand")
