@@ -1110,18 +1110,10 @@ int check_linear(const clef::LinearArgs& p, bool gate_up, int32_t bias_dtype, in
   return CLEF_OK;
 }
 
-// Rows of one element size that all start on multiples of `to` bytes.
-bool rows_aligned(const void* p, int64_t stride, int64_t bytes, int64_t to) {
-  return reinterpret_cast<uintptr_t>(p) % to == 0 && stride * bytes % to == 0;
-}
-
 int linear(clef::LinearArgs& p, bool gate_up, int32_t bias_dtype, int32_t out_dtype, clef_stream_t stream) {
   if (int rc = check_linear(p, gate_up, bias_dtype, out_dtype)) return rc;
   if (p.m == 0) return CLEF_OK;
   p.bias_f32 = bias_dtype != 0, p.out_f32 = out_dtype != 0;
-  p.wide = rows_aligned(p.out, p.out_stride, p.out_f32 ? 4 : 2, 16) &&
-           (!p.residual || rows_aligned(p.residual, p.residual_stride, 2, 16)) && rows_aligned(p.bias, 0, 1, 16) &&
-           rows_aligned(p.bias2, 0, 1, 16);
   return hip_status(clef::launch_linear(p, gate_up, hs(stream)));
 }
 

@@ -83,14 +83,427 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinearArgs p) {
     const int64_t row = m0 + 32 * wm + 16 * i + lr;
     if (row >= p.m) continue;
     if constexpr (GU) {
-      linear_store4<true>(p, row, n0 + 16 * wn + 4 * g, acc[i][0], acc[i][1]);
+      linear_epilogue4<true>(p, row, n0 + 16 * wn + 4 * g, acc[i][0], acc[i][1]);
     } else {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
-        linear_store4<false>(p, row, n0 + 32 * wn + 16 * j + 4 * g, acc[i][j], v4f{0, 0, 0, 0});
+        linear_epilogue4<false>(p, row, n0 + 32 * wn + 16 * j + 4 * g, acc[i][j], v4f{0, 0, 0, 0});
     }
   }
 #endif
+}
+
+// Tile of linear_tile_kernel: KG groups of WAVES_M x WAVES_N waves of WM rows x WN
+// weight rows, group g multiplying step g of each KG steps of 64 k; two LDS stages
+// of KG steps each. A row is 128 bytes of a step, its 16-byte chunk c at c ^ ((r >>
+// 1) & 7) (no bank conflicts in reads of 16 rows).
+template <int WM_, int WN_, int WAVES_M_, int WAVES_N_, int GROUPS_ = 1, int KG_ = 1>
+struct LinearTile {
+  static constexpr int GROUPS = GROUPS_;  // workgroups per CU
+  static constexpr int WM = WM_, WN = WN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_;
+  static constexpr int KG = KG_, NWB = WAVES_M * WAVES_N, NW = NWB * KG, THREADS = 64 * NW;
+  static constexpr int BM = WM * WAVES_M, BN = WN * WAVES_N;
+  static constexpr int TM = WM / 16, TN = WN / 16;  // fragments per wave
+  static constexpr int A_BLOCK = BM * 128, B_BLOCK = BN * 128;
+  static constexpr int A_BYTES = KG * A_BLOCK, B_BYTES = KG * B_BLOCK, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int A_SLOTS = A_BYTES / 1024 / NW, B_SLOTS = B_BYTES / 1024 / NW;
+  // a wave's DMA instructions per stage: first (X) the weight rows and the rows of
+  // its first TM / 2 activation fragments, then (Y) the other rows
+  static constexpr int Y = A_SLOTS / 2, X = B_SLOTS + A_SLOTS - Y, DMA = X + Y;
+  static constexpr int LDS = 2 * STAGE_BYTES;
+  static constexpr int EPI = 16 * WN * 2;  // epilogue staging per wave
+  static_assert(NW == 8 && LDS <= 160 * 1024, "eight waves");
+  static_assert(A_BYTES % (2048 * NW) == 0 && B_BYTES % (2048 * NW) == 0, "whole instructions per wave");
+  static_assert(TM % 2 == 0 && TN % 2 == 0 && TM % KG == 0 && KG <= 2, "step");
+  static_assert(NW * (TM - TM / KG) * TN * 1024 <= LDS && NW * EPI <= LDS, "the groups' sums and rows meet in the stages");
+  static_assert(X <= TM * TN && Y <= 2 * TN, "one DMA instruction per MFMA behind each barrier");
+};
+
+// Many rows: tiles of BM rows x BN weight rows through two LDS stages filled by
+// DMA, as the FP8 products' (gemm_f8.hip): a stage is filled in two parts, X and Y.
+// Behind a barrier in the middle of a step X has been read by every wave and is
+// loaded for two steps on, behind one before the step's last row of MFMAs the same
+// goes for Y; each barrier also waits for the part that the MFMAs behind it read.
+// So every load has a step and a half to land.
+template <class T, bool GU, bool RESID>
+__global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(const LinearArgs p, int tiles_m,
+                                                                                int tiles_n) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  extern __shared__ __align__(16) char lds[];
+  constexpr int TM = T::TM, TN = T::TN, COLS = GU ? T::BN / 2 : T::BN;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, g = lane >> 4;
+  const int kg = T::KG == 1 ? 0 : wave / T::NWB, wb = wave % T::NWB;  // group, wave in it
+  const int wm = wb / T::WAVES_N, wn = wb % T::WAVES_N;
+  int tm, tn;
+  tile_of_block(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
+  const int64_t m0 = (int64_t)tm * T::BM;
+  const int n0 = tn * COLS;
+  const int here = p.m - m0 < T::BM ? (int)(p.m - m0) : T::BM, cols = p.n - n0 < COLS ? p.n - n0 : COLS;
+  const int blocks = (p.k + 63) / 64, steps = (blocks + T::KG - 1) / T::KG;
+
+  // This wave's DMA: an instruction moves 8 rows of a step, the first half of a
+  // wave's A instructions rows of the first TM / 2 fragments of either row of
+  // waves. Rows past the end repeat the last.
+  auto a_piece = [&](int s) {  // 8 rows of the block
+    constexpr int H = T::A_SLOTS / 2;
+    constexpr int PER = T::WM / 16;
+    const int hi = s >= H, q = wb * H + s % H;
+    return q / PER * (2 * PER) + hi * PER + q % PER;
+  };
+  auto chunk_of = [&](int r) { return (lane & 7) ^ ((r >> 1) & 7); };
+  int a_voff[T::A_SLOTS], b_voff[T::B_SLOTS];
+#pragma unroll
+  for (int s = 0; s < T::A_SLOTS; ++s) {
+    const int r = 8 * a_piece(s) + (lane >> 3), from = r < here ? r : here - 1;
+    a_voff[s] = (int)(from * p.x_stride) * 2 + (chunk_of(r) << 4);
+  }
+#pragma unroll
+  for (int s = 0; s < T::B_SLOTS; ++s) {
+    const int r = 8 * (wb * T::B_SLOTS + s) + (lane >> 3);
+    const int col = GU ? r % COLS : r, from = col < cols ? col : cols - 1;
+    b_voff[s] = (int)(from * p.w_stride) * 2 + (chunk_of(r) << 4);
+  }
+  // gate/up: the first half of a group's waves load the gate's rows
+  const bool up = GU && wb >= T::NWB / 2;
+  const __amdgpu_buffer_rsrc_t a_rsrc =
+      make_rsrc(p.x + m0 * p.x_stride, (uint32_t)(((here - 1) * p.x_stride + p.k) * 2));
+  const __amdgpu_buffer_rsrc_t b_rsrc =
+      make_rsrc((up ? p.w2 : p.w) + n0 * p.w_stride, (uint32_t)(((cols - 1) * p.w_stride + p.k) * 2));
+  const __amdgpu_buffer_rsrc_t none = make_rsrc(p.x, 0);
+  // Where k ends inside a step, this lane's chunk of it: past the end (an offset that
+  // reads zeros) or not. A lane has two chunks, of odd and even pieces.
+  int past[2];
+#pragma unroll
+  for (int o = 0; o < 2; ++o)
+    past[o] = p.k % 64 != 0 && 8 * ((lane & 7) ^ (4 * o + (lane >> 4))) >= p.k % 64 ? (int)0x80000000u : 0;
+  // DMA instruction x of step kt into `stage`, X first (steps past the end: zeros
+  // that nothing counts, so that every step issues and waits alike)
+  auto issue = [&](char* stage, int kt, int x) {
+    const int block = T::KG * kt + kg;
+    const bool in = block < blocks, last = block == blocks - 1;
+    const int k = in ? block * 128 : 0;
+    if (x < T::B_SLOTS) {
+      const int piece = wb * T::B_SLOTS + x;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? b_rsrc : none,
+                                               (lds_ptr_t)(stage + T::A_BYTES + kg * T::B_BLOCK + piece * 1024), 16,
+                                               b_voff[x] | (last ? past[piece & 1] : 0), k, 0, 0);
+    } else {
+      const int piece = a_piece(x - T::B_SLOTS);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? a_rsrc : none, (lds_ptr_t)(stage + kg * T::A_BLOCK + piece * 1024),
+                                               16, a_voff[x - T::B_SLOTS] | (last ? past[piece & 1] : 0), k, 0, 0);
+    }
+  };
+
+  // a fragment's two halves (32 k each) in a stage
+  const int swz = (g ^ (lr >> 1)) << 4;
+  const int a_at = kg * T::A_BLOCK + (wm * T::WM + lr) * 128;
+  const int b_at = T::A_BYTES + kg * T::B_BLOCK + ((GU ? wn * (T::WN / 2) : wn * T::WN) + lr) * 128;
+
+  v4f acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
+  auto body = [&](char* __restrict__ r0, char* __restrict__ r1) {
+    u4 av[2][2], bv[TN][2];
+    auto read_a = [&](const char* stage, int i, u4 (&v)[2]) {
+      v[0] = *reinterpret_cast<const u4*>(stage + a_at + i * 2048 + swz);
+      v[1] = *reinterpret_cast<const u4*>(stage + a_at + i * 2048 + (swz ^ 64));
+    };
+    auto read_b = [&](const char* stage, int j, u4 (&v)[2]) {
+      const char* at = stage + b_at + (GU && j >= TN / 2 ? T::B_BLOCK / 2 + (j - TN / 2) * 2048 : j * 2048);
+      v[0] = *reinterpret_cast<const u4*>(at + swz);
+      v[1] = *reinterpret_cast<const u4*>(at + (swz ^ 64));
+    };
+    // at most one stage's DMA behind what is waited for
+    auto landed = [&]() {
+      wait_vmcnt<T::DMA>();
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto step = [&](char* cur, const char* next, int kt) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        if (i == TM / 2 - 1) landed();  // this stage's Y; its X has been read
+        if (i == TM - 1) landed();      // the next stage's X; this stage has been read
+        if (i + 1 < TM)
+          read_a(cur, i + 1, av[(i + 1) & 1]);
+        else
+          read_a(next, 0, av[(i + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            acc[i][j] = mfma_bf16(bv[j][h], av[i & 1][h], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (i == TM - 1) read_b(next, j, bv[j]);
+          // X behind the first barrier, Y behind the second
+          constexpr int SPAN = TM / 2 * TN;
+          const int u = (i - (TM / 2 - 1)) * TN + j;
+          if (u >= 0 && u < SPAN) {
+#pragma unroll
+            for (int x = u * T::X / SPAN; x < (u + 1) * T::X / SPAN; ++x) issue(cur, kt + 2, x);
+          } else if (i == TM - 1) {
+#pragma unroll
+            for (int x = j * T::Y / TN; x < (j + 1) * T::Y / TN; ++x) issue(cur, kt + 2, T::X + x);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    };
+#pragma unroll
+    for (int x = 0; x < T::DMA; ++x) issue(r0, 0, x);
+#pragma unroll
+    for (int x = 0; x < T::DMA; ++x) issue(r1, 1, x);
+    wait_vmcnt<T::DMA>();
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    read_a(r0, 0, av[0]);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) read_b(r0, j, bv[j]);
+    for (int kt = 0; kt < steps; kt += 2) {
+      step(r0, r1, kt);
+      if (kt + 1 < steps) step(r1, r0, kt + 1);
+    }
+  };
+  body(lds, lds + T::STAGE_BYTES);
+
+  // Epilogue. A lane has four columns of row lr of each fragment; bf16 rows pass
+  // through the wave's own LDS, 16 at a time (16-byte chunk c of row r at c ^ (r &
+  // 7)), and are stored in 16-byte pieces of whole row segments.
+  constexpr int EM = TM / T::KG;  // rows of fragments that this wave stores, from fragment kg EM
+  constexpr int NC = GU ? TN / 2 : TN;
+  const int w0 = wm * T::WM + kg * EM * 16, c0 = n0 + wn * (16 * NC);
+  v4f bias[NC], bias2[GU ? NC : 1];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    bias[j] = linear_bias4(p.bias, p.bias_f32, c0 + 16 * j + 4 * g, p.n);
+    if constexpr (GU) bias2[j] = linear_bias4(p.bias2, p.bias_f32, c0 + 16 * j + 4 * g, p.n);
+  }
+  wait_vmcnt<0>();
+  __syncthreads();
+  v4f sum[EM][TN];
+  if constexpr (T::KG == 1) {
+#pragma unroll
+    for (int i = 0; i < EM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) sum[i][j] = acc[i][j];
+  } else {
+    // two groups: each gives the other its part of the rows that the other stores
+    v4f* const mine = reinterpret_cast<v4f*>(lds) + wave * (EM * TN * 64) + lane;
+    const v4f* const theirs = reinterpret_cast<v4f*>(lds) + (wave ^ T::NWB) * (EM * TN * 64) + lane;
+#pragma unroll
+    for (int i = 0; i < EM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sum[i][j][t] = kg ? acc[i][j][t] : acc[EM + i][j][t];
+        mine[(i * TN + j) * 64] = sum[i][j];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sum[i][j][t] = kg ? acc[EM + i][j][t] : acc[i][j][t];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) sum[i][j] += theirs[(i * TN + j) * 64];
+    __syncthreads();
+  }
+  constexpr int ROW = 32 * NC, CH = 2 * NC, PER = 64 / CH;  // bytes and chunks of a row, rows per store
+  char* own = lds + wave * T::EPI;
+#pragma unroll
+  for (int i = 0; i < EM; ++i) {
+    const int r0 = w0 + 16 * i;
+    v4f res[NC];
+    if constexpr (RESID) {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        res[j] = v4f{0, 0, 0, 0};
+        if (r0 + lr < here) res[j] = linear_residual4(p, m0 + r0 + lr, c0 + 16 * j + 4 * g);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      v4f y = linear_finish4<GU>(p, sum[i][j], bias[j], sum[i][GU ? j + NC : j], bias2[GU ? j : 0]);
+      if constexpr (RESID) y += res[j];
+      if (p.out_f32) {
+        if (r0 + lr < here) linear_store4(p, m0 + r0 + lr, c0 + 16 * j + 4 * g, y);
+        continue;
+      }
+      const int chunk = 2 * j + (g >> 1);
+      *reinterpret_cast<uint2*>(own + lr * ROW + ((chunk ^ (lr & (CH - 1))) << 4) + 8 * (g & 1)) =
+          uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+    }
+    if (p.out_f32) continue;
+#pragma unroll
+    for (int q = 0; q < (16 + PER - 1) / PER; ++q) {
+      const int r = q * PER + lane / CH, chunk = lane % CH, col = c0 + 8 * chunk;
+      if (PER > 16 && r >= 16) continue;
+      const uint4 v = *reinterpret_cast<const uint4*>(own + r * ROW + ((chunk ^ (r & (CH - 1))) << 4));
+      if (r0 + r >= here || col >= p.n) continue;
+      uint16_t* to = static_cast<uint16_t*>(p.out) + (m0 + r0 + r) * p.out_stride + col;
+      if (col + 8 <= p.n) {
+        __builtin_memcpy(to, &v, 16);
+      } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int t = 0; t < 7; ++t)
+          if (col + t < p.n) to[t] = (uint16_t)(w[t / 2] >> (16 * (t % 2)));
+      }
+    }
+    asm volatile("" ::: "memory");
+  }
+#endif
+}
+
+using Tile256 = LinearTile<128, 64, 2, 4>;        // 256 x 256
+using Tile128 = LinearTile<64, 32, 2, 4, 2>;      // 128 x 128, two workgroups per CU
+using Tile128K = LinearTile<64, 64, 2, 2, 1, 2>;  // 128 x 128, two steps of k at a time
+
+template <class T, bool GU, bool RESID>
+hipError_t launch_tile(const LinearArgs& p, hipStream_t stream) {
+  static LaunchCache cache;
+  auto* kernel = &linear_tile_kernel<T, GU, RESID>;
+  if (hipError_t e = ensure_dynamic_lds(cache, reinterpret_cast<const void*>(kernel), T::LDS)) return e;
+  constexpr int COLS = GU ? T::BN / 2 : T::BN;
+  const int64_t tiles_m = (p.m + T::BM - 1) / T::BM, tiles_n = (p.n + COLS - 1) / COLS;
+  if (tiles_m * tiles_n > kMaxTiles) return hipErrorInvalidValue;
+  kernel<<<(unsigned)(tiles_m * tiles_n), T::THREADS, T::LDS, stream>>>(p, (int)tiles_m, (int)tiles_n);
+  return hipGetLastError();
+}
+
+// Few rows: a workgroup owns 16 MT rows x 16 NT weight rows (gate/up: NT / 2
+// fragments of gate rows and the same of up), its eight waves split k in steps of 64
+// (wave w: steps w, w + 8, ..), D steps of each on their way. Operands go straight
+// into registers: a weight row is used by this workgroup's rows only. The waves'
+// sums meet in LDS and are added in wave order (the result does not depend on
+// timing).
+//
+// R: weight rows per fragment. A fragment of R = 4 or 8 rows (for as many rows of
+// x) holds 16 / R pieces of k of each, its lanes lr / R of both operands piece lr /
+// R: of the 16 x 16 sums the blocks on the diagonal count, one per piece. So a tile
+// has as few columns as fill the card, and a load takes 16 / R times 64 contiguous
+// bytes of a row.
+template <int R, int MT, int NT, int D, bool GU>
+__global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int NW = 8, Q = 16 / R, NG = GU ? NT / 2 : NT, BM = R * MT, COLS = R * NG;
+  constexpr int SK = 64 * Q;  // k per step
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, g = lane >> 4;
+  const int64_t m0 = (int64_t)blockIdx.y * BM;
+  const int n0 = blockIdx.x * COLS;
+  const int here = p.m - m0 < BM ? (int)(p.m - m0) : BM, cols = p.n - n0 < COLS ? p.n - n0 : COLS;
+  const int steps = (p.k + SK - 1) / SK;
+  const int fr = lr % R, k_lane = 8 * (lr / R * 4 + g);  // row in the fragment, first k of this lane in a step's half
+  const __amdgpu_buffer_rsrc_t a_rsrc =
+      make_rsrc(p.x + m0 * p.x_stride, (uint32_t)(((here - 1) * p.x_stride + p.k) * 2));
+  const uint32_t w_bytes = (uint32_t)(((cols - 1) * p.w_stride + p.k) * 2);
+  const __amdgpu_buffer_rsrc_t w_rsrc = make_rsrc(p.w + n0 * p.w_stride, w_bytes);
+  const __amdgpu_buffer_rsrc_t w2_rsrc = make_rsrc(GU ? p.w2 + n0 * p.w_stride : p.w, GU ? w_bytes : 0);
+  int a_voff[MT], w_voff[NG];  // rows past the end repeat the last
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int r = R * i + fr < here ? R * i + fr : here - 1;
+    a_voff[i] = (int)(r * p.x_stride + k_lane) * 2;
+  }
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    const int r = R * j + fr < cols ? R * j + fr : cols - 1;
+    w_voff[j] = (int)(r * p.w_stride + k_lane) * 2;
+  }
+  struct Step {
+    u4 w[NT][2], a[MT][2];
+  } ring[D];
+  auto load = [&](Step& b, int s) {
+    if (s >= steps) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // chunks past the end of k: an offset that reads zeros
+      const int past = SK * s + SK / 2 * h + k_lane >= p.k ? (int)0x80000000u : 0;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        b.w[j][h] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(
+                                               GU && j >= NG ? w2_rsrc : w_rsrc, (w_voff[j % NG] + SK * h) | past, s * (2 * SK), 0));
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        b.a[i][h] = __builtin_bit_cast(
+            u4, __builtin_amdgcn_raw_buffer_load_b128(a_rsrc, (a_voff[i] + SK * h) | past, s * (2 * SK), 0));
+    }
+  };
+  v4f acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0, 0, 0, 0};
+#pragma unroll
+  for (int d = 0; d < D; ++d) load(ring[d], wave + NW * d);
+  for (int s = wave; s < steps; s += NW * D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (s + NW * d >= steps) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j] = mfma_bf16(ring[d].w[j][h], ring[d].a[i][h], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+      load(ring[d], s + NW * (d + D));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  // the waves' sums: fragment (i, j) of wave w at ((w MT + i) NT + j) KiB
+  v4f* sums = reinterpret_cast<v4f*>(lds);
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) sums[((wave * MT + i) * NT + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  // R rows x R / 4 quads of columns of a fragment
+  constexpr int ITEMS = R * R / 4;
+  for (int u = threadIdx.x; u < MT * NG * ITEMS; u += NW * 64) {
+    const int fr = u % R, quad = u / R % (R / 4), j = u / ITEMS % NG, i = u / (ITEMS * NG);
+    const int r = R * i + fr, col = n0 + R * j + 4 * quad;
+    if (r >= here || col >= p.n) continue;
+    v4f y = {0, 0, 0, 0}, y2 = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int at = (w * MT + i) * NT * 64 + R * q + fr + 16 * (R / 4 * q + quad);
+        y += sums[at + j * 64];
+        if constexpr (GU) y2 += sums[at + (NG + j) * 64];
+      }
+    linear_epilogue4<GU>(p, m0 + r, col, y, y2);
+  }
+#endif
+}
+
+template <int R, int MT, int NT, int D, bool GU>
+hipError_t launch_stream(const LinearArgs& p, hipStream_t stream) {
+  constexpr int COLS = R * NT / (GU ? 2 : 1), lds = 8 * MT * NT * 1024;
+  static LaunchCache cache;
+  auto* kernel = &linear_stream_kernel<R, MT, NT, D, GU>;
+  if (lds > 64 * 1024)
+    if (hipError_t e = ensure_dynamic_lds(cache, reinterpret_cast<const void*>(kernel), lds)) return e;
+  const int64_t tiles_m = (p.m + R * MT - 1) / (R * MT);
+  if (tiles_m > 65535) return hipErrorInvalidValue;
+  kernel<<<dim3((unsigned)((p.n + COLS - 1) / COLS), (unsigned)tiles_m), 512, lds, stream>>>(p);
+  return hipGetLastError();
+}
+
+// Whether both operands' rows start on multiples of 16 bytes, k is whole chunks of
+// those and 256 rows lie within 2 GiB (the fast kernels' loads).
+bool rows_of_16(const LinearArgs& p) {
+  auto at16 = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
+  constexpr int64_t most = (int64_t)1 << 21;
+  return at16(p.x) && at16(p.w) && at16(p.w2) && p.k % 8 == 0 && p.x_stride % 8 == 0 && p.w_stride % 8 == 0 &&
+         p.x_stride <= most && p.w_stride <= most;
 }
 
 template <bool GU>
@@ -101,10 +514,49 @@ hipError_t launch_any(const LinearArgs& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
+
+constexpr int64_t kCus = 256;
+
+enum class LinearKernel { any, s8x8, s8x16, s8x32, s16x16, s16x32, s16x64, s32x64, s64x64, t128x128, t128x128k, t256x256 };
+
+// The kernel for a product of m rows against n weight rows (gate/up: both).
+LinearKernel linear_kernel(int64_t m, int64_t rows_of_w, int k, bool gate_up) {
+  auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((rows_of_w + bn - 1) / bn); };
+  if (m <= 8) return gate_up || (m > 4 && rows_of_w > 8192) ? LinearKernel::s8x16 : LinearKernel::s8x8;
+  if (tiles(16, 16) <= kCus && !gate_up) return LinearKernel::s16x16;
+  if (tiles(16, 32) <= kCus) return LinearKernel::s16x32;
+  if (m <= 16) return tiles(16, 64) > kCus ? LinearKernel::s16x32 : LinearKernel::s16x64;
+  if (tiles(32, 64) <= kCus) return LinearKernel::s32x64;
+  if (tiles(64, 64) <= kCus) return LinearKernel::s64x64;
+  auto rounds = [&](int b) { return (tiles(b, b) + kCus - 1) / kCus; };
+  if (rounds(128) >= 3 * rounds(256)) return LinearKernel::t256x256;
+  return rounds(128) <= 1 ? LinearKernel::t128x128k : LinearKernel::t128x128;
+}
+
+template <bool GU>
+hipError_t launch_rows(const LinearArgs& p, hipStream_t stream) {
+  switch (rows_of_16(p) ? linear_kernel(p.m, (int64_t)p.n * (GU ? 2 : 1), p.k, GU) : LinearKernel::any) {
+    case LinearKernel::s8x8: if constexpr (!GU) return launch_stream<8, 1, 1, 2, GU>(p, stream);
+    case LinearKernel::s8x16: return launch_stream<8, 1, 2, 1, GU>(p, stream);
+    case LinearKernel::s16x16: if constexpr (!GU) return launch_stream<16, 1, 1, 1, GU>(p, stream);
+    case LinearKernel::s16x32: return launch_stream<16, 1, 2, 1, GU>(p, stream);
+    case LinearKernel::s16x64: return launch_stream<16, 1, 4, 1, GU>(p, stream);
+    case LinearKernel::s32x64: return launch_stream<16, 2, 4, 1, GU>(p, stream);
+    case LinearKernel::s64x64: return launch_stream<16, 4, 4, 1, GU>(p, stream);
+    case LinearKernel::t128x128:
+      return p.residual ? launch_tile<Tile128, GU, !GU>(p, stream) : launch_tile<Tile128, GU, false>(p, stream);
+    case LinearKernel::t128x128k:
+      return p.residual ? launch_tile<Tile128K, GU, !GU>(p, stream) : launch_tile<Tile128K, GU, false>(p, stream);
+    case LinearKernel::t256x256:
+      return p.residual ? launch_tile<Tile256, GU, !GU>(p, stream) : launch_tile<Tile256, GU, false>(p, stream);
+    default: return launch_any<GU>(p, stream);
+  }
+}
+
 }  // namespace
 
 hipError_t launch_linear(const LinearArgs& p, bool gate_up, hipStream_t stream) {
-  return gate_up ? launch_any<true>(p, stream) : launch_any<false>(p, stream);
+  return gate_up ? launch_rows<true>(p, stream) : launch_rows<false>(p, stream);
 }
 
 }  // namespace clef

@@ -32,7 +32,6 @@ struct LinearArgs {
   void* out;  // bf16 or f32, rows out_stride apart
   int64_t out_stride;
   bool out_f32;
-  bool wide;  // residual and output rows start on multiples of 16 bytes (bias of 8)
 };
 
 hipError_t launch_linear(const LinearArgs& p, bool gate_up, hipStream_t stream);
@@ -88,28 +87,81 @@ __device__ __forceinline__ float linear_act(float v, int act) {
   }
 }
 
-__device__ __forceinline__ float linear_bias(const void* bias, bool f32, int col) {
-  return f32 ? static_cast<const float*>(bias)[col] : bf16_to_f32(static_cast<const uint16_t*>(bias)[col]);
+// Columns col .. + 3 of a bias, and of a residual row: loads of any alignment
+// (one instruction), columns past the last are zeros.
+__device__ __forceinline__ v4f linear_bias4(const void* bias, bool f32, int col, int n) {
+  v4f v = {0, 0, 0, 0};
+  if (!bias) return v;
+  if (f32) {
+    const float* from = static_cast<const float*>(bias) + col;
+    if (col + 4 <= n) {
+      __builtin_memcpy(&v, from, 16);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (col + t < n) v[t] = from[t];
+    }
+    return v;
+  }
+  const uint16_t* from = static_cast<const uint16_t*>(bias) + col;
+  uint2 w = {0, 0};
+  if (col + 4 <= n) {
+    __builtin_memcpy(&w, from, 8);
+  } else {
+    if (col < n) w.x = from[0];
+    if (col + 1 < n) w.x |= (uint32_t)from[1] << 16;
+    if (col + 2 < n) w.y = from[2];
+  }
+  return v4f{bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)};
 }
 
-// The epilogue of columns col .. + 3 of one row: sums y (gate/up: y the gate's, y2
-// the up's). Any alignment, any number of columns left.
+__device__ __forceinline__ v4f linear_residual4(const LinearArgs& p, int64_t row, int col) {
+  return linear_bias4(p.residual + row * p.residual_stride, false, col, p.n);
+}
+
+// act(y + bias), and the product with the up sums for gate/up.
 template <bool GU>
-__device__ __forceinline__ void linear_store4(const LinearArgs& p, int64_t row, int col, v4f y, v4f y2) {
+__device__ __forceinline__ v4f linear_finish4(const LinearArgs& p, v4f y, v4f bias, v4f y2, v4f bias2) {
+  y += bias;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    if (col + t >= p.n) return;
-    float v = y[t];
-    if (p.bias) v += linear_bias(p.bias, p.bias_f32, col + t);
-    v = linear_act(v, p.act);
-    if constexpr (GU) v *= y2[t] + (p.bias2 ? linear_bias(p.bias2, p.bias_f32, col + t) : 0.0f);
-    if (p.residual) v += bf16_to_f32(p.residual[row * p.residual_stride + col + t]);
-    const int64_t at = row * p.out_stride + col + t;
-    if (p.out_f32)
-      static_cast<float*>(p.out)[at] = v;
-    else
-      static_cast<uint16_t*>(p.out)[at] = (uint16_t)f32_to_bf16(v);
+  for (int t = 0; t < 4; ++t) y[t] = linear_act(y[t], p.act);
+  if constexpr (GU) y *= y2 + bias2;
+  return y;
+}
+
+// Columns col .. + 3 of an output row, any alignment, those past the last left out.
+__device__ __forceinline__ void linear_store4(const LinearArgs& p, int64_t row, int col, v4f y) {
+  const int64_t at = row * p.out_stride + col;
+  if (p.out_f32) {
+    float* to = static_cast<float*>(p.out) + at;
+    if (col + 4 <= p.n) {
+      __builtin_memcpy(to, &y, 16);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (col + t < p.n) to[t] = y[t];
+    }
+    return;
   }
+  uint16_t* to = static_cast<uint16_t*>(p.out) + at;
+  const uint2 v = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+  if (col + 4 <= p.n) {
+    __builtin_memcpy(to, &v, 8);
+  } else {
+    if (col < p.n) to[0] = (uint16_t)v.x;
+    if (col + 1 < p.n) to[1] = (uint16_t)(v.x >> 16);
+    if (col + 2 < p.n) to[2] = (uint16_t)v.y;
+  }
+}
+
+// All of it: sums y (gate/up: y the gate's, y2 the up's) of one row.
+template <bool GU>
+__device__ __forceinline__ void linear_epilogue4(const LinearArgs& p, int64_t row, int col, v4f y, v4f y2) {
+  v4f bias2 = {0, 0, 0, 0};
+  if constexpr (GU) bias2 = linear_bias4(p.bias2, p.bias_f32, col, p.n);
+  y = linear_finish4<GU>(p, y, linear_bias4(p.bias, p.bias_f32, col, p.n), y2, bias2);
+  if (p.residual) y += linear_residual4(p, row, col);
+  linear_store4(p, row, col, y);
 }
 
 }  // namespace
