@@ -31,77 +31,121 @@ struct FewTable {
   int16_t slot[kMaxExperts][kTokens];
 };
 
-// Routing of all tokens by one workgroup of 512 threads, in LDS.
+// Routing of all tokens, in LDS of each workgroup of 512 threads, by expert.
 struct FewRoutes {
-  float v[kTokens][kMaxExperts];         // the logits; -inf: takes no part
-  float p[kTokens][kMaxExperts];         // by rank
-  uint8_t rank[kTokens][kMaxExperts];    // by expert
-  uint32_t tokens[kMaxExperts];          // by expert: the tokens that name it
-  unsigned long long named[2];
+  float p[kTokens][kMaxExperts];       // the probability
+  uint8_t rank[kTokens][kMaxExperts];
+  uint32_t tokens[kMaxExperts];        // the tokens that name it
+  // more than 16 ranks: the chosen logits and their experts by rank
+  float v[kTokens][kMaxExperts];
+  uint8_t id[kTokens][kMaxExperts];
 };
 
-__device__ __forceinline__ float few_logit(const MoeFewArgs& a, int i) {
-  const float v = a.logits_f32 ? static_cast<const float*>(a.logits)[i]
-                               : bf16_to_f32(static_cast<const uint16_t*>(a.logits)[i]);
-  return v != v ? -__builtin_huge_valf() : v;
+// The experts named, one bit each, in scalar registers of every wave.
+struct FewNamed {
+  unsigned long long low, high;
+  __device__ __forceinline__ int count() const { return __popcll(low) + __popcll(high); }
+  // the i-th, i < count()
+  __device__ __forceinline__ int expert(int i) const {
+    const int lows = __popcll(low);
+    unsigned long long mask = i < lows ? low : high;
+    for (int n = i < lows ? i : i - lows; n > 0; --n) mask &= mask - 1;
+    return (i < lows ? 0 : 64) + __builtin_ctzll(mask);
+  }
+};
+
+// (equal ones first: infinities have no difference)
+__device__ __forceinline__ float few_exp(float v, float best) {
+  return v == -__builtin_huge_valf() ? 0.0f : v == best ? 1.0f : __builtin_amdgcn_exp2f((v - best) * 1.44269504088896341f);
 }
 
-// An expert's rank is the number of logits in front of its own (larger, or equal
-// at a lower id). Logits of -inf and NaN take no part, nor does a probability that
-// is zero: a token may name fewer than topk experts, or none.
-__device__ __forceinline__ void few_route(const MoeFewArgs& a, FewRoutes& r) {
-  const int tid = threadIdx.x, experts = a.experts, pairs = a.tokens * experts;
-  for (int i = tid; i < pairs; i += 512) r.v[i / experts][i % experts] = few_logit(a, i);
+__device__ __forceinline__ void few_choose(FewRoutes& r, int t, int k, int id, float p) {
+  if (!(p > 0.0f)) return;
+  r.p[t][id] = p;
+  r.rank[t][id] = (uint8_t)k;
+  atomicOr(&r.tokens[id], 1u << t);
+}
+
+// 16 lanes (a DPP row) take a token, 8 experts each, through topk rounds of "the
+// largest logit left, the lowest id that has it"; lane k keeps rank k. Logits of -inf
+// and NaN take no part, nor does a probability that is zero: a token may name fewer
+// than topk experts, or none.
+__device__ __forceinline__ FewNamed few_route(const MoeFewArgs& a, FewRoutes& r) {
+  const int tid = threadIdx.x, experts = a.experts, topk = a.topk;
+  constexpr float none = -__builtin_huge_valf();
+  const int t = tid >> 4, li = tid & 15, e0 = 8 * li;
+  const bool routes = tid < 64 * ((a.tokens + 3) / 4);  // whole waves
+  const bool wide = topk > 16;
   if (tid < kMaxExperts) r.tokens[tid] = 0;
-  __syncthreads();
-  // by rank, into p: the logits; ranks of those in front
-  for (int i = tid; i < pairs; i += 512) {
-    const int t = i / experts, e = i % experts;
-    const float v = r.v[t][e];
-    int before = 0;
-    for (int o = 0; o < experts; ++o) before += r.v[t][o] > v || (r.v[t][o] == v && o < e);
-    r.rank[t][e] = (uint8_t)before;
-    if (before < a.topk) r.p[t][before] = v;
+  float mine = none;
+  int mine_id = 0;
+  if (routes) {
+    // all loads at once, past the end zeros
+    const int first = t * experts + e0;
+    uint32_t bits[8];
+    if (a.logits_f32) {
+      const __amdgpu_buffer_rsrc_t lr = make_rsrc(a.logits, (uint32_t)(a.tokens * experts * 4));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) bits[j] = __builtin_amdgcn_raw_buffer_load_b32(lr, (first + j) * 4, 0, 0);
+    } else {
+      const __amdgpu_buffer_rsrc_t lr = make_rsrc(a.logits, (uint32_t)(a.tokens * experts * 2));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) bits[j] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(lr, (first + j) * 2, 0, 0) << 16;
+    }
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float l = as_float(bits[j]);
+      v[j] = t < a.tokens && e0 + j < experts && l == l ? l : none;
+    }
+    for (int k = 0; k < topk; ++k) {
+      float m = v[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) m = __builtin_fmaxf(m, v[j]);
+      const float best = route_impl::row_max(m);
+      int of = route_impl::kInvalidId;
+#pragma unroll
+      for (int j = 7; j >= 0; --j)
+        if (v[j] == best) of = e0 + j;
+      const int id = route_impl::row_min(of);  // (past the last finite logit: not used)
+      if (wide && li == 0) {
+        r.v[t][k] = best;
+        r.id[t][k] = (uint8_t)id;
+      }
+      if (li == k) {
+        mine = best;
+        mine_id = id;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (id == e0 + j) v[j] = none;
+    }
   }
   __syncthreads();
-  float mine[4];  // at most 16 x 128 ranks over 512 threads
-  int n = 0;
-  for (int i = tid; i < a.tokens * a.topk; i += 512, ++n) {
-    const int t = i / a.topk, k = i % a.topk;
-    const float best = r.p[t][0];
-    float sum = 0.0f;
-    for (int o = 0; o < a.topk; ++o) sum += r.p[t][o] == best ? 1.0f : cephes_expf(r.p[t][o] - best);
-    const float v = r.p[t][k];
-    mine[n & 3] = v == -__builtin_huge_valf() ? 0.0f : (v == best ? 1.0f : cephes_expf(v - best)) / sum;
+  if (!wide) {
+    if (routes) {
+      // lane 0 holds the largest; the sum over the row (lanes past the last rank: 0)
+      const float e = few_exp(mine, as_float((uint32_t)__builtin_amdgcn_ds_swizzle((int)as_uint(mine), 0x10)));
+      float sum = e;
+      sum += as_float((uint32_t)route_impl::dpp_row<0xB1>((int)as_uint(sum)));
+      sum += as_float((uint32_t)route_impl::dpp_row<0x4E>((int)as_uint(sum)));
+      sum += as_float((uint32_t)route_impl::dpp_row<0x124>((int)as_uint(sum)));
+      sum += as_float((uint32_t)route_impl::dpp_row<0x128>((int)as_uint(sum)));
+      few_choose(r, t, li, mine_id, e / sum);
+    }
+  } else {
+    const int ranks = a.tokens * topk;
+    for (int i = tid; i < ranks; i += 512) {
+      const int of = i / topk, k = i % topk;
+      const float best = r.v[of][0];
+      float sum = 0.0f;
+      for (int o = 0; o < topk; ++o) sum += few_exp(r.v[of][o], best);
+      few_choose(r, of, k, r.id[of][k], few_exp(r.v[of][k], best) / sum);
+    }
   }
   __syncthreads();
-  n = 0;
-  for (int i = tid; i < a.tokens * a.topk; i += 512, ++n) r.p[i / a.topk][i % a.topk] = mine[n & 3];
-  __syncthreads();
-  for (int i = tid; i < pairs; i += 512) {
-    const int t = i / experts, e = i % experts, k = r.rank[t][e];
-    if (k < a.topk && r.p[t][k] > 0.0f) atomicOr(&r.tokens[e], 1u << t);
-  }
-  __syncthreads();
-  if (tid < 128) {
-    const unsigned long long mask = __ballot(r.tokens[tid] != 0);
-    if ((tid & 63) == 0) r.named[tid >> 6] = mask;
-  }
-  __syncthreads();
-}
-
-// The i-th expert named, i < their number.
-__device__ __forceinline__ int few_expert(const FewRoutes& r, int i) {
-  unsigned long long mask = r.named[0];
-  int base = 0;
-  const int low = __popcll(mask);
-  if (i >= low) {
-    i -= low;
-    mask = r.named[1];
-    base = 64;
-  }
-  for (; i > 0; --i) mask &= mask - 1;
-  return base + __builtin_ctzll(mask);
+  const int lane = tid & 63;
+  return {__ballot(r.tokens[lane] != 0), __ballot(r.tokens[64 + lane] != 0)};
 }
 
 // A block's scale as 2^e, which the codes are converted with, and the factor that is
@@ -126,163 +170,351 @@ __device__ __forceinline__ void few_bf16(v4i codes, float pow2, u4 (&out)[2]) {
   }
 }
 
-// One unit is the 16 columns `tile` of h of the i-th expert named: eight waves
-// split the blocks of k, their sums meet in LDS and are added in wave order.
+// Workgroup barrier behind this wave's LDS accesses alone: global loads stay on
+// their way (__syncthreads would wait for them).
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Operands of a fragment of R weight rows. R = 16: a block's half h as it lies
+// (f8.hpp), lane l row l % 16, k = 64 h + 16 (l / 16) ..; R = 8, for up to 8 tokens:
+// both halves in one load, lane l row l % 8 of half l / 8 % 2. The tokens' rows lie
+// the same way, so that of R = 8's sums the two blocks on the diagonal count, one per
+// half. Twice as many tiles cover the output that way.
+template <int R>
+struct FewLane {
+  static constexpr int HALVES = R == 16 ? 2 : 1;  // loads per fragment and block
+  int row, k;                                     // row of the fragment (and of x), first k in a block
+  __device__ __forceinline__ FewLane() {
+    const int lane = threadIdx.x & 63, lr = lane & 15;
+    row = lr % R;
+    k = 64 * (lr / R) + 16 * (lane >> 4);
+  }
+  // bytes into a block of this lane's 16 codes: rows from `first` (a multiple of R)
+  __device__ __forceinline__ int at(int first) const {
+    return (first >> 4) * 2048 + (first & 15) * 16 + (k >> 6) * 1024 + (k >> 4 & 3) * 256 + row * 16;
+  }
+};
+
+// Route, gate/up and SwiGLU. One unit is 16 columns of h of one expert named; its
+// eight waves split the blocks of k, wave w the blocks w, w + 8, .., whose part of x
+// stays in registers (NB blocks; 0: any number, loaded each time). The next unit's
+// weights are on their way while a unit's sums meet in LDS, where one wave in turn
+// adds them in wave order.
+template <int NB>
 __global__ __launch_bounds__(512) void few_gate_up_kernel(const MoeFewArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ FewRoutes routes;
-  __shared__ v4f sums[8][2][64];
-  few_route(a, routes);
+  __shared__ v4f sums[2][8][2][64];
+  constexpr int R = 16, H = FewLane<R>::HALVES, XB = NB ? NB : 1;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lr = lane & 15, g = lane >> 4;
-  const int count = __popcll(routes.named[0]) + __popcll(routes.named[1]);
+  const FewLane<R> me;
+  const int kb = f8_blocks(a.hidden), tiles = (a.inter + R - 1) / R, panels = f8_blocks(a.inter);
+  const int token = me.row < a.tokens ? me.row : a.tokens - 1;
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(a.x, (uint32_t)(((a.tokens - 1) * a.x_stride + a.hidden) * 2));
+  u4 xv[XB][2 * H];
+  auto load_x = [&](int b, u4 (&v)[2 * H]) {
+#pragma unroll
+    for (int s = 0; s < 2 * H; ++s) {
+      const int k = 128 * b + me.k + 64 * (s / 2) + 8 * (s % 2);
+      v[s] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(
+                                        xr, k < a.hidden ? (int)(token * a.x_stride + k) * 2 : (int)0x80000000u, 0, 0));
+    }
+  };
+  if constexpr (NB > 0) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) load_x(wave + 8 * i, xv[i]);
+  }
+  const FewNamed named = few_route(a, routes);
+  const int count = named.count(), units = count * tiles;
   FewTable& table = *static_cast<FewTable*>(a.table);
   if (blockIdx.x == 0) {
     if (tid == 0) table.count = count;
     for (int i = tid; i < count * kTokens; i += 512) {
-      const int t = i % kTokens, e = few_expert(routes, i / kTokens);
+      const int t = i % kTokens, e = named.expert(i / kTokens);
       if (t == 0) table.expert[i / kTokens] = e;
       table.slot[i / kTokens][t] = routes.tokens[e] >> t & 1 ? (int16_t)(t * a.topk + routes.rank[t][e]) : (int16_t)-1;
     }
+    for (int i = tid; i < a.down_tiles; i += 512) a.arrived[i] = 0;
   }
-  const int kb = f8_blocks(a.hidden), tiles = (a.inter + 15) / 16, panels = f8_blocks(a.inter);
-  const int row = lr < a.tokens ? lr : a.tokens - 1;
-  const __amdgpu_buffer_rsrc_t xr = make_rsrc(a.x, (uint32_t)(((a.tokens - 1) * a.x_stride + a.hidden) * 2));
-  for (int u = blockIdx.x; u < count * tiles; u += gridDim.x) {
-    const int e = __builtin_amdgcn_readfirstlane(few_expert(routes, u / tiles)), n0 = u % tiles * 16;
-    const int64_t panel = ((int64_t)e * panels + n0 / 128) * kb;
-    v4f acc[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
-    for (int b = wave; b < kb; b += 8) {
-      u4 xv[4];
+  struct Unit {
+    int e, n0;
+    v4i w[XB][2][H];
+    float scale[XB][2];
+  };
+  auto load_block = [&](Unit& q, int i, int b) {
+    const int64_t block = ((int64_t)q.e * panels + q.n0 / 128) * kb + b;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int k = 128 * b + 64 * (s / 2) + 16 * g + 8 * (s % 2);
-        xv[s] = k < a.hidden ? __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(
-                                   xr, (int)(row * a.x_stride + k) * 2, 0, 0))
-                             : u4{0, 0, 0, 0};
+    for (int m = 0; m < 2; ++m) {
+      const uint8_t* at = (m ? a.up : a.gate) + block * 16384 + me.at(q.n0 & 127);
+#pragma unroll
+      for (int h = 0; h < H; ++h) q.w[i][m][h] = *reinterpret_cast<const v4i*>(at + 1024 * h);
+      q.scale[i][m] = (m ? a.up_scales : a.gate_scales)[block];
+    }
+  };
+  // (without branches, which would make the loads wait for each other: past the
+  // last unit or block the last one again, which nothing adds)
+  auto load_unit = [&](Unit& q, int u) {
+    u = u < units ? u : units - 1;
+    q.e = __builtin_amdgcn_readfirstlane(named.expert(u / tiles));
+    q.n0 = u % tiles * R;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) load_block(q, i, wave + 8 * i < kb ? wave + 8 * i : kb - 1);
+  };
+  v4f acc[2];
+  auto add_block = [&](const Unit& q, int i, const u4 (&x)[2 * H]) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const FewScale scale = few_scale(q.scale[i][m]);
+      v4f part = {0, 0, 0, 0};
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        u4 wv[2];
+        few_bf16(q.w[i][m][h], scale.pow2, wv);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) part = mfma_bf16(wv[s], x[2 * h + s], part);
       }
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const FewScale sw = few_scale((m ? a.up_scales : a.gate_scales)[panel + b]);
-        const uint8_t* at = (m ? a.up : a.gate) + (panel + b) * 16384 + (n0 & 127) * 128 + lane * 16;
-        v4f part = {0, 0, 0, 0};
+      for (int t = 0; t < 4; ++t) acc[m][t] = __builtin_fmaf(part[t], scale.factor, acc[m][t]);
+    }
+  };
+  if ((int)blockIdx.x >= units) return;
+  Unit q;
+  load_unit(q, blockIdx.x);
+  int turn = 0;
+  for (int u = blockIdx.x; u < units; u += gridDim.x, ++turn) {
+    acc[0] = acc[1] = v4f{0, 0, 0, 0};
+    const int e = q.e, n0 = q.n0;
+    if constexpr (NB > 0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          u4 wv[2];
-          few_bf16(*reinterpret_cast<const v4i*>(at + 1024 * h), sw.pow2, wv);
-#pragma unroll
-          for (int s = 0; s < 2; ++s) part = mfma_bf16(wv[s], xv[2 * h + s], part);
-        }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) acc[m][t] = __builtin_fmaf(part[t], sw.factor, acc[m][t]);
+      for (int i = 0; i < NB; ++i)
+        if (wave + 8 * i < kb) add_block(q, i, xv[i]);
+    } else {
+      for (int b = wave; b < kb; b += 8) {
+        load_x(b, xv[0]);
+        load_block(q, 0, b);
+        add_block(q, 0, xv[0]);
       }
     }
+    load_unit(q, u + gridDim.x);
 #pragma unroll
-    for (int m = 0; m < 2; ++m) sums[wave][m][lane] = acc[m];
-    __syncthreads();
-    if (tid < 64) {
-      const int col = n0 + 4 * g;
-      if (lr < a.tokens && (routes.tokens[e] >> lr & 1) && col < a.inter) {
-        v4f gate = {0, 0, 0, 0}, up = {0, 0, 0, 0};
+    for (int m = 0; m < 2; ++m) sums[turn & 1][wave][m][lane] = acc[m];
+    lds_barrier();
+    if (wave != (turn & 7)) continue;
+    const int t = lane & 15, col = n0 + 4 * (lane >> 4);
+    if (t >= a.tokens || !(routes.tokens[e] >> t & 1) || col >= a.inter) continue;
+    v4f gate = {0, 0, 0, 0}, up = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < 8; ++w) {
-          gate += sums[w][0][lane];
-          up += sums[w][1][lane];
-        }
-        const int k = routes.rank[lr][e];
-        const float p = routes.p[lr][k];
-        uint16_t* at = a.h + (int64_t)(lr * a.topk + k) * a.inter + col;
-        const int64_t low = (int64_t)a.tokens * a.topk * a.inter;
-        uint2 hi, lo;
-        float y[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) y[t] = gate[t] * sigmoid_f32(gate[t]) * up[t] * p;
-        hi.x = pack_bf16x2(y[0], y[1]);
-        hi.y = pack_bf16x2(y[2], y[3]);
-        // (nothing is left of what became infinite)
-        auto left = [](float v, float r) { return __builtin_isinf(r) ? 0.0f : v - r; };
-        lo.x = pack_bf16x2(left(y[0], bf16_lo(hi.x)), left(y[1], bf16_hi(hi.x)));
-        lo.y = pack_bf16x2(left(y[2], bf16_lo(hi.y)), left(y[3], bf16_hi(hi.y)));
-        *reinterpret_cast<uint2*>(at) = hi;
-        *reinterpret_cast<uint2*>(at + low) = lo;
-      }
+    for (int w = 0; w < 8; ++w) {
+      gate += sums[turn & 1][w][0][lane];
+      up += sums[turn & 1][w][1][lane];
     }
-    __syncthreads();
+    const float p = routes.p[t][e];
+    uint16_t* at = a.h + (int64_t)(t * a.topk + routes.rank[t][e]) * a.inter + col;
+    const int64_t low = (int64_t)a.tokens * a.topk * a.inter;
+    uint2 hi, lo;
+    float y[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) y[s] = gate[s] * sigmoid_f32(gate[s]) * up[s] * p;
+    hi.x = pack_bf16x2(y[0], y[1]);
+    hi.y = pack_bf16x2(y[2], y[3]);
+    // (nothing is left of what became infinite)
+    auto left = [](float v, float r) { return __builtin_isinf(r) ? 0.0f : v - r; };
+    lo.x = pack_bf16x2(left(y[0], bf16_lo(hi.x)), left(y[1], bf16_hi(hi.x)));
+    lo.y = pack_bf16x2(left(y[2], bf16_lo(hi.y)), left(y[3], bf16_hi(hi.y)));
+    *reinterpret_cast<uint2*>(at) = hi;
+    *reinterpret_cast<uint2*>(at + low) = lo;
   }
 #endif
 }
 
-// 16 columns of the output: the waves split the pairs (expert named, block of k).
+// Down, combine and residual: R NT columns of the output. The pairs (expert named,
+// block of k) of part blockIdx.y of gridDim.y are split among the eight waves, D on
+// their way; their sums meet in LDS. With several parts the last workgroup of a
+// tile to arrive adds the parts' sums, in their order.
+template <int R, int NT, int D>
 __global__ __launch_bounds__(512) void few_down_kernel(const MoeFewArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  __shared__ v4f sums[8][64];
+  __shared__ v4f sums[8][NT][64];
+  __shared__ int last;
+  constexpr int H = FewLane<R>::HALVES, COLS = R * NT;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lr = lane & 15, g = lane >> 4;
+  const FewLane<R> me;
+  __shared__ int experts[kMaxExperts];
+  __shared__ int16_t slots[kMaxExperts][kTokens];
   const FewTable& table = *static_cast<const FewTable*>(a.table);
-  const int kb = f8_blocks(a.inter), panels = f8_blocks(a.hidden), pairs = table.count * kb;
-  const int n0 = blockIdx.x * 16;
+  {  // all of the table with one round trip (entries past the last are not used)
+    const int e = table.expert[tid % kMaxExperts];
+    const uint2 v = reinterpret_cast<const uint2*>(table.slot)[tid];
+    if (tid < kMaxExperts) experts[tid] = e;
+    reinterpret_cast<uint2*>(slots)[tid] = v;
+    static_assert(sizeof(slots) == 512 * 8, "eight bytes per thread");
+  }
+  const int kb = f8_blocks(a.inter), panels = f8_blocks(a.hidden), n0 = blockIdx.x * COLS;
+  const int parts = gridDim.y, part = blockIdx.y, all = table.count * kb;
+  const int q0 = all * part / parts, q1 = all * (part + 1) / parts;  // all <= 128 * 256
   const int64_t low = (int64_t)a.tokens * a.topk * a.inter;
-  v4f acc = {0, 0, 0, 0};
-  for (int q = wave; q < pairs; q += 8) {
-    const int i = q / kb, b = q % kb, e = table.expert[i], slot = table.slot[i][lr];
-    const int64_t block = ((int64_t)e * panels + n0 / 128) * kb + b;
-    const FewScale sw = few_scale(a.down_scales[block]);
-    const uint8_t* at = a.down + block * 16384 + (n0 & 127) * 128 + lane * 16;
-    v4f part = {0, 0, 0, 0};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      u4 wv[2];
-      few_bf16(*reinterpret_cast<const v4i*>(at + 1024 * h), sw.pow2, wv);
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int k = 128 * b + 64 * h + 16 * g + 8 * s;
-        u4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
-        if (slot >= 0 && k < a.inter) {
-          const uint16_t* from = a.h + (int64_t)slot * a.inter + k;
-          hi = *reinterpret_cast<const u4*>(from);
-          lo = *reinterpret_cast<const u4*>(from + low);
-        }
-        part = mfma_bf16(wv[s], hi, part);
-        part = mfma_bf16(wv[s], lo, part);
-      }
-    }
-    // (a token's sum takes nothing of an expert it does not name, NaN weights neither)
-    if (slot >= 0) {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) acc[t] = __builtin_fmaf(part[t], sw.factor, acc[t]);
-    }
-  }
-  sums[wave][lane] = acc;
+  const __amdgpu_buffer_rsrc_t hr = make_rsrc(a.h, (uint32_t)(low * 2)), lr = make_rsrc(a.h + low, (uint32_t)(low * 2));
   __syncthreads();
-  const int col = n0 + 4 * g;
-  if (tid >= 64 || lr >= a.tokens || col >= a.hidden) return;
-  v4f y = {0, 0, 0, 0};
+  struct Pair {
+    int slot;
+    float scale;
+    v4i w[NT][H];
+    u4 hi[2 * H], lo[2 * H];
+  } ring[D];
+  // Pairs of this wave in turn: expert i of those named, block b. (Loads without
+  // branches, which would make them wait for each other: past the last pair the
+  // last one read again, which nothing adds.)
+  int q = q0 + wave, i = q / kb, b = q - i * kb;
+  const int i_step = 8 / kb, b_step = 8 - i_step * kb;
+  auto load = [&](Pair& p) {
+    const int e = __builtin_amdgcn_readfirstlane(experts[i]);
+    const int64_t block = ((int64_t)e * panels + n0 / 128) * kb + b;
+    p.slot = slots[i][me.row];
+    p.scale = a.down_scales[block];
 #pragma unroll
-  for (int w = 0; w < 8; ++w) y += sums[w][lane];
-  if (a.residual) {
-    const uint2 r = *reinterpret_cast<const uint2*>(a.residual + (int64_t)lr * a.hidden + col);
-    y += v4f{bf16_lo(r.x), bf16_hi(r.x), bf16_lo(r.y), bf16_hi(r.y)};
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+        p.w[j][h] = *reinterpret_cast<const v4i*>(a.down + block * 16384 + me.at((n0 & 127) + R * j) + 1024 * h);
+#pragma unroll
+    for (int s = 0; s < 2 * H; ++s) {
+      const int k = 128 * b + me.k + 64 * (s / 2) + 8 * (s % 2);
+      // tokens that name others: an offset that reads zeros
+      const int at = (p.slot * a.inter + k) * 2 | ((p.slot | (a.inter - 1 - k)) & (int)0x80000000u);
+      p.hi[s] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(hr, at, 0, 0));
+      p.lo[s] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(lr, at, 0, 0));
+    }
+    if (q + 8 < q1) {
+      q += 8;
+      i += i_step;
+      b += b_step;
+      i += b >= kb;
+      b -= b >= kb ? kb : 0;
+    }
+  };
+  // R tokens x R / 4 quads of columns of each fragment, a thread each
+  constexpr int ITEMS = R * R / 4;
+  const int t = tid % R, quad = tid / R % (R / 4), j = tid / ITEMS, col = n0 + R * j + 4 * quad;
+  const bool mine = j < NT && t < a.tokens && col < a.hidden;
+  uint2 residual = {0, 0};
+  if (a.residual && mine) residual = *reinterpret_cast<const uint2*>(a.residual + (int64_t)t * a.hidden + col);
+  v4f acc[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) acc[n] = v4f{0, 0, 0, 0};
+  if (q < q1) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(ring[d]);
   }
-  *reinterpret_cast<uint2*>(a.out + (int64_t)lr * a.hidden + col) = uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+  for (int at = q0 + wave; at < q1; at += 8 * D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (at + 8 * d >= q1) break;
+      Pair& p = ring[d];
+      const FewScale scale = few_scale(p.scale);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        v4f sum = {0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          u4 wv[2];
+          few_bf16(p.w[n][h], scale.pow2, wv);
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            sum = mfma_bf16(wv[s], p.hi[2 * h + s], sum);
+            sum = mfma_bf16(wv[s], p.lo[2 * h + s], sum);
+          }
+        }
+        // (a token's sum takes nothing of an expert it does not name, NaN weights neither)
+        if (p.slot >= 0) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) acc[n][t] = __builtin_fmaf(sum[t], scale.factor, acc[n][t]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load(p);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) sums[wave][n][lane] = acc[n];
+  __syncthreads();
+  v4f y = {0, 0, 0, 0};
+  if (mine) {
+#pragma unroll
+    for (int w = 0; w < 8; ++w)
+#pragma unroll
+      for (int s = 0; s < 16 / R; ++s) y += sums[w][j][R * s + t + 16 * (R / 4 * s + quad)];
+  }
+  if (parts > 1) {
+    // The sums go through memory as atomics of device scope, which no cache holds
+    // back: a workgroup's are there once its stores have ended (fences of that scope,
+    // which write back and drop whole caches, took half of this kernel's time).
+    float* const at = static_cast<float*>(a.partial) + ((int64_t)blockIdx.x * parts * (NT * ITEMS) + tid) * 4;
+    if (mine) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        __hip_atomic_store(at + part * (NT * ITEMS * 4) + s, y[s], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    wait_vmcnt<0>();
+    __syncthreads();
+    if (tid == 0)
+      last = __hip_atomic_fetch_add(&a.arrived[blockIdx.x], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+    __syncthreads();
+    if (!last || !mine) return;
+    y = v4f{0, 0, 0, 0};
+    for (int o = 0; o < parts; ++o) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        y[s] += __hip_atomic_load(at + o * (NT * ITEMS * 4) + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  if (!mine) return;
+  y += v4f{bf16_lo(residual.x), bf16_hi(residual.x), bf16_lo(residual.y), bf16_hi(residual.y)};
+  *reinterpret_cast<uint2*>(a.out + (int64_t)t * a.hidden + col) = uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
 #endif
 }
 
-constexpr size_t kTableBytes = (sizeof(FewTable) + 255) / 256 * 256;
+constexpr int kNT = 2, kMostTiles = 32768 / (16 * kNT), kWorkgroups = 512, kCus = 256;
+constexpr size_t kTableBytes = (sizeof(FewTable) + 255) / 256 * 256, kArrivedBytes = kMostTiles * 4;
+
+// Tiles of the output with several parts, and the parts: two workgroups per CU
+// together.
+int few_tiles(int hidden) { return (hidden + 16 * kNT - 1) / (16 * kNT); }
+int few_parts(int hidden) {
+  const int parts = kWorkgroups / few_tiles(hidden);
+  return parts < 1 ? 1 : parts > 4 ? 4 : parts;
+}
+size_t few_partial_bytes(int hidden) { return (size_t)few_tiles(hidden) * few_parts(hidden) * kNT * 64 * 16; }
 
 }  // namespace
 
-size_t moe_few_workspace_bytes(int tokens, int topk, int inter) {
-  return kTableBytes + (size_t)tokens * topk * inter * 4;
+size_t moe_few_workspace_bytes(int tokens, int topk, int hidden, int inter) {
+  return kTableBytes + kArrivedBytes + few_partial_bytes(hidden) + (size_t)tokens * topk * inter * 4;
 }
 
 hipError_t launch_moe_few(MoeFewArgs a, void* workspace, hipStream_t stream) {
-  a.table = workspace;
-  a.h = reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) + kTableBytes);
+  char* at = static_cast<char*>(workspace);
+  a.table = at;
+  a.arrived = reinterpret_cast<int*>(at += kTableBytes);
+  a.partial = at += kArrivedBytes;
+  a.h = reinterpret_cast<uint16_t*>(at + few_partial_bytes(a.hidden));
   const int slots = a.tokens * a.topk, most = slots < a.experts ? slots : a.experts;
-  const int units = most * ((a.inter + 15) / 16);
-  few_gate_up_kernel<<<units < 512 ? units : 512, 512, 0, stream>>>(a);
+  const int blocks = (f8_blocks(a.hidden) + 7) / 8;  // per wave
+  const bool few = a.tokens <= 8;
+  a.down_tiles = few_tiles(a.hidden);
+  const int units = most * ((a.inter + 15) / 16), grid = units < kCus ? units : kCus;
+  if (blocks <= 1)
+    few_gate_up_kernel<1><<<grid, 512, 0, stream>>>(a);
+  else if (blocks <= 2)
+    few_gate_up_kernel<2><<<grid, 512, 0, stream>>>(a);
+  else if (blocks <= 4)
+    few_gate_up_kernel<4><<<grid, 512, 0, stream>>>(a);
+  else
+    few_gate_up_kernel<0><<<grid, 512, 0, stream>>>(a);
   if (hipError_t e = hipGetLastError()) return e;
-  few_down_kernel<<<(a.hidden + 15) / 16, 512, 0, stream>>>(a);
+  if (few && slots <= 16)
+    few_down_kernel<8, 1, 2><<<(a.hidden + 7) / 8, 512, 0, stream>>>(a);
+  else
+    few_down_kernel<16, kNT, 1><<<dim3(a.down_tiles, few_parts(a.hidden)), 512, 0, stream>>>(a);
   return hipGetLastError();
 }
 

@@ -19,11 +19,15 @@ struct MoeFewArgs {
   const float *gate_scales, *up_scales, *down_scales;
   const uint16_t* residual;  // bf16 [tokens][hidden] or NULL
   uint16_t* out;
-  void* table;  // in the workspace
-  uint16_t* h;  // in the workspace: bf16 [tokens * topk][inter], then what its rounding left
+  // in the workspace:
+  void* table;
+  int down_tiles;  // of the output, with several parts
+  int* arrived;    // per tile, the parts done
+  void* partial;   // their sums
+  uint16_t* h;     // bf16 [tokens * topk][inter], then what its rounding left
 };
 
-size_t moe_few_workspace_bytes(int tokens, int topk, int inter);
+size_t moe_few_workspace_bytes(int tokens, int topk, int hidden, int inter);
 hipError_t launch_moe_few(MoeFewArgs a, void* workspace, hipStream_t stream);
 
 }  // namespace clef
