@@ -97,10 +97,12 @@ SIGNATURES = {
                                           _P]),
     "clef_moe_expert_gate_up_f8": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32,
                                                   _I32, _I32, _P, _P]),
+    "clef_linear_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32]),
+    "clef_linear_kernel_name": (ctypes.c_char_p, [_I64, _I32, _I32, _I32]),
     "clef_linear": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _I32, _I64, _P, _I32, _I32, _P, _I64, _P, _I32, _I64,
-                                   _P]),
+                                   _P, _SZ, _P]),
     "clef_linear_gate_up": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _P, _I32, _I64, _P, _P, _I32, _I32, _P, _I64,
-                                           _P]),
+                                           _P, _SZ, _P]),
     "clef_moe_layer_f8_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32]),
     "clef_moe_layer_f8": (ctypes.c_int, [_P, _I64, _P, _I32, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P,
                                          _P, _P, _P, _SZ, _P]),
@@ -1266,6 +1268,12 @@ def _linear_out(like: torch.Tensor, rows: int, cols: int, out: torch.Tensor | No
     return out, out.stride(0) if rows > 1 else cols
 
 
+def _linear_scratch(like: torch.Tensor, m: int, n: int, k: int, gate_up: int):
+    """(workspace, bytes) of a product; few rows need none."""
+    nbytes = _n.value(_n.clef_linear_workspace_bytes, m, n, k, gate_up) if m > 8 else 0
+    return (_n.empty(like, torch.uint8, nbytes), nbytes) if nbytes > 0 else (None, 0)
+
+
 def _activation_code(activation: str | None) -> int:
     code = ACTIVATIONS.get(activation)
     if code is None:
@@ -1303,7 +1311,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     code = _activation_code(activation)
     out, out_pitch = _linear_out(x, m, n, out, dtype, device)
     _n.launch(_n.clef_linear, x.data_ptr(), m, k, x_pitch, weight.data_ptr(), n, w_pitch, bias, bias_dtype, code,
-              residual, residual_pitch, out.data_ptr(), int(dtype is torch.float32), out_pitch)
+              residual, residual_pitch, out.data_ptr(), int(dtype is torch.float32), out_pitch,
+              *_linear_scratch(x, m, n, k, 0))
     return out
 
 
@@ -1328,5 +1337,6 @@ def linear_gate_up(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, activa
     m = x.shape[0]
     out, out_pitch = _linear_out(x, m, n, out, torch.bfloat16, device)
     _n.launch(_n.clef_linear_gate_up, x.data_ptr(), m, k, x_pitch, gate.data_ptr(), up.data_ptr(), n, w_pitch,
-              gate_bias, up_bias, bias_dtype | up_dtype, code, out.data_ptr(), out_pitch)
+              gate_bias, up_bias, bias_dtype | up_dtype, code, out.data_ptr(), out_pitch,
+              *_linear_scratch(x, m, n, k, 1))
     return out

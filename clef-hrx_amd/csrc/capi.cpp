@@ -1083,6 +1083,22 @@ bool overlap(const Pieces& a, const Pieces& b) {
   return behind < a.width || behind + b.width > a.step;
 }
 
+Pieces linear_result(const clef::LinearArgs& p, int32_t out_dtype) {
+  const int64_t size = out_dtype ? 4 : 2;
+  return {p.out, p.m, p.out_stride * size, p.n * size};
+}
+
+// Whether `piece` shares a byte with an operand (`onto`: the residual aside).
+bool linear_over(const clef::LinearArgs& p, bool gate_up, int32_t bias_dtype, const Pieces& piece, bool onto = false) {
+  auto over = [&](const void* at, int64_t rows, int64_t step, int64_t width) {
+    return at != nullptr && overlap(piece, Pieces{at, rows, step, width});
+  };
+  const int64_t bias = p.n * (bias_dtype ? 4ll : 2ll);
+  return over(p.x, p.m, p.x_stride * 2, p.k * 2ll) || over(p.w, p.n, p.w_stride * 2, p.k * 2ll) ||
+         (gate_up && over(p.w2, p.n, p.w_stride * 2, p.k * 2ll)) || over(p.bias, 1, 0, bias) ||
+         over(p.bias2, 1, 0, bias) || (!onto && over(p.residual, p.m, p.residual_stride * 2, p.n * 2ll));
+}
+
 int check_linear(const clef::LinearArgs& p, bool gate_up, int32_t bias_dtype, int32_t out_dtype) {
   constexpr int64_t most = 1048576;
   auto dtype = [](int32_t d) { return d == 0 || d == 1; };
@@ -1097,24 +1113,24 @@ int check_linear(const clef::LinearArgs& p, bool gate_up, int32_t bias_dtype, in
   if (!aligned(p.x, 2) || !aligned(p.w, 2) || (gate_up && !aligned(p.w2, 2)) || !aligned(p.out, out_bytes) ||
       !optional(p.bias, bias_bytes) || !optional(p.bias2, bias_bytes) || !optional(p.residual, 2))
     return fail(kLinearAlign);
-  const Pieces out{p.out, p.m, p.out_stride * (int64_t)out_bytes, p.n * (int64_t)out_bytes};
-  auto over = [&](const void* at, int64_t rows, int64_t step, int64_t width) {
-    return at != nullptr && overlap(out, Pieces{at, rows, step, width});
-  };
   const bool onto = p.residual == p.out && p.residual_stride == p.out_stride && out_dtype == 0;
-  if (over(p.x, p.m, p.x_stride * 2, p.k * 2ll) || over(p.w, p.n, p.w_stride * 2, p.k * 2ll) ||
-      over(p.w2, p.n, p.w_stride * 2, p.k * 2ll) || over(p.bias, 1, 0, p.n * (int64_t)bias_bytes) ||
-      over(p.bias2, 1, 0, p.n * (int64_t)bias_bytes) ||
-      (!onto && over(p.residual, p.m, p.residual_stride * 2, p.n * 2ll)))
-    return fail(kLinearOverlap);
+  if (linear_over(p, gate_up, bias_dtype, linear_result(p, out_dtype), onto)) return fail(kLinearOverlap);
   return CLEF_OK;
 }
 
-int linear(clef::LinearArgs& p, bool gate_up, int32_t bias_dtype, int32_t out_dtype, clef_stream_t stream) {
+int linear(clef::LinearArgs& p, bool gate_up, int32_t bias_dtype, int32_t out_dtype, void* workspace,
+           size_t workspace_bytes, clef_stream_t stream) {
   if (int rc = check_linear(p, gate_up, bias_dtype, out_dtype)) return rc;
   if (p.m == 0) return CLEF_OK;
+  if (const size_t need = clef::linear_workspace_bytes(p.m, p.n, p.k, gate_up)) {
+    if (!aligned(workspace, 16)) return fail(kAlign);
+    if (workspace_bytes < need) return fail(kWorkspace);
+    if (linear_over(p, gate_up, bias_dtype, Pieces{workspace, 1, 0, (int64_t)need}) ||
+        overlap(Pieces{workspace, 1, 0, (int64_t)need}, linear_result(p, out_dtype)))
+      return fail("linear workspace overlaps an operand");
+  }
   p.bias_f32 = bias_dtype != 0, p.out_f32 = out_dtype != 0;
-  return hip_status(clef::launch_linear(p, gate_up, hs(stream)));
+  return hip_status(clef::launch_linear(p, gate_up, workspace, hs(stream)));
 }
 
 constexpr const char* kFewShape = "unsupported MoE shape for few tokens";
@@ -1128,22 +1144,34 @@ bool few_shape(int64_t tokens, int32_t hidden, int32_t inter, int32_t experts, i
 
 extern "C" {
 
+size_t clef_linear_workspace_bytes(int64_t m, int32_t n, int32_t k, int32_t gate_up) {
+  if (m < 1 || m > 1048576 || n < 1 || n > 1048576 || k < 1 || k > 1048576) return 0;
+  return clef::linear_workspace_bytes(m, n, k, gate_up != 0);
+}
+
+const char* clef_linear_kernel_name(int64_t m, int32_t n, int32_t k, int32_t gate_up) {
+  if (m < 1 || m > 1048576 || n < 1 || n > 1048576 || k < 1 || k > 1048576) return "";
+  return clef::linear_kernel_name(m, n, k, gate_up != 0);
+}
+
 int clef_linear(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint16_t* w, int32_t n,
                 int64_t w_stride, const void* bias, int32_t bias_dtype, int32_t activation, const uint16_t* residual,
-                int64_t residual_stride, void* out, int32_t out_dtype, int64_t out_stride, clef_stream_t stream) {
+                int64_t residual_stride, void* out, int32_t out_dtype, int64_t out_stride, void* workspace,
+                size_t workspace_bytes, clef_stream_t stream) {
   clef::LinearArgs p{};
   p.x = x, p.m = m, p.x_stride = x_stride, p.n = n, p.k = k, p.w = w, p.w_stride = w_stride, p.bias = bias;
   p.act = activation, p.residual = residual, p.residual_stride = residual_stride, p.out = out, p.out_stride = out_stride;
-  return linear(p, false, bias_dtype, out_dtype, stream);
+  return linear(p, false, bias_dtype, out_dtype, workspace, workspace_bytes, stream);
 }
 
 int clef_linear_gate_up(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint16_t* gate,
                         const uint16_t* up, int32_t n, int64_t w_stride, const void* gate_bias, const void* up_bias,
-                        int32_t bias_dtype, int32_t activation, uint16_t* h, int64_t h_stride, clef_stream_t stream) {
+                        int32_t bias_dtype, int32_t activation, uint16_t* h, int64_t h_stride, void* workspace,
+                        size_t workspace_bytes, clef_stream_t stream) {
   clef::LinearArgs p{};
   p.x = x, p.m = m, p.x_stride = x_stride, p.n = n, p.k = k, p.w = gate, p.w2 = up, p.w_stride = w_stride;
   p.bias = gate_bias, p.bias2 = up_bias, p.act = activation, p.out = h, p.out_stride = h_stride;
-  return linear(p, true, bias_dtype, 0, stream);
+  return linear(p, true, bias_dtype, 0, workspace, workspace_bytes, stream);
 }
 
 size_t clef_moe_layer_f8_workspace_bytes(int64_t tokens, int32_t hidden, int32_t inter, int32_t experts,

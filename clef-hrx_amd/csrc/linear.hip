@@ -136,11 +136,14 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(
   const int kg = T::KG == 1 ? 0 : wave / T::NWB, wb = wave % T::NWB;  // group, wave in it
   const int wm = wb / T::WAVES_N, wn = wb % T::WAVES_N;
   int tm, tn;
-  tile_of_block(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
+  const int tiles = tiles_m * tiles_n, part = p.parts == 1 ? 0 : blockIdx.x / tiles;
+  tile_of_block(blockIdx.x - part * tiles, tiles, tiles_m, tiles_n, tm, tn);
   const int64_t m0 = (int64_t)tm * T::BM;
   const int n0 = tn * COLS;
   const int here = p.m - m0 < T::BM ? (int)(p.m - m0) : T::BM, cols = p.n - n0 < COLS ? p.n - n0 : COLS;
-  const int blocks = (p.k + 63) / 64, steps = (blocks + T::KG - 1) / T::KG;
+  // blocks of 64 k: this part's
+  const int all = (p.k + 63) / 64, first = (int)((int64_t)all * part / p.parts);
+  const int blocks = (int)((int64_t)all * (part + 1) / p.parts) - first, steps = (blocks + T::KG - 1) / T::KG;
 
   // This wave's DMA: an instruction moves 8 rows of a step, the first half of a
   // wave's A instructions rows of the first TM / 2 fragments of either row of
@@ -181,8 +184,8 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(
   // that nothing counts, so that every step issues and waits alike)
   auto issue = [&](char* stage, int kt, int x) {
     const int block = T::KG * kt + kg;
-    const bool in = block < blocks, last = block == blocks - 1;
-    const int k = in ? block * 128 : 0;
+    const bool in = block < blocks, last = first + block == all - 1;
+    const int k = in ? (first + block) * 128 : 0;
     if (x < T::B_SLOTS) {
       const int piece = wb * T::B_SLOTS + x;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(in ? b_rsrc : none,
@@ -312,6 +315,20 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(
       for (int j = 0; j < TN; ++j) sum[i][j] += theirs[(i * TN + j) * 64];
     __syncthreads();
   }
+  if (p.parts > 1) {
+    constexpr int MATS = GU ? 2 : 1;
+#pragma unroll
+    for (int i = 0; i < EM; ++i) {
+      const int r = w0 + 16 * i + lr;
+      if (r >= here) continue;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int col = c0 + 16 * (j % NC) + 4 * g;
+        if (col < p.n) *reinterpret_cast<v4f*>(linear_partial4(p, part, j / NC, MATS, m0 + r, col)) = sum[i][j];
+      }
+    }
+    return;
+  }
   constexpr int ROW = 32 * NC, CH = 2 * NC, PER = 64 / CH;  // bytes and chunks of a row, rows per store
   char* own = lds + wave * T::EPI;
 #pragma unroll
@@ -359,9 +376,34 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(
 #endif
 }
 
+// The parts' sums, in their order, and the epilogue: four columns of a row per thread.
+template <bool GU>
+__global__ __launch_bounds__(256) void linear_join_kernel(const LinearArgs p) {
+  const int quads = (p.n + 3) / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / quads;
+  if (row >= p.m) return;
+  const int col = (int)(i - row * quads) * 4;
+  constexpr int MATS = GU ? 2 : 1;
+  v4f y = {0, 0, 0, 0}, y2 = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = 0; s < p.parts; ++s) {
+    y += *reinterpret_cast<const v4f*>(linear_partial4(p, s, 0, MATS, row, col));
+    if constexpr (GU) y2 += *reinterpret_cast<const v4f*>(linear_partial4(p, s, 1, MATS, row, col));
+  }
+  linear_epilogue4<GU>(p, row, col, y, y2);
+}
+
+template <bool GU>
+hipError_t launch_join(const LinearArgs& p, hipStream_t stream) {
+  const int64_t quads = p.m * ((p.n + 3) / 4);
+  linear_join_kernel<GU><<<(unsigned)((quads + 255) / 256), 256, 0, stream>>>(p);
+  return hipGetLastError();
+}
+
 using Tile256 = LinearTile<128, 64, 2, 4>;        // 256 x 256
 using Tile128 = LinearTile<64, 32, 2, 4, 2>;      // 128 x 128, two workgroups per CU
 using Tile128K = LinearTile<64, 64, 2, 2, 1, 2>;  // 128 x 128, two steps of k at a time
+using Tile128x256 = LinearTile<64, 64, 2, 4>;
 
 template <class T, bool GU, bool RESID>
 hipError_t launch_tile(const LinearArgs& p, hipStream_t stream) {
@@ -370,8 +412,8 @@ hipError_t launch_tile(const LinearArgs& p, hipStream_t stream) {
   if (hipError_t e = ensure_dynamic_lds(cache, reinterpret_cast<const void*>(kernel), T::LDS)) return e;
   constexpr int COLS = GU ? T::BN / 2 : T::BN;
   const int64_t tiles_m = (p.m + T::BM - 1) / T::BM, tiles_n = (p.n + COLS - 1) / COLS;
-  if (tiles_m * tiles_n > kMaxTiles) return hipErrorInvalidValue;
-  kernel<<<(unsigned)(tiles_m * tiles_n), T::THREADS, T::LDS, stream>>>(p, (int)tiles_m, (int)tiles_n);
+  if (tiles_m * tiles_n * p.parts > kMaxTiles) return hipErrorInvalidValue;
+  kernel<<<(unsigned)(tiles_m * tiles_n * p.parts), T::THREADS, T::LDS, stream>>>(p, (int)tiles_m, (int)tiles_n);
   return hipGetLastError();
 }
 
@@ -517,25 +559,70 @@ hipError_t launch_any(const LinearArgs& p, hipStream_t stream) {
 
 constexpr int64_t kCus = 256;
 
-enum class LinearKernel { any, s8x8, s8x16, s8x32, s16x16, s16x32, s16x64, s32x64, s64x64, t128x128, t128x128k, t256x256 };
+enum class LinearKernel { any, s8x8, s8x16, s16x16, s16x32, s16x64, s32x64, s64x64, t128x128, t128x128k, t256x256, t128x256 };
 
-// The kernel for a product of m rows against n weight rows (gate/up: both).
-LinearKernel linear_kernel(int64_t m, int64_t rows_of_w, int k, bool gate_up) {
+struct LinearPlan {
+  LinearKernel kernel;
+  int parts;
+};
+
+// The kernel for a product of m rows against n weight rows (gate/up: both): of the
+// kernels' times as modelled here, in us, the least.
+LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up) {
+  if (m <= 8) return {gate_up || (m > 4 && rows_of_w > 8192) ? LinearKernel::s8x16 : LinearKernel::s8x8, 1};
   auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((rows_of_w + bn - 1) / bn); };
-  if (m <= 8) return gate_up || (m > 4 && rows_of_w > 8192) ? LinearKernel::s8x16 : LinearKernel::s8x8;
-  if (tiles(16, 16) <= kCus && !gate_up) return LinearKernel::s16x16;
-  if (tiles(16, 32) <= kCus) return LinearKernel::s16x32;
-  if (m <= 16) return tiles(16, 64) > kCus ? LinearKernel::s16x32 : LinearKernel::s16x64;
-  if (tiles(32, 64) <= kCus) return LinearKernel::s32x64;
-  if (tiles(64, 64) <= kCus) return LinearKernel::s64x64;
-  auto rounds = [&](int b) { return (tiles(b, b) + kCus - 1) / kCus; };
-  if (rounds(128) >= 3 * rounds(256)) return LinearKernel::t256x256;
-  return rounds(128) <= 1 ? LinearKernel::t128x128k : LinearKernel::t128x128;
+  auto rounds = [](int64_t workgroups, int64_t at_once) { return (float)((workgroups + at_once - 1) / at_once); };
+  const float memory = ((float)(rows_of_w + m) * k + (float)m * rows_of_w) * 2 / 4.9e6f;
+  LinearPlan best{LinearKernel::any, 1};
+  float least = __builtin_huge_valf();
+  auto consider = [&](LinearKernel kernel, int parts, float t) {
+    if (t >= least) return;
+    least = t;
+    best = {kernel, parts};
+  };
+  auto stream = [&](LinearKernel kernel, int bm, int bn) {
+    if (m > 4096) return;  // (a launch has 65535 tiles of rows)
+    const float loads = rounds(tiles(bm, bn), kCus) * (bm + bn) * k * 2 / 33e3f;
+    consider(kernel, 1, 2.5f + (loads > memory ? loads : memory));
+  };
+  if (!gate_up) stream(LinearKernel::s16x16, 16, 16);
+  stream(LinearKernel::s16x32, 16, 32);
+  stream(LinearKernel::s16x64, 16, 64);
+  stream(LinearKernel::s32x64, 32, 64);
+  stream(LinearKernel::s64x64, 64, 64);
+  const int steps = (k + 63) / 64;
+  auto tile = [&](LinearKernel kernel, int bm, int bn, float start, float step, float pair) {
+    const int64_t of = tiles(bm, bn);
+    for (int parts : {1, 2, 3, 4, 6, 8}) {
+      const bool two = pair > 0 && of * parts > kCus;
+      const float r = rounds(of * parts, two ? 2 * kCus : kCus);
+      if (parts > 1 && (r > 1 || steps < 8 * parts)) break;
+      const float t = r * (start + (steps + parts - 1) / parts * (two ? pair : step));
+      consider(kernel, parts, (t > memory + start ? t : memory + start) +
+                                  (parts > 1 ? 3 + (float)(parts * m * rows_of_w) * 8 / 5e6f : 0));
+    }
+  };
+  tile(LinearKernel::t128x128, 128, 128, 4.5f, 0.57f, 1.0f);
+  tile(LinearKernel::t128x128k, 128, 128, 5.5f, 0.53f, 0);
+  tile(LinearKernel::t128x256, 128, 256, 6, 0.86f, 0);
+  tile(LinearKernel::t256x256, 256, 256, 10, 1.40f, 0);
+  return best;
+}
+
+template <class T, bool GU>
+hipError_t launch_parts(const LinearArgs& p, hipStream_t stream) {
+  if (p.parts == 1 && p.residual) return launch_tile<T, GU, !GU>(p, stream);
+  if (hipError_t e = launch_tile<T, GU, false>(p, stream)) return e;
+  return p.parts > 1 ? launch_join<GU>(p, stream) : hipSuccess;
 }
 
 template <bool GU>
-hipError_t launch_rows(const LinearArgs& p, hipStream_t stream) {
-  switch (rows_of_16(p) ? linear_kernel(p.m, (int64_t)p.n * (GU ? 2 : 1), p.k, GU) : LinearKernel::any) {
+hipError_t launch_rows(LinearArgs& p, void* workspace, hipStream_t stream) {
+  LinearPlan plan{LinearKernel::any, 1};
+  if (rows_of_16(p)) plan = linear_plan(p.m, (int64_t)p.n * (GU ? 2 : 1), p.k, GU);
+  p.parts = plan.parts;
+  p.partial = static_cast<float*>(workspace);
+  switch (plan.kernel) {
     case LinearKernel::s8x8: if constexpr (!GU) return launch_stream<8, 1, 1, 2, GU>(p, stream);
     case LinearKernel::s8x16: return launch_stream<8, 1, 2, 1, GU>(p, stream);
     case LinearKernel::s16x16: if constexpr (!GU) return launch_stream<16, 1, 1, 1, GU>(p, stream);
@@ -543,20 +630,30 @@ hipError_t launch_rows(const LinearArgs& p, hipStream_t stream) {
     case LinearKernel::s16x64: return launch_stream<16, 1, 4, 1, GU>(p, stream);
     case LinearKernel::s32x64: return launch_stream<16, 2, 4, 1, GU>(p, stream);
     case LinearKernel::s64x64: return launch_stream<16, 4, 4, 1, GU>(p, stream);
-    case LinearKernel::t128x128:
-      return p.residual ? launch_tile<Tile128, GU, !GU>(p, stream) : launch_tile<Tile128, GU, false>(p, stream);
-    case LinearKernel::t128x128k:
-      return p.residual ? launch_tile<Tile128K, GU, !GU>(p, stream) : launch_tile<Tile128K, GU, false>(p, stream);
-    case LinearKernel::t256x256:
-      return p.residual ? launch_tile<Tile256, GU, !GU>(p, stream) : launch_tile<Tile256, GU, false>(p, stream);
+    case LinearKernel::t128x128: return launch_parts<Tile128, GU>(p, stream);
+    case LinearKernel::t128x128k: return launch_parts<Tile128K, GU>(p, stream);
+    case LinearKernel::t256x256: return launch_parts<Tile256, GU>(p, stream);
+    case LinearKernel::t128x256: return launch_parts<Tile128x256, GU>(p, stream);
     default: return launch_any<GU>(p, stream);
   }
 }
 
 }  // namespace
 
-hipError_t launch_linear(const LinearArgs& p, bool gate_up, hipStream_t stream) {
-  return gate_up ? launch_rows<true>(p, stream) : launch_rows<false>(p, stream);
+size_t linear_workspace_bytes(int64_t m, int n, int k, bool gate_up) {
+  const int64_t matrices = gate_up ? 2 : 1;
+  const LinearPlan plan = linear_plan(m, n * matrices, k, gate_up);
+  return plan.parts > 1 ? (size_t)(plan.parts * matrices * m * ((n + 3) & ~3)) * 4 : 0;
+}
+
+const char* linear_kernel_name(int64_t m, int n, int k, bool gate_up) {
+  static const char* const names[] = {"any",   "8x8",     "8x16",     "16x16",   "16x32",  "16x64",
+                                      "32x64", "64x64", "128x128", "128x128x2", "256x256", "128x256"};
+  return names[(int)linear_plan(m, (int64_t)n * (gate_up ? 2 : 1), k, gate_up).kernel];
+}
+
+hipError_t launch_linear(LinearArgs p, bool gate_up, void* workspace, hipStream_t stream) {
+  return gate_up ? launch_rows<true>(p, workspace, stream) : launch_rows<false>(p, workspace, stream);
 }
 
 }  // namespace clef

@@ -32,9 +32,16 @@ struct LinearArgs {
   void* out;  // bf16 or f32, rows out_stride apart
   int64_t out_stride;
   bool out_f32;
+  // Products split along k: parts 1, or each part's sums go to partial (f32 [part]
+  // [matrix][m][n rounded up to 4]) and another launch adds them
+  int parts;
+  float* partial;
 };
 
-hipError_t launch_linear(const LinearArgs& p, bool gate_up, hipStream_t stream);
+// Scratch for the parts of a product whose operands' rows lie on 16 bytes.
+size_t linear_workspace_bytes(int64_t m, int n, int k, bool gate_up);
+const char* linear_kernel_name(int64_t m, int n, int k, bool gate_up);
+hipError_t launch_linear(LinearArgs p, bool gate_up, void* workspace, hipStream_t stream);
 
 namespace {
 
@@ -152,6 +159,13 @@ __device__ __forceinline__ void linear_store4(const LinearArgs& p, int64_t row, 
     if (col + 1 < p.n) to[1] = (uint16_t)(v.x >> 16);
     if (col + 2 < p.n) to[2] = (uint16_t)v.y;
   }
+}
+
+// A part's sums of columns col .. + 3 (of matrix `which` of `matrices`).
+__device__ __forceinline__ float* linear_partial4(const LinearArgs& p, int part, int which, int matrices, int64_t row,
+                                                  int col) {
+  const int64_t pitch = (p.n + 3) & ~3;
+  return p.partial + (((int64_t)part * matrices + which) * p.m + row) * pitch + col;
 }
 
 // All of it: sums y (gate/up: y the gate's, y2 the up's) of one row.

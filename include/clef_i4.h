@@ -619,18 +619,32 @@ int clef_moe_expert_gate_up_f8(const uint8_t* a, int64_t a_rows, const uint8_t* 
  * "linear operand is NULL or not aligned". The output may be the residual
  * itself (the same rows, bf16); over a part of it, x, w or the bias -> "linear
  * output overlaps an operand" (columns beside an operand's in rows of one
- * stride do not overlap). With no rows a call does nothing. */
+ * stride do not overlap). With no rows a call does nothing.
+ *
+ * Products of some rows whose tiles do not fill the card are split along k; the
+ * workspace (bytes below, 0 for up to 8 rows and wherever none is needed; 16-byte
+ * aligned, apart from every operand -> "linear workspace overlaps an operand")
+ * takes the parts' sums, which are added in a fixed order. */
+size_t clef_linear_workspace_bytes(int64_t m, int32_t n, int32_t k, int32_t gate_up);
+
+/* The tile (rows x weight rows) that the library's rule picks for operands whose
+ * rows lie on 16 bytes, for tests and profiles: "8x8", "8x16", "16x16", "16x32",
+ * "16x64", "32x64", "64x64", "128x128", "128x128x2" (two steps of k at a time),
+ * "128x256", "256x256"; other operands run "any". "" for a shape the products
+ * reject. */
+const char* clef_linear_kernel_name(int64_t m, int32_t n, int32_t k, int32_t gate_up);
+
 int clef_linear(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint16_t* w, int32_t n,
                 int64_t w_stride, const void* bias, int32_t bias_dtype, int32_t activation,
                 const uint16_t* residual, int64_t residual_stride, void* out, int32_t out_dtype,
-                int64_t out_stride, clef_stream_t stream);
+                int64_t out_stride, void* workspace, size_t workspace_bytes, clef_stream_t stream);
 
 /* h[m][n] = act(x gate^T + gate_bias) * (x up^T + up_bias) in f32, bf16 once
  * (SiLU: SwiGLU); gate and up [n][k] share w_stride. As clef_linear otherwise. */
 int clef_linear_gate_up(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint16_t* gate,
                         const uint16_t* up, int32_t n, int64_t w_stride, const void* gate_bias,
                         const void* up_bias, int32_t bias_dtype, int32_t activation, uint16_t* h,
-                        int64_t h_stride, clef_stream_t stream);
+                        int64_t h_stride, void* workspace, size_t workspace_bytes, clef_stream_t stream);
 
 /* The Omni MoE block (src/omni.rs:760-857) of up to 16 tokens on block-scaled
  * FP8 experts (the tiled weights of clef_f8_pack_weight, one matrix per

@@ -16,15 +16,17 @@ def call(name, *args):
 
 
 def linear(x=FAKE, m=4, k=128, xs=None, w=FAR, n=64, ws=None, bias=None, bias_dtype=0, act=0, res=None, rs=None, out=2 * FAR,
-           out_dtype=0, os=None):
+           out_dtype=0, os=None, ws_at=5 * FAR, nbytes=1 << 40):
     xs, ws, rs, os = (d if v is None else v for v, d in ((xs, k), (ws, k), (rs, n), (os, n)))
-    return call("clef_linear", x, m, k, xs, w, n, ws, bias, bias_dtype, act, res, rs, out, out_dtype, os, None)
+    return call("clef_linear", x, m, k, xs, w, n, ws, bias, bias_dtype, act, res, rs, out, out_dtype, os, ws_at,
+                nbytes, None)
 
 
 def gate_up(x=FAKE, m=4, k=128, xs=None, gate=FAR, up=3 * FAR, n=64, ws=None, gb=None, ub=None, bias_dtype=0, act=4,
-            h=2 * FAR, hs=None):
+            h=2 * FAR, hs=None, ws_at=5 * FAR, nbytes=1 << 40):
     xs, ws, hs = (d if v is None else v for v, d in ((xs, k), (ws, k), (hs, n)))
-    return call("clef_linear_gate_up", x, m, k, xs, gate, up, n, ws, gb, ub, bias_dtype, act, h, hs, None)
+    return call("clef_linear_gate_up", x, m, k, xs, gate, up, n, ws, gb, ub, bias_dtype, act, h, hs, ws_at,
+                nbytes, None)
 
 
 BAD = [dict(m=-1), dict(m=(1 << 20) + 1), dict(k=0), dict(k=(1 << 20) + 1), dict(n=0), dict(n=(1 << 20) + 1), dict(xs=127),
