@@ -5,18 +5,51 @@ namespace clef {
 
 namespace {
 
-// Eight values of a row from column k on, zeros past column K: rows start at any
-// even byte, so the load is an unaligned one.
-__device__ __forceinline__ u4 load8_any(const uint16_t* row, int k, int K) {
-  u4 v = {0, 0, 0, 0};
-  if (k + 8 <= K) {
-    __builtin_memcpy(&v, row + k, 16);
-  } else {
-#pragma unroll
-    for (int t = 0; t < 8; ++t)
-      if (k + t < K) v[t / 2] |= (uint32_t)row[k + t] << (16 * (t % 2));
+// Rows that start at any even byte: eight values from column k (a multiple of 8) on
+// are loaded as the five dwords that hold them and shifted into place at their use
+// (16-byte loads from odd multiples of two bytes took three times as long: 512 x
+// 2049 x 4096 104 us on 64 x 64 tiles, 512 x 2050 x 4096 42).
+struct AnyRow {
+  const char* down;  // the row's start, rounded down to 4 bytes
+  int shift;         // bits of the first dword in front of the row: 0 or 16
+  __device__ __forceinline__ explicit AnyRow(const uint16_t* row)
+      : down(reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)3)),
+        shift((int)(reinterpret_cast<uintptr_t>(row) & 2) * 8) {}
+  AnyRow() = default;
+};
+
+struct AnyEight {
+  u4 low;
+  uint32_t high;
+  __device__ __forceinline__ u4 values(int shift) const {
+    return u4{__builtin_amdgcn_alignbit(low[1], low[0], shift), __builtin_amdgcn_alignbit(low[2], low[1], shift),
+              __builtin_amdgcn_alignbit(low[3], low[2], shift), __builtin_amdgcn_alignbit(high, low[3], shift)};
   }
-  return v;
+};
+
+// k + 8 <= K. (Without a shift the fifth dword is not used, and may lie past the end.)
+__device__ __forceinline__ AnyEight any_load(const AnyRow& r, int k) {
+  typedef u4 __attribute__((aligned(4))) u4_any;
+  const char* at = r.down + 2 * (int64_t)k;
+  return {*reinterpret_cast<const u4_any*>(at), *reinterpret_cast<const uint32_t*>(at + 12 + r.shift / 4)};
+}
+
+// Any k: zeros past column K. Dwords past the row's last value are read there, so that
+// no branch makes the loads wait for each other.
+__device__ __forceinline__ AnyEight any_load_tail(const AnyRow& r, int k, int K) {
+  const int odd = r.shift / 16, last = (2 * (K - 1 + odd)) & ~3;  // of the dword that holds value K - 1
+  uint32_t d[5];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) {
+    const int at = 2 * k + 4 * j;
+    d[j] = *reinterpret_cast<const uint32_t*>(r.down + (at < last ? at : last));
+  }
+#pragma unroll
+  for (int j = 0; j < 5; ++j) {
+    const int left = K - k + odd - 2 * j;  // halves of this dword that are values
+    d[j] = left >= 2 ? d[j] : left == 1 ? d[j] & 0xFFFFu : 0u;
+  }
+  return {u4{d[0], d[1], d[2], d[3]}, d[4]};
 }
 
 // Every shape, stride and alignment: 64 rows x 64 weight rows (gate/up: 32 gate
@@ -34,20 +67,32 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinearArgs p) {
   const int n0 = blockIdx.x * COLS;
   // this thread's chunks: chunk threadIdx.x % 8 of rows threadIdx.x / 8 and + 32
   const int chunk = threadIdx.x & 7;
-  const uint16_t *xr[2], *wr[2];
+  const uint16_t *xr[2], *wr[2];  // rows past the end repeat the last
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = (threadIdx.x >> 3) + 32 * i;
-    xr[i] = m0 + r < p.m ? p.x + (m0 + r) * p.x_stride : nullptr;
+    xr[i] = p.x + (m0 + r < p.m ? m0 + r : p.m - 1) * p.x_stride;
     const int col = n0 + (GU ? r % 32 : r);
-    wr[i] = col < p.n ? (GU && i ? p.w2 : p.w) + col * p.w_stride : nullptr;
+    wr[i] = (GU && i ? p.w2 : p.w) + (col < p.n ? col : p.n - 1) * p.w_stride;
   }
   u4 xv[2], wv[2];
+  // (16-byte loads of any alignment: here eight lanes take 128 bytes in a row, and the
+  // dwords of AnyRow took 160 us where these take 122, 512 x 2049 x 17408)
   auto load = [&](int k0) {
+    const int k = k0 + 8 * chunk;
+    if (k0 + 64 <= p.k) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      xv[i] = xr[i] ? load8_any(xr[i], k0 + 8 * chunk, p.k) : u4{0, 0, 0, 0};
-      wv[i] = wr[i] ? load8_any(wr[i], k0 + 8 * chunk, p.k) : u4{0, 0, 0, 0};
+      for (int i = 0; i < 2; ++i) {
+        __builtin_memcpy(&xv[i], xr[i] + k, 16);
+        __builtin_memcpy(&wv[i], wr[i] + k, 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const AnyRow x(xr[i]), w(wr[i]);
+        xv[i] = any_load_tail(x, k, p.k).values(x.shift);
+        wv[i] = any_load_tail(w, k, p.k).values(w.shift);
+      }
     }
   };
   v4f acc[2][2] = {};
@@ -429,7 +474,10 @@ hipError_t launch_tile(const LinearArgs& p, hipStream_t stream) {
 // R: of the 16 x 16 sums the blocks on the diagonal count, one per piece. So a tile
 // has as few columns as fill the card, and a load takes 16 / R times 64 contiguous
 // bytes of a row.
-template <int R, int MT, int NT, int D, bool GU>
+//
+// ANY: rows that start at any even byte (AnyRow); only the last step takes values one
+// by one.
+template <bool ANY, int R, int MT, int NT, int D, bool GU>
 __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int NW = 8, Q = 16 / R, NG = GU ? NT / 2 : NT, BM = R * MT, COLS = R * NG;
@@ -458,11 +506,42 @@ __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p) 
     const int r = R * j + fr < cols ? R * j + fr : cols - 1;
     w_voff[j] = (int)(r * p.w_stride + k_lane) * 2;
   }
+  using Eight = std::conditional_t<ANY, AnyEight, u4>;
   struct Step {
-    u4 w[NT][2], a[MT][2];
+    Eight w[NT][2], a[MT][2];
   } ring[D];
+  AnyRow a_row[ANY ? MT : 1], w_row[ANY ? NT : 1];
+  if constexpr (ANY) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int r = R * i + fr < here ? R * i + fr : here - 1;
+      a_row[i] = AnyRow(p.x + (m0 + r) * p.x_stride);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int r = R * (j % NG) + fr < cols ? R * (j % NG) + fr : cols - 1;
+      w_row[j] = AnyRow((GU && j >= NG ? p.w2 : p.w) + (n0 + r) * p.w_stride);
+    }
+  }
   auto load = [&](Step& b, int s) {
     if (s >= steps) return;
+    if constexpr (ANY) {
+      auto all = [&](auto load8) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int k = SK * s + SK / 2 * h + k_lane;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) b.w[j][h] = load8(w_row[j], k);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) b.a[i][h] = load8(a_row[i], k);
+        }
+      };
+      if (SK * (s + 1) <= p.k)
+        all([](const AnyRow& row, int k) { return any_load(row, k); });
+      else
+        all([&](const AnyRow& row, int k) { return any_load_tail(row, k, p.k); });
+      return;
+    } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       // chunks past the end of k: an offset that reads zeros
@@ -475,6 +554,7 @@ __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p) 
       for (int i = 0; i < MT; ++i)
         b.a[i][h] = __builtin_bit_cast(
             u4, __builtin_amdgcn_raw_buffer_load_b128(a_rsrc, (a_voff[i] + SK * h) | past, s * (2 * SK), 0));
+    }
     }
   };
   v4f acc[MT][NT];
@@ -489,11 +569,23 @@ __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p) 
     for (int d = 0; d < D; ++d) {
       if (s + NW * d >= steps) break;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        u4 w[NT], a[MT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          if constexpr (ANY) w[j] = ring[d].w[j][h].values(w_row[j].shift);
+          else w[j] = ring[d].w[j][h];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          if constexpr (ANY) a[i] = ring[d].a[i][h].values(a_row[i].shift);
+          else a[i] = ring[d].a[i][h];
+        }
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] = mfma_bf16(ring[d].w[j][h], ring[d].a[i][h], acc[i][j]);
+          for (int j = 0; j < NT; ++j) acc[i][j] = mfma_bf16(w[j], a[i], acc[i][j]);
+      }
       __builtin_amdgcn_sched_barrier(0);
       load(ring[d], s + NW * (d + D));
       __builtin_amdgcn_sched_barrier(0);
@@ -526,11 +618,11 @@ __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p) 
 #endif
 }
 
-template <int R, int MT, int NT, int D, bool GU>
+template <bool ANY, int R, int MT, int NT, int D, bool GU>
 hipError_t launch_stream(const LinearArgs& p, hipStream_t stream) {
   constexpr int COLS = R * NT / (GU ? 2 : 1), lds = 8 * MT * NT * 1024;
   static LaunchCache cache;
-  auto* kernel = &linear_stream_kernel<R, MT, NT, D, GU>;
+  auto* kernel = &linear_stream_kernel<ANY, R, MT, NT, D, GU>;
   if (lds > 64 * 1024)
     if (hipError_t e = ensure_dynamic_lds(cache, reinterpret_cast<const void*>(kernel), lds)) return e;
   const int64_t tiles_m = (p.m + R * MT - 1) / (R * MT);
@@ -568,7 +660,7 @@ struct LinearPlan {
 
 // The kernel for a product of m rows against n weight rows (gate/up: both): of the
 // kernels' times as modelled here, in us, the least.
-LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up) {
+LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up, bool aligned) {
   if (m <= 8) return {gate_up || (m > 4 && rows_of_w > 8192) ? LinearKernel::s8x16 : LinearKernel::s8x8, 1};
   auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((rows_of_w + bn - 1) / bn); };
   auto rounds = [](int64_t workgroups, int64_t at_once) { return (float)((workgroups + at_once - 1) / at_once); };
@@ -582,8 +674,10 @@ LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up) {
   };
   auto stream = [&](LinearKernel kernel, int bm, int bn) {
     if (m > 4096) return;  // (a launch has 65535 tiles of rows)
-    const float loads = rounds(tiles(bm, bn), kCus) * (bm + bn) * k * 2 / 33e3f;
-    consider(kernel, 1, 2.5f + (loads > memory ? loads : memory));
+    const float r = rounds(tiles(bm, bn), kCus);
+    float t = r * (bm + bn) * k * 2 / (aligned ? 33e3f : bm < 64 ? 22e3f : 15e3f);
+    t = t > memory ? t : memory;
+    consider(kernel, 1, 2.5f + t + (aligned ? 0 : 5 * (r - 1)));
   };
   if (!gate_up) stream(LinearKernel::s16x16, 16, 16);
   stream(LinearKernel::s16x32, 16, 32);
@@ -591,6 +685,11 @@ LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up) {
   stream(LinearKernel::s32x64, 32, 64);
   stream(LinearKernel::s64x64, 64, 64);
   const int steps = (k + 63) / 64;
+  if (!aligned) {
+    const float r = rounds(tiles(64, 64), kCus);
+    consider(LinearKernel::any, 1, 3 + 1.2f * r + steps * (0.42f * r > 0.9f ? 0.42f * r : 0.9f));
+    return best;
+  }
   auto tile = [&](LinearKernel kernel, int bm, int bn, float start, float step, float pair) {
     const int64_t of = tiles(bm, bn);
     for (int parts : {1, 2, 3, 4, 6, 8}) {
@@ -618,23 +717,29 @@ hipError_t launch_parts(const LinearArgs& p, hipStream_t stream) {
 
 template <bool GU>
 hipError_t launch_rows(LinearArgs& p, void* workspace, hipStream_t stream) {
-  LinearPlan plan{LinearKernel::any, 1};
-  if (rows_of_16(p)) plan = linear_plan(p.m, (int64_t)p.n * (GU ? 2 : 1), p.k, GU);
+  const bool aligned = rows_of_16(p);
+  const LinearPlan plan = linear_plan(p.m, (int64_t)p.n * (GU ? 2 : 1), p.k, GU, aligned);
   p.parts = plan.parts;
   p.partial = static_cast<float*>(workspace);
+  auto few = [&](auto any) {
+    constexpr bool ANY = decltype(any)::value;
+    switch (plan.kernel) {
+      case LinearKernel::s8x8: if constexpr (!GU) return launch_stream<ANY, 8, 1, 1, 2, GU>(p, stream);
+      case LinearKernel::s8x16: return launch_stream<ANY, 8, 1, 2, 1, GU>(p, stream);
+      case LinearKernel::s16x16: if constexpr (!GU) return launch_stream<ANY, 16, 1, 1, 1, GU>(p, stream);
+      case LinearKernel::s16x32: return launch_stream<ANY, 16, 1, 2, 1, GU>(p, stream);
+      case LinearKernel::s16x64: return launch_stream<ANY, 16, 1, 4, 1, GU>(p, stream);
+      case LinearKernel::s32x64: return launch_stream<ANY, 16, 2, 4, 1, GU>(p, stream);
+      default: return launch_stream<ANY, 16, 4, 4, 1, GU>(p, stream);
+    }
+  };
   switch (plan.kernel) {
-    case LinearKernel::s8x8: if constexpr (!GU) return launch_stream<8, 1, 1, 2, GU>(p, stream);
-    case LinearKernel::s8x16: return launch_stream<8, 1, 2, 1, GU>(p, stream);
-    case LinearKernel::s16x16: if constexpr (!GU) return launch_stream<16, 1, 1, 1, GU>(p, stream);
-    case LinearKernel::s16x32: return launch_stream<16, 1, 2, 1, GU>(p, stream);
-    case LinearKernel::s16x64: return launch_stream<16, 1, 4, 1, GU>(p, stream);
-    case LinearKernel::s32x64: return launch_stream<16, 2, 4, 1, GU>(p, stream);
-    case LinearKernel::s64x64: return launch_stream<16, 4, 4, 1, GU>(p, stream);
     case LinearKernel::t128x128: return launch_parts<Tile128, GU>(p, stream);
     case LinearKernel::t128x128k: return launch_parts<Tile128K, GU>(p, stream);
     case LinearKernel::t256x256: return launch_parts<Tile256, GU>(p, stream);
     case LinearKernel::t128x256: return launch_parts<Tile128x256, GU>(p, stream);
-    default: return launch_any<GU>(p, stream);
+    case LinearKernel::any: return launch_any<GU>(p, stream);
+    default: return aligned ? few(std::false_type{}) : few(std::true_type{});
   }
 }
 
@@ -642,14 +747,14 @@ hipError_t launch_rows(LinearArgs& p, void* workspace, hipStream_t stream) {
 
 size_t linear_workspace_bytes(int64_t m, int n, int k, bool gate_up) {
   const int64_t matrices = gate_up ? 2 : 1;
-  const LinearPlan plan = linear_plan(m, n * matrices, k, gate_up);
+  const LinearPlan plan = linear_plan(m, n * matrices, k, gate_up, true);
   return plan.parts > 1 ? (size_t)(plan.parts * matrices * m * ((n + 3) & ~3)) * 4 : 0;
 }
 
 const char* linear_kernel_name(int64_t m, int n, int k, bool gate_up) {
   static const char* const names[] = {"any",   "8x8",     "8x16",     "16x16",   "16x32",  "16x64",
                                       "32x64", "64x64", "128x128", "128x128x2", "256x256", "128x256"};
-  return names[(int)linear_plan(m, (int64_t)n * (gate_up ? 2 : 1), k, gate_up).kernel];
+  return names[(int)linear_plan(m, (int64_t)n * (gate_up ? 2 : 1), k, gate_up, true).kernel];
 }
 
 hipError_t launch_linear(LinearArgs p, bool gate_up, void* workspace, hipStream_t stream) {

@@ -188,6 +188,18 @@ def test_linear_of_column_ranges(m, k, n, pitch, skip):
     assert (rest == 7.0).all()
 
 
+@pytest.mark.parametrize("k", [*range(1, 20), 63, 64, 65, 127, 129, 513, 1023, 1025])
+@pytest.mark.parametrize("skip", [0, 1, 2, 8])
+def test_linear_of_every_width_and_start(k, skip):
+    """Whole numbers in rows that start at any even byte, between NaN columns, on the
+    kernels for few rows, some and many."""
+    for m, n in ((1, 9), (8, 40), (23, 70), (150, 200), (500, 600)):
+        x, w = whole((m, k + skip), 3, m + k), whole((n, k + skip + 1), 1, n + k)
+        x[:, :skip], w[:, :skip], w[:, k + skip:] = NAN, NAN, NAN
+        x, w = x[:, skip:], w[:, skip:k + skip]
+        assert torch.equal(clef_i4.linear(x, w, dtype=F32).double(), x.double() @ w.double().t()), (m, n)
+
+
 @pytest.mark.parametrize("m,k,n", [(1, 256, 64), (37, 520, 129), (300, 1024, 512)])
 def test_linear_onto_its_residual_and_beside_its_rows(m, k, n):
     x, w, r = randn((m, k), 1.0, 1), randn((n, k), 0.05, 2), randn((m, n), 1.0, 3)
