@@ -156,13 +156,98 @@ struct LinearTile {
   // its first TM / 2 activation fragments, then (Y) the other rows
   static constexpr int Y = A_SLOTS / 2, X = B_SLOTS + A_SLOTS - Y, DMA = X + Y;
   static constexpr int LDS = 2 * STAGE_BYTES;
-  static constexpr int EPI = 16 * WN * 2;  // epilogue staging per wave
   static_assert(NW == 8 && LDS <= 160 * 1024, "eight waves");
   static_assert(A_BYTES % (2048 * NW) == 0 && B_BYTES % (2048 * NW) == 0, "whole instructions per wave");
   static_assert(TM % 2 == 0 && TN % 2 == 0 && TM % KG == 0 && KG <= 2, "step");
-  static_assert(NW * (TM - TM / KG) * TN * 1024 <= LDS && NW * EPI <= LDS, "the groups' sums and rows meet in the stages");
+  static_assert(NW * (TM - TM / KG) * TN * 1024 <= LDS, "the groups' sums meet in the stages");
   static_assert(X <= TM * TN && Y <= 2 * TN, "one DMA instruction per MFMA behind each barrier");
 };
+
+// The epilogue of a wave's EM x TN fragments of 16 x 16 sums (gate/up: the first half of
+// each row of them the gate's, the other the up's): rows w0 .. of the tile's `here`
+// from m0, columns from c0. A lane has four columns of row l % 16 of each fragment.
+template <int EM, int TN, bool GU, bool RESID>
+__device__ __forceinline__ void linear_store_tile(const LinearArgs& p, const v4f (&sum)[EM][TN], int part, int64_t m0,
+                                                  int here, int w0, int c0) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int NC = GU ? TN / 2 : TN;
+  const int lr = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
+  if (p.parts > 1) {
+    constexpr int MATS = GU ? 2 : 1;
+#pragma unroll
+    for (int i = 0; i < EM; ++i) {
+      const int r = w0 + 16 * i + lr;
+      if (r >= here) continue;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int col = c0 + 16 * (j % NC) + 4 * g;
+        if (col < p.n) *reinterpret_cast<v4f*>(linear_partial4(p, part, j / NC, MATS, m0 + r, col)) = sum[i][j];
+      }
+    }
+    return;
+  }
+  v4f bias[NC], bias2[GU ? NC : 1];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    bias[j] = linear_bias4(p.bias, p.bias_f32, c0 + 16 * j + 4 * g, p.n);
+    if constexpr (GU) bias2[j] = linear_bias4(p.bias2, p.bias_f32, c0 + 16 * j + 4 * g, p.n);
+  }
+  // Two fragments side by side (or, of one column of them, one below the other) trade
+  // halves, so that a lane has eight columns of a row, 16 bytes: lanes of even
+  // groups of 16 the first's columns 4 g .., those of odd groups the second's 4 (g -
+  // 1) ..
+  constexpr bool SIDE = NC > 1;
+  auto trade = [](uint2 (&v)[2]) {
+    auto swap = [](uint32_t& x, uint32_t& y) {
+      const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+      x = r[0], y = r[1];
+    };
+    swap(v[0].x, v[1].x);
+    swap(v[0].y, v[1].y);
+  };
+  // row and first column of this lane's eight of the pair (i, j)
+  auto row_of = [&](int i) { return w0 + 16 * i + (SIDE || !(g & 1) ? 0 : 16) + lr; };
+  auto col_of = [&](int j) { return c0 + 16 * j + (SIDE && (g & 1) ? 16 : 0) + 8 * (g >> 1); };
+  constexpr int IS = SIDE ? 1 : 2, JS = SIDE ? 2 : 1;
+#pragma unroll
+  for (int i = 0; i < EM; i += IS)
+#pragma unroll
+    for (int j = 0; j < NC; j += JS) {
+      const int row = row_of(i), col = col_of(j);
+      const bool inside = row < here && col < p.n;
+      uint2 res[2] = {{0, 0}, {0, 0}};
+      if constexpr (RESID) {
+        if (inside) linear_load8(p.residual + (m0 + row) * p.residual_stride + col, p.n - col, res);
+        trade(res);
+      }
+      uint2 out[2];
+      v4f y[2], y2[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int ii = i + (SIDE ? 0 : h), jj = j + (SIDE ? h : 0);
+        y[h] = sum[ii][jj] + bias[jj];
+        if constexpr (GU) y2[h] = sum[ii][jj + NC] + bias2[jj];
+      }
+      linear_act(y, p.act);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (GU) y[h] *= y2[h];
+        if constexpr (RESID) y[h] += v4f{bf16_lo(res[h].x), bf16_hi(res[h].x), bf16_lo(res[h].y), bf16_hi(res[h].y)};
+        out[h] = uint2{pack_bf16x2(y[h][0], y[h][1]), pack_bf16x2(y[h][2], y[h][3])};
+      }
+      if (p.out_f32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = w0 + 16 * (i + (SIDE ? 0 : h)) + lr, c = c0 + 16 * (j + (SIDE ? h : 0)) + 4 * g;
+          if (r < here && c < p.n) linear_store4(p, m0 + r, c, y[h]);
+        }
+        continue;
+      }
+      trade(out);
+      if (inside) linear_store8(static_cast<uint16_t*>(p.out) + (m0 + row) * p.out_stride + col, p.n - col, out);
+    }
+#endif
+}
 
 // Many rows: tiles of BM rows x BN weight rows through two LDS stages filled by
 // DMA, as the FP8 products' (gemm_f8.hip): a stage is filled in two parts, X and Y.
@@ -319,20 +404,11 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(
   };
   body(lds, lds + T::STAGE_BYTES);
 
-  // Epilogue. A lane has four columns of row lr of each fragment; bf16 rows pass
-  // through the wave's own LDS, 16 at a time (16-byte chunk c of row r at c ^ (r &
-  // 7)), and are stored in 16-byte pieces of whole row segments.
   constexpr int EM = TM / T::KG;  // rows of fragments that this wave stores, from fragment kg EM
   constexpr int NC = GU ? TN / 2 : TN;
   const int w0 = wm * T::WM + kg * EM * 16, c0 = n0 + wn * (16 * NC);
-  v4f bias[NC], bias2[GU ? NC : 1];
-#pragma unroll
-  for (int j = 0; j < NC; ++j) {
-    bias[j] = linear_bias4(p.bias, p.bias_f32, c0 + 16 * j + 4 * g, p.n);
-    if constexpr (GU) bias2[j] = linear_bias4(p.bias2, p.bias_f32, c0 + 16 * j + 4 * g, p.n);
-  }
+  // no DMA is on its way into LDS that another workgroup may have next
   wait_vmcnt<0>();
-  __syncthreads();
   v4f sum[EM][TN];
   if constexpr (T::KG == 1) {
 #pragma unroll
@@ -341,6 +417,7 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(
       for (int j = 0; j < TN; ++j) sum[i][j] = acc[i][j];
   } else {
     // two groups: each gives the other its part of the rows that the other stores
+    __syncthreads();
     v4f* const mine = reinterpret_cast<v4f*>(lds) + wave * (EM * TN * 64) + lane;
     const v4f* const theirs = reinterpret_cast<v4f*>(lds) + (wave ^ T::NWB) * (EM * TN * 64) + lane;
 #pragma unroll
@@ -360,64 +437,7 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(
       for (int j = 0; j < TN; ++j) sum[i][j] += theirs[(i * TN + j) * 64];
     __syncthreads();
   }
-  if (p.parts > 1) {
-    constexpr int MATS = GU ? 2 : 1;
-#pragma unroll
-    for (int i = 0; i < EM; ++i) {
-      const int r = w0 + 16 * i + lr;
-      if (r >= here) continue;
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int col = c0 + 16 * (j % NC) + 4 * g;
-        if (col < p.n) *reinterpret_cast<v4f*>(linear_partial4(p, part, j / NC, MATS, m0 + r, col)) = sum[i][j];
-      }
-    }
-    return;
-  }
-  constexpr int ROW = 32 * NC, CH = 2 * NC, PER = 64 / CH;  // bytes and chunks of a row, rows per store
-  char* own = lds + wave * T::EPI;
-#pragma unroll
-  for (int i = 0; i < EM; ++i) {
-    const int r0 = w0 + 16 * i;
-    v4f res[NC];
-    if constexpr (RESID) {
-#pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        res[j] = v4f{0, 0, 0, 0};
-        if (r0 + lr < here) res[j] = linear_residual4(p, m0 + r0 + lr, c0 + 16 * j + 4 * g);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      v4f y = linear_finish4<GU>(p, sum[i][j], bias[j], sum[i][GU ? j + NC : j], bias2[GU ? j : 0]);
-      if constexpr (RESID) y += res[j];
-      if (p.out_f32) {
-        if (r0 + lr < here) linear_store4(p, m0 + r0 + lr, c0 + 16 * j + 4 * g, y);
-        continue;
-      }
-      const int chunk = 2 * j + (g >> 1);
-      *reinterpret_cast<uint2*>(own + lr * ROW + ((chunk ^ (lr & (CH - 1))) << 4) + 8 * (g & 1)) =
-          uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-    }
-    if (p.out_f32) continue;
-#pragma unroll
-    for (int q = 0; q < (16 + PER - 1) / PER; ++q) {
-      const int r = q * PER + lane / CH, chunk = lane % CH, col = c0 + 8 * chunk;
-      if (PER > 16 && r >= 16) continue;
-      const uint4 v = *reinterpret_cast<const uint4*>(own + r * ROW + ((chunk ^ (r & (CH - 1))) << 4));
-      if (r0 + r >= here || col >= p.n) continue;
-      uint16_t* to = static_cast<uint16_t*>(p.out) + (m0 + r0 + r) * p.out_stride + col;
-      if (col + 8 <= p.n) {
-        __builtin_memcpy(to, &v, 16);
-      } else {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int t = 0; t < 7; ++t)
-          if (col + t < p.n) to[t] = (uint16_t)(w[t / 2] >> (16 * (t % 2)));
-      }
-    }
-    asm volatile("" ::: "memory");
-  }
+  linear_store_tile<EM, TN, GU, RESID>(p, sum, part, m0, here, w0, c0);
 #endif
 }
 
@@ -675,7 +695,7 @@ LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up, bool a
   auto stream = [&](LinearKernel kernel, int bm, int bn) {
     if (m > 4096) return;  // (a launch has 65535 tiles of rows)
     const float r = rounds(tiles(bm, bn), kCus);
-    float t = r * (bm + bn) * k * 2 / (aligned ? 33e3f : bm < 64 ? 22e3f : 15e3f);
+    float t = r * (bm + bn) * k * 2 / (aligned ? 33e3f : 22e3f);
     t = t > memory ? t : memory;
     consider(kernel, 1, 2.5f + t + (aligned ? 0 : 5 * (r - 1)));
   };
@@ -683,7 +703,7 @@ LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up, bool a
   stream(LinearKernel::s16x32, 16, 32);
   stream(LinearKernel::s16x64, 16, 64);
   stream(LinearKernel::s32x64, 32, 64);
-  stream(LinearKernel::s64x64, 64, 64);
+  if (aligned) stream(LinearKernel::s64x64, 64, 64);  // (64 rows of AnyRow do not fit the registers)
   const int steps = (k + 63) / 64;
   if (!aligned) {
     const float r = rounds(tiles(64, 64), kCus);
@@ -729,8 +749,8 @@ hipError_t launch_rows(LinearArgs& p, void* workspace, hipStream_t stream) {
       case LinearKernel::s16x16: if constexpr (!GU) return launch_stream<ANY, 16, 1, 1, 1, GU>(p, stream);
       case LinearKernel::s16x32: return launch_stream<ANY, 16, 1, 2, 1, GU>(p, stream);
       case LinearKernel::s16x64: return launch_stream<ANY, 16, 1, 4, 1, GU>(p, stream);
-      case LinearKernel::s32x64: return launch_stream<ANY, 16, 2, 4, 1, GU>(p, stream);
-      default: return launch_stream<ANY, 16, 4, 4, 1, GU>(p, stream);
+      case LinearKernel::s64x64: if constexpr (!ANY) return launch_stream<ANY, 16, 4, 4, 1, GU>(p, stream);
+      default: return launch_stream<ANY, 16, 2, 4, 1, GU>(p, stream);
     }
   };
   switch (plan.kernel) {

@@ -81,17 +81,27 @@ __device__ __forceinline__ float gelu_f32(float v) {
   return v * (v < 0.0f ? q : 1.0f - q);
 }
 
-// One value; `act` is uniform. NaN stays NaN (relu too).
-__device__ __forceinline__ float linear_act(float v, int act) {
-  switch (act) {
-    case kActRelu: return v < 0.0f ? 0.0f : v;
-    case kActGelu: return gelu_f32(v);
-    // 0.5 v (1 + tanh(z)) = v sigmoid(2 z), z = sqrt(2 / pi) (v + 0.044715 v^3)
-    case kActGeluTanh: return v * sigmoid_f32(v * __builtin_fmaf(v * v, 0.0713548162726f, 1.59576912160573f));
-    case kActSilu: return v * sigmoid_f32(v);
-    case kActSigmoid: return sigmoid_f32(v);
-    default: return v;
-  }
+// Of every value; `act` is uniform. A tile's epilogue holds the bodies once per eight
+// values, so the last three share one: v or 1 times sigmoid(v (a + b v^2)), b = 0 but
+// for the tanh form of GELU, 0.5 v (1 + tanh(z)) = v sigmoid(2 z) with z = sqrt(2 /
+// pi) (v + 0.044715 v^3). NaN stays NaN (ReLU too).
+template <int N>
+__device__ __forceinline__ void linear_act(v4f (&y)[N], int act) {
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) y[i][t] = f(y[i][t]);
+  };
+  if (act == kActNone) return;
+  if (act == kActGelu) return each([](float v) { return gelu_f32(v); });
+  if (act == kActRelu) return each([](float v) { return v < 0.0f ? 0.0f : v; });
+  const float a = act == kActGeluTanh ? 1.59576912160573f : 1.0f, b = act == kActGeluTanh ? 0.0713548162726f : 0.0f;
+  each([=](float v) {
+    const float square = __builtin_fminf(v * v, 1e30f);  // (0 times infinity)
+    const float s = sigmoid_f32(v * __builtin_fmaf(square, b, a));
+    return act == kActSigmoid ? s : v * s;
+  });
 }
 
 // Columns col .. + 3 of a bias, and of a residual row: loads of any alignment
@@ -122,6 +132,31 @@ __device__ __forceinline__ v4f linear_bias4(const void* bias, bool f32, int col,
   return v4f{bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)};
 }
 
+// Eight bf16 of which `left` are inside the row (those past it are zeros; not stored).
+__device__ __forceinline__ void linear_load8(const uint16_t* from, int left, uint2 (&v)[2]) {
+  if (left >= 8) {
+    __builtin_memcpy(v, from, 16);
+    return;
+  }
+  uint32_t w[4] = {};
+#pragma unroll
+  for (int t = 0; t < 7; ++t)
+    if (t < left) w[t / 2] |= (uint32_t)from[t] << (16 * (t % 2));
+  v[0] = uint2{w[0], w[1]};
+  v[1] = uint2{w[2], w[3]};
+}
+
+__device__ __forceinline__ void linear_store8(uint16_t* to, int left, const uint2 (&v)[2]) {
+  if (left >= 8) {
+    __builtin_memcpy(to, v, 16);
+    return;
+  }
+  const uint32_t w[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
+#pragma unroll
+  for (int t = 0; t < 7; ++t)
+    if (t < left) to[t] = (uint16_t)(w[t / 2] >> (16 * (t % 2)));
+}
+
 __device__ __forceinline__ v4f linear_residual4(const LinearArgs& p, int64_t row, int col) {
   return linear_bias4(p.residual + row * p.residual_stride, false, col, p.n);
 }
@@ -129,11 +164,10 @@ __device__ __forceinline__ v4f linear_residual4(const LinearArgs& p, int64_t row
 // act(y + bias), and the product with the up sums for gate/up.
 template <bool GU>
 __device__ __forceinline__ v4f linear_finish4(const LinearArgs& p, v4f y, v4f bias, v4f y2, v4f bias2) {
-  y += bias;
-#pragma unroll
-  for (int t = 0; t < 4; ++t) y[t] = linear_act(y[t], p.act);
-  if constexpr (GU) y *= y2 + bias2;
-  return y;
+  v4f v[1] = {y + bias};
+  linear_act(v, p.act);
+  if constexpr (GU) v[0] *= y2 + bias2;
+  return v[0];
 }
 
 // Columns col .. + 3 of an output row, any alignment, those past the last left out.
