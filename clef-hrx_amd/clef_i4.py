@@ -153,7 +153,7 @@ def _check(rc: int) -> None:
 
 class _Native:
     """The call module (csrc/host_call.cpp: launch, value, pointer, holds, empty,
-    matrix) and its handle of every entry point, as attributes; filled on first use."""
+    matrix, linear, linear_gate_up) and its handle of every entry point, as attributes; filled on first use."""
 
     def __getattr__(self, name):
         handle = lib()
@@ -168,7 +168,7 @@ class _Native:
                                    "".join("p" if a is _P else "i" for a in args))
                  for entry, (_, args) in SIGNATURES.items()}
         found.update(launch=host.launch, value=host.value, pointer=host.pointer, holds=host.holds, empty=host.empty,
-                     matrix=host.matrix)
+                     matrix=host.matrix, linear=host.linear, linear_gate_up=host.linear_gate_up)
         if name not in found:
             raise AttributeError(name)
         self.__dict__.update(found)
@@ -1228,7 +1228,7 @@ ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "sigmoi
 _BAD_LINEAR = "linear shape/dtype mismatch"
 
 
-def _linear_rows(t: torch.Tensor, cols: int, device: int) -> int:
+def _check_linear_rows(t: torch.Tensor, cols: int, device: int) -> int:
     """Row pitch of bf16 rows of `cols` contiguous elements on the current
     device: a matrix, or a column range of a wider one."""
     if t.dim() != 2 or t.dtype != torch.bfloat16 or t.shape[1] != cols:
@@ -1242,43 +1242,35 @@ def _linear_rows(t: torch.Tensor, cols: int, device: int) -> int:
     return t.stride(0) if t.shape[0] > 1 else cols
 
 
-def _linear_bias(bias: torch.Tensor | None, n: int, device: int):
-    """(address, dtype) of a bias of n values."""
-    if bias is None:
-        return None, 0
-    if bias.dtype not in (torch.bfloat16, torch.float32) or tuple(bias.shape) != (n,):
-        raise ClefError(-1, _BAD_LINEAR)
-    if bias.get_device() != device:
-        raise ClefError(-1, _ELSEWHERE)
-    return bias, int(bias.dtype == torch.float32)
-
-
-def _linear_out(like: torch.Tensor, rows: int, cols: int, out: torch.Tensor | None, dtype, device: int):
-    """The output and its row pitch."""
-    if out is None:
-        return _n.empty(like, dtype, rows, cols), cols
-    if tuple(out.shape) != (rows, cols) or out.dtype != dtype:
-        raise ClefError(-1, "output shape/dtype mismatch")
-    if out.get_device() != device:
-        raise ClefError(-1, _ELSEWHERE)
-    if out.is_contiguous():
-        return out, cols
-    if (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
-        raise ClefError(-1, "output shape/dtype mismatch")
-    return out, out.stride(0) if rows > 1 else cols
-
-
-def _linear_scratch(like: torch.Tensor, m: int, n: int, k: int, gate_up: int):
-    """(workspace, bytes) of a product; few rows need none."""
-    nbytes = _n.value(_n.clef_linear_workspace_bytes, m, n, k, gate_up) if m > 8 else 0
-    return (_n.empty(like, torch.uint8, nbytes), nbytes) if nbytes > 0 else (None, 0)
-
-
-def _activation_code(activation: str | None) -> int:
-    code = ACTIVATIONS.get(activation)
-    if code is None:
+def _refuse_linear(x, weights, biases, residual, out, dtype, activation) -> None:
+    """What is wrong with a product's operands, which the call module did not take."""
+    device = torch._C._cuda_getDevice()
+    if activation not in ACTIVATIONS:
         raise ClefError(-1, "unknown activation")
-    return code
+    if any(w.dim() != 2 or w.shape != weights[0].shape for w in weights):
+        raise ClefError(-1, _BAD_LINEAR)
+    n, k = weights[0].shape
+    _check_linear_rows(x, k, device)
+    if len({_check_linear_rows(w, k, device) for w in weights}) > 1:
+        raise ClefError(-1, _BAD_LINEAR)  # rows of different pitch
+    for bias in biases:
+        if bias is None:
+            continue
+        if bias.dtype not in (torch.bfloat16, torch.float32) or tuple(bias.shape) != (n,):
+            raise ClefError(-1, _BAD_LINEAR)
+        if bias.get_device() != device:
+            raise ClefError(-1, _ELSEWHERE)
+        if not bias.is_contiguous():
+            raise ClefError(-1, "linear bias must be contiguous")
+    if residual is not None:
+        if residual.shape[0] != x.shape[0]:
+            raise ClefError(-1, "residual shape/dtype mismatch")
+        _check_linear_rows(residual, n, device)
+    if dtype not in (None, torch.bfloat16, torch.float32):
+        raise ClefError(-1, _BAD_LINEAR)
+    if out is not None and out.get_device() != device and tuple(out.shape) == (x.shape[0], n):
+        raise ClefError(-1, _ELSEWHERE)
+    raise ClefError(-1, "output shape/dtype mismatch" if out is not None else _BAD_LINEAR)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
@@ -1291,29 +1283,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     [n] bf16 or f32, residual bf16, activation one of ACTIVATIONS. x, weight,
     residual and out may be column ranges of wider rows; out may be the residual
     itself."""
-    if weight.dim() != 2:
-        raise ClefError(-1, _BAD_LINEAR)
-    n, k = weight.shape
-    device = torch._C._cuda_getDevice()
-    x_pitch, w_pitch = _linear_rows(x, k, device), _linear_rows(weight, k, device)
-    bias, bias_dtype = _linear_bias(bias, n, device)
-    m = x.shape[0]
-    if dtype is None:
-        dtype = torch.bfloat16 if out is None else out.dtype
-    if dtype is not torch.bfloat16 and dtype is not torch.float32:
-        raise ClefError(-1, _BAD_LINEAR)
-    residual_pitch = n
-    if residual is not None:
-        if residual.shape[0] != m:
-            raise ClefError(-1, "residual shape/dtype mismatch")
-        residual_pitch = _linear_rows(residual, n, device)
-        residual = residual.data_ptr()
-    code = _activation_code(activation)
-    out, out_pitch = _linear_out(x, m, n, out, dtype, device)
-    _n.launch(_n.clef_linear, x.data_ptr(), m, k, x_pitch, weight.data_ptr(), n, w_pitch, bias, bias_dtype, code,
-              residual, residual_pitch, out.data_ptr(), int(dtype is torch.float32), out_pitch,
-              *_linear_scratch(x, m, n, k, 0))
-    return out
+    y = _n.linear(_n.clef_linear, _n.clef_linear_workspace_bytes, x, weight, bias, ACTIVATIONS.get(activation, -1),
+                  residual, out, dtype)
+    if y is None:
+        _refuse_linear(x, (weight,), (bias,), residual, out, dtype, activation)
+    return y
 
 
 def linear_gate_up(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, activation: str | None = "silu",
@@ -1322,21 +1296,8 @@ def linear_gate_up(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, activa
     """h = act(x @ gate.T + gate_bias) * (x @ up.T + up_bias) on weights that
     stay bf16, in one product (clef_linear_gate_up): bf16 [rows][gate.shape[0]],
     rounded once. Operands as in linear; the biases are of one type."""
-    if gate.dim() != 2 or gate.shape != up.shape:
-        raise ClefError(-1, _BAD_LINEAR)
-    n, k = gate.shape
-    device = torch._C._cuda_getDevice()
-    x_pitch, w_pitch = _linear_rows(x, k, device), _linear_rows(gate, k, device)
-    if _linear_rows(up, k, device) != w_pitch:
-        raise ClefError(-1, _BAD_LINEAR)
-    if gate_bias is not None and up_bias is not None and gate_bias.dtype != up_bias.dtype:
-        raise ClefError(-1, _BAD_LINEAR)
-    gate_bias, bias_dtype = _linear_bias(gate_bias, n, device)
-    up_bias, up_dtype = _linear_bias(up_bias, n, device)
-    code = _activation_code(activation)
-    m = x.shape[0]
-    out, out_pitch = _linear_out(x, m, n, out, torch.bfloat16, device)
-    _n.launch(_n.clef_linear_gate_up, x.data_ptr(), m, k, x_pitch, gate.data_ptr(), up.data_ptr(), n, w_pitch,
-              gate_bias, up_bias, bias_dtype | up_dtype, code, out.data_ptr(), out_pitch,
-              *_linear_scratch(x, m, n, k, 1))
-    return out
+    h = _n.linear_gate_up(_n.clef_linear_gate_up, _n.clef_linear_workspace_bytes, x, gate, up,
+                          ACTIVATIONS.get(activation, -1), gate_bias, up_bias, out)
+    if h is None:
+        _refuse_linear(x, (gate, up), (gate_bias, up_bias), None, out, torch.bfloat16, activation)
+    return h

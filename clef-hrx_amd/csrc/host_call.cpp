@@ -15,6 +15,12 @@
 //   holds(device, tensor, dtype, count, ..): whether each is a contiguous tensor of
 //     that dtype and at least count elements on that device (-1: the host).
 //   empty(like, dtype, *sizes): torch.empty on like's device.
+//   linear(entry, bytes_entry, x, weight, bias, activation, residual, out, dtype):
+//     clef_linear with its workspace and output, the output returned; None, and
+//     nothing done, unless every operand is as the entry takes it (the caller
+//     finds out what is wrong).
+//   linear_gate_up(entry, bytes_entry, x, gate, up, activation, gate_bias, up_bias,
+//     out): clef_linear_gate_up likewise.
 //   matrix(buffer, dtype, byte, rows, cols, row_step, col_step): a 2-d tensor of
 //     dtype on buffer's memory from its byte `byte`, steps in elements; bounds
 //     and alignment checked. (torch's view and as_strided take 1.4 us each.)
@@ -229,6 +235,172 @@ PyObject* empty(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The operands of the bf16 products. Each function gives false for what the C entry
+// would not take.
+struct Rows {
+  int64_t at = 0, rows = 0, cols = 0, pitch = 0;
+};
+
+// Rows of contiguous elements of `type` on `device`, a matrix or a column range of one.
+bool rows_of(PyObject* o, at::ScalarType type, int64_t device, Rows& r) {
+  if (!THPVariable_Check(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.dim() != 2 || t.scalar_type() != type || !t.is_cuda() || t.get_device() != device) return false;
+  r.rows = t.size(0), r.cols = t.size(1);
+  r.at = reinterpret_cast<int64_t>(t.data_ptr());
+  r.pitch = r.rows > 1 && !t.is_contiguous() ? t.stride(0) : r.cols;
+  return t.is_contiguous() || ((r.cols <= 1 || t.stride(1) == 1) && r.pitch >= r.cols);
+}
+
+// A bias of n values, or none.
+bool bias_of(PyObject* o, int64_t n, int64_t device, int64_t& at, int64_t& f32) {
+  at = f32 = 0;
+  if (o == Py_None) return true;
+  if (!THPVariable_Check(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  f32 = t.scalar_type() == at::kFloat;
+  at = reinterpret_cast<int64_t>(t.data_ptr());
+  return (f32 || t.scalar_type() == at::kBFloat16) && t.dim() == 1 && t.size(0) == n && t.is_cuda() &&
+         t.get_device() == device && t.is_contiguous();
+}
+
+at::Tensor empty_like(PyObject* o, at::ScalarType type, at::IntArrayRef sizes) {
+  pybind11::gil_scoped_release no_gil;
+  return at::empty(sizes, at::TensorOptions().device(THPVariable_Unpack(o).device()).dtype(type));
+}
+
+bool current(int64_t& device, int64_t& stream) {
+  PyObject* d = PyObject_CallNoArgs(g_device);
+  if (d == nullptr) return false;
+  device = PyLong_AsLongLong(d);
+  PyObject* s = PyObject_CallOneArg(g_raw_stream, d);
+  Py_DECREF(d);
+  if (s == nullptr) return false;
+  const bool ok = convert(s, true, stream);
+  Py_DECREF(s);
+  return ok;
+}
+
+// The entry with v's arguments, workspace, its bytes and the stream behind them; the
+// status to the function given to set_check.
+bool call_with_workspace(const Entry* entry, const Entry* bytes_entry, PyObject* like, int64_t m, int64_t n, int64_t k,
+                         int64_t gate_up, int64_t* v, size_t args, int64_t stream) {
+  at::Tensor scratch;
+  v[args] = v[args + 1] = 0;
+  if (m > 8) {  // few rows need none
+    const int64_t sizes[] = {m, n, k, gate_up};
+    const int64_t bytes = pick(4, std::make_index_sequence<kMaxArgs + 1>{})(bytes_entry->f, sizes);
+    if (bytes > 0) {
+      scratch = empty_like(like, at::kByte, bytes);
+      v[args] = reinterpret_cast<int64_t>(scratch.data_ptr());
+      v[args + 1] = bytes;
+    }
+  }
+  v[args + 2] = stream;
+  const Invoker call = pick(args + 3, std::make_index_sequence<kMaxArgs + 1>{});
+  int32_t rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = static_cast<int32_t>(call(entry->f, v));
+  Py_END_ALLOW_THREADS
+  if (rc == 0) return true;
+  PyObject* r = PyObject_CallFunction(g_check, "i", rc);
+  Py_XDECREF(r);
+  return r != nullptr;
+}
+
+// args[0] and args[1] as handles, args[at] as an activation's code.
+bool linear_entries(PyObject* const* args, Py_ssize_t n, Py_ssize_t at, const Entry*& entry, const Entry*& bytes_entry,
+                    int64_t& activation) {
+  if (n != 9) {
+    PyErr_SetString(PyExc_TypeError, "two entries and seven arguments expected");
+    return false;
+  }
+  entry = static_cast<const Entry*>(PyLong_AsVoidPtr(args[0]));
+  bytes_entry = entry != nullptr ? static_cast<const Entry*>(PyLong_AsVoidPtr(args[1])) : nullptr;
+  if (bytes_entry == nullptr) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "no entry");
+    return false;
+  }
+  activation = PyLong_AsLongLong(args[at]);
+  return activation != -1 || !PyErr_Occurred();
+}
+
+PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Entry *entry, *bytes_entry;
+  int64_t act, device, stream, v[kMaxArgs];
+  if (!linear_entries(args, n, 5, entry, bytes_entry, act) || !current(device, stream)) return nullptr;
+  if (act < 0) Py_RETURN_NONE;
+  PyObject *const x = args[2], *const weight = args[3], *const residual = args[6], *const out = args[7], *const dtype = args[8];
+  Rows rx, rw, rr, ro;
+  int64_t bias, bias_f32;
+  if (!rows_of(x, at::kBFloat16, device, rx) || !rows_of(weight, at::kBFloat16, device, rw) || rx.cols != rw.cols ||
+      !bias_of(args[4], rw.rows, device, bias, bias_f32))
+    Py_RETURN_NONE;
+  rr.pitch = rw.rows;
+  if (residual != Py_None &&
+      (!rows_of(residual, at::kBFloat16, device, rr) || rr.rows != rx.rows || rr.cols != rw.rows))
+    Py_RETURN_NONE;
+  at::ScalarType type = at::kBFloat16;
+  if (dtype != Py_None) {
+    if (!THPDtype_Check(dtype)) Py_RETURN_NONE;
+    type = reinterpret_cast<THPDtype*>(dtype)->scalar_type;
+  } else if (out != Py_None && THPVariable_Check(out)) {
+    type = THPVariable_Unpack(out).scalar_type();
+  }
+  if (type != at::kBFloat16 && type != at::kFloat) Py_RETURN_NONE;
+  at::Tensor made;
+  if (out == Py_None) {
+    const int64_t sizes[] = {rx.rows, rw.rows};
+    made = empty_like(x, type, at::IntArrayRef(sizes, 2));
+    ro.at = reinterpret_cast<int64_t>(made.data_ptr()), ro.pitch = rw.rows;
+  } else if (!rows_of(out, type, device, ro) || ro.rows != rx.rows || ro.cols != rw.rows) {
+    Py_RETURN_NONE;
+  }
+  const int64_t given[] = {rx.at, rx.rows, rx.cols,  rx.pitch, rw.at,              rw.rows, rw.pitch, bias, bias_f32,
+                           act,   rr.at,   rr.pitch, ro.at,    type == at::kFloat, ro.pitch};
+  constexpr size_t count = sizeof(given) / sizeof(*given);
+  std::memcpy(v, given, sizeof(given));
+  if (!call_with_workspace(entry, bytes_entry, x, rx.rows, rw.rows, rx.cols, 0, v, count, stream)) return nullptr;
+  if (made.defined()) return THPVariable_Wrap(std::move(made));
+  Py_INCREF(out);
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* linear_gate_up(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Entry *entry, *bytes_entry;
+  int64_t act, device, stream, v[kMaxArgs];
+  if (!linear_entries(args, n, 5, entry, bytes_entry, act) || !current(device, stream)) return nullptr;
+  if (act < 0) Py_RETURN_NONE;
+  PyObject *const x = args[2], *const out = args[8];
+  Rows rx, rg, ru, ro;
+  int64_t gate_bias, gate_f32, up_bias, up_f32;
+  if (!rows_of(x, at::kBFloat16, device, rx) || !rows_of(args[3], at::kBFloat16, device, rg) ||
+      !rows_of(args[4], at::kBFloat16, device, ru) || rx.cols != rg.cols || rg.rows != ru.rows || rg.cols != ru.cols ||
+      rg.pitch != ru.pitch || !bias_of(args[6], rg.rows, device, gate_bias, gate_f32) ||
+      !bias_of(args[7], rg.rows, device, up_bias, up_f32) || (gate_bias != 0 && up_bias != 0 && gate_f32 != up_f32))
+    Py_RETURN_NONE;
+  at::Tensor made;
+  if (out == Py_None) {
+    const int64_t sizes[] = {rx.rows, rg.rows};
+    made = empty_like(x, at::kBFloat16, at::IntArrayRef(sizes, 2));
+    ro.at = reinterpret_cast<int64_t>(made.data_ptr()), ro.pitch = rg.rows;
+  } else if (!rows_of(out, at::kBFloat16, device, ro) || ro.rows != rx.rows || ro.cols != rg.rows) {
+    Py_RETURN_NONE;
+  }
+  const int64_t given[] = {rx.at,    rx.rows,   rx.cols, rx.pitch,          rg.at, ru.at, rg.rows,
+                           rg.pitch, gate_bias, up_bias, gate_f32 | up_f32, act,   ro.at, ro.pitch};
+  constexpr size_t count = sizeof(given) / sizeof(*given);
+  std::memcpy(v, given, sizeof(given));
+  if (!call_with_workspace(entry, bytes_entry, x, rx.rows, rg.rows, rx.cols, 1, v, count, stream)) return nullptr;
+  if (made.defined()) return THPVariable_Wrap(std::move(made));
+  Py_INCREF(out);
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* matrix(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 7 || !THPVariable_Check(args[0]) || !THPDtype_Check(args[1])) {
@@ -278,6 +450,8 @@ PyMethodDef methods[] = {
     {"holds", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&holds)), METH_FASTCALL, nullptr},
     {"empty", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&empty)), METH_FASTCALL, nullptr},
     {"matrix", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&matrix)), METH_FASTCALL, nullptr},
+    {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&linear)), METH_FASTCALL, nullptr},
+    {"linear_gate_up", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&linear_gate_up)), METH_FASTCALL, nullptr},
     {"set_check", &set_check, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
