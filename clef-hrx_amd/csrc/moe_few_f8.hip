@@ -33,12 +33,9 @@ struct FewTable {
 
 // Routing of all tokens, in LDS of each workgroup of 512 threads, by expert.
 struct FewRoutes {
-  float p[kTokens][kMaxExperts];       // the probability
+  float p[kTokens][kMaxExperts];  // the probability
   uint8_t rank[kTokens][kMaxExperts];
-  uint32_t tokens[kMaxExperts];        // the tokens that name it
-  // more than 16 ranks: the chosen logits and their experts by rank
-  float v[kTokens][kMaxExperts];
-  uint8_t id[kTokens][kMaxExperts];
+  uint32_t tokens[kMaxExperts];   // the tokens that name it
 };
 
 // The experts named, one bit each, in scalar registers of every wave.
@@ -54,97 +51,114 @@ struct FewNamed {
   }
 };
 
-// (equal ones first: infinities have no difference)
-__device__ __forceinline__ float few_exp(float v, float best) {
-  return v == -__builtin_huge_valf() ? 0.0f : v == best ? 1.0f : __builtin_amdgcn_exp2f((v - best) * 1.44269504088896341f);
+// Workgroup barrier behind this wave's LDS accesses alone: global loads stay on
+// their way (__syncthreads would wait for them).
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// f32 as integers of the same order, and back. Zeros are one number (v + 0); logits
+// that take no part are the least of all.
+constexpr int kNoLogit = (int)0x80000000u;
+__device__ __forceinline__ int few_key(float v) {
+  const int bits = (int)as_uint(v + 0.0f), key = bits ^ (bits >> 31 & 0x7FFFFFFF);
+  return v > -__builtin_huge_valf() ? key : kNoLogit;  // (NaN too)
+}
+__device__ __forceinline__ float few_value(int key) { return as_float((uint32_t)(key ^ (key >> 31 & 0x7FFFFFFF))); }
+
+__device__ __forceinline__ int few_row_max(int v) {
+  auto larger = [](int x, int y) { return x > y ? x : y; };
+  v = larger(v, route_impl::dpp_row<0xB1>(v));
+  v = larger(v, route_impl::dpp_row<0x4E>(v));
+  v = larger(v, route_impl::dpp_row<0x124>(v));
+  return larger(v, route_impl::dpp_row<0x128>(v));
+}
+__device__ __forceinline__ float few_row_sum(float v) {
+  auto turned = [](float x, auto ctrl) {
+    return as_float((uint32_t)route_impl::dpp_row<decltype(ctrl)::value>((int)as_uint(x)));
+  };
+  v += turned(v, std::integral_constant<int, 0xB1>{});
+  v += turned(v, std::integral_constant<int, 0x4E>{});
+  v += turned(v, std::integral_constant<int, 0x124>{});
+  return v + turned(v, std::integral_constant<int, 0x128>{});
 }
 
-__device__ __forceinline__ void few_choose(FewRoutes& r, int t, int k, int id, float p) {
-  if (!(p > 0.0f)) return;
-  r.p[t][id] = p;
-  r.rank[t][id] = (uint8_t)k;
-  atomicOr(&r.tokens[id], 1u << t);
-}
-
-// 16 lanes (a DPP row) take a token, 8 experts each, through topk rounds of "the
-// largest logit left, the lowest id that has it"; lane k keeps rank k. Logits of -inf
-// and NaN take no part, nor does a probability that is zero: a token may name fewer
-// than topk experts, or none.
+// A wave takes a token (and the eighth behind it), its lanes two experts each,
+// through topk rounds of "the largest logit left, the lowest id that has it", the
+// maximum and the id as scalars; lane k % 64 keeps rank k. Logits of -inf and NaN take
+// no part, nor does a probability that is zero: a token may name fewer than topk
+// experts, or none.
 __device__ __forceinline__ FewNamed few_route(const MoeFewArgs& a, FewRoutes& r) {
-  const int tid = threadIdx.x, experts = a.experts, topk = a.topk;
-  constexpr float none = -__builtin_huge_valf();
-  const int t = tid >> 4, li = tid & 15, e0 = 8 * li;
-  const bool routes = tid < 64 * ((a.tokens + 3) / 4);  // whole waves
-  const bool wide = topk > 16;
-  if (tid < kMaxExperts) r.tokens[tid] = 0;
-  float mine = none;
-  int mine_id = 0;
-  if (routes) {
-    // all loads at once, past the end zeros
-    const int first = t * experts + e0;
-    uint32_t bits[8];
-    if (a.logits_f32) {
-      const __amdgpu_buffer_rsrc_t lr = make_rsrc(a.logits, (uint32_t)(a.tokens * experts * 4));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), experts = a.experts;
+  constexpr int PER = kTokens / 8;
+  uint32_t bits[PER][2];  // past the last expert or token: of another, not used
+  const int logits = a.tokens * experts;
+  if (a.logits_f32) {
+    const __amdgpu_buffer_rsrc_t lr = make_rsrc(a.logits, (uint32_t)logits * 4);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) bits[j] = __builtin_amdgcn_raw_buffer_load_b32(lr, (first + j) * 4, 0, 0);
-    } else {
-      const __amdgpu_buffer_rsrc_t lr = make_rsrc(a.logits, (uint32_t)(a.tokens * experts * 2));
+    for (int n = 0; n < PER; ++n)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) bits[j] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(lr, (first + j) * 2, 0, 0) << 16;
-    }
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float l = as_float(bits[j]);
-      v[j] = t < a.tokens && e0 + j < experts && l == l ? l : none;
-    }
-    for (int k = 0; k < topk; ++k) {
-      float m = v[0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) m = __builtin_fmaxf(m, v[j]);
-      const float best = route_impl::row_max(m);
-      int of = route_impl::kInvalidId;
-#pragma unroll
-      for (int j = 7; j >= 0; --j)
-        if (v[j] == best) of = e0 + j;
-      const int id = route_impl::row_min(of);  // (past the last finite logit: not used)
-      if (wide && li == 0) {
-        r.v[t][k] = best;
-        r.id[t][k] = (uint8_t)id;
-      }
-      if (li == k) {
-        mine = best;
-        mine_id = id;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (id == e0 + j) v[j] = none;
-    }
-  }
-  __syncthreads();
-  if (!wide) {
-    if (routes) {
-      // lane 0 holds the largest; the sum over the row (lanes past the last rank: 0)
-      const float e = few_exp(mine, as_float((uint32_t)__builtin_amdgcn_ds_swizzle((int)as_uint(mine), 0x10)));
-      float sum = e;
-      sum += as_float((uint32_t)route_impl::dpp_row<0xB1>((int)as_uint(sum)));
-      sum += as_float((uint32_t)route_impl::dpp_row<0x4E>((int)as_uint(sum)));
-      sum += as_float((uint32_t)route_impl::dpp_row<0x124>((int)as_uint(sum)));
-      sum += as_float((uint32_t)route_impl::dpp_row<0x128>((int)as_uint(sum)));
-      few_choose(r, t, li, mine_id, e / sum);
-    }
+      for (int s = 0; s < 2; ++s)
+        bits[n][s] = __builtin_amdgcn_raw_buffer_load_b32(lr, ((wave + 8 * n) * experts + 64 * s + lane) * 4, 0, 0);
   } else {
-    const int ranks = a.tokens * topk;
-    for (int i = tid; i < ranks; i += 512) {
-      const int of = i / topk, k = i % topk;
-      const float best = r.v[of][0];
-      float sum = 0.0f;
-      for (int o = 0; o < topk; ++o) sum += few_exp(r.v[of][o], best);
-      few_choose(r, of, k, r.id[of][k], few_exp(r.v[of][k], best) / sum);
+    const __amdgpu_buffer_rsrc_t lr = make_rsrc(a.logits, (uint32_t)logits * 2);
+#pragma unroll
+    for (int n = 0; n < PER; ++n)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        bits[n][s] =
+            (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(lr, ((wave + 8 * n) * experts + 64 * s + lane) * 2, 0, 0) << 16;
+  }
+  if (threadIdx.x < kMaxExperts) r.tokens[threadIdx.x] = 0;
+  lds_barrier();
+  for (int n = 0; n < PER; ++n) {
+    const int t = wave + 8 * n;
+    if (t >= a.tokens) break;
+    int key[2], mine[2] = {kNoLogit, kNoLogit}, id[2] = {0, 0}, first = kNoLogit;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) key[s] = 64 * s + lane < experts ? few_key(as_float(bits[n][s])) : kNoLogit;
+    for (int k = 0; k < a.topk; ++k) {
+      const int row = few_row_max(key[0] > key[1] ? key[0] : key[1]);
+      int best = __builtin_amdgcn_readlane(row, 0);
+#pragma unroll
+      for (int l = 16; l < 64; l += 16) {
+        const int other = __builtin_amdgcn_readlane(row, l);
+        best = other > best ? other : best;
+      }
+      if (best == kNoLogit) break;
+      const unsigned long long low = __ballot(key[0] == best), high = __ballot(key[1] == best);
+      const int e = low != 0 ? __builtin_ctzll(low) : 64 + __builtin_ctzll(high);
+      first = k == 0 ? best : first;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (64 * s + lane == k) {
+          mine[s] = best;
+          id[s] = e;
+        }
+        key[s] = 64 * s + lane == e ? kNoLogit : key[s];
+      }
+    }
+    const float best = few_value(first);
+    float p[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      // (equal ones first: infinities have no difference)
+      const float v = few_value(mine[s]);
+      p[s] = mine[s] == kNoLogit ? 0.0f : v == best ? 1.0f : __builtin_amdgcn_exp2f((v - best) * 1.44269504088896341f);
+    }
+    const int rows = (int)as_uint(few_row_sum(p[0] + p[1]));
+    float sum = 0.0f;
+#pragma unroll
+    for (int l = 0; l < 64; l += 16) sum += as_float((uint32_t)__builtin_amdgcn_readlane(rows, l));
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const float q = p[s] / sum;
+      if (q > 0.0f) {
+        r.p[t][id[s]] = q;
+        r.rank[t][id[s]] = (uint8_t)(64 * s + lane);
+        atomicOr(&r.tokens[id[s]], 1u << t);
+      }
     }
   }
   __syncthreads();
-  const int lane = tid & 63;
   return {__ballot(r.tokens[lane] != 0), __ballot(r.tokens[64 + lane] != 0)};
 }
 
@@ -169,10 +183,6 @@ __device__ __forceinline__ void few_bf16(v4i codes, float pow2, u4 (&out)[2]) {
     out[i / 2][2 * (i % 2) + 1] = __builtin_bit_cast(uint32_t, hi);
   }
 }
-
-// Workgroup barrier behind this wave's LDS accesses alone: global loads stay on
-// their way (__syncthreads would wait for them).
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Operands of a fragment of R weight rows. R = 16: a block's half h as it lies
 // (f8.hpp), lane l row l % 16, k = 64 h + 16 (l / 16) ..; R = 8, for up to 8 tokens:
