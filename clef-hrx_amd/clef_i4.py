@@ -98,7 +98,7 @@ SIGNATURES = {
     "clef_moe_expert_gate_up_f8": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32,
                                                   _I32, _I32, _P, _P]),
     "clef_linear_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32]),
-    "clef_linear_kernel_name": (ctypes.c_char_p, [_I64, _I32, _I32, _I32]),
+    "clef_linear_kernel_name": (ctypes.c_char_p, [_I64, _I32, _I32, _I32, _I32]),
     "clef_linear": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _I32, _I64, _P, _I32, _I32, _P, _I64, _P, _I32, _I64,
                                    _P, _SZ, _P]),
     "clef_linear_gate_up": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _P, _I32, _I64, _P, _P, _I32, _I32, _P, _I64,

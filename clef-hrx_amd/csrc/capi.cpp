@@ -1149,9 +1149,9 @@ size_t clef_linear_workspace_bytes(int64_t m, int32_t n, int32_t k, int32_t gate
   return clef::linear_workspace_bytes(m, n, k, gate_up != 0);
 }
 
-const char* clef_linear_kernel_name(int64_t m, int32_t n, int32_t k, int32_t gate_up) {
+const char* clef_linear_kernel_name(int64_t m, int32_t n, int32_t k, int32_t gate_up, int32_t aligned) {
   if (m < 1 || m > 1048576 || n < 1 || n > 1048576 || k < 1 || k > 1048576) return "";
-  return clef::linear_kernel_name(m, n, k, gate_up != 0);
+  return clef::linear_kernel_name(m, n, k, gate_up != 0, aligned != 0 && k % 8 == 0);
 }
 
 int clef_linear(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint16_t* w, int32_t n,
@@ -1189,7 +1189,8 @@ int clef_moe_layer_f8(const uint16_t* x, int64_t x_stride, const void* logits, i
         x_stride <= (1 << 24) && (logits_dtype == 0 || logits_dtype == 1)))
     return fail(kFewShape);
   if (tokens == 0) return CLEF_OK;
-  for (const void* p : {(const void*)x, logits, (const void*)gate, (const void*)gate_scales, (const void*)up,
+  if (!aligned(logits, logits_dtype ? 4 : 2)) return fail(kAlign);
+  for (const void* p : {(const void*)x, (const void*)gate, (const void*)gate_scales, (const void*)up,
                         (const void*)up_scales, (const void*)down, (const void*)down_scales, (const void*)out,
                         (const void*)workspace})
     if (!aligned(p, 16)) return fail(kAlign);

@@ -692,12 +692,15 @@ LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up, bool a
     least = t;
     best = {kernel, parts};
   };
+  // the bytes that the product cannot do without, shared by the CUs as the tiles are
+  auto from_memory = [&](int64_t workgroups) { return memory * rounds(workgroups, kCus) * kCus / workgroups; };
   auto stream = [&](LinearKernel kernel, int bm, int bn) {
     if (m > 4096) return;  // (a launch has 65535 tiles of rows)
-    const float r = rounds(tiles(bm, bn), kCus);
-    float t = r * (bm + bn) * k * 2 / (aligned ? 33e3f : 22e3f);
-    t = t > memory ? t : memory;
-    consider(kernel, 1, 2.5f + t + (aligned ? 0 : 5 * (r - 1)));
+    const int64_t of = tiles(bm, bn);
+    const float r = rounds(of, kCus), rate = of < 175 ? 48e3f : of < kCus ? 8.4e6f / of : 33e3f;
+    const float loads = r * (bm + bn) * k * 2 / (aligned ? rate : 22e3f), least_t = from_memory(of);
+    const float joins = r * (bm * bn) * (2.0f / 4096);
+    consider(kernel, 1, 2 + joins + (loads > least_t ? loads : least_t) + (aligned ? 0 : 5 * (r - 1)));
   };
   if (!gate_up) stream(LinearKernel::s16x16, 16, 16);
   stream(LinearKernel::s16x32, 16, 32);
@@ -717,8 +720,9 @@ LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up, bool a
       const float r = rounds(of * parts, two ? 2 * kCus : kCus);
       if (parts > 1 && (r > 1 || steps < 8 * parts)) break;
       const float t = r * (start + (steps + parts - 1) / parts * (two ? pair : step));
-      consider(kernel, parts, (t > memory + start ? t : memory + start) +
-                                  (parts > 1 ? 3 + (float)(parts * m * rows_of_w) * 8 / 5e6f : 0));
+      const float least_t = from_memory(of * parts) + start;
+      consider(kernel, parts,
+               (t > least_t ? t : least_t) + (parts > 1 ? 3 + (float)(parts * m * rows_of_w) * 8 / 5e6f : 0));
     }
   };
   tile(LinearKernel::t128x128, 128, 128, 4.5f, 0.57f, 1.0f);
@@ -771,10 +775,10 @@ size_t linear_workspace_bytes(int64_t m, int n, int k, bool gate_up) {
   return plan.parts > 1 ? (size_t)(plan.parts * matrices * m * ((n + 3) & ~3)) * 4 : 0;
 }
 
-const char* linear_kernel_name(int64_t m, int n, int k, bool gate_up) {
+const char* linear_kernel_name(int64_t m, int n, int k, bool gate_up, bool aligned) {
   static const char* const names[] = {"any",   "8x8",     "8x16",     "16x16",   "16x32",  "16x64",
                                       "32x64", "64x64", "128x128", "128x128x2", "256x256", "128x256"};
-  return names[(int)linear_plan(m, (int64_t)n * (gate_up ? 2 : 1), k, gate_up, true).kernel];
+  return names[(int)linear_plan(m, (int64_t)n * (gate_up ? 2 : 1), k, gate_up, aligned).kernel];
 }
 
 hipError_t launch_linear(LinearArgs p, bool gate_up, void* workspace, hipStream_t stream) {

@@ -40,7 +40,7 @@ struct LinearArgs {
 
 // Scratch for the parts of a product whose operands' rows lie on 16 bytes.
 size_t linear_workspace_bytes(int64_t m, int n, int k, bool gate_up);
-const char* linear_kernel_name(int64_t m, int n, int k, bool gate_up);
+const char* linear_kernel_name(int64_t m, int n, int k, bool gate_up, bool aligned);
 hipError_t launch_linear(LinearArgs p, bool gate_up, void* workspace, hipStream_t stream);
 
 namespace {

@@ -627,12 +627,12 @@ int clef_moe_expert_gate_up_f8(const uint8_t* a, int64_t a_rows, const uint8_t* 
  * takes the parts' sums, which are added in a fixed order. */
 size_t clef_linear_workspace_bytes(int64_t m, int32_t n, int32_t k, int32_t gate_up);
 
-/* The tile (rows x weight rows) that the library's rule picks for operands whose
- * rows lie on 16 bytes, for tests and profiles: "8x8", "8x16", "16x16", "16x32",
- * "16x64", "32x64", "64x64", "128x128", "128x128x2" (two steps of k at a time),
- * "128x256", "256x256"; other operands run "any". "" for a shape the products
- * reject. */
-const char* clef_linear_kernel_name(int64_t m, int32_t n, int32_t k, int32_t gate_up);
+/* The tile (rows x weight rows) that the library's rule picks, for tests and
+ * profiles: "8x8", "8x16", "16x16", "16x32", "16x64", "32x64", "64x64", "128x128",
+ * "128x128x2" (two steps of k at a time), "128x256", "256x256", "any" (64x64 for
+ * operands of any alignment). aligned: every row of x and the weights starts on a
+ * multiple of 16 bytes (as far as k % 8 == 0). "" for a shape the products reject. */
+const char* clef_linear_kernel_name(int64_t m, int32_t n, int32_t k, int32_t gate_up, int32_t aligned);
 
 int clef_linear(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint16_t* w, int32_t n,
                 int64_t w_stride, const void* bias, int32_t bias_dtype, int32_t activation,
@@ -659,7 +659,7 @@ int clef_linear_gate_up(const uint16_t* x, int64_t m, int32_t k, int64_t x_strid
  * and x may be the output itself. Preconditions: 0 <= tokens <= 16, 1 <= topk <=
  * experts <= 128, hidden and inter as the FP8 widths, x_stride >= hidden, x_stride
  * % 8 == 0, x_stride <= 2^24 -> "unsupported MoE shape for few tokens"; pointers
- * 16-byte aligned. The workspace (bytes below; 0 for shapes the call rejects)
+ * 16-byte aligned (logits: as their elements). The workspace (bytes below; 0 for shapes the call rejects)
  * lies apart from every operand -> "MoE workspace overlaps an operand"; the
  * output over a part of x, the residual or the logits -> "MoE output overlaps an
  * operand". */

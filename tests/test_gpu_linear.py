@@ -133,6 +133,68 @@ def test_linear_of_whole_numbers_is_exact(m, k, n):
     assert torch.equal(clef_i4.linear(x, w, bias=b, residual=r), got.to(BF))
 
 
+# rows, k, columns, the kernel that the rule picks and the parts of k: every kernel
+# with ends inside its tile and its last step (projections, gate/up)
+KERNELS = ([(3, 200, 43, "8x8", 1), (7, 136, 8209, "8x16", 1), (11, 72, 45, "16x16", 1), (19, 72, 2059, "16x32", 1),
+            (35, 72, 8201, "16x64", 1), (17, 72, 12301, "32x64", 1), (51, 72, 12301, "64x64", 1), (525, 136, 6003, "128x128", 1),
+            (9, 8200, 45, "128x128", 8), (133, 2056, 8203, "128x128x2", 1), (131, 8200, 3001, "128x128x2", 4),
+            (403, 1032, 8203, "128x256", 1), (131, 8200, 4107, "128x256", 6), (1303, 264, 6001, "256x256", 1),
+            (401, 4104, 8203, "256x256", 3)],
+           [(5, 72, 43, "8x16", 1), (11, 72, 45, "16x32", 1), (19, 72, 2059, "16x64", 1), (33, 72, 3001, "32x64", 1),
+            (33, 136, 6003, "64x64", 1), (33, 520, 8203, "128x128", 1), (9, 4104, 43, "128x128", 8),
+            (131, 2056, 4107, "128x128x2", 1), (131, 4104, 3001, "128x128x2", 2), (133, 1032, 8203, "128x256", 1),
+            (131, 4104, 4107, "128x256", 3), (403, 264, 8203, "256x256", 1), (131, 4104, 8203, "256x256", 3)])
+# the same for rows that start at any even byte
+ODD_KERNELS = ([(3, 201, 43, "8x8"), (7, 137, 8209, "8x16"), (11, 73, 45, "16x16"), (19, 73, 2059, "16x32"), (21, 73, 4107, "16x64"),
+                (18, 73, 8203, "32x64"), (500, 1001, 2059, "any")],
+               [(5, 73, 43, "8x16"), (11, 73, 45, "16x32"), (19, 73, 2059, "16x64"), (21, 73, 4107, "32x64"), (300, 1001, 2059, "any")])
+
+
+@pytest.mark.parametrize("m,k,n", [c[:3] for c in KERNELS[0] + ODD_KERNELS[0]])
+def test_linear_on_every_kernel(m, k, n):
+    seed = m * 17 + k * 3 + n
+    x, w, r = randn((m, k), 1.0, seed), randn((n, k), k ** -0.5, seed + 1), randn((m, n), 1.0, seed + 3)
+    for bias, act, res, dtype in EPILOGUES:
+        b = make_bias(n, bias, seed + 2)
+        got = clef_i4.linear(x, w, bias=b, activation=act, residual=r if res else None, dtype=dtype)
+        check(got, *linear64(x, w, b, act, r if res else None))
+    again = r.clone()
+    clef_i4.linear(x, w, residual=again, out=again)
+    assert torch.equal(again, clef_i4.linear(x, w, residual=r))
+    x, w, b = whole((m, k), 3, m + k), whole((n, k), 1, n + k), whole((n,), 4, 5)
+    want = x.double() @ w.double().t() + b.double() + r.double()
+    assert torch.equal(clef_i4.linear(x, w, bias=b, residual=r), want.float().to(BF))
+
+
+@pytest.mark.parametrize("m,k,n", [c[:3] for c in KERNELS[0] + ODD_KERNELS[0]])
+def test_linear_non_finite_values_on_every_kernel(m, k, n):
+    """A NaN row and a NaN weight row touch their row and column alone; the columns
+    behind the last one and the rows behind the last stay as they were."""
+    x, w = randn((m, k), 1.0, 1), randn((n, k), 0.05, 2)
+    clean = clef_i4.linear(x, w)
+    wide = torch.full((m + 1, n + 5), 7.0, dtype=BF, device="cuda")
+    x[m // 2, k - 1], w[n - 2, 0] = NAN, INF
+    clef_i4.linear(x, w, out=wide[:m, :n])
+    keep = torch.ones((m, n), dtype=torch.bool, device="cuda")
+    keep[m // 2], keep[:, n - 2] = False, False
+    assert torch.equal(wide[:m, :n][keep], clean[keep])
+    assert torch.isnan(wide[m // 2, :n]).all() and not torch.isfinite(wide[:m, n - 2]).any()
+    assert (wide[m] == 7.0).all() and (wide[:, n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("m,k,n", [c[:3] for c in KERNELS[1] + ODD_KERNELS[1]])
+def test_gate_up_on_every_kernel(m, k, n):
+    seed = m * 11 + k * 3 + n
+    x, wg, wu = randn((m, k), 1.0, seed), randn((n, k), k ** -0.5, seed + 1), randn((n, k), k ** -0.5, seed + 2)
+    bg, bu = randn((n,), 1.0, seed + 3), randn((n,), 1.0, seed + 4)
+    check(clef_i4.linear_gate_up(x, wg, wu), *gate_up64(x, wg, wu))
+    check(clef_i4.linear_gate_up(x, wg, wu, activation="gelu", gate_bias=bg, up_bias=bu), *gate_up64(x, wg, wu, "gelu", bg, bu))
+    x = (whole((m, k), 1, m + k).float() * (torch.arange(k, device="cuda") % 8 == 0)).to(BF)
+    wg, wu = whole((n, k), 1, 1), whole((n, k), 1, 2)
+    want = (x.double() @ wg.double().t()) * (x.double() @ wu.double().t())
+    assert torch.equal(clef_i4.linear_gate_up(x, wg, wu, activation=None), want.float().to(BF))
+
+
 @pytest.mark.parametrize("act", [None, "relu", "gelu", "gelu_tanh", "silu", "sigmoid"])
 def test_activations_over_their_range(act):
     """Every bf16 value between -2^7 and 2^7 through a weight of one."""
@@ -361,7 +423,8 @@ def layer(experts, hidden, inter, topk, kind, seed, router=None):
 
 MOE = [(1, 2048, 768, 128, 8, "e8m0"), (1, 8, 8, 1, 1, "f32"), (2, 136, 72, 3, 2, "f32"), (3, 256, 128, 8, 1, "f32"),
        (5, 1000, 520, 60, 4, "f32"), (7, 128, 2048, 8, 6, "e8m0"), (8, 512, 256, 128, 8, "e8m0"), (13, 4096, 264, 32, 2, "f32"),
-       (16, 264, 136, 16, 16, "f32"), (16, 640, 384, 128, 8, "f32"), (16, 128, 8, 128, 128, "f32"), (4, 256, 136, 65, 3, "e8m0")]
+       (2, 5000, 136, 8, 2, "f32"), (12, 4232, 72, 12, 3, "e8m0"), (2, 32768, 8, 4, 2, "f32"), (11, 32768, 16, 4, 2, "f32"),
+       (3, 8, 32768, 4, 2, "f32"), (16, 264, 136, 16, 16, "f32"), (16, 640, 384, 128, 8, "f32"), (16, 128, 8, 128, 128, "f32"), (4, 256, 136, 65, 3, "e8m0")]
 
 
 @pytest.mark.parametrize("t,hidden,inter,experts,topk,kind", MOE)
@@ -460,6 +523,9 @@ def test_decode_in_place_strided_and_with_its_router():
     router = randn((experts, hidden), 0.05, 9)
     moe, w = layer(experts, hidden, inter, topk, "f32", 3, router)
     x = randn((t, hidden), 1.0, 1)
+    many = randn((9, 25), 1.0, 7)
+    part = many.flatten()[1:1 + t * experts].view(t, experts)  # logits that start at any element
+    assert torch.equal(moe.decode(x, part), moe.decode(x, part.clone()))
     logits = clef_i4.linear(x, router, dtype=F32)
     want = moe.decode(x, logits, residual=x)
     assert torch.equal(moe.decode(x, residual=x), want)
@@ -541,6 +607,44 @@ def test_block_graphs_replay_beside_eager_calls(parts):
         torch.cuda.synchronize()
         for out, want in zip(outs, wants):
             assert torch.equal(out, want)
+
+
+def test_split_products_in_graphs_and_on_two_streams():
+    """Products whose parts meet in scratch of their own: two captured graphs, eager
+    calls in between, then two streams."""
+    shapes = [(131, 8200, 3001), (300, 8200, 1040)]
+    ws = [randn((n, k), 0.02, n) for _, k, n in shapes]
+    xs = [torch.zeros((m, k), dtype=BF, device="cuda") for m, k, _ in shapes]
+    assert all(clef_i4.lib().clef_linear_workspace_bytes(m, n, k, g) > 0 for m, k, n in shapes for g in (0, 1))
+
+    def both(i, x):
+        return clef_i4.linear(x, ws[i], activation="silu"), clef_i4.linear_gate_up(x, ws[i], ws[i])
+
+    for i, x in enumerate(xs):
+        both(i, x)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i, x in enumerate(xs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(both(i, x))
+        graphs.append(g)
+    for turn in range(4):
+        for i, x in enumerate(xs):
+            x.copy_(randn(x.shape, 1.0, 10 * turn + i))
+        wants = [both(i, x.clone()) for i, x in enumerate(xs)]
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for out, want in zip(outs, wants) for o, w in zip(out, want))
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[] for _ in xs]
+    for _ in range(5):
+        for i, (s, x) in enumerate(zip(streams, xs)):
+            with torch.cuda.stream(s):
+                got[i].append(both(i, x))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for g, want in zip(got, wants) for out in g for o, w in zip(out, want))
 
 
 def test_block_on_two_streams_at_once(parts):
