@@ -1177,7 +1177,7 @@ int clef_linear_gate_up(const uint16_t* x, int64_t m, int32_t k, int64_t x_strid
 size_t clef_moe_layer_f8_workspace_bytes(int64_t tokens, int32_t hidden, int32_t inter, int32_t experts,
                                          int32_t topk) {
   if (tokens < 1 || !few_shape(tokens, hidden, inter, experts, topk)) return 0;
-  return clef::moe_few_workspace_bytes((int)tokens, topk, hidden, inter);
+  return clef::moe_few_workspace_bytes((int)tokens, topk, experts, hidden, inter);
 }
 
 int clef_moe_layer_f8(const uint16_t* x, int64_t x_stride, const void* logits, int32_t logits_dtype, int64_t tokens,
@@ -1195,7 +1195,7 @@ int clef_moe_layer_f8(const uint16_t* x, int64_t x_stride, const void* logits, i
                         (const void*)workspace})
     if (!aligned(p, 16)) return fail(kAlign);
   if (residual && !aligned(residual, 16)) return fail(kAlign);
-  const size_t need = clef::moe_few_workspace_bytes((int)tokens, topk, hidden, inter);
+  const size_t need = clef::moe_few_workspace_bytes((int)tokens, topk, experts, hidden, inter);
   if (workspace_bytes < need) return fail(kWorkspace);
   const size_t logits_bytes = (size_t)tokens * experts * (logits_dtype ? 4 : 2), rows_bytes = (size_t)tokens * hidden * 2;
   const Pieces rows{x, tokens, x_stride * 2, hidden * 2ll}, result{out, tokens, hidden * 2ll, hidden * 2ll};

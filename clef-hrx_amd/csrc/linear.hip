@@ -1,4 +1,9 @@
 // bf16 products with bias, activation and residual in the epilogue (linear.hpp).
+//
+// Few rows are bound by the weight's bytes (and by the rows', which every tile of
+// columns reads again), many by the matrix unit, whose rate the board's power holds
+// at about 1.5 PFLOP/s. Times below are in us, operands from memory (in turn past the
+// last-level cache, in a graph); what is compared ran in turn on one card.
 #include "linear.hpp"
 
 namespace clef {
@@ -52,10 +57,10 @@ __device__ __forceinline__ AnyEight any_load_tail(const AnyRow& r, int k, int K)
   return {u4{d[0], d[1], d[2], d[3]}, d[4]};
 }
 
-// Every shape, stride and alignment: 64 rows x 64 weight rows (gate/up: 32 gate
-// and 32 up) per workgroup of four waves, 64 k at a time through registers into one
-// LDS stage (16-byte chunk c of row r at c ^ ((r >> 1) & 7)), the next 64 k on
-// their way meanwhile.
+// Many rows of any alignment: 64 rows x 64 weight rows (gate/up: 32 gate and 32 up)
+// per workgroup of four waves, 64 k at a time through registers into one LDS stage
+// (16-byte chunk c of row r at c ^ ((r >> 1) & 7)), the next 64 k on their way
+// meanwhile. 512 x 2049 x 17408 123 us, 0.3 PFLOP/s.
 template <bool GU>
 __global__ __launch_bounds__(256) void linear_any_kernel(const LinearArgs p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -141,7 +146,8 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinearArgs p) {
 // Tile of linear_tile_kernel: KG groups of WAVES_M x WAVES_N waves of WM rows x WN
 // weight rows, group g multiplying step g of each KG steps of 64 k; two LDS stages
 // of KG steps each. A row is 128 bytes of a step, its 16-byte chunk c at c ^ ((r >>
-// 1) & 7) (no bank conflicts in reads of 16 rows).
+// 1) & 7) (no bank conflicts in reads of 16 rows). v_mfma_f32_32x32x16_bf16 on the
+// same tiles: 4096 x 4096 x 12288 342 against 329 (8192 x 8192 x 8192 842, 775).
 template <int WM_, int WN_, int WAVES_M_, int WAVES_N_, int GROUPS_ = 1, int KG_ = 1>
 struct LinearTile {
   static constexpr int GROUPS = GROUPS_;  // workgroups per CU
@@ -166,6 +172,8 @@ struct LinearTile {
 // The epilogue of a wave's EM x TN fragments of 16 x 16 sums (gate/up: the first half of
 // each row of them the gate's, the other the up's): rows w0 .. of the tile's `here`
 // from m0, columns from c0. A lane has four columns of row l % 16 of each fragment.
+// Rows that went through LDS to be stored took 4096 x 4096 x 12288 338 us, not 312
+// (with bias and tanh GELU 345, 320).
 template <int EM, int TN, bool GU, bool RESID>
 __device__ __forceinline__ void linear_store_tile(const LinearArgs& p, const v4f (&sum)[EM][TN], int part, int64_t m0,
                                                   int here, int w0, int c0) {
@@ -255,6 +263,13 @@ __device__ __forceinline__ void linear_store_tile(const LinearArgs& p, const v4f
 // loaded for two steps on, behind one before the step's last row of MFMAs the same
 // goes for Y; each barrier also waits for the part that the MFMAs behind it read.
 // So every load has a step and a half to land.
+//
+// 256 x 256 tiles: 4096 x 4096 x 12288 303 to 313 by card, 1.32 to 1.36 PFLOP/s (the
+// library's product 330), 8192 x 8192 x 8192 743 (715). MFMA busy two thirds of the
+// cycles at 1.9 to 2.0 GHz; with operands of zeros the same code takes 257, so a fifth
+// of the time is the clock that the power leaves. Without the epilogue 278. Four
+// waves of 128 x 128, which read a third less LDS, run the same main loop in the same
+// time and a longer epilogue (322).
 template <class T, bool GU, bool RESID>
 __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(const LinearArgs p, int tiles_m,
                                                                                 int tiles_n) {
@@ -442,6 +457,7 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(
 }
 
 // The parts' sums, in their order, and the epilogue: four columns of a row per thread.
+// Bound by the sums' bytes: 620 x 5120 in four parts 51 MB, 13 us.
 template <bool GU>
 __global__ __launch_bounds__(256) void linear_join_kernel(const LinearArgs p) {
   const int quads = (p.n + 3) / 4;
@@ -482,21 +498,22 @@ hipError_t launch_tile(const LinearArgs& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Few rows: a workgroup owns 16 MT rows x 16 NT weight rows (gate/up: NT / 2
-// fragments of gate rows and the same of up), its eight waves split k in steps of 64
-// (wave w: steps w, w + 8, ..), D steps of each on their way. Operands go straight
-// into registers: a weight row is used by this workgroup's rows only. The waves'
-// sums meet in LDS and are added in wave order (the result does not depend on
-// timing).
+// Few rows: a workgroup owns R MT rows x R NT weight rows (gate/up: NT / 2 fragments
+// of gate rows and the same of up), its eight waves split k in steps (wave w: steps w,
+// w + 8, ..), D steps of each on their way. Operands go straight into registers: a
+// weight row is used by this workgroup's rows only. The waves' sums meet in LDS and
+// are added in wave order (the result does not depend on timing).
 //
-// R: weight rows per fragment. A fragment of R = 4 or 8 rows (for as many rows of
-// x) holds 16 / R pieces of k of each, its lanes lr / R of both operands piece lr /
-// R: of the 16 x 16 sums the blocks on the diagonal count, one per piece. So a tile
-// has as few columns as fill the card, and a load takes 16 / R times 64 contiguous
-// bytes of a row.
+// R, the weight rows per fragment: 16, or 8 for up to 8 rows of x. A fragment of 8
+// rows holds two pieces of k of each, lanes lr / 8 of both operands piece lr / 8: of
+// the 16 x 16 sums the two blocks on the diagonal count, one per piece. So twice as
+// many tiles share the bytes, and a load takes 128 contiguous bytes of a row. One row,
+// R = 16, 8 and 4, the best of one to four fragments each: 2048 x 128 4.5, 3.4, 3.2; 4096
+// x 12288 22.4, 18.5 (5.4 TB/s), 21.8; 17408 x 5120 38.9, 37.4, 35.8; gate/up 5120 x 2
+// 17408 70.3, 65.5, 89.8. Two steps on their way gain where a step is one fragment
+// (4096 x 12288 21.8, 18.5) and nothing in larger ones.
 //
-// ANY: rows that start at any even byte (AnyRow); only the last step takes values one
-// by one.
+// ANY: rows that start at any even byte (AnyRow).
 template <bool ANY, int R, int MT, int NT, int D, bool GU>
 __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -678,8 +695,20 @@ struct LinearPlan {
   int parts;
 };
 
-// The kernel for a product of m rows against n weight rows (gate/up: both): of the
-// kernels' times as modelled here, in us, the least.
+// The kernel for a product of m rows against n weight rows (gate/up: both), and the
+// parts that k is split into: of the kernels' times as modelled here, in us, the least.
+// The model's rates are measured ones:
+//  * few rows: a CU takes 33 bytes per ns of weights and rows (48 where fewer than 175
+//    CUs do, 22 of AnyRow's), 2 us to start and end, 2 us to join a tile of 64 x 64;
+//  * tiles: a start and an end, and a step of 64 k each (two workgroups of 128 x 128
+//    per CU: 1.0 for both); split, another launch that reads what they wrote;
+//  * either no faster than memory, by the CUs that have a tile.
+// What it decides, in both forms: 64 x 17408 x 5120 on 64 x 64 tiles of few rows 101, on
+// 128 x 128 tiles in 6 parts 43.5; 200 x 17408 x 5120 whole 140, in 3 parts 67; 620 x
+// 17408 x 5120 on 128 x 128 tiles 150, on 256 x 256 in 4 parts 125; 512 x 4096 x 4096
+// 40, in 2 parts 32; 37 x 4160 x 1352 on 16 x 16 tiles 10.6, on 128 x 128 in 12 parts
+// 13.1. Over 160 random shapes its choice takes 0.7 % longer than the best of twenty
+// fixed ones (2.6 % over 40 of odd widths).
 LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up, bool aligned) {
   if (m <= 8) return {gate_up || (m > 4 && rows_of_w > 8192) ? LinearKernel::s8x16 : LinearKernel::s8x8, 1};
   auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((rows_of_w + bn - 1) / bn); };

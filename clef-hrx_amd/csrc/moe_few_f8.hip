@@ -8,10 +8,19 @@
 // themselves, whether they name the expert or not, and there are no lists of rows.
 // The rows stay bf16 (quantizing them would save no byte that counts): a weight's
 // e4m3 codes become bf16 on their way to the matrix unit, exact with the scale's
-// power of two, whose remaining factor enters the f32 sums behind each block of 128 k. The router's probability goes into h (in f32, in front of
-// its rounding), so that the down products of all experts add up in one
-// accumulator. h is held as two bf16 that together keep 16 bits of it: the second
-// product costs nothing beside the weights' bytes, and the output is rounded once.
+// power of two, whose remaining factor enters the f32 sums behind each block of 128 k.
+// The router's probability goes into h (in f32, in front of its rounding), so that
+// the down products of all experts add up in one accumulator. h is held as two bf16
+// that together keep 16 bits of it: the second product costs nothing beside the
+// weights' bytes, and the output is rounded once.
+//
+// Hidden 2048, width 768, 128 experts, top-8, weights from memory, in a graph: one
+// token 17 us (9.7 and 7.3; 38 MB), sixteen 79 (46 and 33; 83 experts, 390 MB, 5
+// TB/s). What it took: loads without branches between them (a branch makes the
+// compiler wait for each, 5 us of the first launch at one token); one workgroup per
+// CU over units with the next one's weights on their way (sixteen tokens' first
+// launch 57 -> 46); the parts' sums by device-scope atomics instead of fences that
+// write back whole caches (the second launch 143 -> 66 -> 33).
 #include "f8.hpp"
 #include "linear.hpp"
 #include "moe_few_f8.hpp"
@@ -204,20 +213,21 @@ struct FewLane {
   }
 };
 
-// Route, gate/up and SwiGLU. One unit is 16 columns of h of one expert named; its
-// eight waves split the blocks of k, wave w the blocks w, w + 8, .., whose part of x
-// stays in registers (NB blocks; 0: any number, loaded each time). The next unit's
-// weights are on their way while a unit's sums meet in LDS, where one wave in turn
-// adds them in wave order.
-template <int NB>
+// Route, gate/up and SwiGLU. W waves split the blocks of k of 16 columns of h of one
+// expert named, wave w of them the blocks w, w + W, .., whose part of x stays in
+// registers (NB blocks; 0: any number, loaded each time); a unit is the 8 / W times 16
+// columns of the workgroup's waves. The next unit's weights are on their way while a
+// unit's sums meet in LDS, where one of the W waves in turn adds them in wave order.
+template <int W, int NB>
 __global__ __launch_bounds__(512) void few_gate_up_kernel(const MoeFewArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ FewRoutes routes;
   __shared__ v4f sums[2][8][2][64];
-  constexpr int R = 16, H = FewLane<R>::HALVES, XB = NB ? NB : 1;
+  constexpr int COLS = 16 * (8 / W), R = 16, H = FewLane<R>::HALVES, XB = NB ? NB : 1;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const FewLane<R> me;
-  const int kb = f8_blocks(a.hidden), tiles = (a.inter + R - 1) / R, panels = f8_blocks(a.inter);
+  const int kw = wave % W, column = 16 * (wave / W);  // wave of the W, first column in the unit
+  const int kb = f8_blocks(a.hidden), tiles = (a.inter + COLS - 1) / COLS, panels = f8_blocks(a.inter);
   const int token = me.row < a.tokens ? me.row : a.tokens - 1;
   const __amdgpu_buffer_rsrc_t xr = make_rsrc(a.x, (uint32_t)(((a.tokens - 1) * a.x_stride + a.hidden) * 2));
   u4 xv[XB][2 * H];
@@ -231,7 +241,7 @@ __global__ __launch_bounds__(512) void few_gate_up_kernel(const MoeFewArgs a) {
   };
   if constexpr (NB > 0) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) load_x(wave + 8 * i, xv[i]);
+    for (int i = 0; i < NB; ++i) load_x(kw + W * i, xv[i]);
   }
   const FewNamed named = few_route(a, routes);
   const int count = named.count(), units = count * tiles;
@@ -265,9 +275,9 @@ __global__ __launch_bounds__(512) void few_gate_up_kernel(const MoeFewArgs a) {
   auto load_unit = [&](Unit& q, int u) {
     u = u < units ? u : units - 1;
     q.e = __builtin_amdgcn_readfirstlane(named.expert(u / tiles));
-    q.n0 = u % tiles * R;
+    q.n0 = u % tiles * COLS + column;
 #pragma unroll
-    for (int i = 0; i < NB; ++i) load_block(q, i, wave + 8 * i < kb ? wave + 8 * i : kb - 1);
+    for (int i = 0; i < NB; ++i) load_block(q, i, kw + W * i < kb ? kw + W * i : kb - 1);
   };
   v4f acc[2];
   auto add_block = [&](const Unit& q, int i, const u4 (&x)[2 * H]) {
@@ -296,9 +306,9 @@ __global__ __launch_bounds__(512) void few_gate_up_kernel(const MoeFewArgs a) {
     if constexpr (NB > 0) {
 #pragma unroll
       for (int i = 0; i < NB; ++i)
-        if (wave + 8 * i < kb) add_block(q, i, xv[i]);
+        if (kw + W * i < kb) add_block(q, i, xv[i]);
     } else {
-      for (int b = wave; b < kb; b += 8) {
+      for (int b = kw; b < kb; b += W) {
         load_x(b, xv[0]);
         load_block(q, 0, b);
         add_block(q, 0, xv[0]);
@@ -308,14 +318,14 @@ __global__ __launch_bounds__(512) void few_gate_up_kernel(const MoeFewArgs a) {
 #pragma unroll
     for (int m = 0; m < 2; ++m) sums[turn & 1][wave][m][lane] = acc[m];
     lds_barrier();
-    if (wave != (turn & 7)) continue;
+    if (kw != turn % W) continue;
     const int t = lane & 15, col = n0 + 4 * (lane >> 4);
     if (t >= a.tokens || !(routes.tokens[e] >> t & 1) || col >= a.inter) continue;
     v4f gate = {0, 0, 0, 0}, up = {0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      gate += sums[turn & 1][w][0][lane];
-      up += sums[turn & 1][w][1][lane];
+    for (int w = 0; w < W; ++w) {
+      gate += sums[turn & 1][wave - kw + w][0][lane];
+      up += sums[turn & 1][wave - kw + w][1][lane];
     }
     const float p = routes.p[t][e];
     uint16_t* at = a.h + (int64_t)(t * a.topk + routes.rank[t][e]) * a.inter + col;
@@ -483,48 +493,70 @@ __global__ __launch_bounds__(512) void few_down_kernel(const MoeFewArgs a) {
 #endif
 }
 
-constexpr int kNT = 2, kMostTiles = 32768 / (16 * kNT), kWorkgroups = 512, kCus = 256;
+constexpr int kCus = 256, kMostTiles = 32768 / 8, kMostParts = 16;
 constexpr size_t kTableBytes = (sizeof(FewTable) + 255) / 256 * 256, kArrivedBytes = kMostTiles * 4;
 
-// Tiles of the output with several parts, and the parts: two workgroups per CU
-// together.
-int few_tiles(int hidden) { return (hidden + 16 * kNT - 1) / (16 * kNT); }
-int few_parts(int hidden) {
-  const int parts = kWorkgroups / few_tiles(hidden);
-  return parts < 1 ? 1 : parts > 4 ? 4 : parts;
+// The tiles of the output and their parts, as many as fill the CUs (a workgroup each:
+// 16 x 2048 x 768, 64 tiles, 79 us in 4 parts, 83 in 8, 87 in 16) but of 70 KB of
+// weights at least, for joining them takes 2 us (two tokens of 4 of 64 experts, 512 x
+// 512, 32 KB per tile: 10.4 whole, 12.3 in 4 parts; nine of 4 of 128, 256 x 2048, 2 MB
+// per tile: 46 in 4 parts, 27 in 16). Up to 16 routes: 8 columns, whose workgroups hold
+// all of h's few rows on their way (one token of 8 experts 17.0 against 18.5 on 32
+// columns, two 24.3 and 26.0; three 31.1 and 30.4).
+struct FewDown {
+  bool small;
+  int tiles, parts;
+};
+FewDown few_down(int tokens, int topk, int experts, int hidden, int inter) {
+  const bool small = tokens <= 8 && tokens * topk <= 16;
+  const int columns = small ? 8 : 32, tiles = (hidden + columns - 1) / columns;
+  float others = 1.0f;  // that no token names an expert, evenly chosen
+  for (int t = 0; t < tokens; ++t) others *= 1.0f - (float)topk / experts;
+  int parts = (int)((1.0f - others) * experts * inter * columns / 70e3f);
+  parts = parts < kMostParts ? parts : kMostParts;
+  parts = parts < kCus / tiles ? parts : kCus / tiles;
+  return {small, tiles, parts < 1 ? 1 : parts};
 }
-size_t few_partial_bytes(int hidden) { return (size_t)few_tiles(hidden) * few_parts(hidden) * kNT * 64 * 16; }
+// f32 of each part: 16 (or 8) tokens of the tile's columns
+size_t few_partial_bytes(const FewDown& d) { return (size_t)d.tiles * d.parts * (d.small ? 8 * 8 : 16 * 32) * 4; }
 
 }  // namespace
 
-size_t moe_few_workspace_bytes(int tokens, int topk, int hidden, int inter) {
-  return kTableBytes + kArrivedBytes + few_partial_bytes(hidden) + (size_t)tokens * topk * inter * 4;
+size_t moe_few_workspace_bytes(int tokens, int topk, int experts, int hidden, int inter) {
+  return kTableBytes + kArrivedBytes + few_partial_bytes(few_down(tokens, topk, experts, hidden, inter)) + (size_t)tokens * topk * inter * 4;
 }
 
 hipError_t launch_moe_few(MoeFewArgs a, void* workspace, hipStream_t stream) {
+  const FewDown down = few_down(a.tokens, a.topk, a.experts, a.hidden, a.inter);
   char* at = static_cast<char*>(workspace);
   a.table = at;
   a.arrived = reinterpret_cast<int*>(at += kTableBytes);
   a.partial = at += kArrivedBytes;
-  a.h = reinterpret_cast<uint16_t*>(at + few_partial_bytes(a.hidden));
-  const int slots = a.tokens * a.topk, most = slots < a.experts ? slots : a.experts;
-  const int blocks = (f8_blocks(a.hidden) + 7) / 8;  // per wave
-  const bool few = a.tokens <= 8;
-  a.down_tiles = few_tiles(a.hidden);
-  const int units = most * ((a.inter + 15) / 16), grid = units < kCus ? units : kCus;
-  if (blocks <= 1)
-    few_gate_up_kernel<1><<<grid, 512, 0, stream>>>(a);
-  else if (blocks <= 2)
-    few_gate_up_kernel<2><<<grid, 512, 0, stream>>>(a);
-  else if (blocks <= 4)
-    few_gate_up_kernel<4><<<grid, 512, 0, stream>>>(a);
+  a.h = reinterpret_cast<uint16_t*>(at + few_partial_bytes(down));
+  a.down_tiles = down.tiles;
+  const int slots = a.tokens * a.topk, most = slots < a.experts ? slots : a.experts, kb = f8_blocks(a.hidden);
+  auto gate_up = [&](auto kernel, int columns) {
+    const int units = most * ((a.inter + columns - 1) / columns);
+    kernel<<<units < kCus ? units : kCus, 512, 0, stream>>>(a);
+  };
+  if (kb <= 2)
+    gate_up(few_gate_up_kernel<2, 1>, 64);
+  else if (kb <= 4)
+    gate_up(few_gate_up_kernel<4, 1>, 32);
+  else if (kb <= 8)
+    gate_up(few_gate_up_kernel<8, 1>, 16);
+  else if (kb <= 16)
+    gate_up(few_gate_up_kernel<8, 2>, 16);
+  else if (kb <= 32)
+    gate_up(few_gate_up_kernel<8, 4>, 16);
   else
-    few_gate_up_kernel<0><<<grid, 512, 0, stream>>>(a);
+    gate_up(few_gate_up_kernel<8, 0>, 16);
   if (hipError_t e = hipGetLastError()) return e;
-  if (few && slots <= 16)
-    few_down_kernel<8, 1, 2><<<(a.hidden + 7) / 8, 512, 0, stream>>>(a);
+  const dim3 grid(down.tiles, down.parts);
+  if (down.small)
+    few_down_kernel<8, 1, 2><<<grid, 512, 0, stream>>>(a);
   else
-    few_down_kernel<16, kNT, 1><<<dim3(a.down_tiles, few_parts(a.hidden)), 512, 0, stream>>>(a);
+    few_down_kernel<16, 2, 1><<<grid, 512, 0, stream>>>(a);
   return hipGetLastError();
 }
 

@@ -27,7 +27,7 @@ struct MoeFewArgs {
   uint16_t* h;     // bf16 [tokens * topk][inter], then what its rounding left
 };
 
-size_t moe_few_workspace_bytes(int tokens, int topk, int hidden, int inter);
+size_t moe_few_workspace_bytes(int tokens, int topk, int experts, int hidden, int inter);
 hipError_t launch_moe_few(MoeFewArgs a, void* workspace, hipStream_t stream);
 
 }  // namespace clef

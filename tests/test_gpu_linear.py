@@ -424,7 +424,7 @@ def layer(experts, hidden, inter, topk, kind, seed, router=None):
 MOE = [(1, 2048, 768, 128, 8, "e8m0"), (1, 8, 8, 1, 1, "f32"), (2, 136, 72, 3, 2, "f32"), (3, 256, 128, 8, 1, "f32"),
        (5, 1000, 520, 60, 4, "f32"), (7, 128, 2048, 8, 6, "e8m0"), (8, 512, 256, 128, 8, "e8m0"), (13, 4096, 264, 32, 2, "f32"),
        (2, 5000, 136, 8, 2, "f32"), (12, 4232, 72, 12, 3, "e8m0"), (2, 32768, 8, 4, 2, "f32"), (11, 32768, 16, 4, 2, "f32"),
-       (3, 8, 32768, 4, 2, "f32"), (16, 264, 136, 16, 16, "f32"), (16, 640, 384, 128, 8, "f32"), (16, 128, 8, 128, 128, "f32"), (4, 256, 136, 65, 3, "e8m0")]
+       (3, 8, 32768, 4, 2, "f32"), (9, 256, 2048, 32, 4, "e8m0"), (16, 200, 1032, 24, 8, "f32"), (16, 264, 136, 16, 16, "f32"), (16, 640, 384, 128, 8, "f32"), (16, 128, 8, 128, 128, "f32"), (4, 256, 136, 65, 3, "e8m0")]
 
 
 @pytest.mark.parametrize("t,hidden,inter,experts,topk,kind", MOE)
