@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinearArgs p) {
 // weight rows, group g multiplying step g of each KG steps of 64 k; two LDS stages
 // of KG steps each. A row is 128 bytes of a step, its 16-byte chunk c at c ^ ((r >>
 // 1) & 7) (no bank conflicts in reads of 16 rows). v_mfma_f32_32x32x16_bf16 on the
-// same tiles: 4096 x 4096 x 12288 342 against 329 (8192 x 8192 x 8192 842, 775).
+// same tiles: 4096 x 4096 x 12288 344 against 315 (8192 x 8192 x 8192 844, 775).
 template <int WM_, int WN_, int WAVES_M_, int WAVES_N_, int GROUPS_ = 1, int KG_ = 1>
 struct LinearTile {
   static constexpr int GROUPS = GROUPS_;  // workgroups per CU
@@ -172,8 +172,8 @@ struct LinearTile {
 // The epilogue of a wave's EM x TN fragments of 16 x 16 sums (gate/up: the first half of
 // each row of them the gate's, the other the up's): rows w0 .. of the tile's `here`
 // from m0, columns from c0. A lane has four columns of row l % 16 of each fragment.
-// Rows that went through LDS to be stored took 4096 x 4096 x 12288 338 us, not 312
-// (with bias and tanh GELU 345, 320).
+// Rows that went through LDS to be stored took 4096 x 4096 x 12288 317 us, not 309,
+// and 4096 x 512 x 4096 29, not 22.5.
 template <int EM, int TN, bool GU, bool RESID>
 __device__ __forceinline__ void linear_store_tile(const LinearArgs& p, const v4f (&sum)[EM][TN], int part, int64_t m0,
                                                   int here, int w0, int c0) {
@@ -265,11 +265,11 @@ __device__ __forceinline__ void linear_store_tile(const LinearArgs& p, const v4f
 // So every load has a step and a half to land.
 //
 // 256 x 256 tiles: 4096 x 4096 x 12288 303 to 313 by card, 1.32 to 1.36 PFLOP/s (the
-// library's product 330), 8192 x 8192 x 8192 743 (715). MFMA busy two thirds of the
-// cycles at 1.9 to 2.0 GHz; with operands of zeros the same code takes 257, so a fifth
-// of the time is the clock that the power leaves. Without the epilogue 278. Four
-// waves of 128 x 128, which read a third less LDS, run the same main loop in the same
-// time and a longer epilogue (322).
+// library's product 330 in one call after another), 8192 x 8192 x 8192 743 to 761
+// (715). MFMA busy two thirds of the cycles at 1.9 to 2.0 GHz; with operands of zeros
+// the same code takes 257, so a fifth of the time is the clock that the power leaves.
+// Without the epilogue 278. Four waves of 128 x 128, which read a third less LDS, run
+// the main loop in the same time and a longer epilogue (322 against 309).
 template <class T, bool GU, bool RESID>
 __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(const LinearArgs p, int tiles_m,
                                                                                 int tiles_n) {
@@ -577,21 +577,20 @@ __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p) 
         all([](const AnyRow& row, int k) { return any_load(row, k); });
       else
         all([&](const AnyRow& row, int k) { return any_load_tail(row, k, p.k); });
-      return;
     } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      // chunks past the end of k: an offset that reads zeros
-      const int past = SK * s + SK / 2 * h + k_lane >= p.k ? (int)0x80000000u : 0;
+      for (int h = 0; h < 2; ++h) {
+        // chunks past the end of k: an offset that reads zeros
+        const int past = SK * s + SK / 2 * h + k_lane >= p.k ? (int)0x80000000u : 0;
+        auto load8 = [&](__amdgpu_buffer_rsrc_t rsrc, int voff) {
+          return __builtin_bit_cast(
+              u4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (voff + SK * h) | past, s * (2 * SK), 0));
+        };
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        b.w[j][h] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(
-                                               GU && j >= NG ? w2_rsrc : w_rsrc, (w_voff[j % NG] + SK * h) | past, s * (2 * SK), 0));
+        for (int j = 0; j < NT; ++j) b.w[j][h] = load8(GU && j >= NG ? w2_rsrc : w_rsrc, w_voff[j % NG]);
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-        b.a[i][h] = __builtin_bit_cast(
-            u4, __builtin_amdgcn_raw_buffer_load_b128(a_rsrc, (a_voff[i] + SK * h) | past, s * (2 * SK), 0));
-    }
+        for (int i = 0; i < MT; ++i) b.a[i][h] = load8(a_rsrc, a_voff[i]);
+      }
     }
   };
   v4f acc[MT][NT];
@@ -684,7 +683,6 @@ hipError_t launch_any(const LinearArgs& p, hipStream_t stream) {
   linear_any_kernel<GU><<<grid, 256, 0, stream>>>(p);
   return hipGetLastError();
 }
-
 
 constexpr int64_t kCus = 256;
 

@@ -15,12 +15,12 @@
 // weights' bytes, and the output is rounded once.
 //
 // Hidden 2048, width 768, 128 experts, top-8, weights from memory, in a graph: one
-// token 17 us (9.7 and 7.3; 38 MB), sixteen 79 (46 and 33; 83 experts, 390 MB, 5
+// token 17 us (11 and 6; 38 MB), sixteen 78 (49 and 25; 83 experts, 390 MB, 5
 // TB/s). What it took: loads without branches between them (a branch makes the
 // compiler wait for each, 5 us of the first launch at one token); one workgroup per
 // CU over units with the next one's weights on their way (sixteen tokens' first
-// launch 57 -> 46); the parts' sums by device-scope atomics instead of fences that
-// write back whole caches (the second launch 143 -> 66 -> 33).
+// launch 57 -> 49); the parts' sums by device-scope atomics instead of fences that
+// write back whole caches (the second launch 143 -> 66 -> 25).
 #include "f8.hpp"
 #include "linear.hpp"
 #include "moe_few_f8.hpp"
@@ -37,7 +37,7 @@ constexpr int kTokens = kMoeFewTokens, kMaxExperts = kMoeFewExperts;
 struct FewTable {
   int count;
   int expert[kMaxExperts];
-  int16_t slot[kMaxExperts][kTokens];
+  alignas(8) int16_t slot[kMaxExperts][kTokens];
 };
 
 // Routing of all tokens, in LDS of each workgroup of 512 threads, by expert.
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(512) void few_down_kernel(const MoeFewArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const FewLane<R> me;
   __shared__ int experts[kMaxExperts];
-  __shared__ int16_t slots[kMaxExperts][kTokens];
+  __shared__ __align__(8) int16_t slots[kMaxExperts][kTokens];
   const FewTable& table = *static_cast<const FewTable*>(a.table);
   {  // all of the table with one round trip (entries past the last are not used)
     const int e = table.expert[tid % kMaxExperts];
@@ -497,12 +497,12 @@ constexpr int kCus = 256, kMostTiles = 32768 / 8, kMostParts = 16;
 constexpr size_t kTableBytes = (sizeof(FewTable) + 255) / 256 * 256, kArrivedBytes = kMostTiles * 4;
 
 // The tiles of the output and their parts, as many as fill the CUs (a workgroup each:
-// 16 x 2048 x 768, 64 tiles, 79 us in 4 parts, 83 in 8, 87 in 16) but of 70 KB of
+// 16 x 2048 x 768, 64 tiles, 78 us in 4 parts, 81 in 8, 91 in 2) but of 70 KB of
 // weights at least, for joining them takes 2 us (two tokens of 4 of 64 experts, 512 x
-// 512, 32 KB per tile: 10.4 whole, 12.3 in 4 parts; nine of 4 of 128, 256 x 2048, 2 MB
-// per tile: 46 in 4 parts, 27 in 16). Up to 16 routes: 8 columns, whose workgroups hold
-// all of h's few rows on their way (one token of 8 experts 17.0 against 18.5 on 32
-// columns, two 24.3 and 26.0; three 31.1 and 30.4).
+// 512, 32 KB per tile: 10.4 whole, 12.2 in 4 parts; nine of 4 of 128, 256 x 2048, 2 MB
+// per tile: 77 whole, 34 in 4 parts, 27 in 16). Up to 16 routes: 8 columns, whose
+// workgroups hold all of h's few rows on their way (one token of 8 experts 17.0, on 32
+// columns 18.4; two 24.2 and 24.5; three 30.6 and 29.7).
 struct FewDown {
   bool small;
   int tiles, parts;

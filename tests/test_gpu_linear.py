@@ -296,6 +296,19 @@ def test_linear_of_no_rows():
     x, w = torch.empty((0, 64), dtype=BF, device="cuda"), randn((8, 64), 1.0, 1)
     assert clef_i4.linear(x, w).shape == (0, 8)
     assert clef_i4.linear_gate_up(x, w, w).shape == (0, 8)
+    moe, _ = layer(8, 64, 128, 2, "f32", 1, router=w)
+    assert moe.decode(x).shape == (0, 64)
+    assert moe.decode(x, torch.empty((0, 8), device="cuda"), residual=x).shape == (0, 64)
+
+
+@pytest.mark.parametrize("m,k", [(5, 72), (130, 1032), (300, 77)])
+def test_one_tensor_as_several_operands(m, k):
+    """x is its own weight and its own residual; gate and up are x too."""
+    x = randn((m, max(m, k)), 0.1, m)[:, :k]
+    check(clef_i4.linear(x, x, x[0, :1].expand(m).contiguous(), "silu"), *linear64(x, x, x[0, :1].expand(m), "silu"))
+    check(clef_i4.linear_gate_up(x, x, x), *gate_up64(x, x, x))
+    w = randn((k, k), 0.1, k)
+    check(clef_i4.linear(x, w, residual=x), *linear64(x, w, residual=x))
 
 
 def test_linear_rows_far_apart():
