@@ -10,51 +10,35 @@ namespace clef {
 
 namespace {
 
-// Rows that start at any even byte: eight values from column k (a multiple of 8) on
-// are loaded as the five dwords that hold them and shifted into place at their use
-// (16-byte loads from odd multiples of two bytes took three times as long: 512 x
-// 2049 x 4096 104 us on 64 x 64 tiles, 512 x 2050 x 4096 42).
-struct AnyRow {
-  const char* down;  // the row's start, rounded down to 4 bytes
-  int shift;         // bits of the first dword in front of the row: 0 or 16
-  __device__ __forceinline__ explicit AnyRow(const uint16_t* row)
-      : down(reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)3)),
-        shift((int)(reinterpret_cast<uintptr_t>(row) & 2) * 8) {}
-  AnyRow() = default;
-};
-
-struct AnyEight {
-  u4 low;
-  uint32_t high;
-  __device__ __forceinline__ u4 values(int shift) const {
-    return u4{__builtin_amdgcn_alignbit(low[1], low[0], shift), __builtin_amdgcn_alignbit(low[2], low[1], shift),
-              __builtin_amdgcn_alignbit(low[3], low[2], shift), __builtin_amdgcn_alignbit(high, low[3], shift)};
-  }
-};
-
-// k + 8 <= K. (Without a shift the fifth dword is not used, and may lie past the end.)
-__device__ __forceinline__ AnyEight any_load(const AnyRow& r, int k) {
-  typedef u4 __attribute__((aligned(4))) u4_any;
-  const char* at = r.down + 2 * (int64_t)k;
-  return {*reinterpret_cast<const u4_any*>(at), *reinterpret_cast<const uint32_t*>(at + 12 + r.shift / 4)};
+// Eight values of a row that starts at any even byte.
+__device__ __forceinline__ u4 any_load(const uint16_t* from) {
+  u4 v;
+  __builtin_memcpy(&v, from, 16);
+  return v;
 }
 
-// Any k: zeros past column K. Dwords past the row's last value are read there, so that
-// no branch makes the loads wait for each other.
-__device__ __forceinline__ AnyEight any_load_tail(const AnyRow& r, int k, int K) {
-  const int odd = r.shift / 16, last = (2 * (K - 1 + odd)) & ~3;  // of the dword that holds value K - 1
+// From column k on, a multiple of 8: zeros past column K. The dwords that hold them,
+// those past the row's last value read there (so that no branch makes the loads wait
+// for each other), shifted into place.
+__device__ __forceinline__ u4 any_load_tail(const uint16_t* row, int k, int K) {
+  const char* const down = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)3);
+  const int odd = (int)(reinterpret_cast<uintptr_t>(row) & 2) / 2;
+  const int last = (2 * (K - 1 + odd)) & ~3;  // of the dword that holds value K - 1
   uint32_t d[5];
 #pragma unroll
   for (int j = 0; j < 5; ++j) {
     const int at = 2 * k + 4 * j;
-    d[j] = *reinterpret_cast<const uint32_t*>(r.down + (at < last ? at : last));
+    d[j] = *reinterpret_cast<const uint32_t*>(down + (at < last ? at : last));
   }
 #pragma unroll
   for (int j = 0; j < 5; ++j) {
     const int left = K - k + odd - 2 * j;  // halves of this dword that are values
     d[j] = left >= 2 ? d[j] : left == 1 ? d[j] & 0xFFFFu : 0u;
   }
-  return {u4{d[0], d[1], d[2], d[3]}, d[4]};
+  u4 v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_alignbit(d[j + 1], d[j], 16 * odd);
+  return v;
 }
 
 // Many rows of any alignment: 64 rows x 64 weight rows (gate/up: 32 gate and 32 up)
@@ -81,22 +65,19 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinearArgs p) {
     wr[i] = (GU && i ? p.w2 : p.w) + (col < p.n ? col : p.n - 1) * p.w_stride;
   }
   u4 xv[2], wv[2];
-  // (16-byte loads of any alignment: here eight lanes take 128 bytes in a row, and the
-  // dwords of AnyRow took 160 us where these take 122, 512 x 2049 x 17408)
   auto load = [&](int k0) {
     const int k = k0 + 8 * chunk;
     if (k0 + 64 <= p.k) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        __builtin_memcpy(&xv[i], xr[i] + k, 16);
-        __builtin_memcpy(&wv[i], wr[i] + k, 16);
+        xv[i] = any_load(xr[i] + k);
+        wv[i] = any_load(wr[i] + k);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const AnyRow x(xr[i]), w(wr[i]);
-        xv[i] = any_load_tail(x, k, p.k).values(x.shift);
-        wv[i] = any_load_tail(w, k, p.k).values(w.shift);
+        xv[i] = any_load_tail(xr[i], k, p.k);
+        wv[i] = any_load_tail(wr[i], k, p.k);
       }
     }
   };
@@ -500,99 +481,117 @@ hipError_t launch_tile(const LinearArgs& p, hipStream_t stream) {
 
 // Few rows: a workgroup owns R MT rows x R NT weight rows (gate/up: NT / 2 fragments
 // of gate rows and the same of up), its eight waves split k in steps (wave w: steps w,
-// w + 8, ..), D steps of each on their way. Operands go straight into registers: a
-// weight row is used by this workgroup's rows only. The waves' sums meet in LDS and
-// are added in wave order (the result does not depend on timing).
+// w + 8, ..), D steps of each on their way in registers. Eight lanes load 128 bytes of
+// a row in a row; through LDS of its own, with no barrier, a wave turns them into
+// fragments, whose lanes hold 16 bytes of a row each. (Loads in the fragments' order,
+// whose neighbouring lanes lie in different rows, go through the address unit lane
+// by lane, 33 bytes per ns and CU: 37 x 4160 x 1352 10.3, so 8.2; 64 x 4096 x 12288
+// 40.7, 28.2; 100 x 2048 x 768 7.6, 4.5.) The waves' sums meet in LDS and are added in
+// wave order (the result does not depend on timing).
 //
-// R, the weight rows per fragment: 16, or 8 for up to 8 rows of x. A fragment of 8
-// rows holds two pieces of k of each, lanes lr / 8 of both operands piece lr / 8: of
-// the 16 x 16 sums the two blocks on the diagonal count, one per piece. So twice as
-// many tiles share the bytes, and a load takes 128 contiguous bytes of a row. One row,
-// R = 16, 8 and 4, the best of one to four fragments each: 2048 x 128 4.5, 3.4, 3.2; 4096
-// x 12288 22.4, 18.5 (5.4 TB/s), 21.8; 17408 x 5120 38.9, 37.4, 35.8; gate/up 5120 x 2
-// 17408 70.3, 65.5, 89.8. Two steps on their way gain where a step is one fragment
-// (4096 x 12288 21.8, 18.5) and nothing in larger ones.
+// R, the weight rows per fragment: 16, or 8 for up to 16 rows of x. A fragment of 8
+// rows holds two pieces of k of each: of the 16 x 16 sums the two blocks on the
+// diagonal count, one per piece. So twice as many tiles share the bytes. One row, R = 8
+// and 16: 2048 x 128 2.9, 3.5; 4096 x 12288 19.1 (5.3 TB/s), 20.4; 17408 x 5120 35.9, 43.3.
+// Two steps on their way gain where a step is one fragment (4096 x 12288 21.1, 19.1)
+// and nothing in larger ones.
 //
-// ANY: rows that start at any even byte (AnyRow).
+// together: an XCD's workgroups take tiles whose weight rows are the same one after
+// another, as far as the weights are more than the output (37 x 4160 x 1352 8.2, 7.1;
+// 49 x 8752 x 10278 on 16 x 16 tiles 140, 96; but 200 x 512 x 8192 13.5, 15.0).
+//
+// ANY: rows that start at any even byte. 16-byte loads there take twice the time of
+// aligned ones (64 x 4097 x 1025 12.6, 64 x 4096 x 1024 7).
 template <bool ANY, int R, int MT, int NT, int D, bool GU>
-__global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p) {
+__global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p, bool together) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int NW = 8, Q = 16 / R, NG = GU ? NT / 2 : NT, BM = R * MT, COLS = R * NG;
   constexpr int SK = 64 * Q;  // k per step
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, g = lane >> 4;
-  const int64_t m0 = (int64_t)blockIdx.y * BM;
-  const int n0 = blockIdx.x * COLS;
+  int tm = blockIdx.y, tn = blockIdx.x;
+  if (together) tile_of_block(blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y, gridDim.y, gridDim.x, tm, tn);
+  const int64_t m0 = (int64_t)tm * BM;
+  const int n0 = tn * COLS;
   const int here = p.m - m0 < BM ? (int)(p.m - m0) : BM, cols = p.n - n0 < COLS ? p.n - n0 : COLS;
   const int steps = (p.k + SK - 1) / SK;
-  const int fr = lr % R, k_lane = 8 * (lr / R * 4 + g);  // row in the fragment, first k of this lane in a step's half
+  // Load h of a fragment: eight rows of 128 bytes, row lane / 8 (R = 16: + 8 h), the
+  // lane's 16 bytes at k = k_lane (R = 8: + 64 h) of a step.
+  constexpr int HR = R / 8;  // rows of a fragment per lane
+  const int k_lane = 8 * (lane & 7);
+  auto row_of = [&](int fragment, int h, int rows) {  // rows past the end repeat the last
+    const int r = R * fragment + 8 * h + (lane >> 3);
+    return r < rows ? r : rows - 1;
+  };
   const __amdgpu_buffer_rsrc_t a_rsrc =
       make_rsrc(p.x + m0 * p.x_stride, (uint32_t)(((here - 1) * p.x_stride + p.k) * 2));
   const uint32_t w_bytes = (uint32_t)(((cols - 1) * p.w_stride + p.k) * 2);
   const __amdgpu_buffer_rsrc_t w_rsrc = make_rsrc(p.w + n0 * p.w_stride, w_bytes);
   const __amdgpu_buffer_rsrc_t w2_rsrc = make_rsrc(GU ? p.w2 + n0 * p.w_stride : p.w, GU ? w_bytes : 0);
-  int a_voff[MT], w_voff[NG];  // rows past the end repeat the last
+  int a_voff[MT][HR], w_voff[NG][HR];
+  const uint16_t *a_row[ANY ? MT : 1][HR], *w_row[ANY ? NT : 1][HR];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int r = R * i + fr < here ? R * i + fr : here - 1;
-    a_voff[i] = (int)(r * p.x_stride + k_lane) * 2;
-  }
-#pragma unroll
-  for (int j = 0; j < NG; ++j) {
-    const int r = R * j + fr < cols ? R * j + fr : cols - 1;
-    w_voff[j] = (int)(r * p.w_stride + k_lane) * 2;
-  }
-  using Eight = std::conditional_t<ANY, AnyEight, u4>;
-  struct Step {
-    Eight w[NT][2], a[MT][2];
-  } ring[D];
-  AnyRow a_row[ANY ? MT : 1], w_row[ANY ? NT : 1];
-  if constexpr (ANY) {
+  for (int h = 0; h < HR; ++h) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const int r = R * i + fr < here ? R * i + fr : here - 1;
-      a_row[i] = AnyRow(p.x + (m0 + r) * p.x_stride);
+      const int64_t r = row_of(i, h, here);
+      if constexpr (ANY) a_row[i][h] = p.x + (m0 + r) * p.x_stride;
+      else a_voff[i][h] = (int)(r * p.x_stride + k_lane) * 2;
     }
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int r = R * (j % NG) + fr < cols ? R * (j % NG) + fr : cols - 1;
-      w_row[j] = AnyRow((GU && j >= NG ? p.w2 : p.w) + (n0 + r) * p.w_stride);
+    for (int j = 0; j < (ANY ? NT : NG); ++j) {
+      const int64_t r = row_of(j % NG, h, cols);
+      if constexpr (ANY) w_row[j][h] = (GU && j >= NG ? p.w2 : p.w) + (n0 + r) * p.w_stride;
+      else w_voff[j][h] = (int)(r * p.w_stride + k_lane) * 2;
     }
   }
+  struct Step {
+    u4 w[NT][2], a[MT][2];
+  } ring[D];
   auto load = [&](Step& b, int s) {
     if (s >= steps) return;
     if constexpr (ANY) {
       auto all = [&](auto load8) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int k = SK * s + SK / 2 * h + k_lane;
+          const int k = SK * s + 64 * (R == 8 ? h : 0) + k_lane;
 #pragma unroll
-          for (int j = 0; j < NT; ++j) b.w[j][h] = load8(w_row[j], k);
+          for (int j = 0; j < NT; ++j) b.w[j][h] = load8(w_row[j][h % HR], k);
 #pragma unroll
-          for (int i = 0; i < MT; ++i) b.a[i][h] = load8(a_row[i], k);
+          for (int i = 0; i < MT; ++i) b.a[i][h] = load8(a_row[i][h % HR], k);
         }
       };
       if (SK * (s + 1) <= p.k)
-        all([](const AnyRow& row, int k) { return any_load(row, k); });
+        all([](const uint16_t* row, int k) { return any_load(row + k); });
       else
-        all([&](const AnyRow& row, int k) { return any_load_tail(row, k, p.k); });
+        all([&](const uint16_t* row, int k) { return any_load_tail(row, k, p.k); });
     } else {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        constexpr int PIECE = R == 8 ? 128 : 0;  // bytes of a row between the loads
         // chunks past the end of k: an offset that reads zeros
-        const int past = SK * s + SK / 2 * h + k_lane >= p.k ? (int)0x80000000u : 0;
+        const int past = SK * s + PIECE / 2 * h + k_lane >= p.k ? (int)0x80000000u : 0;
         auto load8 = [&](__amdgpu_buffer_rsrc_t rsrc, int voff) {
           return __builtin_bit_cast(
-              u4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (voff + SK * h) | past, s * (2 * SK), 0));
+              u4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (voff + PIECE * h) | past, s * (2 * SK), 0));
         };
 #pragma unroll
-        for (int j = 0; j < NT; ++j) b.w[j][h] = load8(GU && j >= NG ? w2_rsrc : w_rsrc, w_voff[j % NG]);
+        for (int j = 0; j < NT; ++j) b.w[j][h] = load8(GU && j >= NG ? w2_rsrc : w_rsrc, w_voff[j % NG][h % HR]);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) b.a[i][h] = load8(a_rsrc, a_voff[i]);
+        for (int i = 0; i < MT; ++i) b.a[i][h] = load8(a_rsrc, a_voff[i][h % HR]);
       }
     }
   };
+  // This wave's fragments in LDS, 2 KiB each: 16 rows (R = 8: row r's piece q is row 8 q
+  // + r) of 64 k, 16-byte chunk c of row r at c ^ ((r >> 1) & 7).
+  char* const stage = lds + wave * ((MT + NT) * 2048);
+  const int put_at = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 4)) << 4);
+  const int get_at = lr * 128 + ((g ^ (lr >> 1)) << 4);
+  auto put = [&](int fragment, int h, u4 v) {
+    *reinterpret_cast<u4*>(stage + fragment * 2048 + h * 1024 + (put_at ^ (h * 64))) = v;
+  };
+  auto get = [&](int fragment, int h) { return *reinterpret_cast<const u4*>(stage + fragment * 2048 + (get_at ^ (h * 64))); };
   v4f acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -606,29 +605,33 @@ __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p) 
       if (s + NW * d >= steps) break;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) put(j, h, ring[d].w[j][h]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) put(NT + i, h, ring[d].a[i][h]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load(ring[d], s + NW * (d + D));
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
         u4 w[NT], a[MT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          if constexpr (ANY) w[j] = ring[d].w[j][h].values(w_row[j].shift);
-          else w[j] = ring[d].w[j][h];
-        }
+        for (int j = 0; j < NT; ++j) w[j] = get(j, h);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          if constexpr (ANY) a[i] = ring[d].a[i][h].values(a_row[i].shift);
-          else a[i] = ring[d].a[i][h];
-        }
+        for (int i = 0; i < MT; ++i) a[i] = get(NT + i, h);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int j = 0; j < NT; ++j) acc[i][j] = mfma_bf16(w[j], a[i], acc[i][j]);
       }
-      __builtin_amdgcn_sched_barrier(0);
-      load(ring[d], s + NW * (d + D));
-      __builtin_amdgcn_sched_barrier(0);
     }
   }
-  // the waves' sums: fragment (i, j) of wave w at ((w MT + i) NT + j) KiB
-  v4f* sums = reinterpret_cast<v4f*>(lds);
+  // the waves' sums: fragment (i, j) of wave w at ((w MT + i) NT + j) KiB, behind the
+  // stages (0.1 us less) or, to leave room for other workgroups, over them
+  constexpr bool BEHIND = MT * NT == 1;
+  if constexpr (!BEHIND) __syncthreads();
+  v4f* sums = reinterpret_cast<v4f*>(lds + (BEHIND ? NW * (MT + NT) * 2048 : 0));
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -656,14 +659,16 @@ __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p) 
 
 template <bool ANY, int R, int MT, int NT, int D, bool GU>
 hipError_t launch_stream(const LinearArgs& p, hipStream_t stream) {
-  constexpr int COLS = R * NT / (GU ? 2 : 1), lds = 8 * MT * NT * 1024;
+  constexpr int COLS = R * NT / (GU ? 2 : 1);
+  constexpr int sums = 8 * MT * NT * 1024, stages = 8 * (MT + NT) * 2048, lds = MT * NT == 1 ? sums + stages : sums > stages ? sums : stages;
   static LaunchCache cache;
   auto* kernel = &linear_stream_kernel<ANY, R, MT, NT, D, GU>;
   if (lds > 64 * 1024)
     if (hipError_t e = ensure_dynamic_lds(cache, reinterpret_cast<const void*>(kernel), lds)) return e;
   const int64_t tiles_m = (p.m + R * MT - 1) / (R * MT);
   if (tiles_m > 65535) return hipErrorInvalidValue;
-  kernel<<<dim3((unsigned)((p.n + COLS - 1) / COLS), (unsigned)tiles_m), 512, lds, stream>>>(p);
+  kernel<<<dim3((unsigned)((p.n + COLS - 1) / COLS), (unsigned)tiles_m), 512, lds, stream>>>(
+      p, tiles_m > 1 && p.k >= 4 * p.m);
   return hipGetLastError();
 }
 
@@ -686,7 +691,9 @@ hipError_t launch_any(const LinearArgs& p, hipStream_t stream) {
 
 constexpr int64_t kCus = 256;
 
-enum class LinearKernel { any, s8x8, s8x16, s16x16, s16x32, s16x64, s32x64, s64x64, t128x128, t128x128k, t256x256, t128x256 };
+enum class LinearKernel {
+  any, s8x8, s8x16, s16x16, s16x32, s32x16, s32x32, s64x32, s64x64, t128x128, t128x128k, t256x256, t128x256
+};
 
 struct LinearPlan {
   LinearKernel kernel;
@@ -695,23 +702,26 @@ struct LinearPlan {
 
 // The kernel for a product of m rows against n weight rows (gate/up: both), and the
 // parts that k is split into: of the kernels' times as modelled here, in us, the least.
-// The model's rates are measured ones:
-//  * few rows: a CU takes 33 bytes per ns of weights and rows (48 where fewer than 175
-//    CUs do, 22 of AnyRow's), 2 us to start and end, 2 us to join a tile of 64 x 64;
+// The model's rates are measured ones, fitted to 8 to 12 kernels' times at 310 random
+// shapes:
+//  * few rows: a CU takes 80 bytes per ns of weights and rows (64 x 64: 60; all
+//    together 15 TB/s; rows of any alignment 51 and 10), 2 us to sum and store 64 x 64, a part of a round's
+//    start that another workgroup does not hide;
 //  * tiles: a start and an end, and a step of 64 k each (two workgroups of 128 x 128
 //    per CU: 1.0 for both); split, another launch that reads what they wrote;
-//  * either no faster than memory, by the CUs that have a tile.
-// What it decides, in both forms: 64 x 17408 x 5120 on 64 x 64 tiles of few rows 101, on
-// 128 x 128 tiles in 6 parts 43.5; 200 x 17408 x 5120 whole 140, in 3 parts 67; 620 x
-// 17408 x 5120 on 128 x 128 tiles 150, on 256 x 256 in 4 parts 125; 512 x 4096 x 4096
-// 40, in 2 parts 32; 37 x 4160 x 1352 on 16 x 16 tiles 10.6, on 128 x 128 in 12 parts
-// 13.1. Over 160 random shapes its choice takes 0.7 % longer than the best of twenty
-// fixed ones (2.6 % over 40 of odd widths).
+//  * either no faster than memory (tiles: by the CUs that have one).
+// What it decides, in both forms: 37 x 4160 x 1352 on 16 x 16 tiles 7.2, 32 x 16 8.9, 128
+// x 128 in parts 12.2; 24 x 4096 x 4096 12.5 on 16 x 16, 10.3 on 16 x 32; 64 x 4096 x
+// 12288 on 64 x 64 28.6, on 32 x 32 31.6, on 128 x 128 33.7; 64 x 17408 x 5120 on 64 x
+// 32 67, on 128 x 128 in parts 43.8; 200 x 17408 x 5120 on 64 x 64 128, on 128 x 256 in
+// parts 64; 512 x 4096 x 4096 on 64 x 64 39.3, on 128 x 128 in parts 31.4; 620 x 17408 x
+// 5120 on 128 x 128 150, on 256 x 256 in 4 parts 125; 512 x 2049 x 4096, of any alignment,
+// on 64 x 32 52, on 64 x 64 through LDS shared by the waves 33.5. Over 220 other
+// random shapes its choice takes 2.5 % longer than the best of eight to twelve kernels.
 LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up, bool aligned) {
-  if (m <= 8) return {gate_up || (m > 4 && rows_of_w > 8192) ? LinearKernel::s8x16 : LinearKernel::s8x8, 1};
   auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((rows_of_w + bn - 1) / bn); };
   auto rounds = [](int64_t workgroups, int64_t at_once) { return (float)((workgroups + at_once - 1) / at_once); };
-  const float memory = ((float)(rows_of_w + m) * k + (float)m * rows_of_w) * 2 / 4.9e6f;
+  const float bytes = ((float)(rows_of_w + m) * k + (float)m * rows_of_w) * 2;
   LinearPlan best{LinearKernel::any, 1};
   float least = __builtin_huge_valf();
   auto consider = [&](LinearKernel kernel, int parts, float t) {
@@ -719,27 +729,40 @@ LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up, bool a
     least = t;
     best = {kernel, parts};
   };
-  // the bytes that the product cannot do without, shared by the CUs as the tiles are
-  auto from_memory = [&](int64_t workgroups) { return memory * rounds(workgroups, kCus) * kCus / workgroups; };
-  auto stream = [&](LinearKernel kernel, int bm, int bn) {
-    if (m > 4096) return;  // (a launch has 65535 tiles of rows)
+  // (at_once: workgroups that a CU holds)
+  auto stream = [&](LinearKernel kernel, int bm, int bn, int at_once) {
     const int64_t of = tiles(bm, bn);
-    const float r = rounds(of, kCus), rate = of < 175 ? 48e3f : of < kCus ? 8.4e6f / of : 33e3f;
-    const float loads = r * (bm + bn) * k * 2 / (aligned ? rate : 22e3f), least_t = from_memory(of);
-    const float joins = r * (bm * bn) * (2.0f / 4096);
-    consider(kernel, 1, 2 + joins + (loads > least_t ? loads : least_t) + (aligned ? 0 : 5 * (r - 1)));
+    const float r = rounds(of, kCus), cus = of < kCus ? of : kCus, all = (aligned ? 15e6f : 10e6f) / cus;
+    const float most = !aligned ? 51e3f : bm * bn == 4096 ? 60e3f : 80e3f, rate = most < all ? most : all;
+    const float t = r * ((bm + bn) * k * 2 / rate + bm * bn * (aligned ? 2.1f : 3.9f) / 4096) +
+                    (r - 1) * (aligned ? 0.7f : 3.2f) / at_once + (bm == 8 ? 0.4f : 0);
+    const float least_t = bytes / (bm == 8 && m > 8 ? 3.4e6f : 3.9e6f);
+    consider(kernel, 1, (aligned ? 2.1f : 2.8f) + k * 1.2e-4f + (t > least_t ? t : least_t));
   };
-  if (!gate_up) stream(LinearKernel::s16x16, 16, 16);
-  stream(LinearKernel::s16x32, 16, 32);
-  stream(LinearKernel::s16x64, 16, 64);
-  stream(LinearKernel::s32x64, 32, 64);
-  if (aligned) stream(LinearKernel::s64x64, 64, 64);  // (64 rows of AnyRow do not fit the registers)
+  // (of kernels that memory holds alike the first: gate/up 3 x 472 x 2 12506 on 16 x 32
+  // tiles 7.9, on 8 x 16 12.1; projections 1 x 5512 x 7229 on 8 x 8 17.5, on 16 x 16 19.5)
+  if (m <= 16 && !gate_up) {
+    stream(LinearKernel::s8x8, 8, 8, 4);
+    stream(LinearKernel::s8x16, 8, 16, 3);
+  }
+  if (m <= 4096) {  // (a launch has 65535 tiles of rows)
+    if (!gate_up) stream(LinearKernel::s16x16, 16, 16, 4);
+    stream(LinearKernel::s16x32, 16, 32, 3);
+    if (m <= 16 && gate_up) stream(LinearKernel::s8x16, 8, 16, 3);
+    if (!gate_up) stream(LinearKernel::s32x16, 32, 16, 3);
+    stream(LinearKernel::s32x32, 32, 32, 2);
+    stream(LinearKernel::s64x32, 64, 32, 1);
+    // (64 x 64 of any alignment does not fit the registers)
+    if (aligned) stream(LinearKernel::s64x64, 64, 64, 1);
+  }
   const int steps = (k + 63) / 64;
   if (!aligned) {
     const float r = rounds(tiles(64, 64), kCus);
     consider(LinearKernel::any, 1, 3 + 1.2f * r + steps * (0.42f * r > 0.9f ? 0.42f * r : 0.9f));
     return best;
   }
+  if (m <= 8) return best;  // (no scratch)
+  auto from_memory = [&](int64_t workgroups) { return bytes / 4.9e6f * rounds(workgroups, kCus) * kCus / workgroups; };
   auto tile = [&](LinearKernel kernel, int bm, int bn, float start, float step, float pair) {
     const int64_t of = tiles(bm, bn);
     for (int parts : {1, 2, 3, 4, 6, 8}) {
@@ -777,11 +800,12 @@ hipError_t launch_rows(LinearArgs& p, void* workspace, hipStream_t stream) {
     switch (plan.kernel) {
       case LinearKernel::s8x8: if constexpr (!GU) return launch_stream<ANY, 8, 1, 1, 2, GU>(p, stream);
       case LinearKernel::s8x16: return launch_stream<ANY, 8, 1, 2, 1, GU>(p, stream);
-      case LinearKernel::s16x16: if constexpr (!GU) return launch_stream<ANY, 16, 1, 1, 1, GU>(p, stream);
+      case LinearKernel::s16x16: if constexpr (!GU) return launch_stream<ANY, 16, 1, 1, 2, GU>(p, stream);
       case LinearKernel::s16x32: return launch_stream<ANY, 16, 1, 2, 1, GU>(p, stream);
-      case LinearKernel::s16x64: return launch_stream<ANY, 16, 1, 4, 1, GU>(p, stream);
+      case LinearKernel::s32x16: if constexpr (!GU) return launch_stream<ANY, 16, 2, 1, 1, GU>(p, stream);
+      case LinearKernel::s32x32: return launch_stream<ANY, 16, 2, 2, 1, GU>(p, stream);
       case LinearKernel::s64x64: if constexpr (!ANY) return launch_stream<ANY, 16, 4, 4, 1, GU>(p, stream);
-      default: return launch_stream<ANY, 16, 2, 4, 1, GU>(p, stream);
+      default: return launch_stream<ANY, 16, 4, 2, 1, GU>(p, stream);
     }
   };
   switch (plan.kernel) {
@@ -803,8 +827,8 @@ size_t linear_workspace_bytes(int64_t m, int n, int k, bool gate_up) {
 }
 
 const char* linear_kernel_name(int64_t m, int n, int k, bool gate_up, bool aligned) {
-  static const char* const names[] = {"any",   "8x8",     "8x16",     "16x16",   "16x32",  "16x64",
-                                      "32x64", "64x64", "128x128", "128x128x2", "256x256", "128x256"};
+  static const char* const names[] = {"any",   "8x8",   "8x16",    "16x16",     "16x32",   "32x16", "32x32",
+                                      "64x32", "64x64", "128x128", "128x128x2", "256x256", "128x256"};
   return names[(int)linear_plan(m, (int64_t)n * (gate_up ? 2 : 1), k, gate_up, aligned).kernel];
 }
 

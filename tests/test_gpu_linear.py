@@ -135,19 +135,20 @@ def test_linear_of_whole_numbers_is_exact(m, k, n):
 
 # rows, k, columns, the kernel that the rule picks and the parts of k: every kernel
 # with ends inside its tile and its last step (projections, gate/up)
-KERNELS = ([(3, 200, 43, "8x8", 1), (7, 136, 8209, "8x16", 1), (11, 72, 45, "16x16", 1), (19, 72, 2059, "16x32", 1),
-            (35, 72, 8201, "16x64", 1), (17, 72, 12301, "32x64", 1), (51, 72, 12301, "64x64", 1), (525, 136, 6003, "128x128", 1),
-            (9, 8200, 45, "128x128", 8), (133, 2056, 8203, "128x128x2", 1), (131, 8200, 3001, "128x128x2", 4),
-            (403, 1032, 8203, "128x256", 1), (131, 8200, 4107, "128x256", 6), (1303, 264, 6001, "256x256", 1),
-            (401, 4104, 8203, "256x256", 3)],
-           [(5, 72, 43, "8x16", 1), (11, 72, 45, "16x32", 1), (19, 72, 2059, "16x64", 1), (33, 72, 3001, "32x64", 1),
-            (33, 136, 6003, "64x64", 1), (33, 520, 8203, "128x128", 1), (9, 4104, 43, "128x128", 8),
+KERNELS = ([(3, 776, 41, "8x8", 1), (9, 8200, 45, "8x8", 1), (7, 648, 2563, "8x16", 1), (11, 72, 45, "16x16", 1),
+            (11, 72, 4099, "16x32", 1), (29, 72, 2981, "32x16", 1), (29, 72, 4141, "32x32", 1), (45, 72, 5483, "64x32", 1),
+            (51, 648, 8203, "64x64", 1), (525, 136, 6003, "128x128", 1), (9, 6152, 8097, "128x128", 4),
+            (133, 2056, 8203, "128x128x2", 1), (131, 8200, 3001, "128x128x2", 4), (403, 1032, 8203, "128x256", 1),
+            (131, 8200, 4107, "128x256", 6), (1303, 264, 6001, "256x256", 1), (401, 4104, 8203, "256x256", 3)],
+           [(5, 392, 43, "8x16", 1), (9, 4104, 43, "8x16", 1), (11, 72, 45, "16x32", 1), (29, 72, 2059, "32x32", 1),
+            (45, 72, 2837, "64x32", 1), (51, 648, 4155, "64x64", 1), (141, 72, 9001, "128x128", 1), (9, 6472, 3991, "128x128", 4),
             (131, 2056, 4107, "128x128x2", 1), (131, 4104, 3001, "128x128x2", 2), (133, 1032, 8203, "128x256", 1),
             (131, 4104, 4107, "128x256", 3), (403, 264, 8203, "256x256", 1), (131, 4104, 8203, "256x256", 3)])
 # the same for rows that start at any even byte
-ODD_KERNELS = ([(3, 201, 43, "8x8"), (7, 137, 8209, "8x16"), (11, 73, 45, "16x16"), (19, 73, 2059, "16x32"), (21, 73, 4107, "16x64"),
-                (18, 73, 8203, "32x64"), (500, 1001, 2059, "any")],
-               [(5, 73, 43, "8x16"), (11, 73, 45, "16x32"), (19, 73, 2059, "16x64"), (21, 73, 4107, "32x64"), (300, 1001, 2059, "any")])
+ODD_KERNELS = ([(3, 349, 43, "8x8"), (7, 913, 2059, "8x16"), (11, 73, 45, "16x16"), (11, 73, 4099, "16x32"), (17, 77, 3269, "32x16"),
+                (29, 85, 4115, "32x32"), (45, 89, 4099, "64x32"), (500, 1001, 2059, "any")],
+               [(5, 77, 43, "8x16"), (11, 81, 45, "8x16"), (17, 81, 41, "16x32"), (29, 89, 2067, "32x32"), (45, 85, 2075, "64x32"),
+                (300, 1001, 2059, "any")])
 
 
 @pytest.mark.parametrize("m,k,n", [c[:3] for c in KERNELS[0] + ODD_KERNELS[0]])

@@ -80,16 +80,16 @@ def test_outputs_over_operands_are_refused():
 
 @pytest.mark.parametrize("call_it,gate_up_it", [(linear, 0), (gate_up, 1)])
 def test_workspace(call_it, gate_up_it):
-    shape = dict(m=200, n=512, k=8192)
-    need = clef_i4.lib().clef_linear_workspace_bytes(200, 512, 8192, gate_up_it)
-    assert need > 0 and need % (200 * 512 * 4 * (1 + gate_up_it)) == 0
+    shape = dict(m=200, n=2048, k=8192)
+    need = clef_i4.lib().clef_linear_workspace_bytes(200, 2048, 8192, gate_up_it)
+    assert need > 0 and need % (200 * 2048 * 4 * (1 + gate_up_it)) == 0
     assert call_it(**shape, nbytes=need - 1) == (-1, "workspace too small")
     for ws_at in (None, 5 * FAR + 8):
         rc, msg = call_it(**shape, ws_at=ws_at)
         assert rc == -1 and "aligned" in msg
     for at in (FAKE, FAR, 2 * FAR):  # x, a weight, the output
         assert call_it(**shape, ws_at=at + 16) == (-1, "linear workspace overlaps an operand")
-    for bad in ((0, 512, 8192), (200, 0, 8192), (200, 512, 0), (1 << 21, 512, 8192), (8, 512, 8192), (200, 512, 64)):
+    for bad in ((0, 2048, 8192), (200, 0, 8192), (200, 2048, 0), (1 << 21, 2048, 8192), (8, 2048, 8192), (200, 2048, 64)):
         assert clef_i4.lib().clef_linear_workspace_bytes(*bad, gate_up_it) == 0
 
 
@@ -98,7 +98,7 @@ def test_kernel_name_and_every_kernel_is_compared_with_a_reference():
     from test_gpu_linear import KERNELS, ODD_KERNELS
 
     lib = clef_i4.lib()
-    few = {"8x16", "16x32", "16x64", "32x64"}
+    few = {"8x16", "16x32", "32x32", "64x32"}
     for bad in ((0, 8, 8), (8, 0, 8), (8, 8, 0), (1 << 21, 8, 8)):
         assert lib.clef_linear_kernel_name(*bad, 0, 1) == b""
     for gate_up_it in (0, 1):
@@ -109,13 +109,13 @@ def test_kernel_name_and_every_kernel_is_compared_with_a_reference():
             assert need == (parts * (1 + gate_up_it) * m * -(-n // 4) * 16 if parts > 1 else 0), (m, k, n)
             seen.add((name, parts > 1))
         tiles = {"128x128", "128x128x2", "128x256", "256x256"}
-        whole = few | {"64x64"} | tiles | (set() if gate_up_it else {"8x8", "16x16"})
+        whole = few | {"64x64"} | tiles | (set() if gate_up_it else {"8x8", "16x16", "32x16"})
         assert seen == {(t, False) for t in whole} | {(t, True) for t in tiles}
         odd = set()
         for m, k, n, name in ODD_KERNELS[gate_up_it]:
             assert lib.clef_linear_kernel_name(m, n, k, gate_up_it, 1).decode() == name, (m, k, n)
             odd.add(name)
-        assert odd == few | {"any"} | (set() if gate_up_it else {"8x8", "16x16"})
+        assert odd == few | {"any"} | (set() if gate_up_it else {"8x8", "16x16", "32x16"})
 
 
 def few(x=FAKE, xs=None, logits=FAR, dtype=0, t=4, hidden=256, inter=128, experts=8, topk=2, gate=2 * FAR, gs=3 * FAR,
