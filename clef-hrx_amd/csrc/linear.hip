@@ -334,7 +334,8 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
-  auto body = [&](char* __restrict__ r0, char* __restrict__ r1) {
+  auto body = [&](auto fragments, char* __restrict__ r0, char* __restrict__ r1) {
+    constexpr int LIVE = decltype(fragments)::value;
     u4 av[2][2], bv[TN][2];
     auto read_a = [&](const char* stage, int i, u4 (&v)[2]) {
       v[0] = *reinterpret_cast<const u4*>(stage + a_at + i * 2048 + swz);
@@ -356,19 +357,17 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(
       for (int i = 0; i < TM; ++i) {
         if (i == TM / 2 - 1) landed();  // this stage's Y; its X has been read
         if (i == TM - 1) landed();      // the next stage's X; this stage has been read
-        if (i + 1 < TM)
-          read_a(cur, i + 1, av[(i + 1) & 1]);
-        else
-          read_a(next, 0, av[(i + 1) & 1]);
+        if (i + 1 < LIVE) read_a(cur, i + 1, av[(i + 1) & 1]);
+        if (LIVE && i + 1 == TM) read_a(next, 0, av[0]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; i < LIVE && h < 2; ++h) {
             acc[i][j] = mfma_bf16(bv[j][h], av[i & 1][h], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
           }
-          if (i == TM - 1) read_b(next, j, bv[j]);
+          if (LIVE && i == TM - 1) read_b(next, j, bv[j]);
           // X behind the first barrier, Y behind the second
           constexpr int SPAN = TM / 2 * TN;
           const int u = (i - (TM / 2 - 1)) * TN + j;
@@ -390,15 +389,26 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(
     wait_vmcnt<T::DMA>();
     asm volatile("s_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    read_a(r0, 0, av[0]);
+    if constexpr (LIVE > 0) {
+      read_a(r0, 0, av[0]);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) read_b(r0, j, bv[j]);
+      for (int j = 0; j < TN; ++j) read_b(r0, j, bv[j]);
+    }
     for (int kt = 0; kt < steps; kt += 2) {
       step(r0, r1, kt);
       if (kt + 1 < steps) step(r1, r0, kt + 1);
     }
   };
-  body(lds, lds + T::STAGE_BYTES);
+  // A wave with rows or columns past the end multiplies half of its fragments or none,
+  // and shares the loads and barriers of the others (620 x 17408 x 5120 in 4 parts 125,
+  // so 117; 300 x 5120 x 17408 on 128 x 128 tiles 89, 86).
+  const int rows_left = here - wm * T::WM, cols_left = cols - wn * (GU ? T::WN / 2 : T::WN);
+  if (rows_left <= 0 || cols_left <= 0)
+    body(std::integral_constant<int, 0>{}, lds, lds + T::STAGE_BYTES);
+  else if (rows_left <= T::WM / 2)
+    body(std::integral_constant<int, TM / 2>{}, lds, lds + T::STAGE_BYTES);
+  else
+    body(std::integral_constant<int, TM>{}, lds, lds + T::STAGE_BYTES);
 
   constexpr int EM = TM / T::KG;  // rows of fragments that this wave stores, from fragment kg EM
   constexpr int NC = GU ? TN / 2 : TN;
@@ -715,7 +725,7 @@ struct LinearPlan {
 // 12288 on 64 x 64 28.6, on 32 x 32 31.6, on 128 x 128 33.7; 64 x 17408 x 5120 on 64 x
 // 32 67, on 128 x 128 in parts 43.8; 200 x 17408 x 5120 on 64 x 64 128, on 128 x 256 in
 // parts 64; 512 x 4096 x 4096 on 64 x 64 39.3, on 128 x 128 in parts 31.4; 620 x 17408 x
-// 5120 on 128 x 128 150, on 256 x 256 in 4 parts 125; 512 x 2049 x 4096, of any alignment,
+// 5120 on 128 x 128 159, on 256 x 256 in 4 parts 117; 512 x 2049 x 4096, of any alignment,
 // on 64 x 32 52, on 64 x 64 through LDS shared by the waves 33.5. Over 220 other
 // random shapes its choice takes 2.5 % longer than the best of eight to twelve kernels.
 LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up, bool aligned) {
