@@ -59,15 +59,22 @@ hipError_t resident_per_cu(LaunchCache& c, const void* kern, int threads, int ld
 // launchers keep tiles_m * tiles_n below 2^31 (kMaxTiles), and 64-bit
 // divisions here cost the persistent kernels registers they spill.
 constexpr int64_t kMaxTiles = (int64_t)1 << 30;
-__device__ __forceinline__ void tile_of_block(int b, int blocks, int tiles_m, int tiles_n, int& tm, int& tn) {
+__device__ __forceinline__ int place_of_block(int b, int blocks) {
   const int per = blocks / 8;
-  const int r = b < 8 * per ? (b % 8) * per + b / 8 : b;
+  return b < 8 * per ? (b % 8) * per + b / 8 : b;
+}
+
+__device__ __forceinline__ void tile_of_place(int r, int tiles_m, int tiles_n, int& tm, int& tn) {
   const int band = 8 * tiles_n;
   const int group = r / band, within = r - group * band;
   const int first = group * 8;
   const int height = tiles_m - first < 8 ? tiles_m - first : 8;
   tm = first + within % height;
   tn = within / height;
+}
+
+__device__ __forceinline__ void tile_of_block(int b, int blocks, int tiles_m, int tiles_n, int& tm, int& tn) {
+  tile_of_place(place_of_block(b, blocks), tiles_m, tiles_n, tm, tn);
 }
 
 }  // namespace

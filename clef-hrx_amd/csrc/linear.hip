@@ -262,8 +262,10 @@ __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(
   const int kg = T::KG == 1 ? 0 : wave / T::NWB, wb = wave % T::NWB;  // group, wave in it
   const int wm = wb / T::WAVES_N, wn = wb % T::WAVES_N;
   int tm, tn;
-  const int tiles = tiles_m * tiles_n, part = p.parts == 1 ? 0 : blockIdx.x / tiles;
-  tile_of_block(blockIdx.x - part * tiles, tiles, tiles_m, tiles_n, tm, tn);
+  // (an XCD takes tiles of one part: 620 x 17408 x 5120 in 4 parts 113, so 111)
+  const int tiles = tiles_m * tiles_n, place = place_of_block(blockIdx.x, gridDim.x);
+  const int part = p.parts == 1 ? 0 : place / tiles;
+  tile_of_place(place - part * tiles, tiles_m, tiles_n, tm, tn);
   const int64_t m0 = (int64_t)tm * T::BM;
   const int n0 = tn * COLS;
   const int here = p.m - m0 < T::BM ? (int)(p.m - m0) : T::BM, cols = p.n - n0 < COLS ? p.n - n0 : COLS;
@@ -725,7 +727,7 @@ struct LinearPlan {
 // 12288 on 64 x 64 28.6, on 32 x 32 31.6, on 128 x 128 33.7; 64 x 17408 x 5120 on 64 x
 // 32 67, on 128 x 128 in parts 43.8; 200 x 17408 x 5120 on 64 x 64 128, on 128 x 256 in
 // parts 64; 512 x 4096 x 4096 on 64 x 64 39.3, on 128 x 128 in parts 31.4; 620 x 17408 x
-// 5120 on 128 x 128 159, on 256 x 256 in 4 parts 117; 512 x 2049 x 4096, of any alignment,
+// 5120 on 128 x 128 159, on 256 x 256 in 4 parts 111; 512 x 2049 x 4096, of any alignment,
 // on 64 x 32 52, on 64 x 64 through LDS shared by the waves 33.5. Over 220 other
 // random shapes its choice takes 2.5 % longer than the best of eight to twelve kernels.
 LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up, bool aligned) {
