@@ -41,27 +41,31 @@ __device__ __forceinline__ u4 any_load_tail(const uint16_t* row, int k, int K) {
   return v;
 }
 
-// Many rows of any alignment: 64 rows x 64 weight rows (gate/up: 32 gate and 32 up)
-// per workgroup of four waves, 64 k at a time through registers into one LDS stage
-// (16-byte chunk c of row r at c ^ ((r >> 1) & 7)), the next 64 k on their way
-// meanwhile. 512 x 2049 x 17408 123 us, 0.3 PFLOP/s.
-template <bool GU>
-__global__ __launch_bounds__(256) void linear_any_kernel(const LinearArgs p) {
+// Many rows of any alignment: 32 TM rows x 32 WN weight rows (gate/up: half of them
+// gate and half up) per workgroup of 2 x WN waves, 64 k at a time through registers
+// into one LDS stage (16-byte chunk c of row r at c ^ ((r >> 1) & 7)), the next 64 k
+// on their way meanwhile. Bound by the loads, which take twice the time of aligned
+// ones: 4096 x 4097 x 4097 on 64 x 64 434 us, on 128 x 128 290 (0.47 PFLOP/s), on 256 x
+// 256, of which a CU holds one, 410; 512 x 4097 x 2049, 68 tiles of 128 x 128, 62 and 88.
+template <int TM, int WN, bool GU>
+__global__ __launch_bounds__(128 * WN) void linear_any_kernel(const LinearArgs p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  __shared__ __align__(16) char lds[2 * 64 * 128];
+  constexpr int BM = 32 * TM, BN = 32 * WN, HALF = 16 * WN;  // HALF: rows of a load of all threads
+  static_assert(BM == BN, "two loads of either operand per thread");
+  __shared__ __align__(16) char lds[(BM + BN) * 128];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, g = lane >> 4;
-  const int wm = wave >> 1, wn = wave & 1;
-  constexpr int COLS = GU ? 32 : 64;
-  const int64_t m0 = (int64_t)blockIdx.y * 64;
+  const int wm = wave / WN, wn = wave % WN;
+  constexpr int COLS = GU ? HALF : BN;
+  const int64_t m0 = (int64_t)blockIdx.y * BM;
   const int n0 = blockIdx.x * COLS;
-  // this thread's chunks: chunk threadIdx.x % 8 of rows threadIdx.x / 8 and + 32
+  // this thread's chunks: chunk threadIdx.x % 8 of rows threadIdx.x / 8 and + HALF
   const int chunk = threadIdx.x & 7;
   const uint16_t *xr[2], *wr[2];  // rows past the end repeat the last
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int r = (threadIdx.x >> 3) + 32 * i;
+    const int r = (threadIdx.x >> 3) + HALF * i;
     xr[i] = p.x + (m0 + r < p.m ? m0 + r : p.m - 1) * p.x_stride;
-    const int col = n0 + (GU ? r % 32 : r);
+    const int col = n0 + (GU ? r % HALF : r);
     wr[i] = (GU && i ? p.w2 : p.w) + (col < p.n ? col : p.n - 1) * p.w_stride;
   }
   u4 xv[2], wv[2];
@@ -81,37 +85,36 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinearArgs p) {
       }
     }
   };
-  v4f acc[2][2] = {};
+  v4f acc[TM][2] = {};
   load(0);
   for (int k0 = 0; k0 < p.k; k0 += 64) {
     if (k0) __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = (threadIdx.x >> 3) + 32 * i, at = r * 128 + ((chunk ^ ((r >> 1) & 7)) << 4);
+      const int r = (threadIdx.x >> 3) + HALF * i, at = r * 128 + ((chunk ^ ((r >> 1) & 7)) << 4);
       *reinterpret_cast<u4*>(lds + at) = xv[i];
-      *reinterpret_cast<u4*>(lds + 8192 + at) = wv[i];
+      *reinterpret_cast<u4*>(lds + BM * 128 + at) = wv[i];
     }
     __syncthreads();
     if (k0 + 64 < p.k) load(k0 + 64);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      u4 a[2], b[2];
+      u4 a[TM], b[2];
+      const int off = ((4 * s + g) ^ (lr >> 1)) << 4;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int off = ((4 * s + g) ^ (lr >> 1)) << 4;
-        a[i] = *reinterpret_cast<const u4*>(lds + (32 * wm + 16 * i + lr) * 128 + off);
-        // gate/up: this wave's 16 gate rows, then its 16 up rows
-        b[i] = *reinterpret_cast<const u4*>(lds + 8192 + ((GU ? 32 * i + 16 * wn : 32 * wn + 16 * i) + lr) * 128 + off);
-      }
+      for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const u4*>(lds + (16 * (TM * wm + i) + lr) * 128 + off);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int j = 0; j < 2; ++j)  // gate/up: this wave's 16 gate rows, then its 16 up rows
+        b[j] = *reinterpret_cast<const u4*>(lds + (BM + (GU ? HALF * j + 16 * wn : 32 * wn + 16 * j) + lr) * 128 + off);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = mfma_bf16(b[j], a[i], acc[i][j]);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t row = m0 + 32 * wm + 16 * i + lr;
+  for (int i = 0; i < TM; ++i) {
+    const int64_t row = m0 + 16 * (TM * wm + i) + lr;
     if (row >= p.m) continue;
     if constexpr (GU) {
       linear_epilogue4<true>(p, row, n0 + 16 * wn + 4 * g, acc[i][0], acc[i][1]);
@@ -603,7 +606,9 @@ __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p, 
   auto put = [&](int fragment, int h, u4 v) {
     *reinterpret_cast<u4*>(stage + fragment * 2048 + h * 1024 + (put_at ^ (h * 64))) = v;
   };
-  auto get = [&](int fragment, int h) { return *reinterpret_cast<const u4*>(stage + fragment * 2048 + (get_at ^ (h * 64))); };
+  auto get = [&](int fragment, int h) {
+    return *reinterpret_cast<const u4*>(stage + fragment * 2048 + (get_at ^ (h * 64)));
+  };
   v4f acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -672,7 +677,8 @@ __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p, 
 template <bool ANY, int R, int MT, int NT, int D, bool GU>
 hipError_t launch_stream(const LinearArgs& p, hipStream_t stream) {
   constexpr int COLS = R * NT / (GU ? 2 : 1);
-  constexpr int sums = 8 * MT * NT * 1024, stages = 8 * (MT + NT) * 2048, lds = MT * NT == 1 ? sums + stages : sums > stages ? sums : stages;
+  constexpr int sums = 8 * MT * NT * 1024, stages = 8 * (MT + NT) * 2048;
+  constexpr int lds = MT * NT == 1 ? sums + stages : sums > stages ? sums : stages;
   static LaunchCache cache;
   auto* kernel = &linear_stream_kernel<ANY, R, MT, NT, D, GU>;
   if (lds > 64 * 1024)
@@ -693,18 +699,18 @@ bool rows_of_16(const LinearArgs& p) {
          p.x_stride <= most && p.w_stride <= most;
 }
 
-template <bool GU>
+template <int TM, int WN, bool GU>
 hipError_t launch_any(const LinearArgs& p, hipStream_t stream) {
-  constexpr int COLS = GU ? 32 : 64;
-  const dim3 grid((unsigned)((p.n + COLS - 1) / COLS), (unsigned)((p.m + 63) / 64));
-  linear_any_kernel<GU><<<grid, 256, 0, stream>>>(p);
+  constexpr int BM = 32 * TM, COLS = GU ? 16 * WN : 32 * WN;
+  const dim3 grid((unsigned)((p.n + COLS - 1) / COLS), (unsigned)((p.m + BM - 1) / BM));
+  linear_any_kernel<TM, WN, GU><<<grid, 128 * WN, 0, stream>>>(p);
   return hipGetLastError();
 }
 
 constexpr int64_t kCus = 256;
 
 enum class LinearKernel {
-  any, s8x8, s8x16, s16x16, s16x32, s32x16, s32x32, s64x32, s64x64, t128x128, t128x128k, t256x256, t128x256
+  any, any128, s8x8, s8x16, s16x16, s16x32, s32x16, s32x32, s64x32, s64x64, t128x128, t128x128k, t256x256, t128x256
 };
 
 struct LinearPlan {
@@ -769,8 +775,9 @@ LinearPlan linear_plan(int64_t m, int64_t rows_of_w, int k, bool gate_up, bool a
   }
   const int steps = (k + 63) / 64;
   if (!aligned) {
-    const float r = rounds(tiles(64, 64), kCus);
+    const float r = rounds(tiles(64, 64), kCus), r128 = rounds(tiles(128, 128), kCus);
     consider(LinearKernel::any, 1, 3 + 1.2f * r + steps * (0.42f * r > 0.9f ? 0.42f * r : 0.9f));
+    consider(LinearKernel::any128, 1, 3 + 2.5f * r128 + steps * (0.9f * r128 > 1.3f ? 0.9f * r128 : 1.3f));
     return best;
   }
   if (m <= 8) return best;  // (no scratch)
@@ -825,7 +832,8 @@ hipError_t launch_rows(LinearArgs& p, void* workspace, hipStream_t stream) {
     case LinearKernel::t128x128k: return launch_parts<Tile128K, GU>(p, stream);
     case LinearKernel::t256x256: return launch_parts<Tile256, GU>(p, stream);
     case LinearKernel::t128x256: return launch_parts<Tile128x256, GU>(p, stream);
-    case LinearKernel::any: return launch_any<GU>(p, stream);
+    case LinearKernel::any: return launch_any<2, 2, GU>(p, stream);
+    case LinearKernel::any128: return launch_any<4, 4, GU>(p, stream);
     default: return aligned ? few(std::false_type{}) : few(std::true_type{});
   }
 }
@@ -839,8 +847,8 @@ size_t linear_workspace_bytes(int64_t m, int n, int k, bool gate_up) {
 }
 
 const char* linear_kernel_name(int64_t m, int n, int k, bool gate_up, bool aligned) {
-  static const char* const names[] = {"any",   "8x8",   "8x16",    "16x16",     "16x32",   "32x16", "32x32",
-                                      "64x32", "64x64", "128x128", "128x128x2", "256x256", "128x256"};
+  static const char* const names[] = {"any",   "any128", "8x8",   "8x16",    "16x16",      "16x32",   "32x16",
+                                      "32x32", "64x32",  "64x64", "128x128", "128x128x2", "256x256", "128x256"};
   return names[(int)linear_plan(m, (int64_t)n * (gate_up ? 2 : 1), k, gate_up, aligned).kernel];
 }
 

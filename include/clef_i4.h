@@ -629,9 +629,10 @@ size_t clef_linear_workspace_bytes(int64_t m, int32_t n, int32_t k, int32_t gate
 
 /* The tile (rows x weight rows) that the library's rule picks, for tests and
  * profiles: "8x8", "8x16", "16x16", "16x32", "32x16", "32x32", "64x32", "64x64",
- * "128x128", "128x128x2" (two steps of k at a time), "128x256", "256x256", "any" (64x64 for
- * operands of any alignment). aligned: every row of x and the weights starts on a
- * multiple of 16 bytes (as far as k % 8 == 0). "" for a shape the products reject. */
+ * "128x128", "128x128x2" (two steps of k at a time), "128x256", "256x256", "any" and
+ * "any128" (64x64 and 128x128 for operands of any alignment). aligned: every row of x
+ * and the weights starts on a multiple of 16 bytes (as far as k % 8 == 0). "" for a
+ * shape the products reject. */
 const char* clef_linear_kernel_name(int64_t m, int32_t n, int32_t k, int32_t gate_up, int32_t aligned);
 
 int clef_linear(const uint16_t* x, int64_t m, int32_t k, int64_t x_stride, const uint16_t* w, int32_t n,

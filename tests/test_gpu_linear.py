@@ -146,9 +146,9 @@ KERNELS = ([(3, 776, 41, "8x8", 1), (9, 8200, 45, "8x8", 1), (7, 648, 2563, "8x1
             (131, 4104, 4107, "128x256", 3), (403, 264, 8203, "256x256", 1), (131, 4104, 8203, "256x256", 3)])
 # the same for rows that start at any even byte
 ODD_KERNELS = ([(3, 349, 43, "8x8"), (7, 913, 2059, "8x16"), (11, 73, 45, "16x16"), (11, 73, 4099, "16x32"), (17, 77, 3269, "32x16"),
-                (29, 85, 4115, "32x32"), (45, 89, 4099, "64x32"), (500, 1001, 2059, "any")],
+                (29, 85, 4115, "32x32"), (45, 89, 4099, "64x32"), (500, 1001, 2059, "any"), (901, 137, 5003, "any128")],
                [(5, 77, 43, "8x16"), (11, 81, 45, "8x16"), (17, 81, 41, "16x32"), (29, 89, 2067, "32x32"), (45, 85, 2075, "64x32"),
-                (300, 1001, 2059, "any")])
+                (300, 1001, 2059, "any"), (901, 137, 3003, "any128")])
 
 
 @pytest.mark.parametrize("m,k,n", [c[:3] for c in KERNELS[0] + ODD_KERNELS[0]])
