@@ -515,9 +515,13 @@ hipError_t launch_tile(const LinearArgs& p, hipStream_t stream) {
 // another, as far as the weights are more than the output (37 x 4160 x 1352 8.2, 7.1;
 // 49 x 8752 x 10278 on 16 x 16 tiles 140, 96; but 200 x 512 x 8192 13.5, 15.0).
 //
+// ONCE: weight rows that one workgroup alone reads are loaded past the caches' usual
+// order (1 x 17408 x 5120 36.0, 32.2; 16 x 5120 x 17408 43.7, 39.5; 64 x 4096 x 12288 28.2, 26.7;
+// but rows that other workgroups read too, 64 x 4096 x 12288 on 16 x 16 tiles, 49, 53).
+//
 // ANY: rows that start at any even byte. 16-byte loads there take twice the time of
 // aligned ones (64 x 4097 x 1025 12.6, 64 x 4096 x 1024 7).
-template <bool ANY, int R, int MT, int NT, int D, bool GU>
+template <bool ANY, int R, int MT, int NT, int D, bool GU, bool ONCE>
 __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p, bool together) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int NW = 8, Q = 16 / R, NG = GU ? NT / 2 : NT, BM = R * MT, COLS = R * NG;
@@ -587,14 +591,16 @@ __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p, 
         constexpr int PIECE = R == 8 ? 128 : 0;  // bytes of a row between the loads
         // chunks past the end of k: an offset that reads zeros
         const int past = SK * s + PIECE / 2 * h + k_lane >= p.k ? (int)0x80000000u : 0;
-        auto load8 = [&](__amdgpu_buffer_rsrc_t rsrc, int voff) {
-          return __builtin_bit_cast(
-              u4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (voff + PIECE * h) | past, s * (2 * SK), 0));
+        auto load8 = [&](__amdgpu_buffer_rsrc_t rsrc, int voff, auto policy) {
+          return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (voff + PIECE * h) | past, s * (2 * SK),
+                                                                              decltype(policy)::value));
         };
+        const std::integral_constant<int, 0> usual{};
+        const std::integral_constant<int, ONCE ? 2 : 0> weights{};  // (2: non-temporal)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) b.w[j][h] = load8(GU && j >= NG ? w2_rsrc : w_rsrc, w_voff[j % NG][h % HR]);
+        for (int j = 0; j < NT; ++j) b.w[j][h] = load8(GU && j >= NG ? w2_rsrc : w_rsrc, w_voff[j % NG][h % HR], weights);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) b.a[i][h] = load8(a_rsrc, a_voff[i][h % HR]);
+        for (int i = 0; i < MT; ++i) b.a[i][h] = load8(a_rsrc, a_voff[i][h % HR], usual);
       }
     }
   };
@@ -674,13 +680,13 @@ __global__ __launch_bounds__(512) void linear_stream_kernel(const LinearArgs p, 
 #endif
 }
 
-template <bool ANY, int R, int MT, int NT, int D, bool GU>
-hipError_t launch_stream(const LinearArgs& p, hipStream_t stream) {
+template <bool ANY, int R, int MT, int NT, int D, bool GU, bool ONCE>
+hipError_t launch_stream_kernel(const LinearArgs& p, hipStream_t stream) {
   constexpr int COLS = R * NT / (GU ? 2 : 1);
   constexpr int sums = 8 * MT * NT * 1024, stages = 8 * (MT + NT) * 2048;
   constexpr int lds = MT * NT == 1 ? sums + stages : sums > stages ? sums : stages;
   static LaunchCache cache;
-  auto* kernel = &linear_stream_kernel<ANY, R, MT, NT, D, GU>;
+  auto* kernel = &linear_stream_kernel<ANY, R, MT, NT, D, GU, ONCE>;
   if (lds > 64 * 1024)
     if (hipError_t e = ensure_dynamic_lds(cache, reinterpret_cast<const void*>(kernel), lds)) return e;
   const int64_t tiles_m = (p.m + R * MT - 1) / (R * MT);
@@ -688,6 +694,18 @@ hipError_t launch_stream(const LinearArgs& p, hipStream_t stream) {
   kernel<<<dim3((unsigned)((p.n + COLS - 1) / COLS), (unsigned)tiles_m), 512, lds, stream>>>(
       p, tiles_m > 1 && p.k >= 4 * p.m);
   return hipGetLastError();
+}
+
+// ONCE from 16 MiB of weights on: fewer may still be in the last-level cache from the
+// call before, where it gains nothing (8 x 4096 x 12288 from there 19.0, 20.4) and where
+// others' data are kept from being pushed out. Loads of any alignment gain nothing by
+// it, and the rule takes 32 x 16 tiles for fewer weights only.
+template <bool ANY, int R, int MT, int NT, int D, bool GU>
+hipError_t launch_stream(const LinearArgs& p, hipStream_t stream) {
+  constexpr bool MAY = !ANY && !(MT == 2 && NT == 1);
+  if (MAY && p.m <= R * MT && (int64_t)p.n * p.k * (GU ? 4 : 2) >= 16 << 20)
+    return launch_stream_kernel<ANY, R, MT, NT, D, GU, MAY>(p, stream);
+  return launch_stream_kernel<ANY, R, MT, NT, D, GU, false>(p, stream);
 }
 
 // Whether both operands' rows start on multiples of 16 bytes, k is whole chunks of

@@ -213,12 +213,19 @@ struct FewLane {
   }
 };
 
+// 16 codes, which no other workgroup reads. ONCE: past the caches' usual order.
+template <bool ONCE>
+__device__ __forceinline__ v4i few_weights(const uint8_t* at) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const v4i*>(at));
+  return *reinterpret_cast<const v4i*>(at);
+}
+
 // Route, gate/up and SwiGLU. W waves split the blocks of k of 16 columns of h of one
 // expert named, wave w of them the blocks w, w + W, .., whose part of x stays in
 // registers (NB blocks; 0: any number, loaded each time); a unit is the 8 / W times 16
 // columns of the workgroup's waves. The next unit's weights are on their way while a
 // unit's sums meet in LDS, where one of the W waves in turn adds them in wave order.
-template <int W, int NB>
+template <int W, int NB, bool ONCE>
 __global__ __launch_bounds__(512) void few_gate_up_kernel(const MoeFewArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ FewRoutes routes;
@@ -266,7 +273,7 @@ __global__ __launch_bounds__(512) void few_gate_up_kernel(const MoeFewArgs a) {
     for (int m = 0; m < 2; ++m) {
       const uint8_t* at = (m ? a.up : a.gate) + block * 16384 + me.at(q.n0 & 127);
 #pragma unroll
-      for (int h = 0; h < H; ++h) q.w[i][m][h] = *reinterpret_cast<const v4i*>(at + 1024 * h);
+      for (int h = 0; h < H; ++h) q.w[i][m][h] = few_weights<ONCE>(at + 1024 * h);
       q.scale[i][m] = (m ? a.up_scales : a.gate_scales)[block];
     }
   };
@@ -350,7 +357,7 @@ __global__ __launch_bounds__(512) void few_gate_up_kernel(const MoeFewArgs a) {
 // block of k) of part blockIdx.y of gridDim.y are split among the eight waves, D on
 // their way; their sums meet in LDS. With several parts the last workgroup of a
 // tile to arrive adds the parts' sums, in their order.
-template <int R, int NT, int D>
+template <int R, int NT, int D, bool ONCE>
 __global__ __launch_bounds__(512) void few_down_kernel(const MoeFewArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ v4f sums[8][NT][64];
@@ -394,7 +401,7 @@ __global__ __launch_bounds__(512) void few_down_kernel(const MoeFewArgs a) {
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int h = 0; h < H; ++h)
-        p.w[j][h] = *reinterpret_cast<const v4i*>(a.down + block * 16384 + me.at((n0 & 127) + R * j) + 1024 * h);
+        p.w[j][h] = few_weights<ONCE>(a.down + block * 16384 + me.at((n0 & 127) + R * j) + 1024 * h);
 #pragma unroll
     for (int s = 0; s < 2 * H; ++s) {
       const int k = 128 * b + me.k + 64 * (s / 2) + 8 * (s % 2);
@@ -503,8 +510,12 @@ constexpr size_t kTableBytes = (sizeof(FewTable) + 255) / 256 * 256, kArrivedByt
 // per tile: 77 whole, 34 in 4 parts, 27 in 16). Up to 16 routes: 8 columns, whose
 // workgroups hold all of h's few rows on their way (one token of 8 experts 17.0, on 32
 // columns 18.4; two 24.2 and 24.5; three 30.6 and 29.7).
+//
+// once, how weights are loaded, from 64 MB of them on (four tokens 35.6, so 33.6;
+// sixteen 78.8, 74.4); fewer may still be in the last-level cache from the call before
+// (one token 17.1 and 16.7 from memory, 15.8 and 16.3 from there).
 struct FewDown {
-  bool small;
+  bool small, once;
   int tiles, parts;
 };
 FewDown few_down(int tokens, int topk, int experts, int hidden, int inter) {
@@ -512,10 +523,11 @@ FewDown few_down(int tokens, int topk, int experts, int hidden, int inter) {
   const int columns = small ? 8 : 32, tiles = (hidden + columns - 1) / columns;
   float others = 1.0f;  // that no token names an expert, evenly chosen
   for (int t = 0; t < tokens; ++t) others *= 1.0f - (float)topk / experts;
-  int parts = (int)((1.0f - others) * experts * inter * columns / 70e3f);
+  const float named = (1.0f - others) * experts;
+  int parts = (int)(named * inter * columns / 70e3f);
   parts = parts < kMostParts ? parts : kMostParts;
   parts = parts < kCus / tiles ? parts : kCus / tiles;
-  return {small, tiles, parts < 1 ? 1 : parts};
+  return {small, named * 3 * hidden * inter >= 64e6f, tiles, parts < 1 ? 1 : parts};
 }
 // f32 of each part: 16 (or 8) tokens of the tile's columns
 size_t few_partial_bytes(const FewDown& d) { return (size_t)d.tiles * d.parts * (d.small ? 8 * 8 : 16 * 32) * 4; }
@@ -526,6 +538,38 @@ size_t moe_few_workspace_bytes(int tokens, int topk, int experts, int hidden, in
   return kTableBytes + kArrivedBytes + few_partial_bytes(few_down(tokens, topk, experts, hidden, inter)) + (size_t)tokens * topk * inter * 4;
 }
 
+namespace {
+
+template <bool ONCE>
+hipError_t launch_few(const MoeFewArgs& a, const FewDown& down, hipStream_t stream) {
+  const int slots = a.tokens * a.topk, most = slots < a.experts ? slots : a.experts, kb = f8_blocks(a.hidden);
+  auto gate_up = [&](auto kernel, int columns) {
+    const int units = most * ((a.inter + columns - 1) / columns);
+    kernel<<<units < kCus ? units : kCus, 512, 0, stream>>>(a);
+  };
+  if (kb <= 2)
+    gate_up(few_gate_up_kernel<2, 1, ONCE>, 64);
+  else if (kb <= 4)
+    gate_up(few_gate_up_kernel<4, 1, ONCE>, 32);
+  else if (kb <= 8)
+    gate_up(few_gate_up_kernel<8, 1, ONCE>, 16);
+  else if (kb <= 16)
+    gate_up(few_gate_up_kernel<8, 2, ONCE>, 16);
+  else if (kb <= 32)
+    gate_up(few_gate_up_kernel<8, 4, ONCE>, 16);
+  else
+    gate_up(few_gate_up_kernel<8, 0, ONCE>, 16);
+  if (hipError_t e = hipGetLastError()) return e;
+  const dim3 grid(down.tiles, down.parts);
+  if (down.small)
+    few_down_kernel<8, 1, 2, ONCE><<<grid, 512, 0, stream>>>(a);
+  else
+    few_down_kernel<16, 2, 1, ONCE><<<grid, 512, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
 hipError_t launch_moe_few(MoeFewArgs a, void* workspace, hipStream_t stream) {
   const FewDown down = few_down(a.tokens, a.topk, a.experts, a.hidden, a.inter);
   char* at = static_cast<char*>(workspace);
@@ -534,30 +578,7 @@ hipError_t launch_moe_few(MoeFewArgs a, void* workspace, hipStream_t stream) {
   a.partial = at += kArrivedBytes;
   a.h = reinterpret_cast<uint16_t*>(at + few_partial_bytes(down));
   a.down_tiles = down.tiles;
-  const int slots = a.tokens * a.topk, most = slots < a.experts ? slots : a.experts, kb = f8_blocks(a.hidden);
-  auto gate_up = [&](auto kernel, int columns) {
-    const int units = most * ((a.inter + columns - 1) / columns);
-    kernel<<<units < kCus ? units : kCus, 512, 0, stream>>>(a);
-  };
-  if (kb <= 2)
-    gate_up(few_gate_up_kernel<2, 1>, 64);
-  else if (kb <= 4)
-    gate_up(few_gate_up_kernel<4, 1>, 32);
-  else if (kb <= 8)
-    gate_up(few_gate_up_kernel<8, 1>, 16);
-  else if (kb <= 16)
-    gate_up(few_gate_up_kernel<8, 2>, 16);
-  else if (kb <= 32)
-    gate_up(few_gate_up_kernel<8, 4>, 16);
-  else
-    gate_up(few_gate_up_kernel<8, 0>, 16);
-  if (hipError_t e = hipGetLastError()) return e;
-  const dim3 grid(down.tiles, down.parts);
-  if (down.small)
-    few_down_kernel<8, 1, 2><<<grid, 512, 0, stream>>>(a);
-  else
-    few_down_kernel<16, 2, 1><<<grid, 512, 0, stream>>>(a);
-  return hipGetLastError();
+  return down.once ? launch_few<true>(a, down, stream) : launch_few<false>(a, down, stream);
 }
 
 }  // namespace clef

@@ -151,7 +151,14 @@ ODD_KERNELS = ([(3, 349, 43, "8x8"), (7, 913, 2059, "8x16"), (11, 73, 45, "16x16
                 (300, 1001, 2059, "any"), (901, 137, 3003, "any128")])
 
 
-@pytest.mark.parametrize("m,k,n", [c[:3] for c in KERNELS[0] + ODD_KERNELS[0]])
+# weights of 16 MiB and more that one row of tiles reads
+ONCE = ([(1, 16880, 499, "8x8"), (1, 3368, 2497, "8x16"), (9, 3256, 2579, "16x16"), (1, 152, 55189, "16x32"),
+         (17, 1160, 7235, "32x32"), (33, 1984, 4277, "64x32"), (33, 592, 14251, "64x64")],
+        [(1, 6504, 645, "8x16"), (1, 640, 6555, "16x32"), (17, 824, 5141, "32x32"), (33, 2088, 2065, "64x32"),
+         (33, 608, 6903, "64x64")])
+
+
+@pytest.mark.parametrize("m,k,n", [c[:3] for c in KERNELS[0] + ODD_KERNELS[0] + ONCE[0]])
 def test_linear_on_every_kernel(m, k, n):
     seed = m * 17 + k * 3 + n
     x, w, r = randn((m, k), 1.0, seed), randn((n, k), k ** -0.5, seed + 1), randn((m, n), 1.0, seed + 3)
@@ -183,7 +190,7 @@ def test_linear_non_finite_values_on_every_kernel(m, k, n):
     assert (wide[m] == 7.0).all() and (wide[:, n:] == 7.0).all()
 
 
-@pytest.mark.parametrize("m,k,n", [c[:3] for c in KERNELS[1] + ODD_KERNELS[1]])
+@pytest.mark.parametrize("m,k,n", [c[:3] for c in KERNELS[1] + ODD_KERNELS[1] + ONCE[1]])
 def test_gate_up_on_every_kernel(m, k, n):
     seed = m * 11 + k * 3 + n
     x, wg, wu = randn((m, k), 1.0, seed), randn((n, k), k ** -0.5, seed + 1), randn((n, k), k ** -0.5, seed + 2)
@@ -447,6 +454,16 @@ def test_decode_matches_64_bits(t, hidden, inter, experts, topk, kind, dtype):
     moe, w = layer(experts, hidden, inter, topk, kind, t + hidden)
     x, logits, r = randn((t, hidden), 1.0, 1), randn((t, experts), 2.0, 2, dtype), randn((t, hidden), 1.0, 3)
     check(moe.decode(x, logits), *moe64(x, logits, *w, topk))
+    check(moe.decode(x, logits, residual=r), *moe64(x, logits, *w, topk, r))
+
+
+# 64 MB of experts' weights and more (named by evenly chosen routes), every width of hidden
+@pytest.mark.parametrize("t,hidden,inter,experts,topk", [(16, 200, 5128, 32, 4), (16, 504, 2056, 32, 4), (16, 1000, 1032, 32, 4),
+                                                         (2, 2048, 776, 32, 8), (5, 4096, 520, 16, 4), (5, 5000, 1032, 6, 2)])
+def test_decode_of_large_weights(t, hidden, inter, experts, topk):
+    assert experts * (1 - (1 - topk / experts) ** t) * 3 * hidden * inter >= 64e6
+    moe, w = layer(experts, hidden, inter, topk, "f32", t + hidden)
+    x, logits, r = randn((t, hidden), 1.0, 1), randn((t, experts), 2.0, 2, F32), randn((t, hidden), 1.0, 3)
     check(moe.decode(x, logits, residual=r), *moe64(x, logits, *w, topk, r))
 
 

@@ -95,7 +95,7 @@ def test_workspace(call_it, gate_up_it):
 
 def test_kernel_name_and_every_kernel_is_compared_with_a_reference():
     """The GPU tests' shapes run every kernel of either product, split and whole."""
-    from test_gpu_linear import KERNELS, ODD_KERNELS
+    from test_gpu_linear import KERNELS, ODD_KERNELS, ONCE
 
     lib = clef_i4.lib()
     few = {"8x16", "16x32", "32x32", "64x32"}
@@ -111,6 +111,10 @@ def test_kernel_name_and_every_kernel_is_compared_with_a_reference():
         tiles = {"128x128", "128x128x2", "128x256", "256x256"}
         whole = few | {"64x64"} | tiles | (set() if gate_up_it else {"8x8", "16x16", "32x16"})
         assert seen == {(t, False) for t in whole} | {(t, True) for t in tiles}
+        for m, k, n, name in ONCE[gate_up_it]:
+            assert lib.clef_linear_kernel_name(m, n, k, gate_up_it, 1).decode() == name, (m, k, n)
+            assert m <= int(name.split("x")[0]) and n * k * 2 * (1 + gate_up_it) >= 1 << 24
+        assert {c[3] for c in ONCE[gate_up_it]} == few | {"64x64"} | (set() if gate_up_it else {"8x8", "16x16"})
         odd = set()
         for m, k, n, name in ODD_KERNELS[gate_up_it]:
             assert lib.clef_linear_kernel_name(m, n, k, gate_up_it, 1).decode() == name, (m, k, n)
