@@ -507,7 +507,7 @@ hipError_t launch_tile(const LinearArgs& p, hipStream_t stream) {
 // R, the weight rows per fragment: 16, or 8 for up to 16 rows of x. A fragment of 8
 // rows holds two pieces of k of each: of the 16 x 16 sums the two blocks on the
 // diagonal count, one per piece. So twice as many tiles share the bytes. One row, R = 8
-// and 16: 2048 x 128 2.9, 3.5; 4096 x 12288 19.1 (5.3 TB/s), 20.4; 17408 x 5120 35.9, 43.3.
+// and 16: 2048 x 128 2.9, 3.5; 4096 x 12288 18.3 (5.5 TB/s), 18.5; 17408 x 5120 32.2, 40.3.
 // Two steps on their way gain where a step is one fragment (4096 x 12288 21.1, 19.1)
 // and nothing in larger ones.
 //

@@ -15,11 +15,11 @@
 // weights' bytes, and the output is rounded once.
 //
 // Hidden 2048, width 768, 128 experts, top-8, weights from memory, in a graph: one
-// token 17 us (11 and 6; 38 MB), sixteen 78 (49 and 25; 83 experts, 390 MB, 5
+// token 17 us (11 and 6; 38 MB), sixteen 74 (47 and 25; 83 experts, 390 MB, 5.3
 // TB/s). What it took: loads without branches between them (a branch makes the
 // compiler wait for each, 5 us of the first launch at one token); one workgroup per
 // CU over units with the next one's weights on their way (sixteen tokens' first
-// launch 57 -> 49); the parts' sums by device-scope atomics instead of fences that
+// launch 57 -> 47); the parts' sums by device-scope atomics instead of fences that
 // write back whole caches (the second launch 143 -> 66 -> 25).
 #include "f8.hpp"
 #include "linear.hpp"
