@@ -9,18 +9,19 @@
 // The rows stay bf16 (quantizing them would save no byte that counts): a weight's
 // e4m3 codes become bf16 on their way to the matrix unit, exact with the scale's
 // power of two, whose remaining factor enters the f32 sums behind each block of 128 k.
-// The router's probability goes into h (in f32, in front of its rounding), so that
-// the down products of all experts add up in one accumulator. h is held as two bf16
-// that together keep 16 bits of it: the second product costs nothing beside the
-// weights' bytes, and the output is rounded once.
+// The router's probability goes into h, in f32, so that the down products of all
+// experts add up in one accumulator. h stays f32: it is held as the three bf16 that
+// add up to it, whose products the matrix unit sums one by one, and the output is
+// rounded once. (Two bf16 keep 16 bits of h: the layer of one token takes 15.8 us with
+// them, 16.3 with three, that of sixteen 76.5 and 81.4.)
 //
 // Hidden 2048, width 768, 128 experts, top-8, weights from memory, in a graph: one
-// token 17 us (11 and 6; 38 MB), sixteen 74 (47 and 25; 83 experts, 390 MB, 5.3
+// token 16.4 us (10 and 6; 38 MB), sixteen 82 (48 and 28; 83 experts, 390 MB, 4.8
 // TB/s). What it took: loads without branches between them (a branch makes the
 // compiler wait for each, 5 us of the first launch at one token); one workgroup per
 // CU over units with the next one's weights on their way (sixteen tokens' first
 // launch 57 -> 47); the parts' sums by device-scope atomics instead of fences that
-// write back whole caches (the second launch 143 -> 66 -> 25).
+// write back whole caches (the second launch 143 -> 66, with h in two bf16).
 #include "f8.hpp"
 #include "linear.hpp"
 #include "moe_few_f8.hpp"
@@ -31,6 +32,7 @@ namespace clef {
 namespace {
 
 constexpr int kTokens = kMoeFewTokens, kMaxExperts = kMoeFewExperts;
+constexpr int kHParts = 3;  // bf16 that a value of h is held as
 
 // What the second launch takes from the first: the experts named, ascending, and for
 // each the rows of h of its tokens (-1: the token names others).
@@ -336,19 +338,23 @@ __global__ __launch_bounds__(512) void few_gate_up_kernel(const MoeFewArgs a) {
     }
     const float p = routes.p[t][e];
     uint16_t* at = a.h + (int64_t)(t * a.topk + routes.rank[t][e]) * a.inter + col;
-    const int64_t low = (int64_t)a.tokens * a.topk * a.inter;
-    uint2 hi, lo;
+    const int64_t plane = (int64_t)a.tokens * a.topk * a.inter;
     float y[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) y[s] = gate[s] * sigmoid_f32(gate[s]) * up[s] * p;
-    hi.x = pack_bf16x2(y[0], y[1]);
-    hi.y = pack_bf16x2(y[2], y[3]);
-    // (nothing is left of what became infinite)
-    auto left = [](float v, float r) { return __builtin_isinf(r) ? 0.0f : v - r; };
-    lo.x = pack_bf16x2(left(y[0], bf16_lo(hi.x)), left(y[1], bf16_hi(hi.x)));
-    lo.y = pack_bf16x2(left(y[2], bf16_lo(hi.y)), left(y[3], bf16_hi(hi.y)));
-    *reinterpret_cast<uint2*>(at) = hi;
-    *reinterpret_cast<uint2*>(at + low) = lo;
+    // The upper half of what is left, three times: each takes 8 of the 24 bits, and
+    // what it leaves is exact.
+#pragma unroll
+    for (int part = 0; part < kHParts; ++part) {
+      uint32_t top[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        top[s] = as_uint(y[s]) & 0xFFFF0000u;
+        // (nothing is left of an infinity)
+        y[s] = __builtin_isinf(y[s]) ? 0.0f : y[s] - as_float(top[s]);
+      }
+      *reinterpret_cast<uint2*>(at + part * plane) = uint2{top[1] | top[0] >> 16, top[3] | top[2] >> 16};
+    }
   }
 #endif
 }
@@ -378,14 +384,16 @@ __global__ __launch_bounds__(512) void few_down_kernel(const MoeFewArgs a) {
   const int kb = f8_blocks(a.inter), panels = f8_blocks(a.hidden), n0 = blockIdx.x * COLS;
   const int parts = gridDim.y, part = blockIdx.y, all = table.count * kb;
   const int q0 = all * part / parts, q1 = all * (part + 1) / parts;  // all <= 128 * 256
-  const int64_t low = (int64_t)a.tokens * a.topk * a.inter;
-  const __amdgpu_buffer_rsrc_t hr = make_rsrc(a.h, (uint32_t)(low * 2)), lr = make_rsrc(a.h + low, (uint32_t)(low * 2));
+  const int64_t plane = (int64_t)a.tokens * a.topk * a.inter;
+  const __amdgpu_buffer_rsrc_t hr[kHParts] = {make_rsrc(a.h, (uint32_t)(plane * 2)),
+                                              make_rsrc(a.h + plane, (uint32_t)(plane * 2)),
+                                              make_rsrc(a.h + 2 * plane, (uint32_t)(plane * 2))};
   __syncthreads();
   struct Pair {
     int slot;
     float scale;
     v4i w[NT][H];
-    u4 hi[2 * H], lo[2 * H];
+    u4 h[kHParts][2 * H];
   } ring[D];
   // Pairs of this wave in turn: expert i of those named, block b. (Loads without
   // branches, which would make them wait for each other: past the last pair the
@@ -407,8 +415,9 @@ __global__ __launch_bounds__(512) void few_down_kernel(const MoeFewArgs a) {
       const int k = 128 * b + me.k + 64 * (s / 2) + 8 * (s % 2);
       // tokens that name others: an offset that reads zeros
       const int at = (p.slot * a.inter + k) * 2 | ((p.slot | (a.inter - 1 - k)) & (int)0x80000000u);
-      p.hi[s] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(hr, at, 0, 0));
-      p.lo[s] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(lr, at, 0, 0));
+#pragma unroll
+      for (int part = 0; part < kHParts; ++part)
+        p.h[part][s] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(hr[part], at, 0, 0));
     }
     if (q + 8 < q1) {
       q += 8;
@@ -439,17 +448,17 @@ __global__ __launch_bounds__(512) void few_down_kernel(const MoeFewArgs a) {
       const FewScale scale = few_scale(p.scale);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        v4f sum = {0, 0, 0, 0};
+        v4f by[kHParts] = {};  // (one sum would make each MFMA wait for the one before)
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           u4 wv[2];
           few_bf16(p.w[n][h], scale.pow2, wv);
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            sum = mfma_bf16(wv[s], p.hi[2 * h + s], sum);
-            sum = mfma_bf16(wv[s], p.lo[2 * h + s], sum);
-          }
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int part = 0; part < kHParts; ++part) by[part] = mfma_bf16(wv[s], p.h[part][2 * h + s], by[part]);
         }
+        const v4f sum = by[0] + (by[1] + by[2]);
         // (a token's sum takes nothing of an expert it does not name, NaN weights neither)
         if (p.slot >= 0) {
 #pragma unroll
@@ -504,16 +513,16 @@ constexpr int kCus = 256, kMostTiles = 32768 / 8, kMostParts = 16;
 constexpr size_t kTableBytes = (sizeof(FewTable) + 255) / 256 * 256, kArrivedBytes = kMostTiles * 4;
 
 // The tiles of the output and their parts, as many as fill the CUs (a workgroup each:
-// 16 x 2048 x 768, 64 tiles, 78 us in 4 parts, 81 in 8, 91 in 2) but of 70 KB of
+// 16 x 2048 x 768, 64 tiles, 83 us in 4 parts, 85 in 8, 101 in 2) but of 70 KB of
 // weights at least, for joining them takes 2 us (two tokens of 4 of 64 experts, 512 x
-// 512, 32 KB per tile: 10.4 whole, 12.2 in 4 parts; nine of 4 of 128, 256 x 2048, 2 MB
-// per tile: 77 whole, 34 in 4 parts, 27 in 16). Up to 16 routes: 8 columns, whose
-// workgroups hold all of h's few rows on their way (one token of 8 experts 17.0, on 32
-// columns 18.4; two 24.2 and 24.5; three 30.6 and 29.7).
+// 512, 32 KB per tile: 10.5 whole, 12.2 in 4 parts; nine of 4 of 128, 256 x 2048, 2 MB
+// per tile: 92 whole, 38 in 4 parts, 28 in 16). Up to 16 routes: 8 columns, whose
+// workgroups hold all of h's few rows on their way (one token of 8 experts 16.7, on 32
+// columns 18.1; two 25.3 both; three 32.3 and 31.8).
 //
-// once, how weights are loaded, from 64 MB of them on (four tokens 35.6, so 33.6;
-// sixteen 78.8, 74.4); fewer may still be in the last-level cache from the call before
-// (one token 17.1 and 16.7 from memory, 15.8 and 16.3 from there).
+// once, how weights are loaded, from 64 MB of them on (four tokens 38.2, so 37.5;
+// sixteen 87, 82); fewer may still be in the last-level cache from the call before (one
+// token 16.6 and 17.4 from memory).
 struct FewDown {
   bool small, once;
   int tiles, parts;
@@ -535,7 +544,7 @@ size_t few_partial_bytes(const FewDown& d) { return (size_t)d.tiles * d.parts * 
 }  // namespace
 
 size_t moe_few_workspace_bytes(int tokens, int topk, int experts, int hidden, int inter) {
-  return kTableBytes + kArrivedBytes + few_partial_bytes(few_down(tokens, topk, experts, hidden, inter)) + (size_t)tokens * topk * inter * 4;
+  return kTableBytes + kArrivedBytes + few_partial_bytes(few_down(tokens, topk, experts, hidden, inter)) + (size_t)tokens * topk * inter * 2 * kHParts;
 }
 
 namespace {

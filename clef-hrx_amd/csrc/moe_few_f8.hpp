@@ -24,7 +24,7 @@ struct MoeFewArgs {
   int down_tiles;  // of the output, with several parts
   int* arrived;    // per tile, the parts done
   void* partial;   // their sums
-  uint16_t* h;     // bf16 [tokens * topk][inter], then what its rounding left
+  uint16_t* h;     // three times bf16 [tokens * topk][inter], their sum is h
 };
 
 size_t moe_few_workspace_bytes(int tokens, int topk, int experts, int hidden, int inter);

@@ -655,8 +655,8 @@ int clef_linear_gate_up(const uint16_t* x, int64_t m, int32_t k, int64_t x_strid
  * over them. Logits of NaN and -inf take no part, so a token may have fewer
  * experts or none (its output is the residual, or zero). Unlike the stages
  * (clef_moe_route .. clef_moe_combine) nothing is rounded on the way: the rows
- * stay bf16 as they are, probabilities and the sum over experts f32, h keeps 16
- * bits, the output is rounded once. residual bf16 [tokens][hidden], nullable; it
+ * stay bf16 as they are, probabilities, h and the sum over experts f32, the
+ * output is rounded once. residual bf16 [tokens][hidden], nullable; it
  * and x may be the output itself. Preconditions: 0 <= tokens <= 16, 1 <= topk <=
  * experts <= 128, hidden and inter as the FP8 widths, x_stride >= hidden, x_stride
  * % 8 == 0, x_stride <= 2^24 -> "unsupported MoE shape for few tokens"; pointers

@@ -488,6 +488,45 @@ def test_decode_of_whole_numbers_is_exact():
     assert torch.equal(moe.decode(x, logits), want.float().to(BF))
 
 
+@pytest.mark.parametrize("t,experts,hidden,inter", [(1, 4, 96, 128), (8, 3, 264, 136), (5, 8, 1000, 72), (16, 1, 48, 520),
+                                                    (9, 8, 256, 2048), (16, 12, 520, 1032)])
+def test_decode_keeps_every_bit_of_h(t, experts, hidden, inter):
+    """One expert per token (p = 1) and sums of whole numbers from 2^10 to 2^11, where
+    silu(g) = g in f32, so h = g u needs up to 22 bits. An output is the difference of
+    two columns of h, g u - (g - 1)(u + 1) = u + 1 - g, at most 100: every sum on the
+    way is a whole number below 2^23, the output itself a bf16."""
+    rng = torch.Generator().manual_seed(t * 1000 + inter)
+    triples, pairs = hidden // 3, inter // 2
+    g = torch.randint(1100, 1900, (experts, pairs, triples), generator=rng)
+    want = torch.randint(-100, 101, (experts, pairs, triples), generator=rng)
+    u = want + g - 1
+
+    def digits(a, b):
+        """Weights [experts][inter][hidden]: columns of h 2 i with sums a, 2 i + 1 with b, of three hexadecimal digits."""
+        v = torch.stack((a, b), 2).reshape(experts, inter, triples)
+        w = torch.zeros((experts, inter, hidden))
+        for at, shift in enumerate((8, 4, 0)):
+            w[:, :, at:3 * triples:3] = (v >> shift & 15).float()
+        return w
+
+    order = torch.randperm(inter, generator=rng)  # the columns of a pair lie anywhere
+    pair = torch.randint(0, pairs, (hidden,), generator=rng)
+    down = torch.zeros((experts, hidden, inter))
+    down[:, torch.arange(hidden), 2 * pair], down[:, torch.arange(hidden), 2 * pair + 1] = 1.0, -1.0
+    ones = [torch.ones((experts, -(-r // 128), -(-c // 128)), device="cuda") for r, c in ((inter, hidden), (hidden, inter))]
+    moe = clef_i4.MoeLayerF8(clef_i4.f8_weight(digits(g, g - 1)[:, order].to(F8).cuda(), ones[0]),
+                             clef_i4.f8_weight(digits(u, u + 1)[:, order].to(F8).cuda(), ones[0]),
+                             clef_i4.f8_weight(down[:, :, order].to(F8).cuda(), ones[1]), topk=1)
+    at = torch.arange(t) * 37 % triples
+    x = torch.zeros((t, hidden))
+    for i, place in enumerate((256.0, 16.0, 1.0)):
+        x[torch.arange(t), 3 * at + i] = place
+    e = torch.randint(0, experts, (t,), generator=rng)
+    logits = torch.nn.functional.one_hot(e, experts).float().cuda()
+    got = moe.decode(x.to(BF).cuda(), logits)
+    assert torch.equal(got.cpu().float(), want[e[:, None], pair[None, :], at[:, None]].float())
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_decode_masked_logits(dtype):
     t, hidden, inter, experts, topk = 8, 256, 136, 12, 4
