@@ -490,7 +490,9 @@ __global__ __launch_bounds__(512) void few_down_kernel(const MoeFewArgs a) {
       for (int s = 0; s < 4; ++s)
         __hip_atomic_store(at + part * (NT * ITEMS * 4) + s, y[s], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    wait_vmcnt<0>();
+    // (with the clobber, so that no store is moved behind the wait: neither the waiting
+    // builtin nor a barrier of workgroup scope forbids that)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (tid == 0)
       last = __hip_atomic_fetch_add(&a.arrived[blockIdx.x], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;

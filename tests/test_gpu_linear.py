@@ -624,6 +624,38 @@ def test_decode_does_not_depend_on_its_scratch(t):
         assert (off <= 2.0 ** -7 * first[i].double().abs() + 1e-3 * first[i].double().abs().mean()).all()
 
 
+def decode_on(scratch, moe, x, logits):
+    """decode on a workspace of the caller's."""
+    out, n = torch.full_like(x, NAN), clef_i4._n
+    n.launch(n.clef_moe_layer_f8, x, x.shape[1], logits, int(logits.dtype == F32), x.shape[0], x.shape[1], moe.gate.rows,
+             moe.gate.matrices, moe.topk, moe.gate.codes, moe.gate.scales, moe.up.codes, moe.up.scales, moe.down.codes,
+             moe.down.scales, None, out, scratch, scratch.numel())
+    return out
+
+
+def workspace(moe, t, hidden):
+    nbytes = clef_i4.lib().clef_moe_layer_f8_workspace_bytes(t, hidden, moe.gate.rows, moe.gate.matrices, moe.topk)
+    return torch.zeros((nbytes,), dtype=torch.uint8, device="cuda")
+
+
+# widths whose down products are split in many parts: 8 columns a workgroup, 32
+PARTS = [(4, 64, 8192, 4, 4), (3, 8, 32768, 4, 2), (9, 256, 2048, 32, 4), (16, 128, 4096, 8, 2)]
+
+
+@pytest.mark.parametrize("t,hidden,inter,experts,topk", PARTS)
+def test_decode_adds_parts_that_have_arrived(t, hidden, inter, experts, topk):
+    """A part's sum read before it is there would be the NaN that the
+    scratch held."""
+    moe, w = layer(experts, hidden, inter, topk, "f32", t)
+    x, logits = randn((t, hidden), 1.0, 1), randn((t, experts), 2.0, 2, F32)
+    scratch = workspace(moe, t, hidden)
+    first = decode_on(scratch, moe, x, logits)
+    check(first, *moe64(x, logits, *w, topk))
+    for _ in range(20):
+        scratch.fill_(255)
+        assert torch.equal(decode_on(scratch, moe, x, logits), first)
+
+
 # ---------------------------------------------------------------- together
 
 def block(moe, x, wg, wu, wd, wo, bo):
