@@ -656,6 +656,32 @@ def test_decode_adds_parts_that_have_arrived(t, hidden, inter, experts, topk):
         assert torch.equal(decode_on(scratch, moe, x, logits), first)
 
 
+@pytest.mark.parametrize("t,hidden,inter,experts,topk", [(1, 512, 264, 32, 4), (16, 512, 264, 32, 4), *PARTS])
+def test_decode_takes_nothing_from_its_scratch(t, hidden, inter, experts, topk):
+    """A call on what a call of other tokens left (their table, h, parts' sums and
+    counts), or on all bits set, is a call on zeros, bit for bit. Some tokens name
+    fewer experts than topk, and one none."""
+    moe, w = layer(experts, hidden, inter, topk, "f32", t)
+    sets = []
+    for seed in (1, 2):
+        logits = randn((t, experts), 2.0, seed, F32)
+        if seed == 2:
+            logits[::2, :experts - 1] = -INF
+            logits[t // 2] = NAN
+        sets.append((randn((t, hidden), 1.0, seed + 2), logits))
+    wants = []
+    for x, logits in sets:
+        wants.append(decode_on(workspace(moe, t, hidden), moe, x, logits))
+        check(wants[-1], *moe64(x, logits, *w, topk))
+    assert not torch.equal(*wants)
+    scratch = workspace(moe, t, hidden)
+    for turn in (0, 1, 0, 1, 1, 0):
+        assert torch.equal(decode_on(scratch, moe, *sets[turn]), wants[turn])
+    for turn in (0, 1):
+        scratch.fill_(255)
+        assert torch.equal(decode_on(scratch, moe, *sets[turn]), wants[turn])
+
+
 # ---------------------------------------------------------------- together
 
 def block(moe, x, wg, wu, wd, wo, bo):
