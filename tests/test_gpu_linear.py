@@ -270,6 +270,75 @@ def test_linear_of_every_width_and_start(k, skip):
         assert torch.equal(clef_i4.linear(x, w, dtype=F32).double(), x.double() @ w.double().t()), (m, n)
 
 
+def pitched(which):
+    """(rows, k, columns, first column, columns behind) of operands in wider rows, on
+    every kernel: rows on multiples of 16 bytes as in KERNELS and ONCE, and at any
+    even byte."""
+    aligned = [c[:3] for c in KERNELS[which] + ONCE[which]]
+    return [(*c, 8, 16) for c in aligned] + [(*c, 3, 6) for c in aligned[::3]] + [(*c[:3], 5, 2) for c in ODD_KERNELS[which]]
+
+
+def columns(t, skip, behind):
+    """t as a column range of wider rows of NaN."""
+    wide = torch.full((t.shape[0], skip + t.shape[1] + behind), NAN, dtype=t.dtype, device="cuda")
+    wide[:, skip:skip + t.shape[1]] = t
+    return wide[:, skip:skip + t.shape[1]]
+
+
+class Guarded:
+    """An output among rows and columns that stay as they are."""
+
+    def __init__(self, m, n, skip, behind, dtype=BF):
+        self.wide = torch.full((m + 3, skip + n + behind), 7.0, dtype=dtype, device="cuda")
+        self.out = self.wide[1:m + 1, skip:skip + n]
+
+    def result(self):
+        got = self.out.clone()
+        self.out.fill_(7.0)
+        assert (self.wide == 7.0).all()
+        return got
+
+
+@pytest.mark.parametrize("m,k,n,skip,behind", pitched(0))
+def test_linear_of_column_ranges_on_every_kernel(m, k, n, skip, behind):
+    seed = m * 19 + k * 5 + n + skip
+    x, w, r = randn((m, k), 1.0, seed), randn((n, k), k ** -0.5, seed + 1), randn((m, n), 1.0, seed + 2)
+    b = randn((n,), 1.0, seed + 3)
+    cx, cw, cr = columns(x, skip, behind), columns(w, skip, behind + 8), columns(r, skip, behind + 1)
+    # whole rows run the same kernel where both start on 16 bytes, or neither
+    alike = (skip % 8 == 0) == (k % 8 == 0)
+    for act, res, dtype in ((None, True, BF), ("silu", False, BF), ("gelu", True, F32), (None, False, F32)):
+        to = Guarded(m, n, skip, behind, dtype)
+        clef_i4.linear(cx, cw, bias=b, activation=act, residual=cr if res else None, out=to.out)
+        got = to.result()
+        check(got, *linear64(x, w, b, act, r if res else None))
+        if alike:
+            assert torch.equal(got, clef_i4.linear(x, w, bias=b, activation=act, residual=r if res else None, dtype=dtype))
+    to = Guarded(m, n, skip, behind)
+    to.out.copy_(r)
+    clef_i4.linear(cx, cw, residual=to.out, out=to.out)
+    got = to.result()
+    check(got, *linear64(x, w, residual=r))
+
+
+@pytest.mark.parametrize("m,k,n,skip,behind", pitched(1))
+def test_gate_up_of_column_ranges_on_every_kernel(m, k, n, skip, behind):
+    seed = m * 23 + k * 5 + n + skip
+    x, wg, wu = randn((m, k), 1.0, seed), randn((n, k), k ** -0.5, seed + 1), randn((n, k), k ** -0.5, seed + 2)
+    bg, bu = randn((n,), 1.0, seed + 3, F32), randn((n,), 1.0, seed + 4, F32)
+    cx = columns(x, skip, behind)
+    gap = 8 - k % 8 if skip % 8 == 0 else 2
+    both = columns(torch.cat((wg, torch.full((n, gap), NAN, dtype=BF, device="cuda"), wu), 1), skip, behind)  # side by side
+    cg, cu = both[:, :k], both[:, k + gap:]
+    for act, biases in (("silu", (None, None)), ("gelu_tanh", (bg, bu))):
+        to = Guarded(m, n, skip, behind)
+        clef_i4.linear_gate_up(cx, cg, cu, activation=act, gate_bias=biases[0], up_bias=biases[1], out=to.out)
+        got = to.result()
+        check(got, *gate_up64(x, wg, wu, act, *biases))
+        if (skip % 8 == 0) == (k % 8 == 0):
+            assert torch.equal(got, clef_i4.linear_gate_up(x, wg, wu, act, *biases))
+
+
 @pytest.mark.parametrize("m,k,n", [(1, 256, 64), (37, 520, 129), (300, 1024, 512)])
 def test_linear_onto_its_residual_and_beside_its_rows(m, k, n):
     x, w, r = randn((m, k), 1.0, 1), randn((n, k), 0.05, 2), randn((m, n), 1.0, 3)

@@ -122,6 +122,24 @@ def test_kernel_name_and_every_kernel_is_compared_with_a_reference():
         assert odd == few | {"any", "any128"} | (set() if gate_up_it else {"8x8", "16x16", "32x16"})
 
 
+@pytest.mark.parametrize("which", [0, 1])
+def test_column_ranges_reach_every_kernel(which):
+    """Operands in wider rows run every kernel on the GPU, split and whole, on 16 bytes
+    and at any even byte."""
+    from test_gpu_linear import pitched
+
+    lib = clef_i4.lib()
+    seen = {True: set(), False: set()}
+    for m, k, n, skip, behind in pitched(which):
+        on16 = all(v % 8 == 0 for v in (skip, k, skip + k + behind))
+        split = on16 and lib.clef_linear_workspace_bytes(m, n, k, which) > 0
+        seen[on16].add((lib.clef_linear_kernel_name(m, n, k, which, on16).decode(), split))
+    few = {"8x16", "16x32", "32x32", "64x32"} | (set() if which else {"8x8", "16x16", "32x16"})
+    tiles = {"128x128", "128x128x2", "128x256", "256x256"}
+    assert seen[True] == {(t, False) for t in few | {"64x64"} | tiles} | {(t, True) for t in tiles}
+    assert seen[False] == {(t, False) for t in few | {"any", "any128"}}
+
+
 def few(x=FAKE, xs=None, logits=FAR, dtype=0, t=4, hidden=256, inter=128, experts=8, topk=2, gate=2 * FAR, gs=3 * FAR,
         up=4 * FAR, us=5 * FAR, down=6 * FAR, ds=7 * FAR, res=None, out=8 * FAR, ws=9 * FAR, nbytes=1 << 30):
     xs = hidden if xs is None else xs
