@@ -1199,14 +1199,22 @@ int clef_moe_layer_f8(const uint16_t* x, int64_t x_stride, const void* logits, i
   if (workspace_bytes < need) return fail(kWorkspace);
   const size_t logits_bytes = (size_t)tokens * experts * (logits_dtype ? 4 : 2), rows_bytes = (size_t)tokens * hidden * 2;
   const Pieces rows{x, tokens, x_stride * 2, hidden * 2ll}, result{out, tokens, hidden * 2ll, hidden * 2ll};
-  const size_t weight = (size_t)clef::f8_weight_bytes(experts, inter, hidden);
+  // each weight's codes and scales, of one size all three
+  const size_t codes = (size_t)clef::f8_weight_bytes(experts, inter, hidden), scales = codes / 16384 * 4;
+  auto over_weights = [&](const void* at, size_t bytes) {
+    for (const uint8_t* w : {gate, up, down})
+      if (overlap(at, bytes, w, codes)) return true;
+    for (const float* w : {gate_scales, up_scales, down_scales})
+      if (overlap(at, bytes, w, scales)) return true;
+    return false;
+  };
   if (overlap(workspace, need, x, rows.extent()) || overlap(workspace, need, logits, logits_bytes) ||
       overlap(workspace, need, out, rows_bytes) || (residual && overlap(workspace, need, residual, rows_bytes)) ||
-      overlap(workspace, need, gate, weight) || overlap(workspace, need, up, weight) ||
-      overlap(workspace, need, down, weight))
+      over_weights(workspace, need))
     return fail("MoE workspace overlaps an operand");
-  if ((x != out && overlap(result, rows)) || (residual && residual != out && overlap(residual, rows_bytes, out, rows_bytes)) ||
-      overlap(logits, logits_bytes, out, rows_bytes))
+  const bool onto_x = x == out && (tokens == 1 || x_stride == hidden);
+  if ((!onto_x && overlap(result, rows)) || (residual && residual != out && overlap(residual, rows_bytes, out, rows_bytes)) ||
+      overlap(logits, logits_bytes, out, rows_bytes) || over_weights(out, rows_bytes))
     return fail("MoE output overlaps an operand");
   clef::MoeFewArgs a{};
   a.x = x, a.x_stride = x_stride, a.logits = logits, a.logits_f32 = logits_dtype != 0;

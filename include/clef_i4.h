@@ -662,8 +662,8 @@ int clef_linear_gate_up(const uint16_t* x, int64_t m, int32_t k, int64_t x_strid
  * % 8 == 0, x_stride <= 2^24 -> "unsupported MoE shape for few tokens"; pointers
  * 16-byte aligned (logits: as their elements). The workspace (bytes below; 0 for
  * shapes the call rejects) lies apart from every operand -> "MoE workspace
- * overlaps an operand"; the output over a part of x, the residual or the logits ->
- * "MoE output overlaps an operand". */
+ * overlaps an operand"; the output over a part of x, the residual, the logits, the
+ * weights or their scales -> "MoE output overlaps an operand". */
 size_t clef_moe_layer_f8_workspace_bytes(int64_t tokens, int32_t hidden, int32_t inter, int32_t experts,
                                          int32_t topk);
 int clef_moe_layer_f8(const uint16_t* x, int64_t x_stride, const void* logits, int32_t logits_dtype, int64_t tokens,

@@ -175,3 +175,20 @@ def test_moe_layer_f8_workspace_and_overlaps():
     assert few(out=FAKE + 16) == (-1, "MoE output overlaps an operand")
     assert few(out=FAR) == (-1, "MoE output overlaps an operand")
     assert few(res=8 * FAR + 16) == (-1, "MoE output overlaps an operand")
+
+
+@pytest.mark.parametrize("name,bytes_", [("gate", 8 * 1 * 2 * 16384), ("up", 8 * 1 * 2 * 16384), ("down", 8 * 2 * 1 * 16384),
+                                         ("gs", 8 * 1 * 2 * 4), ("us", 8 * 1 * 2 * 4), ("ds", 8 * 2 * 1 * 4)])
+def test_moe_layer_f8_weights_and_scales_lie_apart(name, bytes_):
+    """The output and the workspace over the first and the last 16 bytes of each."""
+    at = dict(gate=2, gs=3, up=4, us=5, down=6, ds=7)[name] * FAR
+    need = clef_i4.lib().clef_moe_layer_f8_workspace_bytes(4, 256, 128, 8, 2)
+    result = 4 * 256 * 2
+    for first in (at + 16 - result, at, at + bytes_ - 16):
+        assert few(out=first) == (-1, "MoE output overlaps an operand"), (name, first - at)
+    for first in (at + 16 - need // 16 * 16, at, at + bytes_ - 16):
+        assert few(ws=first, nbytes=need) == (-1, "MoE workspace overlaps an operand"), (name, first - at)
+
+
+def test_moe_layer_f8_output_over_rows_of_another_pitch():
+    assert few(out=FAKE, xs=264) == (-1, "MoE output overlaps an operand")
