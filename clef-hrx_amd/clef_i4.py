@@ -1263,7 +1263,7 @@ def _refuse_linear(x, weights, biases, residual, out, dtype, activation) -> None
         if not bias.is_contiguous():
             raise ClefError(-1, "linear bias must be contiguous")
     if residual is not None:
-        if residual.shape[0] != x.shape[0]:
+        if residual.dim() != 2 or residual.shape[0] != x.shape[0]:
             raise ClefError(-1, "residual shape/dtype mismatch")
         _check_linear_rows(residual, n, device)
     if dtype not in (None, torch.bfloat16, torch.float32):

@@ -1,5 +1,6 @@
 """Products with bf16 activations without a GPU: sizes, refusals."""
 import pytest
+import torch
 
 import clef_i4
 
@@ -192,3 +193,13 @@ def test_moe_layer_f8_weights_and_scales_lie_apart(name, bytes_):
 
 def test_moe_layer_f8_output_over_rows_of_another_pitch():
     assert few(out=FAKE, xs=264) == (-1, "MoE output overlaps an operand")
+
+
+@pytest.mark.parametrize("residual", [torch.zeros((), dtype=torch.bfloat16), torch.zeros(4, dtype=torch.bfloat16),
+                                      torch.zeros((1, 4, 32), dtype=torch.bfloat16), torch.zeros((3, 32), dtype=torch.bfloat16)])
+def test_residuals_of_other_dimensions_are_refused(residual, monkeypatch):
+    """What linear says to them (here with the host as the device)."""
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1, raising=False)
+    x, w = torch.zeros((4, 64), dtype=torch.bfloat16), torch.zeros((32, 64), dtype=torch.bfloat16)
+    with pytest.raises(clef_i4.ClefError, match="residual shape/dtype mismatch"):
+        clef_i4._refuse_linear(x, (w,), (None,), residual, None, None, None)
