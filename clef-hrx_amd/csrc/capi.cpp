@@ -1122,7 +1122,7 @@ int linear(clef::LinearArgs& p, bool gate_up, int32_t bias_dtype, int32_t out_dt
            size_t workspace_bytes, clef_stream_t stream) {
   if (int rc = check_linear(p, gate_up, bias_dtype, out_dtype)) return rc;
   if (p.m == 0) return CLEF_OK;
-  if (const size_t need = clef::linear_workspace_bytes(p.m, p.n, p.k, gate_up)) {
+  if (const size_t need = clef::linear_workspace_bytes(p, gate_up)) {
     if (!aligned(workspace, 16)) return fail(kAlign);
     if (workspace_bytes < need) return fail(kWorkspace);
     if (linear_over(p, gate_up, bias_dtype, Pieces{workspace, 1, 0, (int64_t)need}) ||

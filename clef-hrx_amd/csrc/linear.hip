@@ -858,7 +858,12 @@ hipError_t launch_rows(LinearArgs& p, void* workspace, hipStream_t stream) {
 
 }  // namespace
 
+size_t linear_workspace_bytes(const LinearArgs& p, bool gate_up) {
+  return rows_of_16(p) ? linear_workspace_bytes(p.m, p.n, p.k, gate_up) : 0;
+}
+
 size_t linear_workspace_bytes(int64_t m, int n, int k, bool gate_up) {
+  if (k % 8 != 0) return 0;  // (only products of rows on 16 bytes are split)
   const int64_t matrices = gate_up ? 2 : 1;
   const LinearPlan plan = linear_plan(m, n * matrices, k, gate_up, true);
   return plan.parts > 1 ? (size_t)(plan.parts * matrices * m * ((n + 3) & ~3)) * 4 : 0;

@@ -38,8 +38,10 @@ struct LinearArgs {
   float* partial;
 };
 
-// Scratch for the parts of a product whose operands' rows lie on 16 bytes.
+// Scratch for the parts of a product whose operands' rows lie on 16 bytes, and for
+// those of this one.
 size_t linear_workspace_bytes(int64_t m, int n, int k, bool gate_up);
+size_t linear_workspace_bytes(const LinearArgs& p, bool gate_up);
 const char* linear_kernel_name(int64_t m, int n, int k, bool gate_up, bool aligned);
 hipError_t launch_linear(LinearArgs p, bool gate_up, void* workspace, hipStream_t stream);
 

@@ -622,9 +622,10 @@ int clef_moe_expert_gate_up_f8(const uint8_t* a, int64_t a_rows, const uint8_t* 
  * stride do not overlap). With no rows a call does nothing.
  *
  * Products of some rows whose tiles do not fill the card are split along k; the
- * workspace (bytes below, 0 for up to 8 rows and wherever none is needed; 16-byte
- * aligned, apart from every operand -> "linear workspace overlaps an operand")
- * takes the parts' sums, which are added in a fixed order. */
+ * workspace (bytes below, 0 for up to 8 rows and wherever none is needed; rows of x
+ * or a weight that start off 16 bytes, or lie more than 4 MiB apart, need none
+ * either; 16-byte aligned, apart from every operand -> "linear workspace overlaps an
+ * operand") takes the parts' sums, which are added in a fixed order. */
 size_t clef_linear_workspace_bytes(int64_t m, int32_t n, int32_t k, int32_t gate_up);
 
 /* The tile (rows x weight rows) that the library's rule picks, for tests and

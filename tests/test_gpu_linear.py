@@ -339,6 +339,20 @@ def test_gate_up_of_column_ranges_on_every_kernel(m, k, n, skip, behind):
             assert torch.equal(got, clef_i4.linear_gate_up(x, wg, wu, act, *biases))
 
 
+@pytest.mark.parametrize("k,pitch,skip", [(8192, 8200, 1), (8192, 8201, 0), (8191, 8191, 0)])
+def test_rows_off_16_bytes_take_no_workspace(k, pitch, skip):
+    """A caller of the C entries with rows that do not lie on 16 bytes hands none over."""
+    m, n, lib, _n = 200, 2048, clef_i4.lib(), clef_i4._n
+    x = randn((m * pitch + 8,), 1.0, 1).as_strided((m, k), (pitch, 1), skip)
+    w, up = randn((n, k), k ** -0.5, 2), randn((n, k), k ** -0.5, 3)
+    out = torch.empty((m, n), dtype=BF, device="cuda")
+    _n.launch(_n.clef_linear, x.data_ptr(), m, k, pitch, w, n, k, None, 0, 0, None, n, out, 0, n, None, 0)
+    assert torch.equal(out, clef_i4.linear(x, w))
+    check(out, *linear64(x, w))
+    _n.launch(_n.clef_linear_gate_up, x.data_ptr(), m, k, pitch, w, up, n, k, None, None, 0, 4, out, n, None, 0)
+    check(out, *gate_up64(x, w, up))
+
+
 @pytest.mark.parametrize("m,k,n", [(1, 256, 64), (37, 520, 129), (300, 1024, 512)])
 def test_linear_onto_its_residual_and_beside_its_rows(m, k, n):
     x, w, r = randn((m, k), 1.0, 1), randn((n, k), 0.05, 2), randn((m, n), 1.0, 3)

@@ -203,3 +203,11 @@ def test_residuals_of_other_dimensions_are_refused(residual, monkeypatch):
     x, w = torch.zeros((4, 64), dtype=torch.bfloat16), torch.zeros((32, 64), dtype=torch.bfloat16)
     with pytest.raises(clef_i4.ClefError, match="residual shape/dtype mismatch"):
         clef_i4._refuse_linear(x, (w,), (None,), residual, None, None, None)
+
+
+@pytest.mark.parametrize("gate_up_it", [0, 1])
+def test_widths_off_16_bytes_need_no_workspace(gate_up_it):
+    lib = clef_i4.lib()
+    for k in (8185, 8190, 8191, 8193, 8196):
+        assert lib.clef_linear_workspace_bytes(200, 2048, k, gate_up_it) == 0, k
+    assert lib.clef_linear_workspace_bytes(200, 2048, 8184, gate_up_it) > 0
