@@ -67,8 +67,9 @@ __device__ __forceinline__ float sigmoid_f32(float v) {
 
 // v Phi(v), Phi the normal distribution function: Phi(-a) = exp(-a^2 / 2) t P(t)
 // for a >= 0 with t = 1 / (1 + 0.3 a), P of degree 7 fitted to erfcx(a / sqrt 2) /
-// 2 (1.5e-7 of the value for a in 0 .. 14). The tail keeps its relative accuracy
-// (the square's rounding: 2e-6 at a = 5), which 1 + erf(v) would lose.
+// 2 (2.0e-7 of the value for a in 0 .. 14, the coefficients in f32). The tail keeps its
+// relative accuracy (with the square's rounding 2.5e-6 up to a = 5), which 1 + erf(v)
+// would lose.
 __device__ __forceinline__ float gelu_f32(float v) {
   const float a = __builtin_fabsf(v), t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.3f, 1.0f));
   float p = 0.0356752909719944f;

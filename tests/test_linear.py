@@ -1,4 +1,8 @@
 """Products with bf16 activations without a GPU: sizes, refusals."""
+import math
+import os
+import re
+
 import pytest
 import torch
 
@@ -211,3 +215,25 @@ def test_widths_off_16_bytes_need_no_workspace(gate_up_it):
     for k in (8185, 8190, 8191, 8193, 8196):
         assert lib.clef_linear_workspace_bytes(200, 2048, k, gate_up_it) == 0, k
     assert lib.clef_linear_workspace_bytes(200, 2048, 8184, gate_up_it) > 0
+
+
+def test_gelu_polynomial_is_as_near_as_its_comment_says():
+    """The coefficients in the source, rounded to f32, against the normal distribution's
+    tail in 64 bits (14 is where exp(-a^2 / 2) leaves f32's normal range)."""
+    with open(os.path.join(os.path.dirname(clef_i4.__file__), "csrc", "linear.hpp")) as f:
+        source = f.read()
+    body = source[source.index("float gelu_f32(float v) {"):]
+    body = body[:body.index("\n}\n")]
+    c = [torch.tensor(float(v)).item() for v in [re.search(r"float p = ([-\d.e]+)f;", body)[1]]
+         + re.findall(r"p = __builtin_fmaf\(p, t, ([-\d.e]+)f\)", body)]
+    slope = torch.tensor(float(re.search(r"__builtin_fmaf\(a, ([\d.]+)f, 1.0f\)", body)[1])).item()
+    stated = float(re.search(r"\(([\d.]+e-7) of the value for a in 0 \.\. 14", source)[1])
+    assert len(c) == 8 and stated < 1e-6
+    worst = 0.0
+    for i in range(14001):
+        a = i / 1000
+        t, p = 1.0 / (1.0 + slope * a), 0.0
+        for v in c:
+            p = p * t + v
+        worst = max(worst, abs(p * t / (math.exp(a * a / 2) * math.erfc(a / math.sqrt(2.0)) / 2) - 1.0))
+    assert 0.9 * stated < worst <= stated
