@@ -249,11 +249,11 @@ __device__ __forceinline__ void linear_store_tile(const LinearArgs& p, const v4f
 // So every load has a step and a half to land.
 //
 // 256 x 256 tiles: 4096 x 4096 x 12288 303 to 313 by card, 1.32 to 1.36 PFLOP/s (the
-// library's product 330 in one call after another), 8192 x 8192 x 8192 743 to 761
-// (715). MFMA busy two thirds of the cycles at 1.9 to 2.0 GHz; with operands of zeros
-// the same code takes 257, so a fifth of the time is the clock that the power leaves.
-// Without the epilogue 278. Four waves of 128 x 128, which read a third less LDS, run
-// the main loop in the same time and a longer epilogue (322 against 309).
+// library's product 279 to 330), 8192 x 8192 x 8192 743 to 761 (690 to 715). MFMA busy
+// two thirds of the cycles at 1.9 to 2.0 GHz; with operands of zeros the same code
+// takes 257, so a fifth of the time is the clock that the power leaves. Without the
+// epilogue 278. Four waves of 128 x 128, which read a third less LDS, run the main loop
+// in the same time and a longer epilogue (322 against 309).
 template <class T, bool GU, bool RESID>
 __global__ __launch_bounds__(T::THREADS, 2 * T::GROUPS) void linear_tile_kernel(const LinearArgs p, int tiles_m,
                                                                                 int tiles_n) {
