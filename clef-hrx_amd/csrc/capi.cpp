@@ -1113,7 +1113,7 @@ int check_linear(const clef::LinearArgs& p, bool gate_up, int32_t bias_dtype, in
   if (!aligned(p.x, 2) || !aligned(p.w, 2) || (gate_up && !aligned(p.w2, 2)) || !aligned(p.out, out_bytes) ||
       !optional(p.bias, bias_bytes) || !optional(p.bias2, bias_bytes) || !optional(p.residual, 2))
     return fail(kLinearAlign);
-  const bool onto = p.residual == p.out && p.residual_stride == p.out_stride && out_dtype == 0;
+  const bool onto = p.residual == p.out && (p.m == 1 || p.residual_stride == p.out_stride) && out_dtype == 0;
   if (linear_over(p, gate_up, bias_dtype, linear_result(p, out_dtype), onto)) return fail(kLinearOverlap);
   return CLEF_OK;
 }

@@ -353,6 +353,18 @@ def test_rows_off_16_bytes_take_no_workspace(k, pitch, skip):
     check(out, *gate_up64(x, w, up))
 
 
+def test_one_row_onto_its_residual_whatever_the_pitches():
+    """One row has no second that the pitches could place elsewhere."""
+    k, n, _n = 256, 64, clef_i4._n
+    x, w, r = randn((1, k), 1.0, 1), randn((n, k), 0.05, 2), randn((1, n), 1.0, 3)
+    want = clef_i4.linear(x, w, residual=r)
+    _n.launch(_n.clef_linear, x, 1, k, k, w, n, k, None, 0, 0, r, n, r, 0, n + 64, None, 0)
+    assert torch.equal(r, want)
+    with pytest.raises(clef_i4.ClefError, match="overlaps"):  # two do
+        both = randn((3, n + 64), 1.0, 4)
+        _n.launch(_n.clef_linear, x.expand(2, k).contiguous(), 2, k, k, w, n, k, None, 0, 0, both, n, both, 0, n + 64, None, 0)
+
+
 @pytest.mark.parametrize("m,k,n", [(1, 256, 64), (37, 520, 129), (300, 1024, 512)])
 def test_linear_onto_its_residual_and_beside_its_rows(m, k, n):
     x, w, r = randn((m, k), 1.0, 1), randn((n, k), 0.05, 2), randn((m, n), 1.0, 3)
